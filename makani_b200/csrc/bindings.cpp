@@ -816,6 +816,7 @@ void peer_allreduce(const std::vector<int64_t>& data_ptrs, const std::vector<int
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("launches", []() { return mkh::launches(); }, "kernel launches of this thread's layer passes");
   mkh::bind_layers(m);
+  mkh::bind_tokens(m);
   m.def("gemm_row_sums", &gemm_row_sums);
   m.def("gemm", &gemm, "tcgen05 GEMM with fused epilogue");
   m.def("gemm_peer", &gemm_peer, "tcgen05 GEMM reading its B operand from peer devices");

@@ -74,5 +74,6 @@ inline cudaStream_t stream() { return at::cuda::getCurrentCUDAStream().stream();
 int64_t& launches();
 
 void bind_layers(pybind11::module_& m);
+void bind_tokens(pybind11::module_& m);
 
 }  // namespace mkh

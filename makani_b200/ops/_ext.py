@@ -65,7 +65,7 @@ _NON_KERNEL = {"read_error_flag", "clear_error_flag", "lp_scratch_floats", "adam
 
 # passes over whole layers, which count their launches themselves
 _LAYERS = {"conv_forward", "conv_backward", "mlp_forward", "mlp_backward", "norm_forward", "norm_backward", "spectral_forward",
-           "spectral_backward", "afno_forward", "afno_backward"}
+           "spectral_backward", "afno_forward", "afno_backward", "layer_norm_forward", "layer_norm_backward"}
 
 
 class _Counting:

@@ -1,4 +1,5 @@
-"""Instance normalisation over (H, W) with optional fused GELU, fp32 statistics, bf16 data.
+"""Instance normalisation over (H, W) with optional fused GELU, fp32 statistics, bf16 data; layer normalisation over the last
+dimension of tokens, alone or behind a residual sum.
 
 Replaces `nn.InstanceNorm2d(affine=True, eps=1e-6)` followed by the block activation
 (makani/models/networks/sfnonet.py:246-252,379).  Two layouts are served:
@@ -13,9 +14,13 @@ storing them.
 
 from __future__ import annotations
 
+from typing import Optional
+
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _ext
+from .conv import records_grad
 
 
 def _is_cl(x):
@@ -160,3 +165,89 @@ def channel_sums(x: torch.Tensor) -> torch.Tensor:
         ext.inorm_partial_stats(x, sums)
         return sums[:, 0].view(B, C).sum(0)
     return x.float().sum(dim=(0, 2, 3))
+
+
+# ---------------------------------------------------------------------------------------------------- layer norm
+
+LN_CHANNELS = 8192          # most channels of a row in the kernels
+_LN_TYPES = (torch.bfloat16, torch.float32)
+
+
+class _LayerNorm(torch.autograd.Function):
+    """(y,) or, with a residual, (s, y) with s = x + residual and y = LN(s); the backward pass reads s (x) and every row's (mean, rstd)."""
+
+    @staticmethod
+    def forward(ctx, x, residual, weight, bias, eps, out_f32, train):
+        s, y, stats, w = _ext.require().layer_norm_forward(x, residual, weight, bias, float(eps), out_f32, train)
+        if train:
+            ctx.save_for_backward(x if residual is None else s, w, stats)
+        # a residual in bf16 beside an fp32 x takes its gradient in its own type
+        ctx.flags = (weight is not None or bias is not None, residual is not None, residual is not None and residual.dtype != x.dtype)
+        ctx.set_materialize_grads(False)
+        return y if residual is None else (s, y)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, *grads):
+        x, w, stats = ctx.saved_tensors
+        params, added, half = ctx.flags
+        ds, dy = grads if added else (None, grads[0])
+        if dy is None:
+            return ds, (ds.bfloat16() if ds is not None and half else ds), None, None, None, None, None
+        need_params = params and any(ctx.needs_input_grad[2:4])
+        dx, dr, dw, db = _ext.require().layer_norm_backward(x, dy, ds, w, stats, need_params, half and ctx.needs_input_grad[1])
+        need = ctx.needs_input_grad
+        return (dx if need[0] else None, ((dr if half else dx) if need[1] else None), dw if need[2] else None, db if need[3] else None,
+                None, None, None)
+
+
+def _check_layer_norm(x, residual, weight, bias, out_dtype):
+    if x.dim() < 1 or x.shape[-1] < 1 or not x.dtype.is_floating_point:
+        raise ValueError(f"layer norm takes floating-point tokens [..., C], got {x.dtype} {tuple(x.shape)}")
+    for name, p in (("weight", weight), ("bias", bias)):
+        if p is not None and (p.dim() != 1 or p.shape[0] != x.shape[-1]):
+            raise ValueError(f"layer norm over {x.shape[-1]} channels: {name} has shape {tuple(p.shape)}")
+    if residual is not None and (residual.shape != x.shape or residual.device != x.device):
+        raise ValueError(f"the residual {tuple(residual.shape)} on {residual.device} does not match {tuple(x.shape)} on {x.device}")
+    if out_dtype is not None and not out_dtype.is_floating_point:
+        raise ValueError(f"layer norm has no output in {out_dtype}")
+
+
+def _layer_norm_native(x, out_dtype) -> bool:
+    return _ext.native() and x.is_cuda and x.dtype in _LN_TYPES and out_dtype in _LN_TYPES and x.shape[-1] <= LN_CHANNELS
+
+
+def _layer_norm_torch(x, weight, bias, eps, out_dtype):
+    # (the types are explicit here: autocast would choose its own)
+    with torch.autocast(device_type=x.device.type, enabled=False):
+        t = torch.promote_types(x.dtype, torch.float32)
+        y = torch.nn.functional.layer_norm(x.to(t), x.shape[-1:], None if weight is None else weight.to(t),
+                                           None if bias is None else bias.to(t), eps)
+        return y.to(out_dtype)
+
+
+def layer_norm(x: torch.Tensor, weight, bias, eps: float = 1e-5, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """y = (x - mean) / sqrt(var + eps) * weight + bias over the last dimension (biased variance, fp32 statistics), rounded once to
+    `out_dtype` (default: that of x).  `weight` and `bias` [C] or None.
+
+    CUDA tensors in bf16 or fp32 of up to 8192 channels run on one kernel in either direction, whose rows may be strided in two levels (the
+    queries of a fused projection, [B, N, heads, D] out of [B, N, 3, heads, D]); the rest on the torch op."""
+    _check_layer_norm(x, None, weight, bias, out_dtype)
+    out_dtype = out_dtype or x.dtype
+    if _layer_norm_native(x, out_dtype):
+        return _LayerNorm.apply(x, None, weight, bias, eps, out_dtype == torch.float32, records_grad(x, weight, bias))
+    return _layer_norm_torch(x, weight, bias, eps, out_dtype)
+
+
+def add_layer_norm(x: torch.Tensor, residual: torch.Tensor, weight, bias, eps: float = 1e-5, out_dtype: Optional[torch.dtype] = None):
+    """(s, y): s = x + residual, in the wider of their types, and y = layer_norm(s, ...) of that rounded sum, in `out_dtype` (default:
+    that of s); one pass over memory in either direction."""
+    _check_layer_norm(x, residual, weight, bias, out_dtype)
+    if residual.dtype == torch.float32 and x.dtype == torch.bfloat16:
+        x, residual = residual, x
+    dtype = torch.promote_types(x.dtype, residual.dtype)
+    out_dtype = out_dtype or dtype
+    if _layer_norm_native(x, out_dtype) and residual.dtype in _LN_TYPES:
+        return _LayerNorm.apply(x, residual, weight, bias, eps, out_dtype == torch.float32, records_grad(x, residual, weight, bias))
+    s = x + residual
+    return s, _layer_norm_torch(s, weight, bias, eps, out_dtype)
