@@ -1,0 +1,1221 @@
+// Softmax attention on the tensor cores, with S = scale Q K^T:
+//
+//   forward    P = exp(S - max), O = P V / sum P, L = max + log sum P                           (one pass over the keys, running max and sum)
+//   backward   P = exp(S - L), dV = P^T dO, dS = P (dO V^T - delta), dQ = scale dS K, dK = scale dS^T Q,  delta = sum_d O dO
+//
+// Exponentials are powers of two of (scale log2 e) S, one special-function instruction each.  Products take bf16 operands and add in fp32 (tensor
+// memory); P and dS are rounded to bf16 as operands of the second products (half a step 2^-9 of each weight, of the size of the rounding of the
+// outputs), sums, maxima and L stay in fp32.
+//
+// A CTA has an SM to itself.  Warps: 0 loads tiles (TMA), 1 issues the products, 2 clears rows that belong to another sequence, 4 - 11 compute on
+// rows in tensor memory, a thread a row.  Every wait is bounded; on expiry the kernel records a code in *err and drains.
+#include <cuda_bf16.h>
+
+#include <algorithm>
+
+#include "attention.cuh"
+#include "fused_ops.cuh"
+#include "launch.cuh"
+#include "tcgen05.cuh"
+#include "gelu.cuh"
+
+namespace mk {
+
+namespace {
+
+constexpr int TILE = 128;                        // keys (or queries) of a tile
+constexpr int BOX = TILE * 128;                  // bytes of 64 channels of a tile
+constexpr int THREADS = 384;
+constexpr int COMPUTE_WARP = 4;                  // first of eight
+constexpr float LOG2E = 1.4426950408889634f;
+
+// fp32 accumulator, bf16 operands
+constexpr uint32_t IDESC = (1u << 4) | (1u << 7) | (1u << 10) | ((TILE >> 4) << 24);
+__device__ __forceinline__ constexpr uint32_t idesc_n(int n) { return IDESC | (static_cast<uint32_t>(n >> 3) << 17); }
+constexpr uint32_t B_MN = 1u << 16;      // second operand with its rows contiguous
+
+// first operand from tensor memory: a lane a row, two bf16 to a column
+__device__ __forceinline__ void mma_ts(uint32_t tmem_d, uint32_t tmem_a, uint32_t b_lo, uint32_t b_hi, uint32_t idesc, uint32_t accum) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      ".reg .b64 db;\n\t"
+      "mov.b64 db, {%2, %3};\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, p;\n\t"
+      "}\n" ::"r"(tmem_d),
+      "r"(tmem_a), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accum)
+      : "memory");
+}
+
+#define MK_R8(v, o) "=r"(v[o]), "=r"(v[o + 1]), "=r"(v[o + 2]), "=r"(v[o + 3]), "=r"(v[o + 4]), "=r"(v[o + 5]), "=r"(v[o + 6]), "=r"(v[o + 7])
+#define MK_RW8(v, o) "+r"(v[o]), "+r"(v[o + 1]), "+r"(v[o + 2]), "+r"(v[o + 3]), "+r"(v[o + 4]), "+r"(v[o + 5]), "+r"(v[o + 6]), "+r"(v[o + 7])
+#define MK_RD8(v, o) "r"(v[o]), "r"(v[o + 1]), "r"(v[o + 2]), "r"(v[o + 3]), "r"(v[o + 4]), "r"(v[o + 5]), "r"(v[o + 6]), "r"(v[o + 7])
+// 32 columns of the thread's lane: request, and the wait for all requests
+__device__ __forceinline__ void tmem_req32(uint32_t taddr, uint32_t* v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, "
+      "%30, %31}, [%32];"
+      : MK_R8(v, 0), MK_R8(v, 8), MK_R8(v, 16), MK_R8(v, 24)
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait32(uint32_t* v) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" : MK_RW8(v, 0), MK_RW8(v, 8), MK_RW8(v, 16), MK_RW8(v, 24)::"memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, "
+      "%30, %31};" ::MK_RD8(v, 0),
+      MK_RD8(v, 8), MK_RD8(v, 16), MK_RD8(v, 24), "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* v) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::MK_RD8(v, 0),
+               MK_RD8(v, 8), "r"(taddr)
+               : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Registers of a warp group: all of them together stay within the THREADS * 168 of the launch
+constexpr int FEW_REGS = 80, MANY_REGS = 208;
+static_assert(128 * FEW_REGS + 256 * MANY_REGS <= THREADS * 168);
+template <int N>
+__device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// ------------------------------------------------------------------------------------------ sequences and tiles
+
+// What a CTA works on: rows r0 .. of a sequence of `len` tokens that begins at token `lo` of batch `b`
+struct Work {
+  int b, h, lo, len, r0;
+  bool padding;            // rows behind the last sequence
+};
+
+// Tiles of `rows` rows.  Sequence s has the slots from offsets[s] / rows + s on: as many as it can need without knowing the others' lengths, so
+// that a slot finds its sequence by a search over the offsets.  At most one slot of a sequence has no rows.
+struct Slots {
+  int B, N, H, rows, slots;
+  int order;               // of the CTAs: 0: the tiles of one head follow one another; causal, long rows first: 1: last tiles first, 2: first tiles first
+  const int* offsets;
+  int sequences;
+};
+
+__device__ __forceinline__ int clamp_offset(int v, int n) { return min(max(v, 0), n); }
+
+// all lanes of a warp; false: nothing to do
+__device__ __forceinline__ bool find_work(const Slots& g, const int* offsets, uint32_t block, Work& w) {
+  int slot;
+  if (g.order) {
+    w.h = static_cast<int>(block % g.H);
+    const uint32_t rest = block / g.H;
+    slot = static_cast<int>(rest % g.slots);
+    if (g.order == 1) slot = g.slots - 1 - slot;
+    w.b = static_cast<int>(rest / g.slots);
+  } else {
+    slot = static_cast<int>(block % g.slots);
+    const uint32_t rest = block / g.slots;
+    w.h = static_cast<int>(rest % g.H);
+    w.b = static_cast<int>(rest / g.H);
+  }
+  w.padding = false;
+  if (!offsets) {
+    w.lo = 0;
+    w.len = g.N;
+    w.r0 = slot * g.rows;
+    return w.r0 < w.len;
+  }
+  // (the first sequence begins with the first token)
+  auto begin = [&](int s) { return s == 0 ? 0 : clamp_offset(__ldg(offsets + s), g.N); };
+  // the last sequence whose first slot is not behind this one, 32 ways at a time
+  int lo = 0, hi = g.sequences + 1;                    // it is in [lo, hi); `sequences` stands for the rows behind the last one
+  const int lane = threadIdx.x & 31;
+  while (hi - lo > 1) {
+    const int step = (hi - lo + 31) / 32;
+    const int at = lo + lane * step;
+    const bool ok = at < hi && (at == lo || begin(at) / g.rows + at <= slot);
+    const uint32_t m = __ballot_sync(0xffffffffu, ok);
+    const int best = 31 - __clz(m);
+    lo = lo + best * step;
+    hi = min(hi, lo + step);
+  }
+  w.padding = lo == g.sequences;
+  w.lo = begin(lo);
+  w.len = (w.padding ? g.N : max(begin(lo + 1), w.lo)) - w.lo;
+  w.r0 = (slot - (w.lo / g.rows + lo)) * g.rows;
+  return w.r0 >= 0 && w.r0 < w.len;
+}
+
+// Clears the rows from `valid` on of a tile of `boxes` boxes (a warp): they belong to another sequence, and what stands there, NaN perhaps, would
+// be multiplied by zero weights.
+__device__ __forceinline__ void clear_rows(uint8_t* tile, int boxes, int valid) {
+  const int lane = threadIdx.x & 31;
+  for (int b = 0; b < boxes; ++b)
+    for (int i = valid * 8 + lane; i < TILE * 8; i += 32) *reinterpret_cast<uint4*>(tile + b * BOX + i * 16) = make_uint4(0, 0, 0, 0);
+  fence_async_smem();
+  __syncwarp();
+}
+
+// A wait behind `n` tiles (a warp): the bound of one wait for every 64 of them, as the others' waits are bounded tile by tile
+__device__ __forceinline__ bool wait_long(uint32_t bar, uint32_t parity, int n) {
+  for (int i = 0; i <= n; i += 64)
+    if (__all_sync(0xffffffffu, mbar_wait(bar, parity))) return true;
+  return false;
+}
+
+struct TileParams {
+  Slots grid;
+  int D, DP;               // channels of a head, and rounded up to 16
+  int group;               // heads of q that share one of k and v
+  int causal;
+  float scale, scale_log2;
+  int* err;
+};
+
+// The first D columns of an accumulator's row, times f, as bf16: those from `first` on in steps of `step` (multiples of 16)
+__device__ __forceinline__ void store_row(uint32_t taddr, int D, float f, __nv_bfloat16* to, bool here, int first = 0, int step = 16) {
+  for (int c = first; c < D; c += step) {
+    uint32_t v[16];
+    tmem_ld16(taddr + c, v);
+    if (here) {
+      uint4 lo, hi;
+      lo.x = pack_bf16(__uint_as_float(v[0]) * f, __uint_as_float(v[1]) * f);
+      lo.y = pack_bf16(__uint_as_float(v[2]) * f, __uint_as_float(v[3]) * f);
+      lo.z = pack_bf16(__uint_as_float(v[4]) * f, __uint_as_float(v[5]) * f);
+      lo.w = pack_bf16(__uint_as_float(v[6]) * f, __uint_as_float(v[7]) * f);
+      hi.x = pack_bf16(__uint_as_float(v[8]) * f, __uint_as_float(v[9]) * f);
+      hi.y = pack_bf16(__uint_as_float(v[10]) * f, __uint_as_float(v[11]) * f);
+      hi.z = pack_bf16(__uint_as_float(v[12]) * f, __uint_as_float(v[13]) * f);
+      hi.w = pack_bf16(__uint_as_float(v[14]) * f, __uint_as_float(v[15]) * f);
+      *reinterpret_cast<uint4*>(to + c) = lo;
+      if (c + 8 < D) *reinterpret_cast<uint4*>(to + c + 8) = hi;
+    }
+  }
+}
+__device__ __forceinline__ void zero_row(int D, __nv_bfloat16* to) {
+  for (int c = 0; c < D; c += 8) *reinterpret_cast<uint4*>(to + c) = make_uint4(0, 0, 0, 0);
+}
+
+__device__ __forceinline__ void tmem_alloc_all(volatile uint32_t* slot) {
+  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(const_cast<uint32_t*>(slot))), "r"(512u) : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_free_all(uint32_t tmem) {
+  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+}
+
+// ------------------------------------------------------------------------------------------ forward
+
+// Two tiles of 128 queries share every tile of keys and values, so that the products of one run beside the exponentials of the other.  Tensor
+// memory: S of either (128 columns, P takes the first 64 of them), O of either (up to 128).
+template <int DB>
+struct Fwd {
+  static constexpr int STAGES = DB == 1 ? 4 : 2, TILE_BYTES = DB * BOX;
+  static constexpr int K_AT = 2 * TILE_BYTES, V_AT = K_AT + STAGES * TILE_BYTES, BAR_AT = V_AT + STAGES * TILE_BYTES;
+  static constexpr int BARS = 4 * STAGES + 7;
+  static constexpr int SMEM = BAR_AT + 8 * BARS + 16 + 1024;
+  static_assert(SMEM <= SMEM_LIMIT);
+};
+constexpr uint32_t S_COLS = 128, O_AT = 256;
+// O is rescaled where the maximum has grown by more than a factor of 2^8 since: the weights then reach 256 instead of 1, with the same relative
+// rounding, and nearly all tiles leave O alone
+constexpr float MAX_GROWTH = 8.f;
+
+struct FwdParams {
+  TileParams t;
+  __nv_bfloat16* o;
+  float* lse;
+};
+
+template <int DB>
+__global__ void __launch_bounds__(THREADS, 1)
+attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                const FwdParams p) {
+  using L = Fwd<DB>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_addr = smem_u32(smem_raw);
+  const uint32_t pad = (1024u - (raw_addr & 1023u)) & 1023u;
+  const uint32_t base = raw_addr + pad, bars = base + L::BAR_AT;
+  auto k_full = [&](int s) { return bars + 8u * s; };
+  auto k_empty = [&](int s) { return bars + 8u * (L::STAGES + s); };
+  auto v_full = [&](int s) { return bars + 8u * (2 * L::STAGES + s); };
+  auto v_empty = [&](int s) { return bars + 8u * (3 * L::STAGES + s); };
+  const uint32_t q_full = bars + 8u * (4 * L::STAGES), v_fixed = q_full + 8u;
+  auto s_full = [&](int t) { return v_fixed + 8u + 8u * t; };
+  auto p_ready = [&](int t) { return v_fixed + 24u + 8u * t; };
+  const uint32_t v_fix = v_fixed + 40u;
+  volatile uint32_t* const tmem_slot = reinterpret_cast<volatile uint32_t*>(smem_raw + pad + L::BAR_AT + 8 * L::BARS);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < L::STAGES; ++s) {
+      mbar_init(k_full(s), 1);
+      mbar_init(k_empty(s), 1);
+      mbar_init(v_full(s), 1);
+      mbar_init(v_empty(s), 1);
+    }
+    mbar_init(q_full, 1);
+    mbar_init(v_fixed, 1);
+    mbar_init(v_fix, 1);
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(s_full(t), 1);
+      mbar_init(p_ready(t), 4);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    fence_async_smem();
+  }
+  if (warp == 1) tmem_alloc_all(tmem_slot);
+  const int* offsets = p.t.grid.offsets;
+  chain_begin(true, offsets);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  Work w;
+  const bool any = find_work(p.t.grid, offsets, blockIdx.x, w);
+  const int rows = any ? min(w.len - w.r0, 2 * TILE) : 0;
+  const bool causal = p.t.causal != 0;
+  auto tiles_of = [&](int t) {      // of keys, that the queries of tile t see
+    if (w.padding || rows <= t * TILE) return 0;
+    const int last = causal ? w.r0 + min(rows, (t + 1) * TILE) - 1 : w.len - 1;
+    return last / TILE + 1;
+  };
+  const int n0 = tiles_of(0), n1 = tiles_of(1), n = max(n0, n1);
+  // keys of the last tile that belong to the sequence, where other tokens follow it
+  const int tail = w.len - (n - 1) * TILE;
+  const bool fix = n > 0 && tail < TILE && w.lo + w.len < p.t.grid.N;
+
+  if (warp < COMPUTE_WARP) {
+    regs_down<FEW_REGS>();
+    if (warp == 0) {
+    // ------------------------------------------------------------------ tiles
+    if (n > 0 && elect_one()) {
+      const int hk = w.h / p.t.group;
+      mbar_expect_tx(q_full, (n1 > 0 ? 2 : 1) * L::TILE_BYTES);
+      for (int t = 0; t < (n1 > 0 ? 2 : 1); ++t)
+        for (int b = 0; b < DB; ++b) tma_load_4d(base + t * L::TILE_BYTES + b * BOX, &map_q, q_full, b * 64, w.lo + w.r0 + t * TILE, w.h, w.b);
+      int s = 0;
+      uint32_t ph = 0;
+      for (int j = 0; j < n; ++j) {
+        if (!mbar_wait(k_empty(s), ph ^ 1u)) {
+          atomicExch(p.t.err, 80);
+          break;
+        }
+        mbar_expect_tx(k_full(s), L::TILE_BYTES);
+        for (int b = 0; b < DB; ++b) tma_load_4d(base + L::K_AT + s * L::TILE_BYTES + b * BOX, &map_k, k_full(s), b * 64, w.lo + j * TILE, hk, w.b);
+        if (!mbar_wait(v_empty(s), ph ^ 1u)) {
+          atomicExch(p.t.err, 80);
+          break;
+        }
+        mbar_expect_tx(v_full(s), L::TILE_BYTES);
+        for (int b = 0; b < DB; ++b) tma_load_4d(base + L::V_AT + s * L::TILE_BYTES + b * BOX, &map_v, v_full(s), b * 64, w.lo + j * TILE, hk, w.b);
+        if (++s == L::STAGES) {
+          s = 0;
+          ph ^= 1u;
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------ products
+    if (n > 0 && elect_one()) {
+      const uint32_t hi = desc_hi(1024);
+      const uint32_t q_lo = desc_lo(base, 16), k_lo = desc_lo(base + L::K_AT, 16), v_lo = desc_lo(base + L::V_AT, BOX);
+      const uint32_t id_s = idesc_n(TILE), id_o = idesc_n(p.t.DP) | B_MN;
+      const int ksteps = p.t.DP >> 4;
+      auto scores = [&](int t, int s) {
+        const uint32_t a = q_lo + t * (L::TILE_BYTES >> 4), b = k_lo + s * (L::TILE_BYTES >> 4);
+        for (int i = 0; i < ksteps; ++i) {
+          const uint32_t at = (i >> 2) * (BOX >> 4) + (i & 3) * 2;
+          tc_mma<2, 1>(tmem + t * S_COLS, a + at, hi, b + at, hi, id_s, i > 0);
+        }
+        tc_commit(s_full(t));
+      };
+      bool ok = mbar_wait(q_full, 0) && mbar_wait(k_full(0), 0);
+      if (!ok) atomicExch(p.t.err, 81);
+      if (ok) {
+        tc_fence_after();
+        if (n0 > 0) scores(0, 0);
+        if (n1 > 0) scores(1, 0);
+        tc_commit(k_empty(0));
+      }
+      int s = 0;
+      uint32_t ph = 0;
+      for (int j = 0; j < n && ok; ++j) {
+        const int sn = s + 1 == L::STAGES ? 0 : s + 1;
+        const uint32_t phn = sn == 0 ? ph ^ 1u : ph;
+        ok = mbar_wait(v_full(s), ph);
+        if (ok && fix && j == n - 1) {
+          mbar_arrive(v_fix);
+          ok = mbar_wait(v_fixed, 0);
+        }
+        if (ok && j + 1 < n) ok = mbar_wait(k_full(sn), phn);
+        if (!ok) {
+          atomicExch(p.t.err, 82);
+          break;
+        }
+        tc_fence_after();
+        for (int t = 0; t < 2 && ok; ++t) {
+          const int nt = t == 0 ? n0 : n1;
+          if (j >= nt) continue;
+          if (!mbar_wait(p_ready(t), j & 1)) {
+            atomicExch(p.t.err, 83);
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t b = v_lo + s * (L::TILE_BYTES >> 4);
+#pragma unroll
+          for (int i = 0; i < TILE / 16; ++i)
+            mma_ts(tmem + O_AT + t * ATTN_WIDTH, tmem + t * S_COLS + i * 8, b + i * (2048 >> 4), hi, id_o, j > 0 || i > 0);
+          // (in order behind the products above: S takes the place of P)
+          if (j + 1 < nt) scores(t, sn);
+          else tc_commit(s_full(t));
+        }
+        tc_commit(v_empty(s));
+        if (j + 1 < n) tc_commit(k_empty(sn));
+        s = sn;
+        ph = phn;
+      }
+    }
+  } else if (warp == 2) {
+    // ------------------------------------------------------------------ rows of the next sequence
+    // (at the word of warp 1, which has seen the tile arrive)
+    if (fix && wait_long(v_fix, 0, n)) {
+      clear_rows(smem_raw + pad + L::V_AT + (n - 1) % L::STAGES * L::TILE_BYTES, DB, tail);
+      if (lane == 0) mbar_arrive(v_fixed);
+    }
+    }
+  } else {
+    regs_up<MANY_REGS>();
+    // ------------------------------------------------------------------ softmax
+    const int t = (warp - COMPUTE_WARP) >> 2, row = t * TILE + (warp & 3) * 32 + lane, nt = t == 0 ? n0 : n1;
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t s_at = tmem + lanes + t * S_COLS, o_at = tmem + lanes + O_AT + t * ATTN_WIDTH;
+    const float scale = p.t.scale_log2;
+    const bool here = row < rows;
+    float m = 0.f;
+    f32x2 sum[2] = {0ull, 0ull};
+    bool ok = true;
+    for (int j = 0; j < nt && ok; ++j) {
+      ok = __all_sync(0xffffffffu, mbar_wait(s_full(t), j & 1));
+      if (!ok) {
+        if (lane == 0) atomicExch(p.t.err, 84);
+        break;
+      }
+      tc_fence_after();
+      uint32_t v[TILE];
+#pragma unroll
+      for (int c = 0; c < TILE; c += 32) tmem_req32(s_at + c, v + c);
+#pragma unroll
+      for (int c = 0; c < TILE; c += 32) tmem_wait32(v + c);
+      const int k0 = j * TILE;
+      if (k0 + TILE > w.len || (causal && k0 + TILE - 1 > w.r0 + t * TILE)) {
+        const int seen = (causal ? min(w.len, w.r0 + row + 1) : w.len) - k0;
+#pragma unroll
+        for (int c = 0; c < TILE; ++c)
+          if (c >= seen) v[c] = 0xff800000u;
+      }
+      float mx[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) mx[i] = __uint_as_float(v[i]);
+#pragma unroll
+      for (int c = 4; c < TILE; ++c) mx[c & 3] = fmaxf(mx[c & 3], __uint_as_float(v[c]));
+      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
+      if (j == 0) {
+        m = top == -INFINITY ? 0.f : top;
+      } else if (__any_sync(0xffffffffu, top > m + MAX_GROWTH)) {
+        // (the scores of tile j are behind the products of tile j - 1: O is complete up to there)
+        // (row by row: what a row holds does not depend on its neighbours)
+        const float up = top > m + MAX_GROWTH ? top : m, f = ex2(m - up);
+        m = up;
+        const f32x2 f2 = f2_pack(f, f);
+        sum[0] = f2_mul(sum[0], f2);
+        sum[1] = f2_mul(sum[1], f2);
+        for (int c = 0; c < p.t.DP; c += 16) {
+          uint32_t a[16];
+          tmem_ld16(o_at + c, a);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) a[i] = __float_as_uint(__uint_as_float(a[i]) * f);
+          tmem_st16(o_at + c, a);
+        }
+      }
+      const f32x2 scale2 = f2_pack(scale, scale), m2 = f2_pack(-m, -m);
+#pragma unroll
+      for (int c = 0; c < TILE; c += 64) {
+        uint32_t packed[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          float a, b;
+          f2_unpack(f2_fma(f2_pack(__uint_as_float(v[c + 2 * i]), __uint_as_float(v[c + 2 * i + 1])), scale2, m2), a, b);
+          a = ex2(a);
+          b = ex2(b);
+          sum[i & 1] = f2_add(sum[i & 1], f2_pack(a, b));
+          packed[i] = pack_bf16(a, b);
+        }
+        tmem_st32(s_at + c / 2, packed);
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(p_ready(t));
+    }
+    if (nt > 0 && ok) {
+      ok = __all_sync(0xffffffffu, mbar_wait(s_full(t), nt & 1));
+      if (!ok && lane == 0) atomicExch(p.t.err, 84);
+    }
+    const long long token = static_cast<long long>(w.b) * p.t.grid.N + w.lo + w.r0 + row;
+    __nv_bfloat16* const to = p.o + (token * p.t.grid.H + w.h) * p.t.D;
+    if (nt > 0 && ok) {
+      tc_fence_after();
+      float a, b;
+      f2_unpack(f2_add(sum[0], sum[1]), a, b);
+      const float total = a + b;
+      store_row(o_at, p.t.D, 1.f / total, to, here);
+      if (here && p.lse)
+        p.lse[(static_cast<long long>(w.b) * p.t.grid.H + w.h) * p.t.grid.N + w.lo + w.r0 + row] = m + __log2f(total);
+    } else if (here && w.padding) {
+      zero_row(p.t.D, to);
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_free_all(tmem);
+  }
+}
+
+// ------------------------------------------------------------------------------------------ backward
+
+// 64 columns of a tile of scores and of the products dO V^T are a thread's: P = 2^(scale S - L) and dS = P (dP - delta) of them, as operands of the next
+// products where the scores stood.  `at` (S or dP): the first of the 64.
+__device__ __forceinline__ uint32_t half_cols(uint32_t at, int i) { return at + 64u * (i >> 2) + 8u * (i & 3); }      // 16 of 128 rows of the operand
+
+// Gradient of the queries.  A CTA has 128 queries of a head and goes over the keys; its eight computing warps share the rows, 64 keys of a tile to four
+// of them each.  S has two buffers, so that the products of the next tile are there when the warps come to them.  delta is computed on the way and
+// written for the second kernel.
+template <int DB>
+struct Dq {
+  static constexpr int STAGES = DB == 1 ? 4 : 2, TILE_BYTES = DB * BOX;
+  static constexpr int K_AT = 2 * TILE_BYTES, V_AT = K_AT + STAGES * TILE_BYTES, BAR_AT = V_AT + STAGES * TILE_BYTES;
+  static constexpr int BARS = 4 * STAGES + 8;
+  static constexpr int SMEM = BAR_AT + 8 * BARS + 16 + 1024;
+  static_assert(SMEM <= SMEM_LIMIT);
+};
+constexpr uint32_t DQ_DP = 256, DQ_ACC = 384;
+
+struct DqParams {
+  TileParams t;
+  const __nv_bfloat16 *o, *d_o;
+  const float* lse;
+  float* delta;
+  AttnTensor dq;
+};
+
+template <int DB>
+__global__ void __launch_bounds__(THREADS, 1)
+attn_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+               const __grid_constant__ CUtensorMap map_do, const DqParams p) {
+  using L = Dq<DB>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_addr = smem_u32(smem_raw);
+  const uint32_t pad = (1024u - (raw_addr & 1023u)) & 1023u;
+  const uint32_t base = raw_addr + pad, bars = base + L::BAR_AT;
+  auto k_full = [&](int s) { return bars + 8u * s; };
+  auto k_empty = [&](int s) { return bars + 8u * (L::STAGES + s); };
+  auto v_full = [&](int s) { return bars + 8u * (2 * L::STAGES + s); };
+  auto v_empty = [&](int s) { return bars + 8u * (3 * L::STAGES + s); };
+  const uint32_t q_full = bars + 8u * (4 * L::STAGES), k_fixed = q_full + 8u, dp_full = q_full + 16u, ds_ready = q_full + 24u, dq_full = q_full + 32u;
+  auto s_full = [&](int b) { return q_full + 40u + 8u * b; };
+  const uint32_t k_fix = q_full + 56u;
+  volatile uint32_t* const tmem_slot = reinterpret_cast<volatile uint32_t*>(smem_raw + pad + L::BAR_AT + 8 * L::BARS);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < 4 * L::STAGES; ++s) mbar_init(bars + 8u * s, 1);
+    mbar_init(q_full, 1);
+    mbar_init(k_fixed, 1);
+    mbar_init(k_fix, 1);
+    mbar_init(dp_full, 1);
+    mbar_init(ds_ready, 8);
+    mbar_init(dq_full, 1);
+    mbar_init(s_full(0), 1);
+    mbar_init(s_full(1), 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    fence_async_smem();
+  }
+  if (warp == 1) tmem_alloc_all(tmem_slot);
+  const int* offsets = p.t.grid.offsets;
+  const __nv_bfloat16 *out = p.o, *d_out = p.d_o;
+  const float* lse = p.lse;
+  chain_begin(true, offsets, out, d_out, lse);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  Work w;
+  const bool any = find_work(p.t.grid, offsets, blockIdx.x, w);
+  const int rows = any ? min(w.len - w.r0, TILE) : 0;
+  const bool causal = p.t.causal != 0;
+  const int n = rows == 0 || w.padding ? 0 : (causal ? w.r0 + rows - 1 : w.len - 1) / TILE + 1;
+  const int tail = w.len - (n - 1) * TILE;
+  const bool fix = n > 0 && tail < TILE && w.lo + w.len < p.t.grid.N;
+
+  if (warp < COMPUTE_WARP) {
+    regs_down<FEW_REGS>();
+    if (warp == 0) {
+      // ---------------------------------------------------------------- tiles
+      if (n > 0 && elect_one()) {
+        const int hk = w.h / p.t.group;
+        mbar_expect_tx(q_full, 2 * L::TILE_BYTES);
+        for (int b = 0; b < DB; ++b) {
+          tma_load_4d(base + b * BOX, &map_q, q_full, b * 64, w.lo + w.r0, w.h, w.b);
+          tma_load_4d(base + L::TILE_BYTES + b * BOX, &map_do, q_full, b * 64, w.lo + w.r0, w.h, w.b);
+        }
+        int s = 0;
+        uint32_t ph = 0;
+        for (int j = 0; j < n; ++j) {
+          if (!mbar_wait(k_empty(s), ph ^ 1u)) {
+            atomicExch(p.t.err, 85);
+            break;
+          }
+          mbar_expect_tx(k_full(s), L::TILE_BYTES);
+          for (int b = 0; b < DB; ++b) tma_load_4d(base + L::K_AT + s * L::TILE_BYTES + b * BOX, &map_k, k_full(s), b * 64, w.lo + j * TILE, hk, w.b);
+          if (!mbar_wait(v_empty(s), ph ^ 1u)) {
+            atomicExch(p.t.err, 85);
+            break;
+          }
+          mbar_expect_tx(v_full(s), L::TILE_BYTES);
+          for (int b = 0; b < DB; ++b) tma_load_4d(base + L::V_AT + s * L::TILE_BYTES + b * BOX, &map_v, v_full(s), b * 64, w.lo + j * TILE, hk, w.b);
+          if (++s == L::STAGES) {
+            s = 0;
+            ph ^= 1u;
+          }
+        }
+      }
+    } else if (warp == 1) {
+      // ---------------------------------------------------------------- products
+      if (n > 0 && elect_one()) {
+        const uint32_t hi = desc_hi(1024);
+        const uint32_t q_lo = desc_lo(base, 16), do_lo = desc_lo(base + L::TILE_BYTES, 16), k_lo = desc_lo(base + L::K_AT, 16),
+                       v_lo = desc_lo(base + L::V_AT, 16), km_lo = desc_lo(base + L::K_AT, BOX);
+        const uint32_t id_s = idesc_n(TILE), id_q = idesc_n(p.t.DP) | B_MN;
+        const int ksteps = p.t.DP >> 4;
+        auto over_channels = [&](uint32_t d, uint32_t a, uint32_t b) {
+          for (int i = 0; i < ksteps; ++i) {
+            const uint32_t at = (i >> 2) * (BOX >> 4) + (i & 3) * 2;
+            tc_mma<2, 1>(d, a + at, hi, b + at, hi, id_s, i > 0);
+          }
+        };
+        bool ok = mbar_wait(q_full, 0) && mbar_wait(k_full(0), 0);
+        if (!ok) atomicExch(p.t.err, 86);
+        if (ok) {
+          tc_fence_after();
+          over_channels(tmem, q_lo, k_lo);
+          tc_commit(s_full(0));
+        }
+        int s = 0;
+        uint32_t ph = 0;
+        for (int j = 0; j < n && ok; ++j) {
+          const int sn = s + 1 == L::STAGES ? 0 : s + 1;
+          const uint32_t phn = sn == 0 ? ph ^ 1u : ph;
+          const uint32_t at = s * (L::TILE_BYTES >> 4);
+          if (!mbar_wait(v_full(s), ph)) {
+            atomicExch(p.t.err, 87);
+            break;
+          }
+          tc_fence_after();
+          over_channels(tmem + DQ_DP, do_lo, v_lo + at);
+          tc_commit(dp_full);
+          tc_commit(v_empty(s));
+          if (j + 1 < n) {
+            // (the other buffer of S has been read: dS of tile j - 1 was ready)
+            if (!mbar_wait(k_full(sn), phn)) {
+              atomicExch(p.t.err, 87);
+              break;
+            }
+            tc_fence_after();
+            over_channels(tmem + ((j + 1) & 1) * S_COLS, q_lo, k_lo + sn * (L::TILE_BYTES >> 4));
+            tc_commit(s_full((j + 1) & 1));
+          }
+          const bool clear = fix && j == n - 1;
+          if (clear) mbar_arrive(k_fix);
+          ok = (!clear || mbar_wait(k_fixed, 0)) && mbar_wait(ds_ready, j & 1);
+          if (!ok) {
+            atomicExch(p.t.err, 88);
+            break;
+          }
+          tc_fence_after();
+#pragma unroll
+          for (int i = 0; i < TILE / 16; ++i)
+            mma_ts(tmem + DQ_ACC, half_cols(tmem + DQ_DP, i), km_lo + at + i * (2048 >> 4), hi, id_q, j > 0 || i > 0);
+          tc_commit(k_empty(s));
+          s = sn;
+          ph = phn;
+        }
+        if (ok) tc_commit(dq_full);
+      }
+    } else if (warp == 2) {
+      // ---------------------------------------------------------------- keys of the next sequence
+      if (fix && wait_long(k_fix, 0, n)) {
+        clear_rows(smem_raw + pad + L::K_AT + (n - 1) % L::STAGES * L::TILE_BYTES, DB, tail);
+        if (lane == 0) mbar_arrive(k_fixed);
+      }
+    }
+  } else {
+    regs_up<MANY_REGS>();
+    // ------------------------------------------------------------------ P and dS
+    const int x = (warp - COMPUTE_WARP) >> 2, row = (warp & 3) * 32 + lane;
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const bool here = row < rows;
+    const long long token = static_cast<long long>(w.b) * p.t.grid.N + w.lo + w.r0 + row;
+    const long long stat = (static_cast<long long>(w.b) * p.t.grid.H + w.h) * p.t.grid.N + w.lo + w.r0 + row;
+    float l = 0.f, delta = 0.f;
+    if (here && n > 0) {
+      l = __ldg(lse + stat);
+      const uint4* a = reinterpret_cast<const uint4*>(out + (token * p.t.grid.H + w.h) * p.t.D);
+      const uint4* b = reinterpret_cast<const uint4*>(d_out + (token * p.t.grid.H + w.h) * p.t.D);
+      for (int c = 0; c < p.t.D / 8; ++c) {
+        const uint4 u = __ldg(a + c), v = __ldg(b + c);
+        const uint32_t us[4] = {u.x, u.y, u.z, u.w}, vs[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          delta = fmaf(__uint_as_float(us[i] << 16), __uint_as_float(vs[i] << 16), delta);
+          delta = fmaf(__uint_as_float(us[i] & 0xffff0000u), __uint_as_float(vs[i] & 0xffff0000u), delta);
+        }
+      }
+      if (x == 0) p.delta[stat] = delta;
+    }
+    const float scale = p.t.scale_log2;
+    const f32x2 scale2 = f2_pack(scale, scale), l2 = f2_pack(-l, -l), delta2 = f2_pack(-delta, -delta);
+    bool ok = true;
+    for (int j = 0; j < n; ++j) {
+      ok = __all_sync(0xffffffffu, mbar_wait(s_full(j & 1), (j >> 1) & 1));
+      if (!ok) break;
+      tc_fence_after();
+      uint32_t v[64];
+      const uint32_t s_at = tmem + lanes + (j & 1) * S_COLS + x * 64, dp_at = tmem + lanes + DQ_DP + x * 64;
+      tmem_req32(s_at, v);
+      tmem_req32(s_at + 32, v + 32);
+      tmem_wait32(v);
+      tmem_wait32(v + 32);
+#pragma unroll
+      for (int c = 0; c < 64; c += 2) {
+        float a, b;
+        f2_unpack(f2_fma(f2_pack(__uint_as_float(v[c]), __uint_as_float(v[c + 1])), scale2, l2), a, b);
+        v[c] = __float_as_uint(ex2(a));
+        v[c + 1] = __float_as_uint(ex2(b));
+      }
+      ok = __all_sync(0xffffffffu, mbar_wait(dp_full, j & 1));
+      if (!ok) break;
+      tc_fence_after();
+      const int k0 = j * TILE + x * 64;
+      const bool edge = k0 + 64 > w.len || (causal && k0 + 63 > w.r0);
+      const int seen = (causal ? min(w.len, w.r0 + row + 1) : w.len) - k0;
+      uint32_t packed[32];
+#pragma unroll
+      for (int h = 0; h < 64; h += 32) {
+        uint32_t d[32];
+        tmem_req32(dp_at + h, d);
+        tmem_wait32(d);
+#pragma unroll
+        for (int c = 0; c < 32; c += 2) {
+          float a, b;
+          f2_unpack(f2_mul(f2_add(f2_pack(__uint_as_float(d[c]), __uint_as_float(d[c + 1])), delta2),
+                           f2_pack(__uint_as_float(v[h + c]), __uint_as_float(v[h + c + 1]))),
+                    a, b);
+          if (edge) {
+            a = h + c < seen ? a : 0.f;
+            b = h + c + 1 < seen ? b : 0.f;
+          }
+          packed[(h + c) / 2] = pack_bf16(a, b);
+        }
+      }
+      tmem_st32(dp_at, packed);
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(ds_ready);
+    }
+    if (ok && n > 0) ok = __all_sync(0xffffffffu, mbar_wait(dq_full, 0));
+    if (!ok && lane == 0) atomicExch(p.t.err, 89);
+    __nv_bfloat16* const to = p.dq.ptr + w.b * p.dq.batch + (w.lo + w.r0 + row) * p.dq.token + w.h * p.dq.head;
+    if (n > 0 && ok) {
+      tc_fence_after();
+      store_row(tmem + lanes + DQ_ACC, p.t.D, p.t.scale, to, here, x * 16, 32);
+    } else if (here && w.padding && x == 0) {
+      zero_row(p.t.D, to);
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_free_all(tmem);
+  }
+}
+
+// Gradients of keys and values.  A CTA has 128 keys of a head and goes over the queries of all heads that share it, so that nothing is added up
+// afterwards.  Scores are transposed (a thread's row is a key), so that P and dS come out of tensor memory as the first operands of the
+// products with dO and Q.  Heads of up to 64 channels: two buffers of S, the next tile's scores run in front of the products that wait for the
+// warps; above, tensor memory is full with one, and they run behind the first of these.
+template <int DB>
+struct Dkv {
+  static constexpr int STAGES = DB == 1 ? 3 : 2, TILE_BYTES = DB * BOX, S_BUFS = DB == 1 ? 2 : 1;
+  static constexpr int STAGE_AT = 2 * TILE_BYTES, STAGE = 2 * TILE_BYTES, STAT_AT = STAGE_AT + STAGES * STAGE, STAT = 2 * TILE * 4;
+  static constexpr int BAR_AT = STAT_AT + STAGES * STAT, BARS = 4 * STAGES + 9;
+  static constexpr int SMEM = BAR_AT + 8 * BARS + 16 + 1024;
+  static constexpr uint32_t DP_AT = S_BUFS * S_COLS, DV_AT = DP_AT + S_COLS, DK_AT = DV_AT + DB * 64;
+  static_assert(SMEM <= SMEM_LIMIT && DK_AT + DB * 64 == 512);
+};
+
+struct DkvParams {
+  TileParams t;
+  int heads_q;
+  const float *lse, *delta;
+  AttnTensor dk, dv;
+};
+
+template <int DB>
+__global__ void __launch_bounds__(THREADS, 1)
+attn_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                const __grid_constant__ CUtensorMap map_do, const DkvParams p) {
+  using L = Dkv<DB>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_addr = smem_u32(smem_raw);
+  const uint32_t pad = (1024u - (raw_addr & 1023u)) & 1023u;
+  const uint32_t base = raw_addr + pad, bars = base + L::BAR_AT;
+  auto q_full = [&](int s) { return bars + 8u * s; };
+  auto do_full = [&](int s) { return bars + 8u * (L::STAGES + s); };
+  auto empty = [&](int s) { return bars + 8u * (2 * L::STAGES + s); };
+  auto stat_full = [&](int s) { return bars + 8u * (3 * L::STAGES + s); };
+  const uint32_t kv_full = bars + 8u * (4 * L::STAGES), fixed = kv_full + 8u, p_ready = kv_full + 16u, ds_ready = kv_full + 24u,
+                 dp_full = kv_full + 32u, acc_full = kv_full + 40u;
+  auto s_full = [&](int b) { return kv_full + 48u + 8u * b; };
+  const uint32_t fix_bar = kv_full + 64u;
+  volatile uint32_t* const tmem_slot = reinterpret_cast<volatile uint32_t*>(smem_raw + pad + L::BAR_AT + 8 * L::BARS);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < 4 * L::STAGES; ++s) mbar_init(bars + 8u * s, 1);
+    mbar_init(kv_full, 1);
+    mbar_init(fixed, 1);
+    mbar_init(fix_bar, 1);
+    mbar_init(p_ready, 8);
+    mbar_init(ds_ready, 8);
+    mbar_init(dp_full, 1);
+    mbar_init(acc_full, 1);
+    mbar_init(s_full(0), 1);
+    mbar_init(s_full(1), 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    fence_async_smem();
+  }
+  if (warp == 1) tmem_alloc_all(tmem_slot);
+  const int* offsets = p.t.grid.offsets;
+  const float *lse = p.lse, *delta = p.delta;
+  chain_begin(true, offsets, lse, delta);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  Work w;
+  const bool any = find_work(p.t.grid, offsets, blockIdx.x, w);
+  const int rows = any ? min(w.len - w.r0, TILE) : 0;
+  const bool causal = p.t.causal != 0;
+  // tiles of queries, from the first that sees one of these keys, of one head after the other
+  const int q_first = causal ? w.r0 / TILE : 0, q_tiles = rows == 0 || w.padding ? 0 : (w.len + TILE - 1) / TILE - q_first;
+  const int n = q_tiles * p.t.group, h0 = w.h * p.t.group;
+  const int tail = w.len - (q_first + q_tiles - 1) * TILE;
+  const bool fix = n > 0 && tail < TILE && w.lo + w.len < p.t.grid.N;
+
+  if (warp < COMPUTE_WARP) {
+    regs_down<FEW_REGS>();
+    if (warp == 0) {
+      // ---------------------------------------------------------------- tiles
+      if (n > 0 && elect_one()) {
+        mbar_expect_tx(kv_full, 2 * L::TILE_BYTES);
+        for (int b = 0; b < DB; ++b) {
+          tma_load_4d(base + b * BOX, &map_k, kv_full, b * 64, w.lo + w.r0, w.h, w.b);
+          tma_load_4d(base + L::TILE_BYTES + b * BOX, &map_v, kv_full, b * 64, w.lo + w.r0, w.h, w.b);
+        }
+        int s = 0, t = 0, g = 0;
+        uint32_t ph = 0;
+        for (int j = 0; j < n; ++j) {
+          if (!mbar_wait(empty(s), ph ^ 1u)) {
+            atomicExch(p.t.err, 90);
+            break;
+          }
+          const uint32_t at = base + L::STAGE_AT + s * L::STAGE;
+          const int q0 = w.lo + (q_first + t) * TILE;
+          mbar_expect_tx(q_full(s), L::TILE_BYTES);
+          for (int b = 0; b < DB; ++b) tma_load_4d(at + b * BOX, &map_q, q_full(s), b * 64, q0, h0 + g, w.b);
+          mbar_expect_tx(do_full(s), L::TILE_BYTES);
+          for (int b = 0; b < DB; ++b) tma_load_4d(at + L::TILE_BYTES + b * BOX, &map_do, do_full(s), b * 64, q0, h0 + g, w.b);
+          if (++t == q_tiles) {
+            t = 0;
+            ++g;
+          }
+          if (++s == L::STAGES) {
+            s = 0;
+            ph ^= 1u;
+          }
+        }
+      }
+    } else if (warp == 1) {
+      // ---------------------------------------------------------------- products
+      if (n > 0 && elect_one()) {
+        const uint32_t hi = desc_hi(1024);
+        const uint32_t k_lo = desc_lo(base, 16), v_lo = desc_lo(base + L::TILE_BYTES, 16), q_lo = desc_lo(base + L::STAGE_AT, 16),
+                       qm_lo = desc_lo(base + L::STAGE_AT, BOX);
+        const uint32_t id_s = idesc_n(TILE), id_d = idesc_n(p.t.DP) | B_MN;
+        constexpr uint32_t DO = L::TILE_BYTES >> 4;
+        const int ksteps = p.t.DP >> 4;
+        auto over_channels = [&](uint32_t d, uint32_t a, uint32_t b) {
+          for (int i = 0; i < ksteps; ++i) {
+            const uint32_t at = (i >> 2) * (BOX >> 4) + (i & 3) * 2;
+            tc_mma<2, 1>(d, a + at, hi, b + at, hi, id_s, i > 0);
+          }
+        };
+        auto over_queries = [&](uint32_t d, uint32_t a, uint32_t b, uint32_t accum) {
+#pragma unroll
+          for (int i = 0; i < TILE / 16; ++i) mma_ts(d, half_cols(a, i), b + i * (2048 >> 4), hi, id_d, accum | (i > 0));
+        };
+        bool ok = mbar_wait(kv_full, 0) && mbar_wait(q_full(0), 0) && mbar_wait(do_full(0), 0);
+        if (!ok) atomicExch(p.t.err, 91);
+        if (ok) {
+          tc_fence_after();
+          over_channels(tmem, k_lo, q_lo);
+          tc_commit(s_full(0));
+          over_channels(tmem + L::DP_AT, v_lo, q_lo + DO);
+          tc_commit(dp_full);
+        }
+        int s = 0, t = 0, g = 0;
+        uint32_t ph = 0;
+        for (int j = 0; j < n && ok; ++j) {
+          const int sn = s + 1 == L::STAGES ? 0 : s + 1;
+          const uint32_t phn = sn == 0 ? ph ^ 1u : ph;
+          const uint32_t at = s * (L::STAGE >> 4), atn = sn * (L::STAGE >> 4);
+          const int buf = L::S_BUFS == 2 ? j & 1 : 0, bufn = L::S_BUFS == 2 ? (j + 1) & 1 : 0;
+          auto next_scores = [&] {
+            if (j + 1 == n) return true;
+            if (!mbar_wait(q_full(sn), phn)) {
+              atomicExch(p.t.err, 91);
+              return false;
+            }
+            tc_fence_after();
+            over_channels(tmem + bufn * S_COLS, k_lo, q_lo + atn);
+            tc_commit(s_full(bufn));
+            return true;
+          };
+          if (L::S_BUFS == 2) ok = next_scores();
+          if (!ok) break;
+          const bool clear = fix && t == q_tiles - 1;
+          if (clear) mbar_arrive(fix_bar);
+          ok = (!clear || mbar_wait(fixed, g & 1)) && mbar_wait(p_ready, j & 1);
+          if (!ok) {
+            atomicExch(p.t.err, 92);
+            break;
+          }
+          tc_fence_after();
+          over_queries(tmem + L::DV_AT, tmem + buf * S_COLS, qm_lo + at + DO, j > 0);
+          if (L::S_BUFS == 1) ok = next_scores();
+          if (!ok) break;
+          if (!mbar_wait(ds_ready, j & 1)) {
+            atomicExch(p.t.err, 92);
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          over_queries(tmem + L::DK_AT, tmem + L::DP_AT, qm_lo + at, j > 0);
+          tc_commit(empty(s));
+          if (j + 1 < n) {
+            if (!mbar_wait(do_full(sn), phn)) {
+              atomicExch(p.t.err, 91);
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            over_channels(tmem + L::DP_AT, v_lo, q_lo + atn + DO);
+            tc_commit(dp_full);
+          }
+          if (++t == q_tiles) {
+            t = 0;
+            ++g;
+          }
+          s = sn;
+          ph = phn;
+        }
+        if (ok) tc_commit(acc_full);
+      }
+    } else if (warp == 2) {
+      // ---------------------------------------------------------------- L and delta of the queries
+      int s = 0, t = 0, g = 0;
+      uint32_t ph = 0;
+      for (int j = 0; j < n; ++j) {
+        if (!__all_sync(0xffffffffu, mbar_wait(empty(s), ph ^ 1u))) {
+          if (lane == 0) atomicExch(p.t.err, 90);
+          break;
+        }
+        float* const to = reinterpret_cast<float*>(smem_raw + pad + L::STAT_AT + s * L::STAT);
+        const int q0 = (q_first + t) * TILE;
+        const long long from = (static_cast<long long>(w.b) * p.heads_q + h0 + g) * p.t.grid.N + w.lo + q0;
+#pragma unroll
+        for (int i = 0; i < TILE; i += 32) {
+          const bool in = q0 + i + lane < w.len;
+          to[i + lane] = in ? -__ldg(lse + from + i + lane) : 0.f;
+          to[TILE + i + lane] = in ? -__ldg(delta + from + i + lane) : 0.f;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(stat_full(s));
+        if (++t == q_tiles) {
+          t = 0;
+          ++g;
+        }
+        if (++s == L::STAGES) {
+          s = 0;
+          ph ^= 1u;
+        }
+      }
+    } else if (fix) {
+      // ---------------------------------------------------------------- queries of the next sequence
+      for (int g = 0; g < p.t.group; ++g) {
+        if (!wait_long(fix_bar, g & 1, q_tiles)) break;
+        clear_rows(smem_raw + pad + L::STAGE_AT + (g * q_tiles + q_tiles - 1) % L::STAGES * L::STAGE, 2 * DB, tail);
+        if (lane == 0) mbar_arrive(fixed);
+      }
+    }
+  } else {
+    regs_up<MANY_REGS>();
+    // ------------------------------------------------------------------ P and dS, transposed
+    const int x = (warp - COMPUTE_WARP) >> 2, row = (warp & 3) * 32 + lane;
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const bool here = row < rows;
+    const f32x2 scale2 = f2_pack(p.t.scale_log2, p.t.scale_log2);
+    bool ok = true;
+    int s = 0, t = 0;
+    uint32_t ph = 0;
+    for (int j = 0; j < n; ++j) {
+      const int buf = L::S_BUFS == 2 ? j & 1 : 0;
+      ok = __all_sync(0xffffffffu, mbar_wait(stat_full(s), ph) && mbar_wait(s_full(buf), L::S_BUFS == 2 ? (j >> 1) & 1 : j & 1));
+      if (!ok) break;
+      tc_fence_after();
+      const float* const stats = reinterpret_cast<const float*>(smem_raw + pad + L::STAT_AT + s * L::STAT) + x * 64;
+      const int q0 = (q_first + t) * TILE + x * 64;
+      // the queries that see this key are the columns from `from` to `to`
+      const bool edge = q0 + 64 > w.len || (causal && q0 < w.r0 + TILE - 1);
+      const int from = causal ? w.r0 + row - q0 : 0, to = w.len - q0;
+      uint32_t v[64], packed[32];
+      const uint32_t s_at = tmem + lanes + buf * S_COLS + x * 64, dp_at = tmem + lanes + L::DP_AT + x * 64;
+      tmem_req32(s_at, v);
+      tmem_req32(s_at + 32, v + 32);
+      tmem_wait32(v);
+      tmem_wait32(v + 32);
+#pragma unroll
+      for (int c = 0; c < 64; c += 4) {
+        const float4 l = *reinterpret_cast<const float4*>(stats + c);
+        float e[4];
+        f2_unpack(f2_fma(f2_pack(__uint_as_float(v[c]), __uint_as_float(v[c + 1])), scale2, f2_pack(l.x, l.y)), e[0], e[1]);
+        f2_unpack(f2_fma(f2_pack(__uint_as_float(v[c + 2]), __uint_as_float(v[c + 3])), scale2, f2_pack(l.z, l.w)), e[2], e[3]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          e[i] = ex2(e[i]);
+          if (edge) e[i] = c + i >= from && c + i < to ? e[i] : 0.f;
+          v[c + i] = __float_as_uint(e[i]);
+        }
+        packed[c / 2] = pack_bf16(e[0], e[1]);
+        packed[c / 2 + 1] = pack_bf16(e[2], e[3]);
+      }
+      tmem_st32(s_at, packed);
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(p_ready);
+      ok = __all_sync(0xffffffffu, mbar_wait(dp_full, j & 1));
+      if (!ok) break;
+      tc_fence_after();
+#pragma unroll
+      for (int h = 0; h < 64; h += 32) {
+        uint32_t d[32];
+        tmem_req32(dp_at + h, d);
+        tmem_wait32(d);
+#pragma unroll
+        for (int c = 0; c < 32; c += 4) {
+          const float4 l = *reinterpret_cast<const float4*>(stats + TILE + h + c);
+          float e[4];
+          f2_unpack(f2_mul(f2_add(f2_pack(__uint_as_float(d[c]), __uint_as_float(d[c + 1])), f2_pack(l.x, l.y)),
+                           f2_pack(__uint_as_float(v[h + c]), __uint_as_float(v[h + c + 1]))),
+                    e[0], e[1]);
+          f2_unpack(f2_mul(f2_add(f2_pack(__uint_as_float(d[c + 2]), __uint_as_float(d[c + 3])), f2_pack(l.z, l.w)),
+                           f2_pack(__uint_as_float(v[h + c + 2]), __uint_as_float(v[h + c + 3]))),
+                    e[2], e[3]);
+          if (edge) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) e[i] = h + c + i >= from && h + c + i < to ? e[i] : 0.f;
+          }
+          packed[(h + c) / 2] = pack_bf16(e[0], e[1]);
+          packed[(h + c) / 2 + 1] = pack_bf16(e[2], e[3]);
+        }
+      }
+      tmem_st32(dp_at, packed);
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(ds_ready);
+      if (++t == q_tiles) t = 0;
+      if (++s == L::STAGES) {
+        s = 0;
+        ph ^= 1u;
+      }
+    }
+    if (ok && n > 0) ok = __all_sync(0xffffffffu, mbar_wait(acc_full, 0));
+    if (!ok && lane == 0) atomicExch(p.t.err, 93);
+    // half of the warps store either
+    const AttnTensor& d = x == 0 ? p.dv : p.dk;
+    __nv_bfloat16* const to = d.ptr + w.b * d.batch + (w.lo + w.r0 + row) * d.token + w.h * d.head;
+    if (n > 0 && ok) {
+      tc_fence_after();
+      store_row(tmem + lanes + (x == 0 ? L::DV_AT : L::DK_AT), p.t.D, x == 0 ? 1.f : p.t.scale, to, here);
+    } else if (here && w.padding) {
+      zero_row(p.t.D, to);
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_free_all(tmem);
+  }
+}
+
+// ------------------------------------------------------------------------------------------ host
+
+bool map_of(CUtensorMap* map, const AttnTensor& t, const AttnShape& p, int heads) {
+  GemmOperand op;
+  op.ptr = t.ptr;
+  op.rows = p.N;
+  op.mn_major = 0;
+  op.ld = t.token;
+  op.zs_lo = t.head;
+  op.zs_hi = t.batch;
+  return make_map(map, op, p.D, 2, heads, p.B, TILE);
+}
+
+Slots slots_of(const AttnShape& p, int heads, int rows, int causal_order) {
+  Slots g;
+  g.B = p.B;
+  g.N = p.N;
+  g.H = heads;
+  g.rows = rows;
+  g.order = p.causal ? causal_order : 0;
+  g.slots = p.offsets ? p.N / rows + p.sequences + 1 : (p.N + rows - 1) / rows;
+  g.offsets = p.offsets;
+  g.sequences = p.sequences;
+  return g;
+}
+long long blocks_of(const Slots& g) { return 1ll * g.slots * g.H * g.B; }
+
+bool shape_ok(const AttnShape& p) {
+  return p.B > 0 && p.N > 0 && p.H > 0 && p.Hk > 0 && p.H % p.Hk == 0 && p.D > 0 && p.D % 8 == 0 && p.D <= ATTN_WIDTH && p.scale > 0.f &&
+         (!p.offsets || (p.B == 1 && p.sequences >= 0)) && blocks_of(slots_of(p, p.H, TILE, 1)) < (1ll << 31);
+}
+
+TileParams tile_params(const AttnShape& p, const Slots& g, int* err) {
+  TileParams t;
+  t.grid = g;
+  t.D = p.D;
+  t.DP = (p.D + 15) / 16 * 16;
+  t.group = p.H / p.Hk;
+  t.causal = p.causal;
+  t.scale = p.scale;
+  t.scale_log2 = p.scale * LOG2E;
+  t.err = err;
+  return t;
+}
+
+template <int DB>
+cudaError_t launch_fwd(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const FwdParams& p, cudaStream_t s) {
+  static std::atomic<uint64_t> devices;
+  const cudaError_t e = allow_shared_memory(devices, reinterpret_cast<const void*>(&attn_fwd_kernel<DB>), Fwd<DB>::SMEM);
+  if (e != cudaSuccess) return e;
+  return launch_chained(attn_fwd_kernel<DB>, dim3(static_cast<unsigned>(blocks_of(p.t.grid))), dim3(THREADS), Fwd<DB>::SMEM, s, 1, true, q, k, v, p);
+}
+template <int DB>
+cudaError_t launch_dq(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& g, const DqParams& p, cudaStream_t s) {
+  static std::atomic<uint64_t> devices;
+  const cudaError_t e = allow_shared_memory(devices, reinterpret_cast<const void*>(&attn_dq_kernel<DB>), Dq<DB>::SMEM);
+  if (e != cudaSuccess) return e;
+  return launch_chained(attn_dq_kernel<DB>, dim3(static_cast<unsigned>(blocks_of(p.t.grid))), dim3(THREADS), Dq<DB>::SMEM, s, 1, true, q, k, v, g, p);
+}
+template <int DB>
+cudaError_t launch_dkv(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& g, const DkvParams& p, cudaStream_t s) {
+  static std::atomic<uint64_t> devices;
+  const cudaError_t e = allow_shared_memory(devices, reinterpret_cast<const void*>(&attn_dkv_kernel<DB>), Dkv<DB>::SMEM);
+  if (e != cudaSuccess) return e;
+  return launch_chained(attn_dkv_kernel<DB>, dim3(static_cast<unsigned>(blocks_of(p.t.grid))), dim3(THREADS), Dkv<DB>::SMEM, s, 1, true, q, k, v, g, p);
+}
+
+}  // namespace
+
+cudaError_t attention_fwd(const AttnShape& p, const AttnTensor& q, const AttnTensor& k, const AttnTensor& v, __nv_bfloat16* o, float* lse, int* err,
+                          cudaStream_t s) {
+  if (!shape_ok(p) || (reinterpret_cast<uintptr_t>(o) & 15)) return cudaErrorInvalidValue;
+  bind_context(s);
+  CUtensorMap mq, mk_, mv;
+  if (!map_of(&mq, q, p, p.H) || !map_of(&mk_, k, p, p.Hk) || !map_of(&mv, v, p, p.Hk)) return cudaErrorInvalidValue;
+  FwdParams f;
+  f.t = tile_params(p, slots_of(p, p.H, 2 * TILE, 1), err);
+  f.o = o;
+  f.lse = lse;
+  return p.D <= 64 ? launch_fwd<1>(mq, mk_, mv, f, s) : launch_fwd<2>(mq, mk_, mv, f, s);
+}
+
+cudaError_t attention_bwd(const AttnShape& p, const AttnTensor& q, const AttnTensor& k, const AttnTensor& v, const __nv_bfloat16* o,
+                          const __nv_bfloat16* d_o, const float* lse, float* delta, const AttnTensor& dq, const AttnTensor& dk, const AttnTensor& dv,
+                          int* err, cudaStream_t s) {
+  auto bad = [](const AttnTensor& t) { return (reinterpret_cast<uintptr_t>(t.ptr) & 15) || ((t.token | t.head | t.batch) & 7); };
+  if (!shape_ok(p) || ((reinterpret_cast<uintptr_t>(o) | reinterpret_cast<uintptr_t>(d_o)) & 15) || bad(dq) || bad(dk) || bad(dv))
+    return cudaErrorInvalidValue;
+  bind_context(s);
+  const AttnTensor g{const_cast<__nv_bfloat16*>(d_o), 1ll * p.H * p.D, p.D, 1ll * p.N * p.H * p.D};
+  CUtensorMap mq, mk_, mv, mg;
+  if (!map_of(&mq, q, p, p.H) || !map_of(&mk_, k, p, p.Hk) || !map_of(&mv, v, p, p.Hk) || !map_of(&mg, g, p, p.H)) return cudaErrorInvalidValue;
+  DqParams a;
+  a.t = tile_params(p, slots_of(p, p.H, TILE, 1), err);
+  a.o = o;
+  a.d_o = d_o;
+  a.lse = lse;
+  a.delta = delta;
+  a.dq = dq;
+  DkvParams b;
+  b.t = tile_params(p, slots_of(p, p.Hk, TILE, 2), err);
+  b.heads_q = p.H;
+  b.lse = lse;
+  b.delta = delta;
+  b.dk = dk;
+  b.dv = dv;
+  const cudaError_t e = p.D <= 64 ? launch_dq<1>(mq, mk_, mv, mg, a, s) : launch_dq<2>(mq, mk_, mv, mg, a, s);
+  if (e != cudaSuccess) return e;
+  return p.D <= 64 ? launch_dkv<1>(mq, mk_, mv, mg, b, s) : launch_dkv<2>(mq, mk_, mv, mg, b, s);
+}
+
+}  // namespace mk

@@ -1,0 +1,35 @@
+// Softmax attention of tokens with themselves: whole prompts, causal or not, grouped heads, batches or packed sequences (attention.cu).
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace mk {
+
+constexpr int ATTN_WIDTH = 128;        // most channels of a head (a multiple of 8)
+
+// A tensor [B, N, heads, D] in elements; D is dense, strides are multiples of 8 and the base is 16-byte aligned
+struct AttnTensor {
+  __nv_bfloat16* ptr;
+  long long token, head, batch;
+};
+
+struct AttnShape {
+  int B, N, H, Hk, D;        // H: heads of q and o; Hk: of k and v, H / Hk of q share one
+  int causal;
+  float scale;               // > 0
+  // packed sequences (B = 1): sequence i has the tokens offsets[i] .. offsets[i + 1], not decreasing, within N; null: one sequence per batch.
+  // What the offsets do not cover is written as zeros behind the last sequence.
+  const int* offsets;
+  int sequences;
+};
+
+// o [B, N, H, D] dense; lse [B, H, N]: log2 of the sum of exponentials of every row (with `lse` null it is not written)
+cudaError_t attention_fwd(const AttnShape& p, const AttnTensor& q, const AttnTensor& k, const AttnTensor& v, __nv_bfloat16* o, float* lse, int* err,
+                          cudaStream_t s);
+// dq, dk, dv from o and d_o (dense, like o); delta [B, H, N]: room for the row sums of o d_o.  Two launches, no atomics.
+cudaError_t attention_bwd(const AttnShape& p, const AttnTensor& q, const AttnTensor& k, const AttnTensor& v, const __nv_bfloat16* o,
+                          const __nv_bfloat16* d_o, const float* lse, float* delta, const AttnTensor& dq, const AttnTensor& dk, const AttnTensor& dv,
+                          int* err, cudaStream_t s);
+
+}  // namespace mk

@@ -60,12 +60,12 @@ def available() -> bool:
 # number of kernel-launching calls into this extension by the current process (the column sums launch a second kernel)
 LAUNCHES = 0
 _NON_KERNEL = {"read_error_flag", "clear_error_flag", "lp_scratch_floats", "adam_entry_bytes", "peer_alloc", "peer_open",
-               "peer_close", "peer_free", "tensor_from_ptr", "set_gelu_tanh", "stream_state", "launches"}
+               "peer_close", "peer_free", "tensor_from_ptr", "set_gelu_tanh", "stream_state", "launches", "background_launches"}
 
 
 # passes over whole layers, which count their launches themselves
 _LAYERS = {"conv_forward", "conv_backward", "mlp_forward", "mlp_backward", "norm_forward", "norm_backward", "spectral_forward",
-           "spectral_backward", "afno_forward", "afno_backward", "layer_norm_forward", "layer_norm_backward"}
+           "spectral_backward", "afno_forward", "afno_backward", "layer_norm", "attention", "attention_qkv"}
 
 
 class _Counting:
@@ -143,7 +143,8 @@ def gelu_approximation() -> str:
 
 
 def launch_count() -> int:
-    return LAUNCHES
+    # (passes whose autograd nodes are native launch their gradients without a call from here)
+    return LAUNCHES + (_MOD.background_launches() if _MOD is not None else 0)
 
 
 def add_launches(n: int) -> None:
@@ -172,6 +173,20 @@ ERROR_CODES = {
     71: "spectral weight gradient: accumulators never drained",
     72: "spectral weight gradient: operands never arrived",
     73: "spectral weight gradient: accumulators never completed",
+    80: "attention: a stage of keys or values never freed",
+    81: "attention: the first queries or keys never arrived",
+    82: "attention: keys or values never arrived",
+    83: "attention: weights never ready",
+    84: "attention: scores never completed",
+    85: "attention gradient (queries): a stage never freed",
+    86: "attention gradient (queries): the queries or first keys never arrived",
+    87: "attention gradient (queries): keys or values never arrived",
+    88: "attention gradient (queries): weights never ready",
+    89: "attention gradient (queries): products never completed",
+    90: "attention gradient (keys, values): a stage never freed",
+    91: "attention gradient (keys, values): queries or output gradients never arrived",
+    92: "attention gradient (keys, values): weights never ready",
+    93: "attention gradient (keys, values): products never completed",
 }
 
 

@@ -17,10 +17,8 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _ext
-from .conv import records_grad
 
 
 def _is_cl(x):
@@ -173,34 +171,6 @@ LN_CHANNELS = 8192          # most channels of a row in the kernels
 _LN_TYPES = (torch.bfloat16, torch.float32)
 
 
-class _LayerNorm(torch.autograd.Function):
-    """(y,) or, with a residual, (s, y) with s = x + residual and y = LN(s); the backward pass reads s (x) and every row's (mean, rstd)."""
-
-    @staticmethod
-    def forward(ctx, x, residual, weight, bias, eps, out_f32, train):
-        s, y, stats, w = _ext.require().layer_norm_forward(x, residual, weight, bias, float(eps), out_f32, train)
-        if train:
-            ctx.save_for_backward(x if residual is None else s, w, stats)
-        # a residual in bf16 beside an fp32 x takes its gradient in its own type
-        ctx.flags = (weight is not None or bias is not None, residual is not None, residual is not None and residual.dtype != x.dtype)
-        ctx.set_materialize_grads(False)
-        return y if residual is None else (s, y)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, *grads):
-        x, w, stats = ctx.saved_tensors
-        params, added, half = ctx.flags
-        ds, dy = grads if added else (None, grads[0])
-        if dy is None:
-            return ds, (ds.bfloat16() if ds is not None and half else ds), None, None, None, None, None
-        need_params = params and any(ctx.needs_input_grad[2:4])
-        dx, dr, dw, db = _ext.require().layer_norm_backward(x, dy, ds, w, stats, need_params, half and ctx.needs_input_grad[1])
-        need = ctx.needs_input_grad
-        return (dx if need[0] else None, ((dr if half else dx) if need[1] else None), dw if need[2] else None, db if need[3] else None,
-                None, None, None)
-
-
 def _check_layer_norm(x, residual, weight, bias, out_dtype):
     if x.dim() < 1 or x.shape[-1] < 1 or not x.dtype.is_floating_point:
         raise ValueError(f"layer norm takes floating-point tokens [..., C], got {x.dtype} {tuple(x.shape)}")
@@ -235,7 +205,7 @@ def layer_norm(x: torch.Tensor, weight, bias, eps: float = 1e-5, out_dtype: Opti
     _check_layer_norm(x, None, weight, bias, out_dtype)
     out_dtype = out_dtype or x.dtype
     if _layer_norm_native(x, out_dtype):
-        return _LayerNorm.apply(x, None, weight, bias, eps, out_dtype == torch.float32, records_grad(x, weight, bias))
+        return _ext.require().layer_norm(x, None, weight, bias, eps, out_dtype is torch.float32)[0]
     return _layer_norm_torch(x, weight, bias, eps, out_dtype)
 
 
@@ -248,6 +218,6 @@ def add_layer_norm(x: torch.Tensor, residual: torch.Tensor, weight, bias, eps: f
     dtype = torch.promote_types(x.dtype, residual.dtype)
     out_dtype = out_dtype or dtype
     if _layer_norm_native(x, out_dtype) and residual.dtype in _LN_TYPES:
-        return _LayerNorm.apply(x, residual, weight, bias, eps, out_dtype == torch.float32, records_grad(x, residual, weight, bias))
+        return tuple(_ext.require().layer_norm(x, residual, weight, bias, eps, out_dtype is torch.float32))
     s = x + residual
     return s, _layer_norm_torch(s, weight, bias, eps, out_dtype)

@@ -1,0 +1,358 @@
+"""Softmax attention (`makani_b200/ops/attention.py`) against its definition in 64 bits, sequence by sequence and head by head.
+
+Tolerances, element by element.  Half a step of bf16 is B = 2^-8 relative (`eps / 2`); fp32 sums and the special function's 2^x (two steps of
+2^-23) are counted as F = 2^-19 of the sum of magnitudes.  A score is off by at most F times sum |q k| scale, a weight P then by P (F + that).
+
+    o  = sum P v          P is rounded to bf16:     |o|  off by  (B + e) sum P |v|,   then rounded once
+    dS = P (dP - delta)   delta holds the rounded o and do: off by d = B sum |do o|;    dS is rounded to bf16
+    dq = scale sum dS k   off by  scale sum (B |dS| + P (d + e (|dP| + |delta|) + F sum|do v|)) |k|,  then rounded once
+    dk the same over the queries; dv = sum P do  off by  (B + e) sum P |do|."""
+
+import math
+
+import pytest
+import torch
+
+from makani_b200.ops import _ext
+from makani_b200.ops import attention as attn
+
+B_STEP = 2.0 ** -8
+F_STEP = 2.0 ** -19
+
+
+def _oracle(q, k, v, do, causal, scale, bounds, o_low=None):
+    """64-bit outputs and bounds of [N, H, D] tensors; `bounds`: sequences.  Rows of no sequence are zero."""
+    q, k, v, do = (t.detach().double() for t in (q, k, v, do))
+    G = q.shape[1] // k.shape[1]
+    names = ("o", "dq", "dk", "dv")
+    out = {n: torch.zeros_like(t) for n, t in zip(names, (q, q, k, v))}
+    off = {n: torch.zeros_like(t) for n, t in zip(names, (q, q, k, v))}
+    for lo, hi in bounds:
+        n = hi - lo
+        for h in range(q.shape[1]) if n else ():
+            qs, ks, vs, gs = q[lo:hi, h], k[lo:hi, h // G], v[lo:hi, h // G], do[lo:hi, h]
+            s = qs @ ks.mT * scale
+            if causal:
+                s = s.masked_fill(torch.ones(n, n, dtype=torch.bool, device=s.device).triu(1), -math.inf)
+            p = torch.softmax(s, -1)
+            o = p @ vs
+            e = F_STEP * (1 + 2 * (qs.abs() @ ks.abs().mT) * scale)
+            dp = gs @ vs.mT
+            delta = (gs * o).sum(-1, keepdim=True)
+            ds = p * (dp - delta)
+            d = B_STEP * (gs * o).abs().sum(-1, keepdim=True) + F_STEP * (gs.abs() * o.abs()).sum(-1, keepdim=True)
+            ds_off = B_STEP * ds.abs() + p * (d + e * (dp.abs() + delta.abs()) + F_STEP * (gs.abs() @ vs.abs().mT))
+            out["o"][lo:hi, h], off["o"][lo:hi, h] = o, (p * (B_STEP + e)) @ vs.abs()
+            out["dq"][lo:hi, h], off["dq"][lo:hi, h] = scale * ds @ ks, scale * (ds_off + F_STEP * ds.abs()) @ ks.abs()
+            out["dk"][lo:hi, h // G] += scale * ds.mT @ qs
+            off["dk"][lo:hi, h // G] += scale * (ds_off + F_STEP * ds.abs()).mT @ qs.abs()
+            out["dv"][lo:hi, h // G] += p.mT @ gs
+            off["dv"][lo:hi, h // G] += (p * (B_STEP + e)).mT @ gs.abs()
+    return out, off
+
+
+def _close(got, want, off, what):
+    assert got.shape == want.shape and got.dtype == torch.bfloat16, what
+    diff = (got.double() - want).abs()
+    bound = off * (1 + B_STEP) + B_STEP * want.abs() + 1e-30
+    bad = ~(diff <= bound)
+    assert not bad.any(), f"{what}: {int(bad.sum())} of {bad.numel()} off, worst {float((diff / bound).nan_to_num(9e9)[bad].max()):.2f} of the bound"
+
+
+def _inputs(g, *lead, H, Hk, D, amp=1.0):
+    r = lambda h: torch.randn(*lead, h, D, device="cuda", generator=g)  # noqa: E731
+    return (amp * r(H)).bfloat16(), (amp * r(Hk)).bfloat16(), r(Hk).bfloat16(), r(H).bfloat16()
+
+
+def _run(q, k, v, do, **kw):
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    o = attn.attention(*leaves, **kw)
+    return dict(zip(("o", "dq", "dk", "dv"), (o.detach(),) + torch.autograd.grad(o, leaves, do)))
+
+
+def _check_batch(g, B, N, H, Hk, D, causal, scale=None, amp=1.0):
+    q, k, v, do = _inputs(g, B, N, H=H, Hk=Hk, D=D, amp=amp)
+    got = _run(q, k, v, do, causal=causal, scale=scale)
+    torch.cuda.synchronize()
+    _ext.check_device_errors()
+    for b in range(B):
+        want, off = _oracle(q[b], k[b], v[b], do[b], causal, scale or D ** -0.5, [(0, N)])
+        for n in want:
+            _close(got[n][b], want[n], off[n], f"{n} of sample {b}")
+
+
+# ---------------------------------------------------------------------------------------------------- any machine
+
+def test_refusals():
+    q, k = torch.randn(2, 5, 4, 8), torch.randn(2, 5, 2, 8)
+    for bad in ((q, k, k[:, :4]), (q, k[:, :4], k[:, :4]), (q, k[:1], k[:1]), (q, k[..., :4], k[..., :4]), (q, k.double(), k.double()), (q[0], k[0], k[0])):
+        with pytest.raises(ValueError):
+            attn.attention(*bad)
+    with pytest.raises(ValueError, match="divide"):
+        attn.attention(q[:, :, :3], k, k)
+    for s in (0.0, -1.0, math.inf, math.nan):
+        with pytest.raises(ValueError, match="scale"):
+            attn.attention(q, k, k, scale=s)
+    with pytest.raises(ValueError, match="offsets"):
+        attn.attention(q, k, k, offsets=torch.tensor([0, 5]))
+    for off in ([0, 6], [1, 5], [0, 3, 2], [[0, 5]], [0.0, 5.0]):
+        with pytest.raises(ValueError, match="offsets"):
+            attn.attention(q[0], k[0], k[0], offsets=torch.tensor(off))
+    x = torch.randn(2, 5, 64)
+    with pytest.raises(ValueError, match="divide"):
+        attn.attention_qkv(x, 4, 3)
+    with pytest.raises(ValueError, match="channels"):
+        attn.attention_qkv(x, 5)
+    with pytest.raises(ValueError):
+        attn.attention_qkv(x[0], 4, 2)
+    with pytest.raises(ValueError, match="offsets"):
+        attn.attention_qkv(x[0], 4, 2, offsets=torch.tensor([0, 9]))
+
+
+@pytest.mark.parametrize("causal", [False, True])
+def test_cpu_formulation(causal):
+    torch.manual_seed(1)
+    q, k, v, do = (torch.randn(11, h, 6, dtype=torch.float64) for h in (4, 2, 2, 4))
+    bounds = [(0, 3), (3, 3), (3, 4), (4, 9)]
+    want, _ = _oracle(q, k, v, do, causal, 0.3, bounds)
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+    o = attn.attention(*leaves, causal=causal, scale=0.3, offsets=[0, 3, 3, 4, 9])
+    for got, n in zip((o,) + torch.autograd.grad(o, leaves, do), ("o", "dq", "dk", "dv")):
+        assert torch.allclose(got, want[n], atol=1e-12), n
+    x = torch.cat([t.flatten(1) for t in (q, k, v)], 1)
+    assert torch.allclose(attn.attention_qkv(x, 4, 2, causal, 0.3, [0, 3, 3, 4, 9]), want["o"], atol=1e-12)
+    whole, _ = _oracle(q, k, v, do, causal, 6 ** -0.5, [(0, 11)])
+    assert torch.allclose(attn.attention(q[None], k[None], v[None], causal)[0], whole["o"], atol=1e-12)
+    assert torch.allclose(attn.attention_qkv(x[None], 4, 2, causal)[0], whole["o"], atol=1e-12)
+
+
+def test_gradient_formulas_against_differences():
+    torch.manual_seed(2)
+    q, k, v, do = (torch.randn(7, h, 5, dtype=torch.float64) for h in (4, 2, 2, 4))
+    want, _ = _oracle(q, k, v, do, True, 0.4, [(0, 2), (2, 7)])
+    f = lambda *t: (_oracle(*t, do, True, 0.4, [(0, 2), (2, 7)])[0]["o"] * do).sum()  # noqa: E731
+    h = 1e-6
+    for i, n in enumerate(("dq", "dk", "dv")):
+        d = torch.randn_like((q, k, v)[i])
+        up, down = ([t + s * h * d if j == i else t for j, t in enumerate((q, k, v))] for s in (1, -1))
+        assert abs(float((want[n] * d).sum() - (f(*up) - f(*down)) / (2 * h))) < 1e-7, n
+
+
+# ---------------------------------------------------------------------------------------------------- the kernels
+
+@pytest.fixture
+def gen():
+    if not torch.cuda.is_available():
+        pytest.skip("needs a GPU")
+    assert _ext.available()
+    return torch.Generator("cuda").manual_seed(21)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("B,N,H,Hk,D", [
+    (1, 1, 1, 1, 8), (2, 2, 2, 1, 16), (1, 127, 2, 2, 64), (3, 128, 2, 2, 48), (1, 129, 1, 1, 128), (2, 255, 2, 2, 64), (1, 256, 3, 1, 72),
+    (1, 257, 4, 2, 64), (2, 384, 1, 1, 40), (1, 385, 2, 1, 128), (1, 1000, 4, 4, 24), (1, 641, 6, 2, 96), (2, 130, 12, 4, 112), (1, 2050, 2, 2, 56)])
+def test_lengths_heads_and_widths(gen, B, N, H, Hk, D, causal):
+    _check_batch(gen, B, N, H, Hk, D, causal)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [1, 5, 20, 65, 127])
+def test_widths_that_are_padded(gen, D):
+    _check_batch(gen, 1, 200, 2, 1, D, True)
+
+
+@pytest.mark.gpu
+def test_sharp_scores(gen):
+    """Scores of some hundred: one weight of a row is nearly all of it, and maxima grow along the keys."""
+    _check_batch(gen, 1, 700, 2, 2, 64, False, amp=4.0)
+    q, k, v, do = _inputs(gen, 1, 900, H=2, Hk=2, D=64)
+    k = (k.float() * torch.linspace(0.1, 12, 900, device="cuda")[None, :, None, None]).bfloat16()
+    got = _run(q, k, v, do)
+    want, off = _oracle(q[0], k[0], v[0], do[0], False, 0.125, [(0, 900)])
+    for n in want:
+        _close(got[n][0], want[n], off[n], n)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scale", [0.02, 0.7])
+def test_scale(gen, scale):
+    _check_batch(gen, 1, 300, 2, 1, 48, False, scale=scale)
+
+
+LENGTHS = [[5], [0], [1, 1, 1], [128, 128], [0, 130, 0, 257, 1, 0], [64, 300, 63, 1, 129], [31] * 40 + [0] * 30 + [2] * 9, [512, 3, 700]]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("lens", LENGTHS)
+@pytest.mark.parametrize("H,Hk,D,behind", [(4, 2, 64, 0), (3, 3, 128, 140), (2, 1, 40, 3)])
+def test_packed_sequences(gen, lens, H, Hk, D, behind, causal):
+    """Neighbours hold NaN and infinities in their turn: nothing of them may reach a sequence."""
+    T = sum(lens) + behind
+    if T == 0:
+        T = behind = 1
+    at = [0]
+    for n in lens:
+        at.append(at[-1] + n)
+    bounds = list(zip(at, at[1:]))
+    offsets = torch.tensor(at, dtype=torch.int32, device="cuda")
+    q, k, v, do = _inputs(gen, T, H=H, Hk=Hk, D=D)
+    for t in (q, k, v, do):
+        t[at[-1]:] = float("nan")
+    got = _run(q, k, v, do, causal=causal, offsets=offsets)
+    torch.cuda.synchronize()
+    _ext.check_device_errors()
+    want, off = _oracle(q, k, v, do, causal, D ** -0.5, bounds)
+    for n in want:
+        _close(got[n], want[n], off[n], n)
+        assert not got[n][at[-1]:].any()
+    whole = max(range(len(lens)), key=lambda i: lens[i])
+    dirty = [t.clone() for t in (q, k, v, do)]
+    keep = torch.zeros(T, dtype=torch.bool, device="cuda")
+    keep[at[whole]:at[whole + 1]] = True
+    for t, bad in zip(dirty, (float("nan"), float("inf"), float("nan"), float("-inf"))):
+        t[~keep] = bad
+    again = _run(*dirty, causal=causal, offsets=offsets)
+    for n in want:
+        assert torch.equal(again[n][keep], got[n][keep]), n
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("packed", [False, True])
+def test_fused_projection(gen, packed):
+    """The same bits as separate tensors; the gradient of the projection's output in one tensor."""
+    H, Hk, D = 6, 2, 48
+    lead = (500,) if packed else (2, 250)
+    kw = dict(causal=True, offsets=torch.tensor([0, 200, 200, 490], dtype=torch.int32, device="cuda") if packed else None)
+    x = torch.randn(*lead, (H + 2 * Hk) * D, device="cuda", generator=gen).bfloat16().requires_grad_()
+    do = torch.randn(*lead, H, D, device="cuda", generator=gen).bfloat16()
+    o = attn.attention_qkv(x, H, Hk, **kw)
+    dx = torch.autograd.grad(o, x, do)[0]
+    q, k, v = x.detach().unflatten(-1, (-1, D)).split([H, Hk, Hk], -2)
+    got = _run(q, k, v, do, **kw)
+    assert torch.equal(o, got["o"]) and torch.equal(dx, torch.cat([got[n].flatten(-2) for n in ("dq", "dk", "dv")], -1))
+
+
+@pytest.mark.gpu
+def test_strides(gen):
+    """Views of other layouts give the bits of dense tensors."""
+    B, N, H, D = 2, 150, 4, 32
+    q, k, v, do = _inputs(gen, B, N, H=H, Hk=H, D=D)
+    want = _run(q, k, v, do, causal=True)
+
+    def same(*views, g=do):
+        got = _run(*views, g, causal=True)
+        assert all(torch.equal(got[n], want[n]) for n in want)
+
+    heads_first = [t.transpose(1, 2).contiguous().transpose(1, 2) for t in (q, k, v)]
+    same(*heads_first, g=do.transpose(1, 2).contiguous().transpose(1, 2))
+    same(*(t.repeat(1, 1, 1, 2).view(B, N, H, 2, D)[..., 0, :] for t in (q, k, v)))
+    same(*(torch.cat([t, t[..., :1]], -1)[..., :D] for t in (q, k, v)))              # rows off a 16-byte boundary
+    same(*(torch.cat([t.flatten()[:1], t.flatten()])[1:].view(t.shape) for t in (q, k, v)))
+    same(*(t.transpose(0, 3).contiguous().transpose(0, 3) for t in (q, k, v)))
+    # one head's keys and values, seen by all (stride 0): the gradients of the views add up to that of the head
+    one = _run(q, k[:, :, :1].expand(B, N, H, D), v[:, :, :1].expand(B, N, H, D), do)
+    two = _run(q, k[:, :, :1].repeat(1, 1, H, 1), v[:, :, :1].repeat(1, 1, H, 1), do)
+    assert all(torch.equal(one[n], two[n]) for n in one)
+    grad = _run(q, k, v, do[:, :, :1, :1].expand(B, N, H, D))
+    full = _run(q, k, v, do[:, :, :1, :1].expand(B, N, H, D).contiguous())
+    assert all(torch.equal(grad[n], full[n]) for n in full)
+
+
+@pytest.mark.gpu
+def test_empty_and_partial_gradients(gen):
+    q, k, v, do = _inputs(gen, 2, 0, H=2, Hk=2, D=16)
+    got = _run(q, k, v, do)
+    assert all(t.numel() == 0 for t in got.values())
+    q, k, v, do = _inputs(gen, 2, 140, H=2, Hk=2, D=16)
+    want = _run(q, k, v, do)
+    kl = k.clone().requires_grad_()
+    assert torch.equal(torch.autograd.grad(attn.attention(q, kl, v), kl, do)[0], want["dk"])
+    with torch.no_grad():
+        assert torch.equal(attn.attention(q, kl, v), want["o"])
+    ql = q.clone().requires_grad_()
+    dq = torch.autograd.grad(attn.attention(ql, k, v), ql, do, create_graph=True)[0]
+    with pytest.raises(RuntimeError, match="second derivatives"):
+        dq.float().sum().backward()
+
+
+@pytest.mark.gpu
+def test_rows_that_overflow_stay_alone(gen):
+    """A query with NaN and one with infinities spoil their own rows of the output and nothing else."""
+    q, k, v, do = _inputs(gen, 1, 300, H=2, Hk=2, D=32)
+    clean = attn.attention(q, k, v)
+    q[0, 7, 0, 3], q[0, 200, 1, 0] = float("nan"), float("inf")
+    o = attn.attention(q, k, v)
+    assert o[0, 7, 0].isnan().all() and o[0, 200, 1].isnan().all()
+    keep = torch.ones(300, 2, dtype=torch.bool, device="cuda")
+    keep[7, 0] = keep[200, 1] = False
+    assert torch.equal(o[0][keep], clean[0][keep])
+
+
+@pytest.mark.gpu
+def test_repeats_itself_and_replays(gen):
+    """The same bits again, on another stream beside other work, and from a captured graph that reads new inputs and offsets."""
+    q, k, v, do = _inputs(gen, 900, H=4, Hk=2, D=64)
+    offsets = torch.tensor([0, 100, 700, 900], dtype=torch.int32, device="cuda")
+    first = _run(q, k, v, do, causal=True, offsets=offsets)
+    same = lambda a, b: all(torch.equal(a[n], b[n]) for n in a)  # noqa: E731
+    assert same(first, _run(q, k, v, do, causal=True, offsets=offsets))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        beside = _run(q, k, v, do, causal=True, offsets=offsets)
+        held = [t.clone() for t in (q, k, v, do, offsets)]
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            got = _run(*held[:4], causal=True, offsets=held[4])
+    assert same(first, _run(q, k, v, do, causal=True, offsets=offsets))
+    torch.cuda.current_stream().wait_stream(side)
+    assert same(first, beside)
+    for new in ([0, 100, 700, 900], [0, 300, 300, 890]):
+        held[4].copy_(torch.tensor(new, dtype=torch.int32))
+        held[0].copy_(q.flip(0))
+        graph.replay()
+        assert same(got, _run(q.flip(0), k, v, do, causal=True, offsets=held[4].clone()))
+    del graph
+
+
+@pytest.mark.gpu
+def test_offsets_out_of_range_are_clamped(gen):
+    q, k, v, do = _inputs(gen, 300, H=2, Hk=1, D=64)
+    far = _run(q, k, v, do, offsets=torch.tensor([0, 120, 100000], dtype=torch.int32, device="cuda"))
+    want = _run(q, k, v, do, offsets=torch.tensor([0, 120, 300], dtype=torch.int32, device="cuda"))
+    assert all(torch.equal(far[n], want[n]) for n in want)
+    long = _run(q, k, v, do, offsets=torch.tensor([0, 120, 300], device="cuda"))       # int64, and from the host
+    host = _run(q, k, v, do, offsets=[0, 120, 300])
+    assert all(torch.equal(long[n], want[n]) and torch.equal(host[n], want[n]) for n in want)
+
+
+@pytest.mark.gpu
+def test_refusals_on_the_device(gen):
+    q, k, v, _ = _inputs(gen, 4, H=2, Hk=1, D=64)
+    with pytest.raises(ValueError, match="offsets"):
+        attn.attention(q, k, v, offsets=torch.tensor([0.0, 4.0], device="cuda"))
+    with pytest.raises(ValueError, match="device"):
+        attn.attention(q, k.cpu(), v.cpu(), offsets=[0, 4])
+
+
+@pytest.mark.gpu
+def test_gradient_against_differences(gen):
+    """Steps of the kernel's own outputs along its gradient.  Outputs are bf16: the difference is known to the sum of their half steps."""
+    N, H, D, h = 200, 2, 32, 2.0 ** -3
+    q, k, v, do = _inputs(gen, 1, N, H=H, Hk=H, D=D)
+    got = _run(q, k, v, do)
+    for i, n in enumerate(("dq", "dk", "dv")):
+        d = torch.randn(q.shape, device="cuda", generator=gen)
+        up, down = ([(t.float() + s * h * d).bfloat16() if j == i else t for j, t in enumerate((q, k, v))] for s in (1, -1))
+        moved = up[i].double() - down[i].double()
+        f = [(attn.attention(*t).double() * do.double()).sum() for t in (up, down)]
+        ref = [_oracle(*(x[0] for x in t), do[0], False, D ** -0.5, [(0, N)]) for t in (up, down)]
+        left_out = sum(s * (r[0]["o"] * do[0].double()).sum() for s, r in zip((1, -1), ref)) - \
+            (_oracle(q[0], k[0], v[0], do[0], False, D ** -0.5, [(0, N)])[0][n] * moved[0]).sum()
+        off = sum(((r[1]["o"] * (1 + B_STEP) + B_STEP * r[0]["o"].abs()) * do[0].double().abs()).sum() for r in ref)
+        own = _oracle(q[0], k[0], v[0], do[0], False, D ** -0.5, [(0, N)])
+        off = off + ((own[1][n] * (1 + B_STEP) + B_STEP * own[0][n].abs()) * moved[0].abs()).sum()
+        assert abs(float(f[0] - f[1] - left_out - (got[n].double() * moved).sum())) <= float(off), n
