@@ -19,6 +19,7 @@ import torch.nn.functional as F
 from ...ops import afno as afno_ops
 from ...ops import linear as linear_ops
 from ...parallel.helpers import compute_split_shapes
+from ...parallel.layer_norm import LayerNorm, normed, operand_dtype
 from ...parallel.layers import DistributedMLP
 from ...parallel.mappings import gather_from_parallel_region, scatter_to_parallel_region
 from ...utils import comm
@@ -92,7 +93,7 @@ class AFNO2D(nn.Module):
 
 
 class Block(nn.Module):
-    def __init__(self, dim, mlp_ratio=4.0, drop=0.0, drop_path=0.0, act_layer=nn.GELU, norm_layer=nn.LayerNorm,
+    def __init__(self, dim, mlp_ratio=4.0, drop=0.0, drop_path=0.0, act_layer=nn.GELU, norm_layer=LayerNorm,
                  double_skip=True, num_blocks=8, sparsity_threshold=0.01, hard_thresholding_fraction=1.0):
         super().__init__()
         self.norm1 = norm_layer(dim)
@@ -111,11 +112,16 @@ class Block(nn.Module):
 
     def forward(self, x):
         residual = x
-        x = self.filter(self.norm1(x))
-        if self.double_skip:
-            x = x + residual
-            residual = x
-        x = self.norm2(x)
+        # (the filter and the MLP take their products' type; the channel-parallel MLP what torch's norm would hand on)
+        x = self.filter(normed(self.norm1, x, operand_dtype(x)))
+        dtype = None if self.channel_parallel else operand_dtype(x)
+        if self.double_skip and isinstance(self.norm2, LayerNorm):
+            residual, x = self.norm2.after_sum(x, residual, dtype)
+        else:
+            if self.double_skip:
+                x = x + residual
+                residual = x
+            x = self.norm2(x) if dtype is None else normed(self.norm2, x, dtype)
         if self.channel_parallel:
             # the MLP input is sharded over fin, its output is sharded the same way
             x = scatter_to_parallel_region(x, 3, "fin")
@@ -147,7 +153,7 @@ class AdaptiveFourierNeuralOperatorNet(nn.Module):
         self.img_size, self.patch_size = tuple(inp_shape), tuple(patch_size)
         self.inp_chans, self.out_chans, self.embed_dim = inp_chans, out_chans, embed_dim
         self.compute_dtype = None
-        norm_layer = partial(nn.LayerNorm, eps=1e-6)
+        norm_layer = partial(LayerNorm, eps=1e-6)
         self.patch_embed = PatchEmbed(img_size=self.img_size, patch_size=self.patch_size, in_chans=inp_chans, embed_dim=embed_dim)
         self.pos_embed = nn.Parameter(torch.zeros(1, self.patch_embed.num_patches, embed_dim))
         self.pos_drop = nn.Dropout(p=drop_rate)

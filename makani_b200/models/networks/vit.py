@@ -6,19 +6,20 @@ Checkpoint contract (names and shapes of makani/models/networks/vit.py:29-231): 
 channel-parallel groups (makani/mpu/layers.py:352-359,453-529).
 
 Execution: tokens stay in one [B, tokens, E] bf16 matrix.  Every projection (qkv, attention output, both MLP layers with
-bias + GELU / bias epilogues, head) is a GEMM of the in-tree tensor-core engine (`ops/linear.py`); the softmax
-attention itself is `scaled_dot_product_attention` (a library kernel: attention is not among this framework's own
-kernels).  Layer norms are torch's.  On CPU / fp32 every piece is the plain torch op.
+bias + GELU / bias epilogues, head) is a GEMM of the in-tree tensor-core engine (`ops/linear.py`), attention reads the
+fused projection's output where it lies (`ops/attention.py`; with attention dropout in training it is torch's
+`scaled_dot_product_attention`), and the second norm of a block takes the residual sum with it (`ops/norm.py`).  On CPU /
+fp32 every piece is the plain torch op.
 """
 
 from __future__ import annotations
 
 import torch
 import torch.nn as nn
-import torch.nn.functional as F
 
 from ...ops import linear as linear_ops
-from ...parallel.layers import DistributedAttention, DistributedMLP
+from ...parallel.layer_norm import LayerNorm, normed, operand_dtype
+from ...parallel.layers import DistributedAttention, DistributedMLP, attend_normed
 from ...utils import comm
 from ..common.layers import MLP, DropPath, PatchEmbed
 
@@ -34,7 +35,7 @@ class Attention(nn.Module):
     """Multi-head self attention over all tokens; q / k may be layer-normalised per head."""
 
     def __init__(self, dim, input_format="traditional", num_heads=8, qkv_bias=False, qk_norm=False, attn_drop_rate=0.0,
-                 proj_drop_rate=0.0, norm_layer=nn.LayerNorm):
+                 proj_drop_rate=0.0, norm_layer=LayerNorm):
         super().__init__()
         if dim % num_heads:
             raise ValueError(f"dim {dim} is not a multiple of num_heads {num_heads}")
@@ -48,22 +49,20 @@ class Attention(nn.Module):
 
     def forward(self, x):
         B, N, C = x.shape
-        # [B, N, (3, heads, head_dim)] -> three [B, heads, N, head_dim] views, no copies before the attention kernel
-        q, k, v = self.qkv(x).view(B, N, 3, self.num_heads, self.head_dim).permute(2, 0, 3, 1, 4).unbind(0)
-        ctx = F.scaled_dot_product_attention(self.q_norm(q), self.k_norm(k), v,
-                                             dropout_p=self.attn_drop_rate if self.training else 0.0)
-        return self.proj_drop(self.proj(ctx.transpose(1, 2).reshape(B, N, C)))
+        ctx = attend_normed(self.qkv(x), self.num_heads, self.q_norm, self.k_norm, self.attn_drop_rate if self.training else 0.0)
+        return self.proj_drop(self.proj(ctx.reshape(B, N, C)))
 
 
 class Block(nn.Module):
     """x + attn(norm1(x)), then z = norm2(.), z + mlp(z) (the second residual starts after the norm, as upstream)."""
 
     def __init__(self, dim, num_heads, mlp_ratio=4.0, qkv_bias=False, mlp_drop_rate=0.0, attn_drop_rate=0.0,
-                 path_drop_rate=0.0, act_layer=nn.GELU, norm_layer=nn.LayerNorm, comm_inp_name="fin", comm_hidden_name="fout"):
+                 path_drop_rate=0.0, act_layer=nn.GELU, norm_layer=LayerNorm, comm_inp_name="fin", comm_hidden_name="fout"):
         super().__init__()
         hidden = int(dim * mlp_ratio)
         self.norm1, self.norm2 = norm_layer(dim), norm_layer(dim)
-        if comm.get_size(comm_inp_name) * comm.get_size(comm_hidden_name) > 1:
+        self.channel_parallel = comm.get_size(comm_inp_name) * comm.get_size(comm_hidden_name) > 1
+        if self.channel_parallel:
             self.attn = DistributedAttention(dim, input_format="traditional", comm_inp_name=comm_inp_name,
                                              comm_hidden_name=comm_hidden_name, num_heads=num_heads, qkv_bias=qkv_bias,
                                              attn_drop_rate=attn_drop_rate, proj_drop_rate=mlp_drop_rate, norm_layer=None)
@@ -78,9 +77,10 @@ class Block(nn.Module):
         self.drop_path = DropPath(path_drop_rate) if path_drop_rate > 0.0 else nn.Identity()
 
     def forward(self, x):
-        x = x + self.drop_path(self.attn(self.norm1(x)))
-        z = self.norm2(x)
-        return z + self.drop_path(self.mlp(z))
+        # (the products' type where they run on the engine; the channel-parallel layers take what torch's norm would hand on)
+        a = self.drop_path(self.attn(self.norm1(x) if self.channel_parallel else normed(self.norm1, x, operand_dtype(x))))
+        z = self.norm2.after_sum(x, a)[1] if isinstance(self.norm2, LayerNorm) else self.norm2(x + a)
+        return z + self.drop_path(self.mlp(z if self.channel_parallel else z.to(operand_dtype(z))))
 
 
 class VisionTransformer(nn.Module):
@@ -102,9 +102,9 @@ class VisionTransformer(nn.Module):
         rates = torch.linspace(0, path_drop_rate, depth).tolist()
         self.blocks = nn.ModuleList([
             Block(embed_dim, num_heads, mlp_ratio=mlp_ratio, qkv_bias=qkv_bias, mlp_drop_rate=mlp_drop_rate,
-                  attn_drop_rate=attn_drop_rate, path_drop_rate=rates[i], norm_layer=nn.LayerNorm,
+                  attn_drop_rate=attn_drop_rate, path_drop_rate=rates[i], norm_layer=LayerNorm,
                   comm_inp_name=comm_inp_name, comm_hidden_name=comm_hidden_name) for i in range(depth)])
-        self.norm = nn.LayerNorm(embed_dim)
+        self.norm = LayerNorm(embed_dim)
         self.out_size = out_chans * self.patch_size[0] * self.patch_size[1]
         self.head = _Proj(embed_dim, self.out_size, bias=False)
         nn.init.trunc_normal_(self.pos_embed, std=0.02)
@@ -133,4 +133,4 @@ class VisionTransformer(nn.Module):
         tokens = self.prepare_tokens(x)
         for blk in self.blocks:
             tokens = blk(tokens)
-        return self.forward_head(self.norm(tokens))
+        return self.forward_head(self.norm(tokens, operand_dtype(tokens)))

@@ -18,6 +18,7 @@ import torch.distributed as dist
 import torch.nn as nn
 
 from ..ops import _ext
+from ..ops import norm as norm_ops
 from ..utils import comm
 
 
@@ -122,7 +123,6 @@ class DistributedInstanceNorm2d(nn.Module):
         return get_slot("inorm", "spatial", x.shape[0] * x.shape[1] * 8, x.device)
 
     def forward(self, x, act: str = "none"):
-        from ..ops import norm as norm_ops
         w = self.weight if self.affine else None
         b = self.bias if self.affine else None
         cnt = self._global_count(x)
@@ -138,18 +138,60 @@ class DistributedInstanceNorm2d(nn.Module):
         return y
 
 
+def operand_dtype(x: torch.Tensor) -> torch.dtype:
+    """The type in which a matrix product takes `x`: that of autocast where it is on."""
+    if x.is_cuda and torch.is_autocast_enabled() and x.dtype != torch.float64:
+        return torch.get_autocast_dtype("cuda")
+    return x.dtype
+
+
+class LayerNorm(nn.LayerNorm):
+    """`nn.LayerNorm` over the last dimension, on the kernels of `ops/norm.py`.  As torch's it hands fp32 on under autocast, unless the
+    caller names the type: what only feeds a product is wanted in the product's (`operand_dtype`), the same bits as a cast behind it."""
+
+    def _dtype(self, x, out_dtype):
+        if out_dtype is not None:
+            return out_dtype
+        return torch.float32 if x.is_cuda and torch.is_autocast_enabled() and x.dtype != torch.float64 else x.dtype
+
+    def forward(self, x, out_dtype=None):
+        if len(self.normalized_shape) != 1:
+            y = super().forward(x)
+            return y if out_dtype is None else y.to(out_dtype)
+        if x.shape[-1] != self.normalized_shape[0]:
+            raise ValueError(f"layer norm over {self.normalized_shape[0]} channels, got {tuple(x.shape)}")
+        return norm_ops.layer_norm(x, self.weight, self.bias, self.eps, self._dtype(x, out_dtype))
+
+    def after_sum(self, x, residual, out_dtype=None):
+        """(s, norm(s)) with s = x + residual, in one pass over memory."""
+        if len(self.normalized_shape) != 1:
+            s = x + residual
+            return s, self.forward(s, out_dtype)
+        if x.shape[-1] != self.normalized_shape[0]:
+            raise ValueError(f"layer norm over {self.normalized_shape[0]} channels, got {tuple(x.shape)}")
+        s = x if x.dtype == torch.float32 else residual
+        return norm_ops.add_layer_norm(x, residual, self.weight, self.bias, self.eps, self._dtype(s, out_dtype))
+
+
+def normed(norm: nn.Module, x: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """norm(x) in `dtype`, whatever the norm's class."""
+    return norm(x, dtype) if isinstance(norm, LayerNorm) else norm(x).to(dtype)
+
+
 class DistributedLayerNorm(nn.Module):
     """Layer norm over the channel dimension of NCHW data (channels must not be sharded)."""
 
     def __init__(self, normalized_shape, eps=1e-05, elementwise_affine=True, bias=True, device=None, dtype=None):
         super().__init__()
         assert comm.get_size("matmul") == 1, "channel-sharded layer norm is not supported"
-        self.norm = nn.LayerNorm(normalized_shape, eps=eps, elementwise_affine=elementwise_affine, bias=bias,
-                                 device=device, dtype=dtype)
+        self.norm = LayerNorm(normalized_shape, eps=eps, elementwise_affine=elementwise_affine, bias=bias,
+                              device=device, dtype=dtype)
         if elementwise_affine:
             self.norm.weight.is_shared_mp = ["model"]
             if bias:
                 self.norm.bias.is_shared_mp = ["model"]
 
     def forward(self, x):
+        if x.is_cuda and x.dim() == 4 and len(self.norm.normalized_shape) == 1 and x.is_contiguous(memory_format=torch.channels_last):
+            return self.norm(x.permute(0, 2, 3, 1)).permute(0, 3, 1, 2)      # dense rows, and a channels-last result
         return torch.transpose(self.norm(torch.transpose(x, 1, 3)), 1, 3)

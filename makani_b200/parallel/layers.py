@@ -17,8 +17,10 @@ import torch.nn as nn
 import torch.nn.functional as F
 from torch.utils.checkpoint import checkpoint
 
+from ..ops import attention as attn_ops
 from ..utils import comm
 from .helpers import compute_split_shapes
+from .layer_norm import LayerNorm, normed, operand_dtype
 from .mappings import (copy_to_parallel_region, gather_from_parallel_region, reduce_from_parallel_region,
                        scatter_to_parallel_region)
 from .transpose import distributed_transpose_azimuth, distributed_transpose_polar
@@ -237,11 +239,24 @@ class DistributedMLP(nn.Module):
         return self.fwd(x)
 
 
+def attend_normed(qkv, num_heads, q_norm, k_norm, dropout_p=0.0):
+    """Self attention on the output of a fused projection, [B, N, (3, heads, head_dim)], queries and keys normalised per head on the way:
+    [B, N, heads, head_dim].  Dropped weights are left to the library."""
+    plain = isinstance(q_norm, nn.Identity) and isinstance(k_norm, nn.Identity)
+    if plain and dropout_p == 0.0:
+        return attn_ops.attention_qkv(qkv, num_heads)
+    q, k, v = qkv.unflatten(-1, (3, num_heads, -1)).unbind(2)
+    q, k = (t if isinstance(n, nn.Identity) else normed(n, t, operand_dtype(t)) for n, t in ((q_norm, q), (k_norm, k)))
+    if dropout_p == 0.0:
+        return attn_ops.attention(q, k, v)
+    return F.scaled_dot_product_attention(*(t.transpose(1, 2) for t in (q, k, v)), dropout_p=dropout_p).transpose(1, 2)
+
+
 class DistributedAttention(nn.Module):
     """Multi-head self attention with heads split over `comm_hidden_name` (sequence stays whole)."""
 
     def __init__(self, dim, input_format="traditional", comm_inp_name="fin", comm_hidden_name="fout", num_heads=8,
-                 qkv_bias=False, qk_norm=False, attn_drop_rate=0.0, proj_drop_rate=0.0, norm_layer=nn.LayerNorm):
+                 qkv_bias=False, qk_norm=False, attn_drop_rate=0.0, proj_drop_rate=0.0, norm_layer=LayerNorm):
         super().__init__()
         assert dim % num_heads == 0
         assert num_heads % comm.get_size(comm_hidden_name) == 0, "heads must divide over the hidden group"
@@ -267,12 +282,8 @@ class DistributedAttention(nn.Module):
         B, N, C = x.shape
         # local rows of the qkv projection are ordered (q | k | v, local head, head_dim), as in makani/mpu/layers.py:507:
         # at one rank that is the serial layout, and a rank's rows are the q, k and v rows of its own heads
-        qkv = self.qkv(x).reshape(B, N, 3, self.num_heads_local, self.head_dim).permute(2, 0, 3, 1, 4)
-        q, k, v = qkv.unbind(0)
-        q, k = self.q_norm(q), self.k_norm(k)
-        y = F.scaled_dot_product_attention(q, k, v, dropout_p=self.attn_drop_rate if self.training else 0.0)
-        y = y.transpose(1, 2).reshape(B, N, self.num_heads_local * self.head_dim)
-        return self.proj_drop(self.proj(y))
+        y = attend_normed(self.qkv(x), self.num_heads_local, self.q_norm, self.k_norm, self.attn_drop_rate if self.training else 0.0)
+        return self.proj_drop(self.proj(y.reshape(B, N, self.num_heads_local * self.head_dim)))
 
 
 class DistributedAFNO2Dv2(nn.Module):
