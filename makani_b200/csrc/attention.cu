@@ -503,12 +503,48 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
 
 // ------------------------------------------------------------------------------------------ backward
 
-// 64 columns of a tile of scores and of the products dO V^T are a thread's: P = 2^(scale S - L) and dS = P (dP - delta) of them, as operands of the next
-// products where the scores stood.  `at` (S or dP): the first of the 64.
-__device__ __forceinline__ uint32_t half_cols(uint32_t at, int i) { return at + 64u * (i >> 2) + 8u * (i & 3); }      // 16 of 128 rows of the operand
+// Sixteen computing warps: a thread has a row and 32 columns of a tile of scores and of the products dO V^T, P = 2^(scale S - L) and dS = P (dP - delta)
+// of them replace the scores as operands of the next products.  (With eight warps of 64 columns the two warps of a scheduler waited for the same
+// things at the same time: 128 x 128 keys by queries of 64 channels in 2645 and 3300 cycles for dQ and dK, dV, where the exponentials take 1024.)
+constexpr int BWD_WARPS = 16, BWD_THREADS = 32 * (COMPUTE_WARP + BWD_WARPS), BWD_COLS = 32;
+constexpr int BWD_FEW_REGS = 64, BWD_MANY_REGS = 104;
+static_assert(BWD_COLS * BWD_WARPS / 4 == TILE && 128 * BWD_FEW_REGS + 512 * BWD_MANY_REGS <= BWD_THREADS * 96);
+// 16 of the 128 rows of the operand that stands in `at`
+__device__ __forceinline__ uint32_t operand_cols(uint32_t at, int i) { return at + BWD_COLS * (i >> 1) + 8u * (i & 1); }
 
-// Gradient of the queries.  A CTA has 128 queries of a head and goes over the keys; its eight computing warps share the rows, 64 keys of a tile to four
-// of them each.  S has two buffers, so that the products of the next tile are there when the warps come to them.  delta is computed on the way and
+// P of 32 columns, from S in v; statistics (-L, -delta) of a row, or of the columns in shared memory.  `seen(c)`: with EDGE, whether column c counts.
+template <bool EDGE, typename Neg, typename Seen>
+__device__ __forceinline__ void weights_of(uint32_t (&v)[BWD_COLS], f32x2 scale2, Neg neg, Seen seen) {
+#pragma unroll
+  for (int c = 0; c < BWD_COLS; c += 2) {
+    float a, b;
+    f2_unpack(f2_fma(f2_pack(__uint_as_float(v[c]), __uint_as_float(v[c + 1])), scale2, neg(c)), a, b);
+    a = ex2(a);
+    b = ex2(b);
+    if (EDGE) {
+      a = seen(c) ? a : 0.f;
+      b = seen(c + 1) ? b : 0.f;
+    }
+    v[c] = __float_as_uint(a);
+    v[c + 1] = __float_as_uint(b);
+  }
+}
+template <bool EDGE, typename Neg, typename Seen>
+__device__ __forceinline__ void slopes_of(const uint32_t (&v)[BWD_COLS], const uint32_t (&d)[BWD_COLS], uint32_t (&packed)[BWD_COLS / 2], Neg neg, Seen seen) {
+#pragma unroll
+  for (int c = 0; c < BWD_COLS; c += 2) {
+    float a, b;
+    f2_unpack(f2_mul(f2_add(f2_pack(__uint_as_float(d[c]), __uint_as_float(d[c + 1])), neg(c)), f2_pack(__uint_as_float(v[c]), __uint_as_float(v[c + 1]))), a,
+              b);
+    if (EDGE) {      // (what is not seen may be NaN)
+      a = seen(c) ? a : 0.f;
+      b = seen(c + 1) ? b : 0.f;
+    }
+    packed[c / 2] = pack_bf16(a, b);
+  }
+}
+
+// Gradient of the queries.  A CTA has 128 queries of a head and goes over the keys.  S has two buffers, so that the products of the next tile are there when the warps come to them.  delta is computed on the way and
 // written for the second kernel.
 template <int DB>
 struct Dq {
@@ -529,7 +565,7 @@ struct DqParams {
 };
 
 template <int DB>
-__global__ void __launch_bounds__(THREADS, 1)
+__global__ void __launch_bounds__(BWD_THREADS, 1)
 attn_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                const __grid_constant__ CUtensorMap map_do, const DqParams p) {
   using L = Dq<DB>;
@@ -553,7 +589,7 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
     mbar_init(k_fixed, 1);
     mbar_init(k_fix, 1);
     mbar_init(dp_full, 1);
-    mbar_init(ds_ready, 8);
+    mbar_init(ds_ready, BWD_WARPS);
     mbar_init(dq_full, 1);
     mbar_init(s_full(0), 1);
     mbar_init(s_full(1), 1);
@@ -579,7 +615,7 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
   const bool fix = n > 0 && tail < TILE && w.lo + w.len < p.t.grid.N;
 
   if (warp < COMPUTE_WARP) {
-    regs_down<FEW_REGS>();
+    regs_down<BWD_FEW_REGS>();
     if (warp == 0) {
       // ---------------------------------------------------------------- tiles
       if (n > 0 && elect_one()) {
@@ -665,7 +701,7 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
           tc_fence_after();
 #pragma unroll
           for (int i = 0; i < TILE / 16; ++i)
-            mma_ts(tmem + DQ_ACC, half_cols(tmem + DQ_DP, i), km_lo + at + i * (2048 >> 4), hi, id_q, j > 0 || i > 0);
+            mma_ts(tmem + DQ_ACC, operand_cols(tmem + DQ_DP, i), km_lo + at + i * (2048 >> 4), hi, id_q, j > 0 || i > 0);
           tc_commit(k_empty(s));
           s = sn;
           ph = phn;
@@ -680,7 +716,7 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
       }
     }
   } else {
-    regs_up<MANY_REGS>();
+    regs_up<BWD_MANY_REGS>();
     // ------------------------------------------------------------------ P and dS
     const int x = (warp - COMPUTE_WARP) >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
@@ -710,45 +746,24 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
       ok = __all_sync(0xffffffffu, mbar_wait(s_full(j & 1), (j >> 1) & 1));
       if (!ok) break;
       tc_fence_after();
-      uint32_t v[64];
-      const uint32_t s_at = tmem + lanes + (j & 1) * S_COLS + x * 64, dp_at = tmem + lanes + DQ_DP + x * 64;
+      uint32_t v[BWD_COLS];
+      const uint32_t s_at = tmem + lanes + (j & 1) * S_COLS + x * BWD_COLS, dp_at = tmem + lanes + DQ_DP + x * BWD_COLS;
       tmem_req32(s_at, v);
-      tmem_req32(s_at + 32, v + 32);
+      const int k0 = j * TILE + x * BWD_COLS;
+      const bool edge = k0 + BWD_COLS > w.len || (causal && k0 + BWD_COLS - 1 > w.r0);
+      const int keys = (causal ? min(w.len, w.r0 + row + 1) : w.len) - k0;
+      auto seen = [&](int c) { return c < keys; };
       tmem_wait32(v);
-      tmem_wait32(v + 32);
-#pragma unroll
-      for (int c = 0; c < 64; c += 2) {
-        float a, b;
-        f2_unpack(f2_fma(f2_pack(__uint_as_float(v[c]), __uint_as_float(v[c + 1])), scale2, l2), a, b);
-        v[c] = __float_as_uint(ex2(a));
-        v[c + 1] = __float_as_uint(ex2(b));
-      }
+      weights_of<false>(v, scale2, [&](int) { return l2; }, seen);
       ok = __all_sync(0xffffffffu, mbar_wait(dp_full, j & 1));
       if (!ok) break;
       tc_fence_after();
-      const int k0 = j * TILE + x * 64;
-      const bool edge = k0 + 64 > w.len || (causal && k0 + 63 > w.r0);
-      const int seen = (causal ? min(w.len, w.r0 + row + 1) : w.len) - k0;
-      uint32_t packed[32];
-#pragma unroll
-      for (int h = 0; h < 64; h += 32) {
-        uint32_t d[32];
-        tmem_req32(dp_at + h, d);
-        tmem_wait32(d);
-#pragma unroll
-        for (int c = 0; c < 32; c += 2) {
-          float a, b;
-          f2_unpack(f2_mul(f2_add(f2_pack(__uint_as_float(d[c]), __uint_as_float(d[c + 1])), delta2),
-                           f2_pack(__uint_as_float(v[h + c]), __uint_as_float(v[h + c + 1]))),
-                    a, b);
-          if (edge) {
-            a = h + c < seen ? a : 0.f;
-            b = h + c + 1 < seen ? b : 0.f;
-          }
-          packed[(h + c) / 2] = pack_bf16(a, b);
-        }
-      }
-      tmem_st32(dp_at, packed);
+      uint32_t d[BWD_COLS], packed[BWD_COLS / 2];
+      tmem_req32(dp_at, d);
+      tmem_wait32(d);
+      if (edge) slopes_of<true>(v, d, packed, [&](int) { return delta2; }, seen);
+      else slopes_of<false>(v, d, packed, [&](int) { return delta2; }, seen);
+      tmem_st16(dp_at, packed);
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
@@ -759,7 +774,7 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
     __nv_bfloat16* const to = p.dq.ptr + w.b * p.dq.batch + (w.lo + w.r0 + row) * p.dq.token + w.h * p.dq.head;
     if (n > 0 && ok) {
       tc_fence_after();
-      store_row(tmem + lanes + DQ_ACC, p.t.D, p.t.scale, to, here, x * 16, 32);
+      store_row(tmem + lanes + DQ_ACC, p.t.D, p.t.scale, to, here, x * 16, 64);
     } else if (here && w.padding && x == 0) {
       zero_row(p.t.D, to);
     }
@@ -795,7 +810,7 @@ struct DkvParams {
 };
 
 template <int DB>
-__global__ void __launch_bounds__(THREADS, 1)
+__global__ void __launch_bounds__(BWD_THREADS, 1)
 attn_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                 const __grid_constant__ CUtensorMap map_do, const DkvParams p) {
   using L = Dkv<DB>;
@@ -819,8 +834,8 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     mbar_init(kv_full, 1);
     mbar_init(fixed, 1);
     mbar_init(fix_bar, 1);
-    mbar_init(p_ready, 8);
-    mbar_init(ds_ready, 8);
+    mbar_init(p_ready, BWD_WARPS);
+    mbar_init(ds_ready, BWD_WARPS);
     mbar_init(dp_full, 1);
     mbar_init(acc_full, 1);
     mbar_init(s_full(0), 1);
@@ -848,7 +863,7 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
   const bool fix = n > 0 && tail < TILE && w.lo + w.len < p.t.grid.N;
 
   if (warp < COMPUTE_WARP) {
-    regs_down<FEW_REGS>();
+    regs_down<BWD_FEW_REGS>();
     if (warp == 0) {
       // ---------------------------------------------------------------- tiles
       if (n > 0 && elect_one()) {
@@ -897,7 +912,7 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         };
         auto over_queries = [&](uint32_t d, uint32_t a, uint32_t b, uint32_t accum) {
 #pragma unroll
-          for (int i = 0; i < TILE / 16; ++i) mma_ts(d, half_cols(a, i), b + i * (2048 >> 4), hi, id_d, accum | (i > 0));
+          for (int i = 0; i < TILE / 16; ++i) mma_ts(d, operand_cols(a, i), b + i * (2048 >> 4), hi, id_d, accum | (i > 0));
         };
         bool ok = mbar_wait(kv_full, 0) && mbar_wait(q_full(0), 0) && mbar_wait(do_full(0), 0);
         if (!ok) atomicExch(p.t.err, 91);
@@ -1004,7 +1019,7 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       }
     }
   } else {
-    regs_up<MANY_REGS>();
+    regs_up<BWD_MANY_REGS>();
     // ------------------------------------------------------------------ P and dS, transposed
     const int x = (warp - COMPUTE_WARP) >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
@@ -1018,33 +1033,23 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       ok = __all_sync(0xffffffffu, mbar_wait(stat_full(s), ph) && mbar_wait(s_full(buf), L::S_BUFS == 2 ? (j >> 1) & 1 : j & 1));
       if (!ok) break;
       tc_fence_after();
-      const float* const stats = reinterpret_cast<const float*>(smem_raw + pad + L::STAT_AT + s * L::STAT) + x * 64;
-      const int q0 = (q_first + t) * TILE + x * 64;
+      const float* const stats = reinterpret_cast<const float*>(smem_raw + pad + L::STAT_AT + s * L::STAT) + x * BWD_COLS;
+      const int q0 = (q_first + t) * TILE + x * BWD_COLS;
       // the queries that see this key are the columns from `from` to `to`
-      const bool edge = q0 + 64 > w.len || (causal && q0 < w.r0 + TILE - 1);
+      const bool edge = q0 + BWD_COLS > w.len || (causal && q0 < w.r0 + TILE - 1);
       const int from = causal ? w.r0 + row - q0 : 0, to = w.len - q0;
-      uint32_t v[64], packed[32];
-      const uint32_t s_at = tmem + lanes + buf * S_COLS + x * 64, dp_at = tmem + lanes + L::DP_AT + x * 64;
+      auto seen = [&](int c) { return c >= from && c < to; };
+      auto neg_l = [&](int c) { return *reinterpret_cast<const f32x2*>(stats + c); };
+      auto neg_delta = [&](int c) { return *reinterpret_cast<const f32x2*>(stats + TILE + c); };
+      uint32_t v[BWD_COLS], packed[BWD_COLS / 2];
+      const uint32_t s_at = tmem + lanes + buf * S_COLS + x * BWD_COLS, dp_at = tmem + lanes + L::DP_AT + x * BWD_COLS;
       tmem_req32(s_at, v);
-      tmem_req32(s_at + 32, v + 32);
       tmem_wait32(v);
-      tmem_wait32(v + 32);
+      if (edge) weights_of<true>(v, scale2, neg_l, seen);
+      else weights_of<false>(v, scale2, neg_l, seen);
 #pragma unroll
-      for (int c = 0; c < 64; c += 4) {
-        const float4 l = *reinterpret_cast<const float4*>(stats + c);
-        float e[4];
-        f2_unpack(f2_fma(f2_pack(__uint_as_float(v[c]), __uint_as_float(v[c + 1])), scale2, f2_pack(l.x, l.y)), e[0], e[1]);
-        f2_unpack(f2_fma(f2_pack(__uint_as_float(v[c + 2]), __uint_as_float(v[c + 3])), scale2, f2_pack(l.z, l.w)), e[2], e[3]);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          e[i] = ex2(e[i]);
-          if (edge) e[i] = c + i >= from && c + i < to ? e[i] : 0.f;
-          v[c + i] = __float_as_uint(e[i]);
-        }
-        packed[c / 2] = pack_bf16(e[0], e[1]);
-        packed[c / 2 + 1] = pack_bf16(e[2], e[3]);
-      }
-      tmem_st32(s_at, packed);
+      for (int c = 0; c < BWD_COLS; c += 2) packed[c / 2] = pack_bf16(__uint_as_float(v[c]), __uint_as_float(v[c + 1]));
+      tmem_st16(s_at, packed);
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
@@ -1052,30 +1057,12 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       ok = __all_sync(0xffffffffu, mbar_wait(dp_full, j & 1));
       if (!ok) break;
       tc_fence_after();
-#pragma unroll
-      for (int h = 0; h < 64; h += 32) {
-        uint32_t d[32];
-        tmem_req32(dp_at + h, d);
-        tmem_wait32(d);
-#pragma unroll
-        for (int c = 0; c < 32; c += 4) {
-          const float4 l = *reinterpret_cast<const float4*>(stats + TILE + h + c);
-          float e[4];
-          f2_unpack(f2_mul(f2_add(f2_pack(__uint_as_float(d[c]), __uint_as_float(d[c + 1])), f2_pack(l.x, l.y)),
-                           f2_pack(__uint_as_float(v[h + c]), __uint_as_float(v[h + c + 1]))),
-                    e[0], e[1]);
-          f2_unpack(f2_mul(f2_add(f2_pack(__uint_as_float(d[c + 2]), __uint_as_float(d[c + 3])), f2_pack(l.z, l.w)),
-                           f2_pack(__uint_as_float(v[h + c + 2]), __uint_as_float(v[h + c + 3]))),
-                    e[2], e[3]);
-          if (edge) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) e[i] = h + c + i >= from && h + c + i < to ? e[i] : 0.f;
-          }
-          packed[(h + c) / 2] = pack_bf16(e[0], e[1]);
-          packed[(h + c) / 2 + 1] = pack_bf16(e[2], e[3]);
-        }
-      }
-      tmem_st32(dp_at, packed);
+      uint32_t d[BWD_COLS];
+      tmem_req32(dp_at, d);
+      tmem_wait32(d);
+      if (edge) slopes_of<true>(v, d, packed, neg_delta, seen);
+      else slopes_of<false>(v, d, packed, neg_delta, seen);
+      tmem_st16(dp_at, packed);
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
@@ -1089,12 +1076,13 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     if (ok && n > 0) ok = __all_sync(0xffffffffu, mbar_wait(acc_full, 0));
     if (!ok && lane == 0) atomicExch(p.t.err, 93);
     // half of the warps store either
-    const AttnTensor& d = x == 0 ? p.dv : p.dk;
+    const bool values = x < 2;
+    const AttnTensor& d = values ? p.dv : p.dk;
     __nv_bfloat16* const to = d.ptr + w.b * d.batch + (w.lo + w.r0 + row) * d.token + w.h * d.head;
     if (n > 0 && ok) {
       tc_fence_after();
-      store_row(tmem + lanes + (x == 0 ? L::DV_AT : L::DK_AT), p.t.D, x == 0 ? 1.f : p.t.scale, to, here);
-    } else if (here && w.padding) {
+      store_row(tmem + lanes + (values ? L::DV_AT : L::DK_AT), p.t.D, values ? 1.f : p.t.scale, to, here, (x & 1) * 16, 32);
+    } else if (here && w.padding && (x & 1) == 0) {
       zero_row(p.t.D, to);
     }
   }
@@ -1164,14 +1152,14 @@ cudaError_t launch_dq(const CUtensorMap& q, const CUtensorMap& k, const CUtensor
   static std::atomic<uint64_t> devices;
   const cudaError_t e = allow_shared_memory(devices, reinterpret_cast<const void*>(&attn_dq_kernel<DB>), Dq<DB>::SMEM);
   if (e != cudaSuccess) return e;
-  return launch_chained(attn_dq_kernel<DB>, dim3(static_cast<unsigned>(blocks_of(p.t.grid))), dim3(THREADS), Dq<DB>::SMEM, s, 1, true, q, k, v, g, p);
+  return launch_chained(attn_dq_kernel<DB>, dim3(static_cast<unsigned>(blocks_of(p.t.grid))), dim3(BWD_THREADS), Dq<DB>::SMEM, s, 1, true, q, k, v, g, p);
 }
 template <int DB>
 cudaError_t launch_dkv(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& g, const DkvParams& p, cudaStream_t s) {
   static std::atomic<uint64_t> devices;
   const cudaError_t e = allow_shared_memory(devices, reinterpret_cast<const void*>(&attn_dkv_kernel<DB>), Dkv<DB>::SMEM);
   if (e != cudaSuccess) return e;
-  return launch_chained(attn_dkv_kernel<DB>, dim3(static_cast<unsigned>(blocks_of(p.t.grid))), dim3(THREADS), Dkv<DB>::SMEM, s, 1, true, q, k, v, g, p);
+  return launch_chained(attn_dkv_kernel<DB>, dim3(static_cast<unsigned>(blocks_of(p.t.grid))), dim3(BWD_THREADS), Dkv<DB>::SMEM, s, 1, true, q, k, v, g, p);
 }
 
 }  // namespace
