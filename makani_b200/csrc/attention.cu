@@ -12,6 +12,7 @@
 #include <cuda_bf16.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "attention.cuh"
 #include "fused_ops.cuh"
@@ -48,6 +49,21 @@ __device__ __forceinline__ void mma_ts(uint32_t tmem_d, uint32_t tmem_a, uint32_
       : "memory");
 }
 
+// A wait that is mostly over when it begins
+__device__ __forceinline__ bool mbar_wait_soon(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t"
+      ".reg .pred P1;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 P1, [%1], %2;\n\t"
+      "selp.b32 %0, 1, 0, P1;\n\t"
+      "}\n"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok || mbar_wait(bar, parity);
+}
+
 #define MK_R8(v, o) "=r"(v[o]), "=r"(v[o + 1]), "=r"(v[o + 2]), "=r"(v[o + 3]), "=r"(v[o + 4]), "=r"(v[o + 5]), "=r"(v[o + 6]), "=r"(v[o + 7])
 #define MK_RW8(v, o) "+r"(v[o]), "+r"(v[o + 1]), "+r"(v[o + 2]), "+r"(v[o + 3]), "+r"(v[o + 4]), "+r"(v[o + 5]), "+r"(v[o + 6]), "+r"(v[o + 7])
 #define MK_RD8(v, o) "r"(v[o]), "r"(v[o + 1]), "r"(v[o + 2]), "r"(v[o + 3]), "r"(v[o + 4]), "r"(v[o + 5]), "r"(v[o + 6]), "r"(v[o + 7])
@@ -77,6 +93,9 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* v) {
                MK_RD8(v, 8), "r"(taddr)
                : "memory");
 }
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t* v) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::MK_RD8(v, 0), "r"(taddr) : "memory");
+}
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // Registers of a warp group: all of them together stay within the THREADS * 168 of the launch
@@ -87,10 +106,67 @@ __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.
 template <int N>
 __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 
+// Two branches that begin with this stay two: merged, whole tiles pay for the comparisons of those at an edge (4 instructions an element)
+template <bool EDGE>
+__device__ __forceinline__ void apart() { asm volatile("" ::"n"(EDGE ? 1 : 0)); }
+
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+// 2^x of two values with fp32 arithmetic, for a share of a tile's exponentials: the special function unit takes 1024 cycles for 128 x 128 of them, while the
+// FMA pipe has time.  x = n + f with n the integer next to it (1.5 2^23 added and taken away), 2^f from a polynomial (Remez exchange for the least
+// relative error on |f| <= 1/2: 2.7e-6 in fp32), n into the exponent.  Below -126 it stays at 2^-126.
+__device__ __forceinline__ void ex2_poly(float& a, float& b) {
+  const float nearest = 12582912.f;
+  const f32x2 x = f2_pack(fmaxf(a, -126.f), fmaxf(b, -126.f));
+  const f32x2 t = f2_add(x, f2_pack(nearest, nearest));
+  const f32x2 n = f2_add(t, f2_pack(-nearest, -nearest));
+  const f32x2 f = f2_fma(n, f2_pack(-1.f, -1.f), x);
+  f32x2 y = f2_fma(f, f2_pack(0.009570102207362652f, 0.009570102207362652f), f2_pack(0.05591785907745361f, 0.05591785907745361f));
+  y = f2_fma(y, f, f2_pack(0.240247443318367f, 0.240247443318367f));
+  y = f2_fma(y, f, f2_pack(0.6931217908859253f, 0.6931217908859253f));
+  y = f2_fma(y, f, f2_pack(0.9999992847442627f, 0.9999992847442627f));
+  float ta, tb, ya, yb;
+  f2_unpack(t, ta, tb);
+  f2_unpack(y, ya, yb);
+  a = __uint_as_float(__float_as_uint(ya) + (__float_as_uint(ta) << 23));
+  b = __uint_as_float(__float_as_uint(yb) + (__float_as_uint(tb) << 23));
+}
+// Pair `i` of a row: POLY of every eight on the FMA pipe
+template <int POLY>
+__device__ __forceinline__ void ex2_pair(int i, float& a, float& b) {
+  if ((i * POLY) % 8 < POLY) {
+    ex2_poly(a, b);
+  } else {
+    a = ex2(a);
+    b = ex2(b);
+  }
+}
+// The greatest (of what is no NaN) of N values; three at a time where the warp has nothing else to wait for (8192 causal tokens, 16 heads of 128: 284 us
+// with, 266 without; 16200 tokens, 8 heads of 48: 723 with, 728 without)
+template <bool THREE, int N>
+__device__ __forceinline__ float max_of(const uint32_t (&v)[N]) {
+  if (!THREE) {
+    float m[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m[i] = __uint_as_float(v[i]);
+#pragma unroll
+    for (int c = 4; c < N; ++c) m[c & 3] = fmaxf(m[c & 3], __uint_as_float(v[c]));
+    return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+  }
+  float m[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m[i] = __uint_as_float(v[i]);
+#pragma unroll
+  for (int c = 8; c + 15 < N; c += 16)
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      asm("max.f32 %0, %0, %1, %2;" : "+f"(m[i]) : "f"(__uint_as_float(v[c + 2 * i])), "f"(__uint_as_float(v[c + 2 * i + 1])));
+#pragma unroll
+  for (int c = 8 + (N - 8) / 16 * 16; c < N; ++c) m[c & 7] = fmaxf(m[c & 7], __uint_as_float(v[c]));
+  return fmaxf(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), fmaxf(fmaxf(m[4], m[5]), fmaxf(m[6], m[7])));
 }
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   uint32_t r;
@@ -186,24 +262,22 @@ struct TileParams {
   int* err;
 };
 
+// 16 (or the first 8) fp32 values as bf16
+__device__ __forceinline__ void store16(const uint32_t (&v)[16], __nv_bfloat16* to, bool all) {
+  uint32_t h[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) h[i] = pack_bf16(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
+  reinterpret_cast<uint4*>(to)[0] = make_uint4(h[0], h[1], h[2], h[3]);
+  if (all) reinterpret_cast<uint4*>(to)[1] = make_uint4(h[4], h[5], h[6], h[7]);
+}
 // The first D columns of an accumulator's row, times f, as bf16: those from `first` on in steps of `step` (multiples of 16)
 __device__ __forceinline__ void store_row(uint32_t taddr, int D, float f, __nv_bfloat16* to, bool here, int first = 0, int step = 16) {
   for (int c = first; c < D; c += step) {
     uint32_t v[16];
     tmem_ld16(taddr + c, v);
-    if (here) {
-      uint4 lo, hi;
-      lo.x = pack_bf16(__uint_as_float(v[0]) * f, __uint_as_float(v[1]) * f);
-      lo.y = pack_bf16(__uint_as_float(v[2]) * f, __uint_as_float(v[3]) * f);
-      lo.z = pack_bf16(__uint_as_float(v[4]) * f, __uint_as_float(v[5]) * f);
-      lo.w = pack_bf16(__uint_as_float(v[6]) * f, __uint_as_float(v[7]) * f);
-      hi.x = pack_bf16(__uint_as_float(v[8]) * f, __uint_as_float(v[9]) * f);
-      hi.y = pack_bf16(__uint_as_float(v[10]) * f, __uint_as_float(v[11]) * f);
-      hi.z = pack_bf16(__uint_as_float(v[12]) * f, __uint_as_float(v[13]) * f);
-      hi.w = pack_bf16(__uint_as_float(v[14]) * f, __uint_as_float(v[15]) * f);
-      *reinterpret_cast<uint4*>(to + c) = lo;
-      if (c + 8 < D) *reinterpret_cast<uint4*>(to + c + 8) = hi;
-    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * f);
+    if (here) store16(v, to + c, c + 8 < D);
   }
 }
 __device__ __forceinline__ void zero_row(int D, __nv_bfloat16* to) {
@@ -220,32 +294,97 @@ __device__ __forceinline__ void tmem_free_all(uint32_t tmem) {
 
 // ------------------------------------------------------------------------------------------ forward
 
+// O is rescaled where the maximum has grown by more than a factor of 2^8 since: the weights then reach 256 instead of 1, with the same relative
+// rounding, and nearly all tiles leave O alone
+constexpr float MAX_GROWTH = 8.f;
+
+// A row of the running softmax: what its weights are relative to (times scale), and their sum
+struct Row {
+  float m = -INFINITY;
+  f32x2 sum[2] = {0ull, 0ull};
+
+  // Whether the scores of a tile ask for a new maximum; `f`: what sums, and O, are multiplied by then.  Row by row: what a row holds does not depend
+  // on its neighbours.
+  __device__ __forceinline__ bool grows(float top) const { return top > m + MAX_GROWTH; }
+  __device__ __forceinline__ float grow(float top) {
+    const float up = grows(top) ? top : m, f = up == m ? 1.f : ex2(m - up);
+    m = up;
+    sum[0] = f2_mul(sum[0], f2_pack(f, f));
+    sum[1] = f2_mul(sum[1], f2_pack(f, f));
+    return f;
+  }
+  __device__ __forceinline__ float total() const {
+    float a, b;
+    f2_unpack(f2_add(sum[0], sum[1]), a, b);
+    return a + b;
+  }
+  // 128 scores -> weights 2^(scale S - m), as bf16 in the first half of them.  (A share of the exponentials on the FMA pipe, which helps the backward
+  // pass, is slower here: 16200 tokens, 8 heads of 48: 750 us without, 860 - 930 with an eighth to three eighths of them.)
+  __device__ __forceinline__ void weights(uint32_t (&v)[TILE], float scale) {
+    // (a row that has seen nothing but -inf has no maximum yet, and weights of 0)
+    const float from = m == -INFINITY ? 0.f : -m;
+    const f32x2 scale2 = f2_pack(scale, scale), from2 = f2_pack(from, from);
+#pragma unroll
+    for (int c = 0; c < TILE; c += 2) {
+      float a, b;
+      f2_unpack(f2_fma(f2_pack(__uint_as_float(v[c]), __uint_as_float(v[c + 1])), scale2, from2), a, b);
+      a = ex2(a);
+      b = ex2(b);
+      sum[(c >> 1) & 1] = f2_add(sum[(c >> 1) & 1], f2_pack(a, b));
+      v[c / 2] = pack_bf16(a, b);
+    }
+  }
+};
+__device__ __forceinline__ void load_scores(uint32_t s_at, uint32_t (&v)[TILE]) {
+#pragma unroll
+  for (int c = 0; c < TILE; c += 32) tmem_req32(s_at + c, v + c);
+#pragma unroll
+  for (int c = 0; c < TILE; c += 32) tmem_wait32(v + c);
+}
+// what is hidden is -inf, and its weight 0
+__device__ __forceinline__ void hide_scores(uint32_t (&v)[TILE], int seen) {
+#pragma unroll
+  for (int c = 0; c < TILE; ++c)
+    if (c >= seen) v[c] = 0xff800000u;
+}
+__device__ __forceinline__ void store_weights(uint32_t p_at, const uint32_t (&v)[TILE]) {
+  tmem_st32(p_at, v);
+  tmem_st32(p_at + 32, v + 32);
+  tmem_st_wait();
+}
+// O of a row times f
+__device__ __forceinline__ void scale_row(uint32_t o_at, int cols, float f) {
+#pragma unroll 1
+  for (int c = 0; c < cols; c += 8) {
+    uint32_t a[8];
+    tmem_ld8(o_at + c, a);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) a[k] = __float_as_uint(__uint_as_float(a[k]) * f);
+    tmem_st8(o_at + c, a);
+  }
+}
+
 // Two tiles of 128 queries share every tile of keys and values, so that the products of one run beside the exponentials of the other.  Tensor
 // memory: S of either (128 columns, P takes the first 64 of them), O of either (up to 128).
-template <int DB>
-struct Fwd {
-  static constexpr int STAGES = DB == 1 ? 4 : 2, TILE_BYTES = DB * BOX;
+struct FwdWide {
+  static constexpr int DB = 2, STAGES = 2, TILE_BYTES = DB * BOX;
   static constexpr int K_AT = 2 * TILE_BYTES, V_AT = K_AT + STAGES * TILE_BYTES, BAR_AT = V_AT + STAGES * TILE_BYTES;
   static constexpr int BARS = 4 * STAGES + 7;
   static constexpr int SMEM = BAR_AT + 8 * BARS + 16 + 1024;
   static_assert(SMEM <= SMEM_LIMIT);
 };
 constexpr uint32_t S_COLS = 128, O_AT = 256;
-// O is rescaled where the maximum has grown by more than a factor of 2^8 since: the weights then reach 256 instead of 1, with the same relative
-// rounding, and nearly all tiles leave O alone
-constexpr float MAX_GROWTH = 8.f;
-
 struct FwdParams {
   TileParams t;
   __nv_bfloat16* o;
   float* lse;
 };
 
-template <int DB>
 __global__ void __launch_bounds__(THREADS, 1)
 attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                 const FwdParams p) {
-  using L = Fwd<DB>;
+  using L = FwdWide;
+  constexpr int DB = L::DB;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = smem_u32(smem_raw);
   const uint32_t pad = (1024u - (raw_addr & 1023u)) & 1023u;
@@ -408,86 +547,267 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     const uint32_t s_at = tmem + lanes + t * S_COLS, o_at = tmem + lanes + O_AT + t * ATTN_WIDTH;
     const float scale = p.t.scale_log2;
     const bool here = row < rows;
-    float m = 0.f;
-    f32x2 sum[2] = {0ull, 0ull};
+    Row r;
     bool ok = true;
-    for (int j = 0; j < nt && ok; ++j) {
+    for (int j = 0; j < nt; ++j) {
       ok = __all_sync(0xffffffffu, mbar_wait(s_full(t), j & 1));
-      if (!ok) {
-        if (lane == 0) atomicExch(p.t.err, 84);
-        break;
-      }
+      if (!ok) break;
       tc_fence_after();
       uint32_t v[TILE];
-#pragma unroll
-      for (int c = 0; c < TILE; c += 32) tmem_req32(s_at + c, v + c);
-#pragma unroll
-      for (int c = 0; c < TILE; c += 32) tmem_wait32(v + c);
+      load_scores(s_at, v);
       const int k0 = j * TILE;
-      if (k0 + TILE > w.len || (causal && k0 + TILE - 1 > w.r0 + t * TILE)) {
-        const int seen = (causal ? min(w.len, w.r0 + row + 1) : w.len) - k0;
-#pragma unroll
-        for (int c = 0; c < TILE; ++c)
-          if (c >= seen) v[c] = 0xff800000u;
-      }
-      float mx[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) mx[i] = __uint_as_float(v[i]);
-#pragma unroll
-      for (int c = 4; c < TILE; ++c) mx[c & 3] = fmaxf(mx[c & 3], __uint_as_float(v[c]));
-      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
-      if (j == 0) {
-        m = top == -INFINITY ? 0.f : top;
-      } else if (__any_sync(0xffffffffu, top > m + MAX_GROWTH)) {
+      if (k0 + TILE > w.len || (causal && k0 + TILE - 1 > w.r0 + t * TILE)) hide_scores(v, (causal ? min(w.len, w.r0 + row + 1) : w.len) - k0);
+      const float top = max_of<false>(v) * scale;
+      if (__any_sync(0xffffffffu, r.grows(top))) {
         // (the scores of tile j are behind the products of tile j - 1: O is complete up to there)
-        // (row by row: what a row holds does not depend on its neighbours)
-        const float up = top > m + MAX_GROWTH ? top : m, f = ex2(m - up);
-        m = up;
-        const f32x2 f2 = f2_pack(f, f);
-        sum[0] = f2_mul(sum[0], f2);
-        sum[1] = f2_mul(sum[1], f2);
-        for (int c = 0; c < p.t.DP; c += 16) {
-          uint32_t a[16];
-          tmem_ld16(o_at + c, a);
-#pragma unroll
-          for (int i = 0; i < 16; ++i) a[i] = __float_as_uint(__uint_as_float(a[i]) * f);
-          tmem_st16(o_at + c, a);
-        }
+        const float f = r.grow(top);
+        if (j > 0) scale_row(o_at, p.t.DP, f);
       }
-      const f32x2 scale2 = f2_pack(scale, scale), m2 = f2_pack(-m, -m);
-#pragma unroll
-      for (int c = 0; c < TILE; c += 64) {
-        uint32_t packed[32];
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          float a, b;
-          f2_unpack(f2_fma(f2_pack(__uint_as_float(v[c + 2 * i]), __uint_as_float(v[c + 2 * i + 1])), scale2, m2), a, b);
-          a = ex2(a);
-          b = ex2(b);
-          sum[i & 1] = f2_add(sum[i & 1], f2_pack(a, b));
-          packed[i] = pack_bf16(a, b);
-        }
-        tmem_st32(s_at + c / 2, packed);
-      }
-      tmem_st_wait();
+      r.weights(v, scale);
+      store_weights(s_at, v);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(p_ready(t));
     }
-    if (nt > 0 && ok) {
-      ok = __all_sync(0xffffffffu, mbar_wait(s_full(t), nt & 1));
-      if (!ok && lane == 0) atomicExch(p.t.err, 84);
-    }
+    if (nt > 0 && ok) ok = __all_sync(0xffffffffu, mbar_wait(s_full(t), nt & 1));
+    if (!ok && lane == 0) atomicExch(p.t.err, 84);
     const long long token = static_cast<long long>(w.b) * p.t.grid.N + w.lo + w.r0 + row;
     __nv_bfloat16* const to = p.o + (token * p.t.grid.H + w.h) * p.t.D;
     if (nt > 0 && ok) {
       tc_fence_after();
-      float a, b;
-      f2_unpack(f2_add(sum[0], sum[1]), a, b);
-      const float total = a + b;
+      const float total = r.total();
       store_row(o_at, p.t.D, 1.f / total, to, here);
       if (here && p.lse)
-        p.lse[(static_cast<long long>(w.b) * p.t.grid.H + w.h) * p.t.grid.N + w.lo + w.r0 + row] = m + __log2f(total);
+        p.lse[(static_cast<long long>(w.b) * p.t.grid.H + w.h) * p.t.grid.N + w.lo + w.r0 + row] = r.m + __log2f(total);
+    } else if (here && w.padding) {
+      zero_row(p.t.D, to);
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_free_all(tmem);
+  }
+}
+
+// Heads of up to 64 channels: tensor memory has room for S, P and O of both query tiles side by side (128, 64 and 64 columns), so that the next scores are
+// on their way as soon as the last have been read, and no warp waits for products.
+struct FwdNarrow {
+  static constexpr int STAGES = 4;
+  static constexpr int K_AT = 2 * BOX, V_AT = K_AT + STAGES * BOX, BAR_AT = V_AT + STAGES * BOX;
+  static constexpr int BARS = 4 * STAGES + 11;
+  static constexpr int SMEM = BAR_AT + 8 * BARS + 16 + 1024;
+  static constexpr uint32_t P_AT = 256, O_AT = 384;
+  static_assert(SMEM <= SMEM_LIMIT);
+};
+
+__global__ void __launch_bounds__(THREADS, 1)
+attn_fwd_narrow_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                       const FwdParams p) {
+  using L = FwdNarrow;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_addr = smem_u32(smem_raw);
+  const uint32_t pad = (1024u - (raw_addr & 1023u)) & 1023u;
+  const uint32_t base = raw_addr + pad, bars = base + L::BAR_AT;
+  auto k_full = [&](int s) { return bars + 8u * s; };
+  auto k_empty = [&](int s) { return bars + 8u * (L::STAGES + s); };
+  auto v_full = [&](int s) { return bars + 8u * (2 * L::STAGES + s); };
+  auto v_empty = [&](int s) { return bars + 8u * (3 * L::STAGES + s); };
+  const uint32_t q_full = bars + 8u * (4 * L::STAGES), v_fix = q_full + 8u, v_fixed = q_full + 16u;
+  auto s_full = [&](int t) { return q_full + 24u + 32u * t; };
+  auto s_read = [&](int t) { return q_full + 32u + 32u * t; };
+  auto p_ready = [&](int t) { return q_full + 40u + 32u * t; };
+  auto o_done = [&](int t) { return q_full + 48u + 32u * t; };
+  volatile uint32_t* const tmem_slot = reinterpret_cast<volatile uint32_t*>(smem_raw + pad + L::BAR_AT + 8 * L::BARS);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < L::STAGES; ++s) {
+      mbar_init(k_full(s), 1);
+      mbar_init(v_full(s), 1);
+      mbar_init(k_empty(s), 2);
+      mbar_init(v_empty(s), 2);
+    }
+    mbar_init(q_full, 1);
+    mbar_init(v_fix, 2);
+    mbar_init(v_fixed, 1);
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(s_full(t), 1);
+      mbar_init(s_read(t), 4);
+      mbar_init(p_ready(t), 4);
+      mbar_init(o_done(t), 1);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    fence_async_smem();
+  }
+  if (warp == 1) tmem_alloc_all(tmem_slot);
+  const int* offsets = p.t.grid.offsets;
+  chain_begin(true, offsets);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  Work w;
+  const bool any = find_work(p.t.grid, offsets, blockIdx.x, w);
+  const int rows = any ? min(w.len - w.r0, 2 * TILE) : 0;
+  const bool causal = p.t.causal != 0;
+  auto tiles_of = [&](int t) {      // of keys, that the queries of tile t see
+    if (w.padding || rows <= t * TILE) return 0;
+    const int last = causal ? w.r0 + min(rows, (t + 1) * TILE) - 1 : w.len - 1;
+    return last / TILE + 1;
+  };
+  const int n0 = tiles_of(0), n1 = tiles_of(1), n = max(n0, n1);
+  const int tail = w.len - (n - 1) * TILE;
+  const bool fix = n > 0 && tail < TILE && w.lo + w.len < p.t.grid.N;
+
+  if (warp < COMPUTE_WARP) {
+    regs_down<FEW_REGS>();
+    if (warp == 0) {
+      // ---------------------------------------------------------------- tiles
+      if (n > 0 && elect_one()) {
+        const int hk = w.h / p.t.group, nq = rows > TILE ? 2 : 1;
+        mbar_expect_tx(q_full, nq * BOX);
+        for (int t = 0; t < nq; ++t) tma_load_4d(base + t * BOX, &map_q, q_full, 0, w.lo + w.r0 + t * TILE, w.h, w.b);
+        int s = 0;
+        uint32_t ph = 0;
+        for (int j = 0; j < n; ++j) {
+          if (!mbar_wait(k_empty(s), ph ^ 1u)) {
+            atomicExch(p.t.err, 80);
+            break;
+          }
+          mbar_expect_tx(k_full(s), BOX);
+          tma_load_4d(base + L::K_AT + s * BOX, &map_k, k_full(s), 0, w.lo + j * TILE, hk, w.b);
+          if (!mbar_wait(v_empty(s), ph ^ 1u)) {
+            atomicExch(p.t.err, 80);
+            break;
+          }
+          mbar_expect_tx(v_full(s), BOX);
+          tma_load_4d(base + L::V_AT + s * BOX, &map_v, v_full(s), 0, w.lo + j * TILE, hk, w.b);
+          if (++s == L::STAGES) {
+            s = 0;
+            ph ^= 1u;
+          }
+        }
+      }
+    } else if (warp & 1) {
+      // ---------------------------------------------------------------- products, a warp for either query tile
+      if (n > 0 && elect_one()) {
+        const int t = warp >> 1, nt = t == 0 ? n0 : n1;
+        const uint32_t hi = desc_hi(1024);
+        const uint32_t q_lo = desc_lo(base + t * BOX, 16), k_lo = desc_lo(base + L::K_AT, 16), v_lo = desc_lo(base + L::V_AT, BOX);
+        const uint32_t id_s = idesc_n(TILE), id_o = idesc_n(p.t.DP) | B_MN, o = tmem + L::O_AT + t * 64, a = tmem + L::P_AT + t * 64;
+        const int ksteps = p.t.DP >> 4;
+        auto scores = [&](int s) {
+          const uint32_t b = k_lo + s * (BOX >> 4);
+          for (int k = 0; k < ksteps; ++k) tc_mma<2, 1>(tmem + t * S_COLS, q_lo + 2 * k, hi, b + 2 * k, hi, id_s, k > 0);
+          tc_commit(s_full(t));
+        };
+        bool ok = mbar_wait(q_full, 0) && mbar_wait(k_full(0), 0);
+        if (!ok) atomicExch(p.t.err, 81);
+        if (ok) {
+          tc_fence_after();
+          if (nt > 0) scores(0);
+          tc_commit(k_empty(0));
+        }
+        int s = 0;
+        uint32_t ph = 0;
+        for (int j = 0; j < n && ok; ++j) {
+          const int sn = s + 1 == L::STAGES ? 0 : s + 1;
+          const uint32_t phn = sn == 0 ? ph ^ 1u : ph;
+          // (a tile that this warp has no use for is given back as soon as it is there)
+          if (j + 1 < n) {
+            ok = mbar_wait(k_full(sn), phn) && (j + 1 >= nt || mbar_wait(s_read(t), j & 1));
+            if (!ok) {
+              atomicExch(p.t.err, 82);
+              break;
+            }
+            tc_fence_after();
+            if (j + 1 < nt) scores(sn);
+            tc_commit(k_empty(sn));
+          }
+          ok = mbar_wait(v_full(s), ph);
+          if (ok && fix && j == n - 1) {
+            mbar_arrive(v_fix);
+            ok = mbar_wait(v_fixed, 0);
+          }
+          if (ok && j < nt) ok = mbar_wait(p_ready(t), j & 1);
+          if (!ok) {
+            atomicExch(p.t.err, 83);
+            break;
+          }
+          tc_fence_after();
+          if (j < nt) {
+            const uint32_t b = v_lo + s * (BOX >> 4);
+#pragma unroll
+            for (int k = 0; k < TILE / 16; ++k) mma_ts(o, a + k * 8, b + k * (2048 >> 4), hi, id_o, j > 0 || k > 0);
+            tc_commit(o_done(t));
+          }
+          tc_commit(v_empty(s));
+          s = sn;
+          ph = phn;
+        }
+      }
+    } else if (warp == 2) {
+      // ---------------------------------------------------------------- rows of the next sequence, at the word of the warps that multiply
+      if (fix && wait_long(v_fix, 0, n)) {
+        clear_rows(smem_raw + pad + L::V_AT + (n - 1) % L::STAGES * BOX, 1, tail);
+        if (lane == 0) mbar_arrive(v_fixed);
+      }
+    }
+  } else {
+    regs_up<MANY_REGS>();
+    // ------------------------------------------------------------------ softmax
+    const int t = (warp - COMPUTE_WARP) >> 2, row = t * TILE + (warp & 3) * 32 + lane, nt = t == 0 ? n0 : n1;
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t s_at = tmem + lanes + t * S_COLS, p_at = tmem + lanes + L::P_AT + t * 64, o_at = tmem + lanes + L::O_AT + t * 64;
+    const float scale = p.t.scale_log2;
+    const bool here = row < rows;
+    Row r;
+    bool ok = true;
+    for (int j = 0; j < nt; ++j) {
+      ok = __all_sync(0xffffffffu, mbar_wait_soon(s_full(t), j & 1));
+      if (!ok) break;
+      tc_fence_after();
+      uint32_t v[TILE];
+      load_scores(s_at, v);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(s_read(t));
+      const int k0 = j * TILE;
+      if (k0 + TILE > w.len || (causal && k0 + TILE - 1 > w.r0 + t * TILE)) hide_scores(v, (causal ? min(w.len, w.r0 + row + 1) : w.len) - k0);
+      const float top = max_of<true>(v) * scale;
+      if (__any_sync(0xffffffffu, r.grows(top))) {
+        const float f = r.grow(top);
+        if (j > 0) {
+          ok = __all_sync(0xffffffffu, mbar_wait(o_done(t), (j - 1) & 1));
+          if (!ok) break;
+          tc_fence_after();
+          scale_row(o_at, p.t.DP, f);
+        }
+      }
+      r.weights(v, scale);
+      if (j > 0) {
+        ok = __all_sync(0xffffffffu, mbar_wait_soon(o_done(t), (j - 1) & 1));
+        if (!ok) break;
+        tc_fence_after();
+      }
+      store_weights(p_at, v);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(p_ready(t));
+    }
+    if (nt > 0 && ok) ok = __all_sync(0xffffffffu, mbar_wait(o_done(t), (nt - 1) & 1));
+    if (!ok && lane == 0) atomicExch(p.t.err, 84);
+    const long long token = static_cast<long long>(w.b) * p.t.grid.N + w.lo + w.r0 + row;
+    __nv_bfloat16* const to = p.o + (token * p.t.grid.H + w.h) * p.t.D;
+    if (nt > 0 && ok) {
+      tc_fence_after();
+      const float total = r.total();
+      store_row(o_at, p.t.D, 1.f / total, to, here);
+      if (here && p.lse) p.lse[(static_cast<long long>(w.b) * p.t.grid.H + w.h) * p.t.grid.N + w.lo + w.r0 + row] = r.m + __log2f(total);
     } else if (here && w.padding) {
       zero_row(p.t.D, to);
     }
@@ -507,20 +827,21 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
 // of them replace the scores as operands of the next products.  (With eight warps of 64 columns the two warps of a scheduler waited for the same
 // things at the same time: 128 x 128 keys by queries of 64 channels in 2645 and 3300 cycles for dQ and dK, dV, where the exponentials take 1024.)
 constexpr int BWD_WARPS = 16, BWD_THREADS = 32 * (COMPUTE_WARP + BWD_WARPS), BWD_COLS = 32;
-constexpr int BWD_FEW_REGS = 64, BWD_MANY_REGS = 104;
+constexpr int BWD_FEW_REGS = 96, BWD_MANY_REGS = 96;
 static_assert(BWD_COLS * BWD_WARPS / 4 == TILE && 128 * BWD_FEW_REGS + 512 * BWD_MANY_REGS <= BWD_THREADS * 96);
+constexpr int BWD_POLY = 3;      // of eight pairs of exponentials, those on the FMA pipe
 // 16 of the 128 rows of the operand that stands in `at`
 __device__ __forceinline__ uint32_t operand_cols(uint32_t at, int i) { return at + BWD_COLS * (i >> 1) + 8u * (i & 1); }
 
 // P of 32 columns, from S in v; statistics (-L, -delta) of a row, or of the columns in shared memory.  `seen(c)`: with EDGE, whether column c counts.
 template <bool EDGE, typename Neg, typename Seen>
 __device__ __forceinline__ void weights_of(uint32_t (&v)[BWD_COLS], f32x2 scale2, Neg neg, Seen seen) {
+  apart<EDGE>();
 #pragma unroll
   for (int c = 0; c < BWD_COLS; c += 2) {
     float a, b;
     f2_unpack(f2_fma(f2_pack(__uint_as_float(v[c]), __uint_as_float(v[c + 1])), scale2, neg(c)), a, b);
-    a = ex2(a);
-    b = ex2(b);
+    ex2_pair<BWD_POLY>(c / 2, a, b);
     if (EDGE) {
       a = seen(c) ? a : 0.f;
       b = seen(c + 1) ? b : 0.f;
@@ -528,11 +849,14 @@ __device__ __forceinline__ void weights_of(uint32_t (&v)[BWD_COLS], f32x2 scale2
     v[c] = __float_as_uint(a);
     v[c + 1] = __float_as_uint(b);
   }
+  // (here, and not where they are used, behind the wait for the products)
+  asm volatile("" : MK_RW8(v, 0), MK_RW8(v, 8), MK_RW8(v, 16), MK_RW8(v, 24));
 }
 template <bool EDGE, typename Neg, typename Seen>
 __device__ __forceinline__ void slopes_of(const uint32_t (&v)[BWD_COLS], const uint32_t (&d)[BWD_COLS], uint32_t (&packed)[BWD_COLS / 2], Neg neg, Seen seen) {
 #pragma unroll
   for (int c = 0; c < BWD_COLS; c += 2) {
+    if (c == 0) apart<EDGE>();
     float a, b;
     f2_unpack(f2_mul(f2_add(f2_pack(__uint_as_float(d[c]), __uint_as_float(d[c + 1])), neg(c)), f2_pack(__uint_as_float(v[c]), __uint_as_float(v[c + 1]))), a,
               b);
@@ -1140,12 +1464,15 @@ TileParams tile_params(const AttnShape& p, const Slots& g, int* err) {
   return t;
 }
 
-template <int DB>
 cudaError_t launch_fwd(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const FwdParams& p, cudaStream_t s) {
-  static std::atomic<uint64_t> devices;
-  const cudaError_t e = allow_shared_memory(devices, reinterpret_cast<const void*>(&attn_fwd_kernel<DB>), Fwd<DB>::SMEM);
+  static std::atomic<uint64_t> narrow, wide;
+  const bool fits = p.t.D <= 64;
+  const cudaError_t e = fits ? allow_shared_memory(narrow, reinterpret_cast<const void*>(&attn_fwd_narrow_kernel), FwdNarrow::SMEM)
+                             : allow_shared_memory(wide, reinterpret_cast<const void*>(&attn_fwd_kernel), FwdWide::SMEM);
   if (e != cudaSuccess) return e;
-  return launch_chained(attn_fwd_kernel<DB>, dim3(static_cast<unsigned>(blocks_of(p.t.grid))), dim3(THREADS), Fwd<DB>::SMEM, s, 1, true, q, k, v, p);
+  const dim3 grid(static_cast<unsigned>(blocks_of(p.t.grid)));
+  if (fits) return launch_chained(attn_fwd_narrow_kernel, grid, dim3(THREADS), FwdNarrow::SMEM, s, 1, true, q, k, v, p);
+  return launch_chained(attn_fwd_kernel, grid, dim3(THREADS), FwdWide::SMEM, s, 1, true, q, k, v, p);
 }
 template <int DB>
 cudaError_t launch_dq(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& g, const DqParams& p, cudaStream_t s) {
@@ -1174,7 +1501,7 @@ cudaError_t attention_fwd(const AttnShape& p, const AttnTensor& q, const AttnTen
   f.t = tile_params(p, slots_of(p, p.H, 2 * TILE, 1), err);
   f.o = o;
   f.lse = lse;
-  return p.D <= 64 ? launch_fwd<1>(mq, mk_, mv, f, s) : launch_fwd<2>(mq, mk_, mv, f, s);
+  return launch_fwd(mq, mk_, mv, f, s);
 }
 
 cudaError_t attention_bwd(const AttnShape& p, const AttnTensor& q, const AttnTensor& k, const AttnTensor& v, const __nv_bfloat16* o,
