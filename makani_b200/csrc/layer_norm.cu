@@ -3,17 +3,18 @@
 //   mean = sum x / C,  var = sum (x - mean)^2 / C,  xh = (x - mean) / sqrt(var + eps),  y = xh w + b
 //   g = dy w,  dx = rstd (g - mean(g) - xh mean(g xh)),  dw = sum over rows of dy xh,  db = sum over rows of dy
 //
-// One read and one write of memory a row: a group of G threads holds its row in registers, so that the variance is a second sum over
-// registers of deviations (E[x^2] - E[x]^2 loses everything where |mean| >> spread), and the next row is on its way while the sums go
-// through the shuffles.  Groups are 8 or 16 threads for short rows, a warp up to 1024 channels, the block above.  The backward pass keeps
-// its columns' sums of dy xh and dy in registers over all its rows; blocks leave one row of partial sums each, which a second launch
-// adds up in a fixed order.  All sums are fp32; outputs are rounded once.
+// One read and one write of memory a row.  A thread has eight neighbouring channels (16 bytes of bf16; four single ones where rows are not whole
+// vectors) for all rows that its group goes over, so that weights and the sums of dy xh and dy stay in registers; groups are 8 or 16 threads for
+// short rows, else as many warps as a row needs.  A group takes ROWS rows at a time, whose sums share shuffles and barriers, with the next ones on
+// their way.  The variance is a second sum over registers of deviations (E[x^2] - E[x]^2 loses everything where |mean| >> spread).  In the backward
+// pass blocks leave one row of partial sums each, which a second launch adds up in a fixed order.  All sums are fp32; outputs are rounded once.
 #include <cuda_bf16.h>
 
 #include <algorithm>
 #include <type_traits>
 
 #include "fused_ops.cuh"
+#include "gelu.cuh"
 #include "gemm_tcgen05.cuh"
 #include "launch.cuh"
 #include "layer_norm.cuh"
@@ -22,7 +23,7 @@ namespace mk {
 
 namespace {
 
-constexpr int THREADS = 256, WARPS = THREADS / 32;
+constexpr int THREADS = 256, MOST_WARPS = THREADS / 32;
 
 // VEC elements of T as they come from memory
 template <typename T, int VEC>
@@ -86,32 +87,42 @@ struct Raw<float, 1> {
   __device__ __forceinline__ void store(float* p) const { *p = v; }
 };
 
-// Sums of N values over the G threads of a group, in all of them.  `sh` (G = THREADS): N * WARPS floats, another set for each of the sums that
-// follow one another between two uses of the same.
-template <int G, int N>
-__device__ __forceinline__ void group_sum(float (&a)[N], float* sh) {
-  constexpr int W = G < 32 ? G : 32;
+// The threads of one row: SUB of a warp (8, 16), or whole warps (SUB = 32), `warps` of them
+template <int SUB>
+struct Group {
+  int size, lane, index, per_block, warps;
+  __device__ __forceinline__ explicit Group(int w) : warps(SUB < 32 ? 1 : w) {
+    size = SUB < 32 ? SUB : 32 * warps;
+    lane = threadIdx.x % size;
+    index = threadIdx.x / size;
+    per_block = blockDim.x / size;
+  }
+  // Sums of N values over the group, in all of its threads.  `sh`: N * MOST_WARPS floats for every group of the block, another set for each of the sums
+  // that follow one another between two uses of the same.
+  template <int N>
+  __device__ __forceinline__ void sum(float (&a)[N], float* sh) const {
 #pragma unroll
-  for (int o = W / 2; o > 0; o >>= 1)
+    for (int o = SUB / 2; o > 0; o >>= 1)
 #pragma unroll
-    for (int i = 0; i < N; ++i) a[i] += __shfl_xor_sync(0xffffffffu, a[i], o);
-  if constexpr (G > 32) {
-    const int warp = threadIdx.x >> 5;
+      for (int i = 0; i < N; ++i) a[i] += __shfl_xor_sync(0xffffffffu, a[i], o);
+    if (SUB < 32 || warps == 1) return;
+    float* const mine = sh + index * warps * N;
+    const int warp = lane >> 5;
     if ((threadIdx.x & 31) == 0) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) sh[i * WARPS + warp] = a[i];
+      for (int i = 0; i < N; ++i) mine[warp * N + i] = a[i];
     }
-    __syncthreads();
+    asm volatile("bar.sync %0, %1;" ::"r"(1 + index), "r"(size) : "memory");
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      a[i] = 0.f;
+    for (int i = 0; i < N; ++i) a[i] = 0.f;
+    for (int k = 0; k < warps; ++k)
 #pragma unroll
-      for (int k = 0; k < WARPS; ++k) a[i] += sh[i * WARPS + k];
-    }
+      for (int i = 0; i < N; ++i) a[i] += mine[k * N + i];
   }
-}
+};
 
-__device__ __forceinline__ long long row_offset(long long r, long long inner, long long so, long long si) {
+__device__ __forceinline__ long long row_offset(long long r, long long rows, long long inner, long long so, long long si) {
+  if (inner >= rows) return r * si;
   const unsigned long long q = (static_cast<unsigned long long>(r) >> 32) == 0 && (static_cast<unsigned long long>(inner) >> 32) == 0
                                    ? static_cast<uint32_t>(r) / static_cast<uint32_t>(inner)
                                    : static_cast<unsigned long long>(r) / static_cast<unsigned long long>(inner);
@@ -119,319 +130,393 @@ __device__ __forceinline__ long long row_offset(long long r, long long inner, lo
   return o * so + (r - o * inner) * si;
 }
 
+__device__ __forceinline__ float sum_of(f32x2 v) {
+  float a, b;
+  f2_unpack(v, a, b);
+  return a + b;
+}
+
+// A thread's NV vectors of VEC channels, of which the i-th begins at channel (lane + i size) VEC, as PAIRS pairs of values
+template <int VEC, int NV>
+struct Cols {
+  static constexpr int PAIRS = VEC * NV / 2;
+  static_assert(VEC == 8 || NV % 2 == 0, "whole pairs");
+};
+template <typename T, int VEC, int NV>
+__device__ __forceinline__ void unpack(const Raw<T, VEC> (&raw)[NV], f32x2 (&v)[Cols<VEC, NV>::PAIRS]) {
+  float f[VEC * NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    float e[VEC];
+    raw[i].get(e);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) f[i * VEC + j] = e[j];
+  }
+#pragma unroll
+  for (int k = 0; k < Cols<VEC, NV>::PAIRS; ++k) v[k] = f2_pack(f[2 * k], f[2 * k + 1]);
+}
+template <typename T, int VEC, int NV>
+__device__ __forceinline__ void pack(const f32x2 (&v)[Cols<VEC, NV>::PAIRS], Raw<T, VEC> (&raw)[NV]) {
+  float f[VEC * NV];
+#pragma unroll
+  for (int k = 0; k < Cols<VEC, NV>::PAIRS; ++k) f2_unpack(v[k], f[2 * k], f[2 * k + 1]);
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    float e[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) e[j] = f[i * VEC + j];
+    raw[i].set(e);
+  }
+}
+// zeros where a vector is behind the last channel
+template <int VEC, int NV>
+__device__ __forceinline__ void keep(f32x2 (&v)[Cols<VEC, NV>::PAIRS], int lane, int size, int C) {
+  if (VEC == 8) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if ((lane + i * size) * VEC >= C)
+#pragma unroll
+        for (int k = 0; k < VEC / 2; ++k) v[i * (VEC / 2) + k] = 0ull;
+  } else {
+#pragma unroll
+    for (int k = 0; k < Cols<VEC, NV>::PAIRS; ++k) {
+      float a, b;
+      f2_unpack(v[k], a, b);
+      v[k] = f2_pack(lane + 2 * k * size < C ? a : 0.f, lane + (2 * k + 1) * size < C ? b : 0.f);
+    }
+  }
+}
+template <typename T, int VEC, int NV>
+__device__ __forceinline__ void load_row(const T* from, Raw<T, VEC> (&raw)[NV], int lane, int size, int C) {
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (lane + i * size) * VEC;
+    if (c < C) raw[i].load(from + c);
+  }
+}
+template <typename T, int VEC, int NV>
+__device__ __forceinline__ void store_row(T* to, const Raw<T, VEC> (&raw)[NV], int lane, int size, int C) {
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (lane + i * size) * VEC;
+    if (c < C) raw[i].store(to + c);
+  }
+}
+
 // TR: type of the tensor that is added first (void: none)
-template <typename TI, typename TO, typename TR, int VEC, int G, int NV>
-__global__ void __launch_bounds__(THREADS) ln_fwd_kernel(LnForward p) {
+template <typename TI, typename TO, typename TR, int VEC, int NV, int SUB, int ROWS, int BLOCKS>
+__global__ void __launch_bounds__(THREADS, BLOCKS) ln_fwd_kernel(LnForward p, int warps) {
   constexpr bool ADD = !std::is_void<TR>::value;
   using Res = typename std::conditional<ADD, TR, TI>::type;
-  constexpr int GROUPS = THREADS / G, PER_WARP = G < 32 ? 32 / G : 1;
-  __shared__ float sh[3 * WARPS];
+  constexpr int P = Cols<VEC, NV>::PAIRS;
+  __shared__ float sh[3 * ROWS * MOST_WARPS];
   const TI* x = static_cast<const TI*>(p.x);
   const Res* res = static_cast<const Res*>(p.r);
   const float *w = p.w, *b = p.b;
   chain_begin(true, x, res, w, b);
-  const int lane = threadIdx.x % G, group = threadIdx.x / G;
-  const long long step = static_cast<long long>(gridDim.x) * GROUPS;
-  // a warp's groups go through the loop together
-  long long first = static_cast<long long>(blockIdx.x) * GROUPS + group / PER_WARP * PER_WARP;
-  const int mine = group % PER_WARP;
-  const float inv = 1.f / static_cast<float>(p.C);
-
-  Raw<TI, VEC> next[NV];
-  Raw<Res, VEC> next_r[ADD ? NV : 1];
-  auto fetch = [&](long long r) {
-    if (r >= p.rows) return;
-    const TI* const from = x + row_offset(r, p.inner, p.outer_stride, p.inner_stride);
+  const Group<SUB> g(warps);
+  const int C = p.C;
+  const float inv = 1.f / static_cast<float>(C);
+  f32x2 wv[P], bv[P];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (lane + i * G) * VEC;
-      if (c < p.C) {
-        next[i].load(from + c);
-        if constexpr (ADD) next_r[i].load(res + r * p.C + c);
-      }
+  for (int k = 0; k < P; ++k) {
+    wv[k] = f2_pack(1.f, 1.f);
+    bv[k] = 0ull;
+  }
+  Raw<float, VEC> weights[NV];
+  if (w) {
+    load_row(w, weights, g.lane, g.size, C);
+    unpack(weights, wv);
+  }
+  if (b) {
+    load_row(b, weights, g.lane, g.size, C);
+    unpack(weights, bv);
+  }
+  const long long step = static_cast<long long>(gridDim.x) * g.per_block * ROWS;
+  // (the groups of a warp go through the loop together)
+  const int per_warp = SUB < 32 ? 32 / SUB : 1;
+  const int mine = SUB < 32 ? g.index % per_warp : 0;
+  long long first = (static_cast<long long>(blockIdx.x) * g.per_block + (g.index - mine)) * ROWS;
+
+  Raw<TI, VEC> next[ROWS][NV];
+  Raw<Res, VEC> next_r[ADD ? ROWS : 1][NV];
+  auto fetch = [&](long long r0) {
+#pragma unroll
+    for (int q = 0; q < ROWS; ++q) {
+      const long long r = r0 + q;
+      if (r >= p.rows) return;
+      load_row(x + row_offset(r, p.rows, p.inner, p.outer_stride, p.inner_stride), next[q], g.lane, g.size, C);
+      if constexpr (ADD) load_row(res + r * C, next_r[q], g.lane, g.size, C);
     }
   };
-  fetch(first + mine);
+  fetch(first + mine * ROWS);
   for (; first < p.rows; first += step) {
-    const long long r = first + mine;
-    const bool here = r < p.rows;
-    float v[NV][VEC];
+    const long long r0 = first + mine * ROWS;
+    f32x2 v[ROWS][P];
+    float total[ROWS];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (lane + i * G) * VEC;
-      if (here && c < p.C) {
-        next[i].get(v[i]);
-        if constexpr (ADD) {
-          float a[VEC];
-          next_r[i].get(a);
+    for (int q = 0; q < ROWS; ++q) {
+      unpack(next[q], v[q]);
+      if constexpr (ADD) {
+        f32x2 a[P];
+        unpack(next_r[q], a);
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) a[j] += v[i][j];
-          Raw<TI, VEC> sum;
-          sum.set(a);
-          sum.store(static_cast<TI*>(p.s) + r * p.C + c);
-          sum.get(v[i]);
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) v[i][j] = 0.f;
+        for (int k = 0; k < P; ++k) a[k] = f2_add(a[k], v[q][k]);
+        Raw<TI, VEC> sum[NV];
+        pack(a, sum);
+        if (r0 + q < p.rows) store_row(static_cast<TI*>(p.s) + (r0 + q) * C, sum, g.lane, g.size, C);
+        unpack(sum, v[q]);
       }
+      keep<VEC, NV>(v[q], g.lane, g.size, C);
+      f32x2 t = v[q][0];
+#pragma unroll
+      for (int k = 1; k < P; ++k) t = f2_add(t, v[q][k]);
+      total[q] = sum_of(t);
     }
-    fetch(r + step);
-    float total[1] = {0.f};
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) total[0] += v[i][j];
-    group_sum<G>(total, sh);
-    const float near = total[0] * inv;
+    fetch(r0 + step);
+    g.sum(total, sh);
     // Deviations from the rounded mean; their own mean puts it right (a row of one value comes out as zeros)
-    float a[2] = {0.f, 0.f};
+    float dev[2 * ROWS];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      if ((lane + i * G) * VEC < p.C) {
+    for (int q = 0; q < ROWS; ++q) {
+      const float near = total[q] * inv;
+      const f32x2 n2 = f2_pack(-near, -near);
+      f32x2 s = 0ull, s2 = 0ull;
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          v[i][j] -= near;
-          a[0] += v[i][j];
-          a[1] = fmaf(v[i][j], v[i][j], a[1]);
-        }
+      for (int k = 0; k < P; ++k) v[q][k] = f2_add(v[q][k], n2);
+      keep<VEC, NV>(v[q], g.lane, g.size, C);
+#pragma unroll
+      for (int k = 0; k < P; ++k) {
+        s = f2_add(s, v[q][k]);
+        s2 = f2_fma(v[q][k], v[q][k], s2);
       }
+      dev[2 * q] = sum_of(s);
+      dev[2 * q + 1] = sum_of(s2);
     }
-    group_sum<G>(a, sh + WARPS);
-    const float left = a[0] * inv, rstd = 1.f / sqrtf(fmaxf(fmaf(a[1], inv, -left * left), 0.f) + p.eps);
-    if (!here) continue;
-    if (lane == 0 && p.stats) p.stats[r] = make_float2(near + left, rstd);
-    TO* const to = static_cast<TO*>(p.y) + r * p.C;
+    g.sum(dev, sh + ROWS * MOST_WARPS);
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (lane + i * G) * VEC;
-      if (c < p.C) {
-        float f[VEC];
+    for (int q = 0; q < ROWS; ++q) {
+      const long long r = r0 + q;
+      if (r >= p.rows) break;
+      const float left = dev[2 * q] * inv, rstd = 1.f / sqrtf(fmaxf(fmaf(dev[2 * q + 1], inv, -left * left), 0.f) + p.eps);
+      if (g.lane == 0 && p.stats) p.stats[r] = make_float2(fmaf(total[q], inv, left), rstd);
+      const f32x2 l2 = f2_pack(-left, -left), r2 = f2_pack(rstd, rstd);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) f[j] = (v[i][j] - left) * rstd;
-        if (w) {
-          Raw<float, VEC> q;
-          float a[VEC];
-          q.load(w + c);
-          q.get(a);
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) f[j] *= a[j];
-        }
-        if (b) {
-          Raw<float, VEC> q;
-          float a[VEC];
-          q.load(b + c);
-          q.get(a);
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) f[j] += a[j];
-        }
-        Raw<TO, VEC> out;
-        out.set(f);
-        out.store(to + c);
-      }
+      for (int k = 0; k < P; ++k) v[q][k] = f2_fma(f2_mul(f2_add(v[q][k], l2), r2), wv[k], bv[k]);
+      Raw<TO, VEC> out[NV];
+      pack(v[q], out);
+      store_row(static_cast<TO*>(p.y) + r * C, out, g.lane, g.size, C);
     }
   }
 }
 
-template <typename TI, typename TO, int VEC, int G, int NV>
-__global__ void __launch_bounds__(THREADS) ln_bwd_kernel(LnBackward p) {
-  constexpr int GROUPS = THREADS / G, PER_WARP = G < 32 ? 32 / G : 1;
+// ADD: there is a gradient of the sum in front
+template <typename TI, typename TO, bool ADD, int VEC, int NV, int SUB, int ROWS, int BLOCKS>
+__global__ void __launch_bounds__(THREADS, BLOCKS) ln_bwd_kernel(LnBackward p, int warps) {
+  constexpr int P = Cols<VEC, NV>::PAIRS;
   extern __shared__ float cols[];            // [2][C]: the block's sums
-  __shared__ float sh[2][2 * WARPS];
+  __shared__ float sh[2][2 * ROWS * MOST_WARPS];
   const TI *x = static_cast<const TI*>(p.x), *ds = static_cast<const TI*>(p.ds);
   const TO* dy = static_cast<const TO*>(p.dy);
   const float* w = p.w;
   const float2* stats = p.stats;
   chain_begin(true, x, ds, dy, w, stats);
-  const int lane = threadIdx.x % G, group = threadIdx.x / G;
-  const long long step = static_cast<long long>(gridDim.x) * GROUPS;
-  long long first = static_cast<long long>(blockIdx.x) * GROUPS + group / PER_WARP * PER_WARP;
-  const int mine = group % PER_WARP;
-  const float inv = 1.f / static_cast<float>(p.C);
-  float aw[NV][VEC], ab[NV][VEC];
+  const Group<SUB> g(warps);
+  const int C = p.C;
+  const float inv = 1.f / static_cast<float>(C);
+  f32x2 wv[P], aw[P], ab[P];
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) aw[i][j] = ab[i][j] = 0.f;
+  for (int k = 0; k < P; ++k) {
+    wv[k] = f2_pack(1.f, 1.f);
+    aw[k] = ab[k] = 0ull;
+  }
+  if (w) {
+    Raw<float, VEC> weights[NV];
+    load_row(w, weights, g.lane, g.size, C);
+    unpack(weights, wv);
+    keep<VEC, NV>(wv, g.lane, g.size, C);
+  }
+  const long long step = static_cast<long long>(gridDim.x) * g.per_block * ROWS;
+  const int per_warp = SUB < 32 ? 32 / SUB : 1;
+  const int mine = SUB < 32 ? g.index % per_warp : 0;
+  long long first = (static_cast<long long>(blockIdx.x) * g.per_block + (g.index - mine)) * ROWS;
 
-  Raw<TI, VEC> nx[NV];
-  Raw<TO, VEC> ny[NV];
-  float2 nst;
-  auto fetch = [&](long long r) {
-    if (r >= p.rows) return;
-    nst = __ldg(stats + r);
-    const TI* const from = x + row_offset(r, p.inner, p.outer_stride, p.inner_stride);
+  Raw<TI, VEC> nx[ROWS][NV], nd[ADD ? ROWS : 1][NV];
+  Raw<TO, VEC> ny[ROWS][NV];
+  float2 nst[ROWS];
+  auto fetch = [&](long long r0) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (lane + i * G) * VEC;
-      if (c < p.C) {
-        nx[i].load(from + c);
-        ny[i].load(dy + r * p.C + c);
-      }
+    for (int q = 0; q < ROWS; ++q) {
+      const long long r = r0 + q;
+      if (r >= p.rows) return;
+      nst[q] = __ldg(stats + r);
+      load_row(x + row_offset(r, p.rows, p.inner, p.outer_stride, p.inner_stride), nx[q], g.lane, g.size, C);
+      load_row(dy + r * C, ny[q], g.lane, g.size, C);
+      if constexpr (ADD) load_row(ds + r * C, nd[q], g.lane, g.size, C);
     }
   };
-  fetch(first + mine);
+  fetch(first + mine * ROWS);
   for (int turn = 0; first < p.rows; first += step, turn ^= 1) {
-    const long long r = first + mine;
-    const bool here = r < p.rows;
-    float xh[NV][VEC], g[NV][VEC];
-    const float mean = nst.x, rstd = nst.y;
-    float a[2] = {0.f, 0.f};
+    const long long r0 = first + mine * ROWS;
+    f32x2 xh[ROWS][P], gr[ROWS][P];
+    Raw<TI, VEC> d[ADD ? ROWS : 1][NV];
+    float rstd[ROWS], a[2 * ROWS];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (lane + i * G) * VEC;
-      if (here && c < p.C) {
-        nx[i].get(xh[i]);
-        ny[i].get(g[i]);
+    for (int q = 0; q < ROWS; ++q) {
+      const bool here = r0 + q < p.rows;
+      unpack(nx[q], xh[q]);
+      unpack(ny[q], gr[q]);
+      rstd[q] = nst[q].y;
+      if constexpr (ADD) {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          xh[i][j] = (xh[i][j] - mean) * rstd;
-          aw[i][j] = fmaf(g[i][j], xh[i][j], aw[i][j]);
-          ab[i][j] += g[i][j];
-        }
-        if (w) {
-          Raw<float, VEC> q;
-          float f[VEC];
-          q.load(w + c);
-          q.get(f);
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) g[i][j] *= f[j];
-        }
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          a[0] += g[i][j];
-          a[1] = fmaf(g[i][j], xh[i][j], a[1]);
-        }
+        for (int i = 0; i < NV; ++i) d[q][i] = nd[q][i];
       }
+      const f32x2 m2 = f2_pack(-nst[q].x, -nst[q].x), r2 = f2_pack(nst[q].y, nst[q].y);
+#pragma unroll
+      for (int k = 0; k < P; ++k) xh[q][k] = f2_mul(f2_add(xh[q][k], m2), r2);
+      keep<VEC, NV>(xh[q], g.lane, g.size, here ? C : 0);
+      keep<VEC, NV>(gr[q], g.lane, g.size, here ? C : 0);
+      f32x2 s0 = 0ull, s1 = 0ull;
+#pragma unroll
+      for (int k = 0; k < P; ++k) {
+        aw[k] = f2_fma(gr[q][k], xh[q][k], aw[k]);
+        ab[k] = f2_add(ab[k], gr[q][k]);
+        gr[q][k] = f2_mul(gr[q][k], wv[k]);
+        s0 = f2_add(s0, gr[q][k]);
+        s1 = f2_fma(gr[q][k], xh[q][k], s1);
+      }
+      a[2 * q] = sum_of(s0);
+      a[2 * q + 1] = sum_of(s1);
     }
-    fetch(r + step);
-    group_sum<G>(a, sh[turn]);
-    if (!here) continue;
-    const float m0 = a[0] * inv, m1 = a[1] * inv;
+    fetch(r0 + step);
+    g.sum(a, sh[turn]);
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (lane + i * G) * VEC;
-      if (c < p.C) {
-        float f[VEC];
+    for (int q = 0; q < ROWS; ++q) {
+      const long long r = r0 + q;
+      if (r >= p.rows) break;
+      const float m0 = -a[2 * q] * inv, m1 = -a[2 * q + 1] * inv;
+      const f32x2 m02 = f2_pack(m0, m0), m12 = f2_pack(m1, m1), r2 = f2_pack(rstd[q], rstd[q]);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) f[j] = rstd * (g[i][j] - m0 - xh[i][j] * m1);
-        if (ds) {
-          Raw<TI, VEC> q;
-          float e[VEC];
-          q.load(ds + r * p.C + c);
-          q.get(e);
+      for (int k = 0; k < P; ++k) gr[q][k] = f2_mul(f2_fma(xh[q][k], m12, f2_add(gr[q][k], m02)), r2);
+      if constexpr (ADD) {
+        f32x2 e[P];
+        unpack(d[q], e);
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) f[j] += e[j];
-        }
-        Raw<TI, VEC> out;
-        out.set(f);
-        out.store(static_cast<TI*>(p.dx) + r * p.C + c);
-        if (sizeof(TI) == 4 && p.dr) {
-          Raw<__nv_bfloat16, VEC> half;
-          half.set(f);
-          half.store(static_cast<__nv_bfloat16*>(p.dr) + r * p.C + c);
-        }
+        for (int k = 0; k < P; ++k) gr[q][k] = f2_add(gr[q][k], e[k]);
+      }
+      Raw<TI, VEC> out[NV];
+      pack(gr[q], out);
+      store_row(static_cast<TI*>(p.dx) + r * C, out, g.lane, g.size, C);
+      if (sizeof(TI) == 4 && p.dr) {
+        Raw<__nv_bfloat16, VEC> half[NV];
+        pack(gr[q], half);
+        store_row(static_cast<__nv_bfloat16*>(p.dr) + r * C, half, g.lane, g.size, C);
       }
     }
   }
   if (!p.dw) return;
-  // the groups of a warp, then the warps one after the other
-  if constexpr (G < 32) {
+  // the groups of a warp, then those of the block one after the other
+  float fw[2 * P], fb[2 * P];
 #pragma unroll
-    for (int o = G; o < 32; o <<= 1)
-#pragma unroll
-      for (int i = 0; i < NV; ++i)
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          aw[i][j] += __shfl_xor_sync(0xffffffffu, aw[i][j], o);
-          ab[i][j] += __shfl_xor_sync(0xffffffffu, ab[i][j], o);
-        }
+  for (int k = 0; k < P; ++k) {
+    f2_unpack(aw[k], fw[2 * k], fw[2 * k + 1]);
+    f2_unpack(ab[k], fb[2 * k], fb[2 * k + 1]);
   }
-  float* const out_w = gridDim.x == 1 ? p.dw : p.part + static_cast<long long>(blockIdx.x) * p.C;
-  float* const out_b = gridDim.x == 1 ? p.db : p.part + (static_cast<long long>(gridDim.x) + blockIdx.x) * p.C;
-  if constexpr (G <= 32) {
-    for (int k = 0; k < WARPS; ++k) {
-      if ((threadIdx.x >> 5) == k && mine == 0) {
+  if (SUB < 32) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-          const int c = (lane + i * G) * VEC;
-          if (c < p.C) {
+    for (int o = SUB; o < 32; o <<= 1)
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-              cols[c + j] = (k ? cols[c + j] : 0.f) + aw[i][j];
-              cols[p.C + c + j] = (k ? cols[p.C + c + j] : 0.f) + ab[i][j];
-            }
+      for (int k = 0; k < 2 * P; ++k) {
+        fw[k] += __shfl_xor_sync(0xffffffffu, fw[k], o);
+        fb[k] += __shfl_xor_sync(0xffffffffu, fb[k], o);
+      }
+  }
+  const int sets = SUB < 32 ? blockDim.x / 32 : g.per_block, set = SUB < 32 ? threadIdx.x / 32 : g.index;
+  for (int t = 0; t < sets; ++t) {
+    if (set == t && mine == 0) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = (g.lane + i * g.size) * VEC;
+        if (c < C) {
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) {
+            cols[c + j] = (t ? cols[c + j] : 0.f) + fw[i * VEC + j];
+            cols[C + c + j] = (t ? cols[C + c + j] : 0.f) + fb[i * VEC + j];
           }
         }
       }
-      __syncthreads();
     }
-    for (int c = threadIdx.x; c < p.C; c += THREADS) {
-      out_w[c] = cols[c];
-      out_b[c] = cols[p.C + c];
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (lane + i * G) * VEC;
-      if (c < p.C) {
-        Raw<float, VEC> q;
-        q.set(aw[i]);
-        q.store(out_w + c);
-        q.set(ab[i]);
-        q.store(out_b + c);
-      }
-    }
+    __syncthreads();
+  }
+  float* const out_w = gridDim.x == 1 ? p.dw : p.part + static_cast<long long>(blockIdx.x) * C;
+  float* const out_b = gridDim.x == 1 ? p.db : p.part + (static_cast<long long>(gridDim.x) + blockIdx.x) * C;
+  for (int c = threadIdx.x; c < C; c += blockDim.x) {
+    out_w[c] = cols[c];
+    out_b[c] = cols[C + c];
   }
 }
 
-// threads of a row, and blocks
-int ln_group(int C, bool vec) {
-  if (C > 1024) return THREADS;
-  if (vec && C <= 64) return 8;
-  if (vec && C <= 128) return 16;
-  return 32;
+// How a row is spread: warps of a group (0: a part of a warp), threads of a block, rows that it takes at a time; blocks to an SM, rows of a group.  What
+// carries it is bytes on their way.  us by (blocks, rows): forward, 74160 x 1024 bf16, (4, 1) 91, (3, 2) 75, (2, 4) 70 (DRAM 46); 129600 x 48 8.5, 7.6, 8.1;
+// 16471 x 387 fp32 22.5, 19.4, 18.0.  Forward and backward of the first (3, 1) 195, (2, 2) 163, (2, 3) 203 (DRAM 116).  (A warp to a row, its weights
+// read again for every row: 71 and 212; 16471 x 387 74.)  Behind a sum one row at a time: 16200 x 768 (4, 1) 21.4, (3, 2) 25.2 (DRAM 15).
+constexpr int FWD_BLOCKS = 2, BWD_BLOCKS = 2;
+constexpr int WIDE = 2048, RAGGED = 1024;      // most channels of eight warps with one vector, or four single values, a thread
+struct Spread {
+  int warps, threads, rows;
+};
+Spread spread(int C, bool vec, int rows_at_a_time) {
+  if (vec && C <= 128) return {0, THREADS, THREADS / (C <= 64 ? 8 : 16) * rows_at_a_time};
+  const int per_warp = vec ? (C <= WIDE ? 256 : 1024) : (C <= RAGGED ? 128 : 1024);
+  const int warps = (C + per_warp - 1) / per_warp, groups = MOST_WARPS / warps;
+  return {warps, 32 * warps * groups, groups * (C <= (vec ? WIDE : RAGGED) ? rows_at_a_time : 1)};
 }
-unsigned ln_blocks(long long rows, int C, bool vec, int per_sm) {
-  const long long groups = THREADS / ln_group(C, vec);
-  return static_cast<unsigned>(std::max<long long>(1, std::min<long long>((rows + groups - 1) / groups, 1ll * per_sm * sm_count())));
+unsigned blocks_of(long long rows, const Spread& s, int per_sm) {
+  return static_cast<unsigned>(std::max<long long>(1, std::min<long long>((rows + s.rows - 1) / s.rows, 1ll * per_sm * sm_count())));
 }
-constexpr int FWD_PER_SM = 4, BWD_PER_SM = 2;
+constexpr int FWD_ROWS = 4, BWD_ROWS = 2;
+constexpr int FWD_ADD_BLOCKS = 4;      // one row at a time where two tensors are read
 
 bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-template <typename TI, typename TO, int VEC, int G, int NV>
+template <typename TI, typename TO, int VEC, int NV, int SUB>
 cudaError_t launch(const LnForward& p, cudaStream_t s) {
-  const unsigned grid = ln_blocks(p.rows, p.C, VEC > 1, FWD_PER_SM);
-  auto go = [&](auto* kernel) { return launch_chained(kernel, dim3(grid), dim3(THREADS), 0, s, 1, true, p); };
-  if (!p.r) return go(ln_fwd_kernel<TI, TO, void, VEC, G, NV>);
+  constexpr bool BIG = VEC * NV > 8;
+  auto go = [&](auto* kernel, int rows, int blocks) {
+    const Spread q = spread(p.C, VEC > 1, rows);
+    return launch_chained(kernel, dim3(blocks_of(p.rows, q, blocks)), dim3(q.threads), 0, s, 1, true, p, q.warps);
+  };
+  constexpr int ROWS = BIG ? 1 : FWD_ROWS, BLOCKS = BIG ? 1 : FWD_BLOCKS, ADD_BLOCKS = BIG ? 1 : FWD_ADD_BLOCKS;
+  if (!p.r) return go(ln_fwd_kernel<TI, TO, void, VEC, NV, SUB, ROWS, BLOCKS>, FWD_ROWS, FWD_BLOCKS);
   if constexpr (sizeof(TI) == 4)
-    if (!p.r_f32) return go(ln_fwd_kernel<TI, TO, __nv_bfloat16, VEC, G, NV>);
-  return go(ln_fwd_kernel<TI, TO, TI, VEC, G, NV>);
+    if (!p.r_f32) return go(ln_fwd_kernel<TI, TO, __nv_bfloat16, VEC, NV, SUB, 1, ADD_BLOCKS>, 1, FWD_ADD_BLOCKS);
+  return go(ln_fwd_kernel<TI, TO, TI, VEC, NV, SUB, 1, ADD_BLOCKS>, 1, FWD_ADD_BLOCKS);
 }
-template <typename TI, typename TO, int VEC, int G, int NV>
+template <typename TI, typename TO, int VEC, int NV, int SUB>
 cudaError_t launch(const LnBackward& p, cudaStream_t s) {
-  const unsigned grid = ln_blocks(p.rows, p.C, VEC > 1, BWD_PER_SM);
-  return launch_chained(ln_bwd_kernel<TI, TO, VEC, G, NV>, dim3(grid), dim3(THREADS), G <= 32 ? 8 * p.C : 0, s, 1, true, p);
+  constexpr bool BIG = VEC * NV > 8;
+  constexpr int ROWS = BIG ? 1 : BWD_ROWS, BLOCKS = BIG ? 1 : BWD_BLOCKS;
+  const Spread q = spread(p.C, VEC > 1, BWD_ROWS);
+  auto go = [&](auto* kernel, std::atomic<uint64_t>& devices) {
+    const cudaError_t e = BIG ? allow_shared_memory(devices, reinterpret_cast<const void*>(kernel), 8 * LN_CHANNELS) : cudaSuccess;
+    if (e != cudaSuccess) return e;
+    return launch_chained(kernel, dim3(blocks_of(p.rows, q, BWD_BLOCKS)), dim3(q.threads), 8 * p.C, s, 1, true, p, q.warps);
+  };
+  static std::atomic<uint64_t> with, without;
+  return p.ds ? go(ln_bwd_kernel<TI, TO, true, VEC, NV, SUB, ROWS, BLOCKS>, with) : go(ln_bwd_kernel<TI, TO, false, VEC, NV, SUB, ROWS, BLOCKS>, without);
 }
 
 template <typename TI, typename TO, typename P>
 cudaError_t by_size(const P& p, bool vec, cudaStream_t s) {
   const int C = p.C;
   if (vec) {
-    if (C <= 64) return launch<TI, TO, 8, 8, 1>(p, s);
-    if (C <= 128) return launch<TI, TO, 8, 16, 1>(p, s);
-    if (C <= 256) return launch<TI, TO, 8, 32, 1>(p, s);
-    if (C <= 512) return launch<TI, TO, 8, 32, 2>(p, s);
-    if (C <= 768) return launch<TI, TO, 8, 32, 3>(p, s);
-    if (C <= 1024) return launch<TI, TO, 8, 32, 4>(p, s);
-    if (C <= 2048) return launch<TI, TO, 8, THREADS, 1>(p, s);
-    return launch<TI, TO, 8, THREADS, 4>(p, s);
+    if (C <= 64) return launch<TI, TO, 8, 1, 8>(p, s);
+    if (C <= 128) return launch<TI, TO, 8, 1, 16>(p, s);
+    if (C <= WIDE) return launch<TI, TO, 8, 1, 32>(p, s);
+    return launch<TI, TO, 8, 4, 32>(p, s);
   }
-  if (C <= 256) return launch<TI, TO, 1, 32, 8>(p, s);
-  if (C <= 512) return launch<TI, TO, 1, 32, 16>(p, s);
-  if (C <= 1024) return launch<TI, TO, 1, 32, 32>(p, s);
-  return launch<TI, TO, 1, THREADS, 32>(p, s);
+  if (C <= RAGGED) return launch<TI, TO, 1, 4, 32>(p, s);
+  return launch<TI, TO, 1, 32, 32>(p, s);
 }
 template <typename P>
 cudaError_t by_type(const P& p, bool vec, cudaStream_t s) {
@@ -453,7 +538,7 @@ cudaError_t layer_norm_fwd(const LnForward& p, cudaStream_t s) {
 
 long long layer_norm_scratch(long long rows, int C) {
   // (as many blocks as either form of the kernel may take)
-  const long long n = std::max(ln_blocks(rows, C, true, BWD_PER_SM), ln_blocks(rows, C, false, BWD_PER_SM));
+  const long long n = std::max(blocks_of(rows, spread(C, C % 8 == 0, BWD_ROWS), BWD_BLOCKS), blocks_of(rows, spread(C, false, BWD_ROWS), BWD_BLOCKS));
   return n > 1 ? 2 * n * C : 0;
 }
 
@@ -463,7 +548,7 @@ cudaError_t layer_norm_bwd(const LnBackward& p, int* launches, cudaStream_t s) {
   if (p.rows <= 0) return cudaSuccess;
   const bool vec = p.C % 8 == 0 && p.outer_stride % 8 == 0 && p.inner_stride % 8 == 0 && aligned(p.x) && aligned(p.dy) && aligned(p.ds) &&
                    aligned(p.dx) && aligned(p.dr) && aligned(p.w) && aligned(p.dw) && aligned(p.db) && aligned(p.part);
-  const unsigned blocks = ln_blocks(p.rows, p.C, vec, BWD_PER_SM);
+  const unsigned blocks = blocks_of(p.rows, spread(p.C, vec, BWD_ROWS), BWD_BLOCKS);
   if (p.dw && blocks > 1 && !p.part) return cudaErrorInvalidValue;
   ++*launches;
   const cudaError_t e = by_type(p, vec, s);
