@@ -24,12 +24,13 @@ struct AttnShape {
   int sequences;
 };
 
-// o [B, N, H, D] dense; lse [B, H, N]: log2 of the sum of exponentials of every row (with `lse` null it is not written)
-cudaError_t attention_fwd(const AttnShape& p, const AttnTensor& q, const AttnTensor& k, const AttnTensor& v, __nv_bfloat16* o, float* lse, int* err,
-                          cudaStream_t s);
-// dq, dk, dv from o and d_o (dense, like o); delta [B, H, N]: room for the row sums of o d_o.  Two launches, no atomics.
+// o [B, N, H, D] dense.  For a backward pass (both or none): lse [B, H, N], log2 of the sum of exponentials of every row, and o_rest, like o, what the
+// rounding of o has left out, rounded in its turn.
+cudaError_t attention_fwd(const AttnShape& p, const AttnTensor& q, const AttnTensor& k, const AttnTensor& v, __nv_bfloat16* o, __nv_bfloat16* o_rest,
+                          float* lse, int* err, cudaStream_t s);
+// dq, dk, dv from o, o_rest and d_o (dense, like o); delta [B, H, N]: room for the row sums of o d_o.  Two launches, no atomics.
 cudaError_t attention_bwd(const AttnShape& p, const AttnTensor& q, const AttnTensor& k, const AttnTensor& v, const __nv_bfloat16* o,
-                          const __nv_bfloat16* d_o, const float* lse, float* delta, const AttnTensor& dq, const AttnTensor& dk, const AttnTensor& dv,
-                          int* err, cudaStream_t s);
+                          const __nv_bfloat16* o_rest, const __nv_bfloat16* d_o, const float* lse, float* delta, const AttnTensor& dq,
+                          const AttnTensor& dk, const AttnTensor& dv, int* err, cudaStream_t s);
 
 }  // namespace mk

@@ -273,22 +273,28 @@ mk::AttnShape shape_of(const Tensor& q, const Tensor& k, const Tensor& v, const 
   return p;
 }
 
-std::tuple<Tensor, OptTensor> attention_forward(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, const OptTensor& offsets, bool causal,
+// (o, what its rounding left out, L): the last two with `train`
+std::tuple<Tensor, Tensor, Tensor> attention_forward(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, const OptTensor& offsets, bool causal,
                                                 double scale, bool train) {
   const mk::AttnShape p = shape_of(q_in, k_in, v_in, offsets, causal, scale);
   c10::cuda::CUDAGuard guard(q_in.device());
-  Tensor o = at::empty(q_in.sizes(), q_in.options()), lse;
-  if (train) lse = at::empty({p.B, p.H, p.N}, q_in.options().dtype(at::kFloat));
-  if (o.numel() == 0) return {o, maybe(lse)};
+  Tensor o = at::empty(q_in.sizes(), q_in.options()), rest, lse;
+  if (train) {
+    rest = at::empty(q_in.sizes(), q_in.options());
+    lse = at::empty({p.B, p.H, p.N}, q_in.options().dtype(at::kFloat));
+  }
+  if (o.numel() == 0) return {o, rest, lse};
   const Tensor q = readable(q_in), k = readable(k_in), v = readable(v_in);
   ++mkh::launches();
-  mkh::check(mk::attention_fwd(p, view_of(q), view_of(k), view_of(v), bf(o), ptr_or_null<float>(lse), mkh::error_word(q), mkh::stream()), "attention_fwd");
-  return {o, maybe(lse)};
+  mkh::check(mk::attention_fwd(p, view_of(q), view_of(k), view_of(v), bf(o), ptr_or_null<__nv_bfloat16>(rest), ptr_or_null<float>(lse), mkh::error_word(q),
+                               mkh::stream()),
+             "attention_fwd");
+  return {o, rest, lse};
 }
 
 // gradients into tensors [B, N, heads, D] (strides as `readable` has them)
-void attention_backward(const Tensor& d_out, const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, const Tensor& o, const Tensor& lse,
-                        const OptTensor& offsets, bool causal, double scale, const Tensor& dq, const Tensor& dk, const Tensor& dv) {
+void attention_backward(const Tensor& d_out, const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, const Tensor& o, const Tensor& rest,
+                        const Tensor& lse, const OptTensor& offsets, bool causal, double scale, const Tensor& dq, const Tensor& dk, const Tensor& dv) {
   const mk::AttnShape p = shape_of(q_in, k_in, v_in, offsets, causal, scale);
   c10::cuda::CUDAGuard guard(q_in.device());
   MK_CHECK(d_out.device() == o.device() && d_out.sizes() == o.sizes() && d_out.scalar_type() == at::kBFloat16,
@@ -298,7 +304,7 @@ void attention_backward(const Tensor& d_out, const Tensor& q_in, const Tensor& k
   if (reinterpret_cast<uintptr_t>(g.data_ptr()) & 15) g = g.clone();
   const Tensor q = readable(q_in), k = readable(k_in), v = readable(v_in), delta = at::empty_like(lse);
   mkh::launches() += 2;
-  mkh::check(mk::attention_bwd(p, view_of(q), view_of(k), view_of(v), bf(o), bf(g), lse.data_ptr<float>(), delta.data_ptr<float>(), view_of(dq),
+  mkh::check(mk::attention_bwd(p, view_of(q), view_of(k), view_of(v), bf(o), bf(rest), bf(g), lse.data_ptr<float>(), delta.data_ptr<float>(), view_of(dq),
                                view_of(dk), view_of(dv), mkh::error_word(q), mkh::stream()),
              "attention_bwd");
 }
@@ -306,9 +312,9 @@ void attention_backward(const Tensor& d_out, const Tensor& q_in, const Tensor& k
 struct Attention : torch::autograd::Function<Attention> {
   static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& offsets, bool causal, double scale,
                         bool train) {
-    auto [o, lse] = attention_forward(q, k, v, offsets, causal, scale, train);
+    auto [o, rest, lse] = attention_forward(q, k, v, offsets, causal, scale, train);
     if (train) {
-      ctx->save_for_backward({q, k, v, o, *lse, value(offsets)});
+      ctx->save_for_backward({q, k, v, o, rest, lse, value(offsets)});
       ctx->saved_data["causal"] = causal;
       ctx->saved_data["scale"] = scale;
     }
@@ -318,7 +324,7 @@ struct Attention : torch::autograd::Function<Attention> {
     const Backward count;
     const variable_list s = ctx->get_saved_variables();
     const Tensor dq = at::empty(s[0].sizes(), s[0].options()), dk = at::empty(s[1].sizes(), s[1].options()), dv = at::empty(s[2].sizes(), s[2].options());
-    attention_backward(grads[0], s[0], s[1], s[2], s[3], s[4], maybe(s[5]), ctx->saved_data["causal"].toBool(), ctx->saved_data["scale"].toDouble(), dq, dk,
+    attention_backward(grads[0], s[0], s[1], s[2], s[3], s[4], s[5], maybe(s[6]), ctx->saved_data["causal"].toBool(), ctx->saved_data["scale"].toDouble(), dq, dk,
                        dv);
     return once_differentiable({dq, dk, dv, Tensor(), Tensor(), Tensor(), Tensor()});
   }
@@ -345,9 +351,9 @@ struct AttentionQkv : torch::autograd::Function<AttentionQkv> {
   static Tensor forward(AutogradContext* ctx, const Tensor& qkv, int64_t heads, int64_t kv_heads, const OptTensor& offsets, bool causal, double scale,
                         bool train) {
     const Parts p(qkv, heads, kv_heads);
-    auto [o, lse] = attention_forward(p.q, p.k, p.v, offsets, causal, scale, train);
+    auto [o, rest, lse] = attention_forward(p.q, p.k, p.v, offsets, causal, scale, train);
     if (train) {
-      ctx->save_for_backward({qkv, o, *lse, value(offsets)});
+      ctx->save_for_backward({qkv, o, rest, lse, value(offsets)});
       ctx->saved_data["heads"] = heads;
       ctx->saved_data["kv_heads"] = kv_heads;
       ctx->saved_data["causal"] = causal;
@@ -361,7 +367,7 @@ struct AttentionQkv : torch::autograd::Function<AttentionQkv> {
     const int64_t heads = ctx->saved_data["heads"].toInt(), kv_heads = ctx->saved_data["kv_heads"].toInt();
     const Tensor dqkv = at::empty(s[0].sizes(), s[0].options());
     const Parts p(s[0], heads, kv_heads), d(dqkv, heads, kv_heads);
-    attention_backward(grads[0], p.q, p.k, p.v, s[1], s[2], maybe(s[3]), ctx->saved_data["causal"].toBool(), ctx->saved_data["scale"].toDouble(), d.q, d.k,
+    attention_backward(grads[0], p.q, p.k, p.v, s[1], s[2], s[3], maybe(s[4]), ctx->saved_data["causal"].toBool(), ctx->saved_data["scale"].toDouble(), d.q, d.k,
                        d.v);
     return once_differentiable({dqkv, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()});
   }
