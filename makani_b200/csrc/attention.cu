@@ -301,12 +301,14 @@ __device__ __forceinline__ void zero_row(int D, __nv_bfloat16* to) {
   for (int c = 0; c < D; c += 8) *reinterpret_cast<uint4*>(to + c) = make_uint4(0, 0, 0, 0);
 }
 
-__device__ __forceinline__ void tmem_alloc_all(volatile uint32_t* slot) {
-  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(const_cast<uint32_t*>(slot))), "r"(512u) : "memory");
+template <uint32_t COLS>
+__device__ __forceinline__ void tmem_alloc(volatile uint32_t* slot) {
+  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(const_cast<uint32_t*>(slot))), "r"(COLS) : "memory");
   asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
 }
-__device__ __forceinline__ void tmem_free_all(uint32_t tmem) {
-  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+template <uint32_t COLS>
+__device__ __forceinline__ void tmem_free(uint32_t tmem) {
+  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(COLS) : "memory");
 }
 
 // ------------------------------------------------------------------------------------------ forward
@@ -381,27 +383,32 @@ __device__ __forceinline__ void scale_row(uint32_t o_at, int cols, float f) {
   }
 }
 
-// Two tiles of 128 queries share every tile of keys and values, so that the products of one run beside the exponentials of the other.  Tensor
-// memory: S of either (128 columns, P takes the first 64 of them), O of either (up to 128).
-struct FwdWide {
-  static constexpr int DB = 2, STAGES = 2, TILE_BYTES = DB * BOX;
-  static constexpr int K_AT = 2 * TILE_BYTES, V_AT = K_AT + STAGES * TILE_BYTES, BAR_AT = V_AT + STAGES * TILE_BYTES;
+// S in tensor memory (128 columns a query tile) is replaced by P in its first half; O has 128 columns beside it.  Two query tiles share every tile of keys
+// and values, so that the products of one run beside the exponentials of the other; with one (short sequences) two CTAs share an SM instead, each
+// with half of its tensor memory, and one's start and end run beside the other's work.
+template <int DB, int QT>
+struct Fwd {
+  static constexpr int STAGES = QT == 2 ? 2 : 3 - DB, TILE_BYTES = DB * BOX, WARPS = COMPUTE_WARP + 4 * QT, THREADS_ = 32 * WARPS;
+  static constexpr int K_AT = QT * TILE_BYTES, V_AT = K_AT + STAGES * TILE_BYTES, BAR_AT = V_AT + STAGES * TILE_BYTES;
   static constexpr int BARS = 4 * STAGES + 7;
   static constexpr int SMEM = BAR_AT + 8 * BARS + 16 + 1024;
-  static_assert(SMEM <= SMEM_LIMIT);
+  static constexpr uint32_t COLS = 256 * QT, O_AT = 128 * QT;
+  // registers: within the launch's, 168 or (two CTAs) 128 a thread
+  static constexpr int FEW = QT == 2 ? FEW_REGS : 56, MANY = QT == 2 ? MANY_REGS : 200;
+  static_assert(SMEM * (3 - QT) <= SMEM_LIMIT && 128 * FEW + 128 * QT * MANY <= THREADS_ * (QT == 2 ? 168 : 128));
 };
-constexpr uint32_t S_COLS = 128, O_AT = 256;
+constexpr uint32_t S_COLS = 128;
 struct FwdParams {
   TileParams t;
   __nv_bfloat16 *o, *o_rest;
   float* lse;
 };
 
-__global__ void __launch_bounds__(THREADS, 1)
+template <int DB, int QT>
+__global__ void __launch_bounds__(Fwd<DB, QT>::THREADS_, 3 - QT)
 attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                 const FwdParams p) {
-  using L = FwdWide;
-  constexpr int DB = L::DB;
+  using L = Fwd<DB, QT>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = smem_u32(smem_raw);
   const uint32_t pad = (1024u - (raw_addr & 1023u)) & 1023u;
@@ -434,9 +441,11 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_async_smem();
   }
-  if (warp == 1) tmem_alloc_all(tmem_slot);
+  // (two to an SM: not before the kernel in front has given its tensor memory back, which it may want to take on an SM that this one shares)
+  if (QT == 2 && warp == 1) tmem_alloc<L::COLS>(tmem_slot);
   const int* offsets = p.t.grid.offsets;
   chain_begin(true, offsets);
+  if (QT == 1 && warp == 1) tmem_alloc<L::COLS>(tmem_slot);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -444,7 +453,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
 
   Work w;
   const bool any = find_work(p.t.grid, offsets, blockIdx.x, w);
-  const int rows = any ? min(w.len - w.r0, 2 * TILE) : 0;
+  const int rows = any ? min(w.len - w.r0, QT * TILE) : 0;
   const bool causal = p.t.causal != 0;
   auto tiles_of = [&](int t) {      // of keys, that the queries of tile t see
     if (w.padding || rows <= t * TILE) return 0;
@@ -457,7 +466,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
   const bool fix = n > 0 && tail < TILE && w.lo + w.len < p.t.grid.N;
 
   if (warp < COMPUTE_WARP) {
-    regs_down<FEW_REGS>();
+    regs_down<L::FEW>();
     if (warp == 0) {
     // ------------------------------------------------------------------ tiles
     if (n > 0 && elect_one()) {
@@ -537,7 +546,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
           const uint32_t b = v_lo + s * (L::TILE_BYTES >> 4);
 #pragma unroll
           for (int i = 0; i < TILE / 16; ++i)
-            mma_ts(tmem + O_AT + t * ATTN_WIDTH, tmem + t * S_COLS + i * 8, b + i * (2048 >> 4), hi, id_o, j > 0 || i > 0);
+            mma_ts(tmem + L::O_AT + t * ATTN_WIDTH, tmem + t * S_COLS + i * 8, b + i * (2048 >> 4), hi, id_o, j > 0 || i > 0);
           // (in order behind the products above: S takes the place of P)
           if (j + 1 < nt) scores(t, sn);
           else tc_commit(s_full(t));
@@ -557,11 +566,11 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     }
     }
   } else {
-    regs_up<MANY_REGS>();
+    regs_up<L::MANY>();
     // ------------------------------------------------------------------ softmax
     const int t = (warp - COMPUTE_WARP) >> 2, row = t * TILE + (warp & 3) * 32 + lane, nt = t == 0 ? n0 : n1;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t s_at = tmem + lanes + t * S_COLS, o_at = tmem + lanes + O_AT + t * ATTN_WIDTH;
+    const uint32_t s_at = tmem + lanes + t * S_COLS, o_at = tmem + lanes + L::O_AT + t * ATTN_WIDTH;
     const float scale = p.t.scale_log2;
     const bool here = row < rows;
     Row r;
@@ -605,7 +614,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
   __syncthreads();
   if (warp == 1) {
     tc_fence_after();
-    tmem_free_all(tmem);
+    tmem_free<L::COLS>(tmem);
   }
 }
 
@@ -659,7 +668,7 @@ attn_fwd_narrow_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_async_smem();
   }
-  if (warp == 1) tmem_alloc_all(tmem_slot);
+  if (warp == 1) tmem_alloc<512>(tmem_slot);
   const int* offsets = p.t.grid.offsets;
   chain_begin(true, offsets);
   tc_fence_before();
@@ -834,7 +843,7 @@ attn_fwd_narrow_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
   __syncthreads();
   if (warp == 1) {
     tc_fence_after();
-    tmem_free_all(tmem);
+    tmem_free<512>(tmem);
   }
 }
 
@@ -937,7 +946,7 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_async_smem();
   }
-  if (warp == 1) tmem_alloc_all(tmem_slot);
+  if (warp == 1) tmem_alloc<512>(tmem_slot);
   const int* offsets = p.t.grid.offsets;
   const __nv_bfloat16 *out = p.o, *rest = p.o_rest, *d_out = p.d_o;
   const float* lse = p.lse;
@@ -1125,7 +1134,7 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
   __syncthreads();
   if (warp == 1) {
     tc_fence_after();
-    tmem_free_all(tmem);
+    tmem_free<512>(tmem);
   }
 }
 
@@ -1184,7 +1193,7 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_async_smem();
   }
-  if (warp == 1) tmem_alloc_all(tmem_slot);
+  if (warp == 1) tmem_alloc<512>(tmem_slot);
   const int* offsets = p.t.grid.offsets;
   const float *lse = p.lse, *delta = p.delta;
   chain_begin(true, offsets, lse, delta);
@@ -1432,7 +1441,7 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
   __syncthreads();
   if (warp == 1) {
     tc_fence_after();
-    tmem_free_all(tmem);
+    tmem_free<512>(tmem);
   }
 }
 
@@ -1481,15 +1490,30 @@ TileParams tile_params(const AttnShape& p, const Slots& g, int* err) {
   return t;
 }
 
-cudaError_t launch_fwd(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const FwdParams& p, cudaStream_t s) {
-  static std::atomic<uint64_t> narrow, wide;
-  const bool fits = p.t.D <= 64;
-  const cudaError_t e = fits ? allow_shared_memory(narrow, reinterpret_cast<const void*>(&attn_fwd_narrow_kernel), FwdNarrow::SMEM)
-                             : allow_shared_memory(wide, reinterpret_cast<const void*>(&attn_fwd_kernel), FwdWide::SMEM);
+template <typename... Params>
+cudaError_t launch(void (*kernel)(Params...), std::atomic<uint64_t>& devices, int threads, int smem, const CUtensorMap& q, const CUtensorMap& k,
+                   const CUtensorMap& v, const FwdParams& p, cudaStream_t s) {
+  const cudaError_t e = allow_shared_memory(devices, reinterpret_cast<const void*>(kernel), smem);
   if (e != cudaSuccess) return e;
-  const dim3 grid(static_cast<unsigned>(blocks_of(p.t.grid)));
-  if (fits) return launch_chained(attn_fwd_narrow_kernel, grid, dim3(THREADS), FwdNarrow::SMEM, s, 1, true, q, k, v, p);
-  return launch_chained(attn_fwd_kernel, grid, dim3(THREADS), FwdWide::SMEM, s, 1, true, q, k, v, p);
+  return launch_chained(kernel, dim3(static_cast<unsigned>(blocks_of(p.t.grid))), dim3(threads), smem, s, 1, true, q, k, v, p);
+}
+// One query tile to a CTA, two CTAs to an SM, where sequences are short and CTAs of two tiles would take the SMs more than once.  us, two tiles / one, heads of
+// 64 (batch x tokens x heads): 64 x 128 x 8 19.3 / 11.6, 64 x 200 x 8 32.7 / 27.9, 32 x 384 x 8 33.7 / 27.1, 16 x 512 x 8 23.4 / 22.5, 8 x 768 x 8 28.9 / 26.1, 8 x
+// 1024 x 8 35.7 / 36.5, 2 x 4096 x 8 104 / 121; fitting at once 16 x 128 x 8 5.4 / 6.2, 16 x 256 x 8 8.7 / 8.5.  Heads of 96: 64 x 128 x 8 23.4 / 16.3, 32 x 384 x 8
+// 41.6 / 35.4, 16 x 512 x 8 27.7 / 28.3, 8 x 768 x 8 34.0 / 34.9; packed, 41 sequences of 7001 tokens 52.7 / 45.6.  (Lengths of packed sequences are on the
+// device: their mean is known.)
+bool one_tile_pays(const AttnShape& p) {
+  const int mean = p.offsets ? p.N / std::max(1, p.sequences) : p.N;
+  return mean <= (p.D <= 64 ? 768 : 448) && blocks_of(slots_of(p, p.H, 2 * TILE, 1)) > sm_count();
+}
+cudaError_t launch_fwd(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const FwdParams& p, bool one_tile, cudaStream_t s) {
+  static std::atomic<uint64_t> devices[4];
+  if (one_tile) {
+    if (p.t.D <= 64) return launch(attn_fwd_kernel<1, 1>, devices[0], Fwd<1, 1>::THREADS_, Fwd<1, 1>::SMEM, q, k, v, p, s);
+    return launch(attn_fwd_kernel<2, 1>, devices[1], Fwd<2, 1>::THREADS_, Fwd<2, 1>::SMEM, q, k, v, p, s);
+  }
+  if (p.t.D <= 64) return launch(attn_fwd_narrow_kernel, devices[2], THREADS, FwdNarrow::SMEM, q, k, v, p, s);
+  return launch(attn_fwd_kernel<2, 2>, devices[3], Fwd<2, 2>::THREADS_, Fwd<2, 2>::SMEM, q, k, v, p, s);
 }
 template <int DB>
 cudaError_t launch_dq(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& g, const DqParams& p, cudaStream_t s) {
@@ -1516,11 +1540,12 @@ cudaError_t attention_fwd(const AttnShape& p, const AttnTensor& q, const AttnTen
   CUtensorMap mq, mk_, mv;
   if (!map_of(&mq, q, p, p.H) || !map_of(&mk_, k, p, p.Hk) || !map_of(&mv, v, p, p.Hk)) return cudaErrorInvalidValue;
   FwdParams f;
-  f.t = tile_params(p, slots_of(p, p.H, 2 * TILE, 1), err);
+  const bool one_tile = one_tile_pays(p);
+  f.t = tile_params(p, slots_of(p, p.H, one_tile ? TILE : 2 * TILE, 1), err);
   f.o = o;
   f.o_rest = o_rest;
   f.lse = lse;
-  return launch_fwd(mq, mk_, mv, f, s);
+  return launch_fwd(mq, mk_, mv, f, one_tile, s);
 }
 
 cudaError_t attention_bwd(const AttnShape& p, const AttnTensor& q, const AttnTensor& k, const AttnTensor& v, const __nv_bfloat16* o,
