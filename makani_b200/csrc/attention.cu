@@ -398,8 +398,45 @@ struct Fwd {
   static_assert(SMEM * (3 - QT) <= SMEM_LIMIT && 128 * FEW + 128 * QT * MANY <= THREADS_ * (QT == 2 ? 168 : 128));
 };
 constexpr uint32_t S_COLS = 128;
+// Of the pairs of query tiles, those from `whole` on are split over the keys into `parts` CTAs each, which leave O (not divided) and maximum and sum of every
+// row for the kernel that joins them
+struct Split {
+  uint32_t whole;
+  int parts;               // 0: none is split
+  float* o;                // [pair - whole][part][2 TILE][D]
+  float2* ml;              // [pair - whole][part][2 TILE]
+};
+// What a CTA has of it: its pair of tiles, its part (-1: all keys), tiles of keys in front of its own and number of its own
+struct Share {
+  uint32_t pair;
+  int part, first, n;
+  __device__ __forceinline__ explicit Share(const Split& s) : pair(blockIdx.x), part(-1) {
+    if (s.parts > 0 && blockIdx.x >= s.whole) {
+      pair = s.whole + (blockIdx.x - s.whole) / s.parts;
+      part = static_cast<int>((blockIdx.x - s.whole) % s.parts);
+    }
+  }
+  __device__ __forceinline__ void keys(const Split& s, int tiles) {
+    first = part < 0 ? 0 : tiles * part / s.parts;
+    n = (part < 0 ? tiles : tiles * (part + 1) / s.parts) - first;
+  }
+  __device__ __forceinline__ void store(const Split& s, int row, int D, uint32_t o_at, float m, float total, bool here) const {
+    const long long at = (static_cast<long long>(pair - s.whole) * s.parts + part) * (2 * TILE) + row;
+    for (int c = 0; c < D; c += 8) {
+      uint32_t v[8];
+      tmem_ld8(o_at + c, v);
+      if (here) {
+        reinterpret_cast<uint4*>(s.o + at * D + c)[0] = make_uint4(v[0], v[1], v[2], v[3]);
+        reinterpret_cast<uint4*>(s.o + at * D + c)[1] = make_uint4(v[4], v[5], v[6], v[7]);
+      }
+    }
+    if (here) s.ml[at] = make_float2(m, total);
+  }
+};
+
 struct FwdParams {
   TileParams t;
+  Split split;
   __nv_bfloat16 *o, *o_rest;
   float* lse;
 };
@@ -452,7 +489,8 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
   const uint32_t tmem = *tmem_slot;
 
   Work w;
-  const bool any = find_work(p.t.grid, offsets, blockIdx.x, w);
+  Share share(p.split);
+  const bool any = find_work(p.t.grid, offsets, share.pair, w);
   const int rows = any ? min(w.len - w.r0, QT * TILE) : 0;
   const bool causal = p.t.causal != 0;
   auto tiles_of = [&](int t) {      // of keys, that the queries of tile t see
@@ -460,9 +498,15 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     const int last = causal ? w.r0 + min(rows, (t + 1) * TILE) - 1 : w.len - 1;
     return last / TILE + 1;
   };
-  const int n0 = tiles_of(0), n1 = tiles_of(1), n = max(n0, n1);
+  int n0 = tiles_of(0), n1 = tiles_of(1);
+  share.keys(p.split, max(n0, n1));
+  const int n = share.n, j0 = share.first;
+  if (share.part >= 0) {      // (not causal: both see the same keys)
+    n0 = n0 > 0 ? n : 0;
+    n1 = n1 > 0 ? n : 0;
+  }
   // keys of the last tile that belong to the sequence, where other tokens follow it
-  const int tail = w.len - (n - 1) * TILE;
+  const int tail = w.len - (j0 + n - 1) * TILE;
   const bool fix = n > 0 && tail < TILE && w.lo + w.len < p.t.grid.N;
 
   if (warp < COMPUTE_WARP) {
@@ -482,13 +526,13 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
           break;
         }
         mbar_expect_tx(k_full(s), L::TILE_BYTES);
-        for (int b = 0; b < DB; ++b) tma_load_4d(base + L::K_AT + s * L::TILE_BYTES + b * BOX, &map_k, k_full(s), b * 64, w.lo + j * TILE, hk, w.b);
+        for (int b = 0; b < DB; ++b) tma_load_4d(base + L::K_AT + s * L::TILE_BYTES + b * BOX, &map_k, k_full(s), b * 64, w.lo + (j0 + j) * TILE, hk, w.b);
         if (!mbar_wait(v_empty(s), ph ^ 1u)) {
           atomicExch(p.t.err, 80);
           break;
         }
         mbar_expect_tx(v_full(s), L::TILE_BYTES);
-        for (int b = 0; b < DB; ++b) tma_load_4d(base + L::V_AT + s * L::TILE_BYTES + b * BOX, &map_v, v_full(s), b * 64, w.lo + j * TILE, hk, w.b);
+        for (int b = 0; b < DB; ++b) tma_load_4d(base + L::V_AT + s * L::TILE_BYTES + b * BOX, &map_v, v_full(s), b * 64, w.lo + (j0 + j) * TILE, hk, w.b);
         if (++s == L::STAGES) {
           s = 0;
           ph ^= 1u;
@@ -581,7 +625,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       tc_fence_after();
       uint32_t v[TILE];
       load_scores(s_at, v);
-      const int k0 = j * TILE;
+      const int k0 = (j0 + j) * TILE;
       if (k0 + TILE > w.len || (causal && k0 + TILE - 1 > w.r0 + t * TILE)) hide_scores(v, (causal ? min(w.len, w.r0 + row + 1) : w.len) - k0);
       const float top = max_of<false>(v) * scale;
       if (__any_sync(0xffffffffu, r.grows(top))) {
@@ -602,8 +646,9 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     if (nt > 0 && ok) {
       tc_fence_after();
       const float total = r.total();
-      store_output(o_at, p.t.D, 1.f / total, to, p.o_rest ? p.o_rest + (to - p.o) : nullptr, here);
-      if (here && p.lse)
+      if (share.part >= 0) share.store(p.split, row, p.t.D, o_at, r.m, total, here);
+      else store_output(o_at, p.t.D, 1.f / total, to, p.o_rest ? p.o_rest + (to - p.o) : nullptr, here);
+      if (here && p.lse && share.part < 0)
         p.lse[(static_cast<long long>(w.b) * p.t.grid.H + w.h) * p.t.grid.N + w.lo + w.r0 + row] = r.m + __log2f(total);
     } else if (here && w.padding) {
       zero_row(p.t.D, to);
@@ -677,7 +722,8 @@ attn_fwd_narrow_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
   const uint32_t tmem = *tmem_slot;
 
   Work w;
-  const bool any = find_work(p.t.grid, offsets, blockIdx.x, w);
+  Share share(p.split);
+  const bool any = find_work(p.t.grid, offsets, share.pair, w);
   const int rows = any ? min(w.len - w.r0, 2 * TILE) : 0;
   const bool causal = p.t.causal != 0;
   auto tiles_of = [&](int t) {      // of keys, that the queries of tile t see
@@ -685,8 +731,14 @@ attn_fwd_narrow_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     const int last = causal ? w.r0 + min(rows, (t + 1) * TILE) - 1 : w.len - 1;
     return last / TILE + 1;
   };
-  const int n0 = tiles_of(0), n1 = tiles_of(1), n = max(n0, n1);
-  const int tail = w.len - (n - 1) * TILE;
+  int n0 = tiles_of(0), n1 = tiles_of(1);
+  share.keys(p.split, max(n0, n1));
+  const int n = share.n, j0 = share.first;
+  if (share.part >= 0) {      // (not causal: both see the same keys)
+    n0 = n0 > 0 ? n : 0;
+    n1 = n1 > 0 ? n : 0;
+  }
+  const int tail = w.len - (j0 + n - 1) * TILE;
   const bool fix = n > 0 && tail < TILE && w.lo + w.len < p.t.grid.N;
 
   if (warp < COMPUTE_WARP) {
@@ -705,13 +757,13 @@ attn_fwd_narrow_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             break;
           }
           mbar_expect_tx(k_full(s), BOX);
-          tma_load_4d(base + L::K_AT + s * BOX, &map_k, k_full(s), 0, w.lo + j * TILE, hk, w.b);
+          tma_load_4d(base + L::K_AT + s * BOX, &map_k, k_full(s), 0, w.lo + (j0 + j) * TILE, hk, w.b);
           if (!mbar_wait(v_empty(s), ph ^ 1u)) {
             atomicExch(p.t.err, 80);
             break;
           }
           mbar_expect_tx(v_full(s), BOX);
-          tma_load_4d(base + L::V_AT + s * BOX, &map_v, v_full(s), 0, w.lo + j * TILE, hk, w.b);
+          tma_load_4d(base + L::V_AT + s * BOX, &map_v, v_full(s), 0, w.lo + (j0 + j) * TILE, hk, w.b);
           if (++s == L::STAGES) {
             s = 0;
             ph ^= 1u;
@@ -802,7 +854,7 @@ attn_fwd_narrow_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(s_read(t));
-      const int k0 = j * TILE;
+      const int k0 = (j0 + j) * TILE;
       if (k0 + TILE > w.len || (causal && k0 + TILE - 1 > w.r0 + t * TILE)) hide_scores(v, (causal ? min(w.len, w.r0 + row + 1) : w.len) - k0);
       const float top = max_of<true>(v) * scale;
       if (__any_sync(0xffffffffu, r.grows(top))) {
@@ -832,8 +884,9 @@ attn_fwd_narrow_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     if (nt > 0 && ok) {
       tc_fence_after();
       const float total = r.total();
-      store_output(o_at, p.t.D, 1.f / total, to, p.o_rest ? p.o_rest + (to - p.o) : nullptr, here);
-      if (here && p.lse) p.lse[(static_cast<long long>(w.b) * p.t.grid.H + w.h) * p.t.grid.N + w.lo + w.r0 + row] = r.m + __log2f(total);
+      if (share.part >= 0) share.store(p.split, row, p.t.D, o_at, r.m, total, here);
+      else store_output(o_at, p.t.D, 1.f / total, to, p.o_rest ? p.o_rest + (to - p.o) : nullptr, here);
+      if (here && p.lse && share.part < 0) p.lse[(static_cast<long long>(w.b) * p.t.grid.H + w.h) * p.t.grid.N + w.lo + w.r0 + row] = r.m + __log2f(total);
     } else if (here && w.padding) {
       zero_row(p.t.D, to);
     }
@@ -845,6 +898,47 @@ attn_fwd_narrow_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     tc_fence_after();
     tmem_free<512>(tmem);
   }
+}
+
+// Joins the parts of the pairs of tiles that were split: a warp a row
+__global__ void __launch_bounds__(256) attn_join_kernel(FwdParams p) {
+  const Split& s = p.split;
+  const float* parts_o = s.o;
+  const float2* parts_ml = s.ml;
+  chain_begin(true, parts_o, parts_ml);
+  const int lane = threadIdx.x & 31;
+  const uint32_t at = blockIdx.x * 8 + (threadIdx.x >> 5), pair = at / (2 * TILE);
+  const int row = static_cast<int>(at % (2 * TILE));
+  Work w;
+  if (!find_work(p.t.grid, nullptr, s.whole + pair, w) || w.r0 + row >= w.len) return;
+  const long long first = static_cast<long long>(pair) * s.parts * (2 * TILE) + row;
+  float top = -INFINITY, total = 0.f;
+  for (int k = 0; k < s.parts; ++k) top = fmaxf(top, __ldg(&parts_ml[first + k * 2 * TILE].x));
+  if (top == -INFINITY) top = 0.f;
+  const int c = lane * 4;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int k = 0; k < s.parts; ++k) {
+    const long long from = first + k * 2 * TILE;
+    const float2 ml = __ldg(parts_ml + from);
+    const float f = ex2(ml.x - top);
+    total = fmaf(ml.y, f, total);
+    if (c < p.t.D) {
+      const float4 v = __ldg(reinterpret_cast<const float4*>(parts_o + from * p.t.D + c));
+      o = make_float4(fmaf(v.x, f, o.x), fmaf(v.y, f, o.y), fmaf(v.z, f, o.z), fmaf(v.w, f, o.w));
+    }
+  }
+  const long long token = static_cast<long long>(w.b) * p.t.grid.N + w.r0 + row, to = (token * p.t.grid.H + w.h) * p.t.D + c;
+  if (c < p.t.D) {
+    const float f = 1.f / total;
+    o = make_float4(o.x * f, o.y * f, o.z * f, o.w * f);
+    const uint2 h = make_uint2(pack_bf16(o.x, o.y), pack_bf16(o.z, o.w));
+    *reinterpret_cast<uint2*>(p.o + to) = h;
+    if (p.o_rest)
+      *reinterpret_cast<uint2*>(p.o_rest + to) =
+          make_uint2(pack_bf16(o.x - __uint_as_float(h.x << 16), o.y - __uint_as_float(h.x & 0xffff0000u)),
+                     pack_bf16(o.z - __uint_as_float(h.y << 16), o.w - __uint_as_float(h.y & 0xffff0000u)));
+  }
+  if (lane == 0 && p.lse) p.lse[(static_cast<long long>(w.b) * p.t.grid.H + w.h) * p.t.grid.N + w.r0 + row] = top + __log2f(total);
 }
 
 // ------------------------------------------------------------------------------------------ backward
@@ -1495,7 +1589,8 @@ cudaError_t launch(void (*kernel)(Params...), std::atomic<uint64_t>& devices, in
                    const CUtensorMap& v, const FwdParams& p, cudaStream_t s) {
   const cudaError_t e = allow_shared_memory(devices, reinterpret_cast<const void*>(kernel), smem);
   if (e != cudaSuccess) return e;
-  return launch_chained(kernel, dim3(static_cast<unsigned>(blocks_of(p.t.grid))), dim3(threads), smem, s, 1, true, q, k, v, p);
+  const long long pairs = blocks_of(p.t.grid), blocks = p.split.parts > 0 ? p.split.whole + (pairs - p.split.whole) * p.split.parts : pairs;
+  return launch_chained(kernel, dim3(static_cast<unsigned>(blocks)), dim3(threads), smem, s, 1, true, q, k, v, p);
 }
 // One query tile to a CTA, two CTAs to an SM, where sequences are short and CTAs of two tiles would take the SMs more than once.  us, two tiles / one, heads of
 // 64 (batch x tokens x heads): 64 x 128 x 8 19.3 / 11.6, 64 x 200 x 8 32.7 / 27.9, 32 x 384 x 8 33.7 / 27.1, 16 x 512 x 8 23.4 / 22.5, 8 x 768 x 8 28.9 / 26.1, 8 x
@@ -1505,6 +1600,25 @@ cudaError_t launch(void (*kernel)(Params...), std::atomic<uint64_t>& devices, in
 bool one_tile_pays(const AttnShape& p) {
   const int mean = p.offsets ? p.N / std::max(1, p.sequences) : p.N;
   return mean <= (p.D <= 64 ? 768 : 448) && blocks_of(slots_of(p, p.H, 2 * TILE, 1)) > sm_count();
+}
+// CTAs of one length that would be a last wave of their own, or that are fewer than the SMs, are split over the keys so that they fill them, where that saves more
+// than joining them costs: tiles of keys, of some 0.7 us.  us, whole / split: 16200 tokens, 8 heads of 48 720 / 641, 12 of 64 1086 / 955, 8 of 128 943 / 847; 5000
+// tokens, 8 heads of 64 124 / 83; 2048 tokens 30.2 / 26.4; 1536 23.8 / 20.2.
+constexpr int MIN_SAVED = 8;
+Split split_of(const AttnShape& p) {
+  Split s{0, 0, nullptr, nullptr};
+  if (p.offsets || p.causal || one_tile_pays(p)) return s;
+  const long long pairs = blocks_of(slots_of(p, p.H, 2 * TILE, 1)), sms = sm_count(), last = pairs % sms;
+  if (last == 0) return s;
+  const int tiles = (p.N + TILE - 1) / TILE;
+  const long long parts = std::min<long long>(sms / last, std::max(1, tiles / 4));
+  if (parts < 2 || tiles - tiles / parts < MIN_SAVED) return s;
+  s.whole = static_cast<uint32_t>(pairs - last);
+  s.parts = static_cast<int>(parts);
+  return s;
+}
+long long split_rows(const AttnShape& p, const Split& s) {
+  return s.parts > 0 ? (blocks_of(slots_of(p, p.H, 2 * TILE, 1)) - s.whole) * s.parts * (2 * TILE) : 0;
 }
 cudaError_t launch_fwd(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const FwdParams& p, bool one_tile, cudaStream_t s) {
   static std::atomic<uint64_t> devices[4];
@@ -1532,9 +1646,15 @@ cudaError_t launch_dkv(const CUtensorMap& q, const CUtensorMap& k, const CUtenso
 
 }  // namespace
 
+long long attention_scratch(const AttnShape& p) {
+  if (!shape_ok(p)) return 0;
+  return split_rows(p, split_of(p)) * (p.D + 2);
+}
+
 cudaError_t attention_fwd(const AttnShape& p, const AttnTensor& q, const AttnTensor& k, const AttnTensor& v, __nv_bfloat16* o, __nv_bfloat16* o_rest,
-                          float* lse, int* err, cudaStream_t s) {
-  if (!shape_ok(p) || ((reinterpret_cast<uintptr_t>(o) | reinterpret_cast<uintptr_t>(o_rest)) & 15) || (o_rest != nullptr) != (lse != nullptr))
+                          float* lse, float* scratch, int* launches, int* err, cudaStream_t s) {
+  if (!shape_ok(p) || ((reinterpret_cast<uintptr_t>(o) | reinterpret_cast<uintptr_t>(o_rest) | reinterpret_cast<uintptr_t>(scratch)) & 15) ||
+      (o_rest != nullptr) != (lse != nullptr))
     return cudaErrorInvalidValue;
   bind_context(s);
   CUtensorMap mq, mk_, mv;
@@ -1542,10 +1662,18 @@ cudaError_t attention_fwd(const AttnShape& p, const AttnTensor& q, const AttnTen
   FwdParams f;
   const bool one_tile = one_tile_pays(p);
   f.t = tile_params(p, slots_of(p, p.H, one_tile ? TILE : 2 * TILE, 1), err);
+  f.split = scratch ? split_of(p) : Split{0, 0, nullptr, nullptr};
+  f.split.o = scratch;
+  const long long rows = split_rows(p, f.split);
+  f.split.ml = reinterpret_cast<float2*>(scratch + rows * p.D);
   f.o = o;
   f.o_rest = o_rest;
   f.lse = lse;
-  return launch_fwd(mq, mk_, mv, f, one_tile, s);
+  *launches = 1;
+  const cudaError_t e = launch_fwd(mq, mk_, mv, f, one_tile, s);
+  if (e != cudaSuccess || f.split.parts == 0) return e;
+  ++*launches;
+  return launch_chained(attn_join_kernel, dim3(static_cast<unsigned>(rows / f.split.parts / 8)), dim3(256), 0, s, 1, true, f);
 }
 
 cudaError_t attention_bwd(const AttnShape& p, const AttnTensor& q, const AttnTensor& k, const AttnTensor& v, const __nv_bfloat16* o,

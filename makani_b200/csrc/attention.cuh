@@ -25,9 +25,11 @@ struct AttnShape {
 };
 
 // o [B, N, H, D] dense.  For a backward pass (both or none): lse [B, H, N], log2 of the sum of exponentials of every row, and o_rest, like o, what the
-// rounding of o has left out, rounded in its turn.
+// rounding of o has left out, rounded in its turn.  `scratch`: attention_scratch() floats (none: nothing is split over the keys), 16-byte aligned.
+// `launches` counts.
+long long attention_scratch(const AttnShape& p);
 cudaError_t attention_fwd(const AttnShape& p, const AttnTensor& q, const AttnTensor& k, const AttnTensor& v, __nv_bfloat16* o, __nv_bfloat16* o_rest,
-                          float* lse, int* err, cudaStream_t s);
+                          float* lse, float* scratch, int* launches, int* err, cudaStream_t s);
 // dq, dk, dv from o, o_rest and d_o (dense, like o); delta [B, H, N]: room for the row sums of o d_o.  Two launches, no atomics.
 cudaError_t attention_bwd(const AttnShape& p, const AttnTensor& q, const AttnTensor& k, const AttnTensor& v, const __nv_bfloat16* o,
                           const __nv_bfloat16* o_rest, const __nv_bfloat16* d_o, const float* lse, float* delta, const AttnTensor& dq,

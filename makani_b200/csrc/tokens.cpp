@@ -285,10 +285,13 @@ std::tuple<Tensor, Tensor, Tensor> attention_forward(const Tensor& q_in, const T
   }
   if (o.numel() == 0) return {o, rest, lse};
   const Tensor q = readable(q_in), k = readable(k_in), v = readable(v_in);
-  ++mkh::launches();
-  mkh::check(mk::attention_fwd(p, view_of(q), view_of(k), view_of(v), bf(o), ptr_or_null<__nv_bfloat16>(rest), ptr_or_null<float>(lse), mkh::error_word(q),
-                               mkh::stream()),
+  Tensor scratch;
+  if (const int64_t floats = mk::attention_scratch(p)) scratch = at::empty({floats}, q.options().dtype(at::kFloat));
+  int launches = 0;
+  mkh::check(mk::attention_fwd(p, view_of(q), view_of(k), view_of(v), bf(o), ptr_or_null<__nv_bfloat16>(rest), ptr_or_null<float>(lse),
+                               ptr_or_null<float>(scratch), &launches, mkh::error_word(q), mkh::stream()),
              "attention_fwd");
+  mkh::launches() += launches;
   return {o, rest, lse};
 }
 

@@ -158,6 +158,19 @@ def test_lengths_heads_and_widths(gen, B, N, H, Hk, D, causal):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("B,N,H,Hk,D", [(1, 2500, 1, 1, 128), (2, 3001, 3, 1, 72), (1, 4096, 2, 2, 64), (1, 2305, 5, 5, 8), (3, 1921, 2, 2, 48)])
+def test_few_rows_and_long_keys(gen, B, N, H, Hk, D):
+    """What does not fill the SMs is split over the keys and joined."""
+    _check_batch(gen, B, N, H, Hk, D, False)
+    q, k, v, _ = _inputs(gen, B, N, H=H, Hk=Hk, D=D)
+    k = (k.float() * torch.linspace(0.1, 12, N, device="cuda")[None, :, None, None]).bfloat16()      # parts of very different maxima
+    with torch.no_grad():
+        o = attn.attention(q, k, v)
+    want, off = _oracle(q[0], k[0], v[0], torch.zeros_like(q[0]), False, D ** -0.5, [(0, N)])
+    _close(o[0], want["o"], off["o"], "o")
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("D", [1, 5, 20, 65, 127])
 def test_widths_that_are_padded(gen, D):
     _check_batch(gen, 1, 200, 2, 1, D, True)
