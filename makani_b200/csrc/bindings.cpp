@@ -3,6 +3,7 @@
 #include <algorithm>
 #include <cstring>
 #include <map>
+#include <mutex>
 
 #include "host.h"
 
@@ -25,7 +26,11 @@ inline void check_cuda(cudaError_t e, const char* what) {
 
 inline cudaStream_t cur_stream() { return at::cuda::getCurrentCUDAStream().stream(); }
 
-// one error word per device, set by kernels whose bounded waits expire
+// one error word per device, set by kernels whose bounded waits expire (asked for by the threads of autograd too, without Python's lock)
+std::mutex& err_mutex() {
+  static std::mutex m;
+  return m;
+}
 std::map<int, Tensor>& err_flags() {
   static std::map<int, Tensor> m;
   return m;
@@ -33,6 +38,7 @@ std::map<int, Tensor>& err_flags() {
 
 Tensor err_flag_for(const Tensor& t) {
   const int dev = t.get_device();
+  const std::lock_guard<std::mutex> lock(err_mutex());
   auto& m = err_flags();
   auto it = m.find(dev);
   if (it == m.end()) {
@@ -42,17 +48,22 @@ Tensor err_flag_for(const Tensor& t) {
   return it->second;
 }
 
-int64_t read_error_flag(int64_t device) {
+// (undefined: no kernel has asked for it)
+Tensor err_flag_of(int64_t device) {
+  const std::lock_guard<std::mutex> lock(err_mutex());
   auto& m = err_flags();
   auto it = m.find(static_cast<int>(device));
-  if (it == m.end()) return 0;
-  return it->second.cpu().data_ptr<int>()[0];
+  return it == m.end() ? Tensor() : it->second;
+}
+
+int64_t read_error_flag(int64_t device) {
+  const Tensor f = err_flag_of(device);
+  return f.defined() ? f.cpu().data_ptr<int>()[0] : 0;
 }
 
 void clear_error_flag(int64_t device) {
-  auto& m = err_flags();
-  auto it = m.find(static_cast<int>(device));
-  if (it != m.end()) it->second.zero_();
+  Tensor f = err_flag_of(device);
+  if (f.defined()) f.zero_();
 }
 
 // (current stream, what it is capturing) of a device: 0 nothing, -1 unknown, else the number of the capture, unique in the process
