@@ -4,11 +4,12 @@
 //   backward   P = exp(S - L), dV = P^T dO, dS = P (dO V^T - delta), dQ = scale dS K, dK = scale dS^T Q,  delta = sum_d O dO
 //
 // Exponentials are powers of two of (scale log2 e) S, one special-function instruction each.  Products take bf16 operands and add in fp32 (tensor
-// memory); P and dS are rounded to bf16 as operands of the second products (half a step 2^-9 of each weight, of the size of the rounding of the
+// memory); P and dS are rounded to bf16 as operands of the second products (half a step, 2^-8 of each weight at most, as the rounding of the
 // outputs), sums, maxima and L stay in fp32.
 //
-// A CTA has an SM to itself.  Warps: 0 loads tiles (TMA), 1 issues the products, 2 clears rows that belong to another sequence, 4 - 11 compute on
-// rows in tensor memory, a thread a row.  Every wait is bounded; on expiry the kernel records a code in *err and drains.
+// Warps: 0 loads tiles (TMA), 1 (and 3, narrow heads forward) issues products, 2 (and 3, dK and dV) loads statistics and clears rows that belong to another
+// sequence, those from 4 on compute on rows in tensor memory, a thread a row or a part of one.  Every wait is bounded; on expiry the kernel records a
+// code in *err and drains.
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -148,25 +149,26 @@ __device__ __forceinline__ void ex2_pair(int i, float& a, float& b) {
 // with, 266 without; 16200 tokens, 8 heads of 48: 723 with, 728 without)
 template <bool THREE, int N>
 __device__ __forceinline__ float max_of(const uint32_t (&v)[N]) {
-  if (!THREE) {
+  if constexpr (!THREE) {
     float m[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) m[i] = __uint_as_float(v[i]);
 #pragma unroll
     for (int c = 4; c < N; ++c) m[c & 3] = fmaxf(m[c & 3], __uint_as_float(v[c]));
     return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+  } else {
+    float m[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m[i] = __uint_as_float(v[i]);
+#pragma unroll
+    for (int c = 8; c + 15 < N; c += 16)
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        asm("max.f32 %0, %0, %1, %2;" : "+f"(m[i]) : "f"(__uint_as_float(v[c + 2 * i])), "f"(__uint_as_float(v[c + 2 * i + 1])));
+#pragma unroll
+    for (int c = 8 + (N - 8) / 16 * 16; c < N; ++c) m[c & 7] = fmaxf(m[c & 7], __uint_as_float(v[c]));
+    return fmaxf(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), fmaxf(fmaxf(m[4], m[5]), fmaxf(m[6], m[7])));
   }
-  float m[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) m[i] = __uint_as_float(v[i]);
-#pragma unroll
-  for (int c = 8; c + 15 < N; c += 16)
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      asm("max.f32 %0, %0, %1, %2;" : "+f"(m[i]) : "f"(__uint_as_float(v[c + 2 * i])), "f"(__uint_as_float(v[c + 2 * i + 1])));
-#pragma unroll
-  for (int c = 8 + (N - 8) / 16 * 16; c < N; ++c) m[c & 7] = fmaxf(m[c & 7], __uint_as_float(v[c]));
-  return fmaxf(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), fmaxf(fmaxf(m[4], m[5]), fmaxf(m[6], m[7])));
 }
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   uint32_t r;
