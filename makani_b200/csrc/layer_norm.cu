@@ -97,27 +97,49 @@ struct Group {
     index = threadIdx.x / size;
     per_block = blockDim.x / size;
   }
-  // Sums of N values over the group, in all of its threads.  `sh`: N * MOST_WARPS floats for every group of the block, another set for each of the sums
-  // that follow one another between two uses of the same.
+  // Sums of N values (a power of two) over the group, in all of its threads.  While there are several, a step of the butterfly gives half of them away
+  // instead of adding up all: 9 exchanges for eight values in a warp where 40 were.  `sh`: N * MOST_WARPS floats, 16-byte aligned, another set for each of
+  // the sums that follow one another between two uses of the same.
   template <int N>
   __device__ __forceinline__ void sum(float (&a)[N], float* sh) const {
+    const int l = threadIdx.x & 31;
+    int o = SUB / 2;
 #pragma unroll
-    for (int o = SUB / 2; o > 0; o >>= 1)
+    for (int n = N; n > 1; n >>= 1, o >>= 1) {
+      const bool upper = (l & o) != 0;
 #pragma unroll
-      for (int i = 0; i < N; ++i) a[i] += __shfl_xor_sync(0xffffffffu, a[i], o);
-    if (SUB < 32 || warps == 1) return;
-    float* const mine = sh + index * warps * N;
-    const int warp = lane >> 5;
-    if ((threadIdx.x & 31) == 0) {
-#pragma unroll
-      for (int i = 0; i < N; ++i) mine[warp * N + i] = a[i];
+      for (int i = 0; i < n / 2; ++i) {
+        const float mine = upper ? a[i + n / 2] : a[i], other = upper ? a[i] : a[i + n / 2];
+        a[i] = mine + __shfl_xor_sync(0xffffffffu, other, o);
+      }
     }
+#pragma unroll
+    for (; o > 0; o >>= 1) a[0] += __shfl_xor_sync(0xffffffffu, a[0], o);
+    // value i is now with the lanes whose upper bits (below SUB) are i's
+    constexpr int EACH = SUB / N;
+    const float part = a[0];
+    if (SUB < 32 || warps == 1) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) a[i] = __shfl_sync(0xffffffffu, part, (l & ~(SUB - 1)) + i * EACH);
+      return;
+    }
+    float* const all = sh + index * warps * N;
+    if (l % EACH == 0) all[(lane >> 5) * N + l / EACH] = part;
     asm volatile("bar.sync %0, %1;" ::"r"(1 + index), "r"(size) : "memory");
 #pragma unroll
     for (int i = 0; i < N; ++i) a[i] = 0.f;
-    for (int k = 0; k < warps; ++k)
+    for (int k = 0; k < warps; ++k) {
+      if constexpr (N % 4 == 0) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) a[i] += mine[k * N + i];
+        for (int i = 0; i < N; i += 4) {
+          const float4 v = *reinterpret_cast<const float4*>(all + k * N + i);
+          a[i] += v.x, a[i + 1] += v.y, a[i + 2] += v.z, a[i + 3] += v.w;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) a[i] += all[k * N + i];
+      }
+    }
   }
 };
 
@@ -209,7 +231,7 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) ln_fwd_kernel(LnForward p, in
   constexpr bool ADD = !std::is_void<TR>::value;
   using Res = typename std::conditional<ADD, TR, TI>::type;
   constexpr int P = Cols<VEC, NV>::PAIRS;
-  __shared__ float sh[3 * ROWS * MOST_WARPS];
+  __shared__ __align__(16) float sh[3 * ROWS * MOST_WARPS];
   const TI* x = static_cast<const TI*>(p.x);
   const Res* res = static_cast<const Res*>(p.r);
   const float *w = p.w, *b = p.b;
@@ -315,7 +337,7 @@ template <typename TI, typename TO, bool ADD, int VEC, int NV, int SUB, int ROWS
 __global__ void __launch_bounds__(THREADS, BLOCKS) ln_bwd_kernel(LnBackward p, int warps) {
   constexpr int P = Cols<VEC, NV>::PAIRS;
   extern __shared__ float cols[];            // [2][C]: the block's sums
-  __shared__ float sh[2][2 * ROWS * MOST_WARPS];
+  __shared__ __align__(16) float sh[2][2 * ROWS * MOST_WARPS];
   const TI *x = static_cast<const TI*>(p.x), *ds = static_cast<const TI*>(p.ds);
   const TO* dy = static_cast<const TO*>(p.dy);
   const float* w = p.w;
@@ -457,9 +479,10 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) ln_bwd_kernel(LnBackward p, i
 }
 
 // How a row is spread: warps of a group (0: a part of a warp), threads of a block, rows that it takes at a time; blocks to an SM, rows of a group.  What
-// carries it is bytes on their way.  us by (blocks, rows): forward, 74160 x 1024 bf16, (4, 1) 91, (3, 2) 75, (2, 4) 70 (DRAM 46); 129600 x 48 8.5, 7.6, 8.1;
-// 16471 x 387 fp32 22.5, 19.4, 18.0.  Forward and backward of the first (3, 1) 195, (2, 2) 163, (2, 3) 203 (DRAM 116).  (A warp to a row, its weights
-// read again for every row: 71 and 212; 16471 x 387 74.)  Behind a sum one row at a time: 16200 x 768 (4, 1) 21.4, (3, 2) 25.2 (DRAM 15).
+// carries it is that several rows share shuffles and barriers.  us by (blocks, rows): forward, 74160 x 1024 bf16, (3, 2) 71, (2, 4) 63 (DRAM 46; every value through
+// all steps of the butterfly 70); 129600 x 48 7.7, 8.1; 16471 x 387 fp32 18.4, 16.1.  Forward and backward of the first (3, 1) 174, (2, 2) 157, (1, 4) 165 (DRAM
+// 116).  (A warp to a row, its weights read again for every row: 71 and 212; 16471 x 387 74.  Rows through a ring of cp.async, (2, 4) 77 and (4, 2) 86: more bytes on
+// their way are not what is missing.)  Behind a sum one row at a time: 16200 x 768 (4, 1) 21.0, (3, 2) 23.3 (DRAM 15).
 constexpr int FWD_BLOCKS = 2, BWD_BLOCKS = 2;
 constexpr int WIDE = 2048, RAGGED = 1024;      // most channels of eight warps with one vector, or four single values, a thread
 struct Spread {
