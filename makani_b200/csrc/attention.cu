@@ -299,6 +299,44 @@ __device__ __forceinline__ void store_output(uint32_t taddr, int D, float f, __n
     }
   }
 }
+// CTAs that are split over what they go along: those from `whole` on, into `parts`
+struct Parts {
+  uint32_t whole;
+  int parts;               // 0: none is split
+};
+// What this CTA has of it: its unit, its part (-1: all of it), tiles in front of its own and number of its own.  Without SPLIT it has all of its unit: the
+// kernels of the gradients are built both ways, since the part that may begin in the middle costs a whole one 3 % (dQ) and 1 % (dK, dV).
+template <bool SPLIT>
+struct ShareOf {
+  uint32_t unit;
+  int part, first, n;
+  __device__ __forceinline__ explicit ShareOf(const Parts& s) : unit(blockIdx.x), part(-1) {
+    if (SPLIT && s.parts > 0 && blockIdx.x >= s.whole) {
+      unit = s.whole + (blockIdx.x - s.whole) / s.parts;
+      part = static_cast<int>((blockIdx.x - s.whole) % s.parts);
+    }
+  }
+  __device__ __forceinline__ void along(const Parts& s, int tiles) {
+    first = !SPLIT || part < 0 ? 0 : static_cast<int>(static_cast<long long>(tiles) * part / s.parts);
+    n = (!SPLIT || part < 0 ? tiles : static_cast<int>(static_cast<long long>(tiles) * (part + 1) / s.parts)) - first;
+  }
+  // row of a buffer [unit - whole][part][rows]
+  __device__ __forceinline__ long long row(const Parts& s, int rows, int r) const {
+    return (static_cast<long long>(unit - s.whole) * s.parts + part) * rows + r;
+  }
+};
+using Share = ShareOf<true>;
+// An accumulator's row as it is, the first D columns, from `first` on in steps of `step`
+__device__ __forceinline__ void store_part(uint32_t taddr, int D, float* to, bool here, int first = 0, int step = 8) {
+  for (int c = first; c < D; c += step) {
+    uint32_t v[8];
+    tmem_ld8(taddr + c, v);
+    if (here) {
+      reinterpret_cast<uint4*>(to + c)[0] = make_uint4(v[0], v[1], v[2], v[3]);
+      reinterpret_cast<uint4*>(to + c)[1] = make_uint4(v[4], v[5], v[6], v[7]);
+    }
+  }
+}
 __device__ __forceinline__ void zero_row(int D, __nv_bfloat16* to) {
   for (int c = 0; c < D; c += 8) *reinterpret_cast<uint4*>(to + c) = make_uint4(0, 0, 0, 0);
 }
@@ -402,38 +440,9 @@ struct Fwd {
 constexpr uint32_t S_COLS = 128;
 // Of the pairs of query tiles, those from `whole` on are split over the keys into `parts` CTAs each, which leave O (not divided) and maximum and sum of every
 // row for the kernel that joins them
-struct Split {
-  uint32_t whole;
-  int parts;               // 0: none is split
+struct Split : Parts {
   float* o;                // [pair - whole][part][2 TILE][D]
   float2* ml;              // [pair - whole][part][2 TILE]
-};
-// What a CTA has of it: its pair of tiles, its part (-1: all keys), tiles of keys in front of its own and number of its own
-struct Share {
-  uint32_t pair;
-  int part, first, n;
-  __device__ __forceinline__ explicit Share(const Split& s) : pair(blockIdx.x), part(-1) {
-    if (s.parts > 0 && blockIdx.x >= s.whole) {
-      pair = s.whole + (blockIdx.x - s.whole) / s.parts;
-      part = static_cast<int>((blockIdx.x - s.whole) % s.parts);
-    }
-  }
-  __device__ __forceinline__ void keys(const Split& s, int tiles) {
-    first = part < 0 ? 0 : tiles * part / s.parts;
-    n = (part < 0 ? tiles : tiles * (part + 1) / s.parts) - first;
-  }
-  __device__ __forceinline__ void store(const Split& s, int row, int D, uint32_t o_at, float m, float total, bool here) const {
-    const long long at = (static_cast<long long>(pair - s.whole) * s.parts + part) * (2 * TILE) + row;
-    for (int c = 0; c < D; c += 8) {
-      uint32_t v[8];
-      tmem_ld8(o_at + c, v);
-      if (here) {
-        reinterpret_cast<uint4*>(s.o + at * D + c)[0] = make_uint4(v[0], v[1], v[2], v[3]);
-        reinterpret_cast<uint4*>(s.o + at * D + c)[1] = make_uint4(v[4], v[5], v[6], v[7]);
-      }
-    }
-    if (here) s.ml[at] = make_float2(m, total);
-  }
 };
 
 struct FwdParams {
@@ -492,7 +501,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
 
   Work w;
   Share share(p.split);
-  const bool any = find_work(p.t.grid, offsets, share.pair, w);
+  const bool any = find_work(p.t.grid, offsets, share.unit, w);
   const int rows = any ? min(w.len - w.r0, QT * TILE) : 0;
   const bool causal = p.t.causal != 0;
   auto tiles_of = [&](int t) {      // of keys, that the queries of tile t see
@@ -501,7 +510,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     return last / TILE + 1;
   };
   int n0 = tiles_of(0), n1 = tiles_of(1);
-  share.keys(p.split, max(n0, n1));
+  share.along(p.split, max(n0, n1));
   const int n = share.n, j0 = share.first;
   if (share.part >= 0) {      // (not causal: both see the same keys)
     n0 = n0 > 0 ? n : 0;
@@ -648,10 +657,15 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     if (nt > 0 && ok) {
       tc_fence_after();
       const float total = r.total();
-      if (share.part >= 0) share.store(p.split, row, p.t.D, o_at, r.m, total, here);
-      else store_output(o_at, p.t.D, 1.f / total, to, p.o_rest ? p.o_rest + (to - p.o) : nullptr, here);
-      if (here && p.lse && share.part < 0)
-        p.lse[(static_cast<long long>(w.b) * p.t.grid.H + w.h) * p.t.grid.N + w.lo + w.r0 + row] = r.m + __log2f(total);
+      if (share.part >= 0) {
+        const long long at = share.row(p.split, 2 * TILE, row);
+        store_part(o_at, p.t.D, p.split.o + at * p.t.D, here);
+        if (here) p.split.ml[at] = make_float2(r.m, total);
+      } else {
+        store_output(o_at, p.t.D, 1.f / total, to, p.o_rest ? p.o_rest + (to - p.o) : nullptr, here);
+        if (here && p.lse)
+          p.lse[(static_cast<long long>(w.b) * p.t.grid.H + w.h) * p.t.grid.N + w.lo + w.r0 + row] = r.m + __log2f(total);
+      }
     } else if (here && w.padding) {
       zero_row(p.t.D, to);
     }
@@ -725,7 +739,7 @@ attn_fwd_narrow_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
 
   Work w;
   Share share(p.split);
-  const bool any = find_work(p.t.grid, offsets, share.pair, w);
+  const bool any = find_work(p.t.grid, offsets, share.unit, w);
   const int rows = any ? min(w.len - w.r0, 2 * TILE) : 0;
   const bool causal = p.t.causal != 0;
   auto tiles_of = [&](int t) {      // of keys, that the queries of tile t see
@@ -734,7 +748,7 @@ attn_fwd_narrow_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     return last / TILE + 1;
   };
   int n0 = tiles_of(0), n1 = tiles_of(1);
-  share.keys(p.split, max(n0, n1));
+  share.along(p.split, max(n0, n1));
   const int n = share.n, j0 = share.first;
   if (share.part >= 0) {      // (not causal: both see the same keys)
     n0 = n0 > 0 ? n : 0;
@@ -886,9 +900,14 @@ attn_fwd_narrow_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     if (nt > 0 && ok) {
       tc_fence_after();
       const float total = r.total();
-      if (share.part >= 0) share.store(p.split, row, p.t.D, o_at, r.m, total, here);
-      else store_output(o_at, p.t.D, 1.f / total, to, p.o_rest ? p.o_rest + (to - p.o) : nullptr, here);
-      if (here && p.lse && share.part < 0) p.lse[(static_cast<long long>(w.b) * p.t.grid.H + w.h) * p.t.grid.N + w.lo + w.r0 + row] = r.m + __log2f(total);
+      if (share.part >= 0) {
+        const long long at = share.row(p.split, 2 * TILE, row);
+        store_part(o_at, p.t.D, p.split.o + at * p.t.D, here);
+        if (here) p.split.ml[at] = make_float2(r.m, total);
+      } else {
+        store_output(o_at, p.t.D, 1.f / total, to, p.o_rest ? p.o_rest + (to - p.o) : nullptr, here);
+        if (here && p.lse) p.lse[(static_cast<long long>(w.b) * p.t.grid.H + w.h) * p.t.grid.N + w.lo + w.r0 + row] = r.m + __log2f(total);
+      }
     } else if (here && w.padding) {
       zero_row(p.t.D, to);
     }
@@ -1004,13 +1023,15 @@ constexpr uint32_t DQ_DP = 256, DQ_ACC = 384;
 
 struct DqParams {
   TileParams t;
+  Parts split;             // over the keys
+  float* sums;             // [unit - whole][part][TILE][D]
   const __nv_bfloat16 *o, *o_rest, *d_o;
   const float* lse;
   float* delta;
   AttnTensor dq;
 };
 
-template <int DB>
+template <int DB, bool SPLIT>
 __global__ void __launch_bounds__(BWD_THREADS, 1)
 attn_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                const __grid_constant__ CUtensorMap map_do, const DqParams p) {
@@ -1053,11 +1074,13 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
   const uint32_t tmem = *tmem_slot;
 
   Work w;
-  const bool any = find_work(p.t.grid, offsets, blockIdx.x, w);
+  ShareOf<SPLIT> share(p.split);
+  const bool any = find_work(p.t.grid, offsets, share.unit, w);
   const int rows = any ? min(w.len - w.r0, TILE) : 0;
   const bool causal = p.t.causal != 0;
-  const int n = rows == 0 || w.padding ? 0 : (causal ? w.r0 + rows - 1 : w.len - 1) / TILE + 1;
-  const int tail = w.len - (n - 1) * TILE;
+  share.along(p.split, rows == 0 || w.padding ? 0 : (causal ? w.r0 + rows - 1 : w.len - 1) / TILE + 1);
+  const int n = share.n, j0 = share.first;
+  const int tail = w.len - (j0 + n - 1) * TILE;
   const bool fix = n > 0 && tail < TILE && w.lo + w.len < p.t.grid.N;
 
   if (warp < COMPUTE_WARP) {
@@ -1079,13 +1102,13 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
             break;
           }
           mbar_expect_tx(k_full(s), L::TILE_BYTES);
-          for (int b = 0; b < DB; ++b) tma_load_4d(base + L::K_AT + s * L::TILE_BYTES + b * BOX, &map_k, k_full(s), b * 64, w.lo + j * TILE, hk, w.b);
+          for (int b = 0; b < DB; ++b) tma_load_4d(base + L::K_AT + s * L::TILE_BYTES + b * BOX, &map_k, k_full(s), b * 64, w.lo + (j0 + j) * TILE, hk, w.b);
           if (!mbar_wait(v_empty(s), ph ^ 1u)) {
             atomicExch(p.t.err, 85);
             break;
           }
           mbar_expect_tx(v_full(s), L::TILE_BYTES);
-          for (int b = 0; b < DB; ++b) tma_load_4d(base + L::V_AT + s * L::TILE_BYTES + b * BOX, &map_v, v_full(s), b * 64, w.lo + j * TILE, hk, w.b);
+          for (int b = 0; b < DB; ++b) tma_load_4d(base + L::V_AT + s * L::TILE_BYTES + b * BOX, &map_v, v_full(s), b * 64, w.lo + (j0 + j) * TILE, hk, w.b);
           if (++s == L::STAGES) {
             s = 0;
             ph ^= 1u;
@@ -1195,7 +1218,7 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
       uint32_t v[BWD_COLS];
       const uint32_t s_at = tmem + lanes + (j & 1) * S_COLS + x * BWD_COLS, dp_at = tmem + lanes + DQ_DP + x * BWD_COLS;
       tmem_req32(s_at, v);
-      const int k0 = j * TILE + x * BWD_COLS;
+      const int k0 = (j0 + j) * TILE + x * BWD_COLS;
       const bool edge = k0 + BWD_COLS > w.len || (causal && k0 + BWD_COLS - 1 > w.r0);
       const int keys = (causal ? min(w.len, w.r0 + row + 1) : w.len) - k0;
       auto seen = [&](int c) { return c < keys; };
@@ -1220,7 +1243,8 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
     __nv_bfloat16* const to = p.dq.ptr + w.b * p.dq.batch + (w.lo + w.r0 + row) * p.dq.token + w.h * p.dq.head;
     if (n > 0 && ok) {
       tc_fence_after();
-      store_row(tmem + lanes + DQ_ACC, p.t.D, p.t.scale, to, here, x * 16, 64);
+      if (SPLIT && share.part >= 0) store_part(tmem + lanes + DQ_ACC, p.t.D, p.sums + share.row(p.split, TILE, row) * p.t.D, here, x * 8, 32);
+      else store_row(tmem + lanes + DQ_ACC, p.t.D, p.t.scale, to, here, x * 16, 64);
     } else if (here && w.padding && x == 0) {
       zero_row(p.t.D, to);
     }
@@ -1250,12 +1274,14 @@ struct Dkv {
 
 struct DkvParams {
   TileParams t;
+  Parts split;             // over the queries
+  float *dk_sums, *dv_sums;
   int heads_q;
   const float *lse, *delta;
   AttnTensor dk, dv;
 };
 
-template <int DB>
+template <int DB, bool SPLIT>
 __global__ void __launch_bounds__(BWD_THREADS, 1)
 attn_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                 const __grid_constant__ CUtensorMap map_do, const DkvParams p) {
@@ -1299,12 +1325,15 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
   const uint32_t tmem = *tmem_slot;
 
   Work w;
-  const bool any = find_work(p.t.grid, offsets, blockIdx.x, w);
+  ShareOf<SPLIT> share(p.split);
+  const bool any = find_work(p.t.grid, offsets, share.unit, w);
   const int rows = any ? min(w.len - w.r0, TILE) : 0;
   const bool causal = p.t.causal != 0;
   // tiles of queries, from the first that sees one of these keys, of one head after the other
   const int q_first = causal ? w.r0 / TILE : 0, q_tiles = rows == 0 || w.padding ? 0 : (w.len + TILE - 1) / TILE - q_first;
-  const int n = q_tiles * p.t.group, h0 = w.h * p.t.group;
+  share.along(p.split, q_tiles * p.t.group);
+  // first tile of queries and head of this CTA
+  const int n = share.n, t0 = q_tiles > 0 ? share.first % q_tiles : 0, g0 = q_tiles > 0 ? share.first / q_tiles : 0, h0 = w.h * p.t.group;
   const int tail = w.len - (q_first + q_tiles - 1) * TILE;
   const bool fix = n > 0 && tail < TILE && w.lo + w.len < p.t.grid.N;
 
@@ -1318,7 +1347,7 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
           tma_load_4d(base + b * BOX, &map_k, kv_full, b * 64, w.lo + w.r0, w.h, w.b);
           tma_load_4d(base + L::TILE_BYTES + b * BOX, &map_v, kv_full, b * 64, w.lo + w.r0, w.h, w.b);
         }
-        int s = 0, t = 0, g = 0;
+        int s = 0, t = t0, g = g0;
         uint32_t ph = 0;
         for (int j = 0; j < n; ++j) {
           if (!mbar_wait(empty(s), ph ^ 1u)) {
@@ -1369,7 +1398,7 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
           over_channels(tmem + L::DP_AT, v_lo, q_lo + DO);
           tc_commit(dp_full);
         }
-        int s = 0, t = 0, g = 0;
+        int s = 0, t = t0, g = g0;
         uint32_t ph = 0;
         for (int j = 0; j < n && ok; ++j) {
           const int sn = s + 1 == L::STAGES ? 0 : s + 1;
@@ -1429,7 +1458,7 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       }
     } else if (warp == 2) {
       // ---------------------------------------------------------------- L and delta of the queries
-      int s = 0, t = 0, g = 0;
+      int s = 0, t = t0, g = g0;
       uint32_t ph = 0;
       for (int j = 0; j < n; ++j) {
         if (!__all_sync(0xffffffffu, mbar_wait(empty(s), ph ^ 1u))) {
@@ -1472,7 +1501,7 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     const bool here = row < rows;
     const f32x2 scale2 = f2_pack(p.t.scale_log2, p.t.scale_log2);
     bool ok = true;
-    int s = 0, t = 0;
+    int s = 0, t = t0;
     uint32_t ph = 0;
     for (int j = 0; j < n; ++j) {
       const int buf = L::S_BUFS == 2 ? j & 1 : 0;
@@ -1527,7 +1556,10 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     __nv_bfloat16* const to = d.ptr + w.b * d.batch + (w.lo + w.r0 + row) * d.token + w.h * d.head;
     if (n > 0 && ok) {
       tc_fence_after();
-      store_row(tmem + lanes + (values ? L::DV_AT : L::DK_AT), p.t.D, values ? 1.f : p.t.scale, to, here, (x & 1) * 16, 32);
+      const uint32_t acc = tmem + lanes + (values ? L::DV_AT : L::DK_AT);
+      if (SPLIT && share.part >= 0)
+        store_part(acc, p.t.D, (values ? p.dv_sums : p.dk_sums) + share.row(p.split, TILE, row) * p.t.D, here, (x & 1) * 8, 16);
+      else store_row(acc, p.t.D, values ? 1.f : p.t.scale, to, here, (x & 1) * 16, 32);
     } else if (here && w.padding && (x & 1) == 0) {
       zero_row(p.t.D, to);
     }
@@ -1539,6 +1571,31 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     tc_fence_after();
     tmem_free<512>(tmem);
   }
+}
+
+// Adds up the parts of the units that were split, times a factor: a warp a row; blockIdx.y chooses among two tensors
+struct Sums {
+  const float* parts[2];
+  AttnTensor out[2];
+  float factor[2];
+};
+__global__ void __launch_bounds__(256) attn_sum_kernel(Slots grid, Parts split, Sums p, int D) {
+  const float* parts = p.parts[blockIdx.y];
+  chain_begin(true, parts);
+  const int lane = threadIdx.x & 31, c = lane * 4;
+  const uint32_t at = blockIdx.x * 8 + (threadIdx.x >> 5), unit = at / TILE;
+  const int row = static_cast<int>(at % TILE);
+  Work w;
+  if (!find_work(grid, nullptr, split.whole + unit, w) || w.r0 + row >= w.len || c >= D) return;
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int k = 0; k < split.parts; ++k) {
+    const float4 v = __ldcg(reinterpret_cast<const float4*>(parts + ((static_cast<long long>(unit) * split.parts + k) * TILE + row) * D + c));
+    a = make_float4(a.x + v.x, a.y + v.y, a.z + v.z, a.w + v.w);
+  }
+  const float f = p.factor[blockIdx.y];
+  const AttnTensor& o = p.out[blockIdx.y];
+  *reinterpret_cast<uint2*>(o.ptr + w.b * o.batch + (w.r0 + row) * o.token + w.h * o.head + c) =
+      make_uint2(pack_bf16(a.x * f, a.y * f), pack_bf16(a.z * f, a.w * f));
 }
 
 // ------------------------------------------------------------------------------------------ host
@@ -1586,14 +1643,6 @@ TileParams tile_params(const AttnShape& p, const Slots& g, int* err) {
   return t;
 }
 
-template <typename... Params>
-cudaError_t launch(void (*kernel)(Params...), std::atomic<uint64_t>& devices, int threads, int smem, const CUtensorMap& q, const CUtensorMap& k,
-                   const CUtensorMap& v, const FwdParams& p, cudaStream_t s) {
-  const cudaError_t e = allow_shared_memory(devices, reinterpret_cast<const void*>(kernel), smem);
-  if (e != cudaSuccess) return e;
-  const long long pairs = blocks_of(p.t.grid), blocks = p.split.parts > 0 ? p.split.whole + (pairs - p.split.whole) * p.split.parts : pairs;
-  return launch_chained(kernel, dim3(static_cast<unsigned>(blocks)), dim3(threads), smem, s, 1, true, q, k, v, p);
-}
 // One query tile to a CTA, two CTAs to an SM, where sequences are short and CTAs of two tiles would take the SMs more than once.  us, two tiles / one, heads of
 // 64 (batch x tokens x heads): 64 x 128 x 8 19.3 / 11.6, 64 x 200 x 8 32.7 / 27.9, 32 x 384 x 8 33.7 / 27.1, 16 x 512 x 8 23.4 / 22.5, 8 x 768 x 8 28.9 / 26.1, 8 x
 // 1024 x 8 35.7 / 36.5, 2 x 4096 x 8 104 / 121; fitting at once 16 x 128 x 8 5.4 / 6.2, 16 x 256 x 8 8.7 / 8.5.  Heads of 96: 64 x 128 x 8 23.4 / 16.3, 32 x 384 x 8
@@ -1606,21 +1655,35 @@ bool one_tile_pays(const AttnShape& p) {
 // CTAs of one length that would be a last wave of their own, or that are fewer than the SMs, are split over the keys so that they fill them, where that saves more
 // than joining them costs: tiles of keys, of some 0.7 us.  us, whole / split: 16200 tokens, 8 heads of 48 720 / 641, 12 of 64 1086 / 955, 8 of 128 943 / 847; 5000
 // tokens, 8 heads of 64 124 / 83; 2048 tokens 30.2 / 26.4; 1536 23.8 / 20.2.
-constexpr int MIN_SAVED = 8;
-Split split_of(const AttnShape& p) {
-  Split s{0, 0, nullptr, nullptr};
-  if (p.offsets || p.causal || one_tile_pays(p)) return s;
-  const long long pairs = blocks_of(slots_of(p, p.H, 2 * TILE, 1)), sms = sm_count(), last = pairs % sms;
-  if (last == 0) return s;
-  const int tiles = (p.N + TILE - 1) / TILE;
+// The gradients' tiles of queries and of keys in the same way, over the keys and over the queries; heads of more than 64 from 12 tiles on, for what the parts
+// weigh.  us, forward and backward, whole / split: 5000 tokens, 8 heads of 64 365 / 320; 2432 139 / 119; 2048, 4 heads 67.1 / 66.5, 1 head 62 / 49; 1536, 6 heads
+// with 2 of keys 84 / 58; 2560, 8 heads of 128 209 / 181; 16200, 12 of 64 (at the power limit) 3787 / 3734.  8 tiles saved, wide heads: 1536 tokens, 4 heads of 128
+// 82 / 86, 2 x 1536, 2 of 96 75 / 81.
+constexpr int MIN_SAVED = 8, MIN_SAVED_WIDE = 12;
+Parts parts_of(const AttnShape& p, const Slots& g, int tiles, int min_saved) {
+  if (p.offsets || p.causal) return {0, 0};
+  const long long units = blocks_of(g), sms = sm_count(), last = units % sms;
+  if (last == 0) return {0, 0};
   const long long parts = std::min<long long>(sms / last, std::max(1, tiles / 4));
-  if (parts < 2 || tiles - tiles / parts < MIN_SAVED) return s;
-  s.whole = static_cast<uint32_t>(pairs - last);
-  s.parts = static_cast<int>(parts);
-  return s;
+  if (parts < 2 || tiles - tiles / parts < min_saved) return {0, 0};
+  return {static_cast<uint32_t>(units - last), static_cast<int>(parts)};
 }
-long long split_rows(const AttnShape& p, const Split& s) {
-  return s.parts > 0 ? (blocks_of(slots_of(p, p.H, 2 * TILE, 1)) - s.whole) * s.parts * (2 * TILE) : 0;
+long long blocks_of(const Slots& g, const Parts& s) {
+  const long long units = blocks_of(g);
+  return s.parts > 0 ? s.whole + (units - s.whole) * s.parts : units;
+}
+// rows of the buffers of parts
+long long part_rows(const Slots& g, const Parts& s) { return s.parts > 0 ? (blocks_of(g) - s.whole) * s.parts * g.rows : 0; }
+int tiles_of(const AttnShape& p) { return (p.N + TILE - 1) / TILE; }
+Parts forward_parts(const AttnShape& p) { return one_tile_pays(p) ? Parts{0, 0} : parts_of(p, slots_of(p, p.H, 2 * TILE, 1), tiles_of(p), MIN_SAVED); }
+Parts query_parts(const AttnShape& p, const Slots& g) { return parts_of(p, g, tiles_of(p), p.D <= 64 ? MIN_SAVED : MIN_SAVED_WIDE); }
+Parts key_parts(const AttnShape& p, const Slots& g) { return parts_of(p, g, tiles_of(p) * (p.H / p.Hk), p.D <= 64 ? MIN_SAVED : MIN_SAVED_WIDE); }
+template <typename... Params>
+cudaError_t launch(void (*kernel)(Params...), std::atomic<uint64_t>& devices, int threads, int smem, const CUtensorMap& q, const CUtensorMap& k,
+                   const CUtensorMap& v, const FwdParams& p, cudaStream_t s) {
+  const cudaError_t e = allow_shared_memory(devices, reinterpret_cast<const void*>(kernel), smem);
+  if (e != cudaSuccess) return e;
+  return launch_chained(kernel, dim3(static_cast<unsigned>(blocks_of(p.t.grid, p.split))), dim3(threads), smem, s, 1, true, q, k, v, p);
 }
 cudaError_t launch_fwd(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const FwdParams& p, bool one_tile, cudaStream_t s) {
   static std::atomic<uint64_t> devices[4];
@@ -1631,26 +1694,25 @@ cudaError_t launch_fwd(const CUtensorMap& q, const CUtensorMap& k, const CUtenso
   if (p.t.D <= 64) return launch(attn_fwd_narrow_kernel, devices[2], THREADS, FwdNarrow::SMEM, q, k, v, p, s);
   return launch(attn_fwd_kernel<2, 2>, devices[3], Fwd<2, 2>::THREADS_, Fwd<2, 2>::SMEM, q, k, v, p, s);
 }
-template <int DB>
+template <int DB, bool SPLIT>
 cudaError_t launch_dq(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& g, const DqParams& p, cudaStream_t s) {
   static std::atomic<uint64_t> devices;
-  const cudaError_t e = allow_shared_memory(devices, reinterpret_cast<const void*>(&attn_dq_kernel<DB>), Dq<DB>::SMEM);
+  const cudaError_t e = allow_shared_memory(devices, reinterpret_cast<const void*>(&attn_dq_kernel<DB, SPLIT>), Dq<DB>::SMEM);
   if (e != cudaSuccess) return e;
-  return launch_chained(attn_dq_kernel<DB>, dim3(static_cast<unsigned>(blocks_of(p.t.grid))), dim3(BWD_THREADS), Dq<DB>::SMEM, s, 1, true, q, k, v, g, p);
+  return launch_chained(attn_dq_kernel<DB, SPLIT>, dim3(static_cast<unsigned>(blocks_of(p.t.grid, p.split))), dim3(BWD_THREADS), Dq<DB>::SMEM, s, 1, true, q, k, v, g, p);
 }
-template <int DB>
+template <int DB, bool SPLIT>
 cudaError_t launch_dkv(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& g, const DkvParams& p, cudaStream_t s) {
   static std::atomic<uint64_t> devices;
-  const cudaError_t e = allow_shared_memory(devices, reinterpret_cast<const void*>(&attn_dkv_kernel<DB>), Dkv<DB>::SMEM);
+  const cudaError_t e = allow_shared_memory(devices, reinterpret_cast<const void*>(&attn_dkv_kernel<DB, SPLIT>), Dkv<DB>::SMEM);
   if (e != cudaSuccess) return e;
-  return launch_chained(attn_dkv_kernel<DB>, dim3(static_cast<unsigned>(blocks_of(p.t.grid))), dim3(BWD_THREADS), Dkv<DB>::SMEM, s, 1, true, q, k, v, g, p);
+  return launch_chained(attn_dkv_kernel<DB, SPLIT>, dim3(static_cast<unsigned>(blocks_of(p.t.grid, p.split))), dim3(BWD_THREADS), Dkv<DB>::SMEM, s, 1, true, q, k, v, g, p);
 }
 
 }  // namespace
 
 long long attention_scratch(const AttnShape& p) {
-  if (!shape_ok(p)) return 0;
-  return split_rows(p, split_of(p)) * (p.D + 2);
+  return shape_ok(p) ? part_rows(slots_of(p, p.H, 2 * TILE, 1), forward_parts(p)) * (p.D + 2) : 0;
 }
 
 cudaError_t attention_fwd(const AttnShape& p, const AttnTensor& q, const AttnTensor& k, const AttnTensor& v, __nv_bfloat16* o, __nv_bfloat16* o_rest,
@@ -1664,9 +1726,9 @@ cudaError_t attention_fwd(const AttnShape& p, const AttnTensor& q, const AttnTen
   FwdParams f;
   const bool one_tile = one_tile_pays(p);
   f.t = tile_params(p, slots_of(p, p.H, one_tile ? TILE : 2 * TILE, 1), err);
-  f.split = scratch ? split_of(p) : Split{0, 0, nullptr, nullptr};
+  static_cast<Parts&>(f.split) = scratch ? forward_parts(p) : Parts{0, 0};
   f.split.o = scratch;
-  const long long rows = split_rows(p, f.split);
+  const long long rows = part_rows(f.t.grid, f.split);
   f.split.ml = reinterpret_cast<float2*>(scratch + rows * p.D);
   f.o = o;
   f.o_rest = o_rest;
@@ -1678,11 +1740,17 @@ cudaError_t attention_fwd(const AttnShape& p, const AttnTensor& q, const AttnTen
   return launch_chained(attn_join_kernel, dim3(static_cast<unsigned>(rows / f.split.parts / 8)), dim3(256), 0, s, 1, true, f);
 }
 
+long long attention_bwd_scratch(const AttnShape& p) {
+  if (!shape_ok(p)) return 0;
+  const Slots q = slots_of(p, p.H, TILE, 1), k = slots_of(p, p.Hk, TILE, 2);
+  return std::max(part_rows(q, query_parts(p, q)), 2 * part_rows(k, key_parts(p, k))) * p.D;
+}
+
 cudaError_t attention_bwd(const AttnShape& p, const AttnTensor& q, const AttnTensor& k, const AttnTensor& v, const __nv_bfloat16* o,
                           const __nv_bfloat16* o_rest, const __nv_bfloat16* d_o, const float* lse, float* delta, const AttnTensor& dq,
-                          const AttnTensor& dk, const AttnTensor& dv, int* err, cudaStream_t s) {
+                          const AttnTensor& dk, const AttnTensor& dv, float* scratch, int* launches, int* err, cudaStream_t s) {
   auto bad = [](const AttnTensor& t) { return (reinterpret_cast<uintptr_t>(t.ptr) & 15) || ((t.token | t.head | t.batch) & 7); };
-  if (!shape_ok(p) || ((reinterpret_cast<uintptr_t>(o) | reinterpret_cast<uintptr_t>(o_rest) | reinterpret_cast<uintptr_t>(d_o)) & 15) || bad(dq) || bad(dk) || bad(dv))
+  if (!shape_ok(p) || ((reinterpret_cast<uintptr_t>(o) | reinterpret_cast<uintptr_t>(o_rest) | reinterpret_cast<uintptr_t>(d_o) | reinterpret_cast<uintptr_t>(scratch)) & 15) || bad(dq) || bad(dk) || bad(dv))
     return cudaErrorInvalidValue;
   bind_context(s);
   const AttnTensor g{const_cast<__nv_bfloat16*>(d_o), 1ll * p.H * p.D, p.D, 1ll * p.N * p.H * p.D};
@@ -1703,9 +1771,31 @@ cudaError_t attention_bwd(const AttnShape& p, const AttnTensor& q, const AttnTen
   b.delta = delta;
   b.dk = dk;
   b.dv = dv;
-  const cudaError_t e = p.D <= 64 ? launch_dq<1>(mq, mk_, mv, mg, a, s) : launch_dq<2>(mq, mk_, mv, mg, a, s);
+  a.split = scratch ? query_parts(p, a.t.grid) : Parts{0, 0};
+  a.sums = scratch;
+  b.split = scratch ? key_parts(p, b.t.grid) : Parts{0, 0};
+  const long long rows_q = part_rows(a.t.grid, a.split), rows_k = part_rows(b.t.grid, b.split);
+  // (the parts of dQ have been added up where those of dK and dV begin)
+  b.dv_sums = scratch;
+  b.dk_sums = scratch + rows_k * p.D;
+  *launches = 1;
+  cudaError_t e = rows_q > 0 ? (p.D <= 64 ? launch_dq<1, true>(mq, mk_, mv, mg, a, s) : launch_dq<2, true>(mq, mk_, mv, mg, a, s))
+                             : (p.D <= 64 ? launch_dq<1, false>(mq, mk_, mv, mg, a, s) : launch_dq<2, false>(mq, mk_, mv, mg, a, s));
+  if (e == cudaSuccess && rows_q > 0) {
+    ++*launches;
+    const Sums sums{{a.sums, nullptr}, {dq, dq}, {p.scale, 0.f}};
+    e = launch_chained(attn_sum_kernel, dim3(static_cast<unsigned>(rows_q / a.split.parts / 8)), dim3(256), 0, s, 1, true, a.t.grid, a.split, sums, p.D);
+  }
   if (e != cudaSuccess) return e;
-  return p.D <= 64 ? launch_dkv<1>(mq, mk_, mv, mg, b, s) : launch_dkv<2>(mq, mk_, mv, mg, b, s);
+  ++*launches;
+  e = rows_k > 0 ? (p.D <= 64 ? launch_dkv<1, true>(mq, mk_, mv, mg, b, s) : launch_dkv<2, true>(mq, mk_, mv, mg, b, s))
+                 : (p.D <= 64 ? launch_dkv<1, false>(mq, mk_, mv, mg, b, s) : launch_dkv<2, false>(mq, mk_, mv, mg, b, s));
+  if (e == cudaSuccess && rows_k > 0) {
+    ++*launches;
+    const Sums sums{{b.dv_sums, b.dk_sums}, {dv, dk}, {1.f, p.scale}};
+    e = launch_chained(attn_sum_kernel, dim3(static_cast<unsigned>(rows_k / b.split.parts / 8), 2), dim3(256), 0, s, 1, true, b.t.grid, b.split, sums, p.D);
+  }
+  return e;
 }
 
 }  // namespace mk

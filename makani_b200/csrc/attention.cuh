@@ -30,9 +30,11 @@ struct AttnShape {
 long long attention_scratch(const AttnShape& p);
 cudaError_t attention_fwd(const AttnShape& p, const AttnTensor& q, const AttnTensor& k, const AttnTensor& v, __nv_bfloat16* o, __nv_bfloat16* o_rest,
                           float* lse, float* scratch, int* launches, int* err, cudaStream_t s);
-// dq, dk, dv from o, o_rest and d_o (dense, like o); delta [B, H, N]: room for the row sums of o d_o.  Two launches, no atomics.
+// dq, dk, dv from o, o_rest and d_o (dense, like o); delta [B, H, N]: room for the row sums of o d_o.  `scratch`: attention_bwd_scratch() floats.  Two launches,
+// with the sums of what is split four, and no atomics.
+long long attention_bwd_scratch(const AttnShape& p);
 cudaError_t attention_bwd(const AttnShape& p, const AttnTensor& q, const AttnTensor& k, const AttnTensor& v, const __nv_bfloat16* o,
                           const __nv_bfloat16* o_rest, const __nv_bfloat16* d_o, const float* lse, float* delta, const AttnTensor& dq,
-                          const AttnTensor& dk, const AttnTensor& dv, int* err, cudaStream_t s);
+                          const AttnTensor& dk, const AttnTensor& dv, float* scratch, int* launches, int* err, cudaStream_t s);
 
 }  // namespace mk

@@ -306,10 +306,13 @@ void attention_backward(const Tensor& d_out, const Tensor& q_in, const Tensor& k
   Tensor g = d_out.contiguous();
   if (reinterpret_cast<uintptr_t>(g.data_ptr()) & 15) g = g.clone();
   const Tensor q = readable(q_in), k = readable(k_in), v = readable(v_in), delta = at::empty_like(lse);
-  mkh::launches() += 2;
+  Tensor scratch;
+  if (const int64_t floats = mk::attention_bwd_scratch(p)) scratch = at::empty({floats}, q.options().dtype(at::kFloat));
+  int launches = 0;
   mkh::check(mk::attention_bwd(p, view_of(q), view_of(k), view_of(v), bf(o), bf(rest), bf(g), lse.data_ptr<float>(), delta.data_ptr<float>(), view_of(dq),
-                               view_of(dk), view_of(dv), mkh::error_word(q), mkh::stream()),
+                               view_of(dk), view_of(dv), ptr_or_null<float>(scratch), &launches, mkh::error_word(q), mkh::stream()),
              "attention_bwd");
+  mkh::launches() += launches;
 }
 
 struct Attention : torch::autograd::Function<Attention> {

@@ -171,6 +171,16 @@ def test_few_rows_and_long_keys(gen, B, N, H, Hk, D):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("B,N,H,Hk,D", [(1, 2700, 8, 8, 64), (1, 2561, 8, 2, 128), (2, 1700, 6, 1, 48), (1, 5003, 4, 4, 104)])
+def test_last_wave_of_the_gradients(gen, B, N, H, Hk, D):
+    """Tiles of queries and keys behind the last whole wave are split along the other axis (over the heads that share keys, too) and summed; twice, the same bits."""
+    _check_batch(gen, B, N, H, Hk, D, False)
+    q, k, v, do = _inputs(gen, B, N, H=H, Hk=Hk, D=D)
+    first, again = _run(q, k, v, do), _run(q, k, v, do)
+    assert all(torch.equal(first[n], again[n]) for n in first)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("D", [1, 5, 20, 65, 127])
 def test_widths_that_are_padded(gen, D):
     _check_batch(gen, 1, 200, 2, 1, D, True)
