@@ -1009,8 +1009,8 @@ __device__ __forceinline__ void slopes_of(const uint32_t (&v)[BWD_COLS], const u
   }
 }
 
-// Gradient of the queries.  A CTA has 128 queries of a head and goes over the keys.  S has two buffers, so that the products of the next tile are there when the warps come to them.  delta is computed on the way and
-// written for the second kernel.
+// Gradient of the queries.  A CTA has 128 queries of a head and goes over the keys.  S has two buffers, so that the products of the next tile are there when the
+// warps come to them.  delta is computed on the way and written for the second kernel (CTAs that share queries write the same).
 template <int DB>
 struct Dq {
   static constexpr int STAGES = DB == 1 ? 4 : 2, TILE_BYTES = DB * BOX;
@@ -1699,14 +1699,16 @@ cudaError_t launch_dq(const CUtensorMap& q, const CUtensorMap& k, const CUtensor
   static std::atomic<uint64_t> devices;
   const cudaError_t e = allow_shared_memory(devices, reinterpret_cast<const void*>(&attn_dq_kernel<DB, SPLIT>), Dq<DB>::SMEM);
   if (e != cudaSuccess) return e;
-  return launch_chained(attn_dq_kernel<DB, SPLIT>, dim3(static_cast<unsigned>(blocks_of(p.t.grid, p.split))), dim3(BWD_THREADS), Dq<DB>::SMEM, s, 1, true, q, k, v, g, p);
+  return launch_chained(attn_dq_kernel<DB, SPLIT>, dim3(static_cast<unsigned>(blocks_of(p.t.grid, p.split))), dim3(BWD_THREADS), Dq<DB>::SMEM, s, 1, true, q, k, v,
+                        g, p);
 }
 template <int DB, bool SPLIT>
 cudaError_t launch_dkv(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& g, const DkvParams& p, cudaStream_t s) {
   static std::atomic<uint64_t> devices;
   const cudaError_t e = allow_shared_memory(devices, reinterpret_cast<const void*>(&attn_dkv_kernel<DB, SPLIT>), Dkv<DB>::SMEM);
   if (e != cudaSuccess) return e;
-  return launch_chained(attn_dkv_kernel<DB, SPLIT>, dim3(static_cast<unsigned>(blocks_of(p.t.grid, p.split))), dim3(BWD_THREADS), Dkv<DB>::SMEM, s, 1, true, q, k, v, g, p);
+  return launch_chained(attn_dkv_kernel<DB, SPLIT>, dim3(static_cast<unsigned>(blocks_of(p.t.grid, p.split))), dim3(BWD_THREADS), Dkv<DB>::SMEM, s, 1, true, q, k, v,
+                        g, p);
 }
 
 }  // namespace
@@ -1749,9 +1751,9 @@ long long attention_bwd_scratch(const AttnShape& p) {
 cudaError_t attention_bwd(const AttnShape& p, const AttnTensor& q, const AttnTensor& k, const AttnTensor& v, const __nv_bfloat16* o,
                           const __nv_bfloat16* o_rest, const __nv_bfloat16* d_o, const float* lse, float* delta, const AttnTensor& dq,
                           const AttnTensor& dk, const AttnTensor& dv, float* scratch, int* launches, int* err, cudaStream_t s) {
-  auto bad = [](const AttnTensor& t) { return (reinterpret_cast<uintptr_t>(t.ptr) & 15) || ((t.token | t.head | t.batch) & 7); };
-  if (!shape_ok(p) || ((reinterpret_cast<uintptr_t>(o) | reinterpret_cast<uintptr_t>(o_rest) | reinterpret_cast<uintptr_t>(d_o) | reinterpret_cast<uintptr_t>(scratch)) & 15) || bad(dq) || bad(dk) || bad(dv))
-    return cudaErrorInvalidValue;
+  auto off = [](const void* at) { return (reinterpret_cast<uintptr_t>(at) & 15) != 0; };
+  auto bad = [&](const AttnTensor& t) { return off(t.ptr) || ((t.token | t.head | t.batch) & 7); };
+  if (!shape_ok(p) || off(o) || off(o_rest) || off(d_o) || off(scratch) || bad(dq) || bad(dk) || bad(dv)) return cudaErrorInvalidValue;
   bind_context(s);
   const AttnTensor g{const_cast<__nv_bfloat16*>(d_o), 1ll * p.H * p.D, p.D, 1ll * p.N * p.H * p.D};
   CUtensorMap mq, mk_, mv, mg;

@@ -26,8 +26,8 @@ struct LnForward {
 };
 cudaError_t layer_norm_fwd(const LnForward& p, cudaStream_t s);
 
-// dx (type of x; a copy in bf16 in `dr`, if there is one) = rstd (g - mean(g) - xh mean(g xh)) (+ ds), g = dy w (dy: type of y); dw = sum of dy xh, db = sum of dy over the rows (both or
-// none).  `part`: layer_norm_scratch() floats.  The sums are added up in one fixed order.
+// dx (type of x; a copy in bf16 in `dr`, if there is one) = rstd (g - mean(g) - xh mean(g xh)) (+ ds), g = dy w (dy: type of y); dw = sum of dy xh, db = sum
+// of dy over the rows (both or none).  `part`: layer_norm_scratch() floats.  The sums are added up in one fixed order.
 struct LnBackward {
   const void* x;
   const void* dy;
