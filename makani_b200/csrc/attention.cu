@@ -1420,7 +1420,7 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
           if (!ok) break;
           const bool clear = fix && t == q_tiles - 1;
           if (clear) mbar_arrive(fix_bar);
-          ok = (!clear || mbar_wait(fixed, g & 1)) && mbar_wait(p_ready, j & 1);
+          ok = (!clear || mbar_wait(fixed, (g - g0) & 1)) && mbar_wait(p_ready, j & 1);
           if (!ok) {
             atomicExch(p.t.err, 92);
             break;
@@ -1487,7 +1487,7 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       }
     } else if (fix) {
       // ---------------------------------------------------------------- queries of the next sequence
-      for (int g = 0; g < p.t.group; ++g) {
+      for (int g = 0; g < n / q_tiles; ++g) {
         if (!wait_long(fix_bar, g & 1, q_tiles)) break;
         clear_rows(smem_raw + pad + L::STAGE_AT + (g * q_tiles + q_tiles - 1) % L::STAGES * L::STAGE, 2 * DB, tail);
         if (lane == 0) mbar_arrive(fixed);
@@ -1581,12 +1581,13 @@ struct Sums {
 };
 __global__ void __launch_bounds__(256) attn_sum_kernel(Slots grid, Parts split, Sums p, int D) {
   const float* parts = p.parts[blockIdx.y];
-  chain_begin(true, parts);
+  const int* offsets = grid.offsets;
+  chain_begin(true, parts, offsets);
   const int lane = threadIdx.x & 31, c = lane * 4;
   const uint32_t at = blockIdx.x * 8 + (threadIdx.x >> 5), unit = at / TILE;
   const int row = static_cast<int>(at % TILE);
   Work w;
-  if (!find_work(grid, nullptr, split.whole + unit, w) || w.r0 + row >= w.len || c >= D) return;
+  if (!find_work(grid, offsets, split.whole + unit, w) || w.padding || w.r0 + row >= w.len || c >= D) return;
   float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int k = 0; k < split.parts; ++k) {
     const float4 v = __ldcg(reinterpret_cast<const float4*>(parts + ((static_cast<long long>(unit) * split.parts + k) * TILE + row) * D + c));
@@ -1594,7 +1595,7 @@ __global__ void __launch_bounds__(256) attn_sum_kernel(Slots grid, Parts split, 
   }
   const float f = p.factor[blockIdx.y];
   const AttnTensor& o = p.out[blockIdx.y];
-  *reinterpret_cast<uint2*>(o.ptr + w.b * o.batch + (w.r0 + row) * o.token + w.h * o.head + c) =
+  *reinterpret_cast<uint2*>(o.ptr + w.b * o.batch + (w.lo + w.r0 + row) * o.token + w.h * o.head + c) =
       make_uint2(pack_bf16(a.x * f, a.y * f), pack_bf16(a.z * f, a.w * f));
 }
 
@@ -1661,7 +1662,7 @@ bool one_tile_pays(const AttnShape& p) {
 // 82 / 86, 2 x 1536, 2 of 96 75 / 81.
 constexpr int MIN_SAVED = 8, MIN_SAVED_WIDE = 12;
 Parts parts_of(const AttnShape& p, const Slots& g, int tiles, int min_saved) {
-  if (p.offsets || p.causal) return {0, 0};
+  if (p.offsets || p.causal) return {0, 0};      // (not of one length)
   const long long units = blocks_of(g), sms = sm_count(), last = units % sms;
   if (last == 0) return {0, 0};
   const long long parts = std::min<long long>(sms / last, std::max(1, tiles / 4));
@@ -1677,7 +1678,20 @@ long long part_rows(const Slots& g, const Parts& s) { return s.parts > 0 ? (bloc
 int tiles_of(const AttnShape& p) { return (p.N + TILE - 1) / TILE; }
 Parts forward_parts(const AttnShape& p) { return one_tile_pays(p) ? Parts{0, 0} : parts_of(p, slots_of(p, p.H, 2 * TILE, 1), tiles_of(p), MIN_SAVED); }
 Parts query_parts(const AttnShape& p, const Slots& g) { return parts_of(p, g, tiles_of(p), p.D <= 64 ? MIN_SAVED : MIN_SAVED_WIDE); }
-Parts key_parts(const AttnShape& p, const Slots& g) { return parts_of(p, g, tiles_of(p) * (p.H / p.Hk), p.D <= 64 ? MIN_SAVED : MIN_SAVED_WIDE); }
+// Where lengths differ: over the heads that share keys, if CTAs are for two thirds of the SMs at most (in all of them, then).  us, forward and backward, causal,
+// whole / split, 64 channels: 1024 tokens, 8 heads on 2 78 / 56; 2048, 16 on 4 141 / 106; 2000 in 4 sequences 126 / 104; 1000 in 2, 8 on 1 77 / 52; 128 channels, 2048, 8
+// on 2 188 / 117; with more CTAs 4000 in 3, 8 on 4 111 / 120; 9113 in 7, 16 on 4 479 / 501.
+Parts key_parts(const AttnShape& p, const Slots& g) {
+  const int group = p.H / p.Hk, min_saved = p.D <= 64 ? MIN_SAVED : MIN_SAVED_WIDE;
+  if (!p.offsets && !p.causal) return parts_of(p, g, tiles_of(p) * group, min_saved);
+  const long long units = blocks_of(g), sms = sm_count();
+  if (3 * units > 2 * sms) return {0, 0};
+  int parts = static_cast<int>(std::min<long long>(group, 3 * sms / units));
+  while (group % parts) --parts;
+  const int mean = p.offsets ? p.N / std::max(1, p.sequences) : p.N, tiles = (mean + TILE - 1) / TILE * group;
+  if (parts < 2 || tiles - tiles / parts < min_saved) return {0, 0};
+  return {0, parts};
+}
 template <typename... Params>
 cudaError_t launch(void (*kernel)(Params...), std::atomic<uint64_t>& devices, int threads, int smem, const CUtensorMap& q, const CUtensorMap& k,
                    const CUtensorMap& v, const FwdParams& p, cudaStream_t s) {

@@ -181,6 +181,23 @@ def test_last_wave_of_the_gradients(gen, B, N, H, Hk, D):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("H,Hk,D", [(8, 2, 64), (8, 1, 128), (6, 2, 24), (12, 1, 96)])
+def test_shared_heads_apart(gen, H, Hk, D):
+    """Gradients of keys and values with few CTAs: the heads that share them in CTAs of their own, causal and in packed sequences among NaN."""
+    _check_batch(gen, 1, 1100, H, Hk, D, True)
+    at = [0, 700, 700, 701, 1630]
+    for causal in (False, True):
+        q, k, v, do = _inputs(gen, 1700, H=H, Hk=Hk, D=D)
+        for x in (q, k, v, do):
+            x[at[-1]:] = float("nan")
+        got = _run(q, k, v, do, causal=causal, offsets=torch.tensor(at, dtype=torch.int32, device="cuda"))
+        want, off = _oracle(q, k, v, do, causal, D ** -0.5, list(zip(at, at[1:])))
+        for n in want:
+            _close(got[n], want[n], off[n], n)
+            assert not got[n][at[-1]:].any()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("D", [1, 5, 20, 65, 127])
 def test_widths_that_are_padded(gen, D):
     _check_batch(gen, 1, 200, 2, 1, D, True)
