@@ -1259,7 +1259,7 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
 }
 
 // Gradients of keys and values.  A CTA has 128 keys of a head and goes over the queries of all heads that share it, so that nothing is added up
-// afterwards.  Scores are transposed (a thread's row is a key), so that P and dS come out of tensor memory as the first operands of the
+// afterwards but what `key_parts` splits.  Scores are transposed (a thread's row is a key), so that P and dS come out of tensor memory as the first operands of the
 // products with dO and Q.  Heads of up to 64 channels: two buffers of S, the next tile's scores run in front of the products that wait for the
 // warps; above, tensor memory is full with one, and they run behind the first of these.
 template <int DB>
@@ -1679,7 +1679,7 @@ int tiles_of(const AttnShape& p) { return (p.N + TILE - 1) / TILE; }
 Parts forward_parts(const AttnShape& p) { return one_tile_pays(p) ? Parts{0, 0} : parts_of(p, slots_of(p, p.H, 2 * TILE, 1), tiles_of(p), MIN_SAVED); }
 Parts query_parts(const AttnShape& p, const Slots& g) { return parts_of(p, g, tiles_of(p), p.D <= 64 ? MIN_SAVED : MIN_SAVED_WIDE); }
 // Where lengths differ: over the heads that share keys, if CTAs are for two thirds of the SMs at most (in all of them, then).  us, forward and backward, causal,
-// whole / split, 64 channels: 1024 tokens, 8 heads on 2 78 / 56; 2048, 16 on 4 141 / 106; 2000 in 4 sequences 126 / 104; 1000 in 2, 8 on 1 77 / 52; 128 channels, 2048, 8
+// whole / split, 64 channels: 1024 tokens, 8 heads on 2 78 / 56; 2048, 16 on 4 141 / 106; 2000 in 4 sequences 126 / 104; 1000 in 2, 8 on 1 77 / 47; 128 channels, 2048, 8
 // on 2 188 / 117; with more CTAs 4000 in 3, 8 on 4 111 / 120; 9113 in 7, 16 on 4 479 / 501.
 Parts key_parts(const AttnShape& p, const Slots& g) {
   const int group = p.H / p.Hk, min_saved = p.D <= 64 ? MIN_SAVED : MIN_SAVED_WIDE;
