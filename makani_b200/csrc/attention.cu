@@ -3,9 +3,9 @@
 //   forward    P = exp(S - max), O = P V / sum P, L = max + log sum P                           (one pass over the keys, running max and sum)
 //   backward   P = exp(S - L), dV = P^T dO, dS = P (dO V^T - delta), dQ = scale dS K, dK = scale dS^T Q,  delta = sum_d O dO
 //
-// Exponentials are powers of two of (scale log2 e) S, one special-function instruction each.  Products take bf16 operands and add in fp32 (tensor
-// memory); P and dS are rounded to bf16 as operands of the second products (half a step, 2^-8 of each weight at most, as the rounding of the
-// outputs), sums, maxima and L stay in fp32.
+// Exponentials are powers of two of (scale log2 e) S: one special-function instruction each, but for a quarter of those of the backward pass, which are a
+// polynomial on the FMA pipe (`ex2_poly`).  Products take bf16 operands and add in fp32 (tensor memory); P and dS are rounded to bf16 as operands of the
+// second products (half a step, 2^-8 of each weight at most, as the rounding of the outputs), sums, maxima and L stay in fp32.
 //
 // Warps: 0 loads tiles (TMA), 1 (and 3, narrow heads forward) issues products, 2 (and 3, dK and dV) loads statistics and clears rows that belong to another
 // sequence, those from 4 on compute on rows in tensor memory, a thread a row or a part of one.  Every wait is bounded; on expiry the kernel records a
@@ -116,12 +116,19 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// The greater of x and `least`, NaN if x is NaN
+__device__ __forceinline__ float at_least(float x, float least) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(x), "f"(least));
+  return y;
+}
 // 2^x of two values with fp32 arithmetic, for a share of a tile's exponentials: the special function unit takes 1024 cycles for 128 x 128 of them, while the
 // FMA pipe has time.  x = n + f with n the integer next to it (1.5 2^23 added and taken away), 2^f from a polynomial (Remez exchange for the least
-// relative error on |f| <= 1/2: 2.7e-6 in fp32), n into the exponent.  Below -126 it stays at 2^-126.
+// relative error on |f| <= 1/2: 2.7e-6 in fp32), times 2^n made of n's bits.  Below -126 it stays at 2^-126.  NaN comes out as NaN (through the product:
+// n added to the exponent's bits would make a number of it): a row whose scores have no finite sum has L = NaN, and shows it in every gradient.
 __device__ __forceinline__ void ex2_poly(float& a, float& b) {
   const float nearest = 12582912.f;
-  const f32x2 x = f2_pack(fmaxf(a, -126.f), fmaxf(b, -126.f));
+  const f32x2 x = f2_pack(at_least(a, -126.f), at_least(b, -126.f));
   const f32x2 t = f2_add(x, f2_pack(nearest, nearest));
   const f32x2 n = f2_add(t, f2_pack(-nearest, -nearest));
   const f32x2 f = f2_fma(n, f2_pack(-1.f, -1.f), x);
@@ -129,11 +136,10 @@ __device__ __forceinline__ void ex2_poly(float& a, float& b) {
   y = f2_fma(y, f, f2_pack(0.240247443318367f, 0.240247443318367f));
   y = f2_fma(y, f, f2_pack(0.6931217908859253f, 0.6931217908859253f));
   y = f2_fma(y, f, f2_pack(0.9999992847442627f, 0.9999992847442627f));
-  float ta, tb, ya, yb;
+  float ta, tb;
   f2_unpack(t, ta, tb);
-  f2_unpack(y, ya, yb);
-  a = __uint_as_float(__float_as_uint(ya) + (__float_as_uint(ta) << 23));
-  b = __uint_as_float(__float_as_uint(yb) + (__float_as_uint(tb) << 23));
+  constexpr uint32_t one = 0x3f800000u;
+  f2_unpack(f2_mul(y, f2_pack(__uint_as_float((__float_as_uint(ta) << 23) + one), __uint_as_float((__float_as_uint(tb) << 23) + one))), a, b);
 }
 // Pair `i` of a row: POLY of every eight on the FMA pipe
 template <int POLY>

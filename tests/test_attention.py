@@ -396,3 +396,25 @@ def test_gradient_against_differences(gen):
         own = _oracle(q[0], k[0], v[0], do[0], False, D ** -0.5, [(0, N)])
         off = off + ((own[1][n] * (1 + B_STEP) + B_STEP * own[0][n].abs()) * moved[0].abs()).sum()
         assert abs(float(f[0] - f[1] - left_out - (got[n].double() * moved).sum())) <= float(off), n
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("D", [32, 96])
+def test_nan_of_a_query_reaches_what_it_sees(gen, D, causal):
+    """A query with NaN or infinity makes NaN of the gradients of all keys and values that it sees, wherever in a tile it stands, and changes no value's that it
+    does not see."""
+    N, first = 300, 136
+    q, k, v, do = _inputs(gen, 16, N, H=2, Hk=2, D=D)
+    clean = _run(q, k, v, do, causal=causal)
+    dirty = q.clone()
+    for b in range(16):
+        dirty[b, first + b, 0, 3] = float("nan") if b < 8 else float("inf")
+    got = _run(dirty, k, v, do, causal=causal)
+    for b in range(16):
+        seen = first + b + 1 if causal else N
+        assert got["dq"][b, first + b, 0].isnan().all() and got["o"][b, first + b, 0].isnan().all(), b
+        for n in ("dk", "dv"):
+            assert got[n][b, :seen, 0].isnan().all(), (n, b)
+        assert torch.equal(got["dv"][b, seen:, 0], clean["dv"][b, seen:, 0]), b
+    assert all(torch.equal(got[n][:, :, 1], clean[n][:, :, 1]) for n in got)
