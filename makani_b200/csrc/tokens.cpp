@@ -234,12 +234,16 @@ variable_list layer_norm(const Tensor& x, const OptTensor& residual, const OptTe
 
 __nv_bfloat16* bf(const Tensor& t) { return reinterpret_cast<__nv_bfloat16*>(t.data_ptr()); }
 
-mk::AttnTensor view_of(const Tensor& t) { return {bf(t), t.stride(1), t.stride(2), t.stride(0)}; }
+// (what a dimension of size one has for a stride says nothing: torch lets it be anything, in a contiguous tensor too)
+mk::AttnTensor view_of(const Tensor& t) {
+  auto stride = [&](int d) { return t.size(d) == 1 ? t.size(3) : t.stride(d); };
+  return {bf(t), stride(1), stride(2), stride(0)};
+}
 
 // [B, N, heads, D] as the kernels read it: dense channels, strides of whole 16-byte vectors, none of them zero; a copy where it is not
 Tensor readable(const Tensor& t) {
   bool fits = t.stride(3) == 1 && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0;
-  for (int d = 0; d < 3; ++d) fits = fits && t.stride(d) > 0 && t.stride(d) % 8 == 0 && t.stride(d) < (1ll << 34);
+  for (int d = 0; d < 3; ++d) fits = fits && (t.size(d) == 1 || (t.stride(d) > 0 && t.stride(d) % 8 == 0 && t.stride(d) < (1ll << 34)));
   if (fits) return t;
   const Tensor c = t.contiguous();
   return (reinterpret_cast<uintptr_t>(c.data_ptr()) & 15) == 0 ? c : c.clone();

@@ -418,3 +418,29 @@ def test_nan_of_a_query_reaches_what_it_sees(gen, D, causal):
             assert got[n][b, :seen, 0].isnan().all(), (n, b)
         assert torch.equal(got["dv"][b, seen:, 0], clean["dv"][b, seen:, 0]), b
     assert all(torch.equal(got[n][:, :, 1], clean[n][:, :, 1]) for n in got)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,N,H,D", [(2, 1, 4, 8), (1, 70, 2, 16), (2, 40, 1, 16), (1, 1, 3, 24), (3, 1, 1, 64), (1, 1, 1, 8)])
+def test_strides_of_single_dimensions(gen, B, N, H, D):
+    """A dimension of size one may have any stride: torch calls such a tensor contiguous."""
+    q, k, v, do = _inputs(gen, B, N, H=H, Hk=H, D=D)
+    want = _run(q, k, v, do)
+    for odd in (1, 3, 8, 1 << 40):
+        views = [t.as_strided(t.shape, [s if n > 1 else odd for n, s in zip(t.shape, t.stride())]) for t in (q, k, v, do)]
+        got = _run(*views)
+        assert all(torch.equal(got[n], want[n]) for n in want), odd
+    x = torch.cat([t.flatten(2) for t in (q, k, v)], -1)
+    y = x.as_strided(x.shape, [s if n > 1 else 1 for n, s in zip(x.shape, x.stride())]).requires_grad_()
+    o = attn.attention_qkv(y, H)
+    assert torch.equal(o, want["o"])
+    dx = torch.autograd.grad(o, y, do)[0]
+    assert torch.equal(dx, torch.cat([want[n].flatten(2) for n in ("dq", "dk", "dv")], -1))
+
+
+@pytest.mark.gpu
+def test_single_token_of_a_permuted_tensor(gen):
+    t = torch.randn(2, 4, 8, 1, device="cuda", generator=gen).bfloat16()
+    q = t.permute(0, 3, 1, 2)
+    assert q.is_contiguous() and q.stride(1) == 1
+    assert torch.equal(attn.attention(q, q, q), q)          # one key: its weight is 1
