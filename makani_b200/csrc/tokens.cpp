@@ -255,7 +255,7 @@ mk::AttnShape shape_of(const Tensor& q, const Tensor& k, const Tensor& v, const 
   MK_CHECK(k.device() == q.device() && v.device() == q.device(), "attention: tensors must be on one CUDA device");
   MK_CHECK(k.sizes() == v.sizes() && k.size(0) == q.size(0) && k.size(1) == q.size(1) && k.size(3) == q.size(3),
            "attention: queries, keys and values must be of the same tokens and channels");
-  MK_CHECK(k.size(2) > 0 && q.size(2) % k.size(2) == 0, "attention: heads of keys must divide those of queries");
+  MK_CHECK(q.size(2) > 0 && k.size(2) > 0 && q.size(2) % k.size(2) == 0, "attention: heads of keys must divide those of queries");
   MK_CHECK(q.size(3) > 0 && q.size(3) % 8 == 0 && q.size(3) <= mk::ATTN_WIDTH, "attention: 8, 16, .., ", mk::ATTN_WIDTH, " channels of a head expected");
   MK_CHECK(scale > 0.0 && std::isfinite(scale), "attention: a positive scale expected");
   MK_CHECK(q.size(0) * q.size(1) * q.size(2) < (1ll << 31) - (1ll << 24), "attention: too many rows");

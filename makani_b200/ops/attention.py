@@ -70,8 +70,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: bool = 
                          f"{tuple(k.shape)}, {tuple(v.shape)}")
     if k.shape != v.shape or k.shape[:-2] != q.shape[:-2] or k.shape[-1] != q.shape[-1]:
         raise ValueError(f"queries {tuple(q.shape)}, keys {tuple(k.shape)} and values {tuple(v.shape)} must be of the same tokens and channels")
-    if k.shape[-2] < 1 or q.shape[-2] % k.shape[-2]:
-        raise ValueError(f"{k.shape[-2]} heads of keys do not divide {q.shape[-2]} of queries")
+    if q.shape[-2] < 1 or k.shape[-2] < 1 or q.shape[-2] % k.shape[-2]:
+        raise ValueError(f"{q.shape[-2]} heads of queries, {k.shape[-2]} of keys: there must be some, and those of keys divide those of queries")
     if not (q.dtype == k.dtype == v.dtype and q.device == k.device == v.device and q.dtype.is_floating_point):
         raise ValueError("queries, keys and values must share one floating-point type and device")
     if q.shape[-1] < 1:

@@ -444,3 +444,22 @@ def test_single_token_of_a_permuted_tensor(gen):
     q = t.permute(0, 3, 1, 2)
     assert q.is_contiguous() and q.stride(1) == 1
     assert torch.equal(attn.attention(q, q, q), q)          # one key: its weight is 1
+
+
+@pytest.mark.parametrize("packed", [False, True])
+def test_no_query_heads(packed):
+    """Refused: nothing attends, and torch's operator ends the process on a CPU."""
+    lead, kw = ((10,), dict(offsets=[0, 4, 10])) if packed else ((2, 5), {})
+    q, k = torch.randn(*lead, 0, 16), torch.randn(*lead, 2, 16)
+    for dtype in (torch.float32, torch.bfloat16):
+        with pytest.raises(ValueError, match="heads"):
+            attn.attention(q.to(dtype), k.to(dtype), k.to(dtype), **kw)
+
+
+@pytest.mark.gpu
+def test_no_query_heads_in_the_extension(gen):
+    q, k, _, _ = _inputs(gen, 2, 5, H=0, Hk=2, D=16)
+    with pytest.raises(ValueError, match="heads"):
+        attn.attention(q, k, k)
+    with pytest.raises(RuntimeError, match="heads"):
+        _ext.require().attention(q, k, k, None, False, 0.25)
