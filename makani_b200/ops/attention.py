@@ -82,7 +82,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: bool = 
         offsets = _check_offsets(offsets, q.shape[0], q.device)
         if not native_ok(q, D):
             at = offsets.tolist()
-            parts = [_attend_torch(*(t[None, a:b] for t in (q, k, v)), causal, scale)[0] if b > a else q[a:b] for a, b in zip(at, at[1:])]
+            # (an empty sequence in front: with nothing behind it the result is still a function of the inputs)
+            parts = [_attend_torch(*(t[None, a:b] for t in (q, k, v)), causal, scale)[0] for a, b in [(0, 0)] + [r for r in zip(at, at[1:]) if r[1] > r[0]]]
             return torch.cat(parts + [torch.zeros_like(q[at[-1]:])])
         q, k, v = q[None], k[None], v[None]
     if not native_ok(q, D):

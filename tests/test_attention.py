@@ -463,3 +463,17 @@ def test_no_query_heads_in_the_extension(gen):
         attn.attention(q, k, k)
     with pytest.raises(RuntimeError, match="heads"):
         _ext.require().attention(q, k, k, None, False, 0.25)
+
+
+@pytest.mark.parametrize("dev", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("offsets", [[0], [0, 0], [0, 0, 0]])
+def test_tokens_of_no_sequence_only(dev, offsets, dtype):
+    """Nothing but tokens behind the last sequence: outputs and all gradients are zero."""
+    if dev == "cuda" and not torch.cuda.is_available():
+        pytest.skip("needs a GPU")
+    q, k, v = (torch.full((7, h, 16), float("nan"), device=dev, dtype=dtype, requires_grad=True) for h in (4, 2, 2))
+    o = attn.attention(q, k, v, offsets=offsets)
+    assert o.shape == q.shape and not o.any()
+    for d, t in zip(torch.autograd.grad(o, (q, k, v), torch.ones_like(o)), (q, k, v)):
+        assert d.shape == t.shape and not d.any()
