@@ -133,4 +133,4 @@ class VisionTransformer(nn.Module):
         tokens = self.prepare_tokens(x)
         for blk in self.blocks:
             tokens = blk(tokens)
-        return self.forward_head(self.norm(tokens, operand_dtype(tokens)))
+        return self.forward_head(normed(self.norm, tokens, operand_dtype(tokens)))

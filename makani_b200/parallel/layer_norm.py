@@ -149,6 +149,13 @@ class LayerNorm(nn.LayerNorm):
     """`nn.LayerNorm` over the last dimension, on the kernels of `ops/norm.py`.  As torch's it hands fp32 on under autocast, unless the
     caller names the type: what only feeds a product is wanted in the product's (`operand_dtype`), the same bits as a cast behind it."""
 
+    def plain(self) -> bool:
+        """Whether nobody has to see the call of the module: no hooks, its own or of all modules, and this class's `forward`."""
+        m = nn.modules.module
+        return not (self._forward_hooks or self._forward_pre_hooks or self._backward_hooks or self._backward_pre_hooks or m._global_forward_hooks
+                    or m._global_forward_pre_hooks or m._global_backward_hooks or m._global_backward_pre_hooks
+                    or "forward" in self.__dict__ or type(self).forward is not LayerNorm.forward)
+
     def _dtype(self, x, out_dtype):
         if out_dtype is not None:
             return out_dtype
@@ -163,10 +170,10 @@ class LayerNorm(nn.LayerNorm):
         return norm_ops.layer_norm(x, self.weight, self.bias, self.eps, self._dtype(x, out_dtype))
 
     def after_sum(self, x, residual, out_dtype=None):
-        """(s, norm(s)) with s = x + residual, in one pass over memory."""
-        if len(self.normalized_shape) != 1:
+        """(s, norm(s)) with s = x + residual, in one pass over memory; where the module is watched it is called with the sum, as any other."""
+        if len(self.normalized_shape) != 1 or not self.plain():
             s = x + residual
-            return s, self.forward(s, out_dtype)
+            return s, self(s) if out_dtype is None else normed(self, s, out_dtype)
         if x.shape[-1] != self.normalized_shape[0]:
             raise ValueError(f"layer norm over {self.normalized_shape[0]} channels, got {tuple(x.shape)}")
         s = x if x.dtype == torch.float32 else residual
@@ -174,8 +181,8 @@ class LayerNorm(nn.LayerNorm):
 
 
 def normed(norm: nn.Module, x: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
-    """norm(x) in `dtype`, whatever the norm's class."""
-    return norm(x, dtype) if isinstance(norm, LayerNorm) else norm(x).to(dtype)
+    """norm(x) in `dtype`, whatever the norm's class; hooks see one tensor in and what torch's norm hands on."""
+    return norm(x, dtype) if isinstance(norm, LayerNorm) and norm.plain() else norm(x).to(dtype)
 
 
 class DistributedLayerNorm(nn.Module):

@@ -208,3 +208,54 @@ def test_captured_step_follows_eager_steps(dev):
     _ext.check_device_errors(dev)
     for a, b in zip(eager, replayed):
         assert abs(a - b) < 2e-2 * max(1.0, abs(a)), (eager, replayed)
+
+
+@pytest.mark.parametrize("make", [_vit, _afno])
+def test_hooks_of_every_norm_are_called(make):
+    """Hooks see the calls of a plain module, one tensor in and one out, and may change either; what they see is what the network computes with."""
+    m = make("cpu")
+    x = torch.randn(1, 5, 32, 64)
+    want = m(x)
+    norms = {n: mod for n, mod in m.named_modules() if isinstance(mod, nn.LayerNorm)}
+    assert any("norm2" in n for n in norms)
+    calls = {n: [] for n in norms}
+    handles = []
+    for n, mod in norms.items():
+        handles.append(mod.register_forward_pre_hook(lambda mod, args, n=n: calls[n].append(("pre", len(args), args[0].shape))))
+        handles.append(mod.register_forward_hook(lambda mod, args, y, n=n: calls[n].append(("post", len(args), y.shape))))
+        handles.append(mod.register_full_backward_hook(lambda mod, gi, go, n=n: calls[n].append(("back", len(go), go[0].shape))))
+    y = m(x)
+    assert torch.equal(y, want)
+    y.sum().backward()
+    for n, seen in calls.items():
+        assert [(kind, count) for kind, count, _ in seen] == [("pre", 1), ("post", 1), ("back", 1)], (n, seen)
+        assert len({shape for _, _, shape in seen}) == 1
+    for h in handles:
+        h.remove()
+    second = [mod for n, mod in norms.items() if "norm2" in n]
+    handles = [mod.register_forward_hook(lambda mod, args, y: 2 * y) for mod in second]
+    with torch.no_grad():
+        doubled = m(x)
+        for h in handles:
+            h.remove()
+        for mod in second:
+            mod.weight.mul_(2)
+            mod.bias.mul_(2)
+        assert not torch.equal(doubled, want) and torch.equal(doubled, m(x))
+
+
+def test_a_norm_with_a_forward_of_its_own():
+    from makani_b200.parallel.layer_norm import LayerNorm, normed
+
+    class Shifted(LayerNorm):
+        def forward(self, x, out_dtype=None):
+            return super().forward(x, out_dtype) + 1
+
+    torch.manual_seed(0)
+    m = Shifted(12)
+    x, r = torch.randn(3, 12), torch.randn(3, 12)
+    s, y = m.after_sum(x, r)
+    assert torch.equal(s, x + r) and torch.equal(y, m(x + r))
+    plain = LayerNorm(12)
+    plain.forward = lambda x, out_dtype=None: x * 3
+    assert torch.equal(plain.after_sum(x, r)[1], (x + r) * 3) and torch.equal(normed(plain, x, torch.float32), x * 3)
