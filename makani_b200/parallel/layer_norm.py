@@ -156,10 +156,10 @@ class LayerNorm(nn.LayerNorm):
                     or m._global_forward_pre_hooks or m._global_backward_hooks or m._global_backward_pre_hooks
                     or "forward" in self.__dict__ or type(self).forward is not LayerNorm.forward)
 
-    def _dtype(self, x, out_dtype):
+    def _dtype(self, x, dtype, out_dtype):
         if out_dtype is not None:
             return out_dtype
-        return torch.float32 if x.is_cuda and torch.is_autocast_enabled() and x.dtype != torch.float64 else x.dtype
+        return torch.float32 if x.is_cuda and torch.is_autocast_enabled() and dtype != torch.float64 else dtype
 
     def forward(self, x, out_dtype=None):
         if len(self.normalized_shape) != 1:
@@ -167,7 +167,7 @@ class LayerNorm(nn.LayerNorm):
             return y if out_dtype is None else y.to(out_dtype)
         if x.shape[-1] != self.normalized_shape[0]:
             raise ValueError(f"layer norm over {self.normalized_shape[0]} channels, got {tuple(x.shape)}")
-        return norm_ops.layer_norm(x, self.weight, self.bias, self.eps, self._dtype(x, out_dtype))
+        return norm_ops.layer_norm(x, self.weight, self.bias, self.eps, self._dtype(x, x.dtype, out_dtype))
 
     def after_sum(self, x, residual, out_dtype=None):
         """(s, norm(s)) with s = x + residual, in one pass over memory; where the module is watched it is called with the sum, as any other."""
@@ -176,8 +176,8 @@ class LayerNorm(nn.LayerNorm):
             return s, self(s) if out_dtype is None else normed(self, s, out_dtype)
         if x.shape[-1] != self.normalized_shape[0]:
             raise ValueError(f"layer norm over {self.normalized_shape[0]} channels, got {tuple(x.shape)}")
-        s = x if x.dtype == torch.float32 else residual
-        return norm_ops.add_layer_norm(x, residual, self.weight, self.bias, self.eps, self._dtype(s, out_dtype))
+        dtype = torch.promote_types(x.dtype, residual.dtype)
+        return norm_ops.add_layer_norm(x, residual, self.weight, self.bias, self.eps, self._dtype(x, dtype, out_dtype))
 
 
 def normed(norm: nn.Module, x: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:

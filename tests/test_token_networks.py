@@ -259,3 +259,14 @@ def test_a_norm_with_a_forward_of_its_own():
     plain = LayerNorm(12)
     plain.forward = lambda x, out_dtype=None: x * 3
     assert torch.equal(plain.after_sum(x, r)[1], (x + r) * 3) and torch.equal(normed(plain, x, torch.float32), x * 3)
+
+
+def test_sums_in_the_wider_type_stay_there():
+    """`after_sum` of two types hands on what the sum's type is, whichever of the two has it."""
+    from makani_b200.parallel.layer_norm import LayerNorm
+    m = LayerNorm(12)
+    for a, b in ((torch.float64, torch.float32), (torch.float32, torch.float64), (torch.float64, torch.bfloat16), (torch.bfloat16, torch.float32),
+                 (torch.float32, torch.float16), (torch.float16, torch.bfloat16)):
+        wide = torch.promote_types(a, b)
+        s, y = m.after_sum(torch.randn(3, 12).to(a), torch.randn(3, 12).to(b))
+        assert s.dtype == y.dtype == wide, (a, b, s.dtype, y.dtype)
