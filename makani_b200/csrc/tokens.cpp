@@ -184,12 +184,23 @@ std::tuple<Tensor, OptTensor, OptTensor, OptTensor> layer_norm_backward(const Te
   return {dx, maybe(dr), maybe(dw), maybe(db)};
 }
 
+// The same in torch's operations, for gradients that are to be differentiated in their turn: (dx, dweight, dbias) in fp32, dx with `ds`
+std::tuple<Tensor, Tensor, Tensor> layer_norm_backward_graph(const Tensor& x, const Tensor& dy, const Tensor& ds, const Tensor& weight, double eps) {
+  const Tensor xf = x.to(at::kFloat), dyf = dy.to(at::kFloat), off = xf - xf.mean(-1, true);
+  const Tensor rstd = ((off * off).mean(-1, true) + eps).rsqrt(), xh = off * rstd, g = weight.defined() ? dyf * weight.to(at::kFloat) : dyf;
+  Tensor dx = rstd * (g - g.mean(-1, true) - xh * (g * xh).mean(-1, true));
+  if (ds.defined()) dx = dx + ds.to(at::kFloat);
+  const int64_t C = x.size(-1), rows = x.numel() / C;
+  return {dx, (dyf * xh).reshape({rows, C}).sum(0), dyf.reshape({rows, C}).sum(0)};
+}
+
 struct LayerNorm : torch::autograd::Function<LayerNorm> {
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const OptTensor& residual, const OptTensor& weight, const OptTensor& bias, double eps,
                                bool out_f32, bool train) {
     auto [s, y, stats, w] = layer_norm_forward(x, residual, weight, bias, eps, out_f32, train);
     if (train) {
-      ctx->save_for_backward({s.has_value() ? *s : x, value(w), *stats});
+      ctx->save_for_backward({s.has_value() ? *s : x, value(w), *stats, value(weight)});
+      ctx->saved_data["eps"] = eps;
       ctx->saved_data["weight"] = value(weight).defined();
       ctx->saved_data["bias"] = value(bias).defined();
       ctx->saved_data["added"] = s.has_value();
@@ -214,14 +225,23 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     if (!dy.defined()) {
       if (need_x) out[0] = ds;
       if (need_r && ds.defined()) out[1] = half ? ds.to(at::kBFloat16) : ds;
-      return once_differentiable(std::move(out));
+      return out;
+    }
+    if (at::GradMode::is_enabled()) {      // (create_graph)
+      const Tensor& x = saved[0];
+      auto [dx, dw, db] = layer_norm_backward_graph(x, dy, ds, saved[3], ctx->saved_data["eps"].toDouble());
+      if (need_x) out[0] = dx.to(x.scalar_type());
+      if (need_r) out[1] = dx.to(half ? at::kBFloat16 : x.scalar_type());
+      if (need_w) out[2] = dw;
+      if (need_b) out[3] = db;
+      return out;
     }
     auto [dx, dr, dw, db] = layer_norm_backward(saved[0], dy, maybe(ds), maybe(saved[1]), saved[2], need_w || need_b, half && need_r);
     if (need_x) out[0] = dx;
     if (need_r) out[1] = half ? *dr : dx;
     if (need_w) out[2] = *dw;
     if (need_b) out[3] = *db;
-    return once_differentiable(std::move(out));
+    return out;
   }
 };
 

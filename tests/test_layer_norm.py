@@ -311,3 +311,44 @@ def test_kernels_are_counted(gen):
     before = _ext.launch_count()
     norm_ops.layer_norm(x, torch.ones(64, device="cuda", requires_grad=True), None).sum().backward()
     assert _ext.launch_count() > before
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("xt,wt", [(torch.float32, torch.float32), (torch.float32, torch.bfloat16), (torch.bfloat16, torch.float32)])
+def test_second_derivatives(gen, residual, xt, wt):
+    """Gradients that are differentiated once more, against 64 bits.  A first gradient in fp32 is known to E = SUM U of the magnitudes it is made of; a second one
+    is made of products of some four such quantities, sums of them, and one sum more over the rows for the weight: 16 E = 6.1e-5 of its norm.  In bf16 the
+    first gradient is rounded, as torch's is, and what comes back through that rounding too: three roundings of half a step."""
+    C, rows = 40, 9
+    x = _tokens(gen, rows, C, dtype=xt).requires_grad_()
+    r = _tokens(gen, rows, C, dtype=xt).requires_grad_() if residual else None
+    w = (1 + 0.2 * torch.randn(C, device="cuda", generator=gen)).to(wt).requires_grad_()
+    b = torch.zeros(C, device="cuda", dtype=wt, requires_grad=True)
+    dy = torch.randn(rows, C, device="cuda", generator=gen).to(xt).requires_grad_()
+    ds = torch.randn(rows, C, device="cuda", generator=gen).to(xt)
+    tx, tw, tb = (torch.randn(s, device="cuda", generator=gen) for s in ((rows, C), (C,), (C,)))
+
+    def second(f, x, r, w, b, dy, ds):
+        s, y = f(x, r, w, b)
+        first = torch.autograd.grad((s, y) if residual else y, (x, w, b), (ds, dy) if residual else dy, create_graph=True)
+        work = torch.promote_types(s.dtype, torch.float32)
+        score = sum((g.to(work) * t.to(work)).sum() for g, t in zip(first, (tx, tw, tb)))
+        leaves = [t for t in (x, r, w, dy) if t is not None]
+        return torch.autograd.grad(score, leaves)
+
+    def own(x, r, w, b):
+        return norm_ops.add_layer_norm(x, r, w, b, 1e-5, xt) if residual else (x, norm_ops.layer_norm(x, w, b, 1e-5, xt))
+
+    def definition(x, r, w, b):
+        s = x + r if residual else x
+        if residual and xt == torch.bfloat16:
+            s = s + (s.detach().bfloat16().double() - s.detach())       # the sum is rounded; its gradient is not
+        mean = s.mean(-1, keepdim=True)
+        return s, (s - mean) / torch.sqrt(((s - mean) ** 2).mean(-1, keepdim=True) + 1e-5) * w + b
+
+    got = second(own, x, r, w, b, dy, ds)
+    want = second(definition, *(None if t is None else t.detach().double().requires_grad_() for t in (x, r, w, b, dy)), ds.double())
+    for g, t in zip(got, want):
+        off = 16 * SUM * U + (3 * _half_step(torch.bfloat16) if torch.bfloat16 in (xt, wt) else 0)
+        assert (g.double() - t).norm() <= off * t.norm(), (g.shape, float((g.double() - t).norm() / t.norm()))
