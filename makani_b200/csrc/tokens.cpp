@@ -37,6 +37,19 @@ bool records(std::initializer_list<const Tensor*> ts) {
   return any && at::GradMode::is_enabled();
 }
 
+// Whether these tensors are no more than their memory and their autograd graph, so that kernels may take them.  Not so in `torch.func`'s transforms,
+// forward-mode differentiation, tracing and dispatch modes, and for subclasses: what stands for a tensor there has no memory, or somebody has to see each
+// operation.
+bool plain(std::initializer_list<const Tensor*> ts) {
+  using K = c10::DispatchKey;
+  const c10::DispatchKeySet watched({K::Python, K::PythonTLSSnapshot, K::Tracer, K::FuncTorchDynamicLayerFrontMode, K::Functionalize});
+  const c10::DispatchKeySet wrapped({K::Python, K::FuncTorchGradWrapper, K::FuncTorchBatched, K::Functionalize});
+  if (c10::impl::tls_local_dispatch_key_set().included_.has_any(watched)) return false;
+  for (const Tensor* t : ts)
+    if (t->defined() && (t->key_set().has_any(wrapped) || t->_fw_grad(0).defined())) return false;
+  return true;
+}
+
 // Launches of backward passes, which autograd runs in threads of its own
 std::atomic<int64_t> background{0};
 struct Backward {
@@ -245,8 +258,10 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
   }
 };
 
+// (s and) y; nothing where the tensors are not for kernels
 variable_list layer_norm(const Tensor& x, const OptTensor& residual, const OptTensor& weight, const OptTensor& bias, double eps, bool out_f32) {
   const Tensor r = value(residual), w = value(weight), b = value(bias);
+  if (!plain({&x, &r, &w, &b})) return {};
   return LayerNorm::apply(x, residual, weight, bias, eps, out_f32, records({&x, &r, &w, &b}));
 }
 

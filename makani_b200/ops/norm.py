@@ -184,7 +184,7 @@ def _check_layer_norm(x, residual, weight, bias, out_dtype):
 
 
 def _layer_norm_native(x, out_dtype) -> bool:
-    return _ext.native() and x.is_cuda and x.dtype in _LN_TYPES and out_dtype in _LN_TYPES and x.shape[-1] <= LN_CHANNELS
+    return _ext.native() and x.is_cuda and x.dtype in _LN_TYPES and out_dtype in _LN_TYPES and x.shape[-1] <= LN_CHANNELS and not torch.compiler.is_compiling()
 
 
 def _layer_norm_torch(x, weight, bias, eps, out_dtype):
@@ -201,11 +201,14 @@ def layer_norm(x: torch.Tensor, weight, bias, eps: float = 1e-5, out_dtype: Opti
     `out_dtype` (default: that of x).  `weight` and `bias` [C] or None.
 
     CUDA tensors in bf16 or fp32 of up to 8192 channels run on one kernel in either direction, whose rows may be strided in two levels (the
-    queries of a fused projection, [B, N, heads, D] out of [B, N, 3, heads, D]); the rest on the torch op."""
+    queries of a fused projection, [B, N, heads, D] out of [B, N, 3, heads, D]); the rest, and what `torch.func`, forward-mode differentiation, tracing
+    or compilation calls, on the torch op."""
     _check_layer_norm(x, None, weight, bias, out_dtype)
     out_dtype = out_dtype or x.dtype
     if _layer_norm_native(x, out_dtype):
-        return _ext.require().layer_norm(x, None, weight, bias, eps, out_dtype is torch.float32)[0]
+        out = _ext.require().layer_norm(x, None, weight, bias, eps, out_dtype is torch.float32)
+        if out:      # (nothing: the call is a transform's, a trace's or a mode's)
+            return out[0]
     return _layer_norm_torch(x, weight, bias, eps, out_dtype)
 
 
@@ -218,6 +221,8 @@ def add_layer_norm(x: torch.Tensor, residual: torch.Tensor, weight, bias, eps: f
     dtype = torch.promote_types(x.dtype, residual.dtype)
     out_dtype = out_dtype or dtype
     if _layer_norm_native(x, out_dtype) and residual.dtype in _LN_TYPES:
-        return tuple(_ext.require().layer_norm(x, residual, weight, bias, eps, out_dtype is torch.float32))
+        out = _ext.require().layer_norm(x, residual, weight, bias, eps, out_dtype is torch.float32)
+        if out:
+            return tuple(out)
     s = x + residual
     return s, _layer_norm_torch(s, weight, bias, eps, out_dtype)

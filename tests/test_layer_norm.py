@@ -352,3 +352,34 @@ def test_second_derivatives(gen, residual, xt, wt):
     for g, t in zip(got, want):
         off = 16 * SUM * U + (3 * _half_step(torch.bfloat16) if torch.bfloat16 in (xt, wt) else 0)
         assert (g.double() - t).norm() <= off * t.norm(), (g.shape, float((g.double() - t).norm() / t.norm()))
+
+
+@pytest.mark.gpu
+def test_transforms_see_through_the_norms(gen):
+    """vmap, forward mode, tracing, compilation and fake tensors go by torch's operations, as with `nn.LayerNorm`."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+    x, d, r = (torch.randn(4, 6, 24, device="cuda", generator=gen) for _ in range(3))
+    w, b = torch.randn(24, device="cuda", generator=gen), torch.randn(24, device="cuda", generator=gen)
+    own = lambda t: norm_ops.layer_norm(t, w, b)  # noqa: E731
+    added = lambda t: norm_ops.add_layer_norm(t, r[0] if t.dim() == 2 else r, w, b)[1]  # noqa: E731
+    plain = lambda t: torch.nn.functional.layer_norm(t, (24,), w, b)  # noqa: E731
+    near = lambda p, q: torch.allclose(p, q, rtol=1e-5, atol=1e-5)  # noqa: E731
+    assert near(torch.func.vmap(own)(x), plain(x))
+    assert near(torch.func.vmap(added)(x), plain(x + r[0]))
+    assert near(torch.func.jacrev(lambda t: own(t).sum(0))(x[0, 0][None]), torch.func.jacrev(lambda t: plain(t).sum(0))(x[0, 0][None]))
+    for f, g in ((own, plain), (added, lambda t: plain(t + r))):
+        y, dy = torch.func.jvp(f, (x,), (d,))
+        y0, dy0 = torch.func.jvp(g, (x,), (d,))
+        assert near(y, y0) and near(dy, dy0)
+        with torch.autograd.forward_ad.dual_level():
+            dual = torch.autograd.forward_ad.make_dual(x, d)
+            assert near(torch.autograd.forward_ad.unpack_dual(f(dual)).tangent, dy0)
+        traced = torch.jit.trace(f, (x,))
+        assert near(traced(d), g(d))
+        assert near(torch.compile(f, backend="eager", fullgraph=True)(d), g(d))
+        assert near(make_fx(f)(x)(d), g(d))
+    with FakeTensorMode(allow_non_fake_inputs=True) as mode:
+        fake = mode.from_tensor(x)
+        y = norm_ops.layer_norm(fake, None, None)
+    assert y.shape == x.shape
