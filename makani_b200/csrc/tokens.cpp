@@ -375,7 +375,10 @@ struct Attention : torch::autograd::Function<Attention> {
   }
 };
 
-Tensor attention(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& offsets, bool causal, double scale) {
+// (o; nothing where the tensors are not for kernels)
+OptTensor attention(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& offsets, bool causal, double scale) {
+  const Tensor at = value(offsets);
+  if (!plain({&q, &k, &v, &at})) return {};
   return Attention::apply(q, k, v, offsets, causal, scale, records({&q, &k, &v}));
 }
 
@@ -418,7 +421,9 @@ struct AttentionQkv : torch::autograd::Function<AttentionQkv> {
   }
 };
 
-Tensor attention_qkv(const Tensor& qkv, int64_t heads, int64_t kv_heads, const OptTensor& offsets, bool causal, double scale) {
+OptTensor attention_qkv(const Tensor& qkv, int64_t heads, int64_t kv_heads, const OptTensor& offsets, bool causal, double scale) {
+  const Tensor at = value(offsets);
+  if (!plain({&qkv, &at})) return {};
   return AttentionQkv::apply(qkv, heads, kv_heads, offsets, causal, scale, records({&qkv}));
 }
 

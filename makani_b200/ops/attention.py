@@ -10,7 +10,7 @@ not checked (out of range they are clamped to it).  Tokens behind offsets[S] bel
 zero, and what their inputs hold reaches nothing.
 
 bf16 CUDA tensors of up to 128 channels a head run on the in-tree kernels (widths that are no multiple of 8 are padded with zeros);
-anything else through torch.  Weights and their gradients are rounded to bf16 where they are operands of the second products; all sums
+anything else, and what `torch.func`, forward-mode differentiation, tracing or compilation calls, through torch.  Weights and their gradients are rounded to bf16 where they are operands of the second products; all sums
 are fp32.  A key that a causal mask hides has no weight, but its value has to be finite.
 """
 
@@ -27,7 +27,7 @@ WIDTH = 128          # most channels of a head in the kernels
 
 
 def native_ok(x: torch.Tensor, head_dim: int) -> bool:
-    return _ext.native() and x.is_cuda and x.dtype == torch.bfloat16 and 0 < head_dim <= WIDTH
+    return _ext.native() and x.is_cuda and x.dtype == torch.bfloat16 and 0 < head_dim <= WIDTH and not torch.compiler.is_compiling()
 
 
 def _check_offsets(offsets, tokens: int, device):
@@ -52,12 +52,17 @@ def _check_scale(scale, head_dim: int) -> float:
     return scale
 
 
-def _attend_torch(q, k, v, causal, scale):
-    """[B, N, heads, D] through the library."""
+def _attend_torch(q, k, v, causal, scale, offsets=None):
+    """[B, N, heads, D], or packed [T, heads, D], through the library."""
+    if offsets is not None:
+        at = offsets.tolist()
+        # (an empty sequence in front: with nothing behind it the result is still a function of the inputs)
+        parts = [_attend_torch(*(t[None, a:b] for t in (q, k, v)), causal, scale)[0] for a, b in [(0, 0)] + [r for r in zip(at, at[1:]) if r[1] > r[0]]]
+        return torch.cat(parts + [torch.zeros_like(q[at[-1]:])])
     q, k, v = (t.transpose(1, 2) for t in (q, k, v))
     if k.shape[1] != q.shape[1]:
-        k, v = (t.repeat_interleave(q.shape[1] // t.shape[1], dim=1) for t in (k, v))
-    return torch.nn.functional.scaled_dot_product_attention(q, k, v, is_causal=causal, scale=scale).transpose(1, 2)
+        k, v = (t.repeat_interleave(int(q.shape[1] // t.shape[1]), dim=1) for t in (k, v))      # (a trace has tensors for sizes)
+    return torch.nn.functional.scaled_dot_product_attention(q, k, v, is_causal=causal, scale=scale).transpose(1, 2).contiguous()
 
 
 def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: bool = False, scale: Optional[float] = None,
@@ -80,18 +85,15 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: bool = 
     scale = _check_scale(scale, D)
     if packed:
         offsets = _check_offsets(offsets, q.shape[0], q.device)
-        if not native_ok(q, D):
-            at = offsets.tolist()
-            # (an empty sequence in front: with nothing behind it the result is still a function of the inputs)
-            parts = [_attend_torch(*(t[None, a:b] for t in (q, k, v)), causal, scale)[0] for a, b in [(0, 0)] + [r for r in zip(at, at[1:]) if r[1] > r[0]]]
-            return torch.cat(parts + [torch.zeros_like(q[at[-1]:])])
-        q, k, v = q[None], k[None], v[None]
     if not native_ok(q, D):
-        return _attend_torch(q, k, v, causal, scale).contiguous()
+        return _attend_torch(q, k, v, causal, scale, offsets)
+    views = (t[None] for t in (q, k, v)) if packed else (q, k, v)
     more = -D % 8
     if more:
-        q, k, v = (torch.nn.functional.pad(t, (0, more)) for t in (q, k, v))
-    o = _ext.require().attention(q, k, v, offsets, causal, scale)
+        views = (torch.nn.functional.pad(t, (0, more)) for t in views)
+    o = _ext.require().attention(*views, offsets, causal, scale)
+    if o is None:      # (the call is a transform's, a trace's or a mode's)
+        return _attend_torch(q, k, v, causal, scale, offsets)
     if more:
         o = o[..., :D].contiguous()
     return o[0] if packed else o
@@ -110,11 +112,12 @@ def attention_qkv(qkv: torch.Tensor, num_heads: int, num_kv_heads: Optional[int]
     if qkv.shape[-1] < 1 or qkv.shape[-1] % (num_heads + 2 * Hk):
         raise ValueError(f"{qkv.shape[-1]} channels are not those of {num_heads} + 2 x {Hk} heads")
     D = qkv.shape[-1] // (num_heads + 2 * Hk)
-    if not native_ok(qkv, D) or D % 8:
-        q, k, v = qkv.unflatten(-1, (num_heads + 2 * Hk, D)).split([num_heads, Hk, Hk], dim=-2)
-        return attention(q, k, v, causal, scale, offsets)
-    scale = _check_scale(scale, D)
-    if not packed:
-        return _ext.require().attention_qkv(qkv, num_heads, Hk, None, causal, scale)
-    offsets = _check_offsets(offsets, qkv.shape[0], qkv.device)
-    return _ext.require().attention_qkv(qkv[None], num_heads, Hk, offsets, causal, scale)[0]
+    if native_ok(qkv, D) and D % 8 == 0:
+        scale = _check_scale(scale, D)
+        if packed:
+            offsets = _check_offsets(offsets, qkv.shape[0], qkv.device)
+        o = _ext.require().attention_qkv(qkv[None] if packed else qkv, num_heads, Hk, offsets, causal, scale)
+        if o is not None:
+            return o[0] if packed else o
+    q, k, v = qkv.unflatten(-1, (num_heads + 2 * Hk, D)).split([num_heads, Hk, Hk], dim=-2)
+    return attention(q, k, v, causal, scale, offsets)

@@ -477,3 +477,24 @@ def test_tokens_of_no_sequence_only(dev, offsets, dtype):
     assert o.shape == q.shape and not o.any()
     for d, t in zip(torch.autograd.grad(o, (q, k, v), torch.ones_like(o)), (q, k, v)):
         assert d.shape == t.shape and not d.any()
+
+
+@pytest.mark.gpu
+def test_transforms_see_through_attention(gen):
+    """vmap, tracing, compilation and fake tensors go by torch's operations.  Outputs are bf16 of either side: two roundings of weights and of the result."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    q, k, v, _ = _inputs(gen, 3, 20, H=2, Hk=1, D=16)
+    other = _inputs(gen, 3, 20, H=2, Hk=1, D=16)[:3]
+    own = lambda q, k, v: attn.attention(q, k, v, causal=True)  # noqa: E731
+    near = lambda p, t: float((p.double() - t.double()).norm() / t.double().norm()) < 4 * B_STEP  # noqa: E731
+    want = own(q, k, v)
+    assert near(torch.func.vmap(lambda *t: own(*(x[None] for x in t))[0])(q, k, v), want)
+    traced = torch.jit.trace(own, (q, k, v))
+    assert near(traced(*other), own(*other))
+    assert near(torch.compile(own, backend="eager", fullgraph=True)(*other), own(*other))
+    x = torch.cat([t.flatten(2) for t in (q, k, v)], -1)
+    traced = torch.jit.trace(lambda t: attn.attention_qkv(t, 2, 1, True), (x,))
+    assert near(traced(x.flip(0)), attn.attention_qkv(x.flip(0), 2, 1, True))
+    with FakeTensorMode() as mode:
+        y = own(*(mode.from_tensor(t) for t in (q, k, v)))
+    assert y.shape == q.shape
