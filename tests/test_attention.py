@@ -498,3 +498,115 @@ def test_transforms_see_through_attention(gen):
     with FakeTensorMode() as mode:
         y = own(*(mode.from_tensor(t) for t in (q, k, v)))
     assert y.shape == q.shape
+
+
+# What `one_tile_pays` gives to the forward kernels of one query tile (more pairs of tiles than SMs, short sequences), with several tiles of keys
+@pytest.mark.gpu
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("B,N,H,Hk,D", [(32, 384, 8, 8, 64), (20, 440, 8, 2, 128), (16, 768, 8, 4, 48), (27, 257, 6, 6, 72), (160, 129, 1, 1, 24)])
+def test_short_sequences_of_several_tiles(gen, B, N, H, Hk, D, causal):
+    q, k, v, do = _inputs(gen, B, N, H=H, Hk=Hk, D=D)
+    k = (k.float() * torch.linspace(0.3, 3, N, device="cuda")[None, :, None, None]).bfloat16()      # maxima grow along the keys
+    got = _run(q, k, v, do, causal=causal)
+    torch.cuda.synchronize()
+    _ext.check_device_errors()
+    for b in (0, 1, B // 2, B - 1):
+        want, off = _oracle(q[b], k[b], v[b], do[b], causal, D ** -0.5, [(0, N)])
+        for n in want:
+            _close(got[n][b], want[n], off[n], f"{n} of sample {b}")
+    alone = _run(*(t[:1] for t in (q, k, v, do)), causal=causal)                   # few CTAs: another kernel, the same rows but for the order of sums
+    want, off = _oracle(q[0], k[0], v[0], do[0], causal, D ** -0.5, [(0, N)])
+    for n in want:
+        _close(alone[n][0], want[n], off[n], n)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("H,Hk,D", [(8, 8, 64), (6, 2, 96), (8, 4, 40)])
+def test_many_packed_sequences_of_several_tiles(gen, H, Hk, D, causal):
+    lens = [130 + (97 * i) % 271 for i in range(40)] + [0, 1, 400]
+    at = [0]
+    for n in lens:
+        at.append(at[-1] + n)
+    T = at[-1] + 77
+    q, k, v, do = _inputs(gen, T, H=H, Hk=Hk, D=D)
+    for t in (q, k, v, do):
+        t[at[-1]:] = float("nan")
+    offsets = torch.tensor(at, dtype=torch.int32, device="cuda")
+    got = _run(q, k, v, do, causal=causal, offsets=offsets)
+    torch.cuda.synchronize()
+    _ext.check_device_errors()
+    want, off = _oracle(q, k, v, do, causal, D ** -0.5, list(zip(at, at[1:])))
+    for n in want:
+        _close(got[n], want[n], off[n], n)
+        assert not got[n][at[-1]:].any()
+    keep = torch.zeros(T, dtype=torch.bool, device="cuda")
+    for i in range(0, len(lens), 2):
+        keep[at[i]:at[i + 1]] = True
+    for t, bad in zip((q, k, v, do), (float("nan"), float("inf"), float("nan"), float("-inf"))):
+        t[~keep] = bad
+    again = _run(q, k, v, do, causal=causal, offsets=offsets)
+    for n in want:
+        assert torch.equal(again[n][keep], got[n][keep]), n
+
+
+def _kinds(g, B, N, H, D, device, kinds=5):
+    """Queries and keys of a few kinds, so far apart that a query has the same weight for all visible keys of its kind and none for others: the only score that is
+    not 0 is 2048, whose product with any scale and whose difference from itself are exact.  Weights are 1 before they are divided, and sums of the values
+    exact in fp32.  Values are 64 and something, output gradients 1 and something: delta is a sum of large parts, dS a small difference."""
+    kq, kk = (torch.randint(0, kinds, (B, N, H), device=device, generator=g) for _ in range(2))
+    kq[:, :kinds] = kk[:, :kinds] = torch.arange(kinds, device=device)[None, :, None]       # (each query sees a key of its kind)
+    one = torch.nn.functional.one_hot
+    v, do = (c + torch.randn(B, N, H, D, device=device, generator=g) for c in (64, 1))
+    return (2048 * one(kq, D)).bfloat16(), one(kk, D).bfloat16(), v.bfloat16(), do.bfloat16()
+
+
+def _kinds_oracle(q, k, v, do, causal):
+    """64-bit outputs and bounds of a sample [N, H, D] of `_kinds`.
+
+    o: sums are exact, the quotient off by 2^-21.  What is kept of o is its rounding and the rounding of the rest, off by B^2 = 2^-16 of o: delta by
+    (2^-16 + 2^-21 + D 2^-24) sum |do o|, below 2^-15 of it.  L is some 370 at most and rounded by 2^-16, P by 2^-16 for it and 2^-18 for the exponential
+    (a polynomial within 2.7e-6, or two steps of fp32): they are factors of dS.  dS is rounded to bf16."""
+    scale, N, e = q.shape[-1] ** -0.5, q.shape[0], 2.0 ** -16 + 2.0 ** -18
+    q, k, v, do = (t.double().transpose(0, 1) for t in (q, k, v, do))
+    s = q @ k.mT * scale
+    if causal:
+        s = s.masked_fill(torch.ones(N, N, dtype=torch.bool, device=s.device).triu(1), -math.inf)
+    p = torch.softmax(s, -1)
+    o = p @ v
+    delta, size = ((t * u).sum(-1, keepdim=True) for t, u in ((do, o), (do.abs(), o.abs())))
+    ds = p * (do @ v.mT - delta)
+    ds_off = (B_STEP + e) * ds.abs() + p * (2.0 ** -15 * size + F_STEP * (do.abs() @ v.abs().mT))
+    want = dict(o=o, dq=scale * ds @ k, dk=scale * ds.mT @ q, dv=p.mT @ do)
+    off = dict(o=2.0 ** -21 * o.abs(), dq=scale * (ds_off + F_STEP * ds.abs()) @ k.abs(), dk=scale * (ds_off + F_STEP * ds.abs()).mT @ q.abs(),
+               dv=((B_STEP + e) * p).mT @ do.abs())
+    return {n: t.transpose(0, 1) for n, t in want.items()}, {n: t.transpose(0, 1) for n, t in off.items()}, (p, o, delta)
+
+
+@pytest.mark.parametrize("N,D", [(300, 64), (384, 96)])
+def test_bounds_tell_a_rounded_output_apart(N, D):
+    """The gradients of queries with delta from the rounded output alone, or with what the rounding left of the row beside it, are outside the bounds."""
+    q, k, v, do = (t[0] for t in _kinds(torch.Generator().manual_seed(3), 1, N, 2, D, "cpu"))
+    want, off, (p, o, delta) = _kinds_oracle(q, k, v, do, False)
+    d64, k64 = do.double().transpose(0, 1), k.double().transpose(0, 1)
+    low = o.bfloat16().double()
+    rest = (o - low).bfloat16().double()
+    outside = lambda kept: float((((D ** -0.5 * p * (d64 @ v.double().transpose(0, 1).mT - (d64 * kept).sum(-1, keepdim=True))) @ k64).transpose(0, 1)  # noqa: E731
+                                  - want["dq"]).abs().gt(off["dq"] + B_STEP * want["dq"].abs()).any(-1).double().mean())
+    assert outside(low + rest) == 0
+    assert outside(low) > 0.5 and outside(low + rest.roll(1, 1)) > 0.4
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("B,N,H,D", [(1, 300, 2, 64), (2, 300, 2, 96), (32, 384, 8, 64), (20, 440, 8, 96), (1, 2500, 2, 64), (1, 2500, 1, 96), (1, 1030, 1, 40)])
+def test_delta_holds_what_the_output_lost(gen, B, N, H, D, causal):
+    """Whole, of one query tile to a CTA, and split over the keys and joined: the gradients need o to 16 bits."""
+    q, k, v, do = _kinds(gen, B, N, H, D, "cuda")
+    got = _run(q, k, v, do, causal=causal)
+    torch.cuda.synchronize()
+    _ext.check_device_errors()
+    for b in sorted({0, B // 2, B - 1}):
+        want, off, _ = _kinds_oracle(q[b], k[b], v[b], do[b], causal)
+        for n in want:
+            _close(got[n][b], want[n], off[n], f"{n} of sample {b}")

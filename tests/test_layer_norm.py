@@ -383,3 +383,26 @@ def test_transforms_see_through_the_norms(gen):
         fake = mode.from_tensor(x)
         y = norm_ops.layer_norm(fake, None, None)
     assert y.shape == x.shape
+
+
+# Groups that go over three rows or sets of rows and more, the last turn ragged
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,C", [(10007, 384), (5003, 1024), (2501, 387), (40001, 48), (20011, 120), (1501, 2056), (701, 2051), (1203, 8192)])
+@pytest.mark.parametrize("xt,rt,yt", [(torch.bfloat16, torch.bfloat16, torch.bfloat16), (torch.bfloat16, torch.bfloat16, torch.float32),
+                                      (torch.float32, torch.bfloat16, torch.bfloat16), (torch.float32, torch.bfloat16, torch.float32),
+                                      (torch.float32, torch.float32, torch.bfloat16), (torch.float32, torch.float32, torch.float32)])
+def test_add_layer_norm_of_several_turns(gen, rows, C, xt, rt, yt):
+    x, r = _tokens(gen, rows, C, dtype=xt), _tokens(gen, rows, C, dtype=rt)
+    dy, ds = torch.randn(rows, C, device="cuda", generator=gen).to(yt), torch.randn(rows, C, device="cuda", generator=gen).to(xt)
+    w, b = 1 + 0.2 * torch.randn(C, device="cuda", generator=gen), 0.2 * torch.randn(C, device="cuda", generator=gen)
+    _check(x, w, b, dy, yt, residual=r, ds=ds)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,C", [(15001, 384), (7001, 1024), (3001, 387), (60001, 40), (2003, 2056)])
+@pytest.mark.parametrize("xt,yt", [(torch.bfloat16, torch.bfloat16), (torch.float32, torch.bfloat16), (torch.float32, torch.float32),
+                                   (torch.bfloat16, torch.float32)])
+def test_layer_norm_of_several_turns(gen, rows, C, xt, yt):
+    x, dy = _tokens(gen, rows, C, dtype=xt), torch.randn(rows, C, device="cuda", generator=gen).to(yt)
+    w, b = 1 + 0.2 * torch.randn(C, device="cuda", generator=gen), 0.2 * torch.randn(C, device="cuda", generator=gen)
+    _check(x, w, b, dy, yt)
