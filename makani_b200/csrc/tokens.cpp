@@ -4,6 +4,8 @@
 
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/saved_variable.h>
 
 #include <pybind11/stl.h>
 
@@ -108,7 +110,7 @@ Tensor channel_f32(const OptTensor& t, const Tensor& x, const char* what) {
   if (!t.has_value() || !t->defined()) return Tensor();
   MK_CHECK(t->device() == x.device(), "layer norm: tensors must be on one CUDA device");
   MK_CHECK(t->dim() == 1 && t->size(0) == x.size(-1), "layer norm: one ", what, " per channel expected");
-  return t->detach().to(at::kFloat).contiguous();
+  return is_f32(*t) && t->is_contiguous() ? *t : t->detach().to(at::kFloat).contiguous();
 }
 
 // (s, y, statistics, weight in fp32): s and the statistics where they are asked for
@@ -167,9 +169,8 @@ std::tuple<Tensor, OptTensor, OptTensor, OptTensor> layer_norm_backward(const Te
   if (half_copy) dr = at::empty(x.sizes(), x.options().dtype(at::kBFloat16));
   if (need_params) {
     // (no rows: no kernel that writes them)
-    const Tensor both = in.rows ? at::empty({2, in.C}, x.options().dtype(at::kFloat)) : at::zeros({2, in.C}, x.options().dtype(at::kFloat));
-    dw = both.select(0, 0);
-    db = both.select(0, 1);
+    dw = in.rows ? at::empty({in.C}, x.options().dtype(at::kFloat)) : at::zeros({in.C}, x.options().dtype(at::kFloat));
+    db = in.rows ? at::empty_like(dw) : at::zeros_like(dw);
     const int64_t n = mk::layer_norm_scratch(in.rows, static_cast<int>(in.C));
     if (n) part = at::empty({n}, x.options().dtype(at::kFloat));
   }
@@ -207,49 +208,40 @@ std::tuple<Tensor, Tensor, Tensor> layer_norm_backward_graph(const Tensor& x, co
   return {dx, (dyf * xh).reshape({rows, C}).sum(0), dyf.reshape({rows, C}).sum(0)};
 }
 
-struct LayerNorm : torch::autograd::Function<LayerNorm> {
-  static variable_list forward(AutogradContext* ctx, const Tensor& x, const OptTensor& residual, const OptTensor& weight, const OptTensor& bias, double eps,
-                               bool out_f32, bool train) {
-    auto [s, y, stats, w] = layer_norm_forward(x, residual, weight, bias, eps, out_f32, train);
-    if (train) {
-      ctx->save_for_backward({s.has_value() ? *s : x, value(w), *stats, value(weight)});
-      ctx->saved_data["eps"] = eps;
-      ctx->saved_data["weight"] = value(weight).defined();
-      ctx->saved_data["bias"] = value(bias).defined();
-      ctx->saved_data["added"] = s.has_value();
-      // a residual in bf16 beside an fp32 x takes its gradient in its own type
-      ctx->saved_data["half"] = s.has_value() && residual->scalar_type() != x.scalar_type();
-      ctx->set_materialize_grads(false);
-    }
-    if (s.has_value()) return {*s, y};
-    return {y};
-  }
+// The node behind s, if there is a sum, and y; its edges lead to x, the residual, weight and bias.  (A node with fields: torch's Function for extensions, which
+// finds them by name, took 77 us where this takes 69, forward and backward of 256 x 32 in fp32; torch's own norm takes 68.)
+struct LayerNormNode : torch::autograd::Node {
+  torch::autograd::SavedVariable source, weight, weight_f32, stats;      // source: x, or s; weight_f32: where the kernel does not read the weight itself
+  bool added = false, own_weight = false;
+  bool half = false;                     // a residual in bf16 beside an fp32 x takes its gradient in its own type
+  double eps = 0.0;
 
-  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+  void release_variables() override {
+    for (auto* v : {&source, &weight, &weight_f32, &stats}) v->reset_data();
+  }
+  variable_list apply(variable_list&& grads) override {
     const Backward count;
-    const variable_list saved = ctx->get_saved_variables();
-    const bool added = ctx->saved_data["added"].toBool(), half = ctx->saved_data["half"].toBool();
-    const Tensor ds = added ? grads[0] : Tensor(), dy = grads.back();
-    variable_list out(7);
-    const bool need_x = ctx->needs_input_grad(0), need_r = added && ctx->needs_input_grad(1);
-    // (inputs that are there are counted)
-    const bool weight = ctx->saved_data["weight"].toBool(), bias = ctx->saved_data["bias"].toBool();
-    const bool need_w = weight && ctx->needs_input_grad(1 + added), need_b = bias && ctx->needs_input_grad(1 + added + weight);
+    const Tensor ds = added ? grads[0] : Tensor(), &dy = grads.back();
+    variable_list out(4);
+    const bool need_x = task_should_compute_output(0), need_r = task_should_compute_output(1);
+    const bool need_w = task_should_compute_output(2), need_b = task_should_compute_output(3);
     if (!dy.defined()) {
       if (need_x) out[0] = ds;
       if (need_r && ds.defined()) out[1] = half ? ds.to(at::kBFloat16) : ds;
       return out;
     }
+    const Tensor x = source.unpack(added ? getptr() : nullptr);
     if (at::GradMode::is_enabled()) {      // (create_graph)
-      const Tensor& x = saved[0];
-      auto [dx, dw, db] = layer_norm_backward_graph(x, dy, ds, saved[3], ctx->saved_data["eps"].toDouble());
+      auto [dx, dw, db] = layer_norm_backward_graph(x, dy, ds, weight.unpack(), eps);
       if (need_x) out[0] = dx.to(x.scalar_type());
       if (need_r) out[1] = dx.to(half ? at::kBFloat16 : x.scalar_type());
       if (need_w) out[2] = dw;
       if (need_b) out[3] = db;
       return out;
     }
-    auto [dx, dr, dw, db] = layer_norm_backward(saved[0], dy, maybe(ds), maybe(saved[1]), saved[2], need_w || need_b, half && need_r);
+    const at::AutoDispatchBelowAutograd below;
+    const Tensor w = own_weight ? weight.unpack() : weight_f32.unpack();
+    auto [dx, dr, dw, db] = layer_norm_backward(x, dy, maybe(ds), maybe(w), stats.unpack(), need_w || need_b, half && need_r);
     if (need_x) out[0] = dx;
     if (need_r) out[1] = half ? *dr : dx;
     if (need_w) out[2] = *dw;
@@ -262,7 +254,30 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
 variable_list layer_norm(const Tensor& x, const OptTensor& residual, const OptTensor& weight, const OptTensor& bias, double eps, bool out_f32) {
   const Tensor r = value(residual), w = value(weight), b = value(bias);
   if (!plain({&x, &r, &w, &b})) return {};
-  return LayerNorm::apply(x, residual, weight, bias, eps, out_f32, records({&x, &r, &w, &b}));
+  const bool train = records({&x, &r, &w, &b});
+  Tensor s, y, stats, w32;
+  {
+    const at::AutoDispatchBelowAutograd below;
+    auto [sum, out, statistics, weight_f32] = layer_norm_forward(x, residual, weight, bias, eps, out_f32, train);
+    s = value(sum), y = out, stats = value(statistics), w32 = value(weight_f32);
+  }
+  if (train) {
+    const std::shared_ptr<LayerNormNode> node(new LayerNormNode(), torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(x, r, w, b));
+    node->added = s.defined();
+    node->half = s.defined() && r.scalar_type() != x.scalar_type();
+    node->eps = eps;
+    if (s.defined()) torch::autograd::set_history(s, node);
+    torch::autograd::set_history(y, node);
+    using torch::autograd::SavedVariable;
+    node->source = SavedVariable(s.defined() ? s : x, s.defined());
+    node->weight = SavedVariable(w, false);
+    node->own_weight = w32.is_same(w);
+    if (!node->own_weight) node->weight_f32 = SavedVariable(w32, false);
+    node->stats = SavedVariable(stats, false);
+  }
+  if (s.defined()) return {s, y};
+  return {y};
 }
 
 // ------------------------------------------------------------------------------------------ attention
