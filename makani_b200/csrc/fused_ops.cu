@@ -764,7 +764,6 @@ __global__ void __launch_bounds__(1024) colsum_slabs_kernel(const RowSlabs first
   RowSlabs j = blockIdx.z == 0 ? first : second;
   chain_begin(true, j.part);
   const float* const part = j.part;
-  float* const out = j.out;
   const int slabs = j.slabs, C = j.C;
   if (blockIdx.x * 32 >= C || static_cast<int>(blockIdx.y) >= j.groups) return;
   const int c = blockIdx.x * 32 + threadIdx.x;
@@ -781,7 +780,11 @@ __global__ void __launch_bounds__(1024) colsum_slabs_kernel(const RowSlabs first
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
   const int cw = blockIdx.x * 32 + threadIdx.y;
-  if (threadIdx.x == 0 && cw < C) out[static_cast<long long>(blockIdx.y) * C + cw] = a;
+  if (threadIdx.x == 0 && cw < C) {
+    const long long at = static_cast<long long>(blockIdx.y) * C + cw;
+    if (j.half) static_cast<__nv_bfloat16*>(j.out)[at] = __float2bfloat16(a);
+    else static_cast<float*>(j.out)[at] = a;
+  }
 }
 
 // ------------------------------------------------------------------------------------------ Lp norms

@@ -88,11 +88,11 @@ struct GemmPeer {
   void* Dx[7];                     // base pointers matching GemmEpilogue::D (offset already applied)
 };
 
-// Partial sums [groups][slabs][C] that are to be added up over the slabs
+// Partial sums [groups][slabs][C] that are to be added up over the slabs; `out` is fp32, or bf16 with `half`
 struct RowSlabs {
   const float* part = nullptr;
-  float* out = nullptr;
-  int slabs = 0, C = 0, groups = 0;
+  void* out = nullptr;
+  int slabs = 0, C = 0, groups = 0, half = 0;
 };
 
 // Optional: the sums over k of the rows of A (the gradient of a bias, beside the weight gradient), fp32 [M], or [z_lo][M] where the

@@ -225,6 +225,25 @@ __device__ __forceinline__ void store_row(T* to, const Raw<T, VEC> (&raw)[NV], i
   }
 }
 
+// Weights or biases, in fp32 or bf16; of long rows in fp32 (with both types in the kernel the registers do not hold 32 values a thread: 3000 x 4099 in fp32,
+// forward, 45 us where this takes 41)
+template <int VEC, int NV>
+__device__ __forceinline__ void load_params(const void* from, bool f32, f32x2 (&v)[Cols<VEC, NV>::PAIRS], int lane, int size, int C) {
+  if (VEC * NV > 8 || f32) {
+    Raw<float, VEC> raw[NV];
+    load_row(static_cast<const float*>(from), raw, lane, size, C);
+    unpack(raw, v);
+  } else {
+    Raw<__nv_bfloat16, VEC> raw[NV];
+    load_row(static_cast<const __nv_bfloat16*>(from), raw, lane, size, C);
+    unpack(raw, v);
+  }
+}
+__device__ __forceinline__ void store_param(void* to, bool f32, int c, float v) {
+  if (f32) static_cast<float*>(to)[c] = v;
+  else static_cast<__nv_bfloat16*>(to)[c] = __float2bfloat16(v);
+}
+
 // TR: type of the tensor that is added first (void: none)
 template <typename TI, typename TO, typename TR, int VEC, int NV, int SUB, int ROWS, int BLOCKS>
 __global__ void __launch_bounds__(THREADS, BLOCKS) ln_fwd_kernel(LnForward p, int warps) {
@@ -234,7 +253,7 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) ln_fwd_kernel(LnForward p, in
   __shared__ __align__(16) float sh[3 * ROWS * MOST_WARPS];
   const TI* x = static_cast<const TI*>(p.x);
   const Res* res = static_cast<const Res*>(p.r);
-  const float *w = p.w, *b = p.b;
+  const void *w = p.w, *b = p.b;
   chain_begin(true, x, res, w, b);
   const Group<SUB> g(warps);
   const int C = p.C;
@@ -245,15 +264,8 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) ln_fwd_kernel(LnForward p, in
     wv[k] = f2_pack(1.f, 1.f);
     bv[k] = 0ull;
   }
-  Raw<float, VEC> weights[NV];
-  if (w) {
-    load_row(w, weights, g.lane, g.size, C);
-    unpack(weights, wv);
-  }
-  if (b) {
-    load_row(b, weights, g.lane, g.size, C);
-    unpack(weights, bv);
-  }
+  if (w) load_params<VEC, NV>(w, p.w_f32, wv, g.lane, g.size, C);
+  if (b) load_params<VEC, NV>(b, p.b_f32, bv, g.lane, g.size, C);
   const long long step = static_cast<long long>(gridDim.x) * g.per_block * ROWS;
   // (the groups of a warp go through the loop together)
   const int per_warp = SUB < 32 ? 32 / SUB : 1;
@@ -340,7 +352,7 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) ln_bwd_kernel(LnBackward p, i
   __shared__ __align__(16) float sh[2][2 * ROWS * MOST_WARPS];
   const TI *x = static_cast<const TI*>(p.x), *ds = static_cast<const TI*>(p.ds);
   const TO* dy = static_cast<const TO*>(p.dy);
-  const float* w = p.w;
+  const void* w = p.w;
   const float2* stats = p.stats;
   chain_begin(true, x, ds, dy, w, stats);
   const Group<SUB> g(warps);
@@ -353,9 +365,7 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) ln_bwd_kernel(LnBackward p, i
     aw[k] = ab[k] = 0ull;
   }
   if (w) {
-    Raw<float, VEC> weights[NV];
-    load_row(w, weights, g.lane, g.size, C);
-    unpack(weights, wv);
+    load_params<VEC, NV>(w, p.w_f32, wv, g.lane, g.size, C);
     keep<VEC, NV>(wv, g.lane, g.size, C);
   }
   const long long step = static_cast<long long>(gridDim.x) * g.per_block * ROWS;
@@ -470,8 +480,15 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) ln_bwd_kernel(LnBackward p, i
     }
     __syncthreads();
   }
-  float* const out_w = gridDim.x == 1 ? p.dw : p.part + static_cast<long long>(blockIdx.x) * C;
-  float* const out_b = gridDim.x == 1 ? p.db : p.part + (static_cast<long long>(gridDim.x) + blockIdx.x) * C;
+  if (gridDim.x == 1) {
+    for (int c = threadIdx.x; c < C; c += blockDim.x) {
+      store_param(p.dw, p.dw_f32, c, cols[c]);
+      store_param(p.db, p.db_f32, c, cols[C + c]);
+    }
+    return;
+  }
+  float* const out_w = p.part + static_cast<long long>(blockIdx.x) * C;
+  float* const out_b = p.part + (static_cast<long long>(gridDim.x) + blockIdx.x) * C;
   for (int c = threadIdx.x; c < C; c += blockDim.x) {
     out_w[c] = cols[c];
     out_b[c] = cols[C + c];
@@ -484,7 +501,7 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) ln_bwd_kernel(LnBackward p, i
 // 116).  (A warp to a row, its weights read again for every row: 71 and 212; 16471 x 387 74.  Rows through a ring of cp.async, (2, 4) 77 and (4, 2) 86: more bytes on
 // their way are not what is missing.)  Behind a sum one row at a time: 16200 x 768 (4, 1) 21.0, (3, 2) 23.3 (DRAM 15).
 constexpr int FWD_BLOCKS = 2, BWD_BLOCKS = 2;
-constexpr int WIDE = 2048, RAGGED = 1024;      // most channels of eight warps with one vector, or four single values, a thread
+constexpr int WIDE = 2048, RAGGED = LN_HALF_PARAMS;      // most channels of eight warps with one vector, or four single values, a thread
 struct Spread {
   int warps, threads, rows;
 };
@@ -551,7 +568,8 @@ cudaError_t by_type(const P& p, bool vec, cudaStream_t s) {
 
 cudaError_t layer_norm_fwd(const LnForward& p, cudaStream_t s) {
   if (p.rows <= 0) return cudaSuccess;
-  if (p.C <= 0 || p.C > LN_CHANNELS || p.inner <= 0 || (p.r != nullptr) != (p.s != nullptr) || (p.r && p.r_f32 && !p.x_f32))
+  if (p.C <= 0 || p.C > LN_CHANNELS || p.inner <= 0 || (p.r != nullptr) != (p.s != nullptr) || (p.r && p.r_f32 && !p.x_f32) ||
+      (p.C > LN_HALF_PARAMS && ((p.w && !p.w_f32) || (p.b && !p.b_f32))))
     return cudaErrorInvalidValue;
   // whole 16-byte vectors in every tensor
   const bool vec = p.C % 8 == 0 && p.outer_stride % 8 == 0 && p.inner_stride % 8 == 0 && aligned(p.x) && aligned(p.r) && aligned(p.s) && aligned(p.y) &&
@@ -567,7 +585,8 @@ long long layer_norm_scratch(long long rows, int C) {
 
 cudaError_t layer_norm_bwd(const LnBackward& p, int* launches, cudaStream_t s) {
   *launches = 0;
-  if (p.C <= 0 || p.C > LN_CHANNELS || p.inner <= 0 || (p.dw != nullptr) != (p.db != nullptr)) return cudaErrorInvalidValue;
+  if (p.C <= 0 || p.C > LN_CHANNELS || p.inner <= 0 || (p.dw != nullptr) != (p.db != nullptr) || (p.C > LN_HALF_PARAMS && p.w && !p.w_f32))
+    return cudaErrorInvalidValue;
   if (p.rows <= 0) return cudaSuccess;
   const bool vec = p.C % 8 == 0 && p.outer_stride % 8 == 0 && p.inner_stride % 8 == 0 && aligned(p.x) && aligned(p.dy) && aligned(p.ds) &&
                    aligned(p.dx) && aligned(p.dr) && aligned(p.w) && aligned(p.dw) && aligned(p.db) && aligned(p.part);
@@ -578,7 +597,7 @@ cudaError_t layer_norm_bwd(const LnBackward& p, int* launches, cudaStream_t s) {
   if (e != cudaSuccess || !p.dw || blocks == 1) return e;
   ++*launches;
   const int n = static_cast<int>(blocks);
-  return colsum_add_slabs(RowSlabs{p.part, p.dw, n, p.C, 1}, RowSlabs{p.part + static_cast<long long>(n) * p.C, p.db, n, p.C, 1}, s);
+  return colsum_add_slabs(RowSlabs{p.part, p.dw, n, p.C, 1, !p.dw_f32}, RowSlabs{p.part + static_cast<long long>(n) * p.C, p.db, n, p.C, 1, !p.db_f32}, s);
 }
 
 }  // namespace mk

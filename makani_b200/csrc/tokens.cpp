@@ -106,21 +106,23 @@ struct Rows {
   }
 };
 
-Tensor channel_f32(const OptTensor& t, const Tensor& x, const char* what) {
+// A weight or a bias as the kernels read it: dense, in a type of theirs
+Tensor channel_values(const OptTensor& t, const Tensor& x, const char* what) {
   if (!t.has_value() || !t->defined()) return Tensor();
   MK_CHECK(t->device() == x.device(), "layer norm: tensors must be on one CUDA device");
   MK_CHECK(t->dim() == 1 && t->size(0) == x.size(-1), "layer norm: one ", what, " per channel expected");
-  return is_f32(*t) && t->is_contiguous() ? *t : t->detach().to(at::kFloat).contiguous();
+  if (is_f32(*t) || (native_type(*t) && t->size(0) <= mk::LN_HALF_PARAMS)) return t->is_contiguous() ? *t : t->detach().contiguous();
+  return t->detach().to(at::kFloat).contiguous();
 }
 
-// (s, y, statistics, weight in fp32): s and the statistics where they are asked for
+// (s, y, statistics, weight as the kernel reads it): s and the statistics where they are asked for
 std::tuple<OptTensor, Tensor, OptTensor, OptTensor> layer_norm_forward(const Tensor& x, const OptTensor& residual, const OptTensor& weight,
                                                                        const OptTensor& bias, double eps, bool out_f32, bool train) {
   MK_CHECK(x.is_cuda() && native_type(x) && x.dim() >= 1, "layer norm: bf16 or fp32 CUDA tensors expected");
   c10::cuda::CUDAGuard guard(x.device());
   const Rows in(x);
   MK_CHECK(in.C >= 1 && in.C <= mk::LN_CHANNELS, "layer norm: 1 to ", mk::LN_CHANNELS, " channels expected");
-  const Tensor w = channel_f32(weight, x, "weight"), b = channel_f32(bias, x, "bias");
+  const Tensor w = channel_values(weight, x, "weight"), b = channel_values(bias, x, "bias");
   Tensor r, s, stats, y = at::empty(x.sizes(), x.options().dtype(out_f32 ? at::kFloat : at::kBFloat16));
   if (residual.has_value() && residual->defined()) {
     MK_CHECK(residual->device() == x.device() && residual->sizes() == x.sizes() && native_type(*residual) && (is_f32(x) || !is_f32(*residual)),
@@ -134,8 +136,10 @@ std::tuple<OptTensor, Tensor, OptTensor, OptTensor> layer_norm_forward(const Ten
   p.r = ptr_or_null<void>(r);
   p.s = ptr_or_null<void>(s);
   p.y = y.data_ptr();
-  p.w = ptr_or_null<float>(w);
-  p.b = ptr_or_null<float>(b);
+  p.w = ptr_or_null<void>(w);
+  p.b = ptr_or_null<void>(b);
+  p.w_f32 = w.defined() && is_f32(w);
+  p.b_f32 = b.defined() && is_f32(b);
   p.stats = ptr_or_null<float2>(stats);
   p.rows = in.rows;
   p.C = static_cast<int>(in.C);
@@ -151,15 +155,15 @@ std::tuple<OptTensor, Tensor, OptTensor, OptTensor> layer_norm_forward(const Ten
   return {maybe(s), y, maybe(stats), maybe(w)};
 }
 
-// (dx, dr, dweight, dbias); `half_copy`: dr, dx in bf16
+// (dx, dr, dweight, dbias); `half_copy`: dr, dx in bf16; `half_dw`, `half_db`: these in bf16
 std::tuple<Tensor, OptTensor, OptTensor, OptTensor> layer_norm_backward(const Tensor& x, const Tensor& dy, const OptTensor& ds, const OptTensor& weight,
-                                                                        const Tensor& stats, bool need_params, bool half_copy) {
+                                                                        const Tensor& stats, bool need_params, bool half_dw, bool half_db, bool half_copy) {
   MK_CHECK(x.is_cuda() && native_type(x) && native_type(dy) && dy.device() == x.device() && dy.sizes() == x.sizes(),
            "layer norm: gradients in the shape of x and on its device expected");
   c10::cuda::CUDAGuard guard(x.device());
   const Rows in(x);
   MK_CHECK(stats.is_cuda() && is_f32(stats) && stats.is_contiguous() && stats.numel() == 2 * in.rows, "layer norm: statistics of every row expected");
-  const Tensor w = channel_f32(weight, x, "weight"), g = dy.contiguous();
+  const Tensor w = channel_values(weight, x, "weight"), g = dy.contiguous();
   Tensor d, dr, dw, db, part, dx = at::empty(x.sizes(), x.options());
   if (ds.has_value() && ds->defined()) {
     MK_CHECK(ds->device() == x.device() && ds->sizes() == x.sizes() && ds->scalar_type() == x.scalar_type(),
@@ -169,8 +173,12 @@ std::tuple<Tensor, OptTensor, OptTensor, OptTensor> layer_norm_backward(const Te
   if (half_copy) dr = at::empty(x.sizes(), x.options().dtype(at::kBFloat16));
   if (need_params) {
     // (no rows: no kernel that writes them)
-    dw = in.rows ? at::empty({in.C}, x.options().dtype(at::kFloat)) : at::zeros({in.C}, x.options().dtype(at::kFloat));
-    db = in.rows ? at::empty_like(dw) : at::zeros_like(dw);
+    auto room = [&](bool half) {
+      const auto options = x.options().dtype(half ? at::kBFloat16 : at::kFloat);
+      return in.rows ? at::empty({in.C}, options) : at::zeros({in.C}, options);
+    };
+    dw = room(half_dw);
+    db = room(half_db);
     const int64_t n = mk::layer_norm_scratch(in.rows, static_cast<int>(in.C));
     if (n) part = at::empty({n}, x.options().dtype(at::kFloat));
   }
@@ -180,10 +188,13 @@ std::tuple<Tensor, OptTensor, OptTensor, OptTensor> layer_norm_backward(const Te
   p.ds = ptr_or_null<void>(d);
   p.dx = dx.data_ptr();
   p.dr = ptr_or_null<void>(dr);
-  p.w = ptr_or_null<float>(w);
+  p.w = ptr_or_null<void>(w);
+  p.w_f32 = w.defined() && is_f32(w);
   p.stats = static_cast<const float2*>(stats.data_ptr());
-  p.dw = ptr_or_null<float>(dw);
-  p.db = ptr_or_null<float>(db);
+  p.dw = ptr_or_null<void>(dw);
+  p.db = ptr_or_null<void>(db);
+  p.dw_f32 = !half_dw;
+  p.db_f32 = !half_db;
   p.part = ptr_or_null<float>(part);
   p.rows = in.rows;
   p.C = static_cast<int>(in.C);
@@ -211,13 +222,13 @@ std::tuple<Tensor, Tensor, Tensor> layer_norm_backward_graph(const Tensor& x, co
 // The node behind s, if there is a sum, and y; its edges lead to x, the residual, weight and bias.  (A node with fields: torch's Function for extensions, which
 // finds them by name, took 77 us where this takes 69, forward and backward of 256 x 32 in fp32; torch's own norm takes 68.)
 struct LayerNormNode : torch::autograd::Node {
-  torch::autograd::SavedVariable source, weight, weight_f32, stats;      // source: x, or s; weight_f32: where the kernel does not read the weight itself
-  bool added = false, own_weight = false;
+  torch::autograd::SavedVariable source, weight, read_weight, stats;      // source: x, or s; read_weight: where the kernel does not read the weight itself
+  bool added = false, own_weight = false, half_dw = false, half_db = false;
   bool half = false;                     // a residual in bf16 beside an fp32 x takes its gradient in its own type
   double eps = 0.0;
 
   void release_variables() override {
-    for (auto* v : {&source, &weight, &weight_f32, &stats}) v->reset_data();
+    for (auto* v : {&source, &weight, &read_weight, &stats}) v->reset_data();
   }
   variable_list apply(variable_list&& grads) override {
     const Backward count;
@@ -240,8 +251,8 @@ struct LayerNormNode : torch::autograd::Node {
       return out;
     }
     const at::AutoDispatchBelowAutograd below;
-    const Tensor w = own_weight ? weight.unpack() : weight_f32.unpack();
-    auto [dx, dr, dw, db] = layer_norm_backward(x, dy, maybe(ds), maybe(w), stats.unpack(), need_w || need_b, half && need_r);
+    const Tensor w = own_weight ? weight.unpack() : read_weight.unpack();
+    auto [dx, dr, dw, db] = layer_norm_backward(x, dy, maybe(ds), maybe(w), stats.unpack(), need_w || need_b, half_dw, half_db, half && need_r);
     if (need_x) out[0] = dx;
     if (need_r) out[1] = half ? *dr : dx;
     if (need_w) out[2] = *dw;
@@ -255,11 +266,11 @@ variable_list layer_norm(const Tensor& x, const OptTensor& residual, const OptTe
   const Tensor r = value(residual), w = value(weight), b = value(bias);
   if (!plain({&x, &r, &w, &b})) return {};
   const bool train = records({&x, &r, &w, &b});
-  Tensor s, y, stats, w32;
+  Tensor s, y, stats, read;
   {
     const at::AutoDispatchBelowAutograd below;
-    auto [sum, out, statistics, weight_f32] = layer_norm_forward(x, residual, weight, bias, eps, out_f32, train);
-    s = value(sum), y = out, stats = value(statistics), w32 = value(weight_f32);
+    auto [sum, out, statistics, read_weight] = layer_norm_forward(x, residual, weight, bias, eps, out_f32, train);
+    s = value(sum), y = out, stats = value(statistics), read = value(read_weight);
   }
   if (train) {
     const std::shared_ptr<LayerNormNode> node(new LayerNormNode(), torch::autograd::deleteNode);
@@ -272,8 +283,10 @@ variable_list layer_norm(const Tensor& x, const OptTensor& residual, const OptTe
     using torch::autograd::SavedVariable;
     node->source = SavedVariable(s.defined() ? s : x, s.defined());
     node->weight = SavedVariable(w, false);
-    node->own_weight = w32.is_same(w);
-    if (!node->own_weight) node->weight_f32 = SavedVariable(w32, false);
+    node->own_weight = read.is_same(w);
+    if (!node->own_weight) node->read_weight = SavedVariable(read, false);
+    node->half_dw = w.defined() && w.scalar_type() == at::kBFloat16;
+    node->half_db = b.defined() && b.scalar_type() == at::kBFloat16;
     node->stats = SavedVariable(stats, false);
   }
   if (s.defined()) return {s, y};

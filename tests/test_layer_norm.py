@@ -406,3 +406,18 @@ def test_layer_norm_of_several_turns(gen, rows, C, xt, yt):
     x, dy = _tokens(gen, rows, C, dtype=xt), torch.randn(rows, C, device="cuda", generator=gen).to(yt)
     w, b = 1 + 0.2 * torch.randn(C, device="cuda", generator=gen), 0.2 * torch.randn(C, device="cuda", generator=gen)
     _check(x, w, b, dy, yt)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,C", [(1, 8), (64, 48), (700, 128), (333, 387), (5001, 768), (90, 1024), (41, 1023), (70, 1032), (9, 2051), (12, 4096)])
+@pytest.mark.parametrize("wt,bt", [(torch.bfloat16, torch.bfloat16), (torch.bfloat16, torch.float32), (torch.float32, torch.bfloat16), (torch.float16, torch.float64),
+                                   (torch.bfloat16, None), (None, torch.bfloat16)])
+def test_types_of_parameters(gen, rows, C, wt, bt):
+    """Weights and biases in types of their own, each with its gradient rounded once to its type, by one block and by several."""
+    x, dy = _tokens(gen, rows, C), torch.randn(rows, C, device="cuda", generator=gen).bfloat16()
+    w = None if wt is None else (1 + 0.2 * torch.randn(C, device="cuda", generator=gen)).to(wt)
+    b = None if bt is None else (0.2 * torch.randn(C, device="cuda", generator=gen)).to(bt)
+    _check(x, w, b, dy, None)
+    _check(x, w, b, dy, torch.bfloat16, residual=_tokens(gen, rows, C), ds=dy.flip(0))
+    if wt is not None and C > 8:      # off a 16-byte boundary
+        _check(x, torch.cat([w[:1], w])[1:], b, dy, None)
