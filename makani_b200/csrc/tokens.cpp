@@ -6,6 +6,7 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
+#include <torch/csrc/dynamo/compiled_autograd.h>
 
 #include <pybind11/stl.h>
 
@@ -222,41 +223,91 @@ std::tuple<Tensor, Tensor, Tensor> layer_norm_backward_graph(const Tensor& x, co
 // The node behind s, if there is a sum, and y; its edges lead to x, the residual, weight and bias.  (A node with fields: torch's Function for extensions, which
 // finds them by name, took 77 us where this takes 69, forward and backward of 256 x 32 in fp32; torch's own norm takes 68.)
 struct LayerNormNode : torch::autograd::Node {
-  torch::autograd::SavedVariable source, weight, read_weight, stats;      // source: x, or s; read_weight: where the kernel does not read the weight itself
-  bool added = false, own_weight = false, half_dw = false, half_db = false;
-  bool half = false;                     // a residual in bf16 beside an fp32 x takes its gradient in its own type
-  double eps = 0.0;
+  // What it keeps beside tensors.  half: a residual in bf16 beside an fp32 x takes its gradient in its own type; half_dw, half_db: as the parameters;
+  // own_weight: the kernels read the weight as it is, else a copy that is saved too
+  struct Form {
+    double eps = 0.0;
+    bool added = false, half = false, half_dw = false, half_db = false, own_weight = false;
+  };
+  Form form;
+  torch::autograd::SavedVariable source, weight, read_weight, stats;      // source: x, or s
 
   void release_variables() override {
+    const std::lock_guard<std::mutex> lock(mutex_);
     for (auto* v : {&source, &weight, &read_weight, &stats}) v->reset_data();
   }
   variable_list apply(variable_list&& grads) override {
+    const std::lock_guard<std::mutex> lock(mutex_);
+    return gradients(grads, {source.unpack(form.added ? getptr() : nullptr), weight.unpack(), read_weight.unpack(), stats.unpack()}, form, needed());
+  }
+  std::vector<bool> needed() const {
+    return {task_should_compute_output(0), task_should_compute_output(1), task_should_compute_output(2), task_should_compute_output(3)};
+  }
+
+  // `saved`: source, weight, read_weight, stats; `need`: of x, the residual, weight and bias
+  static variable_list gradients(const variable_list& grads, const variable_list& saved, const Form& f, const std::vector<bool>& need) {
     const Backward count;
-    const Tensor ds = added ? grads[0] : Tensor(), &dy = grads.back();
+    const Tensor &x = saved[0], &dy = grads.back(), ds = f.added ? grads[0] : Tensor();
     variable_list out(4);
-    const bool need_x = task_should_compute_output(0), need_r = task_should_compute_output(1);
-    const bool need_w = task_should_compute_output(2), need_b = task_should_compute_output(3);
     if (!dy.defined()) {
-      if (need_x) out[0] = ds;
-      if (need_r && ds.defined()) out[1] = half ? ds.to(at::kBFloat16) : ds;
+      if (need[0]) out[0] = ds;
+      if (need[1] && ds.defined()) out[1] = f.half ? ds.to(at::kBFloat16) : ds;
       return out;
     }
-    const Tensor x = source.unpack(added ? getptr() : nullptr);
     if (at::GradMode::is_enabled()) {      // (create_graph)
-      auto [dx, dw, db] = layer_norm_backward_graph(x, dy, ds, weight.unpack(), eps);
-      if (need_x) out[0] = dx.to(x.scalar_type());
-      if (need_r) out[1] = dx.to(half ? at::kBFloat16 : x.scalar_type());
-      if (need_w) out[2] = dw;
-      if (need_b) out[3] = db;
+      auto [dx, dw, db] = layer_norm_backward_graph(x, dy, ds, saved[1], f.eps);
+      if (need[0]) out[0] = dx.to(x.scalar_type());
+      if (need[1]) out[1] = dx.to(f.half ? at::kBFloat16 : x.scalar_type());
+      if (need[2]) out[2] = dw;
+      if (need[3]) out[3] = db;
       return out;
     }
     const at::AutoDispatchBelowAutograd below;
-    const Tensor w = own_weight ? weight.unpack() : read_weight.unpack();
-    auto [dx, dr, dw, db] = layer_norm_backward(x, dy, maybe(ds), maybe(w), stats.unpack(), need_w || need_b, half_dw, half_db, half && need_r);
-    if (need_x) out[0] = dx;
-    if (need_r) out[1] = half ? *dr : dx;
-    if (need_w) out[2] = *dw;
-    if (need_b) out[3] = *db;
+    auto [dx, dr, dw, db] = layer_norm_backward(x, dy, maybe(ds), maybe(saved[f.own_weight ? 1 : 2]), saved[3], need[2] || need[3], f.half_dw, f.half_db,
+                                                f.half && need[1]);
+    if (need[0]) out[0] = dx;
+    if (need[1]) out[1] = f.half ? *dr : dx;
+    if (need[2]) out[2] = *dw;
+    if (need[3]) out[3] = *db;
+    return out;
+  }
+
+  // A compiled backward pass calls `gradients` as one opaque operation, as it does with nodes of torch's Function
+  static variable_list call(const variable_list& grads, const std::vector<c10::IValue>& args) {
+    torch::dynamo::autograd::PackedArgs packed(args);
+    const auto saved = packed.unpack<variable_list>();
+    Form f;
+    f.eps = packed.unpack<double>();
+    for (bool* b : {&f.added, &f.half, &f.half_dw, &f.half_db, &f.own_weight}) *b = packed.unpack<bool>();
+    return gradients(grads, saved, f, packed.unpack<std::vector<bool>>());
+  }
+  void compiled_args(torch::dynamo::autograd::CompiledNodeArgs& args) const override {
+    args.collect(source, form.added);
+    for (auto* v : {&weight, &read_weight, &stats}) args.collect(*v, false);
+    args.collect(form.eps);
+    for (const bool b : {form.added, form.half, form.half_dw, form.half_db, form.own_weight}) args.collect(b);
+  }
+  variable_list apply_with_saved(const variable_list& grads, torch::dynamo::autograd::SwapSavedVariables& saved) override {
+    using namespace torch::dynamo::autograd;
+    torch::autograd::SavedVariable* const all[] = {&source, &weight, &read_weight, &stats};
+    variable_list tensors;
+    for (auto* v : all) {
+      saved.before(*v);
+      tensors.push_back(v->unpack(v == &source && form.added ? getptr() : nullptr));
+    }
+    PackedArgs packed;
+    packed.pack(tensors);
+    packed.pack(form.eps);
+    for (const bool b : {form.added, form.half, form.half_dw, form.half_db, form.own_weight}) packed.pack(b);
+    packed.pack(needed());
+    const auto metadata = IValuePacker<std::vector<std::optional<torch::autograd::InputMetadata>>>::pack(get_input_metadata(next_edges()));
+    const auto args = std::move(packed).vec();
+    std::vector<at::TypePtr> schema;
+    for (const auto& v : args) schema.emplace_back(v.isTensor() ? at::TypePtr(at::TensorType::get()) : v.type());
+    const auto& python = getPyCompilerInterface();
+    const auto name = python->bind_function(saved.get_py_compiler(), "LayerNormNode", call, schema, /*is_custom_function=*/true, /*is_traceable=*/false);
+    auto out = python->call_function(saved.get_py_compiler(), "apply_functional", name, grads, args, metadata);
+    for (auto* v : all) saved.after(*v);
     return out;
   }
 };
@@ -275,18 +326,14 @@ variable_list layer_norm(const Tensor& x, const OptTensor& residual, const OptTe
   if (train) {
     const std::shared_ptr<LayerNormNode> node(new LayerNormNode(), torch::autograd::deleteNode);
     node->set_next_edges(torch::autograd::collect_next_edges(x, r, w, b));
-    node->added = s.defined();
-    node->half = s.defined() && r.scalar_type() != x.scalar_type();
-    node->eps = eps;
+    node->form = {eps, s.defined(), s.defined() && r.scalar_type() != x.scalar_type(), w.defined() && w.scalar_type() == at::kBFloat16,
+                  b.defined() && b.scalar_type() == at::kBFloat16, read.is_same(w)};
     if (s.defined()) torch::autograd::set_history(s, node);
     torch::autograd::set_history(y, node);
     using torch::autograd::SavedVariable;
     node->source = SavedVariable(s.defined() ? s : x, s.defined());
     node->weight = SavedVariable(w, false);
-    node->own_weight = read.is_same(w);
-    if (!node->own_weight) node->read_weight = SavedVariable(read, false);
-    node->half_dw = w.defined() && w.scalar_type() == at::kBFloat16;
-    node->half_db = b.defined() && b.scalar_type() == at::kBFloat16;
+    if (!node->form.own_weight) node->read_weight = SavedVariable(read, false);
     node->stats = SavedVariable(stats, false);
   }
   if (s.defined()) return {s, y};

@@ -421,3 +421,40 @@ def test_types_of_parameters(gen, rows, C, wt, bt):
     _check(x, w, b, dy, torch.bfloat16, residual=_tokens(gen, rows, C), ds=dy.flip(0))
     if wt is not None and C > 8:      # off a 16-byte boundary
         _check(x, torch.cat([w[:1], w])[1:], b, dy, None)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", ["norm", "sum and norm", "sum", "behind a sum"])
+def test_compiled_backward_pass(gen, which):
+    """The backward pass that is compiled calls the kernels: the same bits."""
+    from torch._dynamo import compiled_autograd
+    x, r = (torch.randn(9, 40, device="cuda", generator=gen).requires_grad_() for _ in range(2))
+    w = torch.randn(40, device="cuda", generator=gen).bfloat16().requires_grad_()
+
+    def grads():
+        s, y = norm_ops.add_layer_norm(x, r, w, None)
+        if which == "norm":
+            y = norm_ops.layer_norm(x, w, None)
+        out = {"norm": y, "sum and norm": s * s + y * y, "sum": s * s, "behind a sum": y * y}[which]
+        return torch.autograd.grad(out.sum(), (x, r, w), allow_unused=True)
+
+    want = grads()
+    with compiled_autograd._enable(torch.compile(backend="eager")):
+        got = grads()
+    for p, q in zip(got, want):
+        assert (p is None and q is None) or torch.equal(p, q)
+
+
+@pytest.mark.gpu
+def test_a_second_backward_pass(gen):
+    x = torch.randn(9, 40, device="cuda", generator=gen).requires_grad_()
+    s, y = norm_ops.add_layer_norm(x, x, None, None)
+    first = torch.autograd.grad(y.sum() + s.sum(), x, retain_graph=True)[0]
+    assert torch.equal(first, torch.autograd.grad(y.sum() + s.sum(), x)[0])
+    with pytest.raises(RuntimeError, match="second time"):
+        torch.autograd.grad(y.sum(), x)
+    s, y = norm_ops.add_layer_norm(x, x, None, None)
+    with torch.no_grad():
+        s.add_(1)
+    with pytest.raises(RuntimeError, match="inplace"):
+        torch.autograd.grad(y.sum(), x)
