@@ -36,15 +36,32 @@ std::map<int, Tensor>& err_flags() {
   return m;
 }
 
+// Memory that is cleared here and now and belongs to nobody else: the first kernel to ask may be one that a graph captures, where an allocation is the graph's
+// and clearing it a part of every replay
+Tensor new_err_flag(int dev) {
+  c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(dev));
+  constexpr int64_t words = 4;
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  check_cuda(cudaThreadExchangeStreamCaptureMode(&mode), "error word");
+  void* p = nullptr;
+  cudaStream_t aside = nullptr;
+  cudaError_t e = cudaMalloc(&p, words * sizeof(int));
+  if (e == cudaSuccess) e = cudaStreamCreateWithFlags(&aside, cudaStreamNonBlocking);
+  if (e == cudaSuccess) e = cudaMemsetAsync(p, 0, words * sizeof(int), aside);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(aside);
+  if (aside) cudaStreamDestroy(aside);
+  if (e != cudaSuccess && p) cudaFree(p);
+  const cudaError_t back = cudaThreadExchangeStreamCaptureMode(&mode);
+  check_cuda(e == cudaSuccess ? back : e, "error word");
+  return torch::from_blob(p, {words}, torch::dtype(torch::kInt32).device(torch::kCUDA, static_cast<c10::DeviceIndex>(dev)));
+}
+
 Tensor err_flag_for(const Tensor& t) {
   const int dev = t.get_device();
   const std::lock_guard<std::mutex> lock(err_mutex());
   auto& m = err_flags();
   auto it = m.find(dev);
-  if (it == m.end()) {
-    Tensor f = torch::zeros({4}, torch::dtype(torch::kInt32).device(t.device()));
-    it = m.emplace(dev, f).first;
-  }
+  if (it == m.end()) it = m.emplace(dev, new_err_flag(dev)).first;
   return it->second;
 }
 

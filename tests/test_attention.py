@@ -9,6 +9,9 @@ Tolerances, element by element.  Half a step of bf16 is B = 2^-8 relative (`eps 
     dk the same over the queries; dv = sum P do  off by  (B + e) sum P |do|."""
 
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -610,3 +613,30 @@ def test_delta_holds_what_the_output_lost(gen, B, N, H, D, causal):
         want, off, _ = _kinds_oracle(q[b], k[b], v[b], do[b], causal)
         for n in want:
             _close(got[n][b], want[n], off[n], f"{n} of sample {b}")
+
+
+@pytest.mark.gpu
+def test_first_call_of_a_process_captured():
+    """The device's error word is nobody's graph's: no memory of a graph is left when it and its results are gone, and a replay clears nothing."""
+    if not torch.cuda.is_available():
+        pytest.skip("needs a GPU")
+    code = """
+import torch
+from makani_b200.ops import _ext, attention as attn
+q = torch.randn(1, 20, 2, 16, device="cuda").bfloat16()
+side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+side.wait_stream(torch.cuda.current_stream())
+with torch.cuda.graph(graph, stream=side):
+    o = attn.attention(q, q, q)
+assert _ext.require().read_error_flag(0) == 0
+graph.replay()
+torch.cuda.synchronize()
+assert torch.equal(o, attn.attention(q, q, q))
+_ext.check_device_errors()
+del o, graph
+torch.cuda.empty_cache()
+left = [s for s in torch.cuda.memory_snapshot() if tuple(s["segment_pool_id"]) != (0, 0)]
+assert not left, left
+"""
+    done = subprocess.run([sys.executable, "-c", code], cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))), capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]
