@@ -172,13 +172,15 @@ _LN_TYPES = (torch.bfloat16, torch.float32)
 
 
 def _check_layer_norm(x, residual, weight, bias, out_dtype):
-    if x.dim() < 1 or x.shape[-1] < 1 or not x.dtype.is_floating_point:
-        raise ValueError(f"layer norm takes floating-point tokens [..., C], got {x.dtype} {tuple(x.shape)}")
+    shape, dtype = x.shape, x.dtype
+    row = shape[-1:]
+    if not row or row[0] < 1 or not dtype.is_floating_point:
+        raise ValueError(f"layer norm takes floating-point tokens [..., C], got {dtype} {tuple(shape)}")
     for name, p in (("weight", weight), ("bias", bias)):
-        if p is not None and (p.dim() != 1 or p.shape[0] != x.shape[-1]):
-            raise ValueError(f"layer norm over {x.shape[-1]} channels: {name} has shape {tuple(p.shape)}")
-    if residual is not None and (residual.shape != x.shape or residual.device != x.device):
-        raise ValueError(f"the residual {tuple(residual.shape)} on {residual.device} does not match {tuple(x.shape)} on {x.device}")
+        if p is not None and p.shape != row:
+            raise ValueError(f"layer norm over {row[0]} channels: {name} has shape {tuple(p.shape)}")
+    if residual is not None and (residual.shape != shape or residual.device != x.device):
+        raise ValueError(f"the residual {tuple(residual.shape)} on {residual.device} does not match {tuple(shape)} on {x.device}")
     if out_dtype is not None and not out_dtype.is_floating_point:
         raise ValueError(f"layer norm has no output in {out_dtype}")
 
@@ -188,12 +190,15 @@ def _layer_norm_native(x, out_dtype) -> bool:
 
 
 def _layer_norm_torch(x, weight, bias, eps, out_dtype):
-    # (the types are explicit here: autocast would choose its own)
-    with torch.autocast(device_type=x.device.type, enabled=False):
-        t = torch.promote_types(x.dtype, torch.float32)
-        y = torch.nn.functional.layer_norm(x.to(t), x.shape[-1:], None if weight is None else weight.to(t),
-                                           None if bias is None else bias.to(t), eps)
-        return y.to(out_dtype)
+    device = x.device.type
+    if device in ("cuda", "cpu") and torch.is_autocast_enabled(device):
+        # (the types are explicit here: autocast would choose its own)
+        with torch.autocast(device_type=device, enabled=False):
+            return _layer_norm_torch(x, weight, bias, eps, out_dtype)
+    t = torch.promote_types(x.dtype, torch.float32)
+    x, weight, bias = (p if p is None or p.dtype is t else p.to(t) for p in (x, weight, bias))
+    y = torch.nn.functional.layer_norm(x, x.shape[-1:], weight, bias, eps)
+    return y if y.dtype is out_dtype else y.to(out_dtype)
 
 
 def layer_norm(x: torch.Tensor, weight, bias, eps: float = 1e-5, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
@@ -218,8 +223,7 @@ def add_layer_norm(x: torch.Tensor, residual: torch.Tensor, weight, bias, eps: f
     _check_layer_norm(x, residual, weight, bias, out_dtype)
     if residual.dtype == torch.float32 and x.dtype == torch.bfloat16:
         x, residual = residual, x
-    dtype = torch.promote_types(x.dtype, residual.dtype)
-    out_dtype = out_dtype or dtype
+    out_dtype = out_dtype or (x.dtype if x.dtype is residual.dtype else torch.promote_types(x.dtype, residual.dtype))
     if _layer_norm_native(x, out_dtype) and residual.dtype in _LN_TYPES:
         out = _ext.require().layer_norm(x, residual, weight, bias, eps, out_dtype is torch.float32)
         if out:

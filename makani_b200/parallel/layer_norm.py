@@ -156,28 +156,28 @@ class LayerNorm(nn.LayerNorm):
                     or m._global_forward_pre_hooks or m._global_backward_hooks or m._global_backward_pre_hooks
                     or "forward" in self.__dict__ or type(self).forward is not LayerNorm.forward)
 
-    def _dtype(self, x, dtype, out_dtype):
-        if out_dtype is not None:
-            return out_dtype
-        return torch.float32 if x.is_cuda and torch.is_autocast_enabled() and dtype != torch.float64 else dtype
+    def _check(self, x):
+        if x.shape[-1] != self.normalized_shape[0]:
+            raise ValueError(f"layer norm over {self.normalized_shape[0]} channels, got {tuple(x.shape)}")
 
     def forward(self, x, out_dtype=None):
         if len(self.normalized_shape) != 1:
             y = super().forward(x)
             return y if out_dtype is None else y.to(out_dtype)
-        if x.shape[-1] != self.normalized_shape[0]:
-            raise ValueError(f"layer norm over {self.normalized_shape[0]} channels, got {tuple(x.shape)}")
-        return norm_ops.layer_norm(x, self.weight, self.bias, self.eps, self._dtype(x, x.dtype, out_dtype))
+        self._check(x)
+        if out_dtype is None and x.is_cuda and torch.is_autocast_enabled() and x.dtype != torch.float64:
+            out_dtype = torch.float32
+        return norm_ops.layer_norm(x, self.weight, self.bias, self.eps, out_dtype)
 
     def after_sum(self, x, residual, out_dtype=None):
         """(s, norm(s)) with s = x + residual, in one pass over memory; where the module is watched it is called with the sum, as any other."""
         if len(self.normalized_shape) != 1 or not self.plain():
             s = x + residual
             return s, self(s) if out_dtype is None else normed(self, s, out_dtype)
-        if x.shape[-1] != self.normalized_shape[0]:
-            raise ValueError(f"layer norm over {self.normalized_shape[0]} channels, got {tuple(x.shape)}")
-        dtype = torch.promote_types(x.dtype, residual.dtype)
-        return norm_ops.add_layer_norm(x, residual, self.weight, self.bias, self.eps, self._dtype(x, dtype, out_dtype))
+        self._check(x)
+        if out_dtype is None and x.is_cuda and torch.is_autocast_enabled() and torch.float64 not in (x.dtype, residual.dtype):
+            out_dtype = torch.float32
+        return norm_ops.add_layer_norm(x, residual, self.weight, self.bias, self.eps, out_dtype)
 
 
 def normed(norm: nn.Module, x: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:

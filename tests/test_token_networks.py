@@ -270,3 +270,23 @@ def test_sums_in_the_wider_type_stay_there():
         wide = torch.promote_types(a, b)
         s, y = m.after_sum(torch.randn(3, 12).to(a), torch.randn(3, 12).to(b))
         assert s.dtype == y.dtype == wide, (a, b, s.dtype, y.dtype)
+
+
+def test_networks_without_memory():
+    """Shapes and types on the meta device, as torch's own modules give them."""
+    from makani_b200.parallel.layer_norm import LayerNorm
+    m = LayerNorm(12).to("meta")
+    s, y = m.after_sum(torch.randn(3, 12, device="meta"), torch.randn(3, 12, device="meta"))
+    assert s.shape == y.shape == (3, 12) and y.is_meta
+    y = _vit("cpu").to("meta")(torch.randn(2, 5, 32, 64, device="meta"))
+    assert y.is_meta and y.shape == (2, 3, 32, 64)
+
+
+def test_norm_under_autocast_of_the_cpu():
+    """As torch's norm there: the types are those of the call."""
+    from makani_b200.parallel.layer_norm import LayerNorm
+    ours, theirs = LayerNorm(12), nn.LayerNorm(12)
+    x = torch.randn(3, 12)
+    with torch.autocast("cpu", dtype=torch.bfloat16):
+        assert ours(x).dtype == theirs(x).dtype and torch.equal(ours(x), theirs(x))
+        assert ours(x, torch.bfloat16).dtype == torch.bfloat16
