@@ -119,5 +119,9 @@ def attention_qkv(qkv: torch.Tensor, num_heads: int, num_kv_heads: Optional[int]
         o = _ext.require().attention_qkv(qkv[None] if packed else qkv, num_heads, Hk, offsets, causal, scale)
         if o is not None:
             return o[0] if packed else o
+    if Hk == num_heads and not packed:      # (views of one tensor, heads in front, whose gradient is one copy)
+        scale = _check_scale(scale, D)
+        q, k, v = qkv.reshape(*qkv.shape[:-1], 3, num_heads, D).permute(2, 0, 3, 1, 4).unbind(0)
+        return torch.nn.functional.scaled_dot_product_attention(q, k, v, is_causal=causal, scale=scale).transpose(1, 2).contiguous()
     q, k, v = qkv.unflatten(-1, (num_heads + 2 * Hk, D)).split([num_heads, Hk, Hk], dim=-2)
     return attention(q, k, v, causal, scale, offsets)
