@@ -499,7 +499,10 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) ln_bwd_kernel(LnBackward p, i
 // carries it is that several rows share shuffles and barriers.  us by (blocks, rows): forward, 74160 x 1024 bf16, (3, 2) 71, (2, 4) 63 (DRAM 46; every value through
 // all steps of the butterfly 70); 129600 x 48 7.7, 8.1; 16471 x 387 fp32 18.4, 16.1.  Forward and backward of the first (3, 1) 174, (2, 2) 157, (1, 4) 165 (DRAM
 // 116).  (A warp to a row, its weights read again for every row: 71 and 212; 16471 x 387 74.  Rows through a ring of cp.async, (2, 4) 77 and (4, 2) 86: more bytes on
-// their way are not what is missing.)  Behind a sum one row at a time: 16200 x 768 (4, 1) 21.0, (3, 2) 23.3 (DRAM 15).
+// their way are not what is missing.  Forward, a scheduler issues in 64 % of the cycles, and its warps wait for fixed latencies, shuffles and one another, hardly for
+// memory.)  Behind a sum one row at a time: 16200 x 768 (4, 1) 21.0, (3, 2) 23.3 (DRAM 15).
+// Registers: what stays in them is more than there is in some forms.  Backward behind a sum in fp32, two rows at a time at 128 registers, 120 to 200 bytes a thread are
+// spilled (16200 x 768, both passes 93 us, DRAM 61); rows of more than 1024 channels that are no whole vectors, behind a sum, 770 to 850.
 constexpr int FWD_BLOCKS = 2, BWD_BLOCKS = 2;
 constexpr int WIDE = 2048, RAGGED = LN_HALF_PARAMS;      // most channels of eight warps with one vector, or four single values, a thread
 struct Spread {
