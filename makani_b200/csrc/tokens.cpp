@@ -45,8 +45,8 @@ bool records(std::initializer_list<const Tensor*> ts) {
 // operation.
 bool plain(std::initializer_list<const Tensor*> ts) {
   using K = c10::DispatchKey;
-  const c10::DispatchKeySet watched({K::Python, K::PythonTLSSnapshot, K::Tracer, K::FuncTorchDynamicLayerFrontMode, K::Functionalize});
-  const c10::DispatchKeySet wrapped({K::Python, K::FuncTorchGradWrapper, K::FuncTorchBatched, K::Functionalize});
+  const c10::DispatchKeySet watched({K::Python, K::PythonTLSSnapshot, K::Tracer, K::FuncTorchDynamicLayerFrontMode, K::VmapMode, K::Functionalize});
+  const c10::DispatchKeySet wrapped({K::Python, K::FuncTorchGradWrapper, K::FuncTorchBatched, K::Batched, K::Functionalize});
   if (c10::impl::tls_local_dispatch_key_set().included_.has_any(watched)) return false;
   for (const Tensor* t : ts)
     if (t->defined() && (t->key_set().has_any(wrapped) || t->_fw_grad(0).defined())) return false;
@@ -210,7 +210,7 @@ std::tuple<Tensor, OptTensor, OptTensor, OptTensor> layer_norm_backward(const Te
   return {dx, maybe(dr), maybe(dw), maybe(db)};
 }
 
-// The same in torch's operations, for gradients that are to be differentiated in their turn: (dx, dweight, dbias) in fp32, dx with `ds`
+// The same in torch's operations, for gradients that are to be differentiated in their turn or are not for kernels: (dx, dweight, dbias) in fp32, dx with `ds`
 std::tuple<Tensor, Tensor, Tensor> layer_norm_backward_graph(const Tensor& x, const Tensor& dy, const Tensor& ds, const Tensor& weight, double eps) {
   const Tensor xf = x.to(at::kFloat), dyf = dy.to(at::kFloat), off = xf - xf.mean(-1, true);
   const Tensor rstd = ((off * off).mean(-1, true) + eps).rsqrt(), xh = off * rstd, g = weight.defined() ? dyf * weight.to(at::kFloat) : dyf;
@@ -254,7 +254,7 @@ struct LayerNormNode : torch::autograd::Node {
       if (need[1] && ds.defined()) out[1] = f.half ? ds.to(at::kBFloat16) : ds;
       return out;
     }
-    if (at::GradMode::is_enabled()) {      // (create_graph)
+    if (at::GradMode::is_enabled() || !plain({&x, &dy, &ds})) {      // (create_graph, batches of gradients, a traced backward pass)
       auto [dx, dw, db] = layer_norm_backward_graph(x, dy, ds, saved[1], f.eps);
       if (need[0]) out[0] = dx.to(x.scalar_type());
       if (need[1]) out[1] = dx.to(f.half ? at::kBFloat16 : x.scalar_type());

@@ -458,3 +458,23 @@ def test_a_second_backward_pass(gen):
         s.add_(1)
     with pytest.raises(RuntimeError, match="inplace"):
         torch.autograd.grad(y.sum(), x)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("residual", [False, True])
+def test_transforms_of_the_backward_pass(gen, residual):
+    """Batches of output gradients and traces of a backward pass, through a graph that the kernels made."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    x, r, dy = (torch.randn(7, 24, device="cuda", generator=gen) for _ in range(3))
+    w = torch.randn(24, device="cuda", generator=gen).requires_grad_()
+    leaves = [t.requires_grad_() for t in ((x, r) if residual else (x,))] + [w]
+    y = norm_ops.add_layer_norm(x, r, w, None)[1] if residual else norm_ops.layer_norm(x, w, None)
+    batch = torch.randn(5, 7, 24, device="cuda", generator=gen)
+    got = torch.autograd.grad(y, leaves, batch, is_grads_batched=True, retain_graph=True)
+    for i in range(5):
+        for g, t in zip(got, torch.autograd.grad(y, leaves, batch[i], retain_graph=True)):
+            assert torch.allclose(g[i], t, rtol=1e-5, atol=1e-5)
+    back = lambda d: torch.autograd.grad(y, leaves, d, retain_graph=True)  # noqa: E731
+    traced = make_fx(back)(dy)
+    for g, t in zip(traced(batch[0]), back(batch[0])):
+        assert torch.allclose(g, t, rtol=1e-5, atol=1e-5)
