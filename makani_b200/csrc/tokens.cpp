@@ -414,6 +414,7 @@ void attention_backward(const Tensor& d_out, const Tensor& q_in, const Tensor& k
                         const Tensor& lse, const OptTensor& offsets, bool causal, double scale, const Tensor& dq, const Tensor& dk, const Tensor& dv) {
   const mk::AttnShape p = shape_of(q_in, k_in, v_in, offsets, causal, scale);
   c10::cuda::CUDAGuard guard(q_in.device());
+  MK_CHECK(plain({&d_out}), "attention: the backward pass takes no batches of gradients, and is not traced");
   MK_CHECK(d_out.device() == o.device() && d_out.sizes() == o.sizes() && d_out.scalar_type() == at::kBFloat16,
            "attention: a gradient like the output expected");
   if (o.numel() == 0) return;

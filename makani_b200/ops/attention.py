@@ -10,9 +10,10 @@ not checked (out of range they are clamped to it).  Tokens behind offsets[S] bel
 zero, and what their inputs hold reaches nothing.
 
 bf16 CUDA tensors of up to 128 channels a head run on the in-tree kernels (widths that are no multiple of 8 are padded with zeros);
-anything else, and what `torch.func`, forward-mode differentiation, tracing or compilation calls, through torch.  Weights and their gradients are rounded to bf16 where they are operands of the second products; all sums
-are fp32.  What a causal mask hides has a weight of zero: queries, keys, values and output gradients of a causal sequence have to be finite, or
-outputs and gradients of earlier tokens may be NaN as well.
+anything else, and what `torch.func`, forward-mode differentiation, tracing or compilation calls, through torch.  A graph that the
+kernels made is differentiated once, and not in batches of gradients or in a trace.  Weights and their gradients are rounded to bf16
+where they are operands of the second products; all sums are fp32.  What a causal mask hides has a weight of zero: queries, keys,
+values and output gradients of a causal sequence have to be finite, or outputs and gradients of earlier tokens may be NaN as well.
 """
 
 from __future__ import annotations

@@ -640,3 +640,22 @@ assert not left, left
 """
     done = subprocess.run([sys.executable, "-c", code], cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))), capture_output=True, text=True, timeout=300)
     assert done.returncode == 0, done.stderr[-2000:]
+
+
+@pytest.mark.gpu
+def test_backward_passes_that_are_refused(gen):
+    """Batches of output gradients, and traces of a backward pass, in which the gradients would be constants."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    q, k, v, do = _inputs(gen, 2, 20, H=2, Hk=2, D=16)
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    o = attn.attention(*leaves)
+    with pytest.raises(RuntimeError, match="batches"):
+        torch.autograd.grad(o, leaves, torch.stack([do, do]), is_grads_batched=True, retain_graph=True)
+    with pytest.raises(RuntimeError, match="traced"):
+        make_fx(lambda d: torch.autograd.grad(o, leaves, d, retain_graph=True))(do)
+    want = torch.autograd.grad(o, leaves, do)
+    x = torch.cat([t.flatten(2) for t in leaves], -1).detach().requires_grad_()
+    y = attn.attention_qkv(x, 2)
+    with pytest.raises(RuntimeError, match="batches"):
+        torch.autograd.grad(y, x, torch.stack([do, do]), is_grads_batched=True, retain_graph=True)
+    assert torch.equal(torch.autograd.grad(y, x, do)[0], torch.cat([t.flatten(2) for t in want], -1))
