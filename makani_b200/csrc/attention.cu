@@ -266,9 +266,55 @@ struct TileParams {
   int D, DP;               // channels of a head, and rounded up to 16
   int group;               // heads of q that share one of k and v
   int causal;
+  int left, right, sinks;  // of a window (instances with WIN): right is 0 where causal
   float scale, scale_log2;
   int* err;
 };
+
+// ------------------------------------------------------------------------------------------ windows
+//
+// Token i sees key j if i - left <= j <= i + right, or j < sinks (and j <= i where causal).  Tiles of keys outside are not visited: a tile of queries goes
+// over those of its window and those with sinks.  Instances of the kernels without WIN are what they are without windows.
+
+// Tiles of keys that a CTA goes over, in order: `front` from `lo` on, those with sinks, and the rest of the window.  Of two query tiles the first sees
+// those up to end[0], and the second those from start on (its window begins a tile later), up to end[1]; what else one of them does not see it hides.
+struct KeyTiles {
+  int lo = 0, front = 0, sinks = 0, start = 0, end[2] = {0, 0};
+  __device__ __forceinline__ int operator()(int j) const { return j < front ? lo + j : j < front + sinks ? j - front : lo + j - sinks; }
+};
+__device__ __forceinline__ int last_seen(const TileParams& p, int i, int len) { return p.causal || i >= len ? min(i, len - 1) : p.right < len - 1 - i ? i + p.right : len - 1; }
+__device__ __forceinline__ KeyTiles key_tiles(const TileParams& p, int r0, int rows, int len) {
+  KeyTiles k;
+  if (rows <= 0) return k;
+  const bool two = rows > TILE;
+  const int last[2] = {r0 + min(rows, TILE) - 1, r0 + rows - 1};
+  const int lo0 = max(r0 - p.left, 0) / TILE, lo1 = max(r0 + TILE - p.left, 0) / TILE;
+  const int hi0 = last_seen(p, last[0], len) / TILE + 1, hi1 = last_seen(p, last[1], len) / TILE + 1;
+  k.sinks = (min(p.sinks, p.causal ? last[1] + 1 : len) + TILE - 1) / TILE;
+  if (k.sinks > 0 && lo0 <= k.sinks) {      // they meet
+    k.end[0] = max(hi0, k.sinks);
+    k.end[1] = two ? max(hi1, k.sinks) : 0;
+    k.sinks = 0;
+    return k;
+  }
+  k.lo = lo0;
+  k.front = k.start = two ? lo1 - lo0 : 0;
+  k.end[0] = hi0 - lo0 + k.sinks;
+  k.end[1] = two ? hi1 - lo0 + k.sinks : 0;
+  return k;
+}
+// The keys from k0 on that token i sees, as columns: from `from` to `to`, and those below `sinks`
+struct SeenKeys {
+  int from, to, sinks;
+  __device__ __forceinline__ SeenKeys(const TileParams& p, int i, int len, int k0)
+      : from(i - p.left - k0), to(last_seen(p, i, len) + 1 - k0), sinks(min(p.sinks, p.causal ? min(i + 1, len) : len) - k0) {}
+  __device__ __forceinline__ bool operator()(int c) const { return (c >= from && c < to) || c < sinks; }
+};
+// Whether every one of the 128 tokens from `first` on sees all of `n` keys from k0 on
+__device__ __forceinline__ bool all_seen(const TileParams& p, int first, int len, int k0, int n) {
+  if (k0 + n > len || (p.causal && k0 + n - 1 > first)) return false;
+  return k0 + n <= p.sinks || (k0 >= first + TILE - 1 - p.left && k0 + n - 1 - first <= p.right);
+}
 
 // 16 (or the first 8) fp32 values as bf16
 __device__ __forceinline__ void store16(const uint32_t (&v)[16], __nv_bfloat16* to, bool all) {
@@ -316,10 +362,11 @@ template <bool SPLIT>
 struct ShareOf {
   uint32_t unit;
   int part, first, n;
-  __device__ __forceinline__ explicit ShareOf(const Parts& s) : unit(blockIdx.x), part(-1) {
-    if (SPLIT && s.parts > 0 && blockIdx.x >= s.whole) {
-      unit = s.whole + (blockIdx.x - s.whole) / s.parts;
-      part = static_cast<int>((blockIdx.x - s.whole) % s.parts);
+  __device__ __forceinline__ explicit ShareOf(const Parts& s) : ShareOf(s, blockIdx.x) {}
+  __device__ __forceinline__ ShareOf(const Parts& s, uint32_t block) : unit(block), part(-1) {
+    if (SPLIT && s.parts > 0 && block >= s.whole) {
+      unit = s.whole + (block - s.whole) / s.parts;
+      part = static_cast<int>((block - s.whole) % s.parts);
     }
   }
   __device__ __forceinline__ void along(const Parts& s, int tiles) {
@@ -412,6 +459,11 @@ __device__ __forceinline__ void hide_scores(uint32_t (&v)[TILE], int seen) {
   for (int c = 0; c < TILE; ++c)
     if (c >= seen) v[c] = 0xff800000u;
 }
+__device__ __forceinline__ void hide_scores(uint32_t (&v)[TILE], const SeenKeys& seen) {
+#pragma unroll
+  for (int c = 0; c < TILE; ++c)
+    if (!seen(c)) v[c] = 0xff800000u;
+}
 __device__ __forceinline__ void store_weights(uint32_t p_at, const uint32_t (&v)[TILE]) {
   tmem_st32(p_at, v);
   tmem_st32(p_at + 32, v + 32);
@@ -458,7 +510,7 @@ struct FwdParams {
   float* lse;
 };
 
-template <int DB, int QT>
+template <int DB, int QT, bool WIN>
 __global__ void __launch_bounds__(Fwd<DB, QT>::THREADS_, 3 - QT)
 attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                 const FwdParams p) {
@@ -515,15 +567,18 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     const int last = causal ? w.r0 + min(rows, (t + 1) * TILE) - 1 : w.len - 1;
     return last / TILE + 1;
   };
-  int n0 = tiles_of(0), n1 = tiles_of(1);
+  KeyTiles keys;
+  if constexpr (WIN) keys = key_tiles(p.t, w.r0, w.padding ? 0 : rows, w.len);
+  int n0 = WIN ? keys.end[0] : tiles_of(0), n1 = WIN ? keys.end[1] : tiles_of(1);
   share.along(p.split, max(n0, n1));
   const int n = share.n, j0 = share.first;
   if (share.part >= 0) {      // (not causal: both see the same keys)
     n0 = n0 > 0 ? n : 0;
     n1 = n1 > 0 ? n : 0;
   }
+  auto tile = [&](int j) { return WIN ? keys(j) : j0 + j; };
   // keys of the last tile that belong to the sequence, where other tokens follow it
-  const int tail = w.len - (j0 + n - 1) * TILE;
+  const int tail = w.len - tile(n - 1) * TILE;
   const bool fix = n > 0 && tail < TILE && w.lo + w.len < p.t.grid.N;
 
   if (warp < COMPUTE_WARP) {
@@ -543,13 +598,13 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
           break;
         }
         mbar_expect_tx(k_full(s), L::TILE_BYTES);
-        for (int b = 0; b < DB; ++b) tma_load_4d(base + L::K_AT + s * L::TILE_BYTES + b * BOX, &map_k, k_full(s), b * 64, w.lo + (j0 + j) * TILE, hk, w.b);
+        for (int b = 0; b < DB; ++b) tma_load_4d(base + L::K_AT + s * L::TILE_BYTES + b * BOX, &map_k, k_full(s), b * 64, w.lo + tile(j) * TILE, hk, w.b);
         if (!mbar_wait(v_empty(s), ph ^ 1u)) {
           atomicExch(p.t.err, 80);
           break;
         }
         mbar_expect_tx(v_full(s), L::TILE_BYTES);
-        for (int b = 0; b < DB; ++b) tma_load_4d(base + L::V_AT + s * L::TILE_BYTES + b * BOX, &map_v, v_full(s), b * 64, w.lo + (j0 + j) * TILE, hk, w.b);
+        for (int b = 0; b < DB; ++b) tma_load_4d(base + L::V_AT + s * L::TILE_BYTES + b * BOX, &map_v, v_full(s), b * 64, w.lo + tile(j) * TILE, hk, w.b);
         if (++s == L::STAGES) {
           s = 0;
           ph ^= 1u;
@@ -576,7 +631,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       if (ok) {
         tc_fence_after();
         if (n0 > 0) scores(0, 0);
-        if (n1 > 0) scores(1, 0);
+        if (n1 > 0 && keys.start == 0) scores(1, 0);
         tc_commit(k_empty(0));
       }
       int s = 0;
@@ -596,9 +651,13 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         }
         tc_fence_after();
         for (int t = 0; t < 2 && ok; ++t) {
-          const int nt = t == 0 ? n0 : n1;
+          const int nt = t == 0 ? n0 : n1, start = t == 0 ? 0 : keys.start;
           if (j >= nt) continue;
-          if (!mbar_wait(p_ready(t), j & 1)) {
+          if (WIN && j < start) {      // (the first is the next one)
+            scores(t, sn);
+            continue;
+          }
+          if (!mbar_wait(p_ready(t), (j - start) & 1)) {
             atomicExch(p.t.err, 83);
             ok = false;
             break;
@@ -607,7 +666,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
           const uint32_t b = v_lo + s * (L::TILE_BYTES >> 4);
 #pragma unroll
           for (int i = 0; i < TILE / 16; ++i)
-            mma_ts(tmem + L::O_AT + t * ATTN_WIDTH, tmem + t * S_COLS + i * 8, b + i * (2048 >> 4), hi, id_o, j > 0 || i > 0);
+            mma_ts(tmem + L::O_AT + t * ATTN_WIDTH, tmem + t * S_COLS + i * 8, b + i * (2048 >> 4), hi, id_o, j > start || i > 0);
           // (in order behind the products above: S takes the place of P)
           if (j + 1 < nt) scores(t, sn);
           else tc_commit(s_full(t));
@@ -636,19 +695,24 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     const bool here = row < rows;
     Row r;
     bool ok = true;
-    for (int j = 0; j < nt; ++j) {
-      ok = __all_sync(0xffffffffu, mbar_wait(s_full(t), j & 1));
+    const int start = t == 0 ? 0 : keys.start;
+    for (int j = start; j < nt; ++j) {
+      ok = __all_sync(0xffffffffu, mbar_wait(s_full(t), (j - start) & 1));
       if (!ok) break;
       tc_fence_after();
       uint32_t v[TILE];
       load_scores(s_at, v);
-      const int k0 = (j0 + j) * TILE;
-      if (k0 + TILE > w.len || (causal && k0 + TILE - 1 > w.r0 + t * TILE)) hide_scores(v, (causal ? min(w.len, w.r0 + row + 1) : w.len) - k0);
+      const int k0 = tile(j) * TILE;
+      if constexpr (WIN) {
+        if (!all_seen(p.t, w.r0 + t * TILE, w.len, k0, TILE)) hide_scores(v, SeenKeys(p.t, w.r0 + row, w.len, k0));
+      } else if (k0 + TILE > w.len || (causal && k0 + TILE - 1 > w.r0 + t * TILE)) {
+        hide_scores(v, (causal ? min(w.len, w.r0 + row + 1) : w.len) - k0);
+      }
       const float top = max_of<false>(v) * scale;
       if (__any_sync(0xffffffffu, r.grows(top))) {
         // (the scores of tile j are behind the products of tile j - 1: O is complete up to there)
         const float f = r.grow(top);
-        if (j > 0) scale_row(o_at, p.t.DP, f);
+        if (j > start) scale_row(o_at, p.t.DP, f);
       }
       r.weights(v, scale);
       store_weights(s_at, v);
@@ -656,7 +720,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       __syncwarp();
       if (lane == 0) mbar_arrive(p_ready(t));
     }
-    if (nt > 0 && ok) ok = __all_sync(0xffffffffu, mbar_wait(s_full(t), nt & 1));
+    if (nt > 0 && ok) ok = __all_sync(0xffffffffu, mbar_wait(s_full(t), (nt - start) & 1));
     if (!ok && lane == 0) atomicExch(p.t.err, 84);
     const long long token = static_cast<long long>(w.b) * p.t.grid.N + w.lo + w.r0 + row;
     __nv_bfloat16* const to = p.o + (token * p.t.grid.H + w.h) * p.t.D;
@@ -696,6 +760,7 @@ struct FwdNarrow {
   static_assert(SMEM <= SMEM_LIMIT);
 };
 
+template <bool WIN>
 __global__ void __launch_bounds__(THREADS, 1)
 attn_fwd_narrow_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                        const FwdParams p) {
@@ -753,14 +818,17 @@ attn_fwd_narrow_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     const int last = causal ? w.r0 + min(rows, (t + 1) * TILE) - 1 : w.len - 1;
     return last / TILE + 1;
   };
-  int n0 = tiles_of(0), n1 = tiles_of(1);
+  KeyTiles keys;
+  if constexpr (WIN) keys = key_tiles(p.t, w.r0, w.padding ? 0 : rows, w.len);
+  int n0 = WIN ? keys.end[0] : tiles_of(0), n1 = WIN ? keys.end[1] : tiles_of(1);
   share.along(p.split, max(n0, n1));
   const int n = share.n, j0 = share.first;
   if (share.part >= 0) {      // (not causal: both see the same keys)
     n0 = n0 > 0 ? n : 0;
     n1 = n1 > 0 ? n : 0;
   }
-  const int tail = w.len - (j0 + n - 1) * TILE;
+  auto tile = [&](int j) { return WIN ? keys(j) : j0 + j; };
+  const int tail = w.len - tile(n - 1) * TILE;
   const bool fix = n > 0 && tail < TILE && w.lo + w.len < p.t.grid.N;
 
   if (warp < COMPUTE_WARP) {
@@ -779,13 +847,13 @@ attn_fwd_narrow_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             break;
           }
           mbar_expect_tx(k_full(s), BOX);
-          tma_load_4d(base + L::K_AT + s * BOX, &map_k, k_full(s), 0, w.lo + (j0 + j) * TILE, hk, w.b);
+          tma_load_4d(base + L::K_AT + s * BOX, &map_k, k_full(s), 0, w.lo + tile(j) * TILE, hk, w.b);
           if (!mbar_wait(v_empty(s), ph ^ 1u)) {
             atomicExch(p.t.err, 80);
             break;
           }
           mbar_expect_tx(v_full(s), BOX);
-          tma_load_4d(base + L::V_AT + s * BOX, &map_v, v_full(s), 0, w.lo + (j0 + j) * TILE, hk, w.b);
+          tma_load_4d(base + L::V_AT + s * BOX, &map_v, v_full(s), 0, w.lo + tile(j) * TILE, hk, w.b);
           if (++s == L::STAGES) {
             s = 0;
             ph ^= 1u;
@@ -795,7 +863,7 @@ attn_fwd_narrow_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     } else if (warp & 1) {
       // ---------------------------------------------------------------- products, a warp for either query tile
       if (n > 0 && elect_one()) {
-        const int t = warp >> 1, nt = t == 0 ? n0 : n1;
+        const int t = warp >> 1, nt = t == 0 ? n0 : n1, start = t == 0 ? 0 : keys.start;
         const uint32_t hi = desc_hi(1024);
         const uint32_t q_lo = desc_lo(base + t * BOX, 16), k_lo = desc_lo(base + L::K_AT, 16), v_lo = desc_lo(base + L::V_AT, BOX);
         const uint32_t id_s = idesc_n(TILE), id_o = idesc_n(p.t.DP) | B_MN, o = tmem + L::O_AT + t * 64, a = tmem + L::P_AT + t * 64;
@@ -809,7 +877,7 @@ attn_fwd_narrow_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         if (!ok) atomicExch(p.t.err, 81);
         if (ok) {
           tc_fence_after();
-          if (nt > 0) scores(0);
+          if (nt > 0 && start == 0) scores(0);
           tc_commit(k_empty(0));
         }
         int s = 0;
@@ -819,7 +887,7 @@ attn_fwd_narrow_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
           const uint32_t phn = sn == 0 ? ph ^ 1u : ph;
           // (a tile that this warp has no use for is given back as soon as it is there)
           if (j + 1 < n) {
-            ok = mbar_wait(k_full(sn), phn) && (j + 1 >= nt || mbar_wait(s_read(t), j & 1));
+            ok = mbar_wait(k_full(sn), phn) && (j + 1 >= nt || j < start || mbar_wait(s_read(t), (j - start) & 1));
             if (!ok) {
               atomicExch(p.t.err, 82);
               break;
@@ -833,16 +901,16 @@ attn_fwd_narrow_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             mbar_arrive(v_fix);
             ok = mbar_wait(v_fixed, 0);
           }
-          if (ok && j < nt) ok = mbar_wait(p_ready(t), j & 1);
+          if (ok && j >= start && j < nt) ok = mbar_wait(p_ready(t), (j - start) & 1);
           if (!ok) {
             atomicExch(p.t.err, 83);
             break;
           }
           tc_fence_after();
-          if (j < nt) {
+          if (j >= start && j < nt) {
             const uint32_t b = v_lo + s * (BOX >> 4);
 #pragma unroll
-            for (int k = 0; k < TILE / 16; ++k) mma_ts(o, a + k * 8, b + k * (2048 >> 4), hi, id_o, j > 0 || k > 0);
+            for (int k = 0; k < TILE / 16; ++k) mma_ts(o, a + k * 8, b + k * (2048 >> 4), hi, id_o, j > start || k > 0);
             tc_commit(o_done(t));
           }
           tc_commit(v_empty(s));
@@ -867,8 +935,9 @@ attn_fwd_narrow_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     const bool here = row < rows;
     Row r;
     bool ok = true;
-    for (int j = 0; j < nt; ++j) {
-      ok = __all_sync(0xffffffffu, mbar_wait_soon(s_full(t), j & 1));
+    const int start = t == 0 ? 0 : keys.start;
+    for (int j = start; j < nt; ++j) {
+      ok = __all_sync(0xffffffffu, mbar_wait_soon(s_full(t), (j - start) & 1));
       if (!ok) break;
       tc_fence_after();
       uint32_t v[TILE];
@@ -876,21 +945,25 @@ attn_fwd_narrow_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(s_read(t));
-      const int k0 = (j0 + j) * TILE;
-      if (k0 + TILE > w.len || (causal && k0 + TILE - 1 > w.r0 + t * TILE)) hide_scores(v, (causal ? min(w.len, w.r0 + row + 1) : w.len) - k0);
+      const int k0 = tile(j) * TILE;
+      if constexpr (WIN) {
+        if (!all_seen(p.t, w.r0 + t * TILE, w.len, k0, TILE)) hide_scores(v, SeenKeys(p.t, w.r0 + row, w.len, k0));
+      } else if (k0 + TILE > w.len || (causal && k0 + TILE - 1 > w.r0 + t * TILE)) {
+        hide_scores(v, (causal ? min(w.len, w.r0 + row + 1) : w.len) - k0);
+      }
       const float top = max_of<true>(v) * scale;
       if (__any_sync(0xffffffffu, r.grows(top))) {
         const float f = r.grow(top);
-        if (j > 0) {
-          ok = __all_sync(0xffffffffu, mbar_wait(o_done(t), (j - 1) & 1));
+        if (j > start) {
+          ok = __all_sync(0xffffffffu, mbar_wait(o_done(t), (j - start - 1) & 1));
           if (!ok) break;
           tc_fence_after();
           scale_row(o_at, p.t.DP, f);
         }
       }
       r.weights(v, scale);
-      if (j > 0) {
-        ok = __all_sync(0xffffffffu, mbar_wait_soon(o_done(t), (j - 1) & 1));
+      if (j > start) {
+        ok = __all_sync(0xffffffffu, mbar_wait_soon(o_done(t), (j - start - 1) & 1));
         if (!ok) break;
         tc_fence_after();
       }
@@ -899,7 +972,7 @@ attn_fwd_narrow_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
       __syncwarp();
       if (lane == 0) mbar_arrive(p_ready(t));
     }
-    if (nt > 0 && ok) ok = __all_sync(0xffffffffu, mbar_wait(o_done(t), (nt - 1) & 1));
+    if (nt > 0 && ok) ok = __all_sync(0xffffffffu, mbar_wait(o_done(t), (nt - start - 1) & 1));
     if (!ok && lane == 0) atomicExch(p.t.err, 84);
     const long long token = static_cast<long long>(w.b) * p.t.grid.N + w.lo + w.r0 + row;
     __nv_bfloat16* const to = p.o + (token * p.t.grid.H + w.h) * p.t.D;
@@ -1037,7 +1110,7 @@ struct DqParams {
   AttnTensor dq;
 };
 
-template <int DB, bool SPLIT>
+template <int DB, bool SPLIT, bool WIN>
 __global__ void __launch_bounds__(BWD_THREADS, 1)
 attn_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                const __grid_constant__ CUtensorMap map_do, const DqParams p) {
@@ -1084,9 +1157,12 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
   const bool any = find_work(p.t.grid, offsets, share.unit, w);
   const int rows = any ? min(w.len - w.r0, TILE) : 0;
   const bool causal = p.t.causal != 0;
-  share.along(p.split, rows == 0 || w.padding ? 0 : (causal ? w.r0 + rows - 1 : w.len - 1) / TILE + 1);
+  KeyTiles keys;
+  if constexpr (WIN) keys = key_tiles(p.t, w.r0, w.padding ? 0 : rows, w.len);
+  share.along(p.split, WIN ? keys.end[0] : rows == 0 || w.padding ? 0 : (causal ? w.r0 + rows - 1 : w.len - 1) / TILE + 1);
   const int n = share.n, j0 = share.first;
-  const int tail = w.len - (j0 + n - 1) * TILE;
+  auto tile = [&](int j) { return WIN ? keys(j) : j0 + j; };
+  const int tail = w.len - tile(n - 1) * TILE;
   const bool fix = n > 0 && tail < TILE && w.lo + w.len < p.t.grid.N;
 
   if (warp < COMPUTE_WARP) {
@@ -1108,13 +1184,13 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
             break;
           }
           mbar_expect_tx(k_full(s), L::TILE_BYTES);
-          for (int b = 0; b < DB; ++b) tma_load_4d(base + L::K_AT + s * L::TILE_BYTES + b * BOX, &map_k, k_full(s), b * 64, w.lo + (j0 + j) * TILE, hk, w.b);
+          for (int b = 0; b < DB; ++b) tma_load_4d(base + L::K_AT + s * L::TILE_BYTES + b * BOX, &map_k, k_full(s), b * 64, w.lo + tile(j) * TILE, hk, w.b);
           if (!mbar_wait(v_empty(s), ph ^ 1u)) {
             atomicExch(p.t.err, 85);
             break;
           }
           mbar_expect_tx(v_full(s), L::TILE_BYTES);
-          for (int b = 0; b < DB; ++b) tma_load_4d(base + L::V_AT + s * L::TILE_BYTES + b * BOX, &map_v, v_full(s), b * 64, w.lo + (j0 + j) * TILE, hk, w.b);
+          for (int b = 0; b < DB; ++b) tma_load_4d(base + L::V_AT + s * L::TILE_BYTES + b * BOX, &map_v, v_full(s), b * 64, w.lo + tile(j) * TILE, hk, w.b);
           if (++s == L::STAGES) {
             s = 0;
             ph ^= 1u;
@@ -1224,10 +1300,11 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
       uint32_t v[BWD_COLS];
       const uint32_t s_at = tmem + lanes + (j & 1) * S_COLS + x * BWD_COLS, dp_at = tmem + lanes + DQ_DP + x * BWD_COLS;
       tmem_req32(s_at, v);
-      const int k0 = (j0 + j) * TILE + x * BWD_COLS;
-      const bool edge = k0 + BWD_COLS > w.len || (causal && k0 + BWD_COLS - 1 > w.r0);
-      const int keys = (causal ? min(w.len, w.r0 + row + 1) : w.len) - k0;
-      auto seen = [&](int c) { return c < keys; };
+      const int k0 = tile(j) * TILE + x * BWD_COLS;
+      const bool edge = WIN ? !all_seen(p.t, w.r0, w.len, k0, BWD_COLS) : k0 + BWD_COLS > w.len || (causal && k0 + BWD_COLS - 1 > w.r0);
+      const int below = (causal ? min(w.len, w.r0 + row + 1) : w.len) - k0;
+      const SeenKeys in_window(p.t, w.r0 + row, w.len, k0);
+      auto seen = [&](int c) { return WIN ? in_window(c) : c < below; };
       tmem_wait32(v);
       weights_of<false>(v, scale2, [&](int) { return l2; }, seen);
       ok = __all_sync(0xffffffffu, mbar_wait_soon(dp_full, j & 1));
@@ -1278,16 +1355,51 @@ struct Dkv {
   static_assert(SMEM <= SMEM_LIMIT && DK_AT + DB * 64 == 512);
 };
 
+// Windows: tiles with sinks are seen by all queries of their sequence, and go apart.  The first units x parts CTAs have them: unit (sequence, head of keys, tile),
+// in as many parts, along queries and heads, as have two tiles of queries each, and leave sums; the others have the rest.
+struct SinkTiles {
+  int parts, tiles;        // parts 0: nothing goes apart
+  uint32_t units;
+  __host__ __device__ int parts_of(int total) const {      // that have something to do
+    const int most = total / 2 > 1 ? total / 2 : 1;
+    return parts < most ? parts : most;
+  }
+};
+// Queries of `len` that see the keys r0 .. of a tile: tiles of them from `first` on
+struct QueryTiles {
+  int first, n;
+  __device__ __forceinline__ QueryTiles(const TileParams& p, int r0, int rows, int len) {
+    const bool sinks = r0 < p.sinks;
+    const int lo = p.causal ? r0 : sinks ? 0 : max(r0 - p.right, 0), key = r0 + rows - 1;
+    const int hi = sinks || p.left >= len - 1 - key ? len - 1 : key + p.left;
+    first = lo / TILE;
+    n = rows > 0 ? hi / TILE + 1 - first : 0;
+  }
+};
+__device__ __forceinline__ bool find_sinks(const Slots& g, const int* offsets, const SinkTiles& s, uint32_t unit, Work& w) {
+  const int tile = static_cast<int>(unit % s.tiles);
+  const uint32_t rest = unit / s.tiles;
+  w.h = static_cast<int>(rest % g.H);
+  const int sequence = static_cast<int>(rest / g.H);
+  w.b = offsets ? 0 : sequence;
+  w.lo = offsets && sequence > 0 ? clamp_offset(__ldg(offsets + sequence), g.N) : 0;
+  w.len = offsets ? max(clamp_offset(__ldg(offsets + sequence + 1), g.N) - w.lo, 0) : g.N;
+  w.r0 = tile * TILE;
+  w.padding = false;
+  return w.r0 < w.len;
+}
+
 struct DkvParams {
   TileParams t;
   Parts split;             // over the queries
+  SinkTiles sinks;
   float *dk_sums, *dv_sums;
   int heads_q;
   const float *lse, *delta;
   AttnTensor dk, dv;
 };
 
-template <int DB, bool SPLIT>
+template <int DB, bool SPLIT, bool WIN>
 __global__ void __launch_bounds__(BWD_THREADS, 1)
 attn_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                 const __grid_constant__ CUtensorMap map_do, const DkvParams p) {
@@ -1332,12 +1444,32 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
 
   Work w;
   ShareOf<SPLIT> share(p.split);
-  const bool any = find_work(p.t.grid, offsets, share.unit, w);
+  bool any, apart = false;
+  if constexpr (WIN && SPLIT) {
+    const uint32_t first = p.sinks.units * p.sinks.parts;
+    apart = blockIdx.x < first;
+    if (!apart) share = ShareOf<SPLIT>(p.split, blockIdx.x - first);
+    any = apart ? find_sinks(p.t.grid, offsets, p.sinks, blockIdx.x / p.sinks.parts, w) : find_work(p.t.grid, offsets, share.unit, w);
+    if (!apart && any && first > 0 && !w.padding && w.r0 < p.t.sinks) any = false;
+  } else {
+    any = find_work(p.t.grid, offsets, share.unit, w);
+  }
   const int rows = any ? min(w.len - w.r0, TILE) : 0;
   const bool causal = p.t.causal != 0;
   // tiles of queries, from the first that sees one of these keys, of one head after the other
-  const int q_first = causal ? w.r0 / TILE : 0, q_tiles = rows == 0 || w.padding ? 0 : (w.len + TILE - 1) / TILE - q_first;
+  const QueryTiles queries(p.t, w.r0, w.padding ? 0 : rows, w.len);
+  const int q_first = WIN ? queries.first : causal ? w.r0 / TILE : 0,
+            q_tiles = WIN ? queries.n : rows == 0 || w.padding ? 0 : (w.len + TILE - 1) / TILE - q_first;
   share.along(p.split, q_tiles * p.t.group);
+  if constexpr (WIN && SPLIT) {
+    if (apart) {
+      const int total = q_tiles * p.t.group, parts = p.sinks.parts_of(total);
+      share.unit = blockIdx.x / p.sinks.parts;
+      share.part = static_cast<int>(blockIdx.x % p.sinks.parts);
+      share.first = share.part < parts ? static_cast<int>(static_cast<long long>(total) * share.part / parts) : 0;
+      share.n = share.part < parts ? static_cast<int>(static_cast<long long>(total) * (share.part + 1) / parts) - share.first : 0;
+    }
+  }
   // first tile of queries and head of this CTA
   const int n = share.n, t0 = q_tiles > 0 ? share.first % q_tiles : 0, g0 = q_tiles > 0 ? share.first / q_tiles : 0, h0 = w.h * p.t.group;
   const int tail = w.len - (q_first + q_tiles - 1) * TILE;
@@ -1493,9 +1625,11 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       }
     } else if (fix) {
       // ---------------------------------------------------------------- queries of the next sequence
-      for (int g = 0; g < n / q_tiles; ++g) {
+      // (a part of a tile with sinks may begin in the middle of a head's queries)
+      const int before = WIN ? t0 : 0;
+      for (int g = 0; g < (before + n) / q_tiles; ++g) {
         if (!wait_long(fix_bar, g & 1, q_tiles)) break;
-        clear_rows(smem_raw + pad + L::STAGE_AT + (g * q_tiles + q_tiles - 1) % L::STAGES * L::STAGE, 2 * DB, tail);
+        clear_rows(smem_raw + pad + L::STAGE_AT + (g * q_tiles + q_tiles - 1 - before) % L::STAGES * L::STAGE, 2 * DB, tail);
         if (lane == 0) mbar_arrive(fixed);
       }
     }
@@ -1517,8 +1651,16 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       const float* const stats = reinterpret_cast<const float*>(smem_raw + pad + L::STAT_AT + s * L::STAT) + x * BWD_COLS;
       const int q0 = (q_first + t) * TILE + x * BWD_COLS;
       // the queries that see this key are the columns from `from` to `to`
-      const bool edge = q0 + BWD_COLS > w.len || (causal && q0 < w.r0 + TILE - 1);
-      const int from = causal ? w.r0 + row - q0 : 0, to = w.len - q0;
+      bool edge = q0 + BWD_COLS > w.len || (causal && q0 < w.r0 + TILE - 1);
+      int from = causal ? w.r0 + row - q0 : 0, to = w.len - q0;
+      if constexpr (WIN) {
+        const int key = w.r0 + row;
+        if (w.r0 + TILE > p.t.sinks) edge = edge || q0 + BWD_COLS - 1 - w.r0 > p.t.left || (!causal && q0 < w.r0 + TILE - 1 - p.t.right);
+        if (key >= p.t.sinks) {
+          if (!causal) from = key - p.t.right - q0;
+          if (p.t.left < w.len - 1 - key) to = key + p.t.left + 1 - q0;
+        }
+      }
       auto seen = [&](int c) { return c >= from && c < to; };
       auto neg_l = [&](int c) { return *reinterpret_cast<const f32x2*>(stats + c); };
       auto neg_delta = [&](int c) { return *reinterpret_cast<const f32x2*>(stats + TILE + c); };
@@ -1563,8 +1705,10 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     if (n > 0 && ok) {
       tc_fence_after();
       const uint32_t acc = tmem + lanes + (values ? L::DV_AT : L::DK_AT);
-      if (SPLIT && share.part >= 0)
-        store_part(acc, p.t.D, (values ? p.dv_sums : p.dk_sums) + share.row(p.split, TILE, row) * p.t.D, here, (x & 1) * 8, 16);
+      if (SPLIT && share.part >= 0) {
+        const long long at = WIN && apart ? static_cast<long long>(blockIdx.x) * TILE + row : share.row(p.split, TILE, row);
+        store_part(acc, p.t.D, (values ? p.dv_sums : p.dk_sums) + at * p.t.D, here, (x & 1) * 8, 16);
+      }
       else store_row(acc, p.t.D, values ? 1.f : p.t.scale, to, here, (x & 1) * 16, 32);
     } else if (here && w.padding && (x & 1) == 0) {
       zero_row(p.t.D, to);
@@ -1605,6 +1749,28 @@ __global__ void __launch_bounds__(256) attn_sum_kernel(Slots grid, Parts split, 
       make_uint2(pack_bf16(a.x * f, a.y * f), pack_bf16(a.z * f, a.w * f));
 }
 
+// The same for tiles with sinks that went apart
+__global__ void __launch_bounds__(256) attn_sink_sum_kernel(TileParams t, SinkTiles s, Sums p) {
+  const float* parts = p.parts[blockIdx.y];
+  const int* offsets = t.grid.offsets;
+  chain_begin(true, parts, offsets);
+  const int lane = threadIdx.x & 31, c = lane * 4;
+  const uint32_t at = blockIdx.x * 8 + (threadIdx.x >> 5), unit = at / TILE;
+  const int row = static_cast<int>(at % TILE);
+  Work w;
+  if (!find_sinks(t.grid, offsets, s, unit, w) || w.r0 + row >= w.len || c >= t.D) return;
+  const int n = s.parts_of(QueryTiles(t, w.r0, min(w.len - w.r0, TILE), w.len).n * t.group);
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int k = 0; k < n; ++k) {
+    const float4 v = __ldcg(reinterpret_cast<const float4*>(parts + ((static_cast<long long>(unit) * s.parts + k) * TILE + row) * t.D + c));
+    a = make_float4(a.x + v.x, a.y + v.y, a.z + v.z, a.w + v.w);
+  }
+  const float f = p.factor[blockIdx.y];
+  const AttnTensor& o = p.out[blockIdx.y];
+  *reinterpret_cast<uint2*>(o.ptr + w.b * o.batch + (w.lo + w.r0 + row) * o.token + w.h * o.head + c) =
+      make_uint2(pack_bf16(a.x * f, a.y * f), pack_bf16(a.z * f, a.w * f));
+}
+
 // ------------------------------------------------------------------------------------------ host
 
 bool map_of(CUtensorMap* map, const AttnTensor& t, const AttnShape& p, int heads) {
@@ -1624,7 +1790,7 @@ Slots slots_of(const AttnShape& p, int heads, int rows, int causal_order) {
   g.N = p.N;
   g.H = heads;
   g.rows = rows;
-  g.order = p.causal ? causal_order : 0;
+  g.order = p.causal && !p.window ? causal_order : 0;
   g.slots = p.offsets ? p.N / rows + p.sequences + 1 : (p.N + rows - 1) / rows;
   g.offsets = p.offsets;
   g.sequences = p.sequences;
@@ -1634,7 +1800,8 @@ long long blocks_of(const Slots& g) { return 1ll * g.slots * g.H * g.B; }
 
 bool shape_ok(const AttnShape& p) {
   return p.B > 0 && p.N > 0 && p.H > 0 && p.Hk > 0 && p.H % p.Hk == 0 && p.D > 0 && p.D % 8 == 0 && p.D <= ATTN_WIDTH && p.scale > 0.f &&
-         (!p.offsets || (p.B == 1 && p.sequences >= 0)) && blocks_of(slots_of(p, p.H, TILE, 1)) < (1ll << 31);
+         (!p.offsets || (p.B == 1 && p.sequences >= 0)) &&
+         (!p.window || (p.left >= 0 && p.left <= p.N && p.right >= 0 && p.right <= p.N && p.sinks >= 0 && p.sinks <= p.N)) && blocks_of(slots_of(p, p.H, TILE, 1)) < (1ll << 31);
 }
 
 TileParams tile_params(const AttnShape& p, const Slots& g, int* err) {
@@ -1644,6 +1811,9 @@ TileParams tile_params(const AttnShape& p, const Slots& g, int* err) {
   t.DP = (p.D + 15) / 16 * 16;
   t.group = p.H / p.Hk;
   t.causal = p.causal;
+  t.left = p.left;
+  t.right = p.causal ? 0 : p.right;
+  t.sinks = p.window ? p.sinks : 0;
   t.scale = p.scale;
   t.scale_log2 = p.scale * LOG2E;
   t.err = err;
@@ -1655,8 +1825,14 @@ TileParams tile_params(const AttnShape& p, const Slots& g, int* err) {
 // 1024 x 8 35.7 / 36.5, 2 x 4096 x 8 104 / 121; fitting at once 16 x 128 x 8 5.4 / 6.2, 16 x 256 x 8 8.7 / 8.5.  Heads of 96: 64 x 128 x 8 23.4 / 16.3, 32 x 384 x 8
 // 41.6 / 35.4, 16 x 512 x 8 27.7 / 28.3, 8 x 768 x 8 34.0 / 34.9; packed, 41 sequences of 7001 tokens 52.7 / 45.6.  (Lengths of packed sequences are on the
 // device: their mean is known.)
+int mean_length(const AttnShape& p) { return p.offsets ? p.N / std::max(1, p.sequences) : p.N; }
+// Tiles that one tile sees through a window, a sequence permitting
+int window_tiles(const AttnShape& p) {
+  const long long span = 1ll * p.left + (p.causal ? 0 : p.right) + TILE;
+  return static_cast<int>(std::min<long long>((span + TILE - 1) / TILE + 1, (mean_length(p) + TILE - 1) / TILE));
+}
 bool one_tile_pays(const AttnShape& p) {
-  const int mean = p.offsets ? p.N / std::max(1, p.sequences) : p.N;
+  const int mean = p.window ? std::min(mean_length(p), window_tiles(p) * TILE) : mean_length(p);
   return mean <= (p.D <= 64 ? 768 : 448) && blocks_of(slots_of(p, p.H, 2 * TILE, 1)) > sm_count();
 }
 // CTAs of one length that would be a last wave of their own, or that are fewer than the SMs, are split over the keys so that they fill them, where that saves more
@@ -1668,7 +1844,7 @@ bool one_tile_pays(const AttnShape& p) {
 // 82 / 86, 2 x 1536, 2 of 96 75 / 81.
 constexpr int MIN_SAVED = 8, MIN_SAVED_WIDE = 12;
 Parts parts_of(const AttnShape& p, const Slots& g, int tiles, int min_saved) {
-  if (p.offsets || p.causal) return {0, 0};      // (not of one length)
+  if (p.offsets || p.causal || p.window) return {0, 0};      // (not of one length)
   const long long units = blocks_of(g), sms = sm_count(), last = units % sms;
   if (last == 0) return {0, 0};
   const long long parts = std::min<long long>(sms / last, std::max(1, tiles / 4));
@@ -1689,15 +1865,27 @@ Parts query_parts(const AttnShape& p, const Slots& g) { return parts_of(p, g, ti
 // on 2 188 / 117; with more CTAs 4000 in 3, 8 on 4 111 / 120; 9113 in 7, 16 on 4 479 / 501.
 Parts key_parts(const AttnShape& p, const Slots& g) {
   const int group = p.H / p.Hk, min_saved = p.D <= 64 ? MIN_SAVED : MIN_SAVED_WIDE;
-  if (!p.offsets && !p.causal) return parts_of(p, g, tiles_of(p) * group, min_saved);
+  if (!p.offsets && !p.causal && !p.window) return parts_of(p, g, tiles_of(p) * group, min_saved);
   const long long units = blocks_of(g), sms = sm_count();
   if (3 * units > 2 * sms) return {0, 0};
   int parts = static_cast<int>(std::min<long long>(group, 3 * sms / units));
   while (group % parts) --parts;
-  const int mean = p.offsets ? p.N / std::max(1, p.sequences) : p.N, tiles = (mean + TILE - 1) / TILE * group;
+  const int tiles = (p.window ? window_tiles(p) : (mean_length(p) + TILE - 1) / TILE) * group;
   if (parts < 2 || tiles - tiles / parts < min_saved) return {0, 0};
   return {0, parts};
 }
+// Tiles with sinks have all queries of a sequence where others have a window's: parts of about that length, in two waves at most
+SinkTiles sink_tiles(const AttnShape& p) {
+  if (!p.window || p.sinks <= 0) return {0, 1, 0};
+  const int tiles = (p.sinks + TILE - 1) / TILE, along = tiles_of(p), each = window_tiles(p);
+  const long long units = 1ll * (p.offsets ? p.sequences : p.B) * p.Hk * tiles;
+  if (units == 0) return {0, 1, 0};
+  const long long parts = std::min<long long>((along + each - 1) / each, 2ll * sm_count() / units);
+  if (parts < 2) return {0, 1, 0};
+  return {static_cast<int>(parts), tiles, static_cast<uint32_t>(units)};
+}
+long long sink_rows(const SinkTiles& s) { return 1ll * s.units * s.parts * TILE; }
+
 template <typename... Params>
 cudaError_t launch(void (*kernel)(Params...), std::atomic<uint64_t>& devices, int threads, int smem, const CUtensorMap& q, const CUtensorMap& k,
                    const CUtensorMap& v, const FwdParams& p, cudaStream_t s) {
@@ -1705,30 +1893,43 @@ cudaError_t launch(void (*kernel)(Params...), std::atomic<uint64_t>& devices, in
   if (e != cudaSuccess) return e;
   return launch_chained(kernel, dim3(static_cast<unsigned>(blocks_of(p.t.grid, p.split))), dim3(threads), smem, s, 1, true, q, k, v, p);
 }
+template <bool WIN>
 cudaError_t launch_fwd(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const FwdParams& p, bool one_tile, cudaStream_t s) {
   static std::atomic<uint64_t> devices[4];
   if (one_tile) {
-    if (p.t.D <= 64) return launch(attn_fwd_kernel<1, 1>, devices[0], Fwd<1, 1>::THREADS_, Fwd<1, 1>::SMEM, q, k, v, p, s);
-    return launch(attn_fwd_kernel<2, 1>, devices[1], Fwd<2, 1>::THREADS_, Fwd<2, 1>::SMEM, q, k, v, p, s);
+    if (p.t.D <= 64) return launch(attn_fwd_kernel<1, 1, WIN>, devices[0], Fwd<1, 1>::THREADS_, Fwd<1, 1>::SMEM, q, k, v, p, s);
+    return launch(attn_fwd_kernel<2, 1, WIN>, devices[1], Fwd<2, 1>::THREADS_, Fwd<2, 1>::SMEM, q, k, v, p, s);
   }
-  if (p.t.D <= 64) return launch(attn_fwd_narrow_kernel, devices[2], THREADS, FwdNarrow::SMEM, q, k, v, p, s);
-  return launch(attn_fwd_kernel<2, 2>, devices[3], Fwd<2, 2>::THREADS_, Fwd<2, 2>::SMEM, q, k, v, p, s);
+  if (p.t.D <= 64) return launch(attn_fwd_narrow_kernel<WIN>, devices[2], THREADS, FwdNarrow::SMEM, q, k, v, p, s);
+  return launch(attn_fwd_kernel<2, 2, WIN>, devices[3], Fwd<2, 2>::THREADS_, Fwd<2, 2>::SMEM, q, k, v, p, s);
 }
-template <int DB, bool SPLIT>
+template <int DB, bool SPLIT, bool WIN>
 cudaError_t launch_dq(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& g, const DqParams& p, cudaStream_t s) {
   static std::atomic<uint64_t> devices;
-  const cudaError_t e = allow_shared_memory(devices, reinterpret_cast<const void*>(&attn_dq_kernel<DB, SPLIT>), Dq<DB>::SMEM);
+  const cudaError_t e = allow_shared_memory(devices, reinterpret_cast<const void*>(&attn_dq_kernel<DB, SPLIT, WIN>), Dq<DB>::SMEM);
   if (e != cudaSuccess) return e;
-  return launch_chained(attn_dq_kernel<DB, SPLIT>, dim3(static_cast<unsigned>(blocks_of(p.t.grid, p.split))), dim3(BWD_THREADS), Dq<DB>::SMEM, s, 1, true, q, k, v,
-                        g, p);
+  return launch_chained(attn_dq_kernel<DB, SPLIT, WIN>, dim3(static_cast<unsigned>(blocks_of(p.t.grid, p.split))), dim3(BWD_THREADS), Dq<DB>::SMEM, s, 1, true,
+                        q, k, v, g, p);
 }
-template <int DB, bool SPLIT>
+template <int DB, bool SPLIT, bool WIN>
 cudaError_t launch_dkv(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& g, const DkvParams& p, cudaStream_t s) {
   static std::atomic<uint64_t> devices;
-  const cudaError_t e = allow_shared_memory(devices, reinterpret_cast<const void*>(&attn_dkv_kernel<DB, SPLIT>), Dkv<DB>::SMEM);
+  const cudaError_t e = allow_shared_memory(devices, reinterpret_cast<const void*>(&attn_dkv_kernel<DB, SPLIT, WIN>), Dkv<DB>::SMEM);
   if (e != cudaSuccess) return e;
-  return launch_chained(attn_dkv_kernel<DB, SPLIT>, dim3(static_cast<unsigned>(blocks_of(p.t.grid, p.split))), dim3(BWD_THREADS), Dkv<DB>::SMEM, s, 1, true, q, k, v,
-                        g, p);
+  const long long blocks = blocks_of(p.t.grid, p.split) + 1ll * p.sinks.units * p.sinks.parts;
+  return launch_chained(attn_dkv_kernel<DB, SPLIT, WIN>, dim3(static_cast<unsigned>(blocks)), dim3(BWD_THREADS), Dkv<DB>::SMEM, s, 1, true, q, k, v, g, p);
+}
+template <int DB>
+cudaError_t launch_dq(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& g, const DqParams& p, bool window, cudaStream_t s) {
+  if (window) return launch_dq<DB, false, true>(q, k, v, g, p, s);
+  return p.split.parts > 0 ? launch_dq<DB, true, false>(q, k, v, g, p, s) : launch_dq<DB, false, false>(q, k, v, g, p, s);
+}
+template <int DB>
+cudaError_t launch_dkv(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& g, const DkvParams& p, bool window,
+                       cudaStream_t s) {
+  const bool split = p.split.parts > 0 || p.sinks.parts > 0;
+  if (window) return split ? launch_dkv<DB, true, true>(q, k, v, g, p, s) : launch_dkv<DB, false, true>(q, k, v, g, p, s);
+  return split ? launch_dkv<DB, true, false>(q, k, v, g, p, s) : launch_dkv<DB, false, false>(q, k, v, g, p, s);
 }
 
 }  // namespace
@@ -1756,7 +1957,7 @@ cudaError_t attention_fwd(const AttnShape& p, const AttnTensor& q, const AttnTen
   f.o_rest = o_rest;
   f.lse = lse;
   *launches = 1;
-  const cudaError_t e = launch_fwd(mq, mk_, mv, f, one_tile, s);
+  const cudaError_t e = p.window ? launch_fwd<true>(mq, mk_, mv, f, one_tile, s) : launch_fwd<false>(mq, mk_, mv, f, one_tile, s);
   if (e != cudaSuccess || f.split.parts == 0) return e;
   ++*launches;
   return launch_chained(attn_join_kernel, dim3(static_cast<unsigned>(rows / f.split.parts / 8)), dim3(256), 0, s, 1, true, f);
@@ -1765,6 +1966,8 @@ cudaError_t attention_fwd(const AttnShape& p, const AttnTensor& q, const AttnTen
 long long attention_bwd_scratch(const AttnShape& p) {
   if (!shape_ok(p)) return 0;
   const Slots q = slots_of(p, p.H, TILE, 1), k = slots_of(p, p.Hk, TILE, 2);
+  const SinkTiles sinks = sink_tiles(p);
+  if (sinks.parts > 0) return 2 * sink_rows(sinks) * p.D;
   return std::max(part_rows(q, query_parts(p, q)), 2 * part_rows(k, key_parts(p, k))) * p.D;
 }
 
@@ -1795,14 +1998,15 @@ cudaError_t attention_bwd(const AttnShape& p, const AttnTensor& q, const AttnTen
   b.dv = dv;
   a.split = scratch ? query_parts(p, a.t.grid) : Parts{0, 0};
   a.sums = scratch;
-  b.split = scratch ? key_parts(p, b.t.grid) : Parts{0, 0};
+  b.sinks = scratch ? sink_tiles(p) : SinkTiles{0, 1, 0};
+  b.split = scratch && b.sinks.parts == 0 ? key_parts(p, b.t.grid) : Parts{0, 0};
   const long long rows_q = part_rows(a.t.grid, a.split), rows_k = part_rows(b.t.grid, b.split);
   // (the parts of dQ have been added up where those of dK and dV begin)
   b.dv_sums = scratch;
-  b.dk_sums = scratch + rows_k * p.D;
+  b.dk_sums = scratch + (b.sinks.parts > 0 ? sink_rows(b.sinks) : rows_k) * p.D;
   *launches = 1;
-  cudaError_t e = rows_q > 0 ? (p.D <= 64 ? launch_dq<1, true>(mq, mk_, mv, mg, a, s) : launch_dq<2, true>(mq, mk_, mv, mg, a, s))
-                             : (p.D <= 64 ? launch_dq<1, false>(mq, mk_, mv, mg, a, s) : launch_dq<2, false>(mq, mk_, mv, mg, a, s));
+  const bool window = p.window != 0;
+  cudaError_t e = p.D <= 64 ? launch_dq<1>(mq, mk_, mv, mg, a, window, s) : launch_dq<2>(mq, mk_, mv, mg, a, window, s);
   if (e == cudaSuccess && rows_q > 0) {
     ++*launches;
     const Sums sums{{a.sums, nullptr}, {dq, dq}, {p.scale, 0.f}};
@@ -1810,11 +2014,14 @@ cudaError_t attention_bwd(const AttnShape& p, const AttnTensor& q, const AttnTen
   }
   if (e != cudaSuccess) return e;
   ++*launches;
-  e = rows_k > 0 ? (p.D <= 64 ? launch_dkv<1, true>(mq, mk_, mv, mg, b, s) : launch_dkv<2, true>(mq, mk_, mv, mg, b, s))
-                 : (p.D <= 64 ? launch_dkv<1, false>(mq, mk_, mv, mg, b, s) : launch_dkv<2, false>(mq, mk_, mv, mg, b, s));
+  e = p.D <= 64 ? launch_dkv<1>(mq, mk_, mv, mg, b, window, s) : launch_dkv<2>(mq, mk_, mv, mg, b, window, s);
+  const Sums sums{{b.dv_sums, b.dk_sums}, {dv, dk}, {1.f, p.scale}};
+  if (e == cudaSuccess && b.sinks.parts > 0) {
+    ++*launches;
+    e = launch_chained(attn_sink_sum_kernel, dim3(static_cast<unsigned>(b.sinks.units * (TILE / 8)), 2), dim3(256), 0, s, 1, true, b.t, b.sinks, sums);
+  }
   if (e == cudaSuccess && rows_k > 0) {
     ++*launches;
-    const Sums sums{{b.dv_sums, b.dk_sums}, {dv, dk}, {1.f, p.scale}};
     e = launch_chained(attn_sum_kernel, dim3(static_cast<unsigned>(rows_k / b.split.parts / 8), 2), dim3(256), 0, s, 1, true, b.t.grid, b.split, sums, p.D);
   }
   return e;

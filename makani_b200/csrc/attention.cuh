@@ -22,6 +22,8 @@ struct AttnShape {
   // What the offsets do not cover is written as zeros behind the last sequence.
   const int* offsets;
   int sequences;
+  // window != 0: token i of a sequence sees those from i - left to i + right (causal: to i), and the first `sinks` of the sequence; 0 <= left, right, sinks <= N
+  int window, left, right, sinks;
 };
 
 // o [B, N, H, D] dense.  For a backward pass (both or none): lse [B, H, N], log2 of the sum of exponentials of every row, and o_rest, like o, what the

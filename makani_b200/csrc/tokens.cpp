@@ -1,4 +1,4 @@
-// Passes of the token operators (layer norm, attention): checks, allocations, launches and their nodes of the autograd graph, without a return to
+// Passes of the token operators (layer norm, attention, rotary positions, dropout): checks, allocations, launches and their nodes of the autograd graph, without a return to
 // Python in between.  (A forward and a backward pass of a layer norm of 16471 x 387 tokens, with the node in Python 122 us, all of it host time.)
 #include "host.h"
 
@@ -14,8 +14,12 @@
 #include <atomic>
 #include <cmath>
 
+#include <ATen/cuda/CUDAGeneratorImpl.h>
+
 #include "attention.cuh"
+#include "dropout.cuh"
 #include "layer_norm.cuh"
+#include "rotary.cuh"
 
 namespace {
 
@@ -359,7 +363,15 @@ Tensor readable(const Tensor& t) {
   return (reinterpret_cast<uintptr_t>(c.data_ptr()) & 15) == 0 ? c : c.clone();
 }
 
-mk::AttnShape shape_of(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& offsets, bool causal, double scale) {
+// Which tokens see which: `left` and `right` below zero are without end
+struct Mask {
+  bool causal = false;
+  int64_t left = -1, right = -1, sinks = 0;
+  std::vector<int64_t> kept() const { return {causal, left, right, sinks}; }
+  static Mask of(const std::vector<int64_t>& v) { return {v[0] != 0, v[1], v[2], v[3]}; }
+};
+
+mk::AttnShape shape_of(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& offsets, const Mask& mask, double scale) {
   auto bf16 = [](const Tensor& t) { return t.is_cuda() && t.scalar_type() == at::kBFloat16 && t.dim() == 4; };
   MK_CHECK(bf16(q) && bf16(k) && bf16(v), "attention: bf16 CUDA tensors [B, N, heads, D] expected");
   MK_CHECK(k.device() == q.device() && v.device() == q.device(), "attention: tensors must be on one CUDA device");
@@ -375,7 +387,14 @@ mk::AttnShape shape_of(const Tensor& q, const Tensor& k, const Tensor& v, const 
   p.H = static_cast<int>(q.size(2));
   p.Hk = static_cast<int>(k.size(2));
   p.D = static_cast<int>(q.size(3));
-  p.causal = causal;
+  p.causal = mask.causal;
+  // (a window over everything is none)
+  const int64_t most = p.N, left = mask.left < 0 ? most : std::min(mask.left, most), right = mask.causal ? 0 : mask.right < 0 ? most : std::min(mask.right, most);
+  MK_CHECK(mask.sinks >= 0, "attention: no negative number of sinks");
+  p.window = left < most - 1 || (!mask.causal && right < most - 1);
+  p.left = static_cast<int>(left);
+  p.right = static_cast<int>(right);
+  p.sinks = static_cast<int>(std::min(mask.sinks, most));
   p.scale = static_cast<float>(scale);
   if (offsets.has_value() && offsets->defined()) {
     MK_CHECK(offsets->device() == q.device() && offsets->scalar_type() == at::kInt && offsets->dim() == 1 && offsets->is_contiguous() && offsets->size(0) >= 1,
@@ -388,9 +407,9 @@ mk::AttnShape shape_of(const Tensor& q, const Tensor& k, const Tensor& v, const 
 }
 
 // (o, what its rounding left out, L): the last two with `train`
-std::tuple<Tensor, Tensor, Tensor> attention_forward(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, const OptTensor& offsets, bool causal,
-                                                double scale, bool train) {
-  const mk::AttnShape p = shape_of(q_in, k_in, v_in, offsets, causal, scale);
+std::tuple<Tensor, Tensor, Tensor> attention_forward(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, const OptTensor& offsets, const Mask& mask,
+                                                     double scale, bool train) {
+  const mk::AttnShape p = shape_of(q_in, k_in, v_in, offsets, mask, scale);
   c10::cuda::CUDAGuard guard(q_in.device());
   Tensor o = at::empty(q_in.sizes(), q_in.options()), rest, lse;
   if (train) {
@@ -411,8 +430,8 @@ std::tuple<Tensor, Tensor, Tensor> attention_forward(const Tensor& q_in, const T
 
 // gradients into tensors [B, N, heads, D] (strides as `readable` has them)
 void attention_backward(const Tensor& d_out, const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, const Tensor& o, const Tensor& rest,
-                        const Tensor& lse, const OptTensor& offsets, bool causal, double scale, const Tensor& dq, const Tensor& dk, const Tensor& dv) {
-  const mk::AttnShape p = shape_of(q_in, k_in, v_in, offsets, causal, scale);
+                        const Tensor& lse, const OptTensor& offsets, const Mask& mask, double scale, const Tensor& dq, const Tensor& dk, const Tensor& dv) {
+  const mk::AttnShape p = shape_of(q_in, k_in, v_in, offsets, mask, scale);
   c10::cuda::CUDAGuard guard(q_in.device());
   MK_CHECK(plain({&d_out}), "attention: the backward pass takes no batches of gradients, and is not traced");
   MK_CHECK(d_out.device() == o.device() && d_out.sizes() == o.sizes() && d_out.scalar_type() == at::kBFloat16,
@@ -430,13 +449,14 @@ void attention_backward(const Tensor& d_out, const Tensor& q_in, const Tensor& k
   mkh::launches() += launches;
 }
 
+// (masks go by value through `saved_data`, as lists of whole numbers)
 struct Attention : torch::autograd::Function<Attention> {
-  static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& offsets, bool causal, double scale,
-                        bool train) {
-    auto [o, rest, lse] = attention_forward(q, k, v, offsets, causal, scale, train);
+  static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& offsets, const std::vector<int64_t>& mask,
+                        double scale, bool train) {
+    auto [o, rest, lse] = attention_forward(q, k, v, offsets, Mask::of(mask), scale, train);
     if (train) {
       ctx->save_for_backward({q, k, v, o, rest, lse, value(offsets)});
-      ctx->saved_data["causal"] = causal;
+      ctx->saved_data["mask"] = mask;
       ctx->saved_data["scale"] = scale;
     }
     return o;
@@ -445,17 +465,18 @@ struct Attention : torch::autograd::Function<Attention> {
     const Backward count;
     const variable_list s = ctx->get_saved_variables();
     const Tensor dq = at::empty(s[0].sizes(), s[0].options()), dk = at::empty(s[1].sizes(), s[1].options()), dv = at::empty(s[2].sizes(), s[2].options());
-    attention_backward(grads[0], s[0], s[1], s[2], s[3], s[4], s[5], maybe(s[6]), ctx->saved_data["causal"].toBool(), ctx->saved_data["scale"].toDouble(), dq, dk,
-                       dv);
+    attention_backward(grads[0], s[0], s[1], s[2], s[3], s[4], s[5], maybe(s[6]), Mask::of(ctx->saved_data["mask"].toIntVector()),
+                       ctx->saved_data["scale"].toDouble(), dq, dk, dv);
     return once_differentiable({dq, dk, dv, Tensor(), Tensor(), Tensor(), Tensor()});
   }
 };
 
 // (o; nothing where the tensors are not for kernels)
-OptTensor attention(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& offsets, bool causal, double scale) {
+OptTensor attention(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& offsets, bool causal, double scale, int64_t left, int64_t right,
+                    int64_t sinks) {
   const Tensor at = value(offsets);
   if (!plain({&q, &k, &v, &at})) return {};
-  return Attention::apply(q, k, v, offsets, causal, scale, records({&q, &k, &v}));
+  return Attention::apply(q, k, v, offsets, Mask{causal, left, right, sinks}.kept(), scale, records({&q, &k, &v}));
 }
 
 // The output of a fused projection: [B, N, (q heads | k heads | v heads) x D], dense; its gradient is written as one tensor
@@ -472,15 +493,15 @@ struct Parts {
 };
 
 struct AttentionQkv : torch::autograd::Function<AttentionQkv> {
-  static Tensor forward(AutogradContext* ctx, const Tensor& qkv, int64_t heads, int64_t kv_heads, const OptTensor& offsets, bool causal, double scale,
-                        bool train) {
+  static Tensor forward(AutogradContext* ctx, const Tensor& qkv, int64_t heads, int64_t kv_heads, const OptTensor& offsets, const std::vector<int64_t>& mask,
+                        double scale, bool train) {
     const Parts p(qkv, heads, kv_heads);
-    auto [o, rest, lse] = attention_forward(p.q, p.k, p.v, offsets, causal, scale, train);
+    auto [o, rest, lse] = attention_forward(p.q, p.k, p.v, offsets, Mask::of(mask), scale, train);
     if (train) {
       ctx->save_for_backward({qkv, o, rest, lse, value(offsets)});
       ctx->saved_data["heads"] = heads;
       ctx->saved_data["kv_heads"] = kv_heads;
-      ctx->saved_data["causal"] = causal;
+      ctx->saved_data["mask"] = mask;
       ctx->saved_data["scale"] = scale;
     }
     return o;
@@ -491,16 +512,434 @@ struct AttentionQkv : torch::autograd::Function<AttentionQkv> {
     const int64_t heads = ctx->saved_data["heads"].toInt(), kv_heads = ctx->saved_data["kv_heads"].toInt();
     const Tensor dqkv = at::empty(s[0].sizes(), s[0].options());
     const Parts p(s[0], heads, kv_heads), d(dqkv, heads, kv_heads);
-    attention_backward(grads[0], p.q, p.k, p.v, s[1], s[2], s[3], maybe(s[4]), ctx->saved_data["causal"].toBool(), ctx->saved_data["scale"].toDouble(), d.q, d.k,
-                       d.v);
+    attention_backward(grads[0], p.q, p.k, p.v, s[1], s[2], s[3], maybe(s[4]), Mask::of(ctx->saved_data["mask"].toIntVector()),
+                       ctx->saved_data["scale"].toDouble(), d.q, d.k, d.v);
     return once_differentiable({dqkv, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()});
   }
 };
 
-OptTensor attention_qkv(const Tensor& qkv, int64_t heads, int64_t kv_heads, const OptTensor& offsets, bool causal, double scale) {
+OptTensor attention_qkv(const Tensor& qkv, int64_t heads, int64_t kv_heads, const OptTensor& offsets, bool causal, double scale, int64_t left, int64_t right,
+                        int64_t sinks) {
   const Tensor at = value(offsets);
   if (!plain({&qkv, &at})) return {};
-  return AttentionQkv::apply(qkv, heads, kv_heads, offsets, causal, scale, records({&qkv}));
+  return AttentionQkv::apply(qkv, heads, kv_heads, offsets, Mask{causal, left, right, sinks}.kept(), scale, records({&qkv}));
+}
+
+// ------------------------------------------------------------------------------------------ rotary positions
+
+// How channels turn: bands of channels, one per axis, and the turns per unit of position of every pair
+struct RotaryPlan {
+  std::vector<int64_t> bands;
+  std::vector<double> turns;
+  bool interleaved = false;
+  // as autograd keeps it
+  std::vector<int64_t> kept_bands() const {
+    std::vector<int64_t> v = bands;
+    v.push_back(interleaved);
+    return v;
+  }
+  static RotaryPlan of(std::vector<int64_t> kept, std::vector<double> turns) {
+    const bool interleaved = kept.back() != 0;
+    kept.pop_back();
+    return {std::move(kept), std::move(turns), interleaved};
+  }
+};
+
+mk::RotTensor rot_view(const Tensor& t) {
+  auto stride = [&](int d) { return t.size(d) == 1 ? t.size(3) : t.stride(d); };
+  return {t.data_ptr(), stride(1), stride(2), stride(0)};
+}
+
+// Tensors of a pass: queries and, perhaps, keys, with weights and biases of their norms; positions
+struct RotInputs {
+  Tensor x[2], w[2], b[2], positions;
+};
+
+mk::RotShape rot_shape(const Tensor& like, const RotInputs& in, const RotaryPlan& plan, int64_t norm, double eps, bool inverse) {
+  MK_CHECK(like.is_cuda() && native_type(like) && like.dim() == 4, "rotary positions: bf16 or fp32 CUDA tensors [B, N, heads, D] expected");
+  MK_CHECK(like.size(3) % 8 == 0 && like.size(3) >= 8 && like.size(3) <= mk::ROT_WIDTH, "rotary positions: 8, 16, .., ", mk::ROT_WIDTH,
+           " channels of a head expected");
+  MK_CHECK(like.size(0) < (1ll << 31) && like.size(1) < (1ll << 31), "rotary positions: too many tokens");
+  MK_CHECK(norm >= 0 && norm <= 2, "rotary positions: an unknown norm");
+  mk::RotShape p{};
+  p.B = static_cast<int>(like.size(0));
+  p.N = static_cast<int>(like.size(1));
+  p.D = static_cast<int>(like.size(3));
+  p.f32 = is_f32(like);
+  p.norm = static_cast<uint8_t>(norm);
+  p.interleaved = plan.interleaved;
+  p.inverse = inverse;
+  p.eps = static_cast<float>(eps);
+  if (in.positions.defined()) {
+    const Tensor& at = in.positions;
+    p.axes = static_cast<int>(plan.bands.size());
+    MK_CHECK(p.axes >= 1 && p.axes <= mk::ROT_AXES && at.device() == like.device() && at.is_contiguous() && (at.dim() == 2 || at.dim() == 3) &&
+                 at.size(-1) == p.axes && at.size(-2) == p.N && (at.dim() == 2 || at.size(0) == p.B),
+             "rotary positions: positions [N, axes] or [B, N, axes] expected");
+    int64_t channels = 0;
+    for (int a = 0; a < p.axes; ++a) {
+      MK_CHECK(plan.bands[a] >= 2 && plan.bands[a] % 2 == 0 && plan.bands[a] <= p.D, "rotary positions: bands of even widths expected");
+      p.band[a] = static_cast<int>(plan.bands[a]);
+      channels += plan.bands[a];
+    }
+    MK_CHECK(channels <= p.D && static_cast<int64_t>(plan.turns.size()) == channels / 2, "rotary positions: ", channels, " channels of ", p.D, " turned");
+    std::copy(plan.turns.begin(), plan.turns.end(), p.turns);
+    switch (at.scalar_type()) {
+      case at::kInt: p.position_type = mk::ROT_POS_I32; break;
+      case at::kLong: p.position_type = mk::ROT_POS_I64; break;
+      case at::kFloat: p.position_type = mk::ROT_POS_F32; break;
+      case at::kDouble: p.position_type = mk::ROT_POS_F64; break;
+      default: MK_CHECK(false, "rotary positions: positions in int32, int64, fp32 or fp64 expected");
+    }
+    p.positions = at.data_ptr();
+    p.position_batch = at.dim() == 3 ? at.size(1) * at.size(2) : 0;
+  }
+  return p;
+}
+
+void rot_weights(mk::RotPart& part, const Tensor& w, const Tensor& b, const Tensor& like) {
+  for (const Tensor* t : {&w, &b})
+    MK_CHECK(!t->defined() || (t->is_cuda() && t->device() == like.device() && is_f32(*t) && t->is_contiguous() && t->dim() == 1 && t->size(0) == like.size(3)),
+             "rotary positions: weights and biases [D] of the norm expected");
+  part.w = ptr_or_null<float>(w);
+  part.b = ptr_or_null<float>(b);
+}
+Tensor rot_param(const Tensor& t) {
+  if (!t.defined()) return t;
+  return (is_f32(t) && t.is_contiguous()) ? t : t.detach().to(at::kFloat).contiguous();
+}
+
+// Results into `out`, tensors [B, N, heads, D]
+void rotary_into(const RotInputs& in, const Tensor (&out)[2], const RotaryPlan& plan, int64_t norm, double eps, bool inverse) {
+  c10::cuda::CUDAGuard guard(in.x[0].device());
+  mk::RotShape p = rot_shape(in.x[0], in, plan, norm, eps, inverse);
+  Tensor x[2];
+  for (int i = 0; i < 2; ++i) {
+    if (!in.x[i].defined() || in.x[i].numel() == 0) continue;
+    MK_CHECK(in.x[i].dim() == 4 && in.x[i].device() == in.x[0].device() && in.x[i].scalar_type() == in.x[0].scalar_type() && in.x[i].size(0) == p.B &&
+                 in.x[i].size(1) == p.N && in.x[i].size(3) == p.D,
+             "rotary positions: queries and keys of the same tokens and channels expected");
+    x[i] = readable(in.x[i]);
+    mk::RotPart& part = p.part[p.parts++];
+    part.x = rot_view(x[i]);
+    part.out = rot_view(out[i]);
+    part.heads = static_cast<int>(x[i].size(2));
+    rot_weights(part, in.w[i], in.b[i], x[i]);
+  }
+  if (p.parts == 0) return;
+  ++mkh::launches();
+  mkh::check(mk::rotary_fwd(p, mkh::stream()), "rotary_fwd");
+}
+// Gradients of x into `out` (which may be `dy`), and of weights and biases; parts whose gradient is not defined are left out
+void rotary_back(const RotInputs& in, const Tensor (&dy)[2], const Tensor (&out)[2], const RotaryPlan& plan, int64_t norm, double eps, bool inverse,
+                 const bool (&sums)[2], Tensor (&dw)[2], Tensor (&db)[2], const int* limit = nullptr) {
+  const Tensor& like = dy[0].defined() ? dy[0] : dy[1];
+  c10::cuda::CUDAGuard guard(like.device());
+  mk::RotShape p = rot_shape(like, in, plan, norm, eps, inverse);
+  p.limit = limit;
+  Tensor x[2], d[2], scratch;
+  for (int i = 0; i < 2; ++i) {
+    if (!dy[i].defined()) continue;
+    const auto params = dy[i].options().dtype(at::kFloat);
+    if (dy[i].numel() == 0) {
+      if (sums[i]) dw[i] = at::zeros({p.D}, params), db[i] = at::zeros({p.D}, params);
+      continue;
+    }
+    mk::RotPart& part = p.part[p.parts++];
+    d[i] = out[i].is_same(dy[i]) ? dy[i] : readable(dy[i]);
+    part.dy = rot_view(d[i]);
+    part.out = rot_view(out[i]);
+    part.heads = static_cast<int>(d[i].size(2));
+    if (norm) {
+      x[i] = readable(in.x[i]);
+      part.x = rot_view(x[i]);
+    }
+    rot_weights(part, in.w[i], in.b[i], d[i]);
+    if (sums[i]) {
+      dw[i] = at::empty({p.D}, params);
+      db[i] = at::empty({p.D}, params);
+      part.dw = dw[i].data_ptr<float>();
+      part.db = db[i].data_ptr<float>();
+    }
+  }
+  if (p.parts == 0) return;
+  if (sums[0] || sums[1]) scratch = at::empty({mk::rotary_scratch(p)}, like.options().dtype(at::kFloat));
+  int launches = 0;
+  mkh::check(mk::rotary_bwd(p, ptr_or_null<float>(scratch), &launches, mkh::stream()), "rotary_bwd");
+  mkh::launches() += launches;
+}
+
+// Whether the gradient of argument i is asked for; `args`: the arguments of a node up to i, of which those that are no tensors have no edge
+bool asked_for(AutogradContext* ctx, const variable_list& args, size_t i) {
+  if (!args[i].defined()) return false;
+  size_t edge = 0;
+  for (size_t k = 0; k < i; ++k) edge += args[k].defined();
+  return ctx->needs_input_grad(edge);
+}
+// Gradients of parameters in their own types, where they are asked for
+Tensor param_grad(const Tensor& g, const Tensor& param, bool needed) {
+  if (!needed || !param.defined() || !g.defined()) return Tensor();
+  return g.scalar_type() == param.scalar_type() ? g : g.to(param.scalar_type());
+}
+
+struct Rotary : torch::autograd::Function<Rotary> {
+  // edges: q, k, their weights and biases, positions
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const OptTensor& k, const OptTensor& qw, const OptTensor& kw, const OptTensor& qb,
+                               const OptTensor& kb, const OptTensor& positions, const std::vector<int64_t>& bands, const std::vector<double>& turns,
+                               int64_t norm, double eps, bool inverse, bool train) {
+    RotInputs in;
+    in.x[0] = q;
+    in.x[1] = value(k);
+    in.w[0] = rot_param(value(qw)), in.w[1] = rot_param(value(kw)), in.b[0] = rot_param(value(qb)), in.b[1] = rot_param(value(kb));
+    in.positions = value(positions);
+    Tensor out[2];
+    for (int i = 0; i < 2; ++i)
+      if (in.x[i].defined()) out[i] = at::empty(in.x[i].sizes(), in.x[i].options());
+    rotary_into(in, out, RotaryPlan::of(bands, turns), norm, eps, inverse);
+    if (train) {
+      if (norm) ctx->save_for_backward({q, value(k), value(qw), value(kw), value(qb), value(kb), in.positions});
+      else ctx->save_for_backward({in.positions});
+      ctx->saved_data["bands"] = bands;
+      ctx->saved_data["turns"] = turns;
+      ctx->saved_data["norm"] = norm;
+      ctx->saved_data["eps"] = eps;
+      ctx->saved_data["inverse"] = inverse;
+    }
+    if (out[1].defined()) return {out[0], out[1]};
+    return {out[0]};
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    const Backward count;
+    const variable_list s = ctx->get_saved_variables();
+    const auto bands = ctx->saved_data["bands"].toIntVector();
+    const auto turns = ctx->saved_data["turns"].toDoubleVector();
+    const int64_t norm = ctx->saved_data["norm"].toInt();
+    const double eps = ctx->saved_data["eps"].toDouble();
+    const bool inverse = ctx->saved_data["inverse"].toBool();
+    Tensor dy[2] = {grads[0], grads.size() > 1 ? grads[1] : Tensor()};
+    variable_list out(13);
+    if (!dy[0].defined() && !dy[1].defined()) return out;
+    MK_CHECK(plain({&dy[0], &dy[1]}), "rotary positions: the backward pass takes no batches of gradients, and is not traced");
+    if (norm == 0 && at::GradMode::is_enabled()) {      // (the same again, the other way round: it can be differentiated as often as one likes)
+      const bool first = dy[0].defined(), both = first && dy[1].defined();
+      auto g = apply(first ? dy[0] : dy[1], both ? OptTensor(dy[1]) : OptTensor(), OptTensor(), OptTensor(), OptTensor(), OptTensor(), maybe(s[0]),
+                     bands, turns, norm, eps, !inverse,
+                     records({&dy[0], &dy[1]}));
+      out[first ? 0 : 1] = g[0];
+      if (both) out[1] = g[1];
+      return out;
+    }
+    const at::AutoDispatchBelowAutograd below;
+    RotInputs in;
+    in.positions = norm ? s[6] : s[0];
+    Tensor dx[2], dw[2], db[2];
+    bool sums[2] = {false, false};
+    for (int i = 0; i < 2; ++i) {
+      if (!dy[i].defined()) continue;
+      if (norm) {
+        in.x[i] = s[i];
+        in.w[i] = rot_param(s[2 + i]);
+        sums[i] = asked_for(ctx, s, 2 + i) || asked_for(ctx, s, 4 + i);
+      }
+      dx[i] = at::empty(dy[i].sizes(), dy[i].options());
+    }
+    rotary_back(in, dy, dx, RotaryPlan::of(bands, turns), norm, eps, inverse, sums, dw, db);
+    for (int i = 0; i < 2; ++i) {
+      out[i] = dx[i];
+      if (norm) {
+        out[2 + i] = param_grad(dw[i], s[2 + i], asked_for(ctx, s, 2 + i));
+        out[4 + i] = param_grad(db[i], s[4 + i], asked_for(ctx, s, 4 + i));
+      }
+    }
+    return once_differentiable(out);
+  }
+};
+
+// (results; nothing where the tensors are not for kernels)
+variable_list rotary(const Tensor& q, const OptTensor& k, const OptTensor& qw, const OptTensor& kw, const OptTensor& qb, const OptTensor& kb,
+                     const OptTensor& positions, const RotaryPlan& plan, int64_t norm, double eps, bool inverse) {
+  const Tensor t[6] = {value(k), value(qw), value(kw), value(qb), value(kb), value(positions)};
+  if (!plain({&q, &t[0], &t[1], &t[2], &t[3], &t[4], &t[5]})) return {};
+  return Rotary::apply(q, k, qw, kw, qb, kb, positions, plan.kept_bands(), plan.turns, norm, eps, inverse,
+                       records({&q, &t[0], &t[1], &t[2], &t[3], &t[4]}));
+}
+
+// A fused projection's queries and keys normed and turned, then attention: one tensor for both, the gradient of the projection written as one
+struct RotaryAttentionQkv : torch::autograd::Function<RotaryAttentionQkv> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& qkv, const OptTensor& qw, const OptTensor& kw, const OptTensor& qb, const OptTensor& kb,
+                        const OptTensor& positions, const OptTensor& offsets, const std::vector<int64_t>& bands, const std::vector<double>& turns,
+                        int64_t norm, double eps, int64_t heads, int64_t kv_heads, const std::vector<int64_t>& mask, double scale, bool train) {
+    const Parts p(qkv, heads, kv_heads);
+    RotInputs in;
+    in.x[0] = p.q;
+    in.x[1] = p.k;
+    in.w[0] = rot_param(value(qw)), in.w[1] = rot_param(value(kw)), in.b[0] = rot_param(value(qb)), in.b[1] = rot_param(value(kb));
+    in.positions = value(positions);
+    const Tensor qk = at::empty({qkv.size(0), qkv.size(1), heads + kv_heads, p.q.size(3)}, qkv.options());
+    const Tensor out[2] = {qk.narrow(2, 0, heads), qk.narrow(2, heads, kv_heads)};
+    rotary_into(in, out, RotaryPlan::of(bands, turns), norm, eps, false);
+    auto [o, rest, lse] = attention_forward(out[0], out[1], p.v, offsets, Mask::of(mask), scale, train);
+    if (train) {
+      ctx->save_for_backward({qkv, value(qw), value(kw), value(qb), value(kb), in.positions, value(offsets), qk, o, rest, lse});
+      ctx->saved_data["bands"] = bands;
+      ctx->saved_data["turns"] = turns;
+      ctx->saved_data["norm"] = norm;
+      ctx->saved_data["eps"] = eps;
+      ctx->saved_data["heads"] = heads;
+      ctx->saved_data["kv_heads"] = kv_heads;
+      ctx->saved_data["mask"] = mask;
+      ctx->saved_data["scale"] = scale;
+    }
+    return o;
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    const Backward count;
+    const variable_list s = ctx->get_saved_variables();
+    const int64_t heads = ctx->saved_data["heads"].toInt(), kv_heads = ctx->saved_data["kv_heads"].toInt(), norm = ctx->saved_data["norm"].toInt();
+    const Parts p(s[0], heads, kv_heads);
+    const Tensor dqkv = at::empty(s[0].sizes(), s[0].options());
+    const Parts d(dqkv, heads, kv_heads);
+    attention_backward(grads[0], s[7].narrow(2, 0, heads), s[7].narrow(2, heads, kv_heads), p.v, s[8], s[9], s[10], maybe(s[6]),
+                       Mask::of(ctx->saved_data["mask"].toIntVector()), ctx->saved_data["scale"].toDouble(), d.q, d.k, d.v);
+    const at::AutoDispatchBelowAutograd below;
+    RotInputs in;
+    in.positions = s[5];
+    const Tensor dx[2] = {d.q, d.k};
+    Tensor dw[2], db[2];
+    bool sums[2] = {false, false};
+    for (int i = 0; i < 2; ++i) {
+      in.x[i] = i ? p.k : p.q;
+      if (norm) {
+        in.w[i] = rot_param(s[1 + i]);
+        sums[i] = asked_for(ctx, s, 1 + i) || asked_for(ctx, s, 3 + i);
+      }
+    }
+    // (in place: a lane writes what it alone has read; tokens of no sequence have the zeros that attention left)
+    const Tensor offsets = s[6];
+    const int* limit = offsets.defined() ? offsets.data_ptr<int>() + offsets.size(0) - 1 : nullptr;
+    rotary_back(in, dx, dx, RotaryPlan::of(ctx->saved_data["bands"].toIntVector(), ctx->saved_data["turns"].toDoubleVector()), norm,
+                ctx->saved_data["eps"].toDouble(), false, sums, dw, db, limit);
+    variable_list out(16);
+    out[0] = dqkv;
+    for (int i = 0; i < 2; ++i) {
+      out[1 + i] = param_grad(dw[i], s[1 + i], asked_for(ctx, s, 1 + i));
+      out[3 + i] = param_grad(db[i], s[3 + i], asked_for(ctx, s, 3 + i));
+    }
+    return once_differentiable(out);
+  }
+};
+
+OptTensor rotary_attention_qkv(const Tensor& qkv, int64_t heads, int64_t kv_heads, const OptTensor& qw, const OptTensor& kw, const OptTensor& qb,
+                               const OptTensor& kb, const OptTensor& positions, const OptTensor& offsets, const RotaryPlan& plan, int64_t norm, double eps,
+                               bool causal, double scale, int64_t left, int64_t right, int64_t sinks) {
+  const Tensor t[6] = {value(qw), value(kw), value(qb), value(kb), value(positions), value(offsets)};
+  if (!plain({&qkv, &t[0], &t[1], &t[2], &t[3], &t[4], &t[5]})) return {};
+  return RotaryAttentionQkv::apply(qkv, qw, kw, qb, kb, positions, offsets, plan.kept_bands(), plan.turns, norm, eps, heads, kv_heads,
+                                   Mask{causal, left, right, sinks}.kept(), scale, records({&qkv, &t[0], &t[1], &t[2], &t[3]}));
+}
+
+// ------------------------------------------------------------------------------------------ dropout
+
+// x (and a residual) dense; the mask from `seed` [2] (key, number of the call), or, where there is none, from torch's generator of the device, whose key and
+// position are then written to `kept`
+std::tuple<Tensor, Tensor> dropout_pass(const Tensor& x_in, const Tensor& residual, const Tensor& seed, const Tensor& kept, double p, at::ScalarType out_type,
+                                        bool copy) {
+  c10::cuda::CUDAGuard guard(x_in.device());
+  const Tensor x = x_in.contiguous(), r = residual.defined() ? residual.contiguous() : Tensor();
+  const Tensor out = at::empty(x.sizes(), x.options().dtype(out_type)), half = copy ? at::empty(x.sizes(), x.options().dtype(at::kBFloat16)) : Tensor();
+  mk::DropParams d{};
+  d.x = x.data_ptr();
+  d.r = ptr_or_null<void>(r);
+  d.out = out.data_ptr();
+  d.copy = ptr_or_null<void>(half);
+  d.n = x.numel();
+  const double words = std::nearbyint(p * 4294967296.0);
+  MK_CHECK(p >= 0.0 && p <= 1.0 && words >= 1.0, "dropout: a probability of 2^-32 to 1 expected");
+  d.last = static_cast<uint32_t>(words - 1.0);
+  d.factor = p < 1.0 ? static_cast<float>(1.0 / (1.0 - p)) : 0.f;
+  if (seed.defined()) {
+    MK_CHECK(seed.device() == x.device() && seed.scalar_type() == at::kLong && seed.is_contiguous() && seed.numel() == 2,
+             "dropout: a seed of two int64 (key, number of the call) on the device of x expected");
+    d.source.key_at = seed.data_ptr<int64_t>();
+    d.source.offset_at = d.source.key_at + 1;
+  } else {
+    // (a call takes four of the positions of every subsequence, as a call of torch's own generator with one block of words does, so that none is used twice)
+    auto* generator = at::get_generator_or_default<at::CUDAGeneratorImpl>(std::nullopt, at::cuda::detail::getDefaultCUDAGenerator());
+    at::PhiloxCudaState state;
+    {
+      const std::lock_guard<std::mutex> lock(generator->mutex_);
+      state = generator->philox_cuda_state(4);
+    }
+    d.source.shift = 2;
+    if (state.captured_) {
+      d.source.key_at = state.seed_.ptr;
+      d.source.offset_at = state.offset_.ptr;
+      d.source.more = state.offset_intragraph_;
+    } else {
+      d.source.key = state.seed_.val;
+      d.source.more = state.offset_.val;
+    }
+    d.source.kept = ptr_or_null<int64_t>(kept);
+  }
+  d.x_f32 = is_f32(x);
+  d.r_f32 = r.defined() && is_f32(r);
+  d.out_f32 = out_type == at::kFloat;
+  mkh::launches() += d.n > 0;
+  mkh::check(mk::dropout(d, mkh::stream()), "dropout");
+  return {out, half};
+}
+
+struct Dropout : torch::autograd::Function<Dropout> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const OptTensor& residual, const OptTensor& seed, double p, bool out_f32, bool train) {
+    const Tensor r = value(residual);
+    Tensor s = value(seed), kept;
+    if (!s.defined() && train) kept = at::empty({2}, x.options().dtype(at::kLong));
+    const Tensor out = std::get<0>(dropout_pass(x, r, s, kept, p, out_f32 ? at::kFloat : at::kBFloat16, false));
+    if (train) {
+      ctx->save_for_backward({s.defined() ? s : kept});
+      ctx->saved_data["p"] = p;
+      ctx->saved_data["x_f32"] = is_f32(x);
+      ctx->saved_data["added"] = r.defined();
+      ctx->saved_data["r_f32"] = r.defined() && is_f32(r);
+    }
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    const Backward count;
+    const Tensor seed = ctx->get_saved_variables()[0], dy = grads[0];
+    const bool x_f32 = ctx->saved_data["x_f32"].toBool(), added = ctx->saved_data["added"].toBool(), r_f32 = ctx->saved_data["r_f32"].toBool();
+    const double p = ctx->saved_data["p"].toDouble();
+    variable_list out(6);
+    if (!dy.defined()) return out;
+    MK_CHECK(plain({&dy}), "dropout: the backward pass takes no batches of gradients, and is not traced");
+    const bool need_r = added && ctx->needs_input_grad(1), half = need_r && !r_f32 && is_f32(dy);
+    if (at::GradMode::is_enabled()) {      // (the same mask on the gradient, which can be differentiated again)
+      if (ctx->needs_input_grad(0)) {
+        out[0] = apply(dy, OptTensor(), OptTensor(seed), p, is_f32(dy), records({&dy}));
+        if (is_f32(dy) && !x_f32) out[0] = out[0].to(at::kBFloat16);
+      }
+      if (need_r) out[1] = half ? dy.to(at::kBFloat16) : dy;
+      return out;
+    }
+    const at::AutoDispatchBelowAutograd below;
+    if (ctx->needs_input_grad(0)) {
+      auto [dx, copy] = dropout_pass(dy, Tensor(), seed, Tensor(), p, x_f32 ? at::kFloat : at::kBFloat16, half);
+      out[0] = dx;
+      if (half) out[1] = copy;
+    } else if (half) {
+      out[1] = dy.to(at::kBFloat16);
+    }
+    if (need_r && !half) out[1] = dy;
+    return out;
+  }
+};
+
+OptTensor dropout(const Tensor& x, const OptTensor& residual, const OptTensor& seed, double p, bool out_f32) {
+  const Tensor r = value(residual), s = value(seed);
+  if (!plain({&x, &r, &s})) return {};
+  MK_CHECK(x.is_cuda() && native_type(x) && (!r.defined() || (native_type(r) && r.device() == x.device() && r.sizes() == x.sizes())),
+           "dropout: bf16 or fp32 CUDA tensors of one shape expected");
+  return Dropout::apply(x, residual, seed, p, out_f32, records({&x, &r}));
 }
 
 }  // namespace
@@ -511,8 +950,18 @@ void bind_tokens(pybind11::module_& m) {
   using Free = pybind11::call_guard<pybind11::gil_scoped_release>;
   m.def("background_launches", []() { return background.load(); }, "kernel launches of backward passes that autograd ran");
   m.def("layer_norm", &layer_norm, Free());
-  m.def("attention", &attention, Free());
-  m.def("attention_qkv", &attention_qkv, Free());
+  using pybind11::arg;
+  m.def("attention", &attention, arg("q"), arg("k"), arg("v"), arg("offsets"), arg("causal"), arg("scale"), arg("left") = -1, arg("right") = -1,
+        arg("sinks") = 0, Free());
+  m.def("attention_qkv", &attention_qkv, arg("qkv"), arg("heads"), arg("kv_heads"), arg("offsets"), arg("causal"), arg("scale"), arg("left") = -1,
+        arg("right") = -1, arg("sinks") = 0, Free());
+  pybind11::class_<RotaryPlan>(m, "RotaryPlan")
+      .def(pybind11::init([](std::vector<int64_t> bands, std::vector<double> turns, bool interleaved) {
+        return RotaryPlan{std::move(bands), std::move(turns), interleaved};
+      }));
+  m.def("rotary", &rotary, Free());
+  m.def("rotary_attention_qkv", &rotary_attention_qkv, Free());
+  m.def("dropout", &dropout, Free());
 }
 
 }  // namespace mkh

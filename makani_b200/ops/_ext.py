@@ -60,12 +60,12 @@ def available() -> bool:
 # number of kernel-launching calls into this extension by the current process (the column sums launch a second kernel)
 LAUNCHES = 0
 _NON_KERNEL = {"read_error_flag", "clear_error_flag", "lp_scratch_floats", "adam_entry_bytes", "peer_alloc", "peer_open",
-               "peer_close", "peer_free", "tensor_from_ptr", "set_gelu_tanh", "stream_state", "launches", "background_launches"}
+               "peer_close", "peer_free", "tensor_from_ptr", "set_gelu_tanh", "stream_state", "launches", "background_launches", "RotaryPlan"}
 
 
 # passes over whole layers, which count their launches themselves
 _LAYERS = {"conv_forward", "conv_backward", "mlp_forward", "mlp_backward", "norm_forward", "norm_backward", "spectral_forward",
-           "spectral_backward", "afno_forward", "afno_backward", "layer_norm", "attention", "attention_qkv"}
+           "spectral_backward", "afno_forward", "afno_backward", "layer_norm", "attention", "attention_qkv", "rotary", "rotary_attention_qkv", "dropout"}
 
 
 class _Counting:
