@@ -303,17 +303,19 @@ __device__ __forceinline__ KeyTiles key_tiles(const TileParams& p, int r0, int r
   k.end[1] = two ? hi1 - lo0 + k.sinks : 0;
   return k;
 }
+__device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
 // The keys from k0 on that token i sees, as columns: from `from` to `to`, and those below `sinks`
 struct SeenKeys {
   int from, to, sinks;
   __device__ __forceinline__ SeenKeys(const TileParams& p, int i, int len, int k0)
       : from(i - p.left - k0), to(last_seen(p, i, len) + 1 - k0), sinks(min(p.sinks, p.causal ? min(i + 1, len) : len) - k0) {}
-  __device__ __forceinline__ bool operator()(int c) const { return (c >= from && c < to) || c < sinks; }
+  // of the 32 columns from c0 on
+  __device__ __forceinline__ uint32_t bits(int c0) const { return (low_bits(to - c0) & ~low_bits(from - c0)) | low_bits(sinks - c0); }
 };
-// Whether every one of the 128 tokens from `first` on sees all of `n` keys from k0 on
-__device__ __forceinline__ bool all_seen(const TileParams& p, int first, int len, int k0, int n) {
-  if (k0 + n > len || (p.causal && k0 + n - 1 > first)) return false;
-  return k0 + n <= p.sinks || (k0 >= first + TILE - 1 - p.left && k0 + n - 1 - first <= p.right);
+// Whether every one of the 128 tokens from `first` on sees all 128 keys from k0 on
+__device__ __forceinline__ bool all_seen(const TileParams& p, int first, int len, int k0) {
+  if (k0 + TILE > len || (p.causal && k0 + TILE - 1 > first)) return false;
+  return k0 + TILE <= p.sinks || (k0 >= first + TILE - 1 - p.left && k0 + TILE - 1 - first <= p.right);
 }
 
 // 16 (or the first 8) fp32 values as bf16
@@ -432,18 +434,28 @@ struct Row {
   }
   // 128 scores -> weights 2^(scale S - m), as bf16 in the first half of them.  (A share of the exponentials on the FMA pipe, which helps the backward
   // pass, is slower here: 16200 tokens, 8 heads of 48: 750 us without, 860 - 930 with an eighth to three eighths of them.)
-  __device__ __forceinline__ void weights(uint32_t (&v)[TILE], float scale) {
+  // `none`: 32 columns each whose weights are 0 without a look.
+  template <bool WIN>
+  __device__ __forceinline__ void weights(uint32_t (&v)[TILE], float scale, uint32_t none) {
     // (a row that has seen nothing but -inf has no maximum yet, and weights of 0)
     const float from = m == -INFINITY ? 0.f : -m;
     const f32x2 scale2 = f2_pack(scale, scale), from2 = f2_pack(from, from);
 #pragma unroll
-    for (int c = 0; c < TILE; c += 2) {
-      float a, b;
-      f2_unpack(f2_fma(f2_pack(__uint_as_float(v[c]), __uint_as_float(v[c + 1])), scale2, from2), a, b);
-      a = ex2(a);
-      b = ex2(b);
-      sum[(c >> 1) & 1] = f2_add(sum[(c >> 1) & 1], f2_pack(a, b));
-      v[c / 2] = pack_bf16(a, b);
+    for (int c0 = 0; c0 < TILE; c0 += 32) {
+      if (WIN && (none >> (c0 / 32) & 1)) {
+#pragma unroll
+        for (int c = 0; c < 16; ++c) v[c0 / 2 + c] = 0u;
+        continue;
+      }
+#pragma unroll
+      for (int c = c0; c < c0 + 32; c += 2) {
+        float a, b;
+        f2_unpack(f2_fma(f2_pack(__uint_as_float(v[c]), __uint_as_float(v[c + 1])), scale2, from2), a, b);
+        a = ex2(a);
+        b = ex2(b);
+        sum[(c >> 1) & 1] = f2_add(sum[(c >> 1) & 1], f2_pack(a, b));
+        v[c / 2] = pack_bf16(a, b);
+      }
     }
   }
 };
@@ -459,10 +471,19 @@ __device__ __forceinline__ void hide_scores(uint32_t (&v)[TILE], int seen) {
   for (int c = 0; c < TILE; ++c)
     if (c >= seen) v[c] = 0xff800000u;
 }
-__device__ __forceinline__ void hide_scores(uint32_t (&v)[TILE], const SeenKeys& seen) {
+// The same through a window, 32 columns at a time; a bit for each of those that no row of the warp sees
+__device__ __forceinline__ uint32_t hide_scores(uint32_t (&v)[TILE], const SeenKeys& seen) {
+  uint32_t none = 0;
 #pragma unroll
-  for (int c = 0; c < TILE; ++c)
-    if (!seen(c)) v[c] = 0xff800000u;
+  for (int c = 0; c < TILE; c += 32) {
+    const uint32_t m = seen.bits(c);
+    if (__all_sync(0xffffffffu, m == 0xffffffffu)) continue;
+    if (!__any_sync(0xffffffffu, m != 0)) none |= 1u << (c / 32);
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (!(m >> i & 1)) v[c + i] = 0xff800000u;
+  }
+  return none;
 }
 __device__ __forceinline__ void store_weights(uint32_t p_at, const uint32_t (&v)[TILE]) {
   tmem_st32(p_at, v);
@@ -703,8 +724,9 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       uint32_t v[TILE];
       load_scores(s_at, v);
       const int k0 = tile(j) * TILE;
+      uint32_t none = 0;
       if constexpr (WIN) {
-        if (!all_seen(p.t, w.r0 + t * TILE, w.len, k0, TILE)) hide_scores(v, SeenKeys(p.t, w.r0 + row, w.len, k0));
+        if (!all_seen(p.t, w.r0 + t * TILE, w.len, k0)) none = hide_scores(v, SeenKeys(p.t, w.r0 + row, w.len, k0));
       } else if (k0 + TILE > w.len || (causal && k0 + TILE - 1 > w.r0 + t * TILE)) {
         hide_scores(v, (causal ? min(w.len, w.r0 + row + 1) : w.len) - k0);
       }
@@ -714,7 +736,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         const float f = r.grow(top);
         if (j > start) scale_row(o_at, p.t.DP, f);
       }
-      r.weights(v, scale);
+      r.weights<WIN>(v, scale, none);
       store_weights(s_at, v);
       tc_fence_before();
       __syncwarp();
@@ -946,8 +968,9 @@ attn_fwd_narrow_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
       __syncwarp();
       if (lane == 0) mbar_arrive(s_read(t));
       const int k0 = tile(j) * TILE;
+      uint32_t none = 0;
       if constexpr (WIN) {
-        if (!all_seen(p.t, w.r0 + t * TILE, w.len, k0, TILE)) hide_scores(v, SeenKeys(p.t, w.r0 + row, w.len, k0));
+        if (!all_seen(p.t, w.r0 + t * TILE, w.len, k0)) none = hide_scores(v, SeenKeys(p.t, w.r0 + row, w.len, k0));
       } else if (k0 + TILE > w.len || (causal && k0 + TILE - 1 > w.r0 + t * TILE)) {
         hide_scores(v, (causal ? min(w.len, w.r0 + row + 1) : w.len) - k0);
       }
@@ -961,7 +984,7 @@ attn_fwd_narrow_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
           scale_row(o_at, p.t.DP, f);
         }
       }
-      r.weights(v, scale);
+      r.weights<WIN>(v, scale, none);
       if (j > start) {
         ok = __all_sync(0xffffffffu, mbar_wait_soon(o_done(t), (j - start - 1) & 1));
         if (!ok) break;
@@ -1301,12 +1324,17 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
       const uint32_t s_at = tmem + lanes + (j & 1) * S_COLS + x * BWD_COLS, dp_at = tmem + lanes + DQ_DP + x * BWD_COLS;
       tmem_req32(s_at, v);
       const int k0 = tile(j) * TILE + x * BWD_COLS;
-      const bool edge = WIN ? !all_seen(p.t, w.r0, w.len, k0, BWD_COLS) : k0 + BWD_COLS > w.len || (causal && k0 + BWD_COLS - 1 > w.r0);
+      bool edge = k0 + BWD_COLS > w.len || (causal && k0 + BWD_COLS - 1 > w.r0), none = false;
       const int below = (causal ? min(w.len, w.r0 + row + 1) : w.len) - k0;
-      const SeenKeys in_window(p.t, w.r0 + row, w.len, k0);
-      auto seen = [&](int c) { return WIN ? in_window(c) : c < below; };
+      uint32_t bits = 0xffffffffu;
+      if constexpr (WIN) {
+        bits = SeenKeys(p.t, w.r0 + row, w.len, k0).bits(0);
+        edge = !__all_sync(0xffffffffu, bits == 0xffffffffu);
+        none = !__any_sync(0xffffffffu, bits != 0);
+      }
+      auto seen = [&](int c) { return WIN ? (bits >> c & 1) != 0 : c < below; };
       tmem_wait32(v);
-      weights_of<false>(v, scale2, [&](int) { return l2; }, seen);
+      if (!WIN || !none) weights_of<false>(v, scale2, [&](int) { return l2; }, seen);
       ok = __all_sync(0xffffffffu, mbar_wait_soon(dp_full, j & 1));
       if (!ok) break;
       tc_fence_after();
@@ -1653,23 +1681,33 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       // the queries that see this key are the columns from `from` to `to`
       bool edge = q0 + BWD_COLS > w.len || (causal && q0 < w.r0 + TILE - 1);
       int from = causal ? w.r0 + row - q0 : 0, to = w.len - q0;
+      uint32_t bits = 0xffffffffu;
+      bool none = false;
       if constexpr (WIN) {
         const int key = w.r0 + row;
-        if (w.r0 + TILE > p.t.sinks) edge = edge || q0 + BWD_COLS - 1 - w.r0 > p.t.left || (!causal && q0 < w.r0 + TILE - 1 - p.t.right);
         if (key >= p.t.sinks) {
           if (!causal) from = key - p.t.right - q0;
           if (p.t.left < w.len - 1 - key) to = key + p.t.left + 1 - q0;
         }
+        bits = low_bits(to) & ~low_bits(from);
+        edge = !__all_sync(0xffffffffu, bits == 0xffffffffu);
+        none = !__any_sync(0xffffffffu, bits != 0);
       }
-      auto seen = [&](int c) { return c >= from && c < to; };
+      auto seen = [&](int c) { return WIN ? (bits >> c & 1) != 0 : c >= from && c < to; };
       auto neg_l = [&](int c) { return *reinterpret_cast<const f32x2*>(stats + c); };
       auto neg_delta = [&](int c) { return *reinterpret_cast<const f32x2*>(stats + TILE + c); };
       uint32_t v[BWD_COLS], packed[BWD_COLS / 2];
       const uint32_t s_at = tmem + lanes + buf * S_COLS + x * BWD_COLS, dp_at = tmem + lanes + L::DP_AT + x * BWD_COLS;
       tmem_req32(s_at, v);
       tmem_wait32(v);
-      if (edge) weights_of<true>(v, scale2, neg_l, seen);
-      else weights_of<false>(v, scale2, neg_l, seen);
+      if (WIN && none) {
+#pragma unroll
+        for (int c = 0; c < BWD_COLS; ++c) v[c] = 0u;
+      } else if (edge) {
+        weights_of<true>(v, scale2, neg_l, seen);
+      } else {
+        weights_of<false>(v, scale2, neg_l, seen);
+      }
 #pragma unroll
       for (int c = 0; c < BWD_COLS; c += 2) packed[c / 2] = pack_bf16(__uint_as_float(v[c]), __uint_as_float(v[c + 1]));
       tmem_st16(s_at, packed);
@@ -1832,6 +1870,7 @@ int window_tiles(const AttnShape& p) {
   return static_cast<int>(std::min<long long>((span + TILE - 1) / TILE + 1, (mean_length(p) + TILE - 1) / TILE));
 }
 bool one_tile_pays(const AttnShape& p) {
+  if (p.window) if (const char* e = getenv("MK_QT")) return e[0] == 49;
   const int mean = p.window ? std::min(mean_length(p), window_tiles(p) * TILE) : mean_length(p);
   return mean <= (p.D <= 64 ? 768 : 448) && blocks_of(slots_of(p, p.H, 2 * TILE, 1)) > sm_count();
 }

@@ -15,6 +15,7 @@
 #include <algorithm>
 
 #include "fused_ops.cuh"
+#include "gelu.cuh"
 #include "gemm_tcgen05.cuh"
 #include "launch.cuh"
 #include "vec8.cuh"
@@ -33,13 +34,29 @@ struct KernelParams {
   float* sums;             // [2: dw, db][blocks][D]
 };
 
-// Sum over the LANES lanes of a group, in all of them
+// Sums of N values (a power of two) over the LANES lanes of a group, in all of them.  While there are several, a step of the butterfly gives half of them away:
+// 15 exchanges for eight values over eight lanes where 24 were.
 template <int LANES, int N>
 __device__ __forceinline__ void group_sum(float (&a)[N]) {
+  const int l = threadIdx.x & 31;
+  int o = LANES / 2;
 #pragma unroll
-  for (int o = LANES / 2; o > 0; o >>= 1)
+  for (int n = N; n > 1 && o > 0; n >>= 1, o >>= 1) {
+    const bool upper = (l & o) != 0;
 #pragma unroll
-    for (int i = 0; i < N; ++i) a[i] += __shfl_xor_sync(0xffffffffu, a[i], o);
+    for (int i = 0; i < n / 2; ++i) {
+      const float mine = upper ? a[i + n / 2] : a[i], other = upper ? a[i] : a[i + n / 2];
+      a[i] = mine + __shfl_xor_sync(0xffffffffu, other, o);
+    }
+  }
+#pragma unroll
+  for (; o > 0; o >>= 1) a[0] += __shfl_xor_sync(0xffffffffu, a[0], o);
+  static_assert(N <= LANES, "a value to a lane at least");
+  // value i is now with the lanes whose upper bits (below LANES) are i's
+  constexpr int EACH = LANES / N;
+  const float part = a[0];
+#pragma unroll
+  for (int i = 0; i < N; ++i) a[i] = __shfl_sync(0xffffffffu, part, (l & ~(LANES - 1)) + i * EACH);
 }
 
 __device__ __forceinline__ double position_of(const void* at, int type, long long i) {
@@ -48,6 +65,19 @@ __device__ __forceinline__ double position_of(const void* at, int type, long lon
     case ROT_POS_I64: return static_cast<double>(static_cast<const long long*>(at)[i]);
     case ROT_POS_F32: return static_cast<double>(static_cast<const float*>(at)[i]);
     default: return static_cast<const double*>(at)[i];
+  }
+}
+
+// Of a fraction of a turn, at most half of one.  For bf16 the special function unit's, which are off by 2^-20 (a step of bf16 is 2^-7 of the value; 16200 tokens, 24
+// heads of 64, SINUS us with the library's).
+template <typename T>
+__device__ __forceinline__ void sine_cosine(float turn, float& sine, float& cosine) {
+  if constexpr (sizeof(T) == 2) {
+    const float angle = turn * 6.283185307179586f;
+    sine = __sinf(angle);
+    cosine = __cosf(angle);
+  } else {
+    sincospif(2.f * turn, &sine, &cosine);
   }
 }
 
@@ -62,78 +92,58 @@ __device__ __forceinline__ int partner_of(const RotShape& s, int c) {
   return c;
 }
 
-// A lane's channels have their partners in runs of four channels, wherever, or (RUN 1) one by one; RUN 0: neighbours
-template <typename T, int RUN>
-__device__ __forceinline__ void partners(const T* row, const int (&at)[RUN == 4 ? 2 : 8], const float (&own)[8], float (&f)[8]) {
-  if constexpr (RUN == 0) {
+// Eight values as four pairs
+__device__ __forceinline__ void pairs_of(const Vec8<__nv_bfloat16>& raw, f32x2 (&f)[4]) {
+  const uint32_t u[4] = {raw.v.x, raw.v.y, raw.v.z, raw.v.w};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = own[i ^ 1];
-  } else if constexpr (RUN == 1) {
+  for (int i = 0; i < 4; ++i) f[i] = f2_pack(__uint_as_float(u[i] << 16), __uint_as_float(u[i] & 0xffff0000u));
+}
+__device__ __forceinline__ void pairs_of(const Vec8<float>& raw, f32x2 (&f)[4]) {
+  f[0] = f2_pack(raw.a.x, raw.a.y), f[1] = f2_pack(raw.a.z, raw.a.w), f[2] = f2_pack(raw.b.x, raw.b.y), f[3] = f2_pack(raw.b.z, raw.b.w);
+}
+template <typename T>
+__device__ __forceinline__ Vec8<T> rounded_pairs(const f32x2 (&f)[4]) {
+  float v[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = value_of(row[at[i]]);
-  } else if constexpr (sizeof(T) == 2) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const uint2 u = *reinterpret_cast<const uint2*>(row + at[i]);
-      f[4 * i] = __uint_as_float(u.x << 16);
-      f[4 * i + 1] = __uint_as_float(u.x & 0xffff0000u);
-      f[4 * i + 2] = __uint_as_float(u.y << 16);
-      f[4 * i + 3] = __uint_as_float(u.y & 0xffff0000u);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const float4 v = *reinterpret_cast<const float4*>(row + at[i]);
-      f[4 * i] = v.x, f[4 * i + 1] = v.y, f[4 * i + 2] = v.z, f[4 * i + 3] = v.w;
-    }
-  }
+  for (int i = 0; i < 4; ++i) f2_unpack(f[i], v[2 * i], v[2 * i + 1]);
+  Vec8<T> raw;
+  raw.set(v);
+  return raw;
+}
+__device__ __forceinline__ float sum_of(const f32x2 (&f)[4]) {
+  float a, b;
+  f2_unpack(f2_add(f2_add(f[0], f[1]), f2_add(f[2], f[3])), a, b);
+  return a + b;
+}
+__device__ __forceinline__ float sum_of_products(const f32x2 (&f)[4], const f32x2 (&g)[4]) {
+  float a, b;
+  f2_unpack(f2_add(f2_fma(f[0], g[0], f2_mul(f[1], g[1])), f2_fma(f[2], g[2], f2_mul(f[3], g[3]))), a, b);
+  return a + b;
 }
 
-// Mean (layer norm) and 1 / sqrt(var + eps) of R heads, whose channels a group has
-template <int LANES, int NORM, int R>
-__device__ __forceinline__ void statistics(const float (&v)[R][8], bool mine, float inv, float eps, float (&mean)[R], float (&rstd)[R]) {
-  if constexpr (NORM == ROT_NORM_LAYER) {
-    float a[R], dev[2 * R];
+// What a lane's channels are turned with.  RUN 4: partners stand side by side in runs of four channels at least; 1: wherever; 0: neighbours
+template <typename T, int RUN>
+__device__ __forceinline__ void partners(const T* row, const int (&at)[RUN == 4 ? 2 : 8], const f32x2 (&own)[4], f32x2 (&f)[4]) {
+  if constexpr (RUN == 0) {
 #pragma unroll
-    for (int q = 0; q < R; ++q) {
-      a[q] = 0.f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) a[q] += v[q][i];
+    for (int i = 0; i < 4; ++i) {
+      float a, b;
+      f2_unpack(own[i], a, b);
+      f[i] = f2_pack(b, a);
     }
-    group_sum<LANES>(a);
+  } else if constexpr (RUN == 1) {
 #pragma unroll
-    for (int q = 0; q < R; ++q) {
-      mean[q] = a[q] * inv;
-      dev[2 * q] = dev[2 * q + 1] = 0.f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float d = mine ? v[q][i] - mean[q] : 0.f;
-        dev[2 * q] += d;
-        dev[2 * q + 1] = fmaf(d, d, dev[2 * q + 1]);
-      }
-    }
-    group_sum<LANES>(dev);
-#pragma unroll
-    for (int q = 0; q < R; ++q) {
-      // (deviations from the rounded mean; their own mean puts it right)
-      const float left = dev[2 * q] * inv;
-      mean[q] += left;
-      rstd[q] = 1.f / sqrtf(fmaxf(fmaf(dev[2 * q + 1], inv, -left * left), 0.f) + eps);
-    }
+    for (int i = 0; i < 4; ++i) f[i] = f2_pack(value_of(row[at[2 * i]]), value_of(row[at[2 * i + 1]]));
   } else {
-    float a[R];
-#pragma unroll
-    for (int q = 0; q < R; ++q) {
-      a[q] = 0.f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) a[q] = fmaf(v[q][i], v[q][i], a[q]);
+    Vec8<T> raw;
+    if constexpr (sizeof(T) == 2) {
+      const uint2 a = *reinterpret_cast<const uint2*>(row + at[0]), b = *reinterpret_cast<const uint2*>(row + at[1]);
+      raw.v = make_uint4(a.x, a.y, b.x, b.y);
+    } else {
+      raw.a = *reinterpret_cast<const float4*>(row + at[0]);
+      raw.b = *reinterpret_cast<const float4*>(row + at[1]);
     }
-    group_sum<LANES>(a);
-#pragma unroll
-    for (int q = 0; q < R; ++q) {
-      mean[q] = 0.f;
-      rstd[q] = 1.f / sqrtf(fmaf(a[q], inv, eps));
-    }
+    pairs_of(raw, f);
   }
 }
 
@@ -141,11 +151,13 @@ __device__ __forceinline__ void statistics(const float (&v)[R][8], bool mine, fl
 template <typename T, int LANES, int NORM, bool BACK, int RUN, int R, int BLOCKS>
 __global__ void __launch_bounds__(THREADS, BLOCKS) rotary_kernel(const __grid_constant__ KernelParams p) {
   constexpr int GROUPS = 32 / LANES, ROW = LANES * 8;
-  constexpr bool XCHG = RUN > 0, NORMED = NORM != ROT_NORM_NONE, READ_X = NORMED || !BACK, SUMS = BACK && NORMED;
+  constexpr bool XCHG = RUN > 0, NORMED = NORM != ROT_NORM_NONE, READ_X = NORMED || !BACK, SUMS = BACK && NORMED, LAYER = NORM == ROT_NORM_LAYER;
   const RotShape& s = p.s;
   __shared__ __align__(16) T rows[XCHG ? WARPS * R * GROUPS * ROW : 8];
   __shared__ __align__(16) float2 angles[WARPS * GROUPS * ROW];      // cos and signed sin of every channel
-  __shared__ float params[NORMED ? 2 : 1][NORMED ? ROT_WIDTH : 1];
+  __shared__ double turns[ROW / 2];                                  // of every pair, and (axis, its channels)
+  __shared__ int places[ROW / 2];
+  __shared__ float params[NORMED ? 2 : 1][NORMED ? ROW : 1];
   const int which = blockIdx.x < static_cast<unsigned>(p.blocks0) ? 0 : 1;
   const RotPart& part = s.part[which];
   const T *x = static_cast<const T*>(part.x.ptr), *dy = static_cast<const T*>(part.dy.ptr);
@@ -154,113 +166,134 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) rotary_kernel(const __grid_co
   chain_begin(true, x, dy, w_at, b_at, positions);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = lane / LANES, l = lane % LANES, c0 = l * 8, D = s.D;
-  const bool mine = c0 < D;                  // (lanes behind the last channel)
+  const bool mine = c0 < D;                  // (lanes behind the last channel have zeros)
   T* const my_rows = rows + (XCHG ? (warp * GROUPS + group) * R * ROW : 0);
   float2* const my_angles = angles + (warp * GROUPS + group) * ROW;
   int at[RUN == 4 ? 2 : 8], pairs = 0;
 #pragma unroll
   for (int i = 0; i < (RUN == 4 ? 2 : 8); ++i) at[i] = RUN == 0 ? 0 : partner_of(s, c0 + i * (RUN == 4 ? 4 : 1));
-  if (positions)
-    for (int a = 0; a < s.axes; ++a) pairs += s.band[a] >> 1;
+  if (positions) {
+    int start = 0;
+    for (int a = 0; a < s.axes; ++a) {
+      const int half = s.band[a] >> 1;
+      for (int i = threadIdx.x; i < half; i += THREADS) {
+        const int lo = start + (RUN == 0 ? 2 * i : i), hi = lo + (RUN == 0 ? 1 : half);
+        turns[pairs + i] = s.turns[pairs + i];
+        places[pairs + i] = a << 16 | lo << 8 | hi;
+      }
+      pairs += half;
+      start += 2 * half;
+    }
+  }
 #pragma unroll
   for (int i = 0; i < 8; ++i) my_angles[c0 + i] = make_float2(1.f, 0.f);
+  if constexpr (NORMED) {
+    for (int c = threadIdx.x; c < ROW; c += THREADS) {
+      params[0][c] = c < D ? (w_at ? w_at[c] : 1.f) : 0.f;
+      params[1][c] = c < D && b_at ? b_at[c] : 0.f;
+    }
+  }
+  __syncthreads();
   // channels that are not turned have no partner (whatever it holds)
   const int alone = 2 * pairs - c0;
-  auto turned = [&](float (&y)[8]) {
+  auto turned = [&](f32x2 (&y)[4]) {
     if (alone >= 8) return;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = i < alone ? y[i] : 0.f;
+    for (int i = 0; i < 4; ++i) y[i] = 2 * i < alone ? y[i] : 0ull;      // (bands are even)
   };
-  if constexpr (NORMED) {
-    for (int c = threadIdx.x; c < D; c += THREADS) {
-      params[0][c] = w_at ? w_at[c] : 1.f;
-      params[1][c] = b_at ? b_at[c] : 0.f;
-    }
-    __syncthreads();
-  }
-  float w[8], dw[8], db[8];
+  f32x2 w[4], dw[4], db[4];
   if constexpr (SUMS) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      w[i] = mine ? params[0][c0 + i] : 0.f;
-      dw[i] = db[i] = 0.f;
+    for (int i = 0; i < 4; ++i) {
+      w[i] = f2_pack(params[0][c0 + 2 * i], params[0][c0 + 2 * i + 1]);
+      dw[i] = db[i] = 0ull;
     }
   }
   const int limit = BACK && s.limit ? *s.limit : s.N;
   const float inv = 1.f / static_cast<float>(D);
   const int chunks = p.chunks[which], per_chunk = (part.heads + chunks - 1) / chunks;
-  const long long units = 1ll * s.B * s.N * chunks;
+  const unsigned units = static_cast<unsigned>(s.B) * s.N * chunks;      // (below 2^31)
   const int block = which ? blockIdx.x - p.blocks0 : blockIdx.x, blocks = which ? p.blocks - p.blocks0 : p.blocks0;
-  const long long step = 1ll * blocks * WARPS * GROUPS;
+  const unsigned step = static_cast<unsigned>(blocks) * WARPS * GROUPS;
   // (the groups of a warp go through the loop together)
-  for (long long first = (1ll * block * WARPS + warp) * GROUPS; first < units; first += step) {
-    const long long u = first + group, t = u < units ? u / chunks : 0;
-    const int chunk = u < units ? static_cast<int>(u - t * chunks) : 0, bat = static_cast<int>(t / s.N), n = static_cast<int>(t - 1ll * bat * s.N);
-    const bool here = u < units && (!BACK || n < limit);
-    const int h0 = chunk * per_chunk, h1 = here ? min(part.heads, h0 + per_chunk) : h0;
-    const T* const x_at = READ_X ? x + bat * part.x.batch + n * part.x.token + c0 : nullptr;
-    const T* const d_at = BACK ? dy + bat * part.dy.batch + n * part.dy.token + c0 : nullptr;
-    T* const o_at = static_cast<T*>(part.out.ptr) + bat * part.out.batch + n * part.out.token + c0;
+  for (unsigned first = (static_cast<unsigned>(block) * WARPS + warp) * GROUPS; first < units; first += step) {
+    const unsigned u = min(first + group, units - 1), t = chunks == 1 ? u : u / chunks;
+    const int chunk = static_cast<int>(u - t * chunks), bat = s.B == 1 ? 0 : static_cast<int>(t / s.N), n = static_cast<int>(t - static_cast<unsigned>(bat) * s.N);
+    const int h0 = chunk * per_chunk;
+    const int count = mine && first + group < units && (!BACK || n < limit) ? min(part.heads - h0, per_chunk) : 0;      // heads that this lane has a part of
+    const T* x_at = READ_X ? x + bat * part.x.batch + n * part.x.token + h0 * part.x.head + c0 : nullptr;
+    const T* d_at = BACK ? dy + bat * part.dy.batch + n * part.dy.token + h0 * part.dy.head + c0 : nullptr;
+    T* o_at = static_cast<T*>(part.out.ptr) + bat * part.out.batch + n * part.out.token + h0 * part.out.head + c0;
 
     Vec8<T> vx[READ_X ? R : 1], vd[BACK ? R : 1];
-    auto fetch = [&](int h) {
+#pragma unroll
+    for (int q = 0; q < R; ++q) {
+      if constexpr (READ_X) vx[q].clear();
+      if constexpr (BACK) vd[q].clear();
+    }
+    auto fetch = [&](int k) {
 #pragma unroll
       for (int q = 0; q < R; ++q) {
-        const bool in = mine && h + q < h1;
+        const bool in = k + q < count;
         if constexpr (READ_X) {
-          if (in) vx[q].load(x_at + (h + q) * part.x.head);
-          else vx[q].clear();
+          if (in) vx[q].load(x_at);
+          x_at += part.x.head;
         }
         if constexpr (BACK) {
-          if (in) vd[q].load(d_at + (h + q) * part.dy.head);
-          else vd[q].clear();
+          if (in) vd[q].load(d_at);
+          else vd[q].clear();      // (they would be added to the sums)
+          d_at += part.dy.head;
         }
       }
     };
-    fetch(h0);
+    fetch(0);
 
     // angles of the token
     if (positions) {
       __syncwarp();
-      for (int i = l; i < pairs; i += LANES) {
-        int a = 0, start = 0, half = s.band[0] >> 1, in = i;
-        while (in >= half) {
-          in -= half;
-          start += 2 * half;
-          half = s.band[++a] >> 1;
-        }
-        const double turns = position_of(positions, s.position_type, bat * s.position_batch + 1ll * n * s.axes + a) * s.turns[i];
+      const long long from = bat * s.position_batch + 1ll * n * s.axes;
+      int place[4];
+      double turn[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {      // (at most half of a lane's eight channels)
+        const int i = l + j * LANES;
+        place[j] = i < pairs ? places[i] : 0;
+        turn[j] = i < pairs ? position_of(positions, s.position_type, from + (place[j] >> 16)) * turns[i] : 0.0;
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
         float sine, cosine;
-        sincospif(2.f * static_cast<float>(turns - rint(turns)), &sine, &cosine);
+        sine_cosine<T>(static_cast<float>(turn[j] - rint(turn[j])), sine, cosine);
         if (BACK != (s.inverse != 0)) sine = -sine;
-        const int lo = start + (RUN == 0 ? 2 * in : in), hi = lo + (RUN == 0 ? 1 : half);
-        my_angles[lo] = make_float2(cosine, -sine);
-        my_angles[hi] = make_float2(cosine, sine);
+        if (l + j * LANES < pairs) {
+          my_angles[place[j] >> 8 & 255] = make_float2(cosine, -sine);
+          my_angles[place[j] & 255] = make_float2(cosine, sine);
+        }
       }
       __syncwarp();
     }
-    float cs[8], sn[8], add[8];
+    f32x2 cs[4], sn[4], add[4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float2 a = my_angles[c0 + i];
-      cs[i] = a.x;
-      sn[i] = a.y;
+    for (int i = 0; i < 4; ++i) {
+      const float4 a = *reinterpret_cast<const float4*>(my_angles + c0 + 2 * i);
+      cs[i] = f2_pack(a.x, a.z);
+      sn[i] = f2_pack(a.y, a.w);
     }
     // forward: out = rstd ((x - mean) (cos w) + (x' - mean) (sin w')) + (cos b + sin b')
     if constexpr (NORMED && !BACK) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int c = RUN == 0 ? (pairs > 0 ? (c0 + i) ^ 1 : c0 + i) : RUN == 4 ? at[i / 4] + i % 4 : at[i];
-        add[i] = mine ? fmaf(cs[i], params[1][c0 + i], sn[i] * params[1][c]) : 0.f;
-        cs[i] *= mine ? params[0][c0 + i] : 0.f;
-        sn[i] *= mine ? params[0][c] : 0.f;
+      for (int i = 0; i < 4; ++i) {
+        auto mate = [&](int c) { return RUN == 0 ? (pairs > 0 ? c ^ 1 : c) : RUN == 4 ? at[(c - c0) / 4] + (c - c0) % 4 : at[c - c0]; };
+        const int c = c0 + 2 * i, m0 = mate(c), m1 = mate(c + 1);
+        add[i] = f2_fma(cs[i], f2_pack(params[1][c], params[1][c + 1]), f2_mul(sn[i], f2_pack(params[1][m0], params[1][m1])));
+        cs[i] = f2_mul(cs[i], f2_pack(params[0][c], params[0][c + 1]));
+        sn[i] = f2_mul(sn[i], f2_pack(params[0][m0], params[0][m1]));
       }
     }
 
     // (all groups of the warp make as many turns)
     for (int k = 0; k < per_chunk; k += R) {
-      const int h = h0 + k;
-      Vec8<T> now[R], now_d[BACK ? R : 1];
+      Vec8<T> now[READ_X ? R : 1], now_d[BACK ? R : 1];
 #pragma unroll
       for (int q = 0; q < R; ++q) {
         if constexpr (READ_X) now[q] = vx[q];
@@ -275,71 +308,95 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) rotary_kernel(const __grid_co
         }
         __syncwarp();
       }
-      if (k + R < per_chunk) fetch(h + R);
+      if (k + R < per_chunk) fetch(k + R);
+      auto put = [&](int q, const f32x2 (&v)[4]) {
+        if (k + q < count) rounded_pairs<T>(v).store(o_at);
+        o_at += part.out.head;
+      };
       if constexpr (!NORMED) {
 #pragma unroll
         for (int q = 0; q < R; ++q) {
-          float v[8], y[8];
-          if constexpr (BACK) now_d[q].get(v);
-          else now[q].get(v);
+          f32x2 v[4], y[4];
+          if constexpr (BACK) pairs_of(now_d[q], v);
+          else pairs_of(now[q], v);
           partners<T, RUN>(my_rows + q * ROW, at, v, y);
           turned(y);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] = fmaf(cs[i], v[i], sn[i] * y[i]);
-          Vec8<T> out;
-          out.set(v);
-          if (mine && h + q < h1) out.store(o_at + (h + q) * part.out.head);
+          for (int i = 0; i < 4; ++i) v[i] = f2_fma(cs[i], v[i], f2_mul(sn[i], y[i]));
+          put(q, v);
         }
       } else {
-        float v[R][8], mean[R], rstd[R];
+        // Sums of a head: of the deviations from a value near the mean (that of its first eight channels: the variance loses little to their own mean) and of their
+        // squares; backward, of g w and its products with them
+        constexpr int EACH = (LAYER ? 2 : 1) * (BACK ? 2 : 1);
+        f32x2 v[R][4], g[BACK ? R : 1][4];
+        float sums[R * EACH], pivot[R];
 #pragma unroll
-        for (int q = 0; q < R; ++q) now[q].get(v[q]);
-        statistics<LANES, NORM, R>(v, mine, inv, s.eps, mean, rstd);
-        if constexpr (!BACK) {
+        for (int q = 0; q < R; ++q) {
+          pairs_of(now[q], v[q]);
+          if constexpr (LAYER) {
+            pivot[q] = __shfl_sync(0xffffffffu, sum_of(v[q]) * 0.125f, lane & ~(LANES - 1));
+            const f32x2 off = f2_pack(mine ? -pivot[q] : 0.f, mine ? -pivot[q] : 0.f);
 #pragma unroll
-          for (int q = 0; q < R; ++q) {
-            float y[8], o[8];
-            partners<T, RUN>(my_rows + q * ROW, at, v[q], y);
-            turned(y);
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              o[i] = NORM == ROT_NORM_RMS ? fmaf(rstd[q], fmaf(cs[i], v[q][i], sn[i] * y[i]), add[i])
-                                          : fmaf(rstd[q], fmaf(cs[i], v[q][i] - mean[q], sn[i] * (y[i] - mean[q])), add[i]);
-            Vec8<T> out;
-            out.set(o);
-            if (mine && h + q < h1) out.store(o_at + (h + q) * part.out.head);
+            for (int i = 0; i < 4; ++i) v[q][i] = f2_add(v[q][i], off);
+          } else {
+            pivot[q] = 0.f;
           }
-        } else {
-          float g[R][8], a[2 * R];
-#pragma unroll
-          for (int q = 0; q < R; ++q) {
-            float y[8];
-            now_d[q].get(g[q]);
+          if constexpr (BACK) {
+            f32x2 y[4];
+            pairs_of(now_d[q], g[q]);
             partners<T, RUN>(my_rows + q * ROW, at, g[q], y);
             turned(y);
-            a[2 * q] = a[2 * q + 1] = 0.f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const float gi = fmaf(cs[i], g[q][i], sn[i] * y[i]);
-              v[q][i] = (v[q][i] - mean[q]) * rstd[q];
-              dw[i] = fmaf(gi, v[q][i], dw[i]);
-              db[i] += gi;
-              y[i] = gi * w[i];
-              a[2 * q] += y[i];
-              a[2 * q + 1] = fmaf(y[i], v[q][i], a[2 * q + 1]);
+            for (int i = 0; i < 4; ++i) {
+              g[q][i] = f2_fma(cs[i], g[q][i], f2_mul(sn[i], y[i]));
+              db[i] = f2_add(db[i], g[q][i]);
+              y[i] = f2_mul(g[q][i], w[i]);
             }
-#pragma unroll
-            for (int i = 0; i < 8; ++i) g[q][i] = y[i];
+            sums[q * EACH + 1] = sum_of_products(y, v[q]);
+            if constexpr (LAYER) sums[q * EACH + 3] = sum_of(y);
           }
-          group_sum<LANES>(a);
+          sums[q * EACH] = sum_of_products(v[q], v[q]);
+          if constexpr (LAYER) sums[q * EACH + (BACK ? 2 : 1)] = sum_of(v[q]);
+        }
+        group_sum<LANES>(sums);
 #pragma unroll
-          for (int q = 0; q < R; ++q) {
-            const float m0 = NORM == ROT_NORM_LAYER ? a[2 * q] * inv : 0.f, m1 = a[2 * q + 1] * inv;
+        for (int q = 0; q < R; ++q) {
+          const float mean = LAYER ? sums[q * EACH + (BACK ? 2 : 1)] * inv : 0.f;      // of the deviations
+          const float rstd = rsqrtf(fmaxf(fmaf(sums[q * EACH], inv, -mean * mean), 0.f) + s.eps);
+          const f32x2 r2 = f2_pack(rstd, rstd), m2 = f2_pack(-mean, -mean);
+          if constexpr (!BACK) {
+            f32x2 y[4], o[4];
+            if constexpr (RUN == 0) {
+              partners<T, RUN>(my_rows, at, v[q], y);
+            } else {
+              partners<T, RUN>(my_rows + q * ROW, at, v[q], y);
+              if constexpr (LAYER) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) g[q][i] = rstd[q] * (g[q][i] - m0 - v[q][i] * m1);
-            Vec8<T> out;
-            out.set(g[q]);
-            if (mine && h + q < h1) out.store(o_at + (h + q) * part.out.head);
+                for (int i = 0; i < 4; ++i) y[i] = f2_add(y[i], f2_pack(-pivot[q], -pivot[q]));
+              }
+            }
+            turned(y);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              if constexpr (LAYER) o[i] = f2_fma(r2, f2_fma(cs[i], f2_add(v[q][i], m2), f2_mul(sn[i], f2_add(y[i], m2))), add[i]);
+              else o[i] = f2_fma(r2, f2_fma(cs[i], v[q][i], f2_mul(sn[i], y[i])), add[i]);
+            }
+            put(q, o);
+          } else {
+            const float over = LAYER ? sums[q * EACH + 3] * inv : 0.f;                  // mean of g w
+            const float along = rstd * fmaf(sums[q * EACH + 1], inv, -mean * over);     // and of g w xh
+            const f32x2 o2 = f2_pack(-over, -over), a2 = f2_pack(-along, -along);
+            f32x2 o[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const f32x2 xh = f2_mul(LAYER ? f2_add(v[q][i], m2) : v[q][i], r2);
+              dw[i] = f2_fma(g[q][i], xh, dw[i]);
+              f32x2 e = f2_mul(g[q][i], w[i]);
+              if (LAYER) e = f2_add(e, o2);
+              o[i] = f2_mul(f2_fma(xh, a2, e), r2);
+            }
+            put(q, o);
           }
         }
       }
@@ -348,20 +405,26 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) rotary_kernel(const __grid_co
   if constexpr (SUMS) {
     if (!p.sums) return;
     // the groups of a warp, then the warps one after the other
-    __shared__ float cols[2][ROT_WIDTH];
+    __shared__ float cols[2][ROW];
+    float fw[8], fb[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f2_unpack(dw[i], fw[2 * i], fw[2 * i + 1]);
+      f2_unpack(db[i], fb[2 * i], fb[2 * i + 1]);
+    }
 #pragma unroll
     for (int o = LANES; o < 32; o <<= 1)
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        dw[i] += __shfl_xor_sync(0xffffffffu, dw[i], o);
-        db[i] += __shfl_xor_sync(0xffffffffu, db[i], o);
+        fw[i] += __shfl_xor_sync(0xffffffffu, fw[i], o);
+        fb[i] += __shfl_xor_sync(0xffffffffu, fb[i], o);
       }
     for (int k = 0; k < WARPS; ++k) {
       if (warp == k && group == 0 && mine) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          cols[0][c0 + i] = (k ? cols[0][c0 + i] : 0.f) + dw[i];
-          cols[1][c0 + i] = (k ? cols[1][c0 + i] : 0.f) + db[i];
+          cols[0][c0 + i] = (k ? cols[0][c0 + i] : 0.f) + fw[i];
+          cols[1][c0 + i] = (k ? cols[1][c0 + i] : 0.f) + fb[i];
         }
       }
       __syncthreads();
@@ -431,7 +494,7 @@ bool shape_ok(const RotShape& s, bool back) {
   auto bad = [](const RotTensor& t) { return !t.ptr || (reinterpret_cast<uintptr_t>(t.ptr) & 15) || ((t.token | t.head | t.batch) & 7); };
   for (int i = 0; i < s.parts; ++i) {
     const RotPart& q = s.part[i];
-    if (q.heads < 1 || bad(q.out) || (back && bad(q.dy)) || ((!back || s.norm) && bad(q.x)) || (q.dw != nullptr) != (q.db != nullptr)) return false;
+    if (q.heads < 1 || 1ll * s.B * s.N * q.heads >= (1ll << 31) - (1ll << 24) || bad(q.out) || (back && bad(q.dy)) || ((!back || s.norm) && bad(q.x)) || (q.dw != nullptr) != (q.db != nullptr)) return false;
   }
   return true;
 }

@@ -135,9 +135,8 @@ def _check_norm(norm, eps, D, device, params):
             raise ValueError(f"norm over {D} channels on {device}: {name} is {p.dtype} {tuple(p.shape)} on {p.device}")
 
 
-def _native(x) -> bool:
-    return (_ext.native() and x.is_cuda and x.dtype in _TYPES and x.shape[-1] % 8 == 0 and 8 <= x.shape[-1] <= WIDTH
-            and not torch.compiler.is_compiling())
+def _native(x, D: int) -> bool:
+    return _ext.native() and x.is_cuda and x.dtype in _TYPES and D % 8 == 0 and 8 <= D <= WIDTH and not torch.compiler.is_compiling()
 
 
 # ---------------------------------------------------------------------------------------------------- torch's operations
@@ -184,7 +183,7 @@ def _torch(x, weight, bias, positions, axes, eps, norm, inverse=False):
 
 def _run(q, k, qw, kw, qb, kb, positions, axes, eps, norm, inverse=False):
     """Results of one or two tensors whose arguments are checked."""
-    if _native(q):
+    if _native(q, q.shape[-1]):
         packed = q.dim() == 3
         views = [t if t is None or not packed else t[None] for t in (q, k)]
         out = _ext.require().rotary(*views, qw, kw, qb, kb, positions, _no_axes() if axes is None else axes.native(), NORMS[norm], eps, inverse)
@@ -238,7 +237,7 @@ def rotary_attention_qkv(qkv: torch.Tensor, num_heads: int, num_kv_heads: Option
     _check_norm(norm, eps, D, qkv.device, dict(q_weight=q_weight, k_weight=k_weight, q_bias=q_bias, k_bias=k_bias))
     if positions is None and norm is None:
         return attn_ops.attention_qkv(qkv, num_heads, num_kv_heads, causal, scale, offsets, window, sinks)
-    if _native(qkv.unflatten(-1, (-1, D))) and attn_ops.native_ok(qkv, D):
+    if _native(qkv, D) and attn_ops.native_ok(qkv, D):
         mask = attn_ops._check_window(window, sinks, causal)
         scale = attn_ops._check_scale(scale, D)
         at = attn_ops._check_offsets(offsets, qkv.shape[0], qkv.device) if packed else None
