@@ -6,10 +6,11 @@
 // and backward, g = dout turned by -a:   dw = sum g xh, db = sum g, dx = rstd (g w - mean(g w) - xh mean(g w xh)), the means of the layer norm alone.
 //
 // Bound by memory: a head's channels are read once and written once (x and dy in the backward pass), and mean and variance are computed again rather than kept.
-// A group of lanes has the channels of a head, eight to a lane, and goes over the heads of a token: the angles of a token are computed once, in 64 bits down to
-// the fraction of a turn (the angle of position 100000 in 32 bits would be off by 4e-3), sine and cosine of that fraction in 32 bits, and stay in registers with the
-// weights.  The partner's channels come through shared memory as they are in memory.  Statistics, sums and gradients of weights are fp32; blocks leave one row of
-// partial sums each, added up in a fixed order by a second launch.
+// A group of lanes has the channels of a head and goes over the heads of a token.  A lane has four pairs of channels, both of each, so that it turns them
+// without its neighbours: two runs of four channels (halves of a band), or eight side by side (neighbours).  (Eight side by side in either case, with partners
+// through shared memory, took 74 instructions a head and lane where this takes INSTR, and 412 instead of FIXED for a token.)  Angles are computed once for a
+// token's heads, in 64 bits down to the fraction of a turn (the angle of position 100000 in 32 bits would be off by 4e-3).  Statistics, sums and gradients of
+// weights are fp32; blocks leave one row of partial sums each, added up in a fixed order by a second launch.
 #include "rotary.cuh"
 
 #include <algorithm>
@@ -28,7 +29,7 @@ constexpr int THREADS = 256, WARPS = THREADS / 32;
 
 struct KernelParams {
   RotShape s;
-  int chunks[2];           // of a token's heads
+  int chunks[2];           // of a token's heads: divisors
   int blocks0;             // blocks of part 0
   int blocks;
   float* sums;             // [2: dw, db][blocks][D]
@@ -68,8 +69,7 @@ __device__ __forceinline__ double position_of(const void* at, int type, long lon
   }
 }
 
-// Of a fraction of a turn, at most half of one.  For bf16 the special function unit's, which are off by 2^-20 (a step of bf16 is 2^-7 of the value; 16200 tokens, 24
-// heads of 64, SINUS us with the library's).
+// Of a fraction of a turn, at most half of one.  For bf16 the special function unit's, which are off by 2^-20 (half a step of bf16 is 2^-8 of the value).
 template <typename T>
 __device__ __forceinline__ void sine_cosine(float turn, float& sine, float& cosine) {
   if constexpr (sizeof(T) == 2) {
@@ -81,83 +81,118 @@ __device__ __forceinline__ void sine_cosine(float turn, float& sine, float& cosi
   }
 }
 
-// The channel that c is turned with; c itself where it is not
-__device__ __forceinline__ int partner_of(const RotShape& s, int c) {
+// Pair i of a head: its channels, its axis (-1: not turned; the channels behind the bands are paired up as they come)
+struct Pair {
+  int lo, hi, axis;
+};
+__device__ __forceinline__ Pair pair_of(const RotShape& s, int i, bool positions) {
   int start = 0;
-  for (int a = 0; a < s.axes; ++a) {
-    const int half = s.band[a] >> 1, in = c - start;
-    if (in >= 0 && in < 2 * half) return s.interleaved ? c ^ 1 : in < half ? c + half : c - half;
-    start += 2 * half;
-  }
-  return c;
+  if (positions)
+    for (int a = 0; a < s.axes; ++a) {
+      const int half = s.band[a] >> 1, in = i - (start >> 1);
+      if (in >= 0 && in < half) return s.interleaved ? Pair{start + 2 * in, start + 2 * in + 1, a} : Pair{start + in, start + half + in, a};
+      start += 2 * half;
+    }
+  return {2 * i, 2 * i + 1, -1};
 }
 
-// Eight values as four pairs
-__device__ __forceinline__ void pairs_of(const Vec8<__nv_bfloat16>& raw, f32x2 (&f)[4]) {
-  const uint32_t u[4] = {raw.v.x, raw.v.y, raw.v.z, raw.v.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) f[i] = f2_pack(__uint_as_float(u[i] << 16), __uint_as_float(u[i] & 0xffff0000u));
-}
-__device__ __forceinline__ void pairs_of(const Vec8<float>& raw, f32x2 (&f)[4]) {
-  f[0] = f2_pack(raw.a.x, raw.a.y), f[1] = f2_pack(raw.a.z, raw.a.w), f[2] = f2_pack(raw.b.x, raw.b.y), f[3] = f2_pack(raw.b.z, raw.b.w);
-}
-template <typename T>
-__device__ __forceinline__ Vec8<T> rounded_pairs(const f32x2 (&f)[4]) {
-  float v[8];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) f2_unpack(f[i], v[2 * i], v[2 * i + 1]);
-  Vec8<T> raw;
-  raw.set(v);
-  return raw;
-}
-__device__ __forceinline__ float sum_of(const f32x2 (&f)[4]) {
-  float a, b;
-  f2_unpack(f2_add(f2_add(f[0], f[1]), f2_add(f[2], f[3])), a, b);
-  return a + b;
-}
-__device__ __forceinline__ float sum_of_products(const f32x2 (&f)[4], const f32x2 (&g)[4]) {
-  float a, b;
-  f2_unpack(f2_add(f2_fma(f[0], g[0], f2_mul(f[1], g[1])), f2_fma(f[2], g[2], f2_mul(f[3], g[3]))), a, b);
-  return a + b;
-}
-
-// What a lane's channels are turned with.  RUN 4: partners stand side by side in runs of four channels at least; 1: wherever; 0: neighbours
+// How a lane's four pairs lie in memory: RUN 0: eight channels side by side, pairs are neighbours; 4: first and second channels in runs of four; 1: anyhow
+template <int RUN>
+struct Place {
+  int at[RUN == 0 ? 1 : RUN == 4 ? 2 : 8];
+};
+// The channels of four pairs as they come from memory; first and second ones as two values each
 template <typename T, int RUN>
-__device__ __forceinline__ void partners(const T* row, const int (&at)[RUN == 4 ? 2 : 8], const f32x2 (&own)[4], f32x2 (&f)[4]) {
-  if constexpr (RUN == 0) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float a, b;
-      f2_unpack(own[i], a, b);
-      f[i] = f2_pack(b, a);
-    }
-  } else if constexpr (RUN == 1) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) f[i] = f2_pack(value_of(row[at[2 * i]]), value_of(row[at[2 * i + 1]]));
-  } else {
-    Vec8<T> raw;
-    if constexpr (sizeof(T) == 2) {
-      const uint2 a = *reinterpret_cast<const uint2*>(row + at[0]), b = *reinterpret_cast<const uint2*>(row + at[1]);
+struct Channels {
+  Vec8<T> raw;
+  __device__ __forceinline__ void load(const T* p, const Place<RUN>& place) {
+    if constexpr (RUN == 0) {
+      raw.load(p);
+    } else if constexpr (RUN == 4 && sizeof(T) == 2) {
+      const uint2 a = *reinterpret_cast<const uint2*>(p), b = *reinterpret_cast<const uint2*>(p + place.at[1]);
       raw.v = make_uint4(a.x, a.y, b.x, b.y);
+    } else if constexpr (RUN == 4) {
+      raw.a = *reinterpret_cast<const float4*>(p);
+      raw.b = *reinterpret_cast<const float4*>(p + place.at[1]);
     } else {
-      raw.a = *reinterpret_cast<const float4*>(row + at[0]);
-      raw.b = *reinterpret_cast<const float4*>(row + at[1]);
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = value_of(p[place.at[i]]);
+      raw.set(v);
     }
-    pairs_of(raw, f);
+  }
+  __device__ __forceinline__ void store(T* p, const Place<RUN>& place) const {
+    if constexpr (RUN == 0) {
+      raw.store(p);
+    } else if constexpr (RUN == 4 && sizeof(T) == 2) {
+      *reinterpret_cast<uint2*>(p) = make_uint2(raw.v.x, raw.v.y);
+      *reinterpret_cast<uint2*>(p + place.at[1]) = make_uint2(raw.v.z, raw.v.w);
+    } else if constexpr (RUN == 4) {
+      *reinterpret_cast<float4*>(p) = raw.a;
+      *reinterpret_cast<float4*>(p + place.at[1]) = raw.b;
+    } else {
+      float v[8];
+      raw.get(v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) p[place.at[i]] = rounded<T>(v[i]);
+    }
+  }
+  // (raw: RUN 0 pair by pair, else the first channels, then the second ones)
+  __device__ __forceinline__ void get(f32x2 (&lo)[2], f32x2 (&hi)[2]) const {
+    float v[8];
+    raw.get(v);
+    if constexpr (RUN == 0) {
+      lo[0] = f2_pack(v[0], v[2]), lo[1] = f2_pack(v[4], v[6]), hi[0] = f2_pack(v[1], v[3]), hi[1] = f2_pack(v[5], v[7]);
+    } else {
+      lo[0] = f2_pack(v[0], v[1]), lo[1] = f2_pack(v[2], v[3]), hi[0] = f2_pack(v[4], v[5]), hi[1] = f2_pack(v[6], v[7]);
+    }
+  }
+  __device__ __forceinline__ void set(const f32x2 (&lo)[2], const f32x2 (&hi)[2]) {
+    float a[4], b[4];
+    f2_unpack(lo[0], a[0], a[1]), f2_unpack(lo[1], a[2], a[3]), f2_unpack(hi[0], b[0], b[1]), f2_unpack(hi[1], b[2], b[3]);
+    const float pairs[8] = {a[0], b[0], a[1], b[1], a[2], b[2], a[3], b[3]}, runs[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+    raw.set(RUN == 0 ? pairs : runs);
+  }
+};
+__device__ __forceinline__ f32x2 both(float v) { return f2_pack(v, v); }
+__device__ __forceinline__ float sum_of(const f32x2 (&a)[2], const f32x2 (&b)[2]) {
+  float x, y;
+  f2_unpack(f2_add(f2_add(a[0], a[1]), f2_add(b[0], b[1])), x, y);
+  return x + y;
+}
+// sum of a c + b d
+__device__ __forceinline__ float sum_of_products(const f32x2 (&a)[2], const f32x2 (&b)[2], const f32x2 (&c)[2], const f32x2 (&d)[2]) {
+  float x, y;
+  f2_unpack(f2_fma(a[0], c[0], f2_fma(a[1], c[1], f2_fma(b[0], d[0], f2_mul(b[1], d[1])))), x, y);
+  return x + y;
+}
+// Turns pairs by (cos, sin); `alone`: a bit for each that is not turned, and has nothing to do with its partner, whatever it holds
+__device__ __forceinline__ void turn(f32x2 (&lo)[2], f32x2 (&hi)[2], const f32x2 (&cs)[2], const f32x2 (&sn)[2], const f32x2 (&neg)[2], bool plain, uint32_t alone) {
+  f32x2 a[2] = {lo[0], lo[1]}, b[2] = {hi[0], hi[1]};
+  if (plain) {      // (some of a head's channels are not turned)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      float x, y;
+      f2_unpack(a[i], x, y);
+      a[i] = f2_pack(alone >> 2 * i & 1 ? 0.f : x, alone >> (2 * i + 1) & 1 ? 0.f : y);
+      f2_unpack(b[i], x, y);
+      b[i] = f2_pack(alone >> 2 * i & 1 ? 0.f : x, alone >> (2 * i + 1) & 1 ? 0.f : y);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    lo[i] = f2_fma(cs[i], lo[i], f2_mul(neg[i], b[i]));
+    hi[i] = f2_fma(cs[i], hi[i], f2_mul(sn[i], a[i]));
   }
 }
 
-// T: type of the tensors; LANES x 8 channels of a head at most; BACK: gradients; RUN: see `partners`; R: heads at a time
+// T: type of the tensors; LANES x 8 channels of a head at most; BACK: gradients; RUN: see `Place`; R: heads at a time
 template <typename T, int LANES, int NORM, bool BACK, int RUN, int R, int BLOCKS>
 __global__ void __launch_bounds__(THREADS, BLOCKS) rotary_kernel(const __grid_constant__ KernelParams p) {
   constexpr int GROUPS = 32 / LANES, ROW = LANES * 8;
-  constexpr bool XCHG = RUN > 0, NORMED = NORM != ROT_NORM_NONE, READ_X = NORMED || !BACK, SUMS = BACK && NORMED, LAYER = NORM == ROT_NORM_LAYER;
+  constexpr bool NORMED = NORM != ROT_NORM_NONE, READ_X = NORMED || !BACK, SUMS = BACK && NORMED, LAYER = NORM == ROT_NORM_LAYER;
   const RotShape& s = p.s;
-  __shared__ __align__(16) T rows[XCHG ? WARPS * R * GROUPS * ROW : 8];
-  __shared__ __align__(16) float2 angles[WARPS * GROUPS * ROW];      // cos and signed sin of every channel
-  __shared__ double turns[ROW / 2];                                  // of every pair, and (axis, its channels)
-  __shared__ int places[ROW / 2];
-  __shared__ float params[NORMED ? 2 : 1][NORMED ? ROW : 1];
+  __shared__ __align__(16) double turns[ROW / 2];      // of every pair per unit of position
   const int which = blockIdx.x < static_cast<unsigned>(p.blocks0) ? 0 : 1;
   const RotPart& part = s.part[which];
   const T *x = static_cast<const T*>(part.x.ptr), *dy = static_cast<const T*>(part.dy.ptr);
@@ -165,239 +200,208 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) rotary_kernel(const __grid_co
   const void* positions = s.positions;
   chain_begin(true, x, dy, w_at, b_at, positions);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = lane / LANES, l = lane % LANES, c0 = l * 8, D = s.D;
-  const bool mine = c0 < D;                  // (lanes behind the last channel have zeros)
-  T* const my_rows = rows + (XCHG ? (warp * GROUPS + group) * R * ROW : 0);
-  float2* const my_angles = angles + (warp * GROUPS + group) * ROW;
-  int at[RUN == 4 ? 2 : 8], pairs = 0;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = lane / LANES, l = lane % LANES, D = s.D;
+  const bool mine = l * 8 < D;                         // (lanes behind the last channel have zeros)
+  Place<RUN> place;
+  uint32_t alone = 0, axes = 0;                        // of the lane's pairs: whether they are not turned, their axes (a byte each)
+  auto pair = [&](int i) { return pair_of(s, mine ? 4 * l + i : i, positions != nullptr); };
 #pragma unroll
-  for (int i = 0; i < (RUN == 4 ? 2 : 8); ++i) at[i] = RUN == 0 ? 0 : partner_of(s, c0 + i * (RUN == 4 ? 4 : 1));
-  if (positions) {
-    int start = 0;
-    for (int a = 0; a < s.axes; ++a) {
-      const int half = s.band[a] >> 1;
-      for (int i = threadIdx.x; i < half; i += THREADS) {
-        const int lo = start + (RUN == 0 ? 2 * i : i), hi = lo + (RUN == 0 ? 1 : half);
-        turns[pairs + i] = s.turns[pairs + i];
-        places[pairs + i] = a << 16 | lo << 8 | hi;
-      }
-      pairs += half;
-      start += 2 * half;
-    }
+  for (int i = 0; i < 4; ++i) {
+    const Pair q = pair(i);
+    axes |= static_cast<uint32_t>(max(q.axis, 0)) << 8 * i;
+    if (q.axis < 0) alone |= 1u << i;
+    if constexpr (RUN == 1) place.at[i] = q.lo, place.at[4 + i] = q.hi;
   }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) my_angles[c0 + i] = make_float2(1.f, 0.f);
-  if constexpr (NORMED) {
-    for (int c = threadIdx.x; c < ROW; c += THREADS) {
-      params[0][c] = c < D ? (w_at ? w_at[c] : 1.f) : 0.f;
-      params[1][c] = c < D && b_at ? b_at[c] : 0.f;
-    }
+  if constexpr (RUN == 4) {      // (what is not turned: four channels, and four more)
+    place.at[0] = alone ? (mine ? 8 * l : 0) : pair(0).lo;
+    place.at[1] = alone ? 4 : pair(0).hi - pair(0).lo;
   }
-  __syncthreads();
-  // channels that are not turned have no partner (whatever it holds)
-  const int alone = 2 * pairs - c0;
-  auto turned = [&](f32x2 (&y)[4]) {
-    if (alone >= 8) return;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) y[i] = 2 * i < alone ? y[i] : 0ull;      // (bands are even)
+  if constexpr (RUN == 0) place.at[0] = mine ? 8 * l : 0;
+  const int offset = RUN == 1 ? 0 : place.at[0];
+  // channels of the pairs: first ones, then second ones
+  auto channel = [&](int i) {
+    if constexpr (RUN == 0) return place.at[0] + 2 * (i & 3) + (i >> 2);
+    else if constexpr (RUN == 4) return place.at[0] + (i & 3) + (i < 4 ? 0 : place.at[1]);
+    else return place.at[i];
   };
-  f32x2 w[4], dw[4], db[4];
-  if constexpr (SUMS) {
+  int rotated = 0;
+  if (positions)
+    for (int a = 0; a < s.axes; ++a) rotated += s.band[a];
+  const bool plain = rotated < D;
+  for (int i = threadIdx.x; i < ROW / 2; i += THREADS) turns[i] = 2 * i < rotated ? s.turns[i] : 0.0;
+  __syncthreads();
+  f32x2 w_lo[2], w_hi[2], b_lo[2], b_hi[2], dw_lo[2], dw_hi[2], db_lo[2], db_hi[2];
+  if constexpr (NORMED) {
+    float w[8], b[8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      w[i] = f2_pack(params[0][c0 + 2 * i], params[0][c0 + 2 * i + 1]);
-      dw[i] = db[i] = 0ull;
+    for (int i = 0; i < 8; ++i) {
+      w[i] = w_at ? w_at[channel(i)] : 1.f;
+      b[i] = b_at ? b_at[channel(i)] : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      w_lo[i] = f2_pack(w[2 * i], w[2 * i + 1]), w_hi[i] = f2_pack(w[4 + 2 * i], w[5 + 2 * i]);
+      b_lo[i] = f2_pack(b[2 * i], b[2 * i + 1]), b_hi[i] = f2_pack(b[4 + 2 * i], b[5 + 2 * i]);
+      dw_lo[i] = dw_hi[i] = db_lo[i] = db_hi[i] = 0ull;
     }
   }
-  const int limit = BACK && s.limit ? *s.limit : s.N;
+  const int limit = BACK && s.limit ? min(max(*s.limit, 0), s.N) : s.N;
   const float inv = 1.f / static_cast<float>(D);
-  const int chunks = p.chunks[which], per_chunk = (part.heads + chunks - 1) / chunks;
-  const unsigned units = static_cast<unsigned>(s.B) * s.N * chunks;      // (below 2^31)
+  const int chunks = p.chunks[which], per_chunk = part.heads / chunks;
+  const unsigned units = limit > 0 ? static_cast<unsigned>(s.B) * s.N * chunks : 0u;      // (below 2^31)
   const int block = which ? blockIdx.x - p.blocks0 : blockIdx.x, blocks = which ? p.blocks - p.blocks0 : p.blocks0;
   const unsigned step = static_cast<unsigned>(blocks) * WARPS * GROUPS;
   // (the groups of a warp go through the loop together)
   for (unsigned first = (static_cast<unsigned>(block) * WARPS + warp) * GROUPS; first < units; first += step) {
     const unsigned u = min(first + group, units - 1), t = chunks == 1 ? u : u / chunks;
-    const int chunk = static_cast<int>(u - t * chunks), bat = s.B == 1 ? 0 : static_cast<int>(t / s.N), n = static_cast<int>(t - static_cast<unsigned>(bat) * s.N);
-    const int h0 = chunk * per_chunk;
-    const int count = mine && first + group < units && (!BACK || n < limit) ? min(part.heads - h0, per_chunk) : 0;      // heads that this lane has a part of
-    const T* x_at = READ_X ? x + bat * part.x.batch + n * part.x.token + h0 * part.x.head + c0 : nullptr;
-    const T* d_at = BACK ? dy + bat * part.dy.batch + n * part.dy.token + h0 * part.dy.head + c0 : nullptr;
-    T* o_at = static_cast<T*>(part.out.ptr) + bat * part.out.batch + n * part.out.token + h0 * part.out.head + c0;
+    const int chunk = static_cast<int>(u - t * chunks), bat = s.B == 1 ? 0 : static_cast<int>(t / s.N);
+    const int n = static_cast<int>(t - static_cast<unsigned>(bat) * s.N), h0 = chunk * per_chunk;
+    // (a group behind the last unit or the limit goes along with zeros)
+    const bool live = mine && first + group < units && (!BACK || n < limit);
+    const T* x_at = READ_X ? x + bat * part.x.batch + n * part.x.token + h0 * part.x.head + offset : nullptr;
+    const T* d_at = BACK ? dy + bat * part.dy.batch + n * part.dy.token + h0 * part.dy.head + offset : nullptr;
+    T* o_at = static_cast<T*>(part.out.ptr) + bat * part.out.batch + n * part.out.token + h0 * part.out.head + offset;
 
-    Vec8<T> vx[READ_X ? R : 1], vd[BACK ? R : 1];
-#pragma unroll
-    for (int q = 0; q < R; ++q) {
-      if constexpr (READ_X) vx[q].clear();
-      if constexpr (BACK) vd[q].clear();
-    }
+    Channels<T, RUN> vx[READ_X ? R : 1], vd[BACK ? R : 1];
     auto fetch = [&](int k) {
 #pragma unroll
       for (int q = 0; q < R; ++q) {
-        const bool in = k + q < count;
+        const bool in = q == 0 || k + q < per_chunk;
         if constexpr (READ_X) {
-          if (in) vx[q].load(x_at);
+          if (in && live) vx[q].load(x_at, place);
           x_at += part.x.head;
         }
         if constexpr (BACK) {
-          if (in) vd[q].load(d_at);
-          else vd[q].clear();      // (they would be added to the sums)
+          if (q > 0 && !in) vd[q].raw.clear();      // (it would be added to the sums)
+          if (in && live) vd[q].load(d_at, place);
           d_at += part.dy.head;
         }
       }
     };
+#pragma unroll
+    for (int q = 0; q < R; ++q) {
+      if constexpr (READ_X) vx[q].raw.clear();
+      if constexpr (BACK) vd[q].raw.clear();
+    }
     fetch(0);
 
-    // angles of the token
-    if (positions) {
-      __syncwarp();
+    // angles of the lane's pairs
+    f32x2 cs[2], sn[2], neg[2];
+    {
+      float c[4], d[4];
       const long long from = bat * s.position_batch + 1ll * n * s.axes;
-      int place[4];
-      double turn[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {      // (at most half of a lane's eight channels)
-        const int i = l + j * LANES;
-        place[j] = i < pairs ? places[i] : 0;
-        turn[j] = i < pairs ? position_of(positions, s.position_type, from + (place[j] >> 16)) * turns[i] : 0.0;
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        float sine, cosine;
-        sine_cosine<T>(static_cast<float>(turn[j] - rint(turn[j])), sine, cosine);
-        if (BACK != (s.inverse != 0)) sine = -sine;
-        if (l + j * LANES < pairs) {
-          my_angles[place[j] >> 8 & 255] = make_float2(cosine, -sine);
-          my_angles[place[j] & 255] = make_float2(cosine, sine);
-        }
-      }
-      __syncwarp();
-    }
-    f32x2 cs[4], sn[4], add[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float4 a = *reinterpret_cast<const float4*>(my_angles + c0 + 2 * i);
-      cs[i] = f2_pack(a.x, a.z);
-      sn[i] = f2_pack(a.y, a.w);
-    }
-    // forward: out = rstd ((x - mean) (cos w) + (x' - mean) (sin w')) + (cos b + sin b')
-    if constexpr (NORMED && !BACK) {
+      double at = positions ? position_of(positions, s.position_type, from + (axes & 255)) : 0.0;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        auto mate = [&](int c) { return RUN == 0 ? (pairs > 0 ? c ^ 1 : c) : RUN == 4 ? at[(c - c0) / 4] + (c - c0) % 4 : at[c - c0]; };
-        const int c = c0 + 2 * i, m0 = mate(c), m1 = mate(c + 1);
-        add[i] = f2_fma(cs[i], f2_pack(params[1][c], params[1][c + 1]), f2_mul(sn[i], f2_pack(params[1][m0], params[1][m1])));
-        cs[i] = f2_mul(cs[i], f2_pack(params[0][c], params[0][c + 1]));
-        sn[i] = f2_mul(sn[i], f2_pack(params[0][m0], params[0][m1]));
+        c[i] = 1.f;
+        d[i] = 0.f;
+        if (positions) {
+          if (RUN != 4 && i > 0) at = position_of(positions, s.position_type, from + (axes >> 8 * i & 255));
+          const double v = at * turns[4 * l + i];
+          sine_cosine<T>(static_cast<float>(v - rint(v)), d[i], c[i]);
+          if (BACK != (s.inverse != 0)) d[i] = -d[i];
+        }
+      }
+      if (plain) {      // (whatever position there is)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          c[i] = alone >> i & 1 ? 1.f : c[i];
+          d[i] = alone >> i & 1 ? 0.f : d[i];
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        cs[i] = f2_pack(c[2 * i], c[2 * i + 1]);
+        sn[i] = f2_pack(d[2 * i], d[2 * i + 1]);
+        neg[i] = f2_pack(-d[2 * i], -d[2 * i + 1]);
       }
     }
 
     // (all groups of the warp make as many turns)
     for (int k = 0; k < per_chunk; k += R) {
-      Vec8<T> now[READ_X ? R : 1], now_d[BACK ? R : 1];
+      Channels<T, RUN> now[READ_X ? R : 1], now_d[BACK ? R : 1];
 #pragma unroll
       for (int q = 0; q < R; ++q) {
         if constexpr (READ_X) now[q] = vx[q];
         if constexpr (BACK) now_d[q] = vd[q];
       }
-      if constexpr (XCHG) {
-        __syncwarp();
-#pragma unroll
-        for (int q = 0; q < R; ++q) {
-          if constexpr (BACK) now_d[q].store(my_rows + q * ROW + c0);
-          else now[q].store(my_rows + q * ROW + c0);
-        }
-        __syncwarp();
-      }
       if (k + R < per_chunk) fetch(k + R);
-      auto put = [&](int q, const f32x2 (&v)[4]) {
-        if (k + q < count) rounded_pairs<T>(v).store(o_at);
+      auto put = [&](int q, const f32x2 (&lo)[2], const f32x2 (&hi)[2]) {
+        Channels<T, RUN> out;
+        out.set(lo, hi);
+        if (live && (q == 0 || k + q < per_chunk)) out.store(o_at, place);
         o_at += part.out.head;
       };
       if constexpr (!NORMED) {
 #pragma unroll
         for (int q = 0; q < R; ++q) {
-          f32x2 v[4], y[4];
-          if constexpr (BACK) pairs_of(now_d[q], v);
-          else pairs_of(now[q], v);
-          partners<T, RUN>(my_rows + q * ROW, at, v, y);
-          turned(y);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) v[i] = f2_fma(cs[i], v[i], f2_mul(sn[i], y[i]));
-          put(q, v);
+          f32x2 lo[2], hi[2];
+          if constexpr (BACK) now_d[q].get(lo, hi);
+          else now[q].get(lo, hi);
+          turn(lo, hi, cs, sn, neg, plain, alone);
+          put(q, lo, hi);
         }
       } else {
-        // Sums of a head: of the deviations from a value near the mean (that of its first eight channels: the variance loses little to their own mean) and of their
+        // Sums of a head: of the deviations from a value near the mean (that of the first lane's channels: the variance loses little to their own mean) and of their
         // squares; backward, of g w and its products with them
         constexpr int EACH = (LAYER ? 2 : 1) * (BACK ? 2 : 1);
-        f32x2 v[R][4], g[BACK ? R : 1][4];
-        float sums[R * EACH], pivot[R];
+        f32x2 lo[R][2], hi[R][2], g_lo[BACK ? R : 1][2], g_hi[BACK ? R : 1][2];
+        float sums[R * EACH];
 #pragma unroll
         for (int q = 0; q < R; ++q) {
-          pairs_of(now[q], v[q]);
+          now[q].get(lo[q], hi[q]);
           if constexpr (LAYER) {
-            pivot[q] = __shfl_sync(0xffffffffu, sum_of(v[q]) * 0.125f, lane & ~(LANES - 1));
-            const f32x2 off = f2_pack(mine ? -pivot[q] : 0.f, mine ? -pivot[q] : 0.f);
+            const float pivot = __shfl_sync(0xffffffffu, sum_of(lo[q], hi[q]) * 0.125f, lane & ~(LANES - 1));
+            const f32x2 off = both(mine ? -pivot : 0.f);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[q][i] = f2_add(v[q][i], off);
-          } else {
-            pivot[q] = 0.f;
+            for (int i = 0; i < 2; ++i) lo[q][i] = f2_add(lo[q][i], off), hi[q][i] = f2_add(hi[q][i], off);
+            sums[q * EACH + (BACK ? 2 : 1)] = sum_of(lo[q], hi[q]);
           }
+          sums[q * EACH] = sum_of_products(lo[q], hi[q], lo[q], hi[q]);
           if constexpr (BACK) {
-            f32x2 y[4];
-            pairs_of(now_d[q], g[q]);
-            partners<T, RUN>(my_rows + q * ROW, at, g[q], y);
-            turned(y);
+            now_d[q].get(g_lo[q], g_hi[q]);
+            turn(g_lo[q], g_hi[q], cs, sn, neg, plain, alone);
+            f32x2 e_lo[2], e_hi[2];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              g[q][i] = f2_fma(cs[i], g[q][i], f2_mul(sn[i], y[i]));
-              db[i] = f2_add(db[i], g[q][i]);
-              y[i] = f2_mul(g[q][i], w[i]);
+            for (int i = 0; i < 2; ++i) {
+              db_lo[i] = f2_add(db_lo[i], g_lo[q][i]), db_hi[i] = f2_add(db_hi[i], g_hi[q][i]);
+              e_lo[i] = f2_mul(g_lo[q][i], w_lo[i]), e_hi[i] = f2_mul(g_hi[q][i], w_hi[i]);
             }
-            sums[q * EACH + 1] = sum_of_products(y, v[q]);
-            if constexpr (LAYER) sums[q * EACH + 3] = sum_of(y);
+            sums[q * EACH + 1] = sum_of_products(e_lo, e_hi, lo[q], hi[q]);
+            if constexpr (LAYER) sums[q * EACH + 3] = sum_of(e_lo, e_hi);
           }
-          sums[q * EACH] = sum_of_products(v[q], v[q]);
-          if constexpr (LAYER) sums[q * EACH + (BACK ? 2 : 1)] = sum_of(v[q]);
         }
         group_sum<LANES>(sums);
 #pragma unroll
         for (int q = 0; q < R; ++q) {
           const float mean = LAYER ? sums[q * EACH + (BACK ? 2 : 1)] * inv : 0.f;      // of the deviations
           const float rstd = rsqrtf(fmaxf(fmaf(sums[q * EACH], inv, -mean * mean), 0.f) + s.eps);
-          const f32x2 r2 = f2_pack(rstd, rstd), m2 = f2_pack(-mean, -mean);
+          const f32x2 r2 = both(rstd), m2 = both(-mean);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            if (LAYER) lo[q][i] = f2_add(lo[q][i], m2), hi[q][i] = f2_add(hi[q][i], m2);
+            lo[q][i] = f2_mul(lo[q][i], r2), hi[q][i] = f2_mul(hi[q][i], r2);
+          }
           if constexpr (!BACK) {
-            f32x2 y[4], o[4];
-            if constexpr (RUN == 0) {
-              partners<T, RUN>(my_rows, at, v[q], y);
-            } else {
-              partners<T, RUN>(my_rows + q * ROW, at, v[q], y);
-              if constexpr (LAYER) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) y[i] = f2_add(y[i], f2_pack(-pivot[q], -pivot[q]));
-              }
-            }
-            turned(y);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              if constexpr (LAYER) o[i] = f2_fma(r2, f2_fma(cs[i], f2_add(v[q][i], m2), f2_mul(sn[i], f2_add(y[i], m2))), add[i]);
-              else o[i] = f2_fma(r2, f2_fma(cs[i], v[q][i], f2_mul(sn[i], y[i])), add[i]);
-            }
-            put(q, o);
+            for (int i = 0; i < 2; ++i) lo[q][i] = f2_fma(lo[q][i], w_lo[i], b_lo[i]), hi[q][i] = f2_fma(hi[q][i], w_hi[i], b_hi[i]);
+            turn(lo[q], hi[q], cs, sn, neg, plain, alone);
           } else {
             const float over = LAYER ? sums[q * EACH + 3] * inv : 0.f;                  // mean of g w
             const float along = rstd * fmaf(sums[q * EACH + 1], inv, -mean * over);     // and of g w xh
-            const f32x2 o2 = f2_pack(-over, -over), a2 = f2_pack(-along, -along);
-            f32x2 o[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const f32x2 xh = f2_mul(LAYER ? f2_add(v[q][i], m2) : v[q][i], r2);
-              dw[i] = f2_fma(g[q][i], xh, dw[i]);
-              f32x2 e = f2_mul(g[q][i], w[i]);
+            const f32x2 o2 = both(-over), a2 = both(-along);
+            auto slope = [&](f32x2 xh, f32x2 g, f32x2 w) {
+              f32x2 e = f2_mul(g, w);
               if (LAYER) e = f2_add(e, o2);
-              o[i] = f2_mul(f2_fma(xh, a2, e), r2);
+              return f2_mul(f2_fma(xh, a2, e), r2);
+            };
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              dw_lo[i] = f2_fma(g_lo[q][i], lo[q][i], dw_lo[i]), dw_hi[i] = f2_fma(g_hi[q][i], hi[q][i], dw_hi[i]);
+              lo[q][i] = slope(lo[q][i], g_lo[q][i], w_lo[i]), hi[q][i] = slope(hi[q][i], g_hi[q][i], w_hi[i]);
             }
-            put(q, o);
           }
+          put(q, lo[q], hi[q]);
         }
       }
     }
@@ -408,9 +412,9 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) rotary_kernel(const __grid_co
     __shared__ float cols[2][ROW];
     float fw[8], fb[8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      f2_unpack(dw[i], fw[2 * i], fw[2 * i + 1]);
-      f2_unpack(db[i], fb[2 * i], fb[2 * i + 1]);
+    for (int i = 0; i < 2; ++i) {
+      f2_unpack(dw_lo[i], fw[2 * i], fw[2 * i + 1]), f2_unpack(dw_hi[i], fw[4 + 2 * i], fw[5 + 2 * i]);
+      f2_unpack(db_lo[i], fb[2 * i], fb[2 * i + 1]), f2_unpack(db_hi[i], fb[4 + 2 * i], fb[5 + 2 * i]);
     }
 #pragma unroll
     for (int o = LANES; o < 32; o <<= 1)
@@ -423,8 +427,8 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) rotary_kernel(const __grid_co
       if (warp == k && group == 0 && mine) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          cols[0][c0 + i] = (k ? cols[0][c0 + i] : 0.f) + fw[i];
-          cols[1][c0 + i] = (k ? cols[1][c0 + i] : 0.f) + fb[i];
+          cols[0][channel(i)] = (k ? cols[0][channel(i)] : 0.f) + fw[i];
+          cols[1][channel(i)] = (k ? cols[1][channel(i)] : 0.f) + fb[i];
         }
       }
       __syncthreads();
@@ -459,8 +463,8 @@ __global__ void __launch_bounds__(1024) rotary_sums_kernel(const __grid_constant
 
 int lanes_of(int D) { return D <= 64 ? 8 : D <= 128 ? 16 : 32; }
 
-// Blocks and shares of heads.  A unit is a token with all of its heads, so that its angles are computed once; with fewer units than threads that the device holds,
-// heads are shared out, four at least to a unit.
+// Blocks and shares of heads.  A unit is a token with all heads of a part, so that its angles are computed once; with fewer units than threads that the device
+// holds, heads are shared out, four at least to a unit.
 constexpr int LEAST_HEADS = 4;
 constexpr int blocks_per_sm(int norm, bool back) { return norm == ROT_NORM_NONE ? 3 : back ? 2 : 3; }
 void plan(KernelParams& k, bool back) {
@@ -477,6 +481,7 @@ void plan(KernelParams& k, bool back) {
     const long long share = std::max<long long>(1, most * h / heads);        // blocks of this part in one wave
     const long long wanted = (share * per_block + tokens - 1) / tokens;
     k.chunks[i] = static_cast<int>(std::max<long long>(1, std::min<long long>(wanted, (h + LEAST_HEADS - 1) / LEAST_HEADS)));
+    while (h % k.chunks[i]) ++k.chunks[i];
     blocks[i] = std::min<long long>(share, (tokens * k.chunks[i] + per_block - 1) / per_block);
   }
   k.blocks0 = static_cast<int>(blocks[0]);
@@ -499,15 +504,12 @@ bool shape_ok(const RotShape& s, bool back) {
   return true;
 }
 
-// Channels that have their partners side by side: see `partners`
+// See `Place`.  Pairs of halves whose bands have a multiple of four of them lie in runs of four.
 int run_of(const RotShape& s) {
   if (!s.positions || s.interleaved) return 0;
-  int all = 0, at = 0;
-  for (int a = 0; a < s.axes; ++a) {
-    all |= at | (s.band[a] >> 1);
-    at += s.band[a];
-  }
-  return (all | at) % 4 == 0 ? 4 : 1;
+  for (int a = 0; a < s.axes; ++a)
+    if (s.band[a] % 8) return 1;
+  return 4;
 }
 
 template <typename T, int LANES, int NORM, bool BACK>
