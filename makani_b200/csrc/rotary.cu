@@ -466,7 +466,12 @@ int lanes_of(int D) { return D <= 64 ? 8 : D <= 128 ? 16 : 32; }
 // Blocks and shares of heads.  A unit is a token with all heads of a part, so that its angles are computed once; with fewer units than threads that the device
 // holds, heads are shared out, four at least to a unit.
 constexpr int LEAST_HEADS = 4;
-constexpr int blocks_per_sm(int norm, bool back) { return norm == ROT_NORM_NONE ? 3 : back ? 2 : 3; }
+// Blocks to an SM and heads at a time (bf16; half of them in fp32): what carries them is how many bytes are on their way.  us by (heads, blocks): rotation of 16200
+// tokens, 24 heads of 64, (4, 3) 20.7, (4, 4) 21.4, (2, 4) 20.8, (6, 2) 20.4, (2, 6) 40.6; with norms, 37080 tokens, 16 heads of 128, (4, 2) 61.4, (2, 3) 69.9,
+// (2, 4) 70.7, (1, 4) 73.1, (1, 5) 83.9, (2, 2) 73.8 (DRAM 46.5); their gradients (2, 2) 105, (1, 3) 128, (1, 2) 127, (2, 3), 508 bytes a thread spilled, 196
+// (DRAM 69.7).
+constexpr int blocks_per_sm(int norm, bool) { return norm == ROT_NORM_NONE ? 3 : 2; }
+constexpr int heads_at_a_time(int norm, bool back, bool half) { return (norm != ROT_NORM_NONE && back ? 2 : 4) / (half ? 1 : 2); }
 void plan(KernelParams& k, bool back) {
   const RotShape& s = k.s;
   const int per_block = WARPS * (32 / lanes_of(s.D));
@@ -514,7 +519,7 @@ int run_of(const RotShape& s) {
 
 template <typename T, int LANES, int NORM, bool BACK>
 cudaError_t by_run(const KernelParams& k, cudaStream_t s) {
-  constexpr int R = NORM == ROT_NORM_NONE ? (sizeof(T) == 2 ? 4 : 2) : (sizeof(T) == 2 ? 2 : 1), BLOCKS = blocks_per_sm(NORM, BACK);
+  constexpr int R = heads_at_a_time(NORM, BACK, sizeof(T) == 2), BLOCKS = blocks_per_sm(NORM, BACK);
   auto go = [&](auto* kernel) { return launch_chained(kernel, dim3(k.blocks), dim3(THREADS), 0, s, 1, true, k); };
   switch (run_of(k.s)) {
     case 0: return go(rotary_kernel<T, LANES, NORM, BACK, 0, R, BLOCKS>);
