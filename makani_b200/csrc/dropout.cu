@@ -17,6 +17,8 @@ namespace mk {
 namespace {
 
 constexpr int THREADS = 256;
+constexpr int LONG = 4;                    // vectors a thread from MANY elements on
+constexpr long long MANY = 1ll << 22;
 
 __device__ __forceinline__ void philox(uint64_t key, uint64_t number, uint64_t block, uint32_t (&w)[4]) {
   uint32_t c0 = static_cast<uint32_t>(number), c1 = static_cast<uint32_t>(number >> 32), c2 = static_cast<uint32_t>(block),
@@ -34,8 +36,9 @@ __device__ __forceinline__ void philox(uint64_t key, uint64_t number, uint64_t b
   w[0] = c0, w[1] = c1, w[2] = c2, w[3] = c3;
 }
 
-// VEC: whole vectors of eight; else one element after the other.  A thread has the eight elements of one vector.
-template <typename TX, typename TR, typename TO, bool VEC>
+// VEC: whole vectors of eight; else one element after the other.  A thread has the eight elements of each of TURNS vectors, a block's width apart, so that the
+// keys of the rounds are made once for them; their loads go out together.
+template <typename TX, typename TR, typename TO, bool VEC, int TURNS>
 __global__ void __launch_bounds__(THREADS) dropout_kernel(DropParams p) {
   constexpr bool ADD = !std::is_void<TR>::value;
   using Res = typename std::conditional<ADD, TR, TX>::type;
@@ -43,71 +46,84 @@ __global__ void __launch_bounds__(THREADS) dropout_kernel(DropParams p) {
   const Res* res = static_cast<const Res*>(p.r);
   const int64_t *key_at = p.source.key_at, *offset_at = p.source.offset_at;
   chain_begin(true, x, res, key_at, offset_at);
+  const long long begin = static_cast<long long>(blockIdx.x) * (TURNS * THREADS * 8) + threadIdx.x * 8;
+  Vec8<TX> a[TURNS];
+  Vec8<Res> r[ADD ? TURNS : 1];
+  if constexpr (VEC) {
+#pragma unroll
+    for (int t = 0; t < TURNS; ++t) {
+      const long long first = begin + t * (THREADS * 8);
+      if (first + 8 <= p.n) {
+        a[t].load(x + first);
+        if constexpr (ADD) r[t].load(res + first);
+      }
+    }
+  }
   const uint64_t key = key_at ? static_cast<uint64_t>(*key_at) : p.source.key;
   const uint64_t number = ((offset_at ? static_cast<uint64_t>(*offset_at) : 0ull) + p.source.more) >> p.source.shift;
-  const long long first = (static_cast<long long>(blockIdx.x) * THREADS + threadIdx.x) * 8;
-  if (first == 0 && p.source.kept) {
+  if (begin == 0 && p.source.kept) {
     p.source.kept[0] = static_cast<int64_t>(key);
     p.source.kept[1] = static_cast<int64_t>(number);
   }
-  if (first >= p.n) return;
-  const bool whole = VEC && first + 8 <= p.n;
-  const int count = static_cast<int>(p.n - first < 8 ? p.n - first : 8);
-  float v[8], r[8];
-  if (whole) {
-    Vec8<TX> a;
-    a.load(x + first);
-    if constexpr (ADD) {
-      Vec8<Res> b;
-      b.load(res + first);
-      b.get(r);
+#pragma unroll
+  for (int t = 0; t < TURNS; ++t) {
+    const long long first = begin + t * (THREADS * 8);
+    if (first >= p.n) return;
+    const bool whole = VEC && first + 8 <= p.n;
+    const int count = static_cast<int>(p.n - first < 8 ? p.n - first : 8);
+    float v[8], add[8];
+    if (whole) {
+      a[t].get(v);
+      if constexpr (ADD) r[t].get(add);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        v[i] = i < count ? value_of(x[first + i]) : 0.f;
+        if constexpr (ADD) add[i] = i < count ? value_of(res[first + i]) : 0.f;
+      }
     }
-    a.get(v);
-  } else {
+    const uint64_t block = static_cast<uint64_t>(first) >> 2;
+    uint32_t w[2][4];
+    philox(key, number, block, w[0]);
+    philox(key, number, block + 1, w[1]);
+    float out[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      v[i] = i < count ? value_of(x[first + i]) : 0.f;
-      if constexpr (ADD) r[i] = i < count ? value_of(res[first + i]) : 0.f;
+      const bool keep = w[i >> 2][i & 3] > p.last;
+      if constexpr (ADD) out[i] = keep ? fmaf(v[i], p.factor, add[i]) : add[i];
+      else out[i] = keep ? v[i] * p.factor : 0.f;
     }
-  }
-  const uint64_t block = static_cast<uint64_t>(first) >> 2;
-  uint32_t w[2][4];
-  philox(key, number, block, w[0]);
-  philox(key, number, block + 1, w[1]);
-  float out[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const bool keep = w[i >> 2][i & 3] > p.last;
-    if constexpr (ADD) out[i] = keep ? fmaf(v[i], p.factor, r[i]) : r[i];
-    else out[i] = keep ? v[i] * p.factor : 0.f;
-  }
-  TO* const to = static_cast<TO*>(p.out) + first;
-  __nv_bfloat16* const copy = p.copy ? static_cast<__nv_bfloat16*>(p.copy) + first : nullptr;
-  if (whole) {
-    Vec8<TO> o;
-    o.set(out);
-    o.store(to);
-    if (copy) {
-      Vec8<__nv_bfloat16> h;
-      h.set(v);
-      h.store(copy);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i < count) {
-        to[i] = rounded<TO>(out[i]);
-        if (copy) copy[i] = __float2bfloat16(v[i]);
+    TO* const to = static_cast<TO*>(p.out) + first;
+    __nv_bfloat16* const copy = p.copy ? static_cast<__nv_bfloat16*>(p.copy) + first : nullptr;
+    if (whole) {
+      Vec8<TO> o;
+      o.set(out);
+      o.store(to);
+      if (copy) {
+        Vec8<__nv_bfloat16> h;
+        h.set(v);
+        h.store(copy);
       }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i < count) {
+          to[i] = rounded<TO>(out[i]);
+          if (copy) copy[i] = __float2bfloat16(v[i]);
+        }
+    }
   }
 }
 
 template <typename TX, typename TR, typename TO>
 cudaError_t launch(const DropParams& p, bool vec, cudaStream_t s) {
-  const long long blocks = ((p.n + 7) / 8 + THREADS - 1) / THREADS;
-  if (blocks >= (1ll << 31)) return cudaErrorInvalidValue;
-  auto* kernel = vec ? dropout_kernel<TX, TR, TO, true> : dropout_kernel<TX, TR, TO, false>;
-  return launch_chained(kernel, dim3(static_cast<unsigned>(blocks)), dim3(THREADS), 0, s, 1, true, p);
+  auto go = [&](auto* kernel, int turns) {
+    const long long each = 8ll * THREADS * turns, blocks = (p.n + each - 1) / each;
+    if (blocks >= (1ll << 31)) return cudaErrorInvalidValue;
+    return launch_chained(kernel, dim3(static_cast<unsigned>(blocks)), dim3(THREADS), 0, s, 1, true, p);
+  };
+  if (!vec) return go(dropout_kernel<TX, TR, TO, false, 1>, 1);
+  return p.n >= MANY ? go(dropout_kernel<TX, TR, TO, true, LONG>, LONG) : go(dropout_kernel<TX, TR, TO, true, 1>, 1);
 }
 
 }  // namespace
