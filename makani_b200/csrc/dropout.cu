@@ -3,8 +3,11 @@
 //   out_i = keep_i x_i / (1 - p) (+ r_i),   keep_i = word_i >= p 2^32
 //
 // word_i is word i % 4 of the Philox4x32 generator with ten rounds (Salmon, Moraes, Dror and Shaw, 2011): a bijection of a 128-bit counter, here (number of the
-// call, i / 4) with 64 bits each, under a 64-bit key.  A round is two 32 x 32 bit products and four exclusive ors; 40 instructions or so for the words of four
-// elements.  All 32 bits are compared, so that p is met to 2^-32.  An element that is dropped is zero whatever x holds.
+// call, i / 4) with 64 bits each, under a 64-bit key.  A round is two 32 x 32 bit products and four exclusive ors.  All 32 bits are compared, so that p is met to
+// 2^-32.  An element that is dropped is zero whatever x holds.
+//
+// What bounds it: in bf16 the arithmetic pipes (a scheduler issues in 60 % of the cycles, and its warps mostly wait for a busy pipe): 16200 x 768 elements 16.8 us,
+// memory 7.6.  With fp32 beside it memory: 64800 x 768 with an fp32 residual, forward, 498 MB, in 74.8 us, 6.7 TB/s.
 #include "dropout.cuh"
 
 #include <type_traits>
@@ -17,24 +20,43 @@ namespace mk {
 namespace {
 
 constexpr int THREADS = 256;
-constexpr int LONG = 4;                    // vectors a thread from MANY elements on
+// Vectors a thread from MANY elements on.  us, bf16, 16200 x 768 elements and 64800 x 768 with an fp32 residual: one 19.5, 74.9; two 18.0, 95.8; four 16.7, 74.4;
+// eight 20.5, 104.  (4M elements: 8.0, two 7.5; 2M one 5.2.)
+constexpr int LONG = 4;
+static_assert((LONG & (LONG - 1)) == 0 && (THREADS & (THREADS - 1)) == 0);
 constexpr long long MANY = 1ll << 22;
 
-__device__ __forceinline__ void philox(uint64_t key, uint64_t number, uint64_t block, uint32_t (&w)[4]) {
-  uint32_t c0 = static_cast<uint32_t>(number), c1 = static_cast<uint32_t>(number >> 32), c2 = static_cast<uint32_t>(block),
-           c3 = static_cast<uint32_t>(block >> 32), k0 = static_cast<uint32_t>(key), k1 = static_cast<uint32_t>(key >> 32);
-#pragma unroll
-  for (int i = 0; i < 10; ++i) {
-    const uint64_t p0 = static_cast<uint64_t>(c0) * 0xD2511F53u, p1 = static_cast<uint64_t>(c2) * 0xCD9E8D57u;
-    c0 = static_cast<uint32_t>(p1 >> 32) ^ c1 ^ k0;
-    c1 = static_cast<uint32_t>(p1);
-    c2 = static_cast<uint32_t>(p0 >> 32) ^ c3 ^ k1;
-    c3 = static_cast<uint32_t>(p0);
-    k0 += 0x9E3779B9u;
-    k1 += 0xBB67AE85u;
+constexpr uint32_t M0 = 0xD2511F53u, M1 = 0xCD9E8D57u, W0 = 0x9E3779B9u, W1 = 0xBB67AE85u;
+__device__ __forceinline__ uint64_t wide(uint32_t a, uint32_t b) { return static_cast<uint64_t>(a) * b; }
+__device__ __forceinline__ uint32_t high(uint64_t v) { return static_cast<uint32_t>(v >> 32); }
+
+// The generator for the blocks i / 4 of a CTA: they differ in their lower 32 bits alone (a CTA's number of them is a power of two), so that one of two products of
+// the first round and of the second are the same for all.
+struct Generator {
+  uint32_t k0, k1, c1, c3a, c1b, high_b;
+  __device__ __forceinline__ Generator(uint64_t key, uint64_t number, uint32_t block_high)
+      : k0(static_cast<uint32_t>(key)), k1(high(key)), c1(high(number)) {
+    const uint64_t p0 = wide(static_cast<uint32_t>(number), M0);
+    c3a = static_cast<uint32_t>(p0);
+    const uint64_t p1 = wide(high(p0) ^ block_high ^ k1, M1);
+    c1b = static_cast<uint32_t>(p1);
+    high_b = high(p1);
   }
-  w[0] = c0, w[1] = c1, w[2] = c2, w[3] = c3;
-}
+  __device__ __forceinline__ void words(uint32_t block, uint32_t (&w)[4]) const {
+    const uint64_t a = wide(block, M1);                                                // first round
+    const uint64_t b = wide(high(a) ^ c1 ^ k0, M0);                                    // second
+    uint32_t c0 = high_b ^ static_cast<uint32_t>(a) ^ (k0 + W0), c_1 = c1b, c2 = high(b) ^ c3a ^ (k1 + W1), c3 = static_cast<uint32_t>(b);
+#pragma unroll
+    for (uint32_t i = 2; i < 10; ++i) {
+      const uint64_t p0 = wide(c0, M0), p1 = wide(c2, M1);
+      c0 = high(p1) ^ c_1 ^ (k0 + i * W0);
+      c_1 = static_cast<uint32_t>(p1);
+      c2 = high(p0) ^ c3 ^ (k1 + i * W1);
+      c3 = static_cast<uint32_t>(p0);
+    }
+    w[0] = c0, w[1] = c_1, w[2] = c2, w[3] = c3;
+  }
+};
 
 // VEC: whole vectors of eight; else one element after the other.  A thread has the eight elements of each of TURNS vectors, a block's width apart, so that the
 // keys of the rounds are made once for them; their loads go out together.
@@ -65,6 +87,7 @@ __global__ void __launch_bounds__(THREADS) dropout_kernel(DropParams p) {
     p.source.kept[0] = static_cast<int64_t>(key);
     p.source.kept[1] = static_cast<int64_t>(number);
   }
+  const Generator generator(key, number, static_cast<uint32_t>(static_cast<uint64_t>(begin) >> 34));
 #pragma unroll
   for (int t = 0; t < TURNS; ++t) {
     const long long first = begin + t * (THREADS * 8);
@@ -82,10 +105,10 @@ __global__ void __launch_bounds__(THREADS) dropout_kernel(DropParams p) {
         if constexpr (ADD) add[i] = i < count ? value_of(res[first + i]) : 0.f;
       }
     }
-    const uint64_t block = static_cast<uint64_t>(first) >> 2;
+    const uint32_t block = static_cast<uint32_t>(static_cast<uint64_t>(first) >> 2);
     uint32_t w[2][4];
-    philox(key, number, block, w[0]);
-    philox(key, number, block + 1, w[1]);
+    generator.words(block, w[0]);
+    generator.words(block + 1, w[1]);
     float out[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
