@@ -16,6 +16,7 @@ import torch.nn.functional as F
 from torch.utils.checkpoint import checkpoint
 
 from ...ops import conv as conv_ops
+from ...ops import dropout as dropout_ops
 from ...ops import linear as linear_ops
 
 
@@ -37,6 +38,29 @@ class DropPath(nn.Module):
 
     def forward(self, x):
         return drop_path(x, self.drop_prob, self.training)
+
+
+class Dropout(nn.Dropout):
+    """`nn.Dropout` on the kernel of `ops/dropout.py`, whose mask is made again in the backward pass instead of being kept (and is another than torch's)."""
+
+    def __init__(self, p: float = 0.5):
+        super().__init__(p)
+
+    def forward(self, x):
+        return dropout_ops.dropout(x, self.p, self.training)
+
+    def add(self, x, residual):
+        """residual + dropout(x), in one pass over memory."""
+        return dropout_ops.dropout_add(x, residual, self.p, self.training)
+
+
+def dropout_layer(p: float, generator: str = "torch") -> nn.Module:
+    """`generator` "torch": torch's dropout; "counter": the one above."""
+    if generator not in ("torch", "counter"):
+        raise ValueError(f"dropout generators are torch and counter, got {generator!r}")
+    if p <= 0.0:
+        return nn.Identity()
+    return Dropout(p) if generator == "counter" else nn.Dropout(p)
 
 
 class PatchEmbed(nn.Module):
@@ -93,7 +117,7 @@ class MLP(nn.Module):
     """fc1 -> act -> drop -> fc2 -> drop, pointwise over NCHW (1x1 convs) or the last dim ("traditional")."""
 
     def __init__(self, in_features, hidden_features=None, out_features=None, act_layer=nn.GELU, output_bias=True,
-                 input_format="nchw", drop_rate=0.0, drop_type="iid", checkpointing=0, gain=1.0, **kwargs):
+                 input_format="nchw", drop_rate=0.0, drop_type="iid", checkpointing=0, gain=1.0, dropout_generator="torch", **kwargs):
         super().__init__()
         self.checkpointing = checkpointing
         out_features = out_features or in_features
@@ -116,7 +140,7 @@ class MLP(nn.Module):
         if fc2.bias is not None:
             nn.init.constant_(fc2.bias, 0.0)
         if drop_rate > 0.0:
-            drop = nn.Dropout(drop_rate) if drop_type == "iid" else nn.Dropout2d(drop_rate)
+            drop = dropout_layer(drop_rate, dropout_generator) if drop_type == "iid" else nn.Dropout2d(drop_rate)
         else:
             drop = nn.Identity()
         self.fwd = nn.Sequential(fc1, act_layer(), drop, fc2, drop)
@@ -134,10 +158,15 @@ class MLP(nn.Module):
         """The forward pass with its activations recomputed in backward (makani/models/common/layers.py `MLP`)."""
         return checkpoint(self._run, x, use_reentrant=False)
 
-    def forward(self, x):
+    def forward(self, x, residual=None):
+        """The stack of x; with a residual, their sum, which takes the last dropout with it where that can."""
         if self.checkpointing >= 2 and self.training:
-            return self.checkpoint_forward(x)
-        return self._run(x)
+            y = self.checkpoint_forward(x)
+        elif residual is not None and isinstance(self.fwd[4], Dropout) and self.training:
+            return self.fwd[4].add(self.fwd[:4](x), residual)
+        else:
+            y = self._run(x)
+        return y if residual is None else residual + y
 
 
 class RealFFT2(nn.Module):

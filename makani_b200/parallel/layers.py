@@ -18,6 +18,7 @@ import torch.nn.functional as F
 from torch.utils.checkpoint import checkpoint
 
 from ..ops import attention as attn_ops
+from ..ops import rotary as rotary_ops
 from ..utils import comm
 from .helpers import compute_split_shapes
 from .layer_norm import LayerNorm, normed, operand_dtype
@@ -239,26 +240,38 @@ class DistributedMLP(nn.Module):
         return self.fwd(x)
 
 
-def attend_normed(qkv, num_heads, q_norm, k_norm, dropout_p=0.0):
-    """Self attention on the output of a fused projection, [B, N, (3, heads, head_dim)], queries and keys normalised per head on the way:
-    [B, N, heads, head_dim].  Dropped weights are left to the library."""
+def attend_normed(qkv, num_heads, q_norm, k_norm, dropout_p=0.0, positions=None, axes=None, window=None, sinks=0):
+    """Self attention on the output of a fused projection, [B, N, (3, heads, head_dim)], queries and keys normalised per head, and turned by their
+    `positions` (`ops/rotary.py`), on the way: [B, N, heads, head_dim]; `window` and `sinks` as in `ops/attention.py`.  Dropped weights are left to the library."""
     plain = isinstance(q_norm, nn.Identity) and isinstance(k_norm, nn.Identity)
-    if plain and dropout_p == 0.0:
-        return attn_ops.attention_qkv(qkv, num_heads)
+    if plain and dropout_p == 0.0 and positions is None:
+        return attn_ops.attention_qkv(qkv, num_heads, window=window, sinks=sinks)
+    if positions is not None and dropout_p == 0.0 and (plain or _one_pass(q_norm, k_norm, qkv.shape[-1] // (3 * num_heads))):
+        params = {} if plain else dict(q_weight=q_norm.weight, k_weight=k_norm.weight, q_bias=q_norm.bias, k_bias=k_norm.bias, eps=q_norm.eps, norm="layer")
+        return rotary_ops.rotary_attention_qkv(qkv, num_heads, None, positions, axes, window=window, sinks=sinks, **params)
     q, k, v = qkv.unflatten(-1, (3, num_heads, -1)).unbind(2)
     q, k = (t if isinstance(n, nn.Identity) else normed(n, t, operand_dtype(t)) for n, t in ((q_norm, q), (k_norm, k)))
+    if positions is not None:
+        q, k = rotary_ops.rotary_qk(q, k, positions, axes)
     if dropout_p == 0.0:
-        return attn_ops.attention(q, k, v)
-    return F.scaled_dot_product_attention(*(t.transpose(1, 2) for t in (q, k, v)), dropout_p=dropout_p).transpose(1, 2)
+        return attn_ops.attention(q, k, v, window=window, sinks=sinks)
+    seen = None if window is None else attn_ops.visible(q.shape[1], False, window, sinks, q.device)
+    return F.scaled_dot_product_attention(*(t.transpose(1, 2) for t in (q, k, v)), attn_mask=seen, dropout_p=dropout_p).transpose(1, 2)
+
+
+def _one_pass(q_norm, k_norm, head_dim) -> bool:
+    """Whether the norms of queries and keys are this package's, of a head's channels, and nobody has to see them called."""
+    return all(type(n) is LayerNorm and n.normalized_shape == (head_dim,) and n.plain() for n in (q_norm, k_norm)) and q_norm.eps == k_norm.eps
 
 
 class DistributedAttention(nn.Module):
     """Multi-head self attention with heads split over `comm_hidden_name` (sequence stays whole)."""
 
     def __init__(self, dim, input_format="traditional", comm_inp_name="fin", comm_hidden_name="fout", num_heads=8,
-                 qkv_bias=False, qk_norm=False, attn_drop_rate=0.0, proj_drop_rate=0.0, norm_layer=LayerNorm):
+                 qkv_bias=False, qk_norm=False, attn_drop_rate=0.0, proj_drop_rate=0.0, norm_layer=LayerNorm, axes=None, window=None, sinks=0):
         super().__init__()
         assert dim % num_heads == 0
+        self.axes, self.window, self.sinks = axes, window, sinks      # as of models/networks/vit.py: Attention
         assert num_heads % comm.get_size(comm_hidden_name) == 0, "heads must divide over the hidden group"
         self.num_heads = num_heads
         self.num_heads_local = num_heads // comm.get_size(comm_hidden_name)
@@ -278,11 +291,12 @@ class DistributedAttention(nn.Module):
             for prm in norm.parameters():
                 prm.is_shared_mp = []
 
-    def forward(self, x):
+    def forward(self, x, positions=None):
         B, N, C = x.shape
         # local rows of the qkv projection are ordered (q | k | v, local head, head_dim), as in makani/mpu/layers.py:507:
         # at one rank that is the serial layout, and a rank's rows are the q, k and v rows of its own heads
-        y = attend_normed(self.qkv(x), self.num_heads_local, self.q_norm, self.k_norm, self.attn_drop_rate if self.training else 0.0)
+        y = attend_normed(self.qkv(x), self.num_heads_local, self.q_norm, self.k_norm, self.attn_drop_rate if self.training else 0.0,
+                          positions, self.axes, self.window, self.sinks)
         return self.proj_drop(self.proj(y.reshape(B, N, self.num_heads_local * self.head_dim)))
 
 

@@ -1,0 +1,225 @@
+"""The token networks' options together: norms of queries and keys, rotary positions, windows with register tokens, dropout from a counter; as a user of the
+recipes has them."""
+
+import pytest
+import torch
+import torch.nn as nn
+
+from makani_b200.ops import _ext
+from makani_b200.ops import attention as attn
+from makani_b200.ops import rotary as rot
+
+
+def _rel(a, b):
+    return ((a.double() - b.double()).norm() / (b.double().norm() + 1e-30)).item()
+
+
+ALL = dict(qk_norm=True, rotary=True, attn_window=2, register_tokens=3)
+
+
+def _vit(dev, **kw):
+    from makani_b200.models.networks.vit import VisionTransformer
+    torch.manual_seed(3)
+    args = dict(inp_shape=(32, 64), patch_size=(4, 4), inp_chans=5, out_chans=3, embed_dim=96, depth=3, num_heads=4)
+    m = VisionTransformer(**{**args, **kw}).to(dev)
+    with torch.no_grad():
+        for p in m.parameters():
+            p.add_(0.02 * torch.randn_like(p))
+    return m
+
+
+# ---------------------------------------------------------------------------------------------------- any machine
+
+def test_attention_module_with_everything():
+    from makani_b200.models.networks.vit import Attention
+    torch.manual_seed(1)
+    axes, at = rot.RotaryAxes((2, 2), base=50.0), rot.grid_positions(3, 4, first=2)
+    m = Attention(24, num_heads=4, qkv_bias=True, qk_norm=True, axes=axes, window=4, sinks=2).eval()
+    x = torch.randn(2, 14, 24)
+    q, k, v = m.qkv(x).view(2, 14, 3, 4, 6).unbind(2)
+    q, k = rot.rotary(m.q_norm(q), at, axes), rot.rotary(m.k_norm(k), at, axes)
+    q, k, v = (t.transpose(1, 2) for t in (q, k, v))
+    s = (q @ k.mT / 6 ** 0.5).masked_fill(~attn.visible(14, False, 4, 2), float("-inf"))
+    want = m.proj((torch.softmax(s, -1) @ v).transpose(1, 2).reshape(2, 14, 24))
+    assert torch.allclose(m(x, at), want, atol=1e-5)
+    # a hook on a norm sees it called, with the same outcome
+    calls = []
+    m.q_norm.register_forward_hook(lambda *a: calls.append(1))
+    assert torch.allclose(m(x, at), want, atol=1e-5) and calls
+    # dropped weights go through the library, behind the same mask
+    m.attn_drop_rate = 1e-9
+    assert torch.allclose(m.train()(x, at), want, atol=1e-5)
+
+
+def test_networks_options_on_the_cpu():
+    plain = _vit("cpu")
+    assert not {n for n, _ in plain.named_parameters()} & {"registers", "blocks.0.attn.q_norm.weight"} and not list(plain.buffers())
+    m = _vit("cpu", **ALL)
+    assert m.registers.shape == (1, 3, 96) and m.token_positions.shape == (131, 2) and "token_positions" not in m.state_dict()
+    assert m.blocks[0].attn.window == 2 * 16 and m.blocks[0].attn.sinks == 3
+    y = m(torch.randn(2, 5, 32, 64))
+    assert y.shape == (2, 3, 32, 64)
+    y.sum().backward()
+    assert all(p.grad is not None for p in m.parameters())
+    assert _vit("cpu", attn_window=0)(torch.randn(1, 5, 32, 64)).shape == (1, 3, 32, 64)
+    for bad in (-1, 1.5, True):
+        with pytest.raises(ValueError, match="attn_window"):
+            _vit("cpu", attn_window=bad)
+    with pytest.raises(ValueError, match="narrow"):
+        _vit("cpu", rotary=True, num_heads=48)
+    with pytest.raises(ValueError, match="generators"):
+        _vit("cpu", mlp_drop_rate=0.1, dropout_generator="philox")
+
+
+def test_windows_keep_what_is_far_away():
+    """One block sees two rows to either side and the registers: a patch further away does not move."""
+    m = _vit("cpu", depth=1, attn_window=2, register_tokens=2).eval()
+    x = torch.randn(1, 5, 32, 64)
+    y = m(x)
+    x[:, :, 28:] += 1.0
+    z = m(x)
+    assert torch.equal(y[:, :, :16], z[:, :, :16]) and not torch.equal(y[:, :, 20:24], z[:, :, 20:24])
+
+
+def test_counter_dropout_on_the_cpu():
+    m = _vit("cpu", mlp_drop_rate=0.3, dropout_generator="counter")
+    x = torch.randn(1, 5, 32, 64)
+    assert torch.equal(m.eval()(x), _vit("cpu", mlp_drop_rate=0.3).eval()(x))
+    m.train()
+    torch.manual_seed(5)
+    a = m(x)
+    torch.manual_seed(5)
+    assert torch.equal(a, m(x)) and not torch.equal(a, m(x))
+
+
+@pytest.mark.parametrize("name", ["vit_73chq_window"])
+def test_recipe(name):
+    from makani_b200.utils.YParams import YParams
+    import os
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    p = YParams(os.path.join(root, "config", "vit.yaml"), name)
+    assert p.qk_norm and p.rotary and p.attn_window > 0 and p.register_tokens > 0 and p.dropout_generator == "counter"
+
+
+# ---------------------------------------------------------------------------------------------------- the kernels
+
+@pytest.fixture
+def dev():
+    if not torch.cuda.is_available():
+        pytest.skip("needs a GPU")
+    assert _ext.available()
+    yield torch.device("cuda", 0)
+    torch.cuda.synchronize()
+    _ext.check_device_errors()
+
+
+def _pass(m, x, dy, autocast, native):
+    _ext.set_native(native)
+    try:
+        m.zero_grad()
+        with torch.autocast("cuda", dtype=torch.bfloat16, enabled=autocast):
+            y = m(x)
+        y.backward(dy.to(y.dtype))
+        return y.detach().float(), {n: p.grad.detach().float().clone() for n, p in m.named_parameters()}
+    finally:
+        _ext.set_native(True)
+
+
+OPTIONS = [dict(qk_norm=True, rotary=True), dict(rotary=True, attn_window=2), dict(attn_window=1, register_tokens=4), ALL,
+           dict(ALL, embed_dim=256, num_heads=2, inp_shape=(64, 128))]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("options", OPTIONS)
+def test_networks_against_fp32(dev, options):
+    """Under autocast, the native pass is no further from the fp32 formulation than torch's own bf16 pass is, give or take a half."""
+    m = _vit(dev, **options)
+    g = torch.Generator(dev).manual_seed(5)
+    H, W = options.get("inp_shape", (32, 64))
+    x = torch.randn(2, 5, H, W, device=dev, generator=g)
+    dy = torch.randn(2, 3, H, W, device=dev, generator=g)
+    y0, g0 = _pass(m, x, dy, False, False)
+    y1, g1 = _pass(m, x, dy, True, False)
+    before = _ext.launch_count()
+    y2, g2 = _pass(m, x, dy, True, True)
+    assert _ext.launch_count() > before
+    assert _rel(y2, y0) < 1.5 * _rel(y1, y0) + 1e-3
+    for n in g0:
+        assert _rel(g2[n], g0[n]) < 1.5 * _rel(g1[n], g0[n]) + 1e-2, n
+
+
+@pytest.mark.gpu
+def test_no_library_attention_norm_or_dropout(dev, monkeypatch):
+    m = _vit(dev, **ALL, mlp_drop_rate=0.1, dropout_generator="counter")
+
+    def refuse(*a, **k):
+        raise AssertionError("library call")
+
+    for name in ("scaled_dot_product_attention", "layer_norm", "dropout"):
+        monkeypatch.setattr(torch.nn.functional, name, refuse)
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        y = m(torch.randn(1, 5, 32, 64, device=dev))
+    y.float().sum().backward()
+
+
+@pytest.mark.gpu
+def test_counter_dropout_has_one_mask_both_ways(dev):
+    """In fp32, a step along the gradient changes the output by what the gradient says, with the masks of one seed."""
+    m = _vit(dev, mlp_drop_rate=0.2, dropout_generator="counter", **ALL).train()
+    g = torch.Generator(dev).manual_seed(5)
+    x, dy = torch.randn(1, 5, 32, 64, device=dev, generator=g), torch.randn(1, 3, 32, 64, device=dev, generator=g)
+
+    def loss():
+        torch.manual_seed(8)
+        return (m(x).double() * dy.double()).sum()
+
+    value = loss()
+    value.backward()
+    assert torch.equal(value, loss())
+    grads = {n: p.grad.clone() for n, p in m.named_parameters()}
+    norm = sum(v.double().square().sum() for v in grads.values()).sqrt().item()
+    h, moved = 1e-2, []
+    for sign in (1, -1):
+        with torch.no_grad():
+            for n, p in m.named_parameters():
+                p.add_(sign * h / norm * grads[n])
+            moved.append(loss().item())
+            for n, p in m.named_parameters():
+                p.sub_(sign * h / norm * grads[n])
+    # (the third derivative leaves h^2 of the slope, fp32 some 1e-6 of the sum of 6144 terms over the difference)
+    assert abs((moved[0] - moved[1]) / (2 * h) - norm) < 2e-2 * norm
+
+
+@pytest.mark.gpu
+def test_captured_step_with_everything(dev):
+    """A training step in a CUDA graph: replays go on learning, with new masks each time, and the loss stays finite."""
+    m = _vit(dev, mlp_drop_rate=0.1, dropout_generator="counter", **ALL).train()
+    opt = torch.optim.SGD(m.parameters(), lr=1e-3)
+    x, t = torch.randn(1, 5, 32, 64, device=dev), torch.randn(1, 3, 32, 64, device=dev)
+
+    def step():
+        opt.zero_grad(set_to_none=False)
+        with torch.autocast("cuda", dtype=torch.bfloat16):
+            loss = (m(x).float() - t).square().mean()
+        loss.backward()
+        opt.step()
+        return loss.detach()
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(3):
+            step()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            loss = step()
+    torch.cuda.current_stream().wait_stream(side)
+    before = [p.detach().clone() for p in m.parameters()]
+    seen = []
+    for _ in range(4):
+        graph.replay()
+        torch.cuda.synchronize()
+        seen.append(loss.item())
+    assert all(torch.isfinite(torch.tensor(v)) for v in seen) and len(set(seen)) == 4
+    assert all(not torch.equal(a, p) for a, p in zip(before, m.parameters()))
