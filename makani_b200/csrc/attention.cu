@@ -266,7 +266,6 @@ struct TileParams {
   int D, DP;               // channels of a head, and rounded up to 16
   int group;               // heads of q that share one of k and v
   int causal;
-  int left, right, sinks;  // of a window (instances with WIN): right is 0 where causal
   float scale, scale_log2;
   int* err;
 };
@@ -276,14 +275,18 @@ struct TileParams {
 // Token i sees key j if i - left <= j <= i + right, or j < sinks (and j <= i where causal).  Tiles of keys outside are not visited: a tile of queries goes
 // over those of its window and those with sinks.  Instances of the kernels without WIN are what they are without windows.
 
+struct Window {
+  int causal, left, right, sinks;      // right is 0 where causal
+};
+
 // Tiles of keys that a CTA goes over, in order: `front` from `lo` on, those with sinks, and the rest of the window.  Of two query tiles the first sees
 // those up to end[0], and the second those from start on (its window begins a tile later), up to end[1]; what else one of them does not see it hides.
 struct KeyTiles {
   int lo = 0, front = 0, sinks = 0, start = 0, end[2] = {0, 0};
   __device__ __forceinline__ int operator()(int j) const { return j < front ? lo + j : j < front + sinks ? j - front : lo + j - sinks; }
 };
-__device__ __forceinline__ int last_seen(const TileParams& p, int i, int len) { return p.causal || i >= len ? min(i, len - 1) : p.right < len - 1 - i ? i + p.right : len - 1; }
-__device__ __forceinline__ KeyTiles key_tiles(const TileParams& p, int r0, int rows, int len) {
+__device__ __forceinline__ int last_seen(const Window& p, int i, int len) { return p.causal || i >= len ? min(i, len - 1) : p.right < len - 1 - i ? i + p.right : len - 1; }
+__device__ __forceinline__ KeyTiles key_tiles(const Window& p, int r0, int rows, int len) {
   KeyTiles k;
   if (rows <= 0) return k;
   const bool two = rows > TILE;
@@ -304,16 +307,21 @@ __device__ __forceinline__ KeyTiles key_tiles(const TileParams& p, int r0, int r
   return k;
 }
 __device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
+template <bool WIN, typename P>
+__device__ __forceinline__ KeyTiles window_keys(const P& p, const Work& w, int rows) {
+  if constexpr (WIN) return key_tiles(p.win, w.r0, w.padding ? 0 : rows, w.len);
+  else return KeyTiles();
+}
 // The keys from k0 on that token i sees, as columns: from `from` to `to`, and those below `sinks`
 struct SeenKeys {
   int from, to, sinks;
-  __device__ __forceinline__ SeenKeys(const TileParams& p, int i, int len, int k0)
+  __device__ __forceinline__ SeenKeys(const Window& p, int i, int len, int k0)
       : from(i - p.left - k0), to(last_seen(p, i, len) + 1 - k0), sinks(min(p.sinks, p.causal ? min(i + 1, len) : len) - k0) {}
   // of the 32 columns from c0 on
   __device__ __forceinline__ uint32_t bits(int c0) const { return (low_bits(to - c0) & ~low_bits(from - c0)) | low_bits(sinks - c0); }
 };
 // Whether every one of the 128 tokens from `first` on sees all 128 keys from k0 on
-__device__ __forceinline__ bool all_seen(const TileParams& p, int first, int len, int k0) {
+__device__ __forceinline__ bool all_seen(const Window& p, int first, int len, int k0) {
   if (k0 + TILE > len || (p.causal && k0 + TILE - 1 > first)) return false;
   return k0 + TILE <= p.sinks || (k0 >= first + TILE - 1 - p.left && k0 + TILE - 1 - first <= p.right);
 }
@@ -351,6 +359,39 @@ __device__ __forceinline__ void store_output(uint32_t taddr, int D, float f, __n
       for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) - __bfloat162float(__float2bfloat16(__uint_as_float(v[i]))));
       store16(v, rest + c, c + 8 < D);
     }
+  }
+}
+// Eight bf16 of eight fp32 values
+__device__ __forceinline__ uint4 pack8(const uint32_t* v) {
+  return make_uint4(pack_bf16(__uint_as_float(v[0]), __uint_as_float(v[1])), pack_bf16(__uint_as_float(v[2]), __uint_as_float(v[3])),
+                    pack_bf16(__uint_as_float(v[4]), __uint_as_float(v[5])), pack_bf16(__uint_as_float(v[6]), __uint_as_float(v[7])));
+}
+// The same through shared memory (`stage`: 32 rows of PITCH bytes), so that lanes side by side write what lies side by side.  `to`: of the warp's first row, `rows` of
+// which are here, `stride` elements apart.
+template <int PITCH>
+__device__ __forceinline__ void stage_output(uint32_t taddr, int D, float f, uint8_t* stage, __nv_bfloat16* to, __nv_bfloat16* rest, long long stride, int rows) {
+  const int lane = threadIdx.x & 31, chunks = D / 8;
+  const uint32_t by_chunks = 65536u / chunks + 1;      // i / chunks = i by_chunks >> 16 for i below 32 x 16
+  auto at = [&](int row, int c) { return reinterpret_cast<uint4*>(stage + row * PITCH + ((c ^ (row & 7)) << 4)); };
+  for (int pass = 0; pass < (rest ? 2 : 1); ++pass) {
+    for (int c = 0; c < D; c += 16) {
+      uint32_t v[16];
+      tmem_ld16(taddr + c, v);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float o = __uint_as_float(v[i]) * f;
+        v[i] = __float_as_uint(pass ? o - __bfloat162float(__float2bfloat16(o)) : o);
+      }
+      *at(lane, c / 8) = pack8(v);
+      if (c + 8 < D) *at(lane, c / 8 + 1) = pack8(v + 8);
+    }
+    __syncwarp();
+    __nv_bfloat16* const out = pass ? rest : to;
+    for (int i = lane; i < rows * chunks; i += 32) {
+      const int row = static_cast<int>(i * by_chunks >> 16), c = i - row * chunks;
+      *reinterpret_cast<uint4*>(out + row * stride + c * 8) = *at(row, c);
+    }
+    __syncwarp();
   }
 }
 // CTAs that are split over what they go along: those from `whole` on, into `parts`
@@ -434,15 +475,27 @@ struct Row {
   }
   // 128 scores -> weights 2^(scale S - m), as bf16 in the first half of them.  (A share of the exponentials on the FMA pipe, which helps the backward
   // pass, is slower here: 16200 tokens, 8 heads of 48: 750 us without, 860 - 930 with an eighth to three eighths of them.)
-  // `none`: 32 columns each whose weights are 0 without a look.
-  template <bool WIN>
-  __device__ __forceinline__ void weights(uint32_t (&v)[TILE], float scale, uint32_t none) {
+  __device__ __forceinline__ void weights(uint32_t (&v)[TILE], float scale) {
     // (a row that has seen nothing but -inf has no maximum yet, and weights of 0)
     const float from = m == -INFINITY ? 0.f : -m;
     const f32x2 scale2 = f2_pack(scale, scale), from2 = f2_pack(from, from);
 #pragma unroll
+    for (int c = 0; c < TILE; c += 2) {
+      float a, b;
+      f2_unpack(f2_fma(f2_pack(__uint_as_float(v[c]), __uint_as_float(v[c + 1])), scale2, from2), a, b);
+      a = ex2(a);
+      b = ex2(b);
+      sum[(c >> 1) & 1] = f2_add(sum[(c >> 1) & 1], f2_pack(a, b));
+      v[c / 2] = pack_bf16(a, b);
+    }
+  }
+  // The same; `none`: a bit for each 32 columns whose weights are 0 without a look
+  __device__ __forceinline__ void weights(uint32_t (&v)[TILE], float scale, uint32_t none) {
+    const float from = m == -INFINITY ? 0.f : -m;
+    const f32x2 scale2 = f2_pack(scale, scale), from2 = f2_pack(from, from);
+#pragma unroll
     for (int c0 = 0; c0 < TILE; c0 += 32) {
-      if (WIN && (none >> (c0 / 32) & 1)) {
+      if (none >> (c0 / 32) & 1) {
 #pragma unroll
         for (int c = 0; c < 16; ++c) v[c0 / 2 + c] = 0u;
         continue;
@@ -530,11 +583,19 @@ struct FwdParams {
   __nv_bfloat16 *o, *o_rest;
   float* lse;
 };
+// What a kernel has of `P`: with a window, that as well.  (In the parameters of all of them it makes the compiler arrange the registers of those without another
+// way: 16200 tokens, 8 heads of 48, 677 us instead of 643.)
+template <typename P>
+struct Windowed : P {
+  Window win;
+};
+template <typename P, bool WIN>
+using With = typename std::conditional<WIN, Windowed<P>, P>::type;
 
 template <int DB, int QT, bool WIN>
 __global__ void __launch_bounds__(Fwd<DB, QT>::THREADS_, 3 - QT)
 attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-                const FwdParams p) {
+                const With<FwdParams, WIN> p) {
   using L = Fwd<DB, QT>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = smem_u32(smem_raw);
@@ -588,8 +649,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     const int last = causal ? w.r0 + min(rows, (t + 1) * TILE) - 1 : w.len - 1;
     return last / TILE + 1;
   };
-  KeyTiles keys;
-  if constexpr (WIN) keys = key_tiles(p.t, w.r0, w.padding ? 0 : rows, w.len);
+  const KeyTiles keys = window_keys<WIN>(p, w, rows);
   int n0 = WIN ? keys.end[0] : tiles_of(0), n1 = WIN ? keys.end[1] : tiles_of(1);
   share.along(p.split, max(n0, n1));
   const int n = share.n, j0 = share.first;
@@ -597,7 +657,10 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     n0 = n0 > 0 ? n : 0;
     n1 = n1 > 0 ? n : 0;
   }
-  auto tile = [&](int j) { return WIN ? keys(j) : j0 + j; };
+  auto tile = [=](int j) {
+    if constexpr (WIN) return keys(j);
+    else return j0 + j;
+  };
   // keys of the last tile that belong to the sequence, where other tokens follow it
   const int tail = w.len - tile(n - 1) * TILE;
   const bool fix = n > 0 && tail < TILE && w.lo + w.len < p.t.grid.N;
@@ -672,7 +735,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         }
         tc_fence_after();
         for (int t = 0; t < 2 && ok; ++t) {
-          const int nt = t == 0 ? n0 : n1, start = t == 0 ? 0 : keys.start;
+          const int nt = t == 0 ? n0 : n1, start = !WIN || t == 0 ? 0 : keys.start;
           if (j >= nt) continue;
           if (WIN && j < start) {      // (the first is the next one)
             scores(t, sn);
@@ -716,7 +779,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     const bool here = row < rows;
     Row r;
     bool ok = true;
-    const int start = t == 0 ? 0 : keys.start;
+    const int start = !WIN || t == 0 ? 0 : keys.start;
     for (int j = start; j < nt; ++j) {
       ok = __all_sync(0xffffffffu, mbar_wait(s_full(t), (j - start) & 1));
       if (!ok) break;
@@ -724,9 +787,9 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       uint32_t v[TILE];
       load_scores(s_at, v);
       const int k0 = tile(j) * TILE;
-      uint32_t none = 0;
+      [[maybe_unused]] uint32_t none = 0;
       if constexpr (WIN) {
-        if (!all_seen(p.t, w.r0 + t * TILE, w.len, k0)) none = hide_scores(v, SeenKeys(p.t, w.r0 + row, w.len, k0));
+        if (!all_seen(p.win, w.r0 + t * TILE, w.len, k0)) none = hide_scores(v, SeenKeys(p.win, w.r0 + row, w.len, k0));
       } else if (k0 + TILE > w.len || (causal && k0 + TILE - 1 > w.r0 + t * TILE)) {
         hide_scores(v, (causal ? min(w.len, w.r0 + row + 1) : w.len) - k0);
       }
@@ -736,7 +799,8 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         const float f = r.grow(top);
         if (j > start) scale_row(o_at, p.t.DP, f);
       }
-      r.weights<WIN>(v, scale, none);
+      if constexpr (WIN) r.weights(v, scale, none);
+      else r.weights(v, scale);
       store_weights(s_at, v);
       tc_fence_before();
       __syncwarp();
@@ -754,7 +818,13 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         store_part(o_at, p.t.D, p.split.o + at * p.t.D, here);
         if (here) p.split.ml[at] = make_float2(r.m, total);
       } else {
-        store_output(o_at, p.t.D, 1.f / total, to, p.o_rest ? p.o_rest + (to - p.o) : nullptr, here);
+        if constexpr (WIN) {
+          __nv_bfloat16* const first = to - static_cast<long long>(lane) * p.t.grid.H * p.t.D;      // (the warp's first row)
+          stage_output<DB * 128>(o_at, p.t.D, 1.f / total, smem_raw + pad + t * L::TILE_BYTES + (warp & 3) * (L::TILE_BYTES / 4), first,
+                                 p.o_rest ? p.o_rest + (first - p.o) : nullptr, 1ll * p.t.grid.H * p.t.D, min(rows - row + lane, 32));
+        } else {
+          store_output(o_at, p.t.D, 1.f / total, to, p.o_rest ? p.o_rest + (to - p.o) : nullptr, here);
+        }
         if (here && p.lse)
           p.lse[(static_cast<long long>(w.b) * p.t.grid.H + w.h) * p.t.grid.N + w.lo + w.r0 + row] = r.m + __log2f(total);
       }
@@ -785,7 +855,7 @@ struct FwdNarrow {
 template <bool WIN>
 __global__ void __launch_bounds__(THREADS, 1)
 attn_fwd_narrow_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-                       const FwdParams p) {
+                       const With<FwdParams, WIN> p) {
   using L = FwdNarrow;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = smem_u32(smem_raw);
@@ -840,8 +910,7 @@ attn_fwd_narrow_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     const int last = causal ? w.r0 + min(rows, (t + 1) * TILE) - 1 : w.len - 1;
     return last / TILE + 1;
   };
-  KeyTiles keys;
-  if constexpr (WIN) keys = key_tiles(p.t, w.r0, w.padding ? 0 : rows, w.len);
+  const KeyTiles keys = window_keys<WIN>(p, w, rows);
   int n0 = WIN ? keys.end[0] : tiles_of(0), n1 = WIN ? keys.end[1] : tiles_of(1);
   share.along(p.split, max(n0, n1));
   const int n = share.n, j0 = share.first;
@@ -849,7 +918,10 @@ attn_fwd_narrow_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     n0 = n0 > 0 ? n : 0;
     n1 = n1 > 0 ? n : 0;
   }
-  auto tile = [&](int j) { return WIN ? keys(j) : j0 + j; };
+  auto tile = [=](int j) {
+    if constexpr (WIN) return keys(j);
+    else return j0 + j;
+  };
   const int tail = w.len - tile(n - 1) * TILE;
   const bool fix = n > 0 && tail < TILE && w.lo + w.len < p.t.grid.N;
 
@@ -885,7 +957,7 @@ attn_fwd_narrow_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     } else if (warp & 1) {
       // ---------------------------------------------------------------- products, a warp for either query tile
       if (n > 0 && elect_one()) {
-        const int t = warp >> 1, nt = t == 0 ? n0 : n1, start = t == 0 ? 0 : keys.start;
+        const int t = warp >> 1, nt = t == 0 ? n0 : n1, start = !WIN || t == 0 ? 0 : keys.start;
         const uint32_t hi = desc_hi(1024);
         const uint32_t q_lo = desc_lo(base + t * BOX, 16), k_lo = desc_lo(base + L::K_AT, 16), v_lo = desc_lo(base + L::V_AT, BOX);
         const uint32_t id_s = idesc_n(TILE), id_o = idesc_n(p.t.DP) | B_MN, o = tmem + L::O_AT + t * 64, a = tmem + L::P_AT + t * 64;
@@ -957,7 +1029,7 @@ attn_fwd_narrow_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     const bool here = row < rows;
     Row r;
     bool ok = true;
-    const int start = t == 0 ? 0 : keys.start;
+    const int start = !WIN || t == 0 ? 0 : keys.start;
     for (int j = start; j < nt; ++j) {
       ok = __all_sync(0xffffffffu, mbar_wait_soon(s_full(t), (j - start) & 1));
       if (!ok) break;
@@ -968,9 +1040,9 @@ attn_fwd_narrow_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
       __syncwarp();
       if (lane == 0) mbar_arrive(s_read(t));
       const int k0 = tile(j) * TILE;
-      uint32_t none = 0;
+      [[maybe_unused]] uint32_t none = 0;
       if constexpr (WIN) {
-        if (!all_seen(p.t, w.r0 + t * TILE, w.len, k0)) none = hide_scores(v, SeenKeys(p.t, w.r0 + row, w.len, k0));
+        if (!all_seen(p.win, w.r0 + t * TILE, w.len, k0)) none = hide_scores(v, SeenKeys(p.win, w.r0 + row, w.len, k0));
       } else if (k0 + TILE > w.len || (causal && k0 + TILE - 1 > w.r0 + t * TILE)) {
         hide_scores(v, (causal ? min(w.len, w.r0 + row + 1) : w.len) - k0);
       }
@@ -984,7 +1056,8 @@ attn_fwd_narrow_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
           scale_row(o_at, p.t.DP, f);
         }
       }
-      r.weights<WIN>(v, scale, none);
+      if constexpr (WIN) r.weights(v, scale, none);
+      else r.weights(v, scale);
       if (j > start) {
         ok = __all_sync(0xffffffffu, mbar_wait_soon(o_done(t), (j - start - 1) & 1));
         if (!ok) break;
@@ -1007,7 +1080,13 @@ attn_fwd_narrow_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         store_part(o_at, p.t.D, p.split.o + at * p.t.D, here);
         if (here) p.split.ml[at] = make_float2(r.m, total);
       } else {
-        store_output(o_at, p.t.D, 1.f / total, to, p.o_rest ? p.o_rest + (to - p.o) : nullptr, here);
+        if constexpr (WIN) {
+          __nv_bfloat16* const first = to - static_cast<long long>(lane) * p.t.grid.H * p.t.D;      // (the warp's first row)
+          stage_output<128>(o_at, p.t.D, 1.f / total, smem_raw + pad + t * BOX + (warp & 3) * (BOX / 4), first, p.o_rest ? p.o_rest + (first - p.o) : nullptr,
+                            1ll * p.t.grid.H * p.t.D, min(rows - row + lane, 32));
+        } else {
+          store_output(o_at, p.t.D, 1.f / total, to, p.o_rest ? p.o_rest + (to - p.o) : nullptr, here);
+        }
         if (here && p.lse) p.lse[(static_cast<long long>(w.b) * p.t.grid.H + w.h) * p.t.grid.N + w.lo + w.r0 + row] = r.m + __log2f(total);
       }
     } else if (here && w.padding) {
@@ -1118,7 +1197,7 @@ struct Dq {
   static constexpr int STAGES = DB == 1 ? 4 : 2, TILE_BYTES = DB * BOX;
   static constexpr int K_AT = 2 * TILE_BYTES, V_AT = K_AT + STAGES * TILE_BYTES, BAR_AT = V_AT + STAGES * TILE_BYTES;
   static constexpr int BARS = 4 * STAGES + 8;
-  static constexpr int SMEM = BAR_AT + 8 * BARS + 16 + 1024;
+  static constexpr int DELTA_AT = BAR_AT + (8 * BARS + 16 + 15) / 16 * 16, SMEM = DELTA_AT + 4 * TILE + 1024;
   static_assert(SMEM <= SMEM_LIMIT);
 };
 constexpr uint32_t DQ_DP = 256, DQ_ACC = 384;
@@ -1133,10 +1212,49 @@ struct DqParams {
   AttnTensor dq;
 };
 
+// delta of the rows of a tile, eight rows to a computing warp, into shared memory and p.delta.  A row is read by lanes side by side: by the thread that computes on it, a
+// warp's load touches 32 lines, and the four threads of a row read it four times: 12000 cycles, a quarter of what a CTA with 13 tiles of keys took.
+template <int DB>
+__device__ __forceinline__ void row_deltas(const DqParams& p, const Work& w, int rows, int warp, const __nv_bfloat16* out, const __nv_bfloat16* rest,
+                                           const __nv_bfloat16* d_out, float* deltas) {
+  constexpr int LANES = 8 * DB, AT_ONCE = 32 / LANES, TURNS = TILE / BWD_WARPS / AT_ONCE;
+  const int lane = threadIdx.x & 31, c = (lane % LANES) * 8;
+  const long long token = static_cast<long long>(w.b) * p.t.grid.N + w.lo + w.r0;
+  uint4 u[TURNS], r[TURNS], v[TURNS];
+#pragma unroll
+  for (int i = 0; i < TURNS; ++i) {
+    const int row = warp * (TILE / BWD_WARPS) + i * AT_ONCE + lane / LANES;
+    u[i] = r[i] = v[i] = make_uint4(0, 0, 0, 0);
+    if (row < rows && c < p.t.D) {
+      const long long at = ((token + row) * p.t.grid.H + w.h) * p.t.D + c;
+      u[i] = __ldg(reinterpret_cast<const uint4*>(out + at));
+      r[i] = __ldg(reinterpret_cast<const uint4*>(rest + at));
+      v[i] = __ldg(reinterpret_cast<const uint4*>(d_out + at));
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < TURNS; ++i) {
+    const uint32_t us[4] = {u[i].x, u[i].y, u[i].z, u[i].w}, rs[4] = {r[i].x, r[i].y, r[i].z, r[i].w}, vs[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+    float delta = 0.f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      delta = fmaf(__uint_as_float(us[k] << 16) + __uint_as_float(rs[k] << 16), __uint_as_float(vs[k] << 16), delta);
+      delta = fmaf(__uint_as_float(us[k] & 0xffff0000u) + __uint_as_float(rs[k] & 0xffff0000u), __uint_as_float(vs[k] & 0xffff0000u), delta);
+    }
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) delta += __shfl_xor_sync(0xffffffffu, delta, o);
+    const int row = warp * (TILE / BWD_WARPS) + i * AT_ONCE + lane / LANES;
+    if (row < rows && lane % LANES == 0) {
+      deltas[row] = delta;
+      p.delta[(static_cast<long long>(w.b) * p.t.grid.H + w.h) * p.t.grid.N + w.lo + w.r0 + row] = delta;
+    }
+  }
+}
+
 template <int DB, bool SPLIT, bool WIN>
 __global__ void __launch_bounds__(BWD_THREADS, 1)
 attn_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-               const __grid_constant__ CUtensorMap map_do, const DqParams p) {
+               const __grid_constant__ CUtensorMap map_do, const With<DqParams, WIN> p) {
   using L = Dq<DB>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = smem_u32(smem_raw);
@@ -1180,11 +1298,13 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
   const bool any = find_work(p.t.grid, offsets, share.unit, w);
   const int rows = any ? min(w.len - w.r0, TILE) : 0;
   const bool causal = p.t.causal != 0;
-  KeyTiles keys;
-  if constexpr (WIN) keys = key_tiles(p.t, w.r0, w.padding ? 0 : rows, w.len);
+  const KeyTiles keys = window_keys<WIN>(p, w, rows);
   share.along(p.split, WIN ? keys.end[0] : rows == 0 || w.padding ? 0 : (causal ? w.r0 + rows - 1 : w.len - 1) / TILE + 1);
   const int n = share.n, j0 = share.first;
-  auto tile = [&](int j) { return WIN ? keys(j) : j0 + j; };
+  auto tile = [=](int j) {
+    if constexpr (WIN) return keys(j);
+    else return j0 + j;
+  };
   const int tail = w.len - tile(n - 1) * TILE;
   const bool fix = n > 0 && tail < TILE && w.lo + w.len < p.t.grid.N;
 
@@ -1301,7 +1421,7 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
     if (here && n > 0) {
       l = __ldg(lse + stat);
       const long long at = (token * p.t.grid.H + w.h) * p.t.D;
-      for (int c = 0; c < p.t.D; c += 8) {
+      for (int c = 0; !WIN && c < p.t.D; c += 8) {
         const uint4 u = __ldg(reinterpret_cast<const uint4*>(out + at + c)), r = __ldg(reinterpret_cast<const uint4*>(rest + at + c)),
                     v = __ldg(reinterpret_cast<const uint4*>(d_out + at + c));
         const uint32_t us[4] = {u.x, u.y, u.z, u.w}, rs[4] = {r.x, r.y, r.z, r.w}, vs[4] = {v.x, v.y, v.z, v.w};
@@ -1311,7 +1431,13 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
           delta = fmaf(__uint_as_float(us[i] & 0xffff0000u) + __uint_as_float(rs[i] & 0xffff0000u), __uint_as_float(vs[i] & 0xffff0000u), delta);
         }
       }
-      if (x == 0) p.delta[stat] = delta;
+      if (!WIN && x == 0) p.delta[stat] = delta;
+    }
+    if constexpr (WIN) {
+      float* const deltas = reinterpret_cast<float*>(smem_raw + pad + L::DELTA_AT);
+      if (n > 0) row_deltas<DB>(p, w, rows, warp - COMPUTE_WARP, out, rest, d_out, deltas);
+      asm volatile("bar.sync 1, %0;" ::"n"(32 * BWD_WARPS) : "memory");
+      delta = here ? deltas[row] : 0.f;
     }
     const float scale = p.t.scale_log2;
     const f32x2 scale2 = f2_pack(scale, scale), l2 = f2_pack(-l, -l), delta2 = f2_pack(-delta, -delta);
@@ -1328,7 +1454,7 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
       const int below = (causal ? min(w.len, w.r0 + row + 1) : w.len) - k0;
       uint32_t bits = 0xffffffffu;
       if constexpr (WIN) {
-        bits = SeenKeys(p.t, w.r0 + row, w.len, k0).bits(0);
+        bits = SeenKeys(p.win, w.r0 + row, w.len, k0).bits(0);
         edge = !__all_sync(0xffffffffu, bits == 0xffffffffu);
         none = !__any_sync(0xffffffffu, bits != 0);
       }
@@ -1396,7 +1522,7 @@ struct SinkTiles {
 // Queries of `len` that see the keys r0 .. of a tile: tiles of them from `first` on
 struct QueryTiles {
   int first, n;
-  __device__ __forceinline__ QueryTiles(const TileParams& p, int r0, int rows, int len) {
+  __device__ __forceinline__ QueryTiles(const Window& p, int r0, int rows, int len) {
     const bool sinks = r0 < p.sinks;
     const int lo = p.causal ? r0 : sinks ? 0 : max(r0 - p.right, 0), key = r0 + rows - 1;
     const int hi = sinks || p.left >= len - 1 - key ? len - 1 : key + p.left;
@@ -1420,17 +1546,21 @@ __device__ __forceinline__ bool find_sinks(const Slots& g, const int* offsets, c
 struct DkvParams {
   TileParams t;
   Parts split;             // over the queries
-  SinkTiles sinks;
   float *dk_sums, *dv_sums;
   int heads_q;
   const float *lse, *delta;
   AttnTensor dk, dv;
 };
+struct DkvWindowParams : DkvParams {
+  SinkTiles sinks;
+};
+template <bool WIN>
+using DkvWith = typename std::conditional<WIN, Windowed<DkvWindowParams>, DkvParams>::type;
 
 template <int DB, bool SPLIT, bool WIN>
 __global__ void __launch_bounds__(BWD_THREADS, 1)
 attn_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-                const __grid_constant__ CUtensorMap map_do, const DkvParams p) {
+                const __grid_constant__ CUtensorMap map_do, const DkvWith<WIN> p) {
   using L = Dkv<DB>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = smem_u32(smem_raw);
@@ -1478,16 +1608,19 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     apart = blockIdx.x < first;
     if (!apart) share = ShareOf<SPLIT>(p.split, blockIdx.x - first);
     any = apart ? find_sinks(p.t.grid, offsets, p.sinks, blockIdx.x / p.sinks.parts, w) : find_work(p.t.grid, offsets, share.unit, w);
-    if (!apart && any && first > 0 && !w.padding && w.r0 < p.t.sinks) any = false;
+    if (!apart && any && first > 0 && !w.padding && w.r0 < p.win.sinks) any = false;
   } else {
     any = find_work(p.t.grid, offsets, share.unit, w);
   }
   const int rows = any ? min(w.len - w.r0, TILE) : 0;
   const bool causal = p.t.causal != 0;
   // tiles of queries, from the first that sees one of these keys, of one head after the other
-  const QueryTiles queries(p.t, w.r0, w.padding ? 0 : rows, w.len);
-  const int q_first = WIN ? queries.first : causal ? w.r0 / TILE : 0,
-            q_tiles = WIN ? queries.n : rows == 0 || w.padding ? 0 : (w.len + TILE - 1) / TILE - q_first;
+  int q_first = causal ? w.r0 / TILE : 0, q_tiles = rows == 0 || w.padding ? 0 : (w.len + TILE - 1) / TILE - q_first;
+  if constexpr (WIN) {
+    const QueryTiles queries(p.win, w.r0, w.padding ? 0 : rows, w.len);
+    q_first = queries.first;
+    q_tiles = queries.n;
+  }
   share.along(p.split, q_tiles * p.t.group);
   if constexpr (WIN && SPLIT) {
     if (apart) {
@@ -1685,9 +1818,9 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       bool none = false;
       if constexpr (WIN) {
         const int key = w.r0 + row;
-        if (key >= p.t.sinks) {
-          if (!causal) from = key - p.t.right - q0;
-          if (p.t.left < w.len - 1 - key) to = key + p.t.left + 1 - q0;
+        if (key >= p.win.sinks) {
+          if (!causal) from = key - p.win.right - q0;
+          if (p.win.left < w.len - 1 - key) to = key + p.win.left + 1 - q0;
         }
         bits = low_bits(to) & ~low_bits(from);
         edge = !__all_sync(0xffffffffu, bits == 0xffffffffu);
@@ -1788,7 +1921,7 @@ __global__ void __launch_bounds__(256) attn_sum_kernel(Slots grid, Parts split, 
 }
 
 // The same for tiles with sinks that went apart
-__global__ void __launch_bounds__(256) attn_sink_sum_kernel(TileParams t, SinkTiles s, Sums p) {
+__global__ void __launch_bounds__(256) attn_sink_sum_kernel(TileParams t, Window win, SinkTiles s, Sums p) {
   const float* parts = p.parts[blockIdx.y];
   const int* offsets = t.grid.offsets;
   chain_begin(true, parts, offsets);
@@ -1797,7 +1930,7 @@ __global__ void __launch_bounds__(256) attn_sink_sum_kernel(TileParams t, SinkTi
   const int row = static_cast<int>(at % TILE);
   Work w;
   if (!find_sinks(t.grid, offsets, s, unit, w) || w.r0 + row >= w.len || c >= t.D) return;
-  const int n = s.parts_of(QueryTiles(t, w.r0, min(w.len - w.r0, TILE), w.len).n * t.group);
+  const int n = s.parts_of(QueryTiles(win, w.r0, min(w.len - w.r0, TILE), w.len).n * t.group);
   float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int k = 0; k < n; ++k) {
     const float4 v = __ldcg(reinterpret_cast<const float4*>(parts + ((static_cast<long long>(unit) * s.parts + k) * TILE + row) * t.D + c));
@@ -1849,14 +1982,13 @@ TileParams tile_params(const AttnShape& p, const Slots& g, int* err) {
   t.DP = (p.D + 15) / 16 * 16;
   t.group = p.H / p.Hk;
   t.causal = p.causal;
-  t.left = p.left;
-  t.right = p.causal ? 0 : p.right;
-  t.sinks = p.window ? p.sinks : 0;
   t.scale = p.scale;
   t.scale_log2 = p.scale * LOG2E;
   t.err = err;
   return t;
 }
+
+Window window_of(const AttnShape& p) { return {p.causal, p.left, p.causal ? 0 : p.right, p.window ? p.sinks : 0}; }
 
 // One query tile to a CTA, two CTAs to an SM, where sequences are short and CTAs of two tiles would take the SMs more than once.  us, two tiles / one, heads of
 // 64 (batch x tokens x heads): 64 x 128 x 8 19.3 / 11.6, 64 x 200 x 8 32.7 / 27.9, 32 x 384 x 8 33.7 / 27.1, 16 x 512 x 8 23.4 / 22.5, 8 x 768 x 8 28.9 / 26.1, 8 x
@@ -1925,15 +2057,15 @@ SinkTiles sink_tiles(const AttnShape& p) {
 }
 long long sink_rows(const SinkTiles& s) { return 1ll * s.units * s.parts * TILE; }
 
-template <typename... Params>
-cudaError_t launch(void (*kernel)(Params...), std::atomic<uint64_t>& devices, int threads, int smem, const CUtensorMap& q, const CUtensorMap& k,
-                   const CUtensorMap& v, const FwdParams& p, cudaStream_t s) {
+template <typename Params>
+cudaError_t launch(void (*kernel)(CUtensorMap, CUtensorMap, CUtensorMap, Params), std::atomic<uint64_t>& devices, int threads, int smem, const CUtensorMap& q,
+                   const CUtensorMap& k, const CUtensorMap& v, const Params& p, cudaStream_t s) {
   const cudaError_t e = allow_shared_memory(devices, reinterpret_cast<const void*>(kernel), smem);
   if (e != cudaSuccess) return e;
   return launch_chained(kernel, dim3(static_cast<unsigned>(blocks_of(p.t.grid, p.split))), dim3(threads), smem, s, 1, true, q, k, v, p);
 }
 template <bool WIN>
-cudaError_t launch_fwd(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const FwdParams& p, bool one_tile, cudaStream_t s) {
+cudaError_t launch_fwd(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const With<FwdParams, WIN>& p, bool one_tile, cudaStream_t s) {
   static std::atomic<uint64_t> devices[4];
   if (one_tile) {
     if (p.t.D <= 64) return launch(attn_fwd_kernel<1, 1, WIN>, devices[0], Fwd<1, 1>::THREADS_, Fwd<1, 1>::SMEM, q, k, v, p, s);
@@ -1943,7 +2075,7 @@ cudaError_t launch_fwd(const CUtensorMap& q, const CUtensorMap& k, const CUtenso
   return launch(attn_fwd_kernel<2, 2, WIN>, devices[3], Fwd<2, 2>::THREADS_, Fwd<2, 2>::SMEM, q, k, v, p, s);
 }
 template <int DB, bool SPLIT, bool WIN>
-cudaError_t launch_dq(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& g, const DqParams& p, cudaStream_t s) {
+cudaError_t launch_dq(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& g, const With<DqParams, WIN>& p, cudaStream_t s) {
   static std::atomic<uint64_t> devices;
   const cudaError_t e = allow_shared_memory(devices, reinterpret_cast<const void*>(&attn_dq_kernel<DB, SPLIT, WIN>), Dq<DB>::SMEM);
   if (e != cudaSuccess) return e;
@@ -1951,20 +2083,22 @@ cudaError_t launch_dq(const CUtensorMap& q, const CUtensorMap& k, const CUtensor
                         q, k, v, g, p);
 }
 template <int DB, bool SPLIT, bool WIN>
-cudaError_t launch_dkv(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& g, const DkvParams& p, cudaStream_t s) {
+cudaError_t launch_dkv(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& g, const DkvWith<WIN>& p, cudaStream_t s) {
   static std::atomic<uint64_t> devices;
   const cudaError_t e = allow_shared_memory(devices, reinterpret_cast<const void*>(&attn_dkv_kernel<DB, SPLIT, WIN>), Dkv<DB>::SMEM);
   if (e != cudaSuccess) return e;
-  const long long blocks = blocks_of(p.t.grid, p.split) + 1ll * p.sinks.units * p.sinks.parts;
+  long long blocks = blocks_of(p.t.grid, p.split);
+  if constexpr (WIN) blocks += 1ll * p.sinks.units * p.sinks.parts;
   return launch_chained(attn_dkv_kernel<DB, SPLIT, WIN>, dim3(static_cast<unsigned>(blocks)), dim3(BWD_THREADS), Dkv<DB>::SMEM, s, 1, true, q, k, v, g, p);
 }
 template <int DB>
-cudaError_t launch_dq(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& g, const DqParams& p, bool window, cudaStream_t s) {
+cudaError_t launch_dq(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& g, const Windowed<DqParams>& p, bool window,
+                      cudaStream_t s) {
   if (window) return launch_dq<DB, false, true>(q, k, v, g, p, s);
   return p.split.parts > 0 ? launch_dq<DB, true, false>(q, k, v, g, p, s) : launch_dq<DB, false, false>(q, k, v, g, p, s);
 }
 template <int DB>
-cudaError_t launch_dkv(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& g, const DkvParams& p, bool window,
+cudaError_t launch_dkv(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& g, const DkvWith<true>& p, bool window,
                        cudaStream_t s) {
   const bool split = p.split.parts > 0 || p.sinks.parts > 0;
   if (window) return split ? launch_dkv<DB, true, true>(q, k, v, g, p, s) : launch_dkv<DB, false, true>(q, k, v, g, p, s);
@@ -1985,7 +2119,7 @@ cudaError_t attention_fwd(const AttnShape& p, const AttnTensor& q, const AttnTen
   bind_context(s);
   CUtensorMap mq, mk_, mv;
   if (!map_of(&mq, q, p, p.H) || !map_of(&mk_, k, p, p.Hk) || !map_of(&mv, v, p, p.Hk)) return cudaErrorInvalidValue;
-  FwdParams f;
+  Windowed<FwdParams> f;
   const bool one_tile = one_tile_pays(p);
   f.t = tile_params(p, slots_of(p, p.H, one_tile ? TILE : 2 * TILE, 1), err);
   static_cast<Parts&>(f.split) = scratch ? forward_parts(p) : Parts{0, 0};
@@ -1995,11 +2129,12 @@ cudaError_t attention_fwd(const AttnShape& p, const AttnTensor& q, const AttnTen
   f.o = o;
   f.o_rest = o_rest;
   f.lse = lse;
+  f.win = window_of(p);
   *launches = 1;
   const cudaError_t e = p.window ? launch_fwd<true>(mq, mk_, mv, f, one_tile, s) : launch_fwd<false>(mq, mk_, mv, f, one_tile, s);
   if (e != cudaSuccess || f.split.parts == 0) return e;
   ++*launches;
-  return launch_chained(attn_join_kernel, dim3(static_cast<unsigned>(rows / f.split.parts / 8)), dim3(256), 0, s, 1, true, f);
+  return launch_chained(attn_join_kernel, dim3(static_cast<unsigned>(rows / f.split.parts / 8)), dim3(256), 0, s, 1, true, static_cast<const FwdParams&>(f));
 }
 
 long long attention_bwd_scratch(const AttnShape& p) {
@@ -2020,7 +2155,7 @@ cudaError_t attention_bwd(const AttnShape& p, const AttnTensor& q, const AttnTen
   const AttnTensor g{const_cast<__nv_bfloat16*>(d_o), 1ll * p.H * p.D, p.D, 1ll * p.N * p.H * p.D};
   CUtensorMap mq, mk_, mv, mg;
   if (!map_of(&mq, q, p, p.H) || !map_of(&mk_, k, p, p.Hk) || !map_of(&mv, v, p, p.Hk) || !map_of(&mg, g, p, p.H)) return cudaErrorInvalidValue;
-  DqParams a;
+  Windowed<DqParams> a;
   a.t = tile_params(p, slots_of(p, p.H, TILE, 1), err);
   a.o = o;
   a.o_rest = o_rest;
@@ -2028,13 +2163,15 @@ cudaError_t attention_bwd(const AttnShape& p, const AttnTensor& q, const AttnTen
   a.lse = lse;
   a.delta = delta;
   a.dq = dq;
-  DkvParams b;
+  a.win = window_of(p);
+  DkvWith<true> b;
   b.t = tile_params(p, slots_of(p, p.Hk, TILE, 2), err);
   b.heads_q = p.H;
   b.lse = lse;
   b.delta = delta;
   b.dk = dk;
   b.dv = dv;
+  b.win = a.win;
   a.split = scratch ? query_parts(p, a.t.grid) : Parts{0, 0};
   a.sums = scratch;
   b.sinks = scratch ? sink_tiles(p) : SinkTiles{0, 1, 0};
@@ -2057,7 +2194,7 @@ cudaError_t attention_bwd(const AttnShape& p, const AttnTensor& q, const AttnTen
   const Sums sums{{b.dv_sums, b.dk_sums}, {dv, dk}, {1.f, p.scale}};
   if (e == cudaSuccess && b.sinks.parts > 0) {
     ++*launches;
-    e = launch_chained(attn_sink_sum_kernel, dim3(static_cast<unsigned>(b.sinks.units * (TILE / 8)), 2), dim3(256), 0, s, 1, true, b.t, b.sinks, sums);
+    e = launch_chained(attn_sink_sum_kernel, dim3(static_cast<unsigned>(b.sinks.units * (TILE / 8)), 2), dim3(256), 0, s, 1, true, b.t, b.win, b.sinks, sums);
   }
   if (e == cudaSuccess && rows_k > 0) {
     ++*launches;
