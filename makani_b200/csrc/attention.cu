@@ -787,20 +787,32 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       uint32_t v[TILE];
       load_scores(s_at, v);
       const int k0 = tile(j) * TILE;
-      [[maybe_unused]] uint32_t none = 0;
+      auto grow = [&] {
+        const float top = max_of<false>(v) * scale;
+        if (__any_sync(0xffffffffu, r.grows(top))) {
+          // (the scores of tile j are behind the products of tile j - 1: O is complete up to there)
+          const float f = r.grow(top);
+          if (j > start) scale_row(o_at, p.t.DP, f);
+        }
+      };
       if constexpr (WIN) {
-        if (!all_seen(p.win, w.r0 + t * TILE, w.len, k0)) none = hide_scores(v, SeenKeys(p.win, w.r0 + row, w.len, k0));
-      } else if (k0 + TILE > w.len || (causal && k0 + TILE - 1 > w.r0 + t * TILE)) {
-        hide_scores(v, (causal ? min(w.len, w.r0 + row + 1) : w.len) - k0);
+        // (two ways from here on: on one for whole tiles and others, 16128 tokens, 8 heads of 48 with a window over nearly all took 925 us where there are 720 without it
+        // and 791 like this)
+        if (all_seen(p.win, w.r0 + t * TILE, w.len, k0)) {
+          apart<false>();
+          grow();
+          r.weights(v, scale);
+        } else {
+          apart<true>();
+          const uint32_t none = hide_scores(v, SeenKeys(p.win, w.r0 + row, w.len, k0));
+          grow();
+          r.weights(v, scale, none);
+        }
+      } else {
+        if (k0 + TILE > w.len || (causal && k0 + TILE - 1 > w.r0 + t * TILE)) hide_scores(v, (causal ? min(w.len, w.r0 + row + 1) : w.len) - k0);
+        grow();
+        r.weights(v, scale);
       }
-      const float top = max_of<false>(v) * scale;
-      if (__any_sync(0xffffffffu, r.grows(top))) {
-        // (the scores of tile j are behind the products of tile j - 1: O is complete up to there)
-        const float f = r.grow(top);
-        if (j > start) scale_row(o_at, p.t.DP, f);
-      }
-      if constexpr (WIN) r.weights(v, scale, none);
-      else r.weights(v, scale);
       store_weights(s_at, v);
       tc_fence_before();
       __syncwarp();
@@ -1040,24 +1052,36 @@ attn_fwd_narrow_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
       __syncwarp();
       if (lane == 0) mbar_arrive(s_read(t));
       const int k0 = tile(j) * TILE;
-      [[maybe_unused]] uint32_t none = 0;
-      if constexpr (WIN) {
-        if (!all_seen(p.win, w.r0 + t * TILE, w.len, k0)) none = hide_scores(v, SeenKeys(p.win, w.r0 + row, w.len, k0));
-      } else if (k0 + TILE > w.len || (causal && k0 + TILE - 1 > w.r0 + t * TILE)) {
-        hide_scores(v, (causal ? min(w.len, w.r0 + row + 1) : w.len) - k0);
-      }
-      const float top = max_of<true>(v) * scale;
-      if (__any_sync(0xffffffffu, r.grows(top))) {
-        const float f = r.grow(top);
-        if (j > start) {
-          ok = __all_sync(0xffffffffu, mbar_wait(o_done(t), (j - start - 1) & 1));
-          if (!ok) break;
-          tc_fence_after();
-          scale_row(o_at, p.t.DP, f);
+      auto grow = [&] {
+        const float top = max_of<true>(v) * scale;
+        if (__any_sync(0xffffffffu, r.grows(top))) {
+          const float f = r.grow(top);
+          if (j > start) {
+            ok = __all_sync(0xffffffffu, mbar_wait(o_done(t), (j - start - 1) & 1));
+            if (!ok) return;
+            tc_fence_after();
+            scale_row(o_at, p.t.DP, f);
+          }
         }
+      };
+      if constexpr (WIN) {
+        // (two ways from here on, as above)
+        if (all_seen(p.win, w.r0 + t * TILE, w.len, k0)) {
+          apart<false>();
+          grow();
+          r.weights(v, scale);
+        } else {
+          apart<true>();
+          const uint32_t none = hide_scores(v, SeenKeys(p.win, w.r0 + row, w.len, k0));
+          grow();
+          r.weights(v, scale, none);
+        }
+      } else {
+        if (k0 + TILE > w.len || (causal && k0 + TILE - 1 > w.r0 + t * TILE)) hide_scores(v, (causal ? min(w.len, w.r0 + row + 1) : w.len) - k0);
+        grow();
+        r.weights(v, scale);
       }
-      if constexpr (WIN) r.weights(v, scale, none);
-      else r.weights(v, scale);
+      if (!ok) break;
       if (j > start) {
         ok = __all_sync(0xffffffffu, mbar_wait_soon(o_done(t), (j - start - 1) & 1));
         if (!ok) break;
@@ -2001,10 +2025,14 @@ int window_tiles(const AttnShape& p) {
   const long long span = 1ll * p.left + (p.causal ? 0 : p.right) + TILE;
   return static_cast<int>(std::min<long long>((span + TILE - 1) / TILE + 1, (mean_length(p) + TILE - 1) / TILE));
 }
+// Through a window: up to 17 tiles, where start and end of a CTA are a quarter of it, and where CTAs of two tiles would leave SMs idle.  16128 tokens, 8 heads of 48, by
+// tokens to either side, two tiles / one: 192 58 / 57, 704 115 / 113, 960 143 / 140, 1472 195 / 195, 3008 342 / 339, 4000 380 / 396; of 128 704 150 / 144, 960 180 / 177, 1472
+// 238 / 240, 3008 402 / 430; 1 head of 64 300 20.5 / 18.0, 2000 63 / 56, 8000 206 / 188; 4000 tokens, 4 of 64 500 24.2 / 21.4.
+constexpr int ONE_TILE_WINDOW = 17;
 bool one_tile_pays(const AttnShape& p) {
-  if (p.window) if (const char* e = getenv("MK_QT")) return e[0] == 49;
-  const int mean = p.window ? std::min(mean_length(p), window_tiles(p) * TILE) : mean_length(p);
-  return mean <= (p.D <= 64 ? 768 : 448) && blocks_of(slots_of(p, p.H, 2 * TILE, 1)) > sm_count();
+  const bool idle = blocks_of(slots_of(p, p.H, 2 * TILE, 1)) <= sm_count();
+  if (p.window) return idle || window_tiles(p) <= ONE_TILE_WINDOW;
+  return mean_length(p) <= (p.D <= 64 ? 768 : 448) && !idle;
 }
 // CTAs of one length that would be a last wave of their own, or that are fewer than the SMs, are split over the keys so that they fill them, where that saves more
 // than joining them costs: tiles of keys, of some 0.7 us.  us, whole / split: 16200 tokens, 8 heads of 48 720 / 641, 12 of 64 1086 / 955, 8 of 128 943 / 847; 5000
