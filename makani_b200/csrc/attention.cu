@@ -320,10 +320,24 @@ struct SeenKeys {
   // of the 32 columns from c0 on
   __device__ __forceinline__ uint32_t bits(int c0) const { return (low_bits(to - c0) & ~low_bits(from - c0)) | low_bits(sinks - c0); }
 };
-// Whether every one of the 128 tokens from `first` on sees all 128 keys from k0 on
-__device__ __forceinline__ bool all_seen(const Window& p, int first, int len, int k0) {
-  if (k0 + TILE > len || (p.causal && k0 + TILE - 1 > first)) return false;
-  return k0 + TILE <= p.sinks || (k0 >= first + TILE - 1 - p.left && k0 + TILE - 1 - first <= p.right);
+// Tiles of a CTA's list that are seen as a whole, as a range (tiles with sinks count for none: they may always be looked at)
+struct Whole {
+  int from = 0;
+  uint32_t n = 0;
+  __device__ __forceinline__ bool operator()(int j) const { return static_cast<uint32_t>(j - from) < n; }
+};
+__device__ __forceinline__ int tiles_over(int n) { return n <= 0 ? 0 : (n + TILE - 1) / TILE; }
+// Of keys, by each of the 128 tokens from `first` on
+__device__ __forceinline__ Whole whole_keys(const Window& p, const KeyTiles& k, int first, int len) {
+  const int from = max(tiles_over(first + TILE - 1 - p.left) - k.lo, k.front), to = (last_seen(p, first, len) + 1) / TILE - k.lo;
+  return {from + k.sinks, static_cast<uint32_t>(max(to - from, 0))};
+}
+// Of queries, by which all 128 keys from r0 on are seen: tiles behind `first`
+__device__ __forceinline__ Whole whole_queries(const Window& p, int r0, int len, int first) {
+  const bool sinks = r0 + TILE <= p.sinks;
+  const int from = max(sinks && !p.causal ? 0 : tiles_over(r0 + TILE - 1 - p.right), first);
+  const int to = sinks || p.left >= len - 1 - r0 ? len / TILE : (r0 + p.left + 1) / TILE;
+  return {from - first, static_cast<uint32_t>(max(to - from, 0))};
 }
 
 // 16 (or the first 8) fp32 values as bf16
@@ -780,13 +794,14 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     Row r;
     bool ok = true;
     const int start = !WIN || t == 0 ? 0 : keys.start;
+    Whole whole;
+    if constexpr (WIN) whole = whole_keys(p.win, keys, w.r0 + t * TILE, w.len);
     for (int j = start; j < nt; ++j) {
       ok = __all_sync(0xffffffffu, mbar_wait(s_full(t), (j - start) & 1));
       if (!ok) break;
       tc_fence_after();
       uint32_t v[TILE];
       load_scores(s_at, v);
-      const int k0 = tile(j) * TILE;
       auto grow = [&] {
         const float top = max_of<false>(v) * scale;
         if (__any_sync(0xffffffffu, r.grows(top))) {
@@ -798,17 +813,18 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       if constexpr (WIN) {
         // (two ways from here on: on one for whole tiles and others, 16128 tokens, 8 heads of 48 with a window over nearly all took 925 us where there are 720 without it
         // and 791 like this)
-        if (all_seen(p.win, w.r0 + t * TILE, w.len, k0)) {
+        if (whole(j)) {
           apart<false>();
           grow();
           r.weights(v, scale);
         } else {
           apart<true>();
-          const uint32_t none = hide_scores(v, SeenKeys(p.win, w.r0 + row, w.len, k0));
+          const uint32_t none = hide_scores(v, SeenKeys(p.win, w.r0 + row, w.len, tile(j) * TILE));
           grow();
           r.weights(v, scale, none);
         }
       } else {
+        const int k0 = tile(j) * TILE;
         if (k0 + TILE > w.len || (causal && k0 + TILE - 1 > w.r0 + t * TILE)) hide_scores(v, (causal ? min(w.len, w.r0 + row + 1) : w.len) - k0);
         grow();
         r.weights(v, scale);
@@ -1042,6 +1058,8 @@ attn_fwd_narrow_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     Row r;
     bool ok = true;
     const int start = !WIN || t == 0 ? 0 : keys.start;
+    Whole whole;
+    if constexpr (WIN) whole = whole_keys(p.win, keys, w.r0 + t * TILE, w.len);
     for (int j = start; j < nt; ++j) {
       ok = __all_sync(0xffffffffu, mbar_wait_soon(s_full(t), (j - start) & 1));
       if (!ok) break;
@@ -1051,7 +1069,6 @@ attn_fwd_narrow_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(s_read(t));
-      const int k0 = tile(j) * TILE;
       auto grow = [&] {
         const float top = max_of<true>(v) * scale;
         if (__any_sync(0xffffffffu, r.grows(top))) {
@@ -1066,17 +1083,18 @@ attn_fwd_narrow_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
       };
       if constexpr (WIN) {
         // (two ways from here on, as above)
-        if (all_seen(p.win, w.r0 + t * TILE, w.len, k0)) {
+        if (whole(j)) {
           apart<false>();
           grow();
           r.weights(v, scale);
         } else {
           apart<true>();
-          const uint32_t none = hide_scores(v, SeenKeys(p.win, w.r0 + row, w.len, k0));
+          const uint32_t none = hide_scores(v, SeenKeys(p.win, w.r0 + row, w.len, tile(j) * TILE));
           grow();
           r.weights(v, scale, none);
         }
       } else {
+        const int k0 = tile(j) * TILE;
         if (k0 + TILE > w.len || (causal && k0 + TILE - 1 > w.r0 + t * TILE)) hide_scores(v, (causal ? min(w.len, w.r0 + row + 1) : w.len) - k0);
         grow();
         r.weights(v, scale);
@@ -1465,6 +1483,8 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
     }
     const float scale = p.t.scale_log2;
     const f32x2 scale2 = f2_pack(scale, scale), l2 = f2_pack(-l, -l), delta2 = f2_pack(-delta, -delta);
+    Whole whole;
+    if constexpr (WIN) whole = whole_keys(p.win, keys, w.r0, w.len);
     bool ok = true;
     for (int j = 0; j < n; ++j) {
       ok = __all_sync(0xffffffffu, mbar_wait_soon(s_full(j & 1), (j >> 1) & 1));
@@ -1478,9 +1498,11 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
       const int below = (causal ? min(w.len, w.r0 + row + 1) : w.len) - k0;
       uint32_t bits = 0xffffffffu;
       if constexpr (WIN) {
-        bits = SeenKeys(p.win, w.r0 + row, w.len, k0).bits(0);
-        edge = !__all_sync(0xffffffffu, bits == 0xffffffffu);
-        none = !__any_sync(0xffffffffu, bits != 0);
+        edge = !whole(j);
+        if (edge) {
+          bits = SeenKeys(p.win, w.r0 + row, w.len, k0).bits(0);
+          none = !__any_sync(0xffffffffu, bits != 0);
+        }
       }
       auto seen = [&](int c) { return WIN ? (bits >> c & 1) != 0 : c < below; };
       tmem_wait32(v);
@@ -1825,6 +1847,8 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const bool here = row < rows;
     const f32x2 scale2 = f2_pack(p.t.scale_log2, p.t.scale_log2);
+    Whole whole;
+    if constexpr (WIN) whole = whole_queries(p.win, w.r0, w.len, q_first);
     bool ok = true;
     int s = 0, t = t0;
     uint32_t ph = 0;
@@ -1841,14 +1865,16 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       uint32_t bits = 0xffffffffu;
       bool none = false;
       if constexpr (WIN) {
-        const int key = w.r0 + row;
-        if (key >= p.win.sinks) {
-          if (!causal) from = key - p.win.right - q0;
-          if (p.win.left < w.len - 1 - key) to = key + p.win.left + 1 - q0;
+        edge = !whole(t);
+        if (edge) {
+          const int key = w.r0 + row;
+          if (key >= p.win.sinks) {
+            if (!causal) from = key - p.win.right - q0;
+            if (p.win.left < w.len - 1 - key) to = key + p.win.left + 1 - q0;
+          }
+          bits = low_bits(to) & ~low_bits(from);
+          none = !__any_sync(0xffffffffu, bits != 0);
         }
-        bits = low_bits(to) & ~low_bits(from);
-        edge = !__all_sync(0xffffffffu, bits == 0xffffffffu);
-        none = !__any_sync(0xffffffffu, bits != 0);
       }
       auto seen = [&](int c) { return WIN ? (bits >> c & 1) != 0 : c >= from && c < to; };
       auto neg_l = [&](int c) { return *reinterpret_cast<const f32x2*>(stats + c); };
@@ -2025,14 +2051,14 @@ int window_tiles(const AttnShape& p) {
   const long long span = 1ll * p.left + (p.causal ? 0 : p.right) + TILE;
   return static_cast<int>(std::min<long long>((span + TILE - 1) / TILE + 1, (mean_length(p) + TILE - 1) / TILE));
 }
-// Through a window: up to 17 tiles, where start and end of a CTA are a quarter of it, and where CTAs of two tiles would leave SMs idle.  16128 tokens, 8 heads of 48, by
+// Through a window: up to 17 tiles, where start and end of a CTA are a quarter of it, and where CTAs of two tiles would leave half of the SMs idle.  16128 tokens, 8 heads of 48, by
 // tokens to either side, two tiles / one: 192 58 / 57, 704 115 / 113, 960 143 / 140, 1472 195 / 195, 3008 342 / 339, 4000 380 / 396; of 128 704 150 / 144, 960 180 / 177, 1472
 // 238 / 240, 3008 402 / 430; 1 head of 64 300 20.5 / 18.0, 2000 63 / 56, 8000 206 / 188; 4000 tokens, 4 of 64 500 24.2 / 21.4.
 constexpr int ONE_TILE_WINDOW = 17;
 bool one_tile_pays(const AttnShape& p) {
-  const bool idle = blocks_of(slots_of(p, p.H, 2 * TILE, 1)) <= sm_count();
-  if (p.window) return idle || window_tiles(p) <= ONE_TILE_WINDOW;
-  return mean_length(p) <= (p.D <= 64 ? 768 : 448) && !idle;
+  const long long blocks = blocks_of(slots_of(p, p.H, 2 * TILE, 1));
+  if (p.window) return 2 * blocks <= sm_count() || window_tiles(p) <= ONE_TILE_WINDOW;
+  return mean_length(p) <= (p.D <= 64 ? 768 : 448) && blocks > sm_count();
 }
 // CTAs of one length that would be a last wave of their own, or that are fewer than the SMs, are split over the keys so that they fill them, where that saves more
 // than joining them costs: tiles of keys, of some 0.7 us.  us, whole / split: 16200 tokens, 8 heads of 48 720 / 641, 12 of 64 1086 / 955, 8 of 128 943 / 847; 5000
