@@ -1549,7 +1549,7 @@ template <int DB>
 struct Dkv {
   static constexpr int STAGES = DB == 1 ? 3 : 2, TILE_BYTES = DB * BOX, S_BUFS = DB == 1 ? 2 : 1;
   static constexpr int STAGE_AT = 2 * TILE_BYTES, STAGE = 2 * TILE_BYTES, STAT_AT = STAGE_AT + STAGES * STAGE, STAT = 2 * TILE * 4;
-  static constexpr int BAR_AT = STAT_AT + STAGES * STAT, BARS = 4 * STAGES + 9;
+  static constexpr int BAR_AT = STAT_AT + STAGES * STAT, BARS = 4 * STAGES + 10;
   static constexpr int SMEM = BAR_AT + 8 * BARS + 16 + 1024;
   static constexpr uint32_t DP_AT = S_BUFS * S_COLS, DV_AT = DP_AT + S_COLS, DK_AT = DV_AT + DB * 64;
   static_assert(SMEM <= SMEM_LIMIT && DK_AT + DB * 64 == 512);
@@ -1616,10 +1616,11 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
   auto do_full = [&](int s) { return bars + 8u * (L::STAGES + s); };
   auto empty = [&](int s) { return bars + 8u * (2 * L::STAGES + s); };
   auto stat_full = [&](int s) { return bars + 8u * (3 * L::STAGES + s); };
-  const uint32_t kv_full = bars + 8u * (4 * L::STAGES), fixed = kv_full + 8u, p_ready = kv_full + 16u, ds_ready = kv_full + 24u,
+  const uint32_t kv_full = bars + 8u * (4 * L::STAGES), fixed = kv_full + 8u, fix_bar = kv_full + 16u, ds_ready = kv_full + 24u,
                  dp_full = kv_full + 32u, acc_full = kv_full + 40u;
   auto s_full = [&](int b) { return kv_full + 48u + 8u * b; };
-  const uint32_t fix_bar = kv_full + 64u;
+  // (one for either buffer of S: where the next scores are there early, a warp with little to do may be done with them before others are with these)
+  auto p_ready = [&](int b) { return kv_full + 64u + 8u * b; };
   volatile uint32_t* const tmem_slot = reinterpret_cast<volatile uint32_t*>(smem_raw + pad + L::BAR_AT + 8 * L::BARS);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -1628,7 +1629,8 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     mbar_init(kv_full, 1);
     mbar_init(fixed, 1);
     mbar_init(fix_bar, 1);
-    mbar_init(p_ready, BWD_WARPS);
+    mbar_init(p_ready(0), BWD_WARPS);
+    mbar_init(p_ready(1), BWD_WARPS);
     mbar_init(ds_ready, BWD_WARPS);
     mbar_init(dp_full, 1);
     mbar_init(acc_full, 1);
@@ -1765,7 +1767,7 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
           if (!ok) break;
           const bool clear = fix && t == q_tiles - 1;
           if (clear) mbar_arrive(fix_bar);
-          ok = (!clear || mbar_wait(fixed, (g - g0) & 1)) && mbar_wait(p_ready, j & 1);
+          ok = (!clear || mbar_wait(fixed, (g - g0) & 1)) && mbar_wait(p_ready(buf), L::S_BUFS == 2 ? (j >> 1) & 1 : j & 1);
           if (!ok) {
             atomicExch(p.t.err, 92);
             break;
@@ -1897,7 +1899,7 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(p_ready);
+      if (lane == 0) mbar_arrive(p_ready(buf));
       ok = __all_sync(0xffffffffu, mbar_wait_soon(dp_full, j & 1));
       if (!ok) break;
       tc_fence_after();

@@ -377,3 +377,19 @@ def test_transforms_and_refusals_of_windows(gen):
     assert torch.allclose(many.float(), o.float(), atol=0.03)
     with pytest.raises(RuntimeError, match="sinks"):
         _ext.require().attention(q, k, v, None, False, 0.25, 4, 4, -1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("N,H,Hk,D,window,sinks", [(4100, 6, 2, 24, 60, 300), (2177, 4, 4, 64, 40, 0), (1030, 8, 1, 8, 129, 3), (2052, 3, 3, 96, 20, 1)])
+def test_last_tiles_of_few_keys_repeat_themselves(gen, N, H, Hk, D, window, sinks, causal):
+    """Warps whose columns nobody sees are through with a tile before the others, and must not run into the next but one: the same bits, many times over."""
+    q, k, v, do = _inputs(gen, 1, N, H=H, Hk=Hk, D=D)
+    mask = dict(causal=causal, window=window, sinks=sinks)
+    first = _run(q, k, v, do, **mask)
+    want, off = _oracle(q[0], k[0], v[0], do[0], D ** -0.5, [(0, N)], **mask)
+    for n in want:
+        _close(first[n][0], want[n], off[n], n)
+    for _ in range(150):
+        again = _run(q, k, v, do, **mask)
+        assert all(torch.equal(first[n], again[n]) for n in first)
