@@ -16,6 +16,7 @@
 #include <cmath>
 
 #include <ATen/cuda/CUDAGeneratorImpl.h>
+#include <ATen/cuda/EmptyTensor.h>
 
 #include "attention.cuh"
 #include "dropout.cuh"
@@ -36,8 +37,13 @@ T* ptr_or_null(const Tensor& t) {
 bool is_f32(const Tensor& t) { return t.scalar_type() == at::kFloat; }
 bool native_type(const Tensor& t) { return is_f32(t) || t.scalar_type() == at::kBFloat16; }
 
-using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
+
+// A dense tensor, without the dispatcher's way there (half a microsecond each, of which a backward pass has seven)
+Tensor room(at::IntArrayRef sizes, const Tensor& like, at::ScalarType type) {
+  return Tensor(at::detail::empty_cuda(sizes, type, like.device(), std::nullopt));
+}
+Tensor room(const Tensor& like) { return room(like.sizes(), like, like.scalar_type()); }
 
 bool records(std::initializer_list<const Tensor*> ts) {
   bool any = false;
@@ -447,8 +453,6 @@ Tensor readable(const Tensor& t) {
 struct Mask {
   bool causal = false;
   int64_t left = -1, right = -1, sinks = 0;
-  std::vector<int64_t> kept() const { return {causal, left, right, sinks}; }
-  static Mask of(const std::vector<int64_t>& v) { return {v[0] != 0, v[1], v[2], v[3]}; }
 };
 
 mk::AttnShape shape_of(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& offsets, const Mask& mask, double scale) {
@@ -491,15 +495,15 @@ std::tuple<Tensor, Tensor, Tensor> attention_forward(const Tensor& q_in, const T
                                                      double scale, bool train) {
   const mk::AttnShape p = shape_of(q_in, k_in, v_in, offsets, mask, scale);
   c10::cuda::CUDAGuard guard(q_in.device());
-  Tensor o = at::empty(q_in.sizes(), q_in.options()), rest, lse;
+  Tensor o = room(q_in), rest, lse;
   if (train) {
-    rest = at::empty(q_in.sizes(), q_in.options());
-    lse = at::empty({p.B, p.H, p.N}, q_in.options().dtype(at::kFloat));
+    rest = room(q_in);
+    lse = room({p.B, p.H, p.N}, q_in, at::kFloat);
   }
   if (o.numel() == 0) return {o, rest, lse};
   const Tensor q = readable(q_in), k = readable(k_in), v = readable(v_in);
   Tensor scratch;
-  if (const int64_t floats = mk::attention_scratch(p)) scratch = at::empty({floats}, q.options().dtype(at::kFloat));
+  if (const int64_t floats = mk::attention_scratch(p)) scratch = room({floats}, q, at::kFloat);
   int launches = 0;
   mkh::check(mk::attention_fwd(p, view_of(q), view_of(k), view_of(v), bf(o), ptr_or_null<__nv_bfloat16>(rest), ptr_or_null<float>(lse),
                                ptr_or_null<float>(scratch), &launches, mkh::error_word(q), mkh::stream()),
@@ -519,9 +523,9 @@ void attention_backward(const Tensor& d_out, const Tensor& q_in, const Tensor& k
   if (o.numel() == 0) return;
   Tensor g = d_out.contiguous();
   if (reinterpret_cast<uintptr_t>(g.data_ptr()) & 15) g = g.clone();
-  const Tensor q = readable(q_in), k = readable(k_in), v = readable(v_in), delta = at::empty_like(lse);
+  const Tensor q = readable(q_in), k = readable(k_in), v = readable(v_in), delta = room(lse);
   Tensor scratch;
-  if (const int64_t floats = mk::attention_bwd_scratch(p)) scratch = at::empty({floats}, q.options().dtype(at::kFloat));
+  if (const int64_t floats = mk::attention_bwd_scratch(p)) scratch = room({floats}, q, at::kFloat);
   int launches = 0;
   mkh::check(mk::attention_bwd(p, view_of(q), view_of(k), view_of(v), bf(o), bf(rest), bf(g), lse.data_ptr<float>(), delta.data_ptr<float>(), view_of(dq),
                                view_of(dk), view_of(dv), ptr_or_null<float>(scratch), &launches, mkh::error_word(q), mkh::stream()),
@@ -529,25 +533,24 @@ void attention_backward(const Tensor& d_out, const Tensor& q_in, const Tensor& k
   mkh::launches() += launches;
 }
 
-// (masks go by value through `saved_data`, as lists of whole numbers)
-struct Attention : torch::autograd::Function<Attention> {
-  static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& offsets, const std::vector<int64_t>& mask,
-                        double scale, bool train) {
-    auto [o, rest, lse] = attention_forward(q, k, v, offsets, Mask::of(mask), scale, train);
-    if (train) {
-      ctx->save_for_backward({q, k, v, o, rest, lse, value(offsets)});
-      ctx->saved_data["mask"] = mask;
-      ctx->saved_data["scale"] = scale;
-    }
-    return o;
-  }
-  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
-    const Backward count;
-    const variable_list s = ctx->get_saved_variables();
-    const Tensor dq = at::empty(s[0].sizes(), s[0].options()), dk = at::empty(s[1].sizes(), s[1].options()), dv = at::empty(s[2].sizes(), s[2].options());
-    attention_backward(grads[0], s[0], s[1], s[2], s[3], s[4], s[5], maybe(s[6]), Mask::of(ctx->saved_data["mask"].toIntVector()),
-                       ctx->saved_data["scale"].toDouble(), dq, dk, dv);
-    return once_differentiable({dq, dk, dv, Tensor(), Tensor(), Tensor(), Tensor()});
+// Numbers of a mask in a node's fields, from `at` on
+void keep_mask(Fields& f, size_t at, const Mask& m) {
+  f.whole[at] = m.causal;
+  f.whole[at + 1] = m.left;
+  f.whole[at + 2] = m.right;
+  f.whole[at + 3] = m.sinks;
+}
+Mask kept_mask(const Fields& f, size_t at) { return {f.whole[at] != 0, f.whole[at + 1], f.whole[at + 2], f.whole[at + 3]}; }
+
+struct AttentionOp {
+  static constexpr const char* NAME = "AttentionNode";
+  // fields: mask; scale.  kept: q, k, v, what the forward pass left, offsets.  edges: q, k, v
+  static variable_list gradients(const variable_list& grads, const variable_list& s, const Fields& f, const std::vector<bool>&) {
+    if (!grads[0].defined()) return variable_list(3);
+    const at::AutoDispatchBelowAutograd below;
+    const Tensor dq = room(s[0]), dk = room(s[1]), dv = room(s[2]);
+    attention_backward(grads[0], s[0], s[1], s[2], s[3], s[4], s[5], maybe(s[6]), kept_mask(f, 0), f.real[0], dq, dk, dv);
+    return once_differentiable({dq, dk, dv});
   }
 };
 
@@ -556,7 +559,20 @@ OptTensor attention(const Tensor& q, const Tensor& k, const Tensor& v, const Opt
                     int64_t sinks) {
   const Tensor at = value(offsets);
   if (!plain({&q, &k, &v, &at})) return {};
-  return Attention::apply(q, k, v, offsets, Mask{causal, left, right, sinks}.kept(), scale, records({&q, &k, &v}));
+  const bool train = records({&q, &k, &v});
+  const Mask mask{causal, left, right, sinks};
+  Tensor o, rest, lse;
+  {
+    const at::AutoDispatchBelowAutograd below;
+    std::tie(o, rest, lse) = attention_forward(q, k, v, offsets, mask, scale, train);
+  }
+  if (train) {
+    Fields f;
+    keep_mask(f, 0, mask);
+    f.real[0] = scale;
+    FieldNode<AttentionOp>::record({o}, {q, k, v}, {q, k, v, o.detach(), rest, lse, at}, f);
+  }
+  return o;
 }
 
 // The output of a fused projection: [B, N, (q heads | k heads | v heads) x D], dense; its gradient is written as one tensor
@@ -572,29 +588,17 @@ struct Parts {
   }
 };
 
-struct AttentionQkv : torch::autograd::Function<AttentionQkv> {
-  static Tensor forward(AutogradContext* ctx, const Tensor& qkv, int64_t heads, int64_t kv_heads, const OptTensor& offsets, const std::vector<int64_t>& mask,
-                        double scale, bool train) {
-    const Parts p(qkv, heads, kv_heads);
-    auto [o, rest, lse] = attention_forward(p.q, p.k, p.v, offsets, Mask::of(mask), scale, train);
-    if (train) {
-      ctx->save_for_backward({qkv, o, rest, lse, value(offsets)});
-      ctx->saved_data["heads"] = heads;
-      ctx->saved_data["kv_heads"] = kv_heads;
-      ctx->saved_data["mask"] = mask;
-      ctx->saved_data["scale"] = scale;
-    }
-    return o;
-  }
-  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
-    const Backward count;
-    const variable_list s = ctx->get_saved_variables();
-    const int64_t heads = ctx->saved_data["heads"].toInt(), kv_heads = ctx->saved_data["kv_heads"].toInt();
-    const Tensor dqkv = at::empty(s[0].sizes(), s[0].options());
+struct AttentionQkvOp {
+  static constexpr const char* NAME = "AttentionQkvNode";
+  // fields: heads, heads of keys, mask; scale.  kept: projection, what the forward pass left, offsets.  edge: projection
+  static variable_list gradients(const variable_list& grads, const variable_list& s, const Fields& f, const std::vector<bool>&) {
+    if (!grads[0].defined()) return variable_list(1);
+    const at::AutoDispatchBelowAutograd below;
+    const int64_t heads = f.whole[0], kv_heads = f.whole[1];
+    const Tensor dqkv = room(s[0]);
     const Parts p(s[0], heads, kv_heads), d(dqkv, heads, kv_heads);
-    attention_backward(grads[0], p.q, p.k, p.v, s[1], s[2], s[3], maybe(s[4]), Mask::of(ctx->saved_data["mask"].toIntVector()),
-                       ctx->saved_data["scale"].toDouble(), d.q, d.k, d.v);
-    return once_differentiable({dqkv, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()});
+    attention_backward(grads[0], p.q, p.k, p.v, s[1], s[2], s[3], maybe(s[4]), kept_mask(f, 2), f.real[0], d.q, d.k, d.v);
+    return once_differentiable({dqkv});
   }
 };
 
@@ -602,7 +606,23 @@ OptTensor attention_qkv(const Tensor& qkv, int64_t heads, int64_t kv_heads, cons
                         int64_t sinks) {
   const Tensor at = value(offsets);
   if (!plain({&qkv, &at})) return {};
-  return AttentionQkv::apply(qkv, heads, kv_heads, offsets, Mask{causal, left, right, sinks}.kept(), scale, records({&qkv}));
+  const bool train = records({&qkv});
+  const Mask mask{causal, left, right, sinks};
+  Tensor o, rest, lse;
+  {
+    const at::AutoDispatchBelowAutograd below;
+    const Parts p(qkv, heads, kv_heads);
+    std::tie(o, rest, lse) = attention_forward(p.q, p.k, p.v, offsets, mask, scale, train);
+  }
+  if (train) {
+    Fields f;
+    f.whole[0] = heads;
+    f.whole[1] = kv_heads;
+    keep_mask(f, 2, mask);
+    f.real[0] = scale;
+    FieldNode<AttentionQkvOp>::record({o}, {qkv}, {qkv, o.detach(), rest, lse, at}, f);
+  }
+  return o;
 }
 
 // ------------------------------------------------------------------------------------------ rotary positions
@@ -715,9 +735,9 @@ void rotary_back(const RotInputs& in, const Tensor (&dy)[2], const Tensor (&out)
   Tensor x[2], d[2], scratch;
   for (int i = 0; i < 2; ++i) {
     if (!dy[i].defined()) continue;
-    const auto params = dy[i].options().dtype(at::kFloat);
     if (dy[i].numel() == 0) {
-      if (sums[i]) dw[i] = at::zeros({p.D}, params), db[i] = at::zeros({p.D}, params);
+      for (Tensor* t : {&dw[i], &db[i]})
+        if (sums[i]) *t = at::zeros({p.D}, dy[i].options().dtype(at::kFloat));
       continue;
     }
     mk::RotPart& part = p.part[p.parts++];
@@ -731,14 +751,14 @@ void rotary_back(const RotInputs& in, const Tensor (&dy)[2], const Tensor (&out)
     }
     rot_weights(part, in.w[i], in.b[i], d[i]);
     if (sums[i]) {
-      dw[i] = at::empty({p.D}, params);
-      db[i] = at::empty({p.D}, params);
+      dw[i] = room({p.D}, dy[i], at::kFloat);
+      db[i] = room({p.D}, dy[i], at::kFloat);
       part.dw = dw[i].data_ptr<float>();
       part.db = db[i].data_ptr<float>();
     }
   }
   if (p.parts == 0) return;
-  if (sums[0] || sums[1]) scratch = at::empty({mk::rotary_scratch(p)}, like.options().dtype(at::kFloat));
+  if (sums[0] || sums[1]) scratch = room({mk::rotary_scratch(p)}, like, at::kFloat);
   int launches = 0;
   mkh::check(mk::rotary_bwd(p, ptr_or_null<float>(scratch), &launches, mkh::stream()), "rotary_bwd");
   mkh::launches() += launches;
@@ -782,7 +802,7 @@ struct RotaryOp {
         in.w[i] = rot_param(s[4 + i]);
         sums[i] = need[2 + i] || need[4 + i];
       }
-      dx[i] = at::empty(dy[i].sizes(), dy[i].options());
+      dx[i] = room(dy[i]);
     }
     rotary_back(in, dy, dx, s[1], norm, f.real[0], inverse, sums, dw, db);
     for (int i = 0; i < 2; ++i) {
@@ -804,7 +824,7 @@ variable_list rotary_pass(const Tensor& q, const Tensor& k, const Tensor (&w)[2]
     Tensor out[2];
     for (int i = 0; i < 2; ++i)
       if (in.x[i].defined()) {
-        out[i] = at::empty(in.x[i].sizes(), in.x[i].options());
+        out[i] = room(in.x[i]);
         results.push_back(out[i]);
       }
     rotary_into(in, out, plan, norm, eps, inverse);
@@ -841,10 +861,10 @@ struct RotaryAttentionOp {
     const Tensor &qkv = s[0], &offsets = s[6], &qk = s[8];
     const at::AutoDispatchBelowAutograd below;
     const Parts p(qkv, heads, kv_heads);
-    const Tensor dqkv = at::empty(qkv.sizes(), qkv.options());
+    const Tensor dqkv = room(qkv);
     const Parts d(dqkv, heads, kv_heads);
     attention_backward(grads[0], qk.narrow(2, 0, heads), qk.narrow(2, heads, kv_heads), p.v, s[9], s[10], s[11], maybe(offsets),
-                       Mask{f.whole[3] != 0, f.whole[4], f.whole[5], f.whole[6]}, f.real[1], d.q, d.k, d.v);
+                       kept_mask(f, 3), f.real[1], d.q, d.k, d.v);
     RotInputs in;
     in.positions = s[5];
     const Tensor dx[2] = {d.q, d.k};
@@ -880,7 +900,7 @@ OptTensor rotary_attention_qkv(const Tensor& qkv, int64_t heads, int64_t kv_head
     const at::AutoDispatchBelowAutograd below;
     const Parts p(qkv, heads, kv_heads);
     const RotInputs in{{p.q, p.k}, {rot_param(w[0]), rot_param(w[1])}, {rot_param(b[0]), rot_param(b[1])}, at};
-    qk = at::empty({qkv.size(0), qkv.size(1), heads + kv_heads, p.q.size(3)}, qkv.options());
+    qk = room({qkv.size(0), qkv.size(1), heads + kv_heads, p.q.size(3)}, qkv, qkv.scalar_type());
     const Tensor out[2] = {qk.narrow(2, 0, heads), qk.narrow(2, heads, kv_heads)};
     rotary_into(in, out, plan.numbers, norm, eps, false);
     std::tie(o, rest, lse) = attention_forward(out[0], out[1], p.v, offsets, Mask{causal, left, right, sinks}, scale, train);
@@ -902,7 +922,7 @@ std::tuple<Tensor, Tensor> dropout_pass(const Tensor& x_in, const Tensor& residu
                                         bool copy) {
   c10::cuda::CUDAGuard guard(x_in.device());
   const Tensor x = x_in.contiguous(), r = residual.defined() ? residual.contiguous() : Tensor();
-  const Tensor out = at::empty(x.sizes(), x.options().dtype(out_type)), half = copy ? at::empty(x.sizes(), x.options().dtype(at::kBFloat16)) : Tensor();
+  const Tensor out = room(x.sizes(), x, out_type), half = copy ? room(x.sizes(), x, at::kBFloat16) : Tensor();
   mk::DropParams d{};
   d.x = x.data_ptr();
   d.r = ptr_or_null<void>(r);
@@ -981,7 +1001,7 @@ Tensor dropout_run(const Tensor& x, const Tensor& residual, const Tensor& seed, 
   Tensor kept, y;
   {
     const at::AutoDispatchBelowAutograd below;
-    if (!seed.defined() && train) kept = at::empty({2}, x.options().dtype(at::kLong));
+    if (!seed.defined() && train) kept = room({2}, x, at::kLong);
     y = std::get<0>(dropout_pass(x, residual, seed, kept, p, out_f32 ? at::kFloat : at::kBFloat16, false));
   }
   if (train) {

@@ -115,9 +115,9 @@ def _check_positions(positions, axes, lead, D, device):
         raise ValueError(f"positions must be int32, int64, fp32 or fp64 on {device}, got {positions.dtype} on {positions.device}")
     if positions.requires_grad:
         raise ValueError("no gradient leads to positions")
-    shapes = [(*lead[-1:], len(axes))] + ([(*lead, len(axes))] if len(lead) == 2 else [])
-    if tuple(positions.shape) not in shapes:
-        raise ValueError(f"positions {tuple(positions.shape)} do not match tokens {tuple(lead)} with {len(axes)} axes")
+    shape = positions.shape
+    if not shape or shape[-1] != len(axes.bands) or shape[:-1] != lead and (len(shape) != 2 or shape[0] != lead[-1]):
+        raise ValueError(f"positions {tuple(shape)} do not match tokens {tuple(lead)} with {len(axes)} axes")
     return positions.contiguous()
 
 
