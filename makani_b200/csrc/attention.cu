@@ -870,21 +870,24 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
 }
 
 // Heads of up to 64 channels: tensor memory has room for S, P and O of both query tiles side by side (128, 64 and 64 columns), so that the next scores are
-// on their way as soon as the last have been read, and no warp waits for products.
+// on their way as soon as the last have been read, and no warp waits for products.  Through windows also with one query tile and two CTAs to an SM (16128 tokens, 8
+// heads of 48, 704 to either side: 102 us where the kernel above takes 113).
+template <int QT>
 struct FwdNarrow {
-  static constexpr int STAGES = 4;
-  static constexpr int K_AT = 2 * BOX, V_AT = K_AT + STAGES * BOX, BAR_AT = V_AT + STAGES * BOX;
+  static constexpr int STAGES = 2 * QT, THREADS_ = 32 * (COMPUTE_WARP + 4 * QT);
+  static constexpr int K_AT = QT * BOX, V_AT = K_AT + STAGES * BOX, BAR_AT = V_AT + STAGES * BOX;
   static constexpr int BARS = 4 * STAGES + 11;
   static constexpr int SMEM = BAR_AT + 8 * BARS + 16 + 1024;
-  static constexpr uint32_t P_AT = 256, O_AT = 384;
-  static_assert(SMEM <= SMEM_LIMIT);
+  static constexpr uint32_t COLS = 256 * QT, P_AT = 128 * QT, O_AT = 192 * QT;
+  static constexpr int FEW = Fwd<1, QT>::FEW, MANY = Fwd<1, QT>::MANY;
+  static_assert(SMEM * (3 - QT) <= SMEM_LIMIT);
 };
 
-template <bool WIN>
-__global__ void __launch_bounds__(THREADS, 1)
+template <int QT, bool WIN>
+__global__ void __launch_bounds__(FwdNarrow<QT>::THREADS_, 3 - QT)
 attn_fwd_narrow_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                        const With<FwdParams, WIN> p) {
-  using L = FwdNarrow;
+  using L = FwdNarrow<QT>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = smem_u32(smem_raw);
   const uint32_t pad = (1024u - (raw_addr & 1023u)) & 1023u;
@@ -905,11 +908,11 @@ attn_fwd_narrow_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     for (int s = 0; s < L::STAGES; ++s) {
       mbar_init(k_full(s), 1);
       mbar_init(v_full(s), 1);
-      mbar_init(k_empty(s), 2);
-      mbar_init(v_empty(s), 2);
+      mbar_init(k_empty(s), QT);
+      mbar_init(v_empty(s), QT);
     }
     mbar_init(q_full, 1);
-    mbar_init(v_fix, 2);
+    mbar_init(v_fix, QT);
     mbar_init(v_fixed, 1);
     for (int t = 0; t < 2; ++t) {
       mbar_init(s_full(t), 1);
@@ -920,9 +923,10 @@ attn_fwd_narrow_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_async_smem();
   }
-  if (warp == 1) tmem_alloc<512>(tmem_slot);
+  if (QT == 2 && warp == 1) tmem_alloc<L::COLS>(tmem_slot);
   const int* offsets = p.t.grid.offsets;
   chain_begin(true, offsets);
+  if (QT == 1 && warp == 1) tmem_alloc<L::COLS>(tmem_slot);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -931,7 +935,7 @@ attn_fwd_narrow_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
   Work w;
   Share share(p.split);
   const bool any = find_work(p.t.grid, offsets, share.unit, w);
-  const int rows = any ? min(w.len - w.r0, 2 * TILE) : 0;
+  const int rows = any ? min(w.len - w.r0, QT * TILE) : 0;
   const bool causal = p.t.causal != 0;
   auto tiles_of = [&](int t) {      // of keys, that the queries of tile t see
     if (w.padding || rows <= t * TILE) return 0;
@@ -954,7 +958,7 @@ attn_fwd_narrow_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
   const bool fix = n > 0 && tail < TILE && w.lo + w.len < p.t.grid.N;
 
   if (warp < COMPUTE_WARP) {
-    regs_down<FEW_REGS>();
+    regs_down<L::FEW>();
     if (warp == 0) {
       // ---------------------------------------------------------------- tiles
       if (n > 0 && elect_one()) {
@@ -982,7 +986,7 @@ attn_fwd_narrow_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
           }
         }
       }
-    } else if (warp & 1) {
+    } else if (QT == 2 ? (warp & 1) != 0 : warp == 1) {
       // ---------------------------------------------------------------- products, a warp for either query tile
       if (n > 0 && elect_one()) {
         const int t = warp >> 1, nt = t == 0 ? n0 : n1, start = !WIN || t == 0 ? 0 : keys.start;
@@ -1048,7 +1052,7 @@ attn_fwd_narrow_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
       }
     }
   } else {
-    regs_up<MANY_REGS>();
+    regs_up<L::MANY>();
     // ------------------------------------------------------------------ softmax
     const int t = (warp - COMPUTE_WARP) >> 2, row = t * TILE + (warp & 3) * 32 + lane, nt = t == 0 ? n0 : n1;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
@@ -1140,7 +1144,7 @@ attn_fwd_narrow_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
   __syncthreads();
   if (warp == 1) {
     tc_fence_after();
-    tmem_free<512>(tmem);
+    tmem_free<L::COLS>(tmem);
   }
 }
 
@@ -2053,9 +2057,9 @@ int window_tiles(const AttnShape& p) {
   const long long span = 1ll * p.left + (p.causal ? 0 : p.right) + TILE;
   return static_cast<int>(std::min<long long>((span + TILE - 1) / TILE + 1, (mean_length(p) + TILE - 1) / TILE));
 }
-// Through a window: up to 17 tiles, where start and end of a CTA are a quarter of it, and where CTAs of two tiles would leave half of the SMs idle.  16128 tokens, 8 heads of 48, by
-// tokens to either side, two tiles / one: 192 58 / 57, 704 115 / 113, 960 143 / 140, 1472 195 / 195, 3008 342 / 339, 4000 380 / 396; of 128 704 150 / 144, 960 180 / 177, 1472
-// 238 / 240, 3008 402 / 430; 1 head of 64 300 20.5 / 18.0, 2000 63 / 56, 8000 206 / 188; 4000 tokens, 4 of 64 500 24.2 / 21.4.
+// Through a window: up to 17 tiles, where start and end of a CTA are a quarter of it, and where CTAs of two tiles would leave half of the SMs idle.  us by tokens to
+// either side, two tiles / one: 16128 tokens, 8 heads of 48 192 58 / 54, 704 115 / 102, 960 143 / 125; of 128 704 150 / 144, 960 180 / 177, 1472 238 / 240, 3008 402 /
+// 430; 1 head of 64 300 20.5 / 16.9, 2000 63 / 48, 8000 206 / 160; 4000 tokens, 4 of 64 500 24.2 / 19.5.
 constexpr int ONE_TILE_WINDOW = 17;
 bool one_tile_pays(const AttnShape& p) {
   const long long blocks = blocks_of(slots_of(p, p.H, 2 * TILE, 1));
@@ -2124,10 +2128,14 @@ template <bool WIN>
 cudaError_t launch_fwd(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const With<FwdParams, WIN>& p, bool one_tile, cudaStream_t s) {
   static std::atomic<uint64_t> devices[4];
   if (one_tile) {
-    if (p.t.D <= 64) return launch(attn_fwd_kernel<1, 1, WIN>, devices[0], Fwd<1, 1>::THREADS_, Fwd<1, 1>::SMEM, q, k, v, p, s);
+    if constexpr (WIN) {
+      if (p.t.D <= 64) return launch(attn_fwd_narrow_kernel<1, true>, devices[0], FwdNarrow<1>::THREADS_, FwdNarrow<1>::SMEM, q, k, v, p, s);
+    } else {
+      if (p.t.D <= 64) return launch(attn_fwd_kernel<1, 1, false>, devices[0], Fwd<1, 1>::THREADS_, Fwd<1, 1>::SMEM, q, k, v, p, s);
+    }
     return launch(attn_fwd_kernel<2, 1, WIN>, devices[1], Fwd<2, 1>::THREADS_, Fwd<2, 1>::SMEM, q, k, v, p, s);
   }
-  if (p.t.D <= 64) return launch(attn_fwd_narrow_kernel<WIN>, devices[2], THREADS, FwdNarrow::SMEM, q, k, v, p, s);
+  if (p.t.D <= 64) return launch(attn_fwd_narrow_kernel<2, WIN>, devices[2], THREADS, FwdNarrow<2>::SMEM, q, k, v, p, s);
   return launch(attn_fwd_kernel<2, 2, WIN>, devices[3], Fwd<2, 2>::THREADS_, Fwd<2, 2>::SMEM, q, k, v, p, s);
 }
 template <int DB, bool SPLIT, bool WIN>
