@@ -393,3 +393,54 @@ def test_last_tiles_of_few_keys_repeat_themselves(gen, N, H, Hk, D, window, sink
     for _ in range(150):
         again = _run(q, k, v, do, **mask)
         assert all(torch.equal(first[n], again[n]) for n in first)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("D", [64, 96])
+def test_nan_of_a_neighbour_stays_there(gen, D, causal):
+    """Sequences side by side in tiles: what one holds, NaN too, reaches no other, through window and sinks, forward and backward."""
+    off = [0, 200, 201, 700, 1000]
+    q, k, v, do = _inputs(gen, 1000, H=4, Hk=2, D=D)
+    kw = dict(offsets=torch.tensor(off, dtype=torch.int32, device="cuda"), causal=causal, window=70, sinks=3)
+    want = _run(q, k, v, do, **kw)
+    for i in (1, 2):
+        bad = [t.clone() for t in (q, k, v, do)]
+        for t in bad:
+            t[off[i]:off[i + 1]] = math.nan
+        got = _run(*bad, **kw)
+        for n in want:
+            for lo, hi in ((0, off[i]), (off[i + 1], 1000)):
+                assert torch.equal(got[n][lo:hi], want[n][lo:hi]), n
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_other_types_through_torch(gen, dtype):
+    q, k, v, do = (t.to(dtype) for t in _inputs(gen, 300, H=4, Hk=2, D=24))
+    off = [0, 120, 120, 290]
+    for causal in (False, True):
+        mask = dict(causal=causal, window=(30, 10), sinks=2)
+        got = _run(q, k, v, do, offsets=torch.tensor(off, dtype=torch.int32, device="cuda"), **mask)
+        want, _ = _oracle(q, k, v, do, 24 ** -0.5, list(zip(off, off[1:])), **mask)
+        for n in want:
+            assert torch.allclose(got[n].double(), want[n], atol=2e-5 if dtype == torch.float32 else 2e-2), n
+    rot.rotary(q.float(), torch.arange(300, device="cuda")[:, None], rot.RotaryAxes((24,)))      # (one call on a kernel)
+
+
+@pytest.mark.gpu
+def test_two_streams_at_once(gen):
+    """Two calls at the same time, each with workspaces of its own."""
+    sets = [_inputs(gen, 1, 5000, H=4, Hk=1, D=64) for _ in range(2)]
+    mask = dict(causal=True, window=200, sinks=4)
+    want = [_run(*s, **mask) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = [None, None]
+    for _ in range(3):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i] = _run(*sets[i], **mask)
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert all(torch.equal(a[n], b[n]) for n in b)
