@@ -8,7 +8,7 @@
 // Bound by memory: a head's channels are read once and written once (x and dy in the backward pass), and mean and variance are computed again rather than kept.
 // A group of lanes has the channels of a head and goes over the heads of a token.  A lane has four pairs of channels, both of each, so that it turns them
 // without its neighbours: two runs of four channels (halves of a band), or eight side by side (neighbours).  (Eight side by side in either case, with partners
-// through shared memory, took 74 instructions a head and lane where this takes INSTR, and 412 instead of FIXED for a token.)  Angles are computed once for a
+// through shared memory: 37080 tokens, 16 heads of 128 with norms, both ways, 188 us where this took 175; 16200 tokens, 16 heads of 48 62 / 54.)  Angles are computed once for a
 // token's heads, in 64 bits down to the fraction of a turn (the angle of position 100000 in 32 bits would be off by 4e-3).  Statistics, sums and gradients of
 // weights are fp32; blocks leave one row of partial sums each, added up in a fixed order by a second launch.
 #include "rotary.cuh"
