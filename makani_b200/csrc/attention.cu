@@ -201,21 +201,8 @@ struct Slots {
 
 __device__ __forceinline__ int clamp_offset(int v, int n) { return min(max(v, 0), n); }
 
-// all lanes of a warp; false: nothing to do
-__device__ __forceinline__ bool find_work(const Slots& g, const int* offsets, uint32_t block, Work& w) {
-  int slot;
-  if (g.order) {
-    w.h = static_cast<int>(block % g.H);
-    const uint32_t rest = block / g.H;
-    slot = static_cast<int>(rest % g.slots);
-    if (g.order == 1) slot = g.slots - 1 - slot;
-    w.b = static_cast<int>(rest / g.slots);
-  } else {
-    slot = static_cast<int>(block % g.slots);
-    const uint32_t rest = block / g.slots;
-    w.h = static_cast<int>(rest % g.H);
-    w.b = static_cast<int>(rest / g.H);
-  }
+// The sequence and the rows of a slot, all lanes of a warp; false: nothing to do
+__device__ __forceinline__ bool find_rows(const Slots& g, const int* offsets, int slot, Work& w) {
   w.padding = false;
   if (!offsets) {
     w.lo = 0;
@@ -242,6 +229,32 @@ __device__ __forceinline__ bool find_work(const Slots& g, const int* offsets, ui
   w.len = (w.padding ? g.N : max(begin(lo + 1), w.lo)) - w.lo;
   w.r0 = (slot - (w.lo / g.rows + lo)) * g.rows;
   return w.r0 >= 0 && w.r0 < w.len;
+}
+__device__ __forceinline__ bool find_work(const Slots& g, const int* offsets, uint32_t block, Work& w) {
+  int slot;
+  if (g.order) {
+    w.h = static_cast<int>(block % g.H);
+    const uint32_t rest = block / g.H;
+    slot = static_cast<int>(rest % g.slots);
+    if (g.order == 1) slot = g.slots - 1 - slot;
+    w.b = static_cast<int>(rest / g.slots);
+  } else {
+    slot = static_cast<int>(block % g.slots);
+    const uint32_t rest = block / g.slots;
+    w.h = static_cast<int>(rest % g.H);
+    w.b = static_cast<int>(rest / g.H);
+  }
+  return find_rows(g, offsets, slot, w);
+}
+// With heads along y, and the tiles of the batches one behind the other along x: a CTA does not begin with divisions that wait for one another.  `unit` comes in as
+// the place along x and goes out as what `find_work` takes (order 0).
+__device__ __forceinline__ bool find_work_of_head(const Slots& g, const int* offsets, uint32_t& unit, Work& w) {
+  const uint32_t b = g.B == 1 ? 0u : unit / g.slots;
+  const int slot = static_cast<int>(unit - b * g.slots);
+  w.h = static_cast<int>(blockIdx.y);
+  w.b = static_cast<int>(b);
+  unit = (b * g.H + w.h) * g.slots + slot;
+  return find_rows(g, offsets, slot, w);
 }
 
 // Clears the rows from `valid` on of a tile of `boxes` boxes (a warp): they belong to another sequence, and what stands there, NaN perhaps, would
@@ -406,6 +419,28 @@ __device__ __forceinline__ void stage_output(uint32_t taddr, int D, float f, uin
       *reinterpret_cast<uint4*>(out + row * stride + c * 8) = *at(row, c);
     }
     __syncwarp();
+  }
+}
+// Columns c0 to c1 (whole eights, 8 CHUNKS of them at most) of an accumulator's rows, times f, as bf16, through shared memory in the same way (`stage`: 32 rows of CHUNKS x 16 bytes)
+template <int CHUNKS>
+__device__ __forceinline__ void stage_rows(uint32_t taddr, int c0, int c1, float f, uint8_t* stage, __nv_bfloat16* to, long long stride, int rows) {
+  const int lane = threadIdx.x & 31;
+  auto at = [&](int row, int c) { return reinterpret_cast<uint4*>(stage + (row * CHUNKS + (c ^ ((row * CHUNKS >> 3) & (CHUNKS - 1)))) * 16); };
+#pragma unroll
+  for (int c = 0; c < 8 * CHUNKS; c += 16) {
+    if (c0 + c >= c1) break;
+    uint32_t v[16];
+    tmem_ld16(taddr + c0 + c, v);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * f);
+    *at(lane, c / 8) = pack8(v);
+    *at(lane, c / 8 + 1) = pack8(v + 8);      // (behind the last column perhaps)
+  }
+  __syncwarp();
+#pragma unroll
+  for (int i = lane; i < 32 * CHUNKS; i += 32) {
+    const int row = i / CHUNKS, c = i % CHUNKS;
+    if (row < rows && c0 + c * 8 < c1) *reinterpret_cast<uint4*>(to + row * stride + c0 + c * 8) = *at(row, c);
   }
 }
 // CTAs that are split over what they go along: those from `whole` on, into `parts`
@@ -655,7 +690,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
 
   Work w;
   Share share(p.split);
-  const bool any = find_work(p.t.grid, offsets, share.unit, w);
+  const bool any = WIN ? find_work_of_head(p.t.grid, offsets, share.unit, w) : find_work(p.t.grid, offsets, share.unit, w);
   const int rows = any ? min(w.len - w.r0, QT * TILE) : 0;
   const bool causal = p.t.causal != 0;
   auto tiles_of = [&](int t) {      // of keys, that the queries of tile t see
@@ -934,7 +969,7 @@ attn_fwd_narrow_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
 
   Work w;
   Share share(p.split);
-  const bool any = find_work(p.t.grid, offsets, share.unit, w);
+  const bool any = WIN ? find_work_of_head(p.t.grid, offsets, share.unit, w) : find_work(p.t.grid, offsets, share.unit, w);
   const int rows = any ? min(w.len - w.r0, QT * TILE) : 0;
   const bool causal = p.t.causal != 0;
   auto tiles_of = [&](int t) {      // of keys, that the queries of tile t see
@@ -1341,7 +1376,7 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
 
   Work w;
   ShareOf<SPLIT> share(p.split);
-  const bool any = find_work(p.t.grid, offsets, share.unit, w);
+  const bool any = WIN ? find_work_of_head(p.t.grid, offsets, share.unit, w) : find_work(p.t.grid, offsets, share.unit, w);
   const int rows = any ? min(w.len - w.r0, TILE) : 0;
   const bool causal = p.t.causal != 0;
   const KeyTiles keys = window_keys<WIN>(p, w, rows);
@@ -1531,6 +1566,9 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
     if (n > 0 && ok) {
       tc_fence_after();
       if (SPLIT && share.part >= 0) store_part(tmem + lanes + DQ_ACC, p.t.D, p.sums + share.row(p.split, TILE, row) * p.t.D, here, x * 8, 32);
+      else if constexpr (WIN)      // (a row to a thread, each of its stores touches 32 lines a warp)
+        stage_rows<4 * DB / 2>(tmem + lanes + DQ_ACC, x * 16 * DB, min(p.t.D, (x + 1) * 16 * DB), p.t.scale, smem_raw + pad + L::K_AT + (warp - COMPUTE_WARP) * 1024 * DB,
+                               to - static_cast<long long>(lane) * p.dq.token, p.dq.token, min(rows - row + lane, 32));
       else store_row(tmem + lanes + DQ_ACC, p.t.D, p.t.scale, to, here, x * 16, 64);
     } else if (here && w.padding && x == 0) {
       zero_row(p.t.D, to);
@@ -1559,11 +1597,11 @@ struct Dkv {
   static_assert(SMEM <= SMEM_LIMIT && DK_AT + DB * 64 == 512);
 };
 
-// Windows: tiles with sinks are seen by all queries of their sequence, and go apart.  The first units x parts CTAs have them: unit (sequence, head of keys, tile),
-// in as many parts, along queries and heads, as have two tiles of queries each, and leave sums; the others have the rest.
+// Windows: tiles with sinks are seen by all queries of their sequence, and go apart.  The `first` CTAs of a head have them: (sequence, tile, part) in as many parts,
+// along queries and heads, as have two tiles of queries each; they leave sums, by units (sequence, head, tile).  The others have the rest.
 struct SinkTiles {
   int parts, tiles;        // parts 0: nothing goes apart
-  uint32_t units;
+  uint32_t units, first;
   __host__ __device__ int parts_of(int total) const {      // that have something to do
     const int most = total / 2 > 1 ? total / 2 : 1;
     return parts < most ? parts : most;
@@ -1580,11 +1618,8 @@ struct QueryTiles {
     n = rows > 0 ? hi / TILE + 1 - first : 0;
   }
 };
-__device__ __forceinline__ bool find_sinks(const Slots& g, const int* offsets, const SinkTiles& s, uint32_t unit, Work& w) {
-  const int tile = static_cast<int>(unit % s.tiles);
-  const uint32_t rest = unit / s.tiles;
-  w.h = static_cast<int>(rest % g.H);
-  const int sequence = static_cast<int>(rest / g.H);
+__device__ __forceinline__ bool place_sinks(const Slots& g, const int* offsets, int sequence, int head, int tile, Work& w) {
+  w.h = head;
   w.b = offsets ? 0 : sequence;
   w.lo = offsets && sequence > 0 ? clamp_offset(__ldg(offsets + sequence), g.N) : 0;
   w.len = offsets ? max(clamp_offset(__ldg(offsets + sequence + 1), g.N) - w.lo, 0) : g.N;
@@ -1656,11 +1691,18 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
   ShareOf<SPLIT> share(p.split);
   bool any, apart = false;
   if constexpr (WIN && SPLIT) {
-    const uint32_t first = p.sinks.units * p.sinks.parts;
-    apart = blockIdx.x < first;
-    if (!apart) share = ShareOf<SPLIT>(p.split, blockIdx.x - first);
-    any = apart ? find_sinks(p.t.grid, offsets, p.sinks, blockIdx.x / p.sinks.parts, w) : find_work(p.t.grid, offsets, share.unit, w);
-    if (!apart && any && first > 0 && !w.padding && w.r0 < p.win.sinks) any = false;
+    apart = blockIdx.x < p.sinks.first;
+    if (apart) {
+      const uint32_t r = blockIdx.x / p.sinks.parts, sequence = r / p.sinks.tiles, tile = r - sequence * p.sinks.tiles;
+      share.unit = (sequence * p.t.grid.H + blockIdx.y) * p.sinks.tiles + tile;
+      share.part = static_cast<int>(blockIdx.x - r * p.sinks.parts);
+      any = place_sinks(p.t.grid, offsets, static_cast<int>(sequence), static_cast<int>(blockIdx.y), static_cast<int>(tile), w);
+    } else {
+      share = ShareOf<SPLIT>(p.split, blockIdx.x - p.sinks.first);
+      any = find_work_of_head(p.t.grid, offsets, share.unit, w) && !(p.sinks.first > 0 && !w.padding && w.r0 < p.win.sinks);
+    }
+  } else if constexpr (WIN) {
+    any = find_work_of_head(p.t.grid, offsets, share.unit, w);
   } else {
     any = find_work(p.t.grid, offsets, share.unit, w);
   }
@@ -1673,12 +1715,10 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     q_first = queries.first;
     q_tiles = queries.n;
   }
-  share.along(p.split, q_tiles * p.t.group);
+  if (!apart) share.along(p.split, q_tiles * p.t.group);
   if constexpr (WIN && SPLIT) {
     if (apart) {
       const int total = q_tiles * p.t.group, parts = p.sinks.parts_of(total);
-      share.unit = blockIdx.x / p.sinks.parts;
-      share.part = static_cast<int>(blockIdx.x % p.sinks.parts);
       share.first = share.part < parts ? static_cast<int>(static_cast<long long>(total) * share.part / parts) : 0;
       share.n = share.part < parts ? static_cast<int>(static_cast<long long>(total) * (share.part + 1) / parts) - share.first : 0;
     }
@@ -1933,9 +1973,15 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       tc_fence_after();
       const uint32_t acc = tmem + lanes + (values ? L::DV_AT : L::DK_AT);
       if (SPLIT && share.part >= 0) {
-        const long long at = WIN && apart ? static_cast<long long>(blockIdx.x) * TILE + row : share.row(p.split, TILE, row);
+        long long at;
+        if constexpr (WIN) at = apart ? (static_cast<long long>(share.unit) * p.sinks.parts + share.part) * TILE + row : share.row(p.split, TILE, row);
+        else at = share.row(p.split, TILE, row);
         store_part(acc, p.t.D, (values ? p.dv_sums : p.dk_sums) + at * p.t.D, here, (x & 1) * 8, 16);
       }
+      else if constexpr (WIN)
+        stage_rows<4 * DB>(acc, (x & 1) * 32 * DB, min(p.t.D, ((x & 1) + 1) * 32 * DB), values ? 1.f : p.t.scale,
+                           smem_raw + pad + L::STAGE_AT + (warp - COMPUTE_WARP) * 2048 * DB, to - static_cast<long long>(lane) * d.token, d.token,
+                           min(rows - row + lane, 32));
       else store_row(acc, p.t.D, values ? 1.f : p.t.scale, to, here, (x & 1) * 16, 32);
     } else if (here && w.padding && (x & 1) == 0) {
       zero_row(p.t.D, to);
@@ -1985,7 +2031,10 @@ __global__ void __launch_bounds__(256) attn_sink_sum_kernel(TileParams t, Window
   const uint32_t at = blockIdx.x * 8 + (threadIdx.x >> 5), unit = at / TILE;
   const int row = static_cast<int>(at % TILE);
   Work w;
-  if (!find_sinks(t.grid, offsets, s, unit, w) || w.r0 + row >= w.len || c >= t.D) return;
+  const uint32_t rest = unit / s.tiles, sequence = rest / t.grid.H;
+  if (!place_sinks(t.grid, offsets, static_cast<int>(sequence), static_cast<int>(rest - sequence * t.grid.H), static_cast<int>(unit - rest * s.tiles), w) ||
+      w.r0 + row >= w.len || c >= t.D)
+    return;
   const int n = s.parts_of(QueryTiles(win, w.r0, min(w.len - w.r0, TILE), w.len).n * t.group);
   float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int k = 0; k < n; ++k) {
@@ -2028,7 +2077,7 @@ long long blocks_of(const Slots& g) { return 1ll * g.slots * g.H * g.B; }
 bool shape_ok(const AttnShape& p) {
   return p.B > 0 && p.N > 0 && p.H > 0 && p.Hk > 0 && p.H % p.Hk == 0 && p.D > 0 && p.D % 8 == 0 && p.D <= ATTN_WIDTH && p.scale > 0.f &&
          (!p.offsets || (p.B == 1 && p.sequences >= 0)) &&
-         (!p.window || (p.left >= 0 && p.left <= p.N && p.right >= 0 && p.right <= p.N && p.sinks >= 0 && p.sinks <= p.N)) && blocks_of(slots_of(p, p.H, TILE, 1)) < (1ll << 31);
+         (!p.window || (p.left >= 0 && p.left <= p.N && p.right >= 0 && p.right <= p.N && p.sinks >= 0 && p.sinks <= p.N && p.H < 65536)) && blocks_of(slots_of(p, p.H, TILE, 1)) < (1ll << 31);
 }
 
 TileParams tile_params(const AttnShape& p, const Slots& g, int* err) {
@@ -2107,22 +2156,28 @@ Parts key_parts(const AttnShape& p, const Slots& g) {
 }
 // Tiles with sinks have all queries of a sequence where others have a window's: parts of about that length, in two waves at most
 SinkTiles sink_tiles(const AttnShape& p) {
-  if (!p.window || p.sinks <= 0) return {0, 1, 0};
+  if (!p.window || p.sinks <= 0) return {0, 1, 0, 0};
   const int tiles = (p.sinks + TILE - 1) / TILE, along = tiles_of(p), each = window_tiles(p);
-  const long long units = 1ll * (p.offsets ? p.sequences : p.B) * p.Hk * tiles;
-  if (units == 0) return {0, 1, 0};
+  const long long rows = 1ll * (p.offsets ? p.sequences : p.B) * tiles, units = rows * p.Hk;
+  if (units == 0) return {0, 1, 0, 0};
   const long long parts = std::min<long long>((along + each - 1) / each, 2ll * sm_count() / units);
-  if (parts < 2) return {0, 1, 0};
-  return {static_cast<int>(parts), tiles, static_cast<uint32_t>(units)};
+  if (parts < 2) return {0, 1, 0, 0};
+  return {static_cast<int>(parts), tiles, static_cast<uint32_t>(units), static_cast<uint32_t>(rows * parts)};
 }
 long long sink_rows(const SinkTiles& s) { return 1ll * s.units * s.parts * TILE; }
 
+// CTAs along x; through a window heads along y, behind `first` CTAs each
+template <bool WIN>
+dim3 grid_of(const Slots& g, const Parts& s, uint32_t first) {
+  if (!WIN) return dim3(static_cast<unsigned>(blocks_of(g, s)));
+  return dim3(static_cast<unsigned>(first + 1ll * g.slots * g.B * std::max(1, s.parts)), static_cast<unsigned>(g.H));
+}
 template <typename Params>
 cudaError_t launch(void (*kernel)(CUtensorMap, CUtensorMap, CUtensorMap, Params), std::atomic<uint64_t>& devices, int threads, int smem, const CUtensorMap& q,
                    const CUtensorMap& k, const CUtensorMap& v, const Params& p, cudaStream_t s) {
   const cudaError_t e = allow_shared_memory(devices, reinterpret_cast<const void*>(kernel), smem);
   if (e != cudaSuccess) return e;
-  return launch_chained(kernel, dim3(static_cast<unsigned>(blocks_of(p.t.grid, p.split))), dim3(threads), smem, s, 1, true, q, k, v, p);
+  return launch_chained(kernel, grid_of<!std::is_same<Params, FwdParams>::value>(p.t.grid, p.split, 0), dim3(threads), smem, s, 1, true, q, k, v, p);
 }
 template <bool WIN>
 cudaError_t launch_fwd(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const With<FwdParams, WIN>& p, bool one_tile, cudaStream_t s) {
@@ -2143,17 +2198,16 @@ cudaError_t launch_dq(const CUtensorMap& q, const CUtensorMap& k, const CUtensor
   static std::atomic<uint64_t> devices;
   const cudaError_t e = allow_shared_memory(devices, reinterpret_cast<const void*>(&attn_dq_kernel<DB, SPLIT, WIN>), Dq<DB>::SMEM);
   if (e != cudaSuccess) return e;
-  return launch_chained(attn_dq_kernel<DB, SPLIT, WIN>, dim3(static_cast<unsigned>(blocks_of(p.t.grid, p.split))), dim3(BWD_THREADS), Dq<DB>::SMEM, s, 1, true,
-                        q, k, v, g, p);
+  return launch_chained(attn_dq_kernel<DB, SPLIT, WIN>, grid_of<WIN>(p.t.grid, p.split, 0), dim3(BWD_THREADS), Dq<DB>::SMEM, s, 1, true, q, k, v, g, p);
 }
 template <int DB, bool SPLIT, bool WIN>
 cudaError_t launch_dkv(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& g, const DkvWith<WIN>& p, cudaStream_t s) {
   static std::atomic<uint64_t> devices;
   const cudaError_t e = allow_shared_memory(devices, reinterpret_cast<const void*>(&attn_dkv_kernel<DB, SPLIT, WIN>), Dkv<DB>::SMEM);
   if (e != cudaSuccess) return e;
-  long long blocks = blocks_of(p.t.grid, p.split);
-  if constexpr (WIN) blocks += 1ll * p.sinks.units * p.sinks.parts;
-  return launch_chained(attn_dkv_kernel<DB, SPLIT, WIN>, dim3(static_cast<unsigned>(blocks)), dim3(BWD_THREADS), Dkv<DB>::SMEM, s, 1, true, q, k, v, g, p);
+  uint32_t first = 0;
+  if constexpr (WIN) first = p.sinks.first;
+  return launch_chained(attn_dkv_kernel<DB, SPLIT, WIN>, grid_of<WIN>(p.t.grid, p.split, first), dim3(BWD_THREADS), Dkv<DB>::SMEM, s, 1, true, q, k, v, g, p);
 }
 template <int DB>
 cudaError_t launch_dq(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& g, const Windowed<DqParams>& p, bool window,
@@ -2238,7 +2292,7 @@ cudaError_t attention_bwd(const AttnShape& p, const AttnTensor& q, const AttnTen
   b.win = a.win;
   a.split = scratch ? query_parts(p, a.t.grid) : Parts{0, 0};
   a.sums = scratch;
-  b.sinks = scratch ? sink_tiles(p) : SinkTiles{0, 1, 0};
+  b.sinks = scratch ? sink_tiles(p) : SinkTiles{0, 1, 0, 0};
   b.split = scratch && b.sinks.parts == 0 ? key_parts(p, b.t.grid) : Parts{0, 0};
   const long long rows_q = part_rows(a.t.grid, a.split), rows_k = part_rows(b.t.grid, b.split);
   // (the parts of dQ have been added up where those of dK and dV begin)
