@@ -64,7 +64,7 @@ bool plain(std::initializer_list<const Tensor*> ts) {
   return true;
 }
 
-// Launches of backward passes, which autograd runs in threads of its own
+// Launches of backward passes, which autograd runs in threads of its own, and of calls that nobody counts from outside
 std::atomic<int64_t> background{0};
 struct Backward {
   int64_t before = mkh::launches();
@@ -558,6 +558,7 @@ struct AttentionOp {
 // (o; nothing where the tensors are not for kernels)
 OptTensor attention(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& offsets, bool causal, double scale, int64_t left, int64_t right,
                     int64_t sinks) {
+  const Backward count;
   const Tensor at = value(offsets);
   if (!plain({&q, &k, &v, &at})) return {};
   const bool train = records({&q, &k, &v});
@@ -605,6 +606,7 @@ struct AttentionQkvOp {
 
 OptTensor attention_qkv(const Tensor& qkv, int64_t heads, int64_t kv_heads, const OptTensor& offsets, bool causal, double scale, int64_t left, int64_t right,
                         int64_t sinks) {
+  const Backward count;
   const Tensor at = value(offsets);
   if (!plain({&qkv, &at})) return {};
   const bool train = records({&qkv});
@@ -845,9 +847,43 @@ variable_list rotary_pass(const Tensor& q, const Tensor& k, const Tensor (&w)[2]
 // (results; nothing where the tensors are not for kernels)
 variable_list rotary(const Tensor& q, const OptTensor& k, const OptTensor& qw, const OptTensor& kw, const OptTensor& qb, const OptTensor& kb,
                      const OptTensor& positions, const RotaryPlan& plan, int64_t norm, double eps, bool inverse) {
+  const Backward count;
   const Tensor keys = value(k), w[2] = {value(qw), value(kw)}, b[2] = {value(qb), value(kb)}, at = value(positions);
   if (!plain({&q, &keys, &w[0], &w[1], &b[0], &b[1], &at})) return {};
   return rotary_pass(q, keys, w, b, at, plan.numbers, norm, eps, inverse);
+}
+
+// The same for queries (and keys) [B, N, heads, D] or packed [T, heads, D]; nothing where the arguments are not for kernels either, or wrong: the caller looks closer then
+variable_list rotary_call(const Tensor& q, const OptTensor& k, const OptTensor& qw, const OptTensor& kw, const OptTensor& qb, const OptTensor& kb,
+                          const OptTensor& positions, const RotaryPlan& plan, int64_t norm, double eps, bool inverse) {
+  const bool packed = q.dim() == 3;
+  if (!q.is_cuda() || !native_type(q) || !(packed || q.dim() == 4) || norm < 0 || norm > 2 || !(eps >= 0.0)) return {};
+  const int64_t D = q.size(-1);
+  if (D < 8 || D > mk::ROT_WIDTH || D % 8) return {};
+  const auto device = q.device();
+  if (k.has_value()) {
+    if (k->dim() != q.dim() || k->scalar_type() != q.scalar_type() || k->device() != device) return {};
+    for (int64_t d = 0; d < q.dim(); ++d)
+      if (d != q.dim() - 2 && k->size(d) != q.size(d)) return {};
+  }
+  for (const OptTensor* t : {&qw, &kw, &qb, &kb})
+    if (t->has_value() && (norm == 0 || (*t)->dim() != 1 || (*t)->size(0) != D || (*t)->device() != device || !(*t)->is_floating_point())) return {};
+  const double* const numbers = plan.numbers.data_ptr<double>();
+  const int64_t axes = static_cast<int64_t>(numbers[1]);
+  if (positions.has_value() != (axes > 0)) return {};
+  OptTensor at = positions;
+  if (axes > 0) {
+    const Tensor& t = *positions;
+    const auto type = t.scalar_type();
+    if (t.device() != device || t.requires_grad() || (type != at::kInt && type != at::kLong && type != at::kFloat && type != at::kDouble)) return {};
+    const bool shared = t.dim() == 2, own = !packed && t.dim() == 3 && t.size(0) == q.size(0);
+    if (!(shared || own) || t.size(-1) != axes || t.size(-2) != q.size(-3) || 2 * (plan.numbers.numel() - 2 - axes) > D) return {};
+    if (!t.is_contiguous()) at = t.contiguous();
+  }
+  if (!packed) return rotary(q, k, qw, kw, qb, kb, at, plan, norm, eps, inverse);
+  variable_list out = rotary(q.unsqueeze(0), k.has_value() ? OptTensor(k->unsqueeze(0)) : k, qw, kw, qb, kb, at, plan, norm, eps, inverse);
+  for (Tensor& t : out) t = t.squeeze(0);
+  return out;
 }
 
 // A fused projection's queries and keys normed and turned, then attention: one tensor for both, the gradient of the projection written as one
@@ -893,6 +929,7 @@ struct RotaryAttentionOp {
 OptTensor rotary_attention_qkv(const Tensor& qkv, int64_t heads, int64_t kv_heads, const OptTensor& qw, const OptTensor& kw, const OptTensor& qb,
                                const OptTensor& kb, const OptTensor& positions, const OptTensor& offsets, const RotaryPlan& plan, int64_t norm, double eps,
                                bool causal, double scale, int64_t left, int64_t right, int64_t sinks) {
+  const Backward count;
   const Tensor w[2] = {value(qw), value(kw)}, b[2] = {value(qb), value(kb)}, at = value(positions), off = value(offsets);
   if (!plain({&qkv, &w[0], &w[1], &b[0], &b[1], &at, &off})) return {};
   const bool train = records({&qkv, &w[0], &w[1], &b[0], &b[1]});
@@ -1017,11 +1054,22 @@ Tensor dropout_run(const Tensor& x, const Tensor& residual, const Tensor& seed, 
 }
 
 OptTensor dropout(const Tensor& x, const OptTensor& residual, const OptTensor& seed, double p, bool out_f32) {
+  const Backward count;
   const Tensor r = value(residual), s = value(seed);
   if (!plain({&x, &r, &s})) return {};
   MK_CHECK(x.is_cuda() && native_type(x) && (!r.defined() || (native_type(r) && r.device() == x.device() && r.sizes() == x.sizes())),
            "dropout: bf16 or fp32 CUDA tensors of one shape expected");
   return dropout_run(x, r, s, p, out_f32);
+}
+
+// The same; nothing where the arguments are not for the kernel either, or wrong
+OptTensor dropout_call(const Tensor& x, const OptTensor& residual, const OptTensor& seed, double p) {
+  if (!x.is_cuda() || !native_type(x) || !(p >= 0.0 && p <= 1.0)) return {};
+  const auto device = x.device();
+  if (residual.has_value() && (!native_type(*residual) || residual->device() != device || residual->sizes() != x.sizes())) return {};
+  if (seed.has_value() && (seed->scalar_type() != at::kLong || seed->dim() != 1 || seed->size(0) != 2 || seed->device() != device)) return {};
+  const OptTensor dense = seed.has_value() && !seed->is_contiguous() ? OptTensor(seed->contiguous()) : seed;
+  return dropout(x, residual, dense, p, is_f32(x) || (residual.has_value() && is_f32(*residual)));
 }
 
 }  // namespace
@@ -1040,6 +1088,8 @@ void bind_tokens(pybind11::module_& m) {
   pybind11::class_<RotaryPlan>(m, "RotaryPlan")
       .def(pybind11::init<const std::vector<int64_t>&, const std::vector<double>&, bool>());
   m.def("rotary", &rotary, Free());
+  m.def("rotary_call", &rotary_call, Free());
+  m.def("dropout_call", &dropout_call, Free());
   m.def("rotary_attention_qkv", &rotary_attention_qkv, Free());
   m.def("dropout", &dropout, Free());
 }

@@ -60,12 +60,14 @@ def available() -> bool:
 # number of kernel-launching calls into this extension by the current process (the column sums launch a second kernel)
 LAUNCHES = 0
 _NON_KERNEL = {"read_error_flag", "clear_error_flag", "lp_scratch_floats", "adam_entry_bytes", "peer_alloc", "peer_open",
-               "peer_close", "peer_free", "tensor_from_ptr", "set_gelu_tanh", "stream_state", "launches", "background_launches", "RotaryPlan"}
+               "peer_close", "peer_free", "tensor_from_ptr", "set_gelu_tanh", "stream_state", "launches", "background_launches", "RotaryPlan",
+               # token operators, whose launches the extension counts itself
+               "attention", "attention_qkv", "rotary", "rotary_call", "rotary_attention_qkv", "dropout", "dropout_call"}
 
 
 # passes over whole layers, which count their launches themselves
 _LAYERS = {"conv_forward", "conv_backward", "mlp_forward", "mlp_backward", "norm_forward", "norm_backward", "spectral_forward",
-           "spectral_backward", "afno_forward", "afno_backward", "layer_norm", "attention", "attention_qkv", "rotary", "rotary_attention_qkv", "dropout"}
+           "spectral_backward", "afno_forward", "afno_backward", "layer_norm"}
 
 
 class _Counting:
@@ -94,6 +96,7 @@ class _Counting:
                     LAUNCHES += 1
                     return __raw(*args, **kwargs)
             self._cache[name] = fn
+            self.__dict__[name] = fn      # (found without a call from now on)
         return fn
 
 
@@ -102,6 +105,8 @@ _PROXY = None
 
 def require():
     global _PROXY
+    if _PROXY is not None:
+        return _PROXY
     _load()
     if _MOD is None:
         raise RuntimeError(

@@ -20,8 +20,6 @@ import torch
 
 from . import _ext
 
-_TYPES = (torch.bfloat16, torch.float32)
-
 
 def _check(x, p, seed, residual=None):
     if not x.dtype.is_floating_point:
@@ -56,32 +54,37 @@ def _dropped_torch(x, p, seed):
     return torch.where(keep, x.to(t) / (1.0 - p) if p < 1.0 else x.to(t), torch.zeros((), dtype=t, device=x.device))
 
 
-def _native(x, residual, seed, p) -> bool:
-    return (_ext.native() and x.is_cuda and x.dtype in _TYPES and (residual is None or residual.dtype in _TYPES) and round(p * 2 ** 32) >= 1
-            and not torch.compiler.is_compiling())
+def _kernel(x, residual, p, seed):
+    """The result where the tensors are for the kernel and the arguments are in order (the extension looks at them); else None."""
+    if not (_ext.native() and x.is_cuda) or torch.compiler.is_compiling():
+        return None
+    return _ext.require().dropout_call(x, residual, seed, p)
+
+
+LEAST = 2.0 ** -33          # p that rounds to no word of 2^32
 
 
 def dropout(x: torch.Tensor, p: float = 0.5, training: bool = True, seed: Optional[torch.Tensor] = None) -> torch.Tensor:
     """x / (1 - p) where an element is kept, zero where it is dropped; x itself where nothing is to be dropped."""
-    _check(x, p, seed)
-    if not training or round(p * 2 ** 32) < 1:
-        return x
-    if _native(x, None, seed, p):
-        y = _ext.require().dropout(x, None, None if seed is None else seed.contiguous(), float(p), x.dtype is torch.float32)
-        if y is not None:      # (None: the call is a transform's, a trace's or a mode's)
+    if training and p > LEAST:
+        y = _kernel(x, None, p, seed)
+        if y is not None:      # (None: the call is a transform's, a trace's or a mode's, too)
             return y
+    _check(x, p, seed)
+    if not training or p <= LEAST:
+        return x
     return _dropped_torch(x, p, seed).to(x.dtype)
 
 
 def dropout_add(x: torch.Tensor, residual: torch.Tensor, p: float = 0.5, training: bool = True, seed: Optional[torch.Tensor] = None) -> torch.Tensor:
     """dropout(x) + residual, in the wider of their types, rounded once; one pass over memory in either direction."""
-    _check(x, p, seed, residual)
-    t = torch.promote_types(x.dtype, residual.dtype)
-    if not training or round(p * 2 ** 32) < 1:
-        return x + residual
-    if _native(x, residual, seed, p):
-        y = _ext.require().dropout(x, residual, None if seed is None else seed.contiguous(), float(p), t is torch.float32)
+    if training and p > LEAST:
+        y = _kernel(x, residual, p, seed)
         if y is not None:
             return y
+    _check(x, p, seed, residual)
+    if not training or p <= LEAST:
+        return x + residual
+    t = torch.promote_types(x.dtype, residual.dtype)
     wide = torch.promote_types(t, torch.float32)
     return (_dropped_torch(x.to(wide), p, seed) + residual.to(wide)).to(t)

@@ -181,19 +181,25 @@ def _torch(x, weight, bias, positions, axes, eps, norm, inverse=False):
 
 # ---------------------------------------------------------------------------------------------------- operators
 
+def _kernels(q, k, qw, kw, qb, kb, positions, axes, eps, norm, inverse=False):
+    """Results where the tensors are for the kernels and the arguments are in order (the extension looks at them: half of a small call's time went into doing so
+    here); else an empty list."""
+    if not (_ext.native() and q.is_cuda) or torch.compiler.is_compiling():
+        return []
+    return _ext.require().rotary_call(q, k, qw, kw, qb, kb, positions, _no_axes() if axes is None else axes.native(), NORMS.get(norm, -1), eps, inverse)
+
+
 def _run(q, k, qw, kw, qb, kb, positions, axes, eps, norm, inverse=False):
-    """Results of one or two tensors whose arguments are checked."""
-    if _native(q, q.shape[-1]):
-        packed = q.dim() == 3
-        views = [t if t is None or not packed else t[None] for t in (q, k)]
-        out = _ext.require().rotary(*views, qw, kw, qb, kb, positions, _no_axes() if axes is None else axes.native(), NORMS[norm], eps, inverse)
-        if out:      # (nothing: the call is a transform's, a trace's or a mode's)
-            return [t[0] if packed else t for t in out]
+    """Results of one or two tensors whose arguments are checked, in torch's operations."""
     return [_torch(t, w, b, positions, axes, eps, norm, inverse) for t, w, b in ((q, qw, qb), (k, kw, kb)) if t is not None]
 
 
 def rotary(x: torch.Tensor, positions: torch.Tensor, axes: RotaryAxes, inverse: bool = False) -> torch.Tensor:
     """x [B, N, heads, D] (or [T, heads, D]) turned by its positions, or back with `inverse`; dense, in the type of x."""
+    if positions is not None:
+        out = _kernels(x, None, None, None, None, None, positions, axes, 0.0, None, bool(inverse))
+        if out:
+            return out[0]
     _check_heads(x)
     positions = _check_positions(positions, axes, x.shape[:-2], x.shape[-1], x.device)
     if positions is None:
@@ -203,6 +209,10 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, axes: RotaryAxes, inverse: 
 
 def rotary_qk(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, axes: RotaryAxes) -> Tuple[torch.Tensor, torch.Tensor]:
     """Queries [.., H, D] and keys [.., Hk, D] of the same tokens turned by their positions, in one launch."""
+    if positions is not None:
+        out = _kernels(q, k, None, None, None, None, positions, axes, 0.0, None)
+        if out:
+            return out[0], out[1]
     _check_heads(q, k)
     positions = _check_positions(positions, axes, q.shape[:-2], q.shape[-1], q.device)
     if positions is None:
@@ -215,6 +225,9 @@ def norm_rotary_qk(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Te
                    k_bias: Optional[torch.Tensor] = None, eps: float = 1e-5, norm: str = "layer") -> Tuple[torch.Tensor, torch.Tensor]:
     """Queries and keys normed over the channels of every head, then turned, in one pass: `norm` "layer" is (x - mean) / sqrt(var + eps) (biased variance),
     "rms" x / sqrt(mean(x^2) + eps), times weight plus bias ([D] each, or None).  Without positions the norm alone."""
+    out = _kernels(q, k, q_weight, k_weight, q_bias, k_bias, positions, axes, float(eps), norm)
+    if out and norm is not None:
+        return out[0], out[1]
     _check_heads(q, k)
     D = q.shape[-1]
     positions = _check_positions(positions, axes, q.shape[:-2], D, q.device)
@@ -246,5 +259,6 @@ def rotary_attention_qkv(qkv: torch.Tensor, num_heads: int, num_kv_heads: Option
         if o is not None:
             return o[0] if packed else o
     q, k, v = qkv.unflatten(-1, (num_heads + 2 * Hk, D)).split([num_heads, Hk, Hk], dim=-2)
-    q, k = _run(q, k, q_weight, k_weight, q_bias, k_bias, positions, axes, float(eps), norm)
+    # (on the kernels still, where only attention has none: heads of 136 channels, fp32)
+    q, k = _kernels(q, k, q_weight, k_weight, q_bias, k_bias, positions, axes, float(eps), norm) or _run(q, k, q_weight, k_weight, q_bias, k_bias, positions, axes, float(eps), norm)
     return attn_ops.attention(q, k, v, causal, scale, offsets, window, sinks)
