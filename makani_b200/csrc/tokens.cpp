@@ -577,6 +577,27 @@ OptTensor attention(const Tensor& q, const Tensor& k, const Tensor& v, const Opt
   return o;
 }
 
+// The same for [B, N, heads, D], or packed [T, heads, D] with offsets; nothing where the arguments are not for kernels as they are either, or wrong
+OptTensor attention_call(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& offsets, bool causal, std::optional<double> scale, int64_t left,
+                         int64_t right, int64_t sinks) {
+  const bool packed = offsets.has_value();
+  const int64_t dim = packed ? 3 : 4;
+  auto fits = [&](const Tensor& t) { return t.is_cuda() && t.scalar_type() == at::kBFloat16 && t.dim() == dim && t.device() == q.device(); };
+  if (!fits(q) || !fits(k) || !fits(v) || k.sizes() != v.sizes() || sinks < 0) return {};
+  for (int64_t d = 0; d < dim; ++d)
+    if (d != dim - 2 && k.size(d) != q.size(d)) return {};
+  const int64_t H = q.size(-2), Hk = k.size(-2), D = q.size(-1);
+  if (H < 1 || Hk < 1 || H % Hk || D < 8 || D % 8 || D > mk::ATTN_WIDTH) return {};
+  const double s = scale.has_value() ? *scale : 1.0 / std::sqrt(static_cast<double>(D));
+  if (!(s > 0.0) || !std::isfinite(s)) return {};
+  if (!packed) return attention(q, k, v, offsets, causal, s, left, right, sinks);
+  if (!offsets->is_cuda() || offsets->device() != q.device() || offsets->scalar_type() != at::kInt || offsets->dim() != 1 || offsets->size(0) < 1 ||
+      !offsets->is_contiguous())
+    return {};
+  const OptTensor o = attention(q.unsqueeze(0), k.unsqueeze(0), v.unsqueeze(0), offsets, causal, s, left, right, sinks);
+  return o.has_value() ? OptTensor(o->squeeze(0)) : o;
+}
+
 // The output of a fused projection: [B, N, (q heads | k heads | v heads) x D], dense; its gradient is written as one tensor
 struct Parts {
   Tensor q, k, v;
@@ -1089,6 +1110,7 @@ void bind_tokens(pybind11::module_& m) {
       .def(pybind11::init<const std::vector<int64_t>&, const std::vector<double>&, bool>());
   m.def("rotary", &rotary, Free());
   m.def("rotary_call", &rotary_call, Free());
+  m.def("attention_call", &attention_call, Free());
   m.def("dropout_call", &dropout_call, Free());
   m.def("rotary_attention_qkv", &rotary_attention_qkv, Free());
   m.def("dropout", &dropout, Free());

@@ -126,6 +126,11 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: bool = 
               offsets: Optional[torch.Tensor] = None, window: Window = None, sinks: int = 0) -> torch.Tensor:
     """softmax(scale q k^T) v per head: q [B, N, H, D], k and v [B, N, Hk, D], or packed [T, H, D] with `offsets`; the result is like q,
     dense.  `scale` defaults to D ** -0.5; `window` and `sinks` as above."""
+    if _ext.native() and q.is_cuda and (offsets is None or isinstance(offsets, torch.Tensor)) and not torch.compiler.is_compiling():
+        # (what is for the kernels and in order needs no closer look)
+        o = _ext.require().attention_call(q, k, v, offsets, causal, scale, *_check_window(window, sinks, causal))
+        if o is not None:
+            return o
     packed = offsets is not None
     if not (q.dim() == k.dim() == v.dim() == (3 if packed else 4)):
         raise ValueError(f"attention takes {'[T, heads, D] with' if packed else '[B, N, heads, D] without'} offsets, got {tuple(q.shape)}, "
