@@ -375,7 +375,9 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) rotary_kernel(const __grid_co
 #pragma unroll
         for (int q = 0; q < R; ++q) {
           const float mean = LAYER ? sums[q * EACH + (BACK ? 2 : 1)] * inv : 0.f;      // of the deviations
-          const float rstd = rsqrtf(fmaxf(fmaf(sums[q * EACH], inv, -mean * mean), 0.f) + s.eps);
+          float rstd = rsqrtf(fmaxf(fmaf(sums[q * EACH], inv, -mean * mean), 0.f) + s.eps);
+          // (what goes along with zeros has no deviation, and the reciprocal is infinite without eps)
+          if (BACK && !(live && (q == 0 || k + q < per_chunk))) rstd = 0.f;
           const f32x2 r2 = both(rstd), m2 = both(-mean);
 #pragma unroll
           for (int i = 0; i < 2; ++i) {

@@ -304,6 +304,27 @@ def test_norms_alone_and_parameters(gen, norm):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("norm", ["layer", "rms"])
+@pytest.mark.parametrize("N,H,Hk,D", [(37, 3, 1, 32), (1, 5, 5, 64), (131, 4, 3, 128), (9, 7, 2, 256)])
+def test_no_eps(gen, N, H, Hk, D, norm):
+    """Lanes that go along with zeros (behind the last token, head or sequence) have no standard deviation, and add nothing to the parameters' gradients."""
+    axes, at = rot.RotaryAxes((16, 16)), _grid(N, 2, "cuda")
+    q, k = (torch.randn(1, N, h, D, device="cuda", generator=gen).bfloat16() for h in (H, Hk))
+    _check(q, k, axes, at, norm, _params(D, "cuda", gen), eps=0.0)
+    if D > 128:
+        return
+    w = [torch.randn(D, device="cuda", generator=gen).requires_grad_() for _ in range(2)]
+    qkv = torch.randn(N + 5, (H + 2 * Hk * (H % Hk == 0) + 2 * (H % Hk != 0)) * D, device="cuda", generator=gen).bfloat16()
+    offsets, heads = torch.tensor([0, (N + 1) // 2, N], device="cuda", dtype=torch.int32), Hk if H % Hk == 0 else 1
+    run = lambda x, at: rot.rotary_attention_qkv(x, H, heads, at, axes, *w, eps=0.0, norm=norm, offsets=offsets)  # noqa: E731
+    o = run(qkv, _grid(N + 5, 2, "cuda"))
+    got = torch.autograd.grad(o, w, torch.ones_like(o))
+    o = run(qkv[:N], at)
+    want = torch.autograd.grad(o, w, torch.ones_like(o))
+    assert all(torch.isfinite(a).all() and torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.gpu
 def test_partial_gradients(gen):
     """One result used, frozen inputs or parameters, none of them."""
     axes, at = rot.RotaryAxes((16, 16)), _grid(50, 2, "cuda")
