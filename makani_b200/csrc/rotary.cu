@@ -6,10 +6,10 @@
 // and backward, g = dout turned by -a:   dw = sum g xh, db = sum g, dx = rstd (g w - mean(g w) - xh mean(g w xh)), the means of the layer norm alone.
 //
 // Bound by memory: a head's channels are read once and written once (x and dy in the backward pass), and mean and variance are computed again rather than kept.
-// A group of lanes has the channels of a head and goes over the heads of a token.  A lane has four pairs of channels, both of each, so that it turns them
-// without its neighbours: two runs of four channels (halves of a band), or eight side by side (neighbours).  (Eight side by side in either case, with partners
-// through shared memory: 37080 tokens, 16 heads of 128 with norms, both ways, 188 us where this took 175; 16200 tokens, 16 heads of 48 62 / 54.)  Angles are computed once for a
-// token's heads, in 64 bits down to the fraction of a turn (the angle of position 100000 in 32 bits would be off by 4e-3).  Statistics, sums and gradients of
+// A group of lanes has the channels of a head and goes over the heads of a token; what comes next, of whichever token, is copied to shared memory meanwhile.  A lane
+// has four pairs of channels, both of each, so that it turns them without its neighbours: two runs of four channels (halves of a band), or eight side by side
+// (neighbours).  (Eight side by side in either case, and partners fetched from their lanes: 37080 tokens, 16 heads of 128 with norms, both ways, 188 us where this took
+// 175 then; 16200 tokens, 16 heads of 48 62 / 54.)  Angles are computed once for a token's heads, in 64 bits down to the fraction of a turn (the angle of position 100000 in 32 bits would be off by 4e-3).  Statistics, sums and gradients of
 // weights are fp32; blocks leave one row of partial sums each, added up in a fixed order by a second launch.
 #include "rotary.cuh"
 
@@ -26,6 +26,9 @@ namespace mk {
 namespace {
 
 constexpr int THREADS = 256, WARPS = THREADS / 32;
+// Steps of heads in the ring: two on their way beside the one that is computed.  us, two / three / four, rotation of 16200 tokens, 24 heads of 64, both ways, 52 / 42 /
+// 41; 37080 tokens, 16 heads of 128 with norms, 154 / 150 / 153.  (The next heads in registers, and none of the next token's: 44, 166.)
+constexpr int STAGES = 3;
 
 struct KernelParams {
   RotShape s;
@@ -154,6 +157,20 @@ struct Channels {
     raw.set(RUN == 0 ? pairs : runs);
   }
 };
+// Eight values to shared memory, zeros where not `in`, as a copy that goes on beside the thread
+template <typename T>
+__device__ __forceinline__ void copy8(T* to, const T* from, bool in) {
+  const uint32_t at = static_cast<uint32_t>(__cvta_generic_to_shared(to));
+#pragma unroll
+  for (uint32_t i = 0; i < sizeof(T) / 2; ++i)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at + 16 * i), "l"(reinterpret_cast<const uint8_t*>(from) + 16 * i), "r"(in ? 16 : 0)
+                 : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
 __device__ __forceinline__ f32x2 both(float v) { return f2_pack(v, v); }
 __device__ __forceinline__ float sum_of(const f32x2 (&a)[2], const f32x2 (&b)[2]) {
   float x, y;
@@ -192,7 +209,10 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) rotary_kernel(const __grid_co
   constexpr int GROUPS = 32 / LANES, ROW = LANES * 8;
   constexpr bool NORMED = NORM != ROT_NORM_NONE, READ_X = NORMED || !BACK, SUMS = BACK && NORMED, LAYER = NORM == ROT_NORM_LAYER;
   const RotShape& s = p.s;
+  constexpr int VALUES = READ_X && BACK ? 2 : 1;
   __shared__ __align__(16) double turns[ROW / 2];      // of every pair per unit of position
+  extern __shared__ __align__(16) uint8_t ring_raw[];  // [STAGES][VALUES][R][WARPS][32 x 8]: steps that are on their way
+  T* const ring = reinterpret_cast<T*>(ring_raw);
   const int which = blockIdx.x < static_cast<unsigned>(p.blocks0) ? 0 : 1;
   const RotPart& part = s.part[which];
   const T *x = static_cast<const T*>(part.x.ptr), *dy = static_cast<const T*>(part.dy.ptr);
@@ -251,53 +271,91 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) rotary_kernel(const __grid_co
   const unsigned units = limit > 0 ? static_cast<unsigned>(s.B) * s.N * chunks : 0u;      // (below 2^31)
   const int block = which ? blockIdx.x - p.blocks0 : blockIdx.x, blocks = which ? p.blocks - p.blocks0 : p.blocks0;
   const unsigned step = static_cast<unsigned>(blocks) * WARPS * GROUPS;
-  // (the groups of a warp go through the loop together)
-  for (unsigned first = (static_cast<unsigned>(block) * WARPS + warp) * GROUPS; first < units; first += step) {
-    const unsigned u = min(first + group, units - 1), t = chunks == 1 ? u : u / chunks;
-    const int chunk = static_cast<int>(u - t * chunks), bat = s.B == 1 ? 0 : static_cast<int>(t / s.N);
-    const int n = static_cast<int>(t - static_cast<unsigned>(bat) * s.N), h0 = chunk * per_chunk;
+  // A unit: its sample, token and first head; whether the group has something to do there
+  struct Unit {
+    int bat, n, h0;
+    bool live;
+  };
+  auto unit_of = [&](unsigned first) {
     // (a group behind the last unit or the limit goes along with zeros)
-    const bool live = mine && first + group < units && (!BACK || n < limit);
-    const T* x_at = READ_X ? x + bat * part.x.batch + n * part.x.token + h0 * part.x.head + offset : nullptr;
-    const T* d_at = BACK ? dy + bat * part.dy.batch + n * part.dy.token + h0 * part.dy.head + offset : nullptr;
-    T* o_at = static_cast<T*>(part.out.ptr) + bat * part.out.batch + n * part.out.token + h0 * part.out.head + offset;
-
-    Channels<T, RUN> vx[READ_X ? R : 1], vd[BACK ? R : 1];
-    auto fetch = [&](int k) {
+    const unsigned u = min(first + group, units - 1), t = chunks == 1 ? u : u / chunks;
+    Unit a;
+    a.h0 = static_cast<int>(u - t * chunks) * per_chunk;
+    a.bat = s.B == 1 ? 0 : static_cast<int>(t / s.N);
+    a.n = static_cast<int>(t - static_cast<unsigned>(a.bat) * s.N);
+    a.live = mine && first + group < units && (!BACK || a.n < limit);
+    return a;
+  };
+  auto start_of = [&](const RotTensor& t, const Unit& u) { return u.bat * t.batch + u.n * t.token + u.h0 * t.head; };
+  // Steps are fetched STAGES - 1 ahead, whatever unit they are of: all lanes of a warp fetch eight channels side by side and read their pairs behind the wait
+  const unsigned begin = (static_cast<unsigned>(block) * WARPS + warp) * GROUPS;
+  unsigned ahead = begin;
+  int ahead_k = 0, ahead_stage = 0;
+  bool ahead_live = false;
+  const T *x_from = nullptr, *d_from = nullptr;
+  auto slot = [&](int stage, int value, int q) { return ring + (((stage * VALUES + value) * R + q) * WARPS + warp) * (32 * 8); };
+  auto enter = [&](const Unit& u) {
+    ahead_live = u.live;
+    if constexpr (READ_X) x_from = x + start_of(part.x, u) + (mine ? 8 * l : 0);
+    if constexpr (BACK) d_from = dy + start_of(part.dy, u) + (mine ? 8 * l : 0);
+  };
+  auto fetch = [&] {
+    if (ahead < units) {
 #pragma unroll
       for (int q = 0; q < R; ++q) {
-        const bool in = q == 0 || k + q < per_chunk;
+        const bool in = ahead_live && (q == 0 || ahead_k + q < per_chunk);
         if constexpr (READ_X) {
-          if (in && live) vx[q].load(x_at, place);
-          x_at += part.x.head;
+          copy8(slot(ahead_stage, 0, q) + lane * 8, in ? x_from : x, in);
+          x_from += part.x.head;
         }
         if constexpr (BACK) {
-          if (q > 0 && !in) vd[q].raw.clear();      // (it would be added to the sums)
-          if (in && live) vd[q].load(d_at, place);
-          d_at += part.dy.head;
+          copy8(slot(ahead_stage, VALUES - 1, q) + lane * 8, in ? d_from : dy, in);
+          d_from += part.dy.head;
         }
       }
-    };
-#pragma unroll
-    for (int q = 0; q < R; ++q) {
-      if constexpr (READ_X) vx[q].raw.clear();
-      if constexpr (BACK) vd[q].raw.clear();
+      ahead_k += R;
+      if (ahead_k >= per_chunk) {
+        ahead_k = 0;
+        ahead += step;
+        if (ahead < units) enter(unit_of(ahead));
+      }
+      ahead_stage = ahead_stage + 1 == STAGES ? 0 : ahead_stage + 1;
     }
-    fetch(0);
+    copies_commit();
+  };
+  Unit next{};
+  if (begin < units) {
+    next = unit_of(begin);
+    enter(next);
+  }
+#pragma unroll
+  for (int i = 0; i < STAGES - 1; ++i) fetch();
+  int stage = 0;
+  // (positions of the next unit are on their way, too)
+  double at[RUN == 4 ? 1 : 4] = {};
+  auto fetch_positions = [&](const Unit& u) {
+    if (!positions) return;
+    const long long from = u.bat * s.position_batch + 1ll * u.n * s.axes;
+#pragma unroll
+    for (int i = 0; i < (RUN == 4 ? 1 : 4); ++i) at[i] = position_of(positions, s.position_type, from + (axes >> 8 * i & 255));
+  };
+  if (begin < units) fetch_positions(next);
+  // (the groups of a warp go through the loop together)
+  for (unsigned first = begin; first < units; first += step) {
+    const Unit unit = next;
+    const bool live = unit.live;
+    T* o_at = static_cast<T*>(part.out.ptr) + start_of(part.out, unit) + offset;
 
     // angles of the lane's pairs
     f32x2 cs[2], sn[2], neg[2];
     {
       float c[4], d[4];
-      const long long from = bat * s.position_batch + 1ll * n * s.axes;
-      double at = positions ? position_of(positions, s.position_type, from + (axes & 255)) : 0.0;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         c[i] = 1.f;
         d[i] = 0.f;
         if (positions) {
-          if (RUN != 4 && i > 0) at = position_of(positions, s.position_type, from + (axes >> 8 * i & 255));
-          const double v = at * turns[4 * l + i];
+          const double v = at[RUN == 4 ? 0 : i] * turns[4 * l + i];
           sine_cosine<T>(static_cast<float>(v - rint(v)), d[i], c[i]);
           if (BACK != (s.inverse != 0)) d[i] = -d[i];
         }
@@ -317,15 +375,26 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) rotary_kernel(const __grid_co
       }
     }
 
+    if (first + step < units) {
+      next = unit_of(first + step);
+      fetch_positions(next);
+    }
     // (all groups of the warp make as many turns)
     for (int k = 0; k < per_chunk; k += R) {
+      copies_wait<STAGES - 2>();
+      __syncwarp();      // (what other lanes fetched is here, and they have read what the next step is fetched to)
+      fetch();
       Channels<T, RUN> now[READ_X ? R : 1], now_d[BACK ? R : 1];
 #pragma unroll
       for (int q = 0; q < R; ++q) {
-        if constexpr (READ_X) now[q] = vx[q];
-        if constexpr (BACK) now_d[q] = vd[q];
+        if constexpr (READ_X) now[q].load(slot(stage, 0, q) + group * ROW + offset, place);
+        if constexpr (BACK) now_d[q].load(slot(stage, VALUES - 1, q) + group * ROW + offset, place);
+        if (NORMED && !mine) {
+          now[q].raw.clear();
+          if constexpr (BACK) now_d[q].raw.clear();
+        }
       }
-      if (k + R < per_chunk) fetch(k + R);
+      stage = stage + 1 == STAGES ? 0 : stage + 1;
       auto put = [&](int q, const f32x2 (&lo)[2], const f32x2 (&hi)[2]) {
         Channels<T, RUN> out;
         out.set(lo, hi);
@@ -468,16 +537,15 @@ int lanes_of(int D) { return D <= 64 ? 8 : D <= 128 ? 16 : 32; }
 // Blocks and shares of heads.  A unit is a token with all heads of a part, so that its angles are computed once; with fewer units than threads that the device
 // holds, heads are shared out, four at least to a unit.
 constexpr int LEAST_HEADS = 4;
-// Blocks to an SM and heads at a time (bf16; half of them in fp32): what carries them is how many bytes are on their way.  us by (heads, blocks): rotation of 16200
-// tokens, 24 heads of 64, (4, 3) 20.7, (4, 4) 21.4, (2, 4) 20.8, (6, 2) 20.4, (2, 6) 40.6; with norms, 37080 tokens, 16 heads of 128, (4, 2) 61.4, (2, 3) 69.9,
-// (2, 4) 70.7, (1, 4) 73.1, (1, 5) 83.9, (2, 2) 73.8 (DRAM 46.5); their gradients (2, 2) 105, (1, 3) 128, (1, 2) 127, (2, 3), 508 bytes a thread spilled, 196
-// (DRAM 69.7).
-constexpr int blocks_per_sm(int norm, bool) { return norm == ROT_NORM_NONE ? 3 : 2; }
+// Blocks to an SM and heads at a time (bf16; half of them in fp32).  us by (heads, blocks): rotation of 16200 tokens, 24 heads of 64, (4, 3) 18.4, (2, 4) 18.3, (6, 2)
+// 19.4, (6, 3) 20.1, (2, 5) 25.0, 15.2 of it memory; 9113 tokens, 20 heads of 96, both ways, (4, 3) 39.7, (2, 4) 42.2, (6, 2) 45.4; with norms, 37080 tokens, 16
+// heads of 128, (4, 2) 59.6, (2, 3) 61.9, (2, 2) 62.7, (4, 3), which spills, 74.4 (memory 46.5); their gradients (2, 2) 90, (1, 3) 113 (memory 69.7).
+constexpr int blocks_per_sm(int norm) { return norm == ROT_NORM_NONE ? 3 : 2; }
 constexpr int heads_at_a_time(int norm, bool back, bool half) { return (norm != ROT_NORM_NONE && back ? 2 : 4) / (half ? 1 : 2); }
-void plan(KernelParams& k, bool back) {
+void plan(KernelParams& k) {
   const RotShape& s = k.s;
   const int per_block = WARPS * (32 / lanes_of(s.D));
-  const long long most = 1ll * blocks_per_sm(s.norm, back) * sm_count(), tokens = 1ll * s.B * s.N;
+  const long long most = 1ll * blocks_per_sm(s.norm) * sm_count(), tokens = 1ll * s.B * s.N;
   int heads = 0;
   for (int i = 0; i < s.parts; ++i) heads += s.part[i].heads;
   long long blocks[2] = {0, 0};
@@ -521,12 +589,17 @@ int run_of(const RotShape& s) {
 
 template <typename T, int LANES, int NORM, bool BACK>
 cudaError_t by_run(const KernelParams& k, cudaStream_t s) {
-  constexpr int R = heads_at_a_time(NORM, BACK, sizeof(T) == 2), BLOCKS = blocks_per_sm(NORM, BACK);
-  auto go = [&](auto* kernel) { return launch_chained(kernel, dim3(k.blocks), dim3(THREADS), 0, s, 1, true, k); };
+  constexpr int R = heads_at_a_time(NORM, BACK, sizeof(T) == 2), BLOCKS = blocks_per_sm(NORM);
+  static std::atomic<uint64_t> devices[3];
+  constexpr int BYTES = STAGES * (NORM != ROT_NORM_NONE && BACK ? 2 : 1) * R * THREADS * 8 * static_cast<int>(sizeof(T));
+  auto go = [&](auto* kernel, std::atomic<uint64_t>& of) {
+    const cudaError_t e = allow_shared_memory(of, reinterpret_cast<const void*>(kernel), BYTES);
+    return e != cudaSuccess ? e : launch_chained(kernel, dim3(k.blocks), dim3(THREADS), BYTES, s, 1, true, k);
+  };
   switch (run_of(k.s)) {
-    case 0: return go(rotary_kernel<T, LANES, NORM, BACK, 0, R, BLOCKS>);
-    case 4: return go(rotary_kernel<T, LANES, NORM, BACK, 4, R, BLOCKS>);
-    default: return go(rotary_kernel<T, LANES, NORM, BACK, 1, R, BLOCKS>);
+    case 0: return go(rotary_kernel<T, LANES, NORM, BACK, 0, R, BLOCKS>, devices[0]);
+    case 4: return go(rotary_kernel<T, LANES, NORM, BACK, 4, R, BLOCKS>, devices[1]);
+    default: return go(rotary_kernel<T, LANES, NORM, BACK, 1, R, BLOCKS>, devices[2]);
   }
 }
 template <typename T, int LANES, bool BACK>
@@ -552,14 +625,14 @@ cudaError_t rotary_fwd(const RotShape& p, cudaStream_t s) {
   if (!shape_ok(p, false)) return cudaErrorInvalidValue;
   KernelParams k{};
   k.s = p;
-  plan(k, false);
+  plan(k);
   return p.f32 ? by_width<float, false>(k, s) : by_width<__nv_bfloat16, false>(k, s);
 }
 
 long long rotary_scratch(const RotShape& p) {
   KernelParams k{};
   k.s = p;
-  plan(k, true);
+  plan(k);
   return 2ll * k.blocks * p.D;
 }
 
@@ -568,7 +641,7 @@ cudaError_t rotary_bwd(const RotShape& p, float* sums, int* launches, cudaStream
   if (!shape_ok(p, true)) return cudaErrorInvalidValue;
   KernelParams k{};
   k.s = p;
-  plan(k, true);
+  plan(k);
   bool asked = false;
   for (int i = 0; i < p.parts; ++i) asked = asked || p.part[i].dw;
   if (asked && (!p.norm || !sums)) return cudaErrorInvalidValue;
