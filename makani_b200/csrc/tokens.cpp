@@ -476,7 +476,6 @@ mk::AttnShape shape_of(const Tensor& q, const Tensor& k, const Tensor& v, const 
   const int64_t most = p.N, left = mask.left < 0 ? most : std::min(mask.left, most), right = mask.causal ? 0 : mask.right < 0 ? most : std::min(mask.right, most);
   MK_CHECK(mask.sinks >= 0, "attention: no negative number of sinks");
   p.window = left < most - 1 || (!mask.causal && right < most - 1);
-  MK_CHECK(!p.window || p.H < 65536, "attention: too many heads for a window");
   p.left = static_cast<int>(left);
   p.right = static_cast<int>(right);
   p.sinks = static_cast<int>(std::min(mask.sinks, most));

@@ -231,6 +231,22 @@ def test_packed_sinks_that_go_apart(gen, causal):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("B,N,H,Hk,window,sinks,causal", [(70001, 3, 1, 1, 1, 0, False), (66000, 4, 2, 1, (1, 1), 1, False), (70001, 5, 1, 1, 2, 0, True),
+                                                          (1, 70, 70001, 70001, 3, 0, False), (2, 5, 33000, 16500, 1, 2, True)])
+def test_many_sequences_and_heads(gen, B, N, H, Hk, window, sinks, causal):
+    """More of either than a grid has along y."""
+    q, k, v, do = _inputs(gen, B, N, H=H, Hk=Hk, D=8)
+    mask = dict(causal=causal, window=window, sinks=sinks)
+    got, G = _run(q, k, v, do, **mask), H // Hk
+    for b in {0, 1, 65534, 65535, 65536, B - 1} & set(range(B)):
+        for h in {0, 1, 65534, 65535, 65536, Hk - 1} & set(range(Hk)):
+            at = (slice(h * G, (h + 1) * G), slice(h, h + 1), slice(h, h + 1), slice(h * G, (h + 1) * G))
+            want, off = _oracle(*(t[b, :, a] for t, a in zip((q, k, v, do), at)), 8 ** -0.5, [(0, N)], **mask)
+            for n, a in zip(want, (at[0], at[0], at[1], at[1])):
+                _close(got[n][b, :, a], want[n], off[n], f"{n} of sample {b}, head {h}")
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("causal", [False, True])
 @pytest.mark.parametrize("B,N,H,Hk,D", [(32, 384, 8, 8, 64), (20, 440, 8, 2, 128), (160, 129, 1, 1, 24), (9, 1300, 8, 8, 48)])
 def test_short_sequences_of_several_tiles(gen, B, N, H, Hk, D, causal):
