@@ -62,7 +62,7 @@ LAUNCHES = 0
 _NON_KERNEL = {"read_error_flag", "clear_error_flag", "lp_scratch_floats", "adam_entry_bytes", "peer_alloc", "peer_open",
                "peer_close", "peer_free", "tensor_from_ptr", "set_gelu_tanh", "stream_state", "launches", "background_launches", "RotaryPlan",
                # token operators, whose launches the extension counts itself
-               "attention", "attention_call", "attention_qkv", "rotary", "rotary_call", "rotary_attention_qkv", "dropout", "dropout_call"}
+               "attention", "attention_call", "attention_qkv", "rotary", "rotary_call", "rotary_attention_qkv", "dropout_call"}
 
 
 # passes over whole layers, which count their launches themselves
