@@ -394,11 +394,25 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) rotary_kernel(const __grid_co
           if constexpr (BACK) now_d[q].raw.clear();
         }
       }
+      const int used = stage;
       stage = stage + 1 == STAGES ? 0 : stage + 1;
       auto put = [&](int q, const f32x2 (&lo)[2], const f32x2 (&hi)[2]) {
         Channels<T, RUN> out;
         out.set(lo, hi);
-        if (live && (q == 0 || k + q < per_chunk)) out.store(o_at, place);
+        const bool in = live && (q == 0 || k + q < per_chunk);
+        if constexpr (RUN == 1) {      // (eight channels side by side to a lane again, by way of the slot that all have read)
+          T* const at = slot(used, 0, q);
+          __syncwarp();
+          if (mine) out.store(at + group * ROW, place);
+          __syncwarp();
+          if (in) {
+            Vec8<T> v;
+            v.load(at + lane * 8);
+            v.store(o_at + 8 * l);
+          }
+        } else {
+          if (in) out.store(o_at, place);
+        }
         o_at += part.out.head;
       };
       if constexpr (!NORMED) {
