@@ -100,10 +100,11 @@ __device__ __forceinline__ Pair pair_of(const RotShape& s, int i, bool positions
   return {2 * i, 2 * i + 1, -1};
 }
 
-// How a lane's four pairs lie in memory: RUN 0: eight channels side by side, pairs are neighbours; 4: first and second channels in runs of four; 1: anyhow
+// How a lane's four pairs lie in memory: RUN 0: eight channels side by side, pairs are neighbours; 4: first and second channels in runs of four; 2: in runs of
+// two, those of the first two pairs, then those of the others; 1: anyhow
 template <int RUN>
 struct Place {
-  int at[RUN == 0 ? 1 : RUN == 4 ? 2 : 8];
+  int at[RUN == 0 ? 1 : RUN == 4 ? 2 : RUN == 2 ? 4 : 8];
 };
 // The channels of four pairs as they come from memory; first and second ones as two values each
 template <typename T, int RUN>
@@ -118,6 +119,14 @@ struct Channels {
     } else if constexpr (RUN == 4) {
       raw.a = *reinterpret_cast<const float4*>(p);
       raw.b = *reinterpret_cast<const float4*>(p + place.at[1]);
+    } else if constexpr (RUN == 2 && sizeof(T) == 2) {
+      auto two = [&](int i) { return *reinterpret_cast<const uint32_t*>(p + place.at[i]); };
+      raw.v = make_uint4(two(0), two(2), two(1), two(3));
+    } else if constexpr (RUN == 2) {
+      auto two = [&](int i) { return *reinterpret_cast<const float2*>(p + place.at[i]); };
+      const float2 a = two(0), b = two(2), c = two(1), d = two(3);
+      raw.a = make_float4(a.x, a.y, b.x, b.y);
+      raw.b = make_float4(c.x, c.y, d.x, d.y);
     } else {
       float v[8];
 #pragma unroll
@@ -134,6 +143,13 @@ struct Channels {
     } else if constexpr (RUN == 4) {
       *reinterpret_cast<float4*>(p) = raw.a;
       *reinterpret_cast<float4*>(p + place.at[1]) = raw.b;
+    } else if constexpr (RUN == 2 && sizeof(T) == 2) {
+      auto two = [&](int i) { return reinterpret_cast<uint32_t*>(p + place.at[i]); };
+      *two(0) = raw.v.x, *two(2) = raw.v.y, *two(1) = raw.v.z, *two(3) = raw.v.w;
+    } else if constexpr (RUN == 2) {
+      auto two = [&](int i) { return reinterpret_cast<float2*>(p + place.at[i]); };
+      *two(0) = make_float2(raw.a.x, raw.a.y), *two(2) = make_float2(raw.a.z, raw.a.w);
+      *two(1) = make_float2(raw.b.x, raw.b.y), *two(3) = make_float2(raw.b.z, raw.b.w);
     } else {
       float v[8];
       raw.get(v);
@@ -232,17 +248,22 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) rotary_kernel(const __grid_co
     axes |= static_cast<uint32_t>(max(q.axis, 0)) << 8 * i;
     if (q.axis < 0) alone |= 1u << i;
     if constexpr (RUN == 1) place.at[i] = q.lo, place.at[4 + i] = q.hi;
+    // (what is not turned: pairs side by side are two runs as well)
+    if constexpr (RUN == 2)
+      if (i % 2 == 0) place.at[i] = q.lo, place.at[i + 1] = q.axis < 0 ? q.lo + 2 : q.hi;
   }
   if constexpr (RUN == 4) {      // (what is not turned: four channels, and four more)
     place.at[0] = alone ? (mine ? 8 * l : 0) : pair(0).lo;
     place.at[1] = alone ? 4 : pair(0).hi - pair(0).lo;
   }
   if constexpr (RUN == 0) place.at[0] = mine ? 8 * l : 0;
-  const int offset = RUN == 1 ? 0 : place.at[0];
+  constexpr bool APART = RUN == 1 || RUN == 2;         // a lane's channels, here and there in a head
+  const int offset = APART ? 0 : place.at[0];
   // channels of the pairs: first ones, then second ones
   auto channel = [&](int i) {
     if constexpr (RUN == 0) return place.at[0] + 2 * (i & 3) + (i >> 2);
     else if constexpr (RUN == 4) return place.at[0] + (i & 3) + (i < 4 ? 0 : place.at[1]);
+    else if constexpr (RUN == 2) return place.at[(i & 2) + (i >> 2)] + (i & 1);
     else return place.at[i];
   };
   int rotated = 0;
@@ -401,7 +422,7 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) rotary_kernel(const __grid_co
         Channels<T, RUN> out;
         out.set(lo, hi);
         const bool in = live && (q == 0 || k + q < per_chunk);
-        if constexpr (RUN == 1) {      // (eight channels side by side to a lane again, by way of the slot that all have read)
+        if constexpr (APART) {      // (eight channels side by side to a lane again, by way of the slot that all have read)
           T* const at = slot(used, 0, q);
           __syncwarp();
           if (mine) out.store(at + group * ROW, place);
@@ -595,18 +616,19 @@ bool shape_ok(const RotShape& s, bool back) {
   return true;
 }
 
-// See `Place`.  Pairs of halves whose bands have a multiple of four of them lie in runs of four.
+// See `Place`.  Pairs of halves whose bands have a multiple of four of them lie in runs of four, of two in runs of two.  (Rotation of
+// 16200 tokens, 24 heads of 64, two bands of 20: one by one 41 us, runs of two 26.)
 int run_of(const RotShape& s) {
   if (!s.positions || s.interleaved) return 0;
-  for (int a = 0; a < s.axes; ++a)
-    if (s.band[a] % 8) return 1;
-  return 4;
+  int run = 4;
+  for (int a = 0; a < s.axes; ++a) run = std::min(run, s.band[a] % 8 == 0 ? 4 : s.band[a] % 4 == 0 ? 2 : 1);
+  return run;
 }
 
 template <typename T, int LANES, int NORM, bool BACK>
 cudaError_t by_run(const KernelParams& k, cudaStream_t s) {
   constexpr int R = heads_at_a_time(NORM, BACK, sizeof(T) == 2), BLOCKS = blocks_per_sm(NORM);
-  static std::atomic<uint64_t> devices[3];
+  static std::atomic<uint64_t> devices[4];
   constexpr int BYTES = STAGES * (NORM != ROT_NORM_NONE && BACK ? 2 : 1) * R * THREADS * 8 * static_cast<int>(sizeof(T));
   auto go = [&](auto* kernel, std::atomic<uint64_t>& of) {
     const cudaError_t e = allow_shared_memory(of, reinterpret_cast<const void*>(kernel), BYTES);
@@ -615,7 +637,8 @@ cudaError_t by_run(const KernelParams& k, cudaStream_t s) {
   switch (run_of(k.s)) {
     case 0: return go(rotary_kernel<T, LANES, NORM, BACK, 0, R, BLOCKS>, devices[0]);
     case 4: return go(rotary_kernel<T, LANES, NORM, BACK, 4, R, BLOCKS>, devices[1]);
-    default: return go(rotary_kernel<T, LANES, NORM, BACK, 1, R, BLOCKS>, devices[2]);
+    case 2: return go(rotary_kernel<T, LANES, NORM, BACK, 2, R, BLOCKS>, devices[2]);
+    default: return go(rotary_kernel<T, LANES, NORM, BACK, 1, R, BLOCKS>, devices[3]);
   }
 }
 template <typename T, int LANES, bool BACK>

@@ -249,7 +249,8 @@ def gen():
 @pytest.mark.parametrize("B,N,H,Hk,D,bands", [
     (1, 1, 1, 1, 8, (8,)), (2, 128, 4, 4, 8, (4, 4)), (1, 37, 12, 3, 64, (32, 32)), (3, 50, 5, 1, 48, (24, 24)), (1, 1000, 8, 8, 128, (32, 48, 48)),
     (2, 19, 3, 3, 40, (10, 6, 4)), (1, 333, 7, 7, 72, (16, 40)), (1, 65, 2, 1, 136, (64, 8)), (1, 40, 6, 2, 256, (128, 64, 32, 32)), (1, 5000, 16, 4, 96, (16, 40, 32)),
-    (1, 77, 9, 3, 24, (2,)), (37, 1, 16, 4, 128, (128,))])
+    (1, 77, 9, 3, 24, (2,)), (37, 1, 16, 4, 128, (128,)),
+    (1, 61, 3, 1, 40, (20, 20)), (2, 33, 5, 5, 72, (36, 12)), (1, 29, 6, 2, 256, (100, 4, 52)), (1, 51, 4, 2, 32, (4, 12)), (1, 90, 7, 1, 16, (6, 2))])
 def test_widths_heads_and_lengths(gen, B, N, H, Hk, D, bands, dtype, inter, norm):
     axes = rot.RotaryAxes(bands, interleaved=inter)
     q, k = ((torch.randn(B, N, h, D, device="cuda", generator=gen) + 0.5).to(dtype) for h in (H, Hk))
