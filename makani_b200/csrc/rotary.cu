@@ -480,7 +480,9 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) rotary_kernel(const __grid_co
 #pragma unroll
         for (int q = 0; q < R; ++q) {
           const float mean = LAYER ? sums[q * EACH + (BACK ? 2 : 1)] * inv : 0.f;      // of the deviations
-          float rstd = rsqrtf(fmaxf(fmaf(sums[q * EACH], inv, -mean * mean), 0.f) + s.eps);
+          // (a variance that rounding has left below zero is none; NaN stays NaN, which a maximum would make a zero of)
+          const float var = fmaf(sums[q * EACH], inv, -mean * mean);
+          float rstd = rsqrtf((var < 0.f ? 0.f : var) + s.eps);
           // (what goes along with zeros has no deviation, and the reciprocal is infinite without eps)
           if (BACK && !(live && (q == 0 || k + q < per_chunk))) rstd = 0.f;
           const f32x2 r2 = both(rstd), m2 = both(-mean);

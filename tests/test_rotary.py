@@ -367,6 +367,44 @@ def test_no_tokens_and_infinities(gen):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("norm", ["layer", "rms"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("D,bands", [(8, (4, 4)), (16, None), (24, (8, 8)), (72, (36, 12)), (128, (128,)), (256, (64, 64))])
+def test_norms_of_nan_and_infinities(gen, D, bands, dtype, norm):
+    """A head with NaN or an infinity has the results that the definition gives it, NaN in every channel but where an infinite root mean square leaves zeros, the
+    gradients of weights and biases with it; the other heads keep theirs."""
+    axes, at = (None, None) if bands is None else (rot.RotaryAxes(bands), _grid(40, len(bands), "cuda"))
+    p = {n: v.requires_grad_() for n, v in _params(D, "cuda", gen).items()}
+    q, k = (torch.randn(1, 40, h, D, device="cuda", generator=gen).to(dtype).requires_grad_() for h in (5, 2))
+    do = [torch.randn(t.shape, device="cuda", generator=gen).to(dtype) for t in (q, k)]
+
+    def call(q, k):
+        out = rot.norm_rotary_qk(q, k, p["q_weight"], p["k_weight"], at, axes, p["q_bias"], p["k_bias"], norm=norm)
+        return out, torch.autograd.grad(out, [q, k, *p.values()], do)
+
+    clean, clean_grads = call(q, k)
+    heads = torch.ones(1, 40, 5, dtype=torch.bool, device="cuda")
+    for value, channel in ((math.nan, 0), (math.nan, D - 1), (math.inf, 1), (-math.inf, D - 1)):
+        bad = q.detach().clone()
+        bad[0, 17, 3, channel] = value
+        out, grads = call(bad.requires_grad_(), k)
+        (want, _), back = _oracle(bad, p["q_weight"], p["q_bias"], at, axes, 1e-5, norm, do[0])
+        heads[0, 17, 3] = False
+        for n, got, w, before in (("q", out[0].detach(), want, clean[0].detach()), ("dq", grads[0], back[0][0], clean_grads[0])):
+            assert torch.equal(got.isnan(), w.isnan()), (n, value)
+            assert torch.equal(got[heads], before[heads]), (n, value)
+            finite = ~w[0, 17, 3].isnan()
+            assert w[0, 17, 3][finite].isfinite().all() and (norm == "rms" and n == "q" and abs(value) == math.inf or not finite.any())
+            # (zeros, biases added and turned: off by A and F of two of these)
+            _close(got[0, 17, 3][finite], w[0, 17, 3][finite], 2 * (A + F) * p["q_bias"].detach().abs().max(), n)
+        # (of the weights; no bias has to do with what is normed)
+        assert torch.equal(grads[2].isnan(), back[1][0].isnan()) and grads[2].isnan().any(), value
+        assert torch.equal(grads[4], clean_grads[4])
+        for i in (1, 3, 5):
+            assert torch.equal(grads[i], clean_grads[i]), i
+
+
+@pytest.mark.gpu
 def test_rotation_can_be_differentiated_again(gen):
     axes, at = rot.RotaryAxes((8, 8)), _grid(9, 2, "cuda")
     x = torch.randn(1, 9, 2, 16, device="cuda", generator=gen).requires_grad_()
