@@ -359,7 +359,8 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) rotary_kernel(const __grid_co
     if (!positions) return;
     const long long from = u.bat * s.position_batch + 1ll * u.n * s.axes;
 #pragma unroll
-    for (int i = 0; i < (RUN == 4 ? 1 : 4); ++i) at[i] = position_of(positions, s.position_type, from + (axes >> 8 * i & 255));
+    for (int i = 0; i < (RUN == 4 ? 1 : 4); ++i)      // (zeros that go along stay zeros, in the sums too, whatever stands behind the limit)
+      at[i] = !SUMS || u.live ? position_of(positions, s.position_type, from + (axes >> 8 * i & 255)) : 0.0;
   };
   if (begin < units) fetch_positions(next);
   // (the groups of a warp go through the loop together)

@@ -376,6 +376,29 @@ def test_path(gen, norm, packed, H, Hk, D, window):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("norm", [None, "layer", "rms"])
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+@pytest.mark.parametrize("D,bands,inter", [(64, (32, 16), False), (24, (12, 12), False), (40, (10, 6), False), (128, (64, 64), True)])
+def test_positions_behind_the_last_sequence_reach_nothing(gen, D, bands, inter, value, norm):
+    """The same bits whatever positions the tokens of no sequence have."""
+    axes = rot.RotaryAxes(bands, interleaved=inter)
+    off = torch.tensor([0, 150, 150, 333], dtype=torch.int32, device="cuda")
+    x = torch.randn(400, 8 * D, device="cuda", generator=gen).bfloat16().requires_grad_()
+    p = [(0.2 * torch.randn(D, device="cuda", generator=gen) + (i < 2)).requires_grad_() for i in range(4)] if norm else [None] * 4
+    do = torch.randn(400, 4, D, device="cuda", generator=gen).bfloat16()
+    at = 100 * torch.rand(400, 2, device="cuda", generator=gen)
+    bad = at.clone()
+    bad[333:] = value
+
+    def call(at):
+        o = rot.rotary_attention_qkv(x, 4, 2, at, axes, *p, norm=norm, offsets=off, window=50, sinks=1)
+        return [o, *torch.autograd.grad(o, [x] + [t for t in p if t is not None], do)]
+
+    for got, want in zip(call(bad), call(at)):
+        assert torch.isfinite(want).all() and torch.equal(got, want)
+
+
+@pytest.mark.gpu
 def test_transforms_and_refusals_of_windows(gen):
     q, k, v, do = _inputs(gen, 2, 60, H=2, Hk=1, D=16)
     mask = dict(window=9, sinks=1)
