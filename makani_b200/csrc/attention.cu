@@ -2109,10 +2109,10 @@ Window window_of(const AttnShape& p) { return {p.causal, p.left, p.causal ? 0 : 
 // 41.6 / 35.4, 16 x 512 x 8 27.7 / 28.3, 8 x 768 x 8 34.0 / 34.9; packed, 41 sequences of 7001 tokens 52.7 / 45.6.  (Lengths of packed sequences are on the
 // device: their mean is known.)
 int mean_length(const AttnShape& p) { return p.offsets ? p.N / std::max(1, p.sequences) : p.N; }
-// Tiles that one tile sees through a window, a sequence permitting
+// Tiles that one tile sees through a window, a sequence permitting: one at least (with more sequences than tokens the mean length is none)
 int window_tiles(const AttnShape& p) {
   const long long span = 1ll * p.left + (p.causal ? 0 : p.right) + TILE;
-  return static_cast<int>(std::min<long long>((span + TILE - 1) / TILE + 1, (mean_length(p) + TILE - 1) / TILE));
+  return static_cast<int>(std::max<long long>(1, std::min<long long>((span + TILE - 1) / TILE + 1, (mean_length(p) + TILE - 1) / TILE)));
 }
 // Through a window: up to 17 tiles, where start and end of a CTA are a quarter of it, and where CTAs of two tiles would leave half of the SMs idle.  us by tokens to
 // either side, two tiles / one: 16128 tokens, 8 heads of 48 192 58 / 54, 704 115 / 102, 960 143 / 125; of 128 704 150 / 144, 960 180 / 177, 1472 238 / 240, 3008 402 /

@@ -225,6 +225,37 @@ def test_packed_sequences(gen, lens, H, Hk, D, behind, causal, window, sinks):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("lens", [(1, 0, 0, 2, 0, 0, 3, 0), (0,) * 7 + (6,), (0, 0, 1), (137, 3) + (0,) * 142, (140, 3) + (0,) * 400, (0,) * 3000 + (1, 299)])
+@pytest.mark.parametrize("H,Hk,D,behind", [(2, 1, 16, 0), (4, 2, 128, 5)])
+@pytest.mark.parametrize("window,sinks", [(1, 1), ((2, 0), 0), (0, 300)])
+def test_more_sequences_than_tokens(gen, lens, H, Hk, D, behind, window, sinks, causal):
+    """Offsets with room for more sequences than there are, as a captured graph has them."""
+    _check_packed(gen, lens, H, Hk, D, behind, causal=causal, window=window, sinks=sinks)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("norm", [None, "rms"])
+def test_path_with_more_sequences_than_tokens(gen, norm):
+    """The fused calls: what the operators one after the other give."""
+    off = torch.tensor([0, 1, 1, 1, 3, 3, 3, 6, 6], dtype=torch.int32, device="cuda")
+    axes, at = rot.RotaryAxes((8, 8)), rot.grid_positions(2, 3, device="cuda")
+    x = torch.randn(6, 8 * 16, device="cuda", generator=gen).bfloat16().requires_grad_()
+    w = [torch.randn(16, device="cuda", generator=gen).requires_grad_() for _ in range(2)] if norm else [None] * 2
+    kw, leaves = dict(offsets=off, window=1, sinks=1), [x] + [t for t in w if norm]
+    q, k, v = x.unflatten(-1, (-1, 16)).split([4, 2, 2], -2)
+    do = torch.randn(6, 4, 16, device="cuda", generator=gen).bfloat16()
+    if norm:
+        turned = rot.norm_rotary_qk(q, k, *w, at, axes, norm=norm)
+    else:
+        turned = rot.rotary_qk(q, k, at, axes)
+    for got, want, of in ((rot.rotary_attention_qkv(x, 4, 2, at, axes, *w, norm=norm, **kw), attn.attention(*turned, v, **kw), leaves),
+                          (attn.attention_qkv(x, 4, 2, **kw), attn.attention(q, k, v, **kw), [x])):
+        assert torch.equal(got, want)
+        assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(got, of, do, retain_graph=True), torch.autograd.grad(want, of, do, retain_graph=True)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("causal", [False, True])
 def test_packed_sinks_that_go_apart(gen, causal):
     _check_packed(gen, (7000, 40, 1500), 4, 1, 64, 5, causal=causal, window=100, sinks=3)
     _check_packed(gen, (3001, 0, 2), 2, 2, 128, 77, causal=causal, window=(30, 60), sinks=131)
