@@ -283,13 +283,13 @@ class DistributedAttention(nn.Module):
         nn.init.trunc_normal_(self.proj.weight, std=0.02)
         self.attn_drop_rate = attn_drop_rate
         self.proj_drop = nn.Dropout(proj_drop_rate)
-        # per-head normalisation of queries and keys only on request (makani/mpu/layers.py:464,482-483); each rank holds
-        # whole heads, so these small parameters are private to it
+        # per-head normalisation of queries and keys only on request (makani/mpu/layers.py:464,482-483); one set of channels for all
+        # heads, of which each rank has its own: gradients are summed over them
         self.q_norm = norm_layer(self.head_dim) if qk_norm else nn.Identity()
         self.k_norm = norm_layer(self.head_dim) if qk_norm else nn.Identity()
         for norm in (self.q_norm, self.k_norm):
             for prm in norm.parameters():
-                prm.is_shared_mp = []
+                prm.is_shared_mp = [comm_hidden_name]
 
     def forward(self, x, positions=None):
         B, N, C = x.shape

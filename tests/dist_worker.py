@@ -576,6 +576,105 @@ def case_attention():
     assert _rel(layer.qkv.weight.grad.reshape(len(rows), -1), ser.qkv.weight.grad[rows][:, cin]) < 1e-5
 
 
+def case_attention_options():
+    """Norms of queries and keys, rotary positions, a window and register tokens of channel-parallel attention: outputs, gradients and weights after a step are
+    those of the serial module, those of the norms (one set for all heads, which the ranks share out) among them."""
+    from makani_b200.models.networks.vit import Attention
+    from makani_b200.ops import rotary
+    from makani_b200.parallel.grad_reduce import GradReducer
+    from makani_b200.parallel.helpers import sync_params
+    from makani_b200.parallel.layer_norm import LayerNorm
+    from makani_b200.parallel.layers import DistributedAttention
+    B, N, C, H = 2, 14, 32, 4
+    hd = C // H
+    nfi, nfo, fi, fo = comm.get_size("fin"), comm.get_size("fout"), comm.get_rank("fin"), comm.get_rank("fout")
+    hl = H // nfo
+    rows = torch.cat([torch.arange(part * C + (fo * hl) * hd, part * C + ((fo + 1) * hl) * hd) for part in range(3)])
+    cin, hid = slice(fi * (C // nfi), (fi + 1) * (C // nfi)), slice(fo * hl * hd, (fo + 1) * hl * hd)
+    at = rotary.grid_positions(3, 4, first=2)
+    for options in (dict(qk_norm=True), dict(qk_norm=True, axes=rotary.RotaryAxes((4, 4), base=20.0), window=4, sinks=2), dict(axes=rotary.RotaryAxes((2, 6)), window=3)):
+        positions = at if "axes" in options else None
+        torch.manual_seed(4)
+        ser = Attention(C, num_heads=H, norm_layer=LayerNorm, **options)
+        with torch.no_grad():
+            for prm in ser.parameters():
+                prm.copy_(torch.randn_like(prm) * 0.3)
+        layer = DistributedAttention(C, num_heads=H, **options)
+        norms = [n for n in ("q_norm", "k_norm") if "qk_norm" in options]
+        with torch.no_grad():
+            layer.qkv.weight.copy_(ser.qkv.weight[rows][:, cin])
+            layer.proj.weight.copy_(ser.proj.weight[cin][:, hid])
+            for n in norms:      # the first rank's are everybody's
+                for prm, want in zip(getattr(layer, n).parameters(), getattr(ser, n).parameters()):
+                    prm.copy_(want if fo == 0 else torch.full_like(want, 7.0))
+        sync_params(layer)
+        reducer = GradReducer(layer, use_peer=False)
+        reducer.zero_grad()
+        x, g = torch.randn(B, N, C), torch.randn(B, N, C)
+        xr, xl = x.clone().requires_grad_(), x[..., cin].contiguous().requires_grad_()
+        y_ref, y = ser(xr, positions) - ser.proj.bias, layer(xl, positions)
+        assert _rel(y, y_ref[..., cin]) < 1e-5
+        y_ref.backward(g)
+        y.backward(g[..., cin].contiguous())
+        reducer.reduce()
+        assert _rel(xl.grad, xr.grad[..., cin]) < 1e-5
+        assert _rel(layer.qkv.weight.grad, ser.qkv.weight.grad[rows][:, cin]) < 1e-5
+        for m in (ser, layer):
+            torch.optim.SGD(m.parameters(), lr=0.1).step()
+        for n in norms:
+            for (name, a), b in zip(getattr(layer, n).named_parameters(), getattr(ser, n).parameters()):
+                # (the bias of the keys' norm is an offset of all scores where nothing is turned, its gradient rounding alone)
+                assert torch.allclose(a.grad, b.grad, rtol=1e-4, atol=1e-5 * g.abs().sum().item() / C), (n, name)
+                assert torch.allclose(a, b, rtol=1e-4, atol=1e-5), (n, name)
+
+
+def case_vit_options():
+    """A ViT with its options over two ranks of attention heads and hidden features: forecasts and gradients of what all ranks hold are the serial network's."""
+    from makani_b200.models.networks.vit import VisionTransformer
+    args = dict(inp_shape=(16, 32), patch_size=(4, 4), inp_chans=3, out_chans=2, embed_dim=32, depth=2, num_heads=4, qkv_bias=False, qk_norm=True, rotary=True,
+                attn_window=1, register_tokens=3)
+    torch.manual_seed(5)
+    ser = VisionTransformer(**args, comm_inp_name="w", comm_hidden_name="w")      # (a group of one)
+    with torch.no_grad():
+        for n, prm in ser.named_parameters():
+            prm.copy_(torch.randn_like(prm) * 0.2)
+            if n.endswith("attn.proj.bias"):      # (the distributed projection has none)
+                prm.zero_()
+    net = VisionTransformer(**args)
+    fo, nfo = comm.get_rank("fout"), comm.get_size("fout")
+    assert net.blocks[0].channel_parallel and not ser.blocks[0].channel_parallel
+    C, H, hidden = 32, 4, 128
+    hid = slice(fo * C // nfo, (fo + 1) * C // nfo)
+    rows = torch.cat([torch.arange(part * C + fo * C // nfo, part * C + (fo + 1) * C // nfo) for part in range(3)])
+    wide = slice(fo * hidden // nfo, (fo + 1) * hidden // nfo)
+    place = {"attn.qkv.weight": lambda t: t[rows], "attn.proj.weight": lambda t: t[:, hid], "mlp.fc1.weight": lambda t: t[wide], "mlp.fc1.bias": lambda t: t[wide],
+             "mlp.fc2.weight": lambda t: t[:, wide]}
+    names = {"mlp.fc1": "mlp.fwd.0", "mlp.fc2": "mlp.fwd.3"}
+    want = dict(ser.named_parameters())
+
+    def of(name):
+        for a, b in names.items():
+            name = name.replace(a, b)
+        return name
+
+    local = {n: next((f for k, f in place.items() if n.endswith(k)), lambda t: t) for n, _ in net.named_parameters()}
+    with torch.no_grad():
+        for n, prm in net.named_parameters():
+            prm.copy_(local[n](want[of(n)]))
+    x, dy = torch.randn(2, 3, 16, 32), torch.randn(2, 2, 16, 32)
+    y, y_ref = net(x), ser(x)
+    assert _rel(y, y_ref) < 1e-5
+    y.backward(dy)
+    y_ref.backward(dy)
+    for n, prm in net.named_parameters():
+        g = prm.grad.clone()
+        if "q_norm" in n or "k_norm" in n:
+            assert prm.is_shared_mp == ["fout"]
+            dist.all_reduce(g, group=comm.get_group("fout"))
+        ref = local[n](want[of(n)].grad)
+        assert (g - ref).norm() < 1e-4 * (ref.norm() + 1e-2 * dy.norm()), n
+
+
 def case_reduction_hooks():
     """`init_gradient_reduction_hooks` in a plain user loop: after every backward pass the gradients equal the average
     over the data-parallel ranks of what a serial model gets on each rank's batch, with either flavour of zero_grad,

@@ -116,3 +116,12 @@ def test_gradient_reduction_hooks_in_a_plain_loop(world):
 @pytest.mark.parametrize("sizes", [(1, 1, 1, 2), (1, 1, 2, 1), (1, 1, 2, 2)])
 def test_channel_parallel_attention_matches_serial(sizes):
     _launch("attention", sizes, sizes[2] * sizes[3])
+
+
+@pytest.mark.parametrize("sizes", [(1, 1, 1, 2), (1, 1, 2, 1), (1, 1, 2, 2), (1, 1, 1, 4)])
+def test_channel_parallel_attention_options_match_serial(sizes):
+    _launch("attention_options", sizes, sizes[2] * sizes[3])
+
+
+def test_channel_parallel_vit_options_match_serial():
+    _launch("vit_options", (1, 1, 1, 2), 2)
