@@ -69,7 +69,7 @@ class Block(nn.Module):
                  path_drop_rate=0.0, act_layer=nn.GELU, norm_layer=LayerNorm, comm_inp_name="fin", comm_hidden_name="fout", qk_norm=False, axes=None,
                  window=None, sinks=0, dropout_generator="torch"):
         super().__init__()
-        sees = dict(qk_norm=qk_norm, axes=axes, window=window, sinks=sinks)
+        sees = dict(qk_norm=qk_norm, axes=axes, window=window, sinks=sinks, dropout_generator=dropout_generator)
         hidden = int(dim * mlp_ratio)
         self.norm1, self.norm2 = norm_layer(dim), norm_layer(dim)
         self.channel_parallel = comm.get_size(comm_inp_name) * comm.get_size(comm_hidden_name) > 1
@@ -79,10 +79,10 @@ class Block(nn.Module):
                                              attn_drop_rate=attn_drop_rate, proj_drop_rate=mlp_drop_rate, norm_layer=LayerNorm if qk_norm else None, **sees)
             self.mlp = DistributedMLP(in_features=dim, hidden_features=hidden, out_features=dim, act_layer=act_layer,
                                       drop_rate=mlp_drop_rate, input_format="traditional", comm_inp_name=comm_inp_name,
-                                      comm_hidden_name=comm_hidden_name)
+                                      comm_hidden_name=comm_hidden_name, dropout_generator=dropout_generator)
         else:
             self.attn = Attention(dim, num_heads=num_heads, qkv_bias=qkv_bias, attn_drop_rate=attn_drop_rate,
-                                  proj_drop_rate=mlp_drop_rate, norm_layer=norm_layer, dropout_generator=dropout_generator, **sees)
+                                  proj_drop_rate=mlp_drop_rate, norm_layer=norm_layer, **sees)
             self.mlp = MLP(in_features=dim, hidden_features=hidden, out_features=dim, act_layer=act_layer, drop_rate=mlp_drop_rate,
                            input_format="traditional", dropout_generator=dropout_generator)      # fused token MLP (ops/linear.py)
         self.drop_path = DropPath(path_drop_rate) if path_drop_rate > 0.0 else nn.Identity()

@@ -213,8 +213,9 @@ class DistributedEncoderDecoder(nn.Module):
 class DistributedMLP(nn.Module):
     def __init__(self, in_features, hidden_features=None, out_features=None, output_bias=True, input_format="nchw",
                  comm_inp_name="fin", comm_hidden_name="fout", act_layer=nn.GELU, drop_rate=0.0, drop_type="iid",
-                 checkpointing=0, gain=1.0, **kwargs):
+                 checkpointing=0, gain=1.0, dropout_generator="torch", **kwargs):
         super().__init__()
+        from ..models.common.layers import dropout_layer
         self.checkpointing = checkpointing
         out_features = out_features or in_features
         hidden_features = hidden_features or in_features
@@ -227,7 +228,7 @@ class DistributedMLP(nn.Module):
             nn.init.constant_(self.fc2.bias, 0.0)
         self.act = act_layer()
         if drop_rate > 0.0:
-            self.drop = nn.Dropout(drop_rate) if drop_type == "iid" else nn.Dropout2d(drop_rate)
+            self.drop = dropout_layer(drop_rate, dropout_generator) if drop_type == "iid" else nn.Dropout2d(drop_rate)
         else:
             self.drop = nn.Identity()
 
@@ -268,8 +269,10 @@ class DistributedAttention(nn.Module):
     """Multi-head self attention with heads split over `comm_hidden_name` (sequence stays whole)."""
 
     def __init__(self, dim, input_format="traditional", comm_inp_name="fin", comm_hidden_name="fout", num_heads=8,
-                 qkv_bias=False, qk_norm=False, attn_drop_rate=0.0, proj_drop_rate=0.0, norm_layer=LayerNorm, axes=None, window=None, sinks=0):
+                 qkv_bias=False, qk_norm=False, attn_drop_rate=0.0, proj_drop_rate=0.0, norm_layer=LayerNorm, axes=None, window=None, sinks=0,
+                 dropout_generator="torch"):
         super().__init__()
+        from ..models.common.layers import dropout_layer
         assert dim % num_heads == 0
         self.axes, self.window, self.sinks = axes, window, sinks      # as of models/networks/vit.py: Attention
         assert num_heads % comm.get_size(comm_hidden_name) == 0, "heads must divide over the hidden group"
@@ -282,7 +285,7 @@ class DistributedAttention(nn.Module):
         nn.init.trunc_normal_(self.qkv.weight, std=0.02)
         nn.init.trunc_normal_(self.proj.weight, std=0.02)
         self.attn_drop_rate = attn_drop_rate
-        self.proj_drop = nn.Dropout(proj_drop_rate)
+        self.proj_drop = dropout_layer(proj_drop_rate, dropout_generator)
         # per-head normalisation of queries and keys only on request (makani/mpu/layers.py:464,482-483); one set of channels for all
         # heads, of which each rank has its own: gradients are summed over them
         self.q_norm = norm_layer(self.head_dim) if qk_norm else nn.Identity()

@@ -675,6 +675,28 @@ def case_vit_options():
         assert (g - ref).norm() < 1e-4 * (ref.norm() + 1e-2 * dy.norm()), n
 
 
+def case_vit_dropout():
+    """The network's dropouts are those of the generator that it is given, in channel-parallel blocks too; another generator is refused."""
+    from makani_b200.models.common.layers import Dropout
+    from makani_b200.models.networks.vit import VisionTransformer
+    args = dict(inp_shape=(16, 32), patch_size=(4, 4), inp_chans=3, out_chans=2, embed_dim=32, depth=2, num_heads=4, mlp_drop_rate=0.3)
+    for generator, kind in (("counter", Dropout), ("torch", torch.nn.Dropout)):
+        torch.manual_seed(6)
+        net = VisionTransformer(**args, dropout_generator=generator)
+        assert all(type(d) is kind and d.p == 0.3 for b in net.blocks for d in (b.attn.proj_drop, b.mlp.drop))
+        x = torch.randn(1, 3, 16, 32)
+        torch.manual_seed(7)
+        y = net(x)
+        torch.manual_seed(7)
+        assert torch.equal(y, net(x)) and not torch.equal(y, net(x)) and torch.equal(net.eval()(x), net(x))
+    try:
+        VisionTransformer(**args, dropout_generator="philox")
+    except ValueError as e:
+        assert "generators" in str(e)
+    else:
+        raise AssertionError("an unknown generator is refused")
+
+
 def case_reduction_hooks():
     """`init_gradient_reduction_hooks` in a plain user loop: after every backward pass the gradients equal the average
     over the data-parallel ranks of what a serial model gets on each rank's batch, with either flavour of zero_grad,

@@ -125,3 +125,7 @@ def test_channel_parallel_attention_options_match_serial(sizes):
 
 def test_channel_parallel_vit_options_match_serial():
     _launch("vit_options", (1, 1, 1, 2), 2)
+
+
+def test_channel_parallel_vit_dropout_generator():
+    _launch("vit_dropout", (1, 1, 1, 2), 2)
