@@ -40,6 +40,13 @@ class DropPath(nn.Module):
         return drop_path(x, self.drop_prob, self.training)
 
 
+def watched(m: nn.Module, forward) -> bool:
+    """Whether somebody has to see the call of a module: hooks, its own or of all modules, or another class's `forward`, for which joint passes stay apart."""
+    g = nn.modules.module
+    return bool(m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks or g._global_forward_hooks or g._global_forward_pre_hooks
+                or g._global_backward_hooks or g._global_backward_pre_hooks or "forward" in m.__dict__ or type(m).forward is not forward)
+
+
 class Dropout(nn.Dropout):
     """`nn.Dropout` on the kernel of `ops/dropout.py`, whose mask is made again in the backward pass instead of being kept (and is another than torch's)."""
 
@@ -52,6 +59,10 @@ class Dropout(nn.Dropout):
     def add(self, x, residual):
         """residual + dropout(x), in one pass over memory."""
         return dropout_ops.dropout_add(x, residual, self.p, self.training)
+
+    def joins(self) -> bool:
+        """Whether `add` may take its place: it drops something, and nobody has to see its call."""
+        return self.training and not watched(self, Dropout.forward)
 
 
 def dropout_layer(p: float, generator: str = "torch") -> nn.Module:
@@ -162,8 +173,10 @@ class MLP(nn.Module):
         """The stack of x; with a residual, their sum, which takes the last dropout with it where that can."""
         if self.checkpointing >= 2 and self.training:
             y = self.checkpoint_forward(x)
-        elif residual is not None and isinstance(self.fwd[4], Dropout) and self.training:
-            return self.fwd[4].add(self.fwd[:4](x), residual)
+        elif residual is not None and isinstance(self.fwd[4], Dropout) and self.fwd[4].joins() and not watched(self.fwd, nn.Sequential.forward):
+            for i in range(4):
+                x = self.fwd[i](x)
+            return self.fwd[4].add(x, residual)
         else:
             y = self._run(x)
         return y if residual is None else residual + y

@@ -26,7 +26,7 @@ from ...ops import rotary as rotary_ops
 from ...parallel.layer_norm import LayerNorm, normed, operand_dtype
 from ...parallel.layers import DistributedAttention, DistributedMLP, attend_normed
 from ...utils import comm
-from ..common.layers import MLP, DropPath, Dropout, PatchEmbed, dropout_layer
+from ..common.layers import MLP, DropPath, Dropout, PatchEmbed, dropout_layer, watched
 
 
 class _Proj(nn.Linear):
@@ -87,11 +87,17 @@ class Block(nn.Module):
                            input_format="traditional", dropout_generator=dropout_generator)      # fused token MLP (ops/linear.py)
         self.drop_path = DropPath(path_drop_rate) if path_drop_rate > 0.0 else nn.Identity()
 
+    def _joint(self) -> bool:
+        """Whether attention and MLP may hand on their sums with what they are added to: there is a dropout that takes it along, and nobody has to see either's own
+        result."""
+        return (self.training and not self.channel_parallel and isinstance(self.attn.proj_drop, Dropout) and self.attn.proj_drop.joins()
+                and not (watched(self.attn, Attention.forward) or watched(self.mlp, MLP.forward) or watched(self.drop_path, nn.Identity.forward)))
+
     def forward(self, x, positions=None):
         # (the products' type where they run on the engine; the channel-parallel layers take what torch's norm would hand on)
         y = self.norm1(x) if self.channel_parallel else normed(self.norm1, x, operand_dtype(x))
         more = {} if positions is None else dict(positions=positions)
-        if self.training and not self.channel_parallel and isinstance(self.attn.proj_drop, Dropout) and isinstance(self.drop_path, nn.Identity):
+        if self._joint():
             # dropouts take the residual sums with them
             z = self.norm2(self.attn(y, residual=x, **more))
             return self.mlp(z.to(operand_dtype(z)), residual=z)

@@ -92,6 +92,57 @@ def test_counter_dropout_on_the_cpu():
     assert torch.equal(a, m(x)) and not torch.equal(a, m(x))
 
 
+@pytest.mark.parametrize("where", ["attn", "attn.proj_drop", "drop_path", "mlp", "mlp.fwd", "mlp.fwd.4", "mlp.fwd.3", "all"])
+def test_hooks_see_the_calls_of_joint_passes(where):
+    """Hooks on what a joint pass takes together: called as often in training as in evaluation, with the module's own result, and the outcome is the same."""
+    m = _vit("cpu", depth=1, mlp_drop_rate=0.3, dropout_generator="counter", **ALL)
+    x = torch.randn(1, 5, 32, 64)
+    torch.manual_seed(5)
+    want = m.train()(x)
+    seen = []
+    hook = lambda mod, args, out: seen.append((args[0].detach(), out.detach()))  # noqa: E731
+    if where == "all":
+        handle = nn.modules.module.register_module_forward_hook(hook)
+    else:
+        handle = m.blocks[0].get_submodule(where).register_forward_hook(hook)
+    calls = {}
+    for training in (True, False):
+        seen.clear()
+        torch.manual_seed(5)
+        y = m.train(training)(x)
+        calls[training] = len(seen)
+        if training:
+            # (watched by all, norms and rotation are calls of their own, each rounded to fp32: some hundred steps of 2^-24 to the end of one block)
+            assert torch.equal(y, want) or where == "all" and (y - want).abs().max() < 2.0 ** -16 * want.abs().max()
+            if where in ("attn.proj_drop", "mlp.fwd.4"):
+                a, b = seen[-1]
+                # (dropped, and nothing added; factor and product, and 0.7 and the quotient, are half a step of 2^-24 each)
+                assert torch.allclose(b[b != 0], (a / 0.7)[b != 0], rtol=2.0 ** -22, atol=0.0) and 0.1 < (b == 0).double().mean() < 0.5
+            if where in ("attn", "mlp", "mlp.fwd"):
+                assert 0.1 < (seen[0][1] == 0).double().mean() < 0.5
+    handle.remove()
+    assert calls[True] == calls[False] > 0
+    # with nobody there, the joint pass again
+    torch.manual_seed(5)
+    assert torch.equal(m.train()(x), want)
+
+
+def test_joint_passes_are_for_the_classes_that_have_them():
+    from makani_b200.models.networks.vit import Attention
+
+    class Mine(Attention):
+        def forward(self, x, positions=None):
+            return super().forward(x, positions)
+
+    m = _vit("cpu", depth=1, mlp_drop_rate=0.3, dropout_generator="counter")
+    x = torch.randn(1, 5, 32, 64)
+    torch.manual_seed(5)
+    want = m.train()(x)
+    m.blocks[0].attn.__class__ = Mine
+    torch.manual_seed(5)
+    assert torch.equal(m(x), want)
+
+
 @pytest.mark.parametrize("name", ["vit_73chq_window"])
 def test_recipe(name):
     from makani_b200.utils.YParams import YParams
