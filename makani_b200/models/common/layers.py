@@ -124,6 +124,13 @@ class EncoderDecoder(nn.Module):
         return self.fwd(x)
 
 
+class TokenLinear(nn.Linear):
+    """`nn.Linear` whose product runs on the GEMM engine where the tokens qualify (`ops/linear.py`)."""
+
+    def forward(self, x):
+        return linear_ops.linear_lastdim(x, self.weight, self.bias)
+
+
 class MLP(nn.Module):
     """fc1 -> act -> drop -> fc2 -> drop, pointwise over NCHW (1x1 convs) or the last dim ("traditional")."""
 
@@ -133,6 +140,7 @@ class MLP(nn.Module):
         self.checkpointing = checkpointing
         out_features = out_features or in_features
         hidden_features = hidden_features or in_features
+        counter = drop_rate > 0.0 and dropout_generator == "counter" and drop_type == "iid" and input_format == "traditional"
         if input_format == "nchw":
             fc1 = nn.Conv2d(in_features, hidden_features, 1, bias=True)
             fc2 = nn.Conv2d(hidden_features, out_features, 1, bias=output_bias)
@@ -141,8 +149,10 @@ class MLP(nn.Module):
         elif input_format == "traditional":
             if drop_type == "features":
                 raise NotImplementedError("feature dropout needs the nchw format")
-            fc1 = nn.Linear(in_features, hidden_features, bias=True)
-            fc2 = nn.Linear(hidden_features, out_features, bias=output_bias)
+            # (behind torch's own dropout torch's own products)
+            linear = TokenLinear if counter else nn.Linear
+            fc1 = linear(in_features, hidden_features, bias=True)
+            fc2 = linear(hidden_features, out_features, bias=output_bias)
         else:
             raise NotImplementedError(f"input format {input_format} not supported")
         nn.init.normal_(fc1.weight, mean=0.0, std=math.sqrt(2.0 / in_features))
@@ -157,13 +167,18 @@ class MLP(nn.Module):
         self.fwd = nn.Sequential(fc1, act_layer(), drop, fc2, drop)
         self._fusable = (input_format == "nchw" and _is_gelu(act_layer) and drop_rate == 0.0)
         self._fusable_tokens = (input_format == "traditional" and _is_gelu(act_layer) and drop_rate == 0.0)
+        self._fusable_forecasts = counter and _is_gelu(act_layer)
 
     def _run(self, x):
         if self._fusable and x.is_cuda and conv_ops.fast_path_ok(x):
             return conv_ops.mlp2(x, self.fwd[0].weight, self.fwd[0].bias, self.fwd[3].weight, self.fwd[3].bias)
-        if self._fusable_tokens and linear_ops.fast_path_ok(x):
+        if (self._fusable_tokens or self._nothing_dropped()) and linear_ops.fast_path_ok(x):
             return linear_ops.mlp2_lastdim(x, self.fwd[0].weight, self.fwd[0].bias, self.fwd[3].weight, self.fwd[3].bias)
         return self.fwd(x)
+
+    def _nothing_dropped(self) -> bool:
+        """Whether the dropouts leave everything as it is, and nobody has to see them, or the layers around them, called."""
+        return self._fusable_forecasts and not self.fwd[2].training and not any(watched(m, type(m).forward) for m in (self.fwd, *self.fwd))
 
     def checkpoint_forward(self, x):
         """The forward pass with its activations recomputed in backward (makani/models/common/layers.py `MLP`)."""

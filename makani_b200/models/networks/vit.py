@@ -10,7 +10,8 @@ their rows and columns on the patch grid), `attn_window` (attention reaches this
 (learned tokens in front of the grid's that stay visible from everywhere), `dropout_generator` "counter" (masks that are never stored).
 
 Execution: tokens stay in one [B, tokens, E] bf16 matrix.  Every projection (qkv, attention output, both MLP layers with
-bias + GELU / bias epilogues, head) is a GEMM of the in-tree tensor-core engine (`ops/linear.py`), attention reads the
+bias + GELU / bias epilogues, head) is a GEMM of the in-tree tensor-core engine (`ops/linear.py`); behind dropout from a
+counter the two of the MLP are two products with bias in training, and around torch's own dropout they are torch's.  Attention reads the
 fused projection's output where it lies (`ops/attention.py`; behind norms and rotation in one call, `ops/rotary.py`; with attention dropout in
 training it is torch's `scaled_dot_product_attention`), and the second norm of a block takes the residual sum with it (`ops/norm.py`).  On CPU /
 fp32 every piece is the plain torch op.
@@ -26,14 +27,7 @@ from ...ops import rotary as rotary_ops
 from ...parallel.layer_norm import LayerNorm, normed, operand_dtype
 from ...parallel.layers import DistributedAttention, DistributedMLP, attend_normed
 from ...utils import comm
-from ..common.layers import MLP, DropPath, Dropout, PatchEmbed, dropout_layer, watched
-
-
-class _Proj(nn.Linear):
-    """nn.Linear whose forward runs on the GEMM engine when the tokens qualify (bf16, CUDA, features % 8 == 0)."""
-
-    def forward(self, x):
-        return linear_ops.linear_lastdim(x, self.weight, self.bias)
+from ..common.layers import MLP, DropPath, Dropout, PatchEmbed, TokenLinear, dropout_layer, watched
 
 
 class Attention(nn.Module):
@@ -45,8 +39,8 @@ class Attention(nn.Module):
         if dim % num_heads:
             raise ValueError(f"dim {dim} is not a multiple of num_heads {num_heads}")
         self.num_heads, self.head_dim = num_heads, dim // num_heads
-        self.qkv = _Proj(dim, 3 * dim, bias=qkv_bias)
-        self.proj = _Proj(dim, dim)
+        self.qkv = TokenLinear(dim, 3 * dim, bias=qkv_bias)
+        self.proj = TokenLinear(dim, dim)
         self.q_norm = norm_layer(self.head_dim) if qk_norm else nn.Identity()
         self.k_norm = norm_layer(self.head_dim) if qk_norm else nn.Identity()
         self.attn_drop_rate = attn_drop_rate
@@ -145,7 +139,7 @@ class VisionTransformer(nn.Module):
             for i in range(depth)])
         self.norm = LayerNorm(embed_dim)
         self.out_size = out_chans * self.patch_size[0] * self.patch_size[1]
-        self.head = _Proj(embed_dim, self.out_size, bias=False)
+        self.head = TokenLinear(embed_dim, self.out_size, bias=False)
         nn.init.trunc_normal_(self.pos_embed, std=0.02)
         if register_tokens:
             nn.init.trunc_normal_(self.registers, std=0.02)

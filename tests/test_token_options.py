@@ -214,6 +214,54 @@ def test_no_library_attention_norm_or_dropout(dev, monkeypatch):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("training", [True, False])
+def test_no_library_products_behind_counter_dropout(dev, training, monkeypatch):
+    """Both layers of the MLP on the engine, too, in training and in forecasts; and its forecast is that of the network without dropout."""
+    m = _vit(dev, **ALL, mlp_drop_rate=0.1, dropout_generator="counter").train(training)
+    x = torch.randn(1, 5, 32, 64, device=dev)
+
+    def refuse(*a, **k):
+        raise AssertionError("library call")
+
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        if not training:
+            want = _vit(dev, **ALL).eval()(x)
+        for name in ("linear", "scaled_dot_product_attention", "layer_norm", "dropout"):
+            monkeypatch.setattr(torch.nn.functional, name, refuse)
+        y = m(x)
+    assert training or torch.equal(y, want)
+    y.float().sum().backward()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("joint", [True, False])
+def test_mlp_behind_counter_dropout(dev, joint):
+    """Values and gradients of the MLP in training against the formula in 64 bits, with the masks that the generator draws: each product, activation and sum is
+    rounded to bf16, 2^-9 of the size on average, four of them one behind the other and as many in the backward pass: 2^-7 in all."""
+    from makani_b200.models.common.layers import MLP
+    torch.manual_seed(2)
+    m = MLP(in_features=64, hidden_features=256, input_format="traditional", drop_rate=0.3, dropout_generator="counter").to(dev)
+    x, r = (torch.randn(2, 300, 64, device=dev).bfloat16().requires_grad_() for _ in range(2))
+    dy = torch.randn(2, 300, 64, device=dev).bfloat16()
+    torch.manual_seed(9)
+    keep = [m.fwd[2](torch.ones(2, 300, c, device=dev)).double() for c in (256, 64)]
+    torch.manual_seed(9)
+    y = m(x, r) if joint else m(x)
+    grads = torch.autograd.grad(y, [x, *m.parameters()], dy)
+    x64, p64 = x.detach().double().requires_grad_(), [p.detach().double().requires_grad_() for p in m.parameters()]
+    h = torch.nn.functional.gelu(x64 @ p64[0].bfloat16().double().T + p64[1])
+    want = (h * keep[0] @ p64[2].bfloat16().double().T + p64[3]) * keep[1] + (r.detach().double() if joint else 0.0)
+    assert _rel(y.detach(), want.detach()) < 2.0 ** -7
+    for got, ref in zip(grads, torch.autograd.grad(want, [x64, *p64], dy.double())):
+        assert _rel(got, ref) < 2.0 ** -7
+    # dropouts alone in training, as for several draws of one forecast, still drop
+    m.eval()
+    plain = m(x)
+    m.fwd[2].train()
+    assert not torch.equal(m(x), plain)
+
+
+@pytest.mark.gpu
 def test_counter_dropout_has_one_mask_both_ways(dev):
     """In fp32, a step along the gradient changes the output by what the gradient says, with the masks of one seed."""
     m = _vit(dev, mlp_drop_rate=0.2, dropout_generator="counter", **ALL).train()
