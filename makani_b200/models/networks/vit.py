@@ -6,8 +6,10 @@ Checkpoint contract (names and shapes of makani/models/networks/vit.py:29-231): 
 channel-parallel groups (makani/mpu/layers.py:352-359,453-529).
 
 Options beyond the reference's, all off by default: `qk_norm` (queries and keys layer-normalised per head), `rotary` (queries and keys turned by
-their rows and columns on the patch grid), `attn_window` (attention reaches this many rows of patches to the north and south), `register_tokens`
-(learned tokens in front of the grid's that stay visible from everywhere), `dropout_generator` "counter" (masks that are never stored).
+their rows and columns on the patch grid), `attn_window` (attention reaches as many tokens before and behind a patch as this many rows of patches have:
+to its north the farthest row counts from its own column on eastwards, to its south up to its own column), `register_tokens` (learned tokens in front of
+the grid's that stay visible from everywhere; they are tokens of the same sequence, so that with a window they see each other and the
+northernmost rows, and what is further south reaches them through the layers), `dropout_generator` "counter" (masks that are never stored).
 
 Execution: tokens stay in one [B, tokens, E] bf16 matrix.  Every projection (qkv, attention output, both MLP layers with
 bias + GELU / bias epilogues, head) is a GEMM of the in-tree tensor-core engine (`ops/linear.py`); behind dropout from a

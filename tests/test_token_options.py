@@ -81,6 +81,38 @@ def test_windows_keep_what_is_far_away():
     assert torch.equal(y[:, :, :16], z[:, :, :16]) and not torch.equal(y[:, :, 20:24], z[:, :, 20:24])
 
 
+@pytest.mark.parametrize("rows,registers", [(2, 3), (1, 1), (0, 2), (3, 0)])
+def test_what_tokens_see_through_a_window(rows, registers):
+    """Patches in the first, a middle and the last column, and registers: the farthest row to the north from the own column on, to the south up to it, whole rows in
+    between, and all registers; registers see what stands as near to them."""
+    m = _vit("cpu", depth=1, attn_window=rows, register_tokens=registers)
+    H, W = m.grid
+    x = torch.randn(1, registers + H * W, 96, requires_grad=True)
+    y = m.blocks[0].attn(x)
+
+    def seen(token):
+        g, = torch.autograd.grad(y[0, token].sum(), x, retain_graph=True)
+        g = g[0].abs().amax(-1) > 0
+        return g[:registers], g[registers:].view(H, W)
+
+    for r in (0, 1, H // 2, H - 1):
+        for c in (0, W // 2, W - 1):
+            want = torch.zeros(H, W, dtype=torch.bool)
+            want[max(r - rows + 1, 0):r + rows] = True
+            if r - rows >= 0:
+                want[r - rows, c:] = True
+            if r + rows < H:
+                want[r + rows, :c + 1] = True
+            if rows == 0:
+                want[:], want[r, c] = False, True
+            at, grid = seen(registers + r * W + c)
+            assert at.all() and torch.equal(grid, want), (r, c)
+    for i in range(registers):
+        at, grid = seen(i)
+        reach = max(0, i + rows * W - registers + 1)
+        assert at.all() and torch.equal(grid.flatten(), torch.arange(H * W) < reach), i
+
+
 def test_counter_dropout_on_the_cpu():
     m = _vit("cpu", mlp_drop_rate=0.3, dropout_generator="counter")
     x = torch.randn(1, 5, 32, 64)
