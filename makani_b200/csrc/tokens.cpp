@@ -1026,10 +1026,10 @@ std::tuple<Tensor, Tensor> dropout_pass(const Tensor& x_in, const Tensor& residu
 Tensor dropout_run(const Tensor& x, const Tensor& residual, const Tensor& seed, double p, bool out_f32);
 struct DropoutOp {
   static constexpr const char* NAME = "DropoutNode";
-  // fields: x in fp32, there is a residual, it is in fp32; p.  kept: seed.  edges: x, residual
+  // fields: x in fp32, the residual in fp32; p.  kept: seed.  edges: x, residual
   static variable_list gradients(const variable_list& grads, const variable_list& s, const Fields& f, const std::vector<bool>& need) {
     const Tensor &seed = s[0], &dy = grads[0];
-    const bool x_f32 = f.whole[0] != 0, r_f32 = f.whole[2] != 0;
+    const bool x_f32 = f.whole[0] != 0, r_f32 = f.whole[1] != 0;
     variable_list out(2);
     if (!dy.defined()) return out;
     MK_CHECK(plain({&dy}), "dropout: the backward pass takes no batches of gradients, and is not traced");
@@ -1065,8 +1065,7 @@ Tensor dropout_run(const Tensor& x, const Tensor& residual, const Tensor& seed, 
   if (train) {
     Fields f;
     f.whole[0] = is_f32(x);
-    f.whole[1] = residual.defined();
-    f.whole[2] = residual.defined() && is_f32(residual);
+    f.whole[1] = residual.defined() && is_f32(residual);
     f.real[0] = p;
     FieldNode<DropoutOp>::record({y}, {x, residual}, {seed.defined() ? seed : kept}, f);
   }
