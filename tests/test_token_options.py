@@ -354,3 +354,58 @@ def test_captured_step_with_everything(dev):
         seen.append(loss.item())
     assert all(torch.isfinite(torch.tensor(v)) for v in seen) and len(set(seen)) == 4
     assert all(not torch.equal(a, p) for a, p in zip(before, m.parameters()))
+
+
+def _compiled_calls(dev):
+    """Every operator with a node of its own: (call, leaves)."""
+    from makani_b200.ops import dropout as drop
+    g = torch.Generator(dev).manual_seed(5)
+    leaf = lambda *s, dtype=torch.bfloat16: torch.randn(*s, device=dev, generator=g).to(dtype).requires_grad_()  # noqa: E731
+    axes, at = rot.RotaryAxes((8, 4)), torch.rand(60, 2, device=dev, generator=g)
+    q, k, v, qkv = leaf(1, 60, 4, 16), leaf(1, 60, 2, 16), leaf(1, 60, 2, 16), leaf(1, 60, 8 * 16)
+    flat = qkv.detach()[0].requires_grad_()
+    off = torch.tensor([0, 13, 13, 55], dtype=torch.int32, device=dev)
+    p = [leaf(16, dtype=torch.float32) for _ in range(4)]
+    x, r, seed = leaf(50, 40), leaf(50, 40, dtype=torch.float32), torch.tensor([3, 4], device=dev)
+    return {
+        "attention": (lambda: attn.attention(q, k, v), [q, k, v]),
+        "window": (lambda: attn.attention(q, k, v, causal=True, window=7, sinks=2), [q, k, v]),
+        "projection": (lambda: attn.attention_qkv(flat, 4, 2, offsets=off, window=(9, 3), scale=0.3), [flat]),
+        "rotation": (lambda: rot.rotary_qk(q, k, at, axes), [q, k]),
+        "rotation back": (lambda: rot.rotary(q, at, axes, inverse=True), [q]),
+        "norms": (lambda: rot.norm_rotary_qk(q, k, p[0], p[1], at, axes, p[2], p[3], eps=1e-3, norm="rms"), [q, k, *p]),
+        "norms without weights": (lambda: rot.norm_rotary_qk(q, k, None, None), [q, k]),
+        "path": (lambda: rot.rotary_attention_qkv(qkv, 4, 2, at, axes, window=7, sinks=1), [qkv]),
+        "path with norms": (lambda: rot.rotary_attention_qkv(flat, 4, 2, at, axes, *p, norm="layer", offsets=off, window=7, sinks=1), [flat, *p]),
+        "dropout": (lambda: drop.dropout(x, 0.3, seed=seed), [x]),
+        "dropout of the generator": (lambda: drop.dropout(x, 0.3), [x]),
+        "dropout and sum": (lambda: drop.dropout_add(x, r, 0.3, seed=seed), [x, r]),
+        "sum in bf16": (lambda: drop.dropout_add(r, x, 0.3, seed=seed), [x, r]),
+    }
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["attention", "window", "projection", "rotation", "rotation back", "norms", "norms without weights", "path", "path with norms", "dropout",
+                                  "dropout of the generator", "dropout and sum", "sum in bf16"])
+def test_compiled_backward_passes(dev, name):
+    """A backward pass that is compiled calls the kernels with what the node keeps: the same bits, again with other tensors of the same sizes."""
+    from torch._dynamo import compiled_autograd
+    call, leaves = _compiled_calls(dev)[name]
+
+    def grads():
+        torch.manual_seed(6)
+        out = call()
+        out = (out,) if isinstance(out, torch.Tensor) else tuple(out)
+        return torch.autograd.grad(sum(t.float().square().sum() for t in out), leaves)
+
+    for _ in range(2):
+        before = _ext.launch_count()
+        want = grads()
+        launches = _ext.launch_count() - before
+        with compiled_autograd._enable(torch.compile(backend="eager")):
+            got = grads()
+        assert _ext.launch_count() - before == 2 * launches > 0
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        with torch.no_grad():
+            for t in leaves:
+                t.add_(torch.randn_like(t))
