@@ -15,6 +15,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 from torch.utils.checkpoint import checkpoint
 
+from ...ops import _ext
 from ...ops import conv as conv_ops
 from ...ops import dropout as dropout_ops
 from ...ops import linear as linear_ops
@@ -178,7 +179,8 @@ class MLP(nn.Module):
 
     def _nothing_dropped(self) -> bool:
         """Whether the dropouts leave everything as it is, and nobody has to see them, or the layers around them, called."""
-        return self._fusable_forecasts and not self.fwd[2].training and not any(watched(m, type(m).forward) for m in (self.fwd, *self.fwd))
+        # (the activation as in training: the engine's other form is for networks that have it throughout)
+        return self._fusable_forecasts and not self.fwd[2].training and _ext.gelu_approximation() == "none" and not any(watched(m, type(m).forward) for m in (self.fwd, *self.fwd))
 
     def checkpoint_forward(self, x):
         """The forward pass with its activations recomputed in backward (makani/models/common/layers.py `MLP`)."""

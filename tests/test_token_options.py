@@ -175,6 +175,19 @@ def test_joint_passes_are_for_the_classes_that_have_them():
     assert torch.equal(m(x), want)
 
 
+def test_when_forecasts_of_the_mlp_are_fused(monkeypatch):
+    """Behind counter dropout: nothing is dropped, nobody watches, and the engine's activation is that of training."""
+    from makani_b200.models.common.layers import MLP
+    m = MLP(in_features=8, input_format="traditional", drop_rate=0.3, dropout_generator="counter").eval()
+    assert m._nothing_dropped() and not m.train()._nothing_dropped() and m.eval()._nothing_dropped()
+    handle = m.fwd[1].register_forward_hook(lambda *a: None)
+    assert not m._nothing_dropped()
+    handle.remove()
+    monkeypatch.setattr(_ext, "_GELU_TANH", True)
+    assert not m._nothing_dropped()
+    assert not MLP(in_features=8, input_format="traditional", drop_rate=0.3).eval()._nothing_dropped()
+
+
 @pytest.mark.parametrize("name", ["vit_73chq_window"])
 def test_recipe(name):
     from makani_b200.utils.YParams import YParams
