@@ -73,15 +73,37 @@ __device__ __forceinline__ double position_of(const void* at, int type, long lon
   }
 }
 
-// Of a fraction of a turn, at most half of one.  For bf16 the special function unit's, which are off by 2^-20 (half a step of bf16 is 2^-8 of the value).
+// Sines and cosines of two angles in turns.  For bf16 from polynomials (the first terms of the series) of what is left, at most half of a quarter, after whole
+// quarters are taken off in 64 bits: the first terms left out are 4e-7 of the sine and 2e-8 of the cosine.  Their error is one of the value, also next to a multiple
+// of a quarter, where that of the special function unit, 2^-21 of one, is all that such a value has (position 355 at one radian each: 1.6 %).
 template <typename T>
-__device__ __forceinline__ void sine_cosine(float turn, float& sine, float& cosine) {
+__device__ __forceinline__ void sines_cosines(double v0, double v1, float (&sine)[2], float (&cosine)[2]) {
+  const double t[2] = {v0 - rint(v0), v1 - rint(v1)};
   if constexpr (sizeof(T) == 2) {
-    const float angle = turn * 6.283185307179586f;
-    sine = __sinf(angle);
-    cosine = __cosf(angle);
+    uint32_t q[2];
+    float r[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const double nearest = 6755399441055744.0, n = fma(t[i], 4.0, nearest);      // 1.5 2^52: the sum's last bits are those of the nearest whole number
+      q[i] = static_cast<uint32_t>(__double2loint(n));
+      r[i] = static_cast<float>(fma(t[i], 4.0, nearest - n));
+    }
+    auto both = [](float v) { return f2_pack(v, v); };
+    const f32x2 a = f2_mul(f2_pack(r[0], r[1]), both(1.5707963267948966f)), a2 = f2_mul(a, a);
+    const f32x2 s = f2_fma(f2_mul(a, a2), f2_fma(f2_fma(both(-1.f / 5040.f), a2, both(1.f / 120.f)), a2, both(-1.f / 6.f)), a);
+    const f32x2 c = f2_fma(f2_fma(f2_fma(f2_fma(both(1.f / 40320.f), a2, both(-1.f / 720.f)), a2, both(1.f / 24.f)), a2, both(-0.5f)), a2, both(1.f));
+    float ss[2], cc[2];
+    f2_unpack(s, ss[0], ss[1]);
+    f2_unpack(c, cc[0], cc[1]);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float x = q[i] & 1 ? cc[i] : ss[i], y = q[i] & 1 ? ss[i] : cc[i];
+      sine[i] = __uint_as_float(__float_as_uint(x) ^ (q[i] & 2) << 30);
+      cosine[i] = __uint_as_float(__float_as_uint(y) ^ ((q[i] + 1) & 2) << 30);
+    }
   } else {
-    sincospif(2.f * turn, &sine, &cosine);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) sincospif(2.f * static_cast<float>(t[i]), &sine[i], &cosine[i]);
   }
 }
 
@@ -372,15 +394,19 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) rotary_kernel(const __grid_co
     // angles of the lane's pairs
     f32x2 cs[2], sn[2], neg[2];
     {
-      float c[4], d[4];
+      float c[4] = {1.f, 1.f, 1.f, 1.f}, d[4] = {0.f, 0.f, 0.f, 0.f};
+      if (positions) {
+        const bool back = BACK != (s.inverse != 0);
+        auto angle = [&](int i) { return at[RUN == 4 ? 0 : i] * turns[4 * l + i]; };
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        c[i] = 1.f;
-        d[i] = 0.f;
-        if (positions) {
-          const double v = at[RUN == 4 ? 0 : i] * turns[4 * l + i];
-          sine_cosine<T>(static_cast<float>(v - rint(v)), d[i], c[i]);
-          if (BACK != (s.inverse != 0)) d[i] = -d[i];
+        for (int i = 0; i < 4; i += 2) {
+          float sine[2], cosine[2];
+          sines_cosines<T>(angle(i), angle(i + 1), sine, cosine);
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            c[i + k] = cosine[k];
+            d[i + k] = back ? -sine[k] : sine[k];
+          }
         }
       }
       if (plain) {      // (whatever position there is)

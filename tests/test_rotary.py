@@ -273,6 +273,25 @@ def test_positions(gen, kind, per_sample):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("inverse", [False, True])
+def test_angles_next_to_quarters_of_a_turn(gen, inverse):
+    """Sines and cosines that are small have as many right bits as others in bf16: half a step of the value, and what fp32 makes of a polynomial of five terms and
+    its argument (4e-7 and eight roundings: 2^-19.8); angles are off by three roundings of 64 bits."""
+    whole = [11, 22, 33, 355, 710, 1065, 103993, 104348, 208341, 312689, 833719]       # (next to multiples of pi)
+    at = torch.tensor([0.0, 1e-7, 3e-6, -2e-5, 1e-4, -1e-3, 0.01, 0.3] + [float(s * n) for n in whole for s in (1, -1)] + [n / 2 + 1e-9 for n in whole],
+                      dtype=torch.float64, device="cuda")
+    axes = rot.RotaryAxes((2,), base=7.0)
+    x = torch.zeros(2, at.numel(), 1, 8, device="cuda", dtype=torch.bfloat16)
+    x[0, ..., 0] = 1.0
+    x[1, ..., 1] = 1.0
+    y = rot.rotary(x, at[:, None], axes, inverse=inverse)[:, :, 0, :2].double()
+    turn = -at if inverse else at
+    want = torch.stack([torch.stack([turn.cos(), turn.sin()], -1), torch.stack([-turn.sin(), turn.cos()], -1)])
+    assert want.abs().min() == 0.0 and (want.abs() < 1e-4).sum() > 20
+    assert ((y - want).abs() <= (2.0 ** -8 + 2.0 ** -19.8) * want.abs() + 3 * 2.0 ** -53 * at.abs()[:, None]).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("norm", [None, "layer", "rms"])
 def test_strides_and_packed_tokens(gen, norm):
     """Views of a fused projection, heads in front, expanded and unaligned tensors, packed tokens."""
