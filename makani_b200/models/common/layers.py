@@ -168,7 +168,7 @@ class MLP(nn.Module):
         self.fwd = nn.Sequential(fc1, act_layer(), drop, fc2, drop)
         self._fusable = (input_format == "nchw" and _is_gelu(act_layer) and drop_rate == 0.0)
         self._fusable_tokens = (input_format == "traditional" and _is_gelu(act_layer) and drop_rate == 0.0)
-        self._fusable_forecasts = counter and _is_gelu(act_layer)
+        self._fusable_forecasts = counter and _is_gelu(act_layer) and hidden_features % 8 == 0 and out_features % 8 == 0
 
     def _run(self, x):
         if self._fusable and x.is_cuda and conv_ops.fast_path_ok(x):

@@ -186,6 +186,9 @@ def test_when_forecasts_of_the_mlp_are_fused(monkeypatch):
     monkeypatch.setattr(_ext, "_GELU_TANH", True)
     assert not m._nothing_dropped()
     assert not MLP(in_features=8, input_format="traditional", drop_rate=0.3).eval()._nothing_dropped()
+    monkeypatch.undo()
+    for more in (dict(hidden_features=20), dict(out_features=12), dict(act_layer=nn.ReLU)):
+        assert not MLP(in_features=8, input_format="traditional", drop_rate=0.3, dropout_generator="counter", **more).eval()._nothing_dropped()
 
 
 @pytest.mark.parametrize("name", ["vit_73chq_window"])
@@ -304,6 +307,21 @@ def test_mlp_behind_counter_dropout(dev, joint):
     plain = m(x)
     m.fwd[2].train()
     assert not torch.equal(m(x), plain)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hidden,out", [(20, 16), (24, 12), (24, 16)])
+def test_widths_of_the_mlp_behind_counter_dropout(dev, hidden, out):
+    """Widths that are no multiple of eight, in training and in forecasts."""
+    from makani_b200.models.common.layers import MLP
+    torch.manual_seed(2)
+    m = MLP(in_features=16, hidden_features=hidden, out_features=out, input_format="traditional", drop_rate=0.3, dropout_generator="counter").to(dev).eval()
+    x = torch.randn(2, 50, 16, device=dev).bfloat16().requires_grad_()
+    p = [t.detach().double() for t in m.parameters()]
+    want = torch.nn.functional.gelu(x.detach().double() @ p[0].bfloat16().double().T + p[1]) @ p[2].bfloat16().double().T + p[3]
+    assert _rel(m(x).detach(), want) < 2.0 ** -7
+    m.train()(x).float().sum().backward()
+    assert all(torch.isfinite(t.grad).all() for t in (x, *m.parameters()))
 
 
 @pytest.mark.gpu
