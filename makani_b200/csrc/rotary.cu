@@ -75,7 +75,8 @@ __device__ __forceinline__ double position_of(const void* at, int type, long lon
 
 // Sines and cosines of two angles in turns.  For bf16 from polynomials (the first terms of the series) of what is left, at most half of a quarter, after whole
 // quarters are taken off in 64 bits: the first terms left out are 4e-7 of the sine and 2e-8 of the cosine.  Their error is one of the value, also next to a multiple
-// of a quarter, where that of the special function unit, 2^-21 of one, is all that such a value has (position 355 at one radian each: 1.6 %).
+// of a quarter, where that of the special function unit, 2^-21 of one, is much of such a value (its sine of position 355 at one radian each, 3e-5, rounded to bf16: 0.7 %;
+// of 2e-6 9 %, of 2e-7 all of it).
 template <typename T>
 __device__ __forceinline__ void sines_cosines(double v0, double v1, float (&sine)[2], float (&cosine)[2]) {
   const double t[2] = {v0 - rint(v0), v1 - rint(v1)};
